@@ -13,6 +13,41 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200, sm_100a)")
 
 
+# tests whose child processes load the front-end library: they see only an exit code
+_IN_CHILDREN = {"test_two_rank_gloo_training_matches_single_process",
+                "test_a_rank_that_leaves_makes_the_exchange_fail_not_hang"}
+
+
+def _without_sources() -> bool:
+    """The front-end and the oracle library are built from MiniTensor's sources;
+    without them and without prebuilt libraries their tests are skipped."""
+    from minitensor_cpp_b200 import _build_host
+    from minitensor_cpp_b200.frontend import LIB
+
+    return not LIB.exists() and not _build_host.sources_present()
+
+
+def pytest_collection_modifyitems(config, items):
+    if not _without_sources():
+        return
+    for item in items:
+        if getattr(item, "originalname", item.name) in _IN_CHILDREN:
+            item.add_marker(pytest.mark.skip(reason="the front-end library needs MiniTensor's sources"))
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_makereport(item, call):
+    e = call.excinfo
+    missing = ("is not built", "oracle library missing")
+    if (e is not None and e.errisinstance(FileNotFoundError) and any(m in str(e.value) for m in missing)
+            and _without_sources()):
+        try:
+            pytest.skip(f"needs MiniTensor's sources: {e.value}")
+        except pytest.skip.Exception as skipped:
+            call.excinfo = pytest.ExceptionInfo.from_exception(skipped)
+    yield
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch
