@@ -247,6 +247,77 @@ int mtc_gather_scatter_add(const mtc_desc *upd, const mtc_desc *idx, int64_t axi
 int mtc_gather_scatter_add_into(const mtc_desc *upd, const mtc_desc *idx, int64_t axis, const mtc_desc *out,
                                 void *stream);
 
+/* ------------------------------------------------ language-model operators --
+ * No reference counterpart: the reference trains dense classifiers (its loss
+ * keeps the logits, src/nn/loss.cpp:41-57, and it has neither an embedding nor
+ * gradient clipping).  Operands are views like everywhere else: any strides,
+ * offsets that need not be aligned.  Outputs must not overlap inputs unless an
+ * entry point says so.
+ *
+ * The entry points that need a workspace take it from the pool for the time of
+ * the call.  Recorded with mtc_capture_begin, a graph owns its workspaces; on a
+ * stream that something else is capturing they return MTC_ERR_UNSUPPORTED,
+ * because the pool would hand the same block to the next caller while the graph
+ * still replays into it. */
+
+/* Value of a `padding_token` / `ignore_target` argument that excludes nothing. */
+#define MTC_NO_TOKEN INT64_MIN
+
+/* Embedding lookup: out[i.., :] = scale * table[tokens[i..], :].
+ * table [V, D] Float32, tokens Int64 of any rank up to 7, out tokens.shape + [D]
+ * Float32.  A position whose token is `padding_token` gets a row of zeros.  A
+ * token outside [0, V) writes nothing for its row and sets the device error
+ * word.  Needs no workspace. */
+int mtc_embedding(const mtc_desc *table, const mtc_desc *tokens, float scale, int64_t padding_token,
+                  const mtc_desc *out, void *stream);
+
+/* Its gradient: dtable[v, :] = scale * sum of dout[i.., :] over the positions
+ * whose token is v, zero where there is none; accumulate != 0 adds to what
+ * dtable holds instead (tied weights: the output layer's gradient).  Positions
+ * that hold `padding_token` contribute nothing, a token outside [0, V) neither
+ * and sets the device error word.  The tokens are sorted first, and every row
+ * is summed in an order fixed by the tokens alone: the same inputs give the same
+ * bits.  At most 2^31 - 1 positions. */
+int mtc_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale, int64_t padding_token,
+                       int32_t accumulate, const mtc_desc *dtable, void *stream);
+
+/* Softmax cross entropy of a linear layer, without keeping the logits:
+ *   z = x . weight^T + bias,  lse[n] = log sum_v exp z[n,v],  loss[n] = lse[n] - z[n, targets[n]]
+ * x [N, D], weight [V, D] (the layout of Linear), bias [V] or NULL, targets
+ * Int64 [N], loss [N], lse [N] or NULL.  A row whose target is `ignore_target`
+ * has loss 0 and lse 0, whatever x holds there; so does a row whose target lies
+ * outside [0, V), which also sets the device error word.  Products have float32
+ * accuracy (each operand as a pair of 16-bit floats, or float32 for small
+ * problems).  A non-finite x makes its own row's loss NaN or infinite, a
+ * non-finite weight or bias every row's. */
+int mtc_linear_cross_entropy(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias, const mtc_desc *targets,
+                             int64_t ignore_target, const mtc_desc *loss, const mtc_desc *lse, void *stream);
+
+/* The same with the gradients of sum_n dloss[n] * loss[n]:
+ *   g[n,v] = dloss[n] * (exp(z[n,v] - lse[n]) - [v = targets[n]]),
+ *   dx = g . weight,  dweight = g^T . x,  dbias[v] = sum_n g[n,v]
+ * in one call (three products; the logits of a piece of the rows at a time).
+ * dloss [N] may be a broadcast view.  loss, lse, dx, dweight and dbias may each
+ * be NULL.  dx rows of ignored targets are zero.  dx, dweight and dbias are
+ * overwritten. */
+int mtc_linear_cross_entropy_grad(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias,
+                                  const mtc_desc *targets, int64_t ignore_target, const mtc_desc *dloss,
+                                  const mtc_desc *loss, const mtc_desc *lse, const mtc_desc *dx,
+                                  const mtc_desc *dweight, const mtc_desc *dbias, void *stream);
+
+/* norm (Float32, one element) = sqrt of the sum of squares over all `n` Float32
+ * tensors, summed in float64 in a fixed order. */
+int mtc_global_norm(const mtc_desc *tensors, int32_t n, const mtc_desc *norm, void *stream);
+
+/* outs[k] = tensors[k] * c with c = max_norm / norm where the global norm
+ * exceeds max_norm, and 1 where it does not (the outputs then equal the inputs
+ * bit for bit).  outs[k] has tensors[k]'s shape and may be the same view (in
+ * place); other overlaps are not allowed.  norm may be NULL.  A NaN norm makes
+ * every output NaN; an infinite one makes finite gradients 0 and infinite ones
+ * NaN.  max_norm >= 0. */
+int mtc_clip_global_norm(const mtc_desc *tensors, int32_t n, float max_norm, const mtc_desc *outs,
+                         const mtc_desc *norm, void *stream);
+
 /* -------------------------------------------------------- reductions (A8, A9) -- */
 
 /* Reduce `in` over `axes` (normalised, distinct).  `out` is contiguous and holds the

@@ -33,6 +33,8 @@ SUM, LOGSUMEXP, MAX, ARGMAX = 0x0301, 0x0302, 0x0380, 0x0381
 UNARY_OPS = (ABS, SIGN, NEGATE, EXP, LOG, SQRT, TANH, SIGMOID, RELU)
 BINARY_OPS = (ADD, SUBTRACT, MULTIPLY, DIVIDE, LOGADDEXP)
 
+NO_TOKEN = -(1 << 63)  # padding_token / ignore_target that excludes nothing
+
 GEMM_AUTO, GEMM_SIMT, GEMM_3XTF32, GEMM_SIMT_FFMA = 0, 1, 2, 3
 
 LIB_DIR = Path(__file__).resolve().parent / "lib"
@@ -189,6 +191,12 @@ def _declare(L):
         "mtc_gather": ([P(Desc), P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_gather_scatter_add": ([P(Desc), P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_gather_scatter_add_into": ([P(Desc), P(Desc), c_i64, P(Desc), c_vp], c_int),
+        "mtc_embedding": ([P(Desc), P(Desc), c_f, c_i64, P(Desc), c_vp], c_int),
+        "mtc_embedding_grad": ([P(Desc), P(Desc), c_f, c_i64, c_i32, P(Desc), c_vp], c_int),
+        "mtc_linear_cross_entropy": ([P(Desc)] * 4 + [c_i64, P(Desc), P(Desc), c_vp], c_int),
+        "mtc_linear_cross_entropy_grad": ([P(Desc)] * 4 + [c_i64] + [P(Desc)] * 6 + [c_vp], c_int),
+        "mtc_global_norm": ([P(Desc), c_i32, P(Desc), c_vp], c_int),
+        "mtc_clip_global_norm": ([P(Desc), c_i32, c_f, P(Desc), P(Desc), c_vp], c_int),
         "mtc_reduce": ([c_i32, P(Desc), P(c_i64), c_i32, P(Desc), c_vp], c_int),
         "mtc_log_softmax": ([P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_matmul": ([P(Desc), P(Desc), P(Desc), c_i32, c_vp], c_int),
@@ -220,7 +228,7 @@ EXPORTED = (
     "mtc_stream_wait_event", "mtc_event_create_timed", "mtc_event_elapsed", "mtc_pool_take", "mtc_pool_take_many", "mtc_pool_protect", "mtc_capture_begin", "mtc_capture_end", "mtc_capture_fused_count", "mtc_graph_launch",
     "mtc_graph_set_constants", "mtc_graph_launches", "mtc_graph_destroy",
     "mtc_check_device_errors", "mtc_watch_device_errors", "mtc_poll_device_errors", "mtc_selftest_bounded_wait", "mtc_unary", "mtc_binary", "mtc_fused", "mtc_copy", "mtc_concat", "mtc_index_scatter",
-    "mtc_gather", "mtc_gather_scatter_add", "mtc_gather_scatter_add_into", "mtc_reduce", "mtc_log_softmax", "mtc_matmul", "mtc_fill", "mtc_uniform",
+    "mtc_gather", "mtc_gather_scatter_add", "mtc_gather_scatter_add_into", "mtc_embedding", "mtc_embedding_grad", "mtc_linear_cross_entropy", "mtc_linear_cross_entropy_grad", "mtc_global_norm", "mtc_clip_global_norm", "mtc_reduce", "mtc_log_softmax", "mtc_matmul", "mtc_fill", "mtc_uniform",
     "mtc_normal", "mtc_launch_count", "mtc_profile_enable", "mtc_profile_gemm", "mtc_gemm_path_counts", "mtc_comm_unique_id", "mtc_comm_init", "mtc_comm_allreduce_f32", "mtc_comm_allreduce_f32_async", "mtc_comm_wait", "mtc_comm_destroy",
 )
 
@@ -307,6 +315,63 @@ def gather(src: View, idx: View, axis: int, out: View, stream=None, prepare: boo
 def gather_scatter_add(upd: View, idx: View, axis: int, out: View, stream=None, prepare: bool = False):
     return _run("mtc_gather_scatter_add", (ctypes.byref(upd.desc()), ctypes.byref(idx.desc()), axis,
                                            ctypes.byref(out.desc()), _stream(stream)), "gather_scatter_add", prepare)
+
+
+def _ref(v: View | None):
+    return None if v is None else ctypes.byref(v.desc())
+
+
+def _token(t: int | None) -> int:
+    return NO_TOKEN if t is None else int(t)
+
+
+def embedding(table: View, tokens: View, out: View, scale: float = 1.0, padding_token: int | None = None, stream=None,
+              prepare: bool = False):
+    """out[i.., :] = scale * table[tokens[i..], :]; zeros where the token is `padding_token`."""
+    return _run("mtc_embedding", (_ref(table), _ref(tokens), scale, _token(padding_token), _ref(out), _stream(stream)),
+                "embedding", prepare)
+
+
+def embedding_grad(dout: View, tokens: View, dtable: View, scale: float = 1.0, padding_token: int | None = None,
+                   accumulate: bool = False, stream=None, prepare: bool = False):
+    """dtable[v, :] = scale * the sum of dout over v's positions (added to dtable with `accumulate`)."""
+    return _run("mtc_embedding_grad", (_ref(dout), _ref(tokens), scale, _token(padding_token), int(accumulate),
+                                       _ref(dtable), _stream(stream)), "embedding_grad", prepare)
+
+
+def linear_cross_entropy(x: View, weight: View, targets: View, loss: View, bias: View | None = None,
+                         lse: View | None = None, ignore_target: int | None = None, stream=None,
+                         prepare: bool = False):
+    """loss[n] = logsumexp(z[n]) - z[n, targets[n]] with z = x . weight^T + bias, the logits never stored."""
+    return _run("mtc_linear_cross_entropy", (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target),
+                                             _ref(loss), _ref(lse), _stream(stream)), "linear_cross_entropy", prepare)
+
+
+def linear_cross_entropy_grad(x: View, weight: View, targets: View, dloss: View, dx: View | None = None,
+                              dweight: View | None = None, bias: View | None = None, dbias: View | None = None,
+                              loss: View | None = None, lse: View | None = None, ignore_target: int | None = None,
+                              stream=None, prepare: bool = False):
+    """linear_cross_entropy with the gradients of sum(dloss * loss) for x, weight and bias."""
+    return _run("mtc_linear_cross_entropy_grad",
+                (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target), _ref(dloss), _ref(loss),
+                 _ref(lse), _ref(dx), _ref(dweight), _ref(dbias), _stream(stream)), "linear_cross_entropy_grad", prepare)
+
+
+def global_norm(tensors: Sequence[View], norm: View, stream=None, prepare: bool = False):
+    """norm = sqrt of the sum of squares of all elements of all tensors."""
+    arr = (Desc * max(len(tensors), 1))(*[v.desc() for v in tensors])
+    return _run("mtc_global_norm", (arr, len(tensors), _ref(norm), _stream(stream)), "global_norm", prepare)
+
+
+def clip_global_norm(tensors: Sequence[View], max_norm: float, norm: View | None = None,
+                     outs: Sequence[View] | None = None, stream=None, prepare: bool = False):
+    """Scales the tensors by max_norm / norm where their global norm exceeds max_norm; into `outs`, or in place."""
+    arr = (Desc * max(len(tensors), 1))(*[v.desc() for v in tensors])
+    if outs is not None and len(outs) != len(tensors):
+        raise ValueError(f"{len(outs)} outputs for {len(tensors)} tensors")
+    to = arr if outs is None else (Desc * max(len(outs), 1))(*[v.desc() for v in outs])
+    return _run("mtc_clip_global_norm", (arr, len(tensors), max_norm, to, _ref(norm), _stream(stream)),
+                "clip_global_norm", prepare)
 
 
 def reduce(op: int, x: View, axes: Sequence[int], out: View, stream=None, prepare: bool = False):

@@ -1,0 +1,157 @@
+"""Refusals of the embedding, linear cross entropy and clipping entry points: every
+malformed call is turned away on the host, before any device work (no GPU needed)."""
+import ctypes
+
+import pytest
+
+from minitensor_cpp_b200 import abi
+
+P = 0x10000  # an address nothing reads: the calls below return before a launch
+
+
+def desc(shape, strides=None, offset=0, capacity=None, dtype=abi.FLOAT32, ptr=P):
+    strides = abi.contiguous_strides(shape) if strides is None else strides
+    if capacity is None:
+        capacity = offset + 1 + sum(abs(s) * (e - 1) for s, e in zip(strides, shape) if e > 0)
+    return abi.make_desc(ptr, capacity, dtype, shape, strides, offset)
+
+
+def ints(shape, **k):
+    return desc(shape, dtype=abi.INT64, **k)
+
+
+def ref(d):
+    return None if d is None else ctypes.byref(d)
+
+
+def embedding(table, tokens, out):
+    return abi.lib().mtc_embedding(ref(table), ref(tokens), 1.0, abi.NO_TOKEN, ref(out), None)
+
+
+def embedding_grad(dout, tokens, dtable):
+    return abi.lib().mtc_embedding_grad(ref(dout), ref(tokens), 1.0, abi.NO_TOKEN, 0, ref(dtable), None)
+
+
+@pytest.mark.parametrize("table, tokens, out, code", [
+    (desc([4, 3]), ints([5]), desc([5, 4]), abi.ERR_INVALID_ARGUMENT),           # columns differ
+    (desc([4, 3]), ints([5]), desc([6, 3]), abi.ERR_INVALID_ARGUMENT),           # positions differ
+    (desc([4, 3]), ints([5]), desc([5, 1, 3]), abi.ERR_INVALID_ARGUMENT),        # rank
+    (desc([4]), ints([5]), desc([5, 4]), abi.ERR_INVALID_ARGUMENT),              # the table is no matrix
+    (desc([4, 3]), desc([5]), desc([5, 3]), abi.ERR_INVALID_ARGUMENT),           # float tokens
+    (ints([4, 3]), ints([5]), desc([5, 3]), abi.ERR_INVALID_ARGUMENT),           # whole numbers in the table
+    (desc([4, 3]), ints([5]), desc([5, 3], [0, 1]), abi.ERR_INVALID_ARGUMENT),   # a written view that repeats
+    (desc([4, 3]), ints([5]), desc([5, 3], [2, 1]), abi.ERR_INVALID_ARGUMENT),   # rows that overlap
+    (desc([4, 3], capacity=11), ints([5]), desc([5, 3]), abi.ERR_OUT_OF_RANGE),
+    (desc([4, 3]), ints([5], capacity=4), desc([5, 3]), abi.ERR_OUT_OF_RANGE),
+    (None, ints([5]), desc([5, 3]), abi.ERR_INVALID_ARGUMENT),
+])
+def test_embedding_refuses(table, tokens, out, code):
+    assert embedding(table, tokens, out) == code
+
+
+def test_embedding_grad_refuses_a_table_whose_rows_overlap():
+    assert embedding_grad(desc([5, 3]), ints([5]), desc([4, 3], [0, 1])) == abi.ERR_INVALID_ARGUMENT
+    assert b"share addresses" in abi.lib().mtc_last_error()
+    assert embedding_grad(desc([5, 3]), ints([5]), desc([4, 4])) == abi.ERR_INVALID_ARGUMENT
+    assert embedding_grad(desc([5, 3]), desc([5]), desc([4, 3])) == abi.ERR_INVALID_ARGUMENT
+
+
+def test_embedding_of_nothing_is_a_call_without_work():
+    assert embedding(desc([4, 3]), ints([0]), desc([0, 3])) == abi.OK
+    assert embedding(desc([4, 0]), ints([5]), desc([5, 0])) == abi.OK
+    assert embedding_grad(desc([5, 0]), ints([5]), desc([4, 0])) == abi.OK
+
+
+def ce(x, w, t, loss, bias=None, lse=None):
+    return abi.lib().mtc_linear_cross_entropy(ref(x), ref(w), ref(bias), ref(t), -100, ref(loss), ref(lse), None)
+
+
+def ce_grad(x, w, t, dloss, dx=None, dw=None, bias=None, db=None, loss=None, lse=None):
+    return abi.lib().mtc_linear_cross_entropy_grad(ref(x), ref(w), ref(bias), ref(t), -100, ref(dloss), ref(loss),
+                                                   ref(lse), ref(dx), ref(dw), ref(db), None)
+
+
+X, W, T, L = desc([6, 4]), desc([9, 4]), ints([6]), desc([6])
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ce(desc([6, 5]), W, T, L),                 # columns of x and weight differ
+    lambda: ce(desc([6, 4, 1]), W, T, L),
+    lambda: ce(X, W, ints([5]), L),
+    lambda: ce(X, W, desc([6]), L),                    # float targets
+    lambda: ce(X, W, T, desc([5])),
+    lambda: ce(X, W, T, desc([6, 1])),
+    lambda: ce(X, W, T, desc([6], [0])),               # a written view that repeats
+    lambda: ce(X, W, T, None),
+    lambda: ce(X, W, T, L, bias=desc([8])),
+    lambda: ce(X, W, T, L, bias=ints([9])),
+    lambda: ce(X, W, T, L, lse=desc([7])),
+    lambda: ce(X, desc([0, 4]), T, L),                 # no classes
+    lambda: ce(None, W, T, L),
+    lambda: ce(X, W, None, L),
+    lambda: ce_grad(X, W, T, None),
+    lambda: ce_grad(X, W, T, desc([5])),
+    lambda: ce_grad(X, W, T, L, dx=desc([6, 5])),
+    lambda: ce_grad(X, W, T, L, dx=desc([6, 4], [0, 1])),
+    lambda: ce_grad(X, W, T, L, dw=desc([4, 9])),
+    lambda: ce_grad(X, W, T, L, dw=desc([9, 4], [2, 1])),
+    lambda: ce_grad(X, W, T, L, db=desc([4])),
+])
+def test_linear_cross_entropy_refuses(call):
+    assert call() == abi.ERR_INVALID_ARGUMENT
+    assert abi.lib().mtc_last_error()
+
+
+def test_linear_cross_entropy_refuses_views_outside_their_buffers():
+    assert ce(desc([6, 4], capacity=23), W, T, L) == abi.ERR_OUT_OF_RANGE
+    assert ce(X, W, ints([6], capacity=5), L) == abi.ERR_OUT_OF_RANGE
+    assert ce_grad(X, W, T, L, dx=desc([6, 4], capacity=20)) == abi.ERR_OUT_OF_RANGE
+
+
+def norm(tensors, out):
+    arr = (abi.Desc * max(len(tensors), 1))(*tensors)
+    return abi.lib().mtc_global_norm(arr, len(tensors), ref(out), None)
+
+
+def clip(tensors, outs, max_norm=1.0, n=None):
+    a = (abi.Desc * max(len(tensors), 1))(*tensors)
+    b = (abi.Desc * max(len(outs), 1))(*outs)
+    return abi.lib().mtc_clip_global_norm(a, len(tensors) if n is None else n, max_norm, b, None, None)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: norm([desc([3])], None),
+    lambda: norm([desc([3])], desc([2])),                                # the norm is one number
+    lambda: norm([ints([3])], desc([])),
+    lambda: clip([desc([3])], [desc([4])]),
+    lambda: clip([desc([3])], [desc([3, 1])]),
+    lambda: clip([desc([3])], [ints([3])]),
+    lambda: clip([desc([3])], [desc([3])], max_norm=-1.0),
+    lambda: clip([desc([3])], [desc([3])], max_norm=float("nan")),
+    lambda: clip([desc([3])], [desc([3], [0])]),                         # a written view that repeats
+    lambda: clip([desc([3]), desc([3])], [desc([3]), desc([3])]),        # one output twice: scaled twice in place
+    lambda: clip([desc([3]), desc([3])], [desc([3]), desc([3], offset=2)]),
+    lambda: clip([desc([3])], [desc([3])], n=-1),
+])
+def test_clipping_refuses(call):
+    assert call() == abi.ERR_INVALID_ARGUMENT
+
+
+def test_clipping_nothing_is_a_call_without_work():
+    assert clip([], []) == abi.OK
+    assert clip([desc([0, 5])], [desc([0, 5])]) == abi.OK
+
+
+def test_python_wrapper_turns_refusals_into_exceptions():
+    import torch
+
+    v = lambda *s: abi.View.of(torch.zeros(*s))
+    t = lambda *s: abi.View.of(torch.zeros(*s, dtype=torch.int64))
+    with pytest.raises(ValueError, match="columns"):
+        abi.embedding(v(4, 3), t(5), v(5, 4), stream=0)
+    with pytest.raises(ValueError, match="columns"):
+        abi.linear_cross_entropy(v(6, 5), v(9, 4), t(6), v(6), stream=0)
+    with pytest.raises(ValueError, match="outputs for"):
+        abi.clip_global_norm([v(3)], 1.0, outs=[], stream=0)
+    with pytest.raises(ValueError, match="max_norm"):
+        abi.clip_global_norm([v(3)], -1.0, stream=0)
