@@ -33,11 +33,24 @@
 #include <mutex>
 
 #include "gemm.cuh"
+#include "tcgen05.cuh"
 
 namespace mtc {
 
 // Device error word (copy.cu) as a device address, for kernels in other files.
 int device_error_word(unsigned long long **out);
+
+EncodeTiled tensor_map_encoder() {
+    static EncodeTiled fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess)
+            fn = reinterpret_cast<EncodeTiled>(p);
+    });
+    return fn;
+}
 
 namespace {
 
@@ -65,7 +78,6 @@ struct TcPipe {
 using PipeDeep = TcPipe<16, 4>;     // 4 x 48 KB
 using PipeWide = TcPipe<32, 2>;     // 2 x 96 KB
 constexpr uint32_t TC_TMEM_COLS = 512;
-constexpr long long kWaitLimit = 20000000;  // bounded spins per wait
 constexpr int kErrTimeout = MTC_ERR_RUNTIME;
 
 struct TcArgs {
@@ -103,46 +115,6 @@ __device__ __forceinline__ void unit_range(const TcArgs &a, int64_t u, int64_t k
     split = static_cast<int>(u - t * a.splits);
     kb0 = static_cast<int64_t>(split) * a.kb_per_split;
     kb1 = kb0 + a.kb_per_split < kblocks ? kb0 + a.kb_per_split : kblocks;
-}
-
-// ------------------------------------------------------------ PTX helpers --
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Bounded wait: false when the limit expired or another role aborted.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    for (long long i = 0; i < kWaitLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 1023) == 1023 && *abort_flag) return false;
-    }
-    *abort_flag = 1;
-    return false;
 }
 
 // The unit after `u` for a CTA (or CTA pair) among `workers`.
@@ -192,25 +164,6 @@ __device__ __forceinline__ void umma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // x = hi + lo with hi = x truncated to TF32 (low 13 mantissa bits cleared) and
 // lo = x - hi exact in float32; non-finite values keep hi = x, lo = 0.
@@ -628,48 +581,8 @@ using PairWide = PairPipe<32, 3>;  // 3 x 64 KB
 constexpr uint32_t kPairInstrDesc = (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(256 >> 3) << 17) |
                                     (uint32_t(256 >> 4) << 24);
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-
-// shared::cluster address of the same shared-memory offset in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
-    uint32_t out;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_u32(p)), "r"(rank));
-    return out;
-}
-
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-
-// Bounded wait with cluster-scope acquire: for barriers another CTA of the
-// cluster arrives on after writing this CTA's shared memory.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    for (long long i = 0; i < kWaitLimit; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if ((i & 1023) == 1023 && *abort_flag) return false;
-    }
-    *abort_flag = 1;
-    return false;
-}
-
 __device__ __forceinline__ void st_cluster_s64(uint32_t cluster_addr, int64_t v) {
     asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(cluster_addr), "l"(v) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 __device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint32_t leader_bar, int x, int y,
@@ -688,20 +601,6 @@ __device__ __forceinline__ void umma_tf32_pair(uint32_t d_tmem, uint64_t a, uint
         "tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(kPairInstrDesc), "r"(accumulate)
         : "memory");
-}
-
-// Arrive once on the barrier at this offset in both CTAs of the pair when the
-// issuing thread's prior MMAs complete.
-__device__ __forceinline__ void umma_commit_both(uint64_t *bar) {
-    const uint16_t mask = 0x3;
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_u32(bar)), "h"(mask)
-                 : "memory");
-}
-
-__device__ __forceinline__ void umma_commit_pair_local(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
 }
 
 __device__ __forceinline__ void pair_tile_coords(const TcArgs &a, int64_t t, int &tm, int &tn, int &tb) {
@@ -1124,22 +1023,6 @@ __global__ void __launch_bounds__(256) k_split_tile4(const PackArgs a) {
     }
 }
 
-using PFN_EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                     const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                     CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-PFN_EncodeTiled encode_fn() {
-    static PFN_EncodeTiled fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess)
-            fn = reinterpret_cast<PFN_EncodeTiled>(p);
-    });
-    return fn;
-}
-
 // One GEMM operand as its tensor maps see it: `rows` K-major rows of `kdim`
 // elements, `pitch` elements apart, batches `bstride` elements apart.  Packed
 // operands have split hi / lo arrays; a raw (direct) operand is the caller's own
@@ -1188,7 +1071,7 @@ bool direct_operand(const float *base, int64_t off, int64_t row_stride, int64_t 
 template <class P>
 int make_map(CUtensorMap &map, const float *base, int64_t kdim, int64_t rows, int64_t batch, int64_t pitch,
              int64_t bstride, uint32_t box_rows) {
-    PFN_EncodeTiled enc = encode_fn();
+    EncodeTiled enc = tensor_map_encoder();
     if (enc == nullptr) return fail(MTC_ERR_RUNTIME, "cuTensorMapEncodeTiled is unavailable");
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kdim), static_cast<cuuint64_t>(rows),
                                 static_cast<cuuint64_t>(batch)};

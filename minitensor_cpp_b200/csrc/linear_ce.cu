@@ -11,37 +11,10 @@
 #include <climits>
 #include <cstring>
 
-#include "operators.cuh"
+#include "linear_ce.cuh"
 
 namespace mtc {
 namespace {
-
-struct Problem {
-    int64_t N, V, D;
-    const float *x;
-    int64_t x_rs, x_cs;
-    const float *w;
-    int64_t w_rs, w_cs;
-    const float *bias;  // null: none
-    int64_t b_s;
-    const int64_t *targets;
-    int64_t t_s;
-    int64_t ignore;
-    const float *dloss;  // null: no gradients
-    int64_t dl_s;
-    float *loss, *lse;  // null: not wanted
-    int64_t loss_s, lse_s;
-    float *dx, *dw, *db;  // null: not wanted
-    int64_t dx_rs, dx_cs, dw_rs, dw_cs, db_s;
-};
-
-// What the device knows about the rows that have a loss.
-struct LiveRows {
-    int *count;      // [1]
-    int *row;        // [N] the row of x
-    int *target;     // [N]
-    float *dloss;    // [N]
-};
 
 __device__ __forceinline__ int block_exclusive(int v, int *warp_sums, int &total) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -64,7 +37,7 @@ __device__ __forceinline__ int block_exclusive(int v, int *warp_sums, int &total
 }
 
 // The rows with a loss, in order; zero loss, lse and dx count for the others.
-__global__ void __launch_bounds__(1024) k_live_rows(const Problem p, const LiveRows live, unsigned long long *err) {
+__global__ void __launch_bounds__(1024) k_live_rows(const LinearCe p, const LiveRows live, unsigned long long *err) {
     __shared__ int warp_sums[32];
     constexpr int U = 4;
     int first = 0;
@@ -103,11 +76,14 @@ __global__ void __launch_bounds__(1024) k_live_rows(const Problem p, const LiveR
         }
         first += total;
     }
-    if (threadIdx.x == 0) *live.count = first;
+    if (threadIdx.x == 0) {
+        live.count[0] = first;
+        live.count[1] = live.count[2] = live.count[3] = 0;
+    }
 }
 
 // dx rows without a loss.
-__global__ void __launch_bounds__(256) k_zero_dx(const Problem p) {
+__global__ void __launch_bounds__(256) k_zero_dx(const LinearCe p) {
     for (int64_t n = blockIdx.x; n < p.N; n += gridDim.x) {
         const int64_t t = p.targets[n * p.t_s];
         if (t != p.ignore && t >= 0 && t < p.V) continue;
@@ -137,11 +113,6 @@ struct SimtArgs {
     int64_t first;
     int64_t k_split;  // K of one blockIdx.z; partial results [z][M][N] in c with several
 };
-
-__device__ __forceinline__ int64_t live_extent(const int *live, int64_t first, int64_t extent) {
-    const int64_t left = *live - first;
-    return left < 0 ? 0 : left < extent ? left : extent;
-}
 
 __global__ void __launch_bounds__(256) k_simt_product(const SimtArgs g) {
     constexpr int T = 64, KT = 16;
@@ -243,7 +214,7 @@ __device__ __forceinline__ float block_reduce(float v, bool take_max) {
 }
 
 // One CTA a row of logits: lse and loss, then g in the place of z.
-__global__ void __launch_bounds__(256) k_softmax_rows(const Problem p, const LiveRows live, int64_t first, int64_t rows,
+__global__ void __launch_bounds__(256) k_softmax_rows(const LinearCe p, const LiveRows live, int64_t first, int64_t rows,
                                                       float *z) {
     const int64_t r = blockIdx.x;
     if (r >= live_extent(live.count, first, rows)) return;
@@ -305,7 +276,7 @@ __global__ void __launch_bounds__(256) k_column_sums(const float *g, int64_t V, 
     db[v * db_s] = add ? db[v * db_s] + sum : sum;
 }
 
-int simt_path(const Problem &p, cudaStream_t stream) {
+int simt_path(const LinearCe &p, cudaStream_t stream) {
     int64_t chunk = (int64_t{1} << 28) / (p.V * 4);
     if (chunk < 64) chunk = 64;
     if (chunk > p.N) chunk = p.N;
@@ -322,14 +293,7 @@ int simt_path(const Problem &p, cudaStream_t stream) {
     live.dloss = ws.take<float>(list);
     float *z = ws.take<float>(zs);
     float *part = ws.take<float>(parts);
-    unsigned long long *err = nullptr;
-    MTC_TRY(device_error_word(&err));
-    k_live_rows<<<1, 1024, 0, stream>>>(p, live, err);
-    MTC_TRY(check_launch("linear cross entropy (rows)"));
-    if (p.dx != nullptr) {
-        k_zero_dx<<<static_cast<unsigned>(p.N < 1184 ? p.N : 1184), 256, 0, stream>>>(p);
-        MTC_TRY(check_launch("linear cross entropy (zero rows)"));
-    }
+    MTC_TRY(list_live_rows(p, live, stream));
     for (int64_t first = 0; first < p.N; first += chunk) {
         const int64_t rows = p.N - first < chunk ? p.N - first : chunk;
         SimtArgs g;
@@ -441,7 +405,7 @@ int zero_view(const mtc_desc *d, cudaStream_t stream) {
 int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias, const mtc_desc *targets,
                   int64_t ignore, const mtc_desc *dloss, const mtc_desc *loss, const mtc_desc *lse, const mtc_desc *dx,
                   const mtc_desc *dw, const mtc_desc *db, bool grads, cudaStream_t stream) {
-    Problem p;
+    LinearCe p;
     std::memset(&p, 0, sizeof(p));
     MTC_TRY(need_float(x, "x"));
     MTC_TRY(need_float(weight, "weight"));
@@ -486,10 +450,23 @@ int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bia
         MTC_TRY(zero_view(dw, stream));
         return zero_view(db, stream);
     }
-    return simt_path(p, stream);
+    // Small problems stay on the FMA units.
+    if (p.N * p.V < (int64_t{1} << 22) / (p.D + 1)) return simt_path(p, stream);
+    return linear_ce_tensor(p, stream);
 }
 
 }  // namespace
+
+int list_live_rows(const LinearCe &p, const LiveRows &live, cudaStream_t stream) {
+    unsigned long long *err = nullptr;
+    MTC_TRY(device_error_word(&err));
+    k_live_rows<<<1, 1024, 0, stream>>>(p, live, err);
+    MTC_TRY(check_launch("linear cross entropy (rows)"));
+    if (p.dx == nullptr || p.D == 0) return MTC_OK;
+    k_zero_dx<<<static_cast<unsigned>(p.N < 1184 ? p.N : 1184), 256, 0, stream>>>(p);
+    return check_launch("linear cross entropy (zero rows)");
+}
+
 }  // namespace mtc
 
 using namespace mtc;

@@ -1,0 +1,979 @@
+// Linear cross entropy on the tensor cores, with float32 accuracy.
+//
+// A float32 operand becomes a pair of 16-bit floats.  Scaled by a power of two that
+// brings the largest finite magnitude of its tensor to [2^14, 2^15), x is kept as
+//   hi = f16(x),  lo = f16((x - hi) * 2^11),   x = hi + lo * 2^-11 within 2^-22 |x|
+// for every |x| down to 2^-29 of the largest, and within 2^-51 of the largest below
+// (f16 ends at 2^-24, so an unscaled lo would end there; scaled, lo reaches 2^-35).
+// A product is three MMAs, hi.lo + lo.hi first and then hi.hi:
+//   a.b = hi.hi + 2^-11 (hi.lo + lo.hi)          (lo.lo is below 2^-22)
+// with the 2^-11 applied by the MMA itself (scale-input-d) when hi.hi is added.  f16
+// MMAs run at twice the rate of the TF32 ones that a split in TF32 would need.
+//
+// The tensor core truncates its accumulator at every addition, which over a long K
+// costs a part in 2^24 each time, always towards zero.  So 64 values of K stay in
+// tensor memory at most: the epilogue warps read each piece of 64 and add it, rounded
+// to nearest, to sums in registers, while the next piece runs in the other half of
+// tensor memory.  (The scale of the cross terms needs a piece to end there too.)
+//
+// All three products read the same packed operands, [row][64 columns][hi, lo], K-major
+// or MN-major by the matrix descriptors alone:
+//   logits   z  = x' w'^T   A = x' K-major,  B = w' K-major      softmax statistics in the epilogue
+//   dx       dx = g' w'     A = g' K-major,  B = w' MN-major     split along V when the tiles are few
+//   dweight  dw = g'^T x'   A = g' MN-major, B = x' MN-major     added up over the pieces of the rows
+// The logits of one piece of the rows are written once, as float32; k_softmax_grad
+// turns them into g' in place, 256 bytes of z into 128 of hi and 128 of lo.
+//
+// A pair of CTAs works on a 256 x 256 tile (tcgen05.mma.cta_group::2): each stages its
+// own 128 rows of A and 128 columns of B, 64 KB a stage for 1536 clocks of MMAs, three
+// stages deep.  Warp 0 loads (TMA), warp 1 of the leader issues, warps 2..9 are the
+// epilogue: two warps for each quarter of the tensor memory's lanes, 128 columns each.
+// Every wait is bounded; on expiry the device error word is set and the roles leave.
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <cstring>
+
+#include "linear_ce.cuh"
+#include "tcgen05.cuh"
+
+namespace mtc {
+namespace {
+
+constexpr int kBlock = 64;                       // columns of a packed block: 64 hi, 64 lo, 256 bytes
+constexpr int kTileRows = 256, kTileCols = 256;  // of a CTA pair
+constexpr int kOperandBytes = 32768;             // 128 rows (or columns) x 64 of K, hi and lo
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 3;
+constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+constexpr int kCtaThreads = 320;
+constexpr uint32_t kTmemCols = 512;
+
+// ---------------------------------------------------------------- packing --
+
+// Largest finite magnitude of a tensor -> the exponent of its scale.
+__device__ __forceinline__ int scale_exponent(int amax_bits) {
+    const float amax = __int_as_float(amax_bits);
+    if (amax == 0.0f) return 0;
+    int e;
+    frexpf(amax, &e);  // amax = m 2^e, 1/2 <= m < 1
+    const int s = 15 - e;
+    return s < 126 ? s : 126;
+}
+
+// x 2^e takes two of them: e reaches 2 x 126.
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+__device__ __forceinline__ void split_pair(float x, __half &hi, __half &lo) {
+    hi = __float2half_rn(x);
+    lo = __float2half_rn((x - __half2float(hi)) * 2048.0f);
+}
+
+struct PackSource {
+    const float *p;
+    int64_t rs, cs;
+    int64_t rows, cols;
+    const int *map;   // rows by way of the list of live rows; null: as they are
+    const int *live;  // their count; null: all
+    int vec;          // float4 loads
+    __half *to;       // [rows_out][blocks][2][64]
+    int64_t rows_out; // with zero rows behind the live ones, up to a multiple of 64
+    int *amax;
+};
+
+struct PackArgs {
+    PackSource s[2];
+    int64_t first_of_second;  // blocks of the grid before the second tensor
+    const float *dloss;       // its largest magnitude too; null: none
+    int *dloss_amax;
+    const int *dloss_count;
+};
+
+__device__ __forceinline__ void keep_max(float v, int *to) {
+    int bits = __float_as_int(v);
+    bits = __reduce_max_sync(0xFFFFFFFFu, bits);  // magnitudes order as their bits
+    __shared__ int part[8];
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = bits;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) bits = max(bits, part[i]);
+        if (bits > 0) atomicMax(to, bits);
+    }
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a <= 3.402823466e38f ? a : 0.0f;
+}
+
+__device__ __forceinline__ int64_t source_rows(const PackSource &s) {
+    return s.live != nullptr ? (*s.live < s.rows ? *s.live : s.rows) : s.rows;
+}
+
+__device__ __forceinline__ const float *source_row(const PackSource &s, int64_t r) {
+    return s.p + (s.map != nullptr ? s.map[r] : r) * s.rs;
+}
+
+// Largest finite magnitudes of x (rows with a loss), weight and dloss.  Each warp
+// takes rows in turn, four 16-byte loads in flight a lane.
+__global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
+    const bool second = blockIdx.x >= a.first_of_second;
+    const PackSource &s = a.s[second];
+    const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
+    const int64_t blocks = second ? gridDim.x - a.first_of_second : a.first_of_second;
+    const int lane = threadIdx.x % 32;
+    float m0 = 0.0f, m1 = 0.0f;
+    const int64_t rows = source_rows(s);
+    for (int64_t r = block * 8 + threadIdx.x / 32; r < rows; r += blocks * 8) {
+        const float *src = source_row(s, r);
+        if (s.vec) {
+            const float4 *v4 = reinterpret_cast<const float4 *>(src);
+            const int n4 = static_cast<int>(s.cols / 4);
+            int c = lane;
+            for (; c + 96 < n4; c += 128) {
+                float4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = __ldg(v4 + c + 32 * u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    m0 = fmaxf(m0, fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)));
+                    m1 = fmaxf(m1, fmaxf(finite_abs(v[u].z), finite_abs(v[u].w)));
+                }
+            }
+            for (; c < n4; c += 32) {
+                const float4 v = __ldg(v4 + c);
+                m0 = fmaxf(m0, fmaxf(finite_abs(v.x), finite_abs(v.y)));
+                m1 = fmaxf(m1, fmaxf(finite_abs(v.z), finite_abs(v.w)));
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t c = lane; c < s.cols; c += 32) m0 = fmaxf(m0, finite_abs(__ldg(src + c * s.cs)));
+        }
+    }
+    keep_max(fmaxf(m0, m1), s.amax);
+    if (a.dloss != nullptr && blockIdx.x == 0) {
+        float m = 0.0f;
+        for (int i = threadIdx.x; i < *a.dloss_count; i += 256) m = fmaxf(m, finite_abs(a.dloss[i]));
+        keep_max(m, a.dloss_amax);
+    }
+}
+
+// Each half-warp packs one block of 64 columns at a time: a lane four columns.
+__global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
+    const bool second = blockIdx.x >= a.first_of_second;
+    const PackSource &s = a.s[second];
+    const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
+    const int64_t grid = second ? gridDim.x - a.first_of_second : a.first_of_second;
+    const int64_t blocks = (s.cols + kBlock - 1) / kBlock;
+    const int64_t rows = source_rows(s);
+    const int64_t rows_out = s.live != nullptr && (rows + 63) / 64 * 64 < s.rows_out ? (rows + 63) / 64 * 64 : s.rows_out;
+    const int e = scale_exponent(*s.amax);
+    const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
+    const int lane = threadIdx.x % 16;
+    constexpr int U = 4;
+    const int64_t total = rows_out * blocks;
+    for (int64_t i0 = block * 16 * U + threadIdx.x / 16; i0 < total; i0 += grid * 16 * U) {
+        float4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = i0 + u * 16;
+            v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i >= total) continue;
+            const int64_t r = i / blocks, c = (i - r * blocks) * kBlock + lane * 4;
+            if (r >= rows || c >= s.cols) continue;
+            const float *src = source_row(s, r);
+            if (s.vec) {
+                v[u] = __ldg(reinterpret_cast<const float4 *>(src + c));
+            } else {
+                v[u].x = __ldg(src + c * s.cs);
+                if (c + 1 < s.cols) v[u].y = __ldg(src + (c + 1) * s.cs);
+                if (c + 2 < s.cols) v[u].z = __ldg(src + (c + 2) * s.cs);
+                if (c + 3 < s.cols) v[u].w = __ldg(src + (c + 3) * s.cs);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = i0 + u * 16;
+            if (i >= total) continue;
+            __half h[4], l[4];
+            split_pair(v[u].x * f0 * f1, h[0], l[0]);
+            split_pair(v[u].y * f0 * f1, h[1], l[1]);
+            split_pair(v[u].z * f0 * f1, h[2], l[2]);
+            split_pair(v[u].w * f0 * f1, h[3], l[3]);
+            __half *to = s.to + i * 2 * kBlock + lane * 4;
+            *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
+            *reinterpret_cast<uint2 *>(to + kBlock) = *reinterpret_cast<const uint2 *>(l);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- products --
+
+enum class Out { Logits, Sum };
+
+struct TileArgs {
+    int64_t M, N, K;  // M or K: of the piece, of which the first live ones count
+    const int *live;
+    int64_t first;
+    bool live_k;      // the live rows bound K instead of M
+    int tiles_n;
+    int group;        // row tiles that share a sweep of the columns
+    int splits;       // of K
+    const int *amax_a, *amax_b;
+    unsigned long long *err;
+    // Logits
+    float *z;         // [M][z_pitch], null: statistics alone
+    int64_t z_pitch;
+    const float *bias;
+    int64_t bias_s;
+    const int *target;
+    float *part_max, *part_sum;  // [M][2 tiles_n]
+    float *z_target;             // [M]
+    // Sum
+    float *out;       // final, or with splits the partial results [splits][M][N]
+    int64_t out_rs, out_cs;
+    const int *out_map;
+    int add;
+    int vec;          // float4 stores
+};
+
+__device__ __forceinline__ void tma_load_operand(void *dst, const CUtensorMap *map, uint32_t leader_bar, int row, int block) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(0), "r"(row), "r"(block), "r"(0)
+        : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle, version 1 (bit 46).  K-major: rows
+// of 128 bytes, eight rows 1024 bytes.  MN-major: 64 columns a row of 128 bytes, eight
+// rows of K 1024 bytes, the next 64 columns 8192 bytes on (64 rows of K).
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+    return ((addr & 0x3FFFFull) >> 4) | ((MN ? 8192ull >> 4 : 1ull) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+
+// D = F32, A = B = F16, M = 256 (two CTAs), N = 256.
+template <bool A_MN, bool B_MN>
+__device__ __forceinline__ constexpr uint32_t instr_desc() {
+    return (1u << 4) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) | (uint32_t(kTileCols >> 3) << 17) |
+           (uint32_t(kTileRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// D = A B + D 2^-11
+__device__ __forceinline__ void mma_pair_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(1)
+        : "memory");
+}
+
+struct Extent {
+    int64_t tiles_m, tiles, units;
+    int kblocks, per_split;
+    int64_t M;
+};
+
+__device__ __forceinline__ Extent extent_of(const TileArgs &a) {
+    Extent e;
+    int64_t K = a.K;
+    e.M = a.M;
+    if (a.live != nullptr) {
+        if (a.live_k) K = live_extent(a.live, a.first, K);
+        else e.M = live_extent(a.live, a.first, e.M);
+    }
+    e.kblocks = static_cast<int>((K + kBlock - 1) / kBlock);
+    e.tiles_m = (e.M + kTileRows - 1) / kTileRows;
+    e.tiles = e.tiles_m * a.tiles_n;
+    e.units = e.tiles * a.splits;
+    if (a.live_k && K == 0 && a.first > 0) e.units = 0;  // nothing left to add
+    e.per_split = (e.kblocks + a.splits - 1) / a.splits;
+    return e;
+}
+
+// Unit u: split u / tiles (the tiles of a split run next to one another and share
+// their panels in L2), and its tile in groups of row tiles.
+__device__ __forceinline__ void unit_of(const TileArgs &a, const Extent &e, int64_t u, int &tm, int &tn, int &split,
+                                        int &kb0, int &kb1) {
+    split = static_cast<int>(u / e.tiles);
+    const int64_t t = u - split * e.tiles;
+    const int64_t span = static_cast<int64_t>(a.group) * a.tiles_n;
+    const int64_t g = t / span;
+    const int64_t first_m = g * a.group;
+    const int64_t size = e.tiles_m - first_m < a.group ? e.tiles_m - first_m : a.group;
+    const int64_t in_group = t - g * span;
+    tm = static_cast<int>(first_m + in_group % size);
+    tn = static_cast<int>(in_group / size);
+    kb0 = split * e.per_split;
+    kb1 = kb0 + e.per_split < e.kblocks ? kb0 + e.per_split : e.kblocks;
+    if (kb1 < kb0) kb1 = kb0;
+}
+
+// The logits' epilogue: this thread's row, 128 columns from col0 on.
+__device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float (&acc)[128], int64_t row, int64_t col0,
+                                             int part, float f0, float f1) {
+    if (row >= M || col0 >= a.N) return;
+    const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
+    const int target = a.target[a.first + row] - static_cast<int>(col0);
+    float top = -INFINITY, zt = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) {
+        float z = acc[j] * f0 * f1;
+        if (a.bias != nullptr && j < n) z += __ldg(a.bias + (col0 + j) * a.bias_s);
+        acc[j] = j < n ? z : -INFINITY;
+        top = fmaxf(top, acc[j]);
+        if (j == target) zt = z;
+    }
+    const float base = isinf(top) ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 128; ++j) sum += expf(acc[j] - base);
+    a.part_max[row * 2 * a.tiles_n + part] = top;
+    a.part_sum[row * 2 * a.tiles_n + part] = sum;
+    if (target >= 0 && target < n) a.z_target[row] = zt;
+    if (a.z == nullptr) return;
+    float4 *to = reinterpret_cast<float4 *>(a.z + row * a.z_pitch + col0);  // rows are padded to 64 columns
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (4 * j < n) to[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+}
+
+__device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&acc)[128], int64_t row, int64_t col0,
+                                          int split, float f0, float f1) {
+    if (row >= M || col0 >= a.N) return;
+    const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
+#pragma unroll
+    for (int j = 0; j < 128; ++j) acc[j] = acc[j] * f0 * f1;
+    float *to;
+    int64_t cs = 1;
+    if (a.splits > 1) {
+        to = a.out + (split * a.M + row) * a.N + col0;
+    } else {
+        cs = a.out_cs;
+        to = a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0 * cs;
+    }
+    const bool add = a.add && a.splits == 1;
+    if (a.vec) {
+        float4 *v = reinterpret_cast<float4 *>(to);
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 4) {
+            float4 old[4];
+            if (add) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (4 * (j0 + j) < n) old[j] = v[j0 + j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = 4 * (j0 + j);
+                float4 x = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                if (add) {
+                    x.x += old[j].x;
+                    x.y += old[j].y;
+                    x.z += old[j].z;
+                    x.w += old[j].w;
+                }
+                if (c < n) v[j0 + j] = x;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+            if (j < n) to[j * cs] = add ? to[j * cs] + acc[j] : acc[j];
+    }
+}
+
+template <bool A_MN, bool B_MN, Out MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
+    k_pair_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const TileArgs args) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    // the same aligned offset in both CTAs (same dynamic size, same static layout)
+    unsigned char *smem =
+        reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes);  // leader's: both CTAs' bytes
+    uint64_t *empty = full + kStages;    // each CTA's: the stage's MMAs are done
+    uint64_t *acc_full = empty + kStages;  // [2] each CTA's: a piece is in tensor memory
+    uint64_t *acc_empty = acc_full + 2;    // [2] leader's: both epilogues have read it
+    uint64_t *drain = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int64_t cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+    const Extent e = extent_of(args);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 16);  // 8 epilogue warps x 2 CTAs
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int64_t it = 0;
+            bool ok = true;
+            for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                int tm, tn, split, kb0, kb1;
+                unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
+                const int b0 = tn * kTileCols + static_cast<int>(rank) * 128;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int s = static_cast<int>(it % kStages);
+                    if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / kStages) & 1u) ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    unsigned char *st = smem + s * kStageBytes;
+                    if (leader) mbar_expect_tx(&full[s], 2 * kStageBytes);
+                    const uint32_t fb = peer_addr(&full[s], 0);
+                    tma_load_operand(st, &map_a, fb, A_MN ? kb * kBlock : a0, A_MN ? a0 / kBlock : kb);
+                    tma_load_operand(st + kOperandBytes, &map_b, fb, B_MN ? kb * kBlock : b0, B_MN ? b0 / kBlock : kb);
+                }
+            }
+            if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+            if (leader) {  // every stage issued by the pair has landed before the cluster exits
+                for (int64_t d = it > kStages ? it - kStages : 0; d < it; ++d) {
+                    const uint32_t round = static_cast<uint32_t>(d / kStages);
+                    for (long long i = 0; i < kWaitLimit && !mbar_try_wait(&full[d % kStages], round & 1u); ++i) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            constexpr uint32_t idesc = instr_desc<A_MN, B_MN>();
+            constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
+            constexpr uint64_t lo = (kOperandBytes / 2) >> 4;
+            int64_t it = 0;
+            bool ok = true;
+            for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                int tm, tn, split, kb0, kb1;
+                unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int s = static_cast<int>(it % kStages);
+                    const int b = static_cast<int>(it & 1);
+                    if (!mbar_wait(&acc_empty[b], (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, abort_flag) ||
+                        !mbar_wait(&full[s], static_cast<uint32_t>(it / kStages) & 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(b * kTileCols);
+                    const uint32_t st = smem_u32(smem + s * kStageBytes);
+                    const uint64_t da = operand_desc<A_MN>(st), db = operand_desc<B_MN>(st + kOperandBytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        mma_pair(d, da + k * a_step, db + lo + k * b_step, idesc, k > 0);
+                        mma_pair(d, da + lo + k * a_step, db + k * b_step, idesc, 1);
+                    }
+                    mma_pair_scaled(d, da, db, idesc);
+#pragma unroll
+                    for (int k = 1; k < 4; ++k) mma_pair(d, da + k * a_step, db + k * b_step, idesc, 1);
+                    umma_commit_both(&empty[s]);
+                    umma_commit_both(&acc_full[b]);
+                }
+            }
+            if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+            umma_commit_pair_local(drain);  // all MMAs of the pair are done before either CTA frees tensor memory
+            for (long long i = 0; i < kWaitLimit && !mbar_try_wait(drain, 0u); ++i) {
+            }
+        }
+    } else {
+        const int quadrant = warp % 4, half = (warp - 2) / 4;
+        const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
+        const int scale = -(scale_exponent(*args.amax_a) + scale_exponent(*args.amax_b));
+        const float f0 = power_of_two(scale / 2), f1 = power_of_two(scale - scale / 2);
+        int64_t it = 0;
+        bool ok = true;
+        for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+            int tm, tn, split, kb0, kb1;
+            unit_of(args, e, u, tm, tn, split, kb0, kb1);
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int b = static_cast<int>(it & 1);
+                if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(it >> 1) & 1u, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t at = tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16) +
+                                    static_cast<uint32_t>(b * kTileCols + half * 128);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float v[32];
+                    tmem_ld32(at + static_cast<uint32_t>(c * 32), v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[c * 32 + j] += v[j];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(release[b]);
+            }
+            if (!ok) break;
+            const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
+            const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
+            if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, f0, f1);
+            else store_sum(args, e.M, acc, row, col0, split, f0, f1);
+            __syncwarp();
+        }
+        if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the leader's MMAs into this CTA's tensor memory have drained
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols));
+    }
+}
+
+// The splits' partial results in order, into the rows of the result.
+__global__ void __launch_bounds__(256) k_join_splits(const TileArgs a) {
+    int64_t M = a.M;
+    if (a.live != nullptr && !a.live_k) M = live_extent(a.live, a.first, M);
+    if (a.live_k && a.first > 0 && live_extent(a.live, a.first, a.K) == 0) return;
+    const float *parts = a.part_sum;
+    const int64_t plane = a.M * a.N;
+    if (a.vec) {
+        const int64_t per_row = a.N / 4;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < M * per_row;
+             i += static_cast<int64_t>(gridDim.x) * 256) {
+            const int64_t r = i / per_row, c = (i - r * per_row) * 4;
+            const float *src = parts + r * a.N + c;
+            float4 sum = *reinterpret_cast<const float4 *>(src);
+            for (int s = 1; s < a.splits; ++s) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + s * plane);
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            }
+            float4 *to = reinterpret_cast<float4 *>(
+                a.out + (a.out_map != nullptr ? a.out_map[a.first + r] : r) * a.out_rs + c);
+            if (a.add) {
+                const float4 o = *to;
+                sum.x += o.x;
+                sum.y += o.y;
+                sum.z += o.z;
+                sum.w += o.w;
+            }
+            *to = sum;
+        }
+        return;
+    }
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < M * a.N;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / a.N, c = i - r * a.N;
+        float sum = parts[i];
+        for (int s = 1; s < a.splits; ++s) sum += parts[s * plane + i];
+        float *to = a.out + (a.out_map != nullptr ? a.out_map[a.first + r] : r) * a.out_rs + c * a.out_cs;
+        *to = a.add ? *to + sum : sum;
+    }
+}
+
+// ----------------------------------------------------------------- softmax --
+
+struct RowArgs {
+    int64_t first, rows;  // of the live rows
+    const int *live;
+    int parts, part_pitch;  // of a row
+    const float *part_max, *part_sum, *z_target;
+    const int *row;       // of x
+    float *lse_live;      // [rows]
+    float *loss, *lse;
+    int64_t loss_s, lse_s;
+};
+
+// One warp a row: the statistics of its tiles make lse and the loss.
+__global__ void __launch_bounds__(256) k_row_loss(const RowArgs a) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (r >= live_extent(a.live, a.first, a.rows)) return;
+    const float *m = a.part_max + r * a.part_pitch, *s = a.part_sum + r * a.part_pitch;
+    float top = -INFINITY;
+    for (int j = lane; j < a.parts; j += 32) top = fmaxf(top, m[j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float base = isinf(top) ? 0.0f : top;
+    float sum = 0.0f;
+    for (int j = lane; j < a.parts; j += 32) {
+        const float mj = isinf(m[j]) ? 0.0f : m[j];
+        if (s[j] != 0.0f) sum += s[j] * expf(mj - base);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane != 0) return;
+    const float lse = base + logf(sum);
+    a.lse_live[r] = lse;
+    const int64_t n = a.row[a.first + r];
+    if (a.lse != nullptr) a.lse[n * a.lse_s] = lse;
+    if (a.loss != nullptr) a.loss[n * a.loss_s] = lse - a.z_target[r];
+}
+
+struct GradArgs {
+    int64_t first, rows;
+    const int *live;
+    int64_t V;
+    float *z;            // [rows][pitch], becomes g'
+    int64_t pitch;
+    const float *lse_live;
+    const int *target;
+    const float *dloss;
+    const int *amax;     // of dloss
+    float *column_parts; // [row blocks][pitch] column sums of g; null: not wanted
+};
+
+constexpr int kGradRows = 64;  // rows of a CTA
+
+// z -> g' in place.  A CTA takes 128 columns of 64 rows, a warp eight of the rows, a lane
+// four columns: 512 bytes of z a load, two blocks of 128 + 128 bytes a store.
+__global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
+    const int64_t live = live_extent(a.live, a.first, a.rows);
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kGradRows;
+    if (r0 >= (live + 63) / 64 * 64) return;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + lane * 4;
+    const bool in = c < a.pitch;
+    const int e = scale_exponent(*a.amax);
+    const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
+    float4 column = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int j0 = 0; j0 < kGradRows / 8; j0 += 4) {
+        float4 z[4];
+        float lse[4], d[4];
+        int t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = r0 + (j0 + j) * 8 + warp;
+            z[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            lse[j] = d[j] = 0.0f;
+            t[j] = -1;
+            if (r < live) {
+                if (in) z[j] = *reinterpret_cast<const float4 *>(a.z + r * a.pitch + c);
+                lse[j] = a.lse_live[r];
+                d[j] = a.dloss[a.first + r];
+                t[j] = a.target[a.first + r];
+            }
+        }
+        __syncwarp();  // the whole block is read before any lane overwrites it
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = r0 + (j0 + j) * 8 + warp;
+            float g[4] = {z[j].x, z[j].y, z[j].z, z[j].w};
+            __half h[4], l[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float x = g[k] - lse[j];
+                g[k] = c + k < a.V && r < live ? d[j] * (c + k == t[j] ? expm1f(x) : expf(x)) : 0.0f;
+                split_pair(g[k] * f0 * f1, h[k], l[k]);
+            }
+            column.x += g[0];
+            column.y += g[1];
+            column.z += g[2];
+            column.w += g[3];
+            if (in && r < a.rows) {
+                __half *to = reinterpret_cast<__half *>(a.z + r * a.pitch + c / kBlock * kBlock) + c % kBlock;
+                *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
+                *reinterpret_cast<uint2 *>(to + kBlock) = *reinterpret_cast<const uint2 *>(l);
+            }
+        }
+    }
+    if (a.column_parts == nullptr) return;
+    __shared__ float4 sums[8][32];
+    sums[warp][lane] = column;
+    __syncthreads();
+    if (warp != 0 || !in) return;
+    for (int w = 1; w < 8; ++w) {
+        column.x += sums[w][lane].x;
+        column.y += sums[w][lane].y;
+        column.z += sums[w][lane].z;
+        column.w += sums[w][lane].w;
+    }
+    *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) = column;
+}
+
+__global__ void __launch_bounds__(256) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
+    const int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (v >= a.V) return;
+    const int blocks = static_cast<int>((live_extent(a.live, a.first, a.rows) + kGradRows - 1) / kGradRows);
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int b = 0; b < blocks; ++b) sum += a.column_parts[b * a.pitch + v];
+    db[v * db_s] = add ? db[v * db_s] + sum : sum;
+}
+
+// ------------------------------------------------------------------- host --
+
+// Tensor map of a packed operand: (64 columns, rows, blocks, hi / lo).
+int operand_map(CUtensorMap &map, const __half *base, int64_t rows, int64_t blocks, int64_t pitch_blocks, bool mn) {
+    EncodeTiled enc = tensor_map_encoder();
+    if (enc == nullptr) return fail(MTC_ERR_RUNTIME, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[4] = {kBlock, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(blocks), 2};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(pitch_blocks) * 256, 256, 128};
+    const cuuint32_t box[4] = {kBlock, mn ? 64u : 128u, mn ? 2u : 1u, 2};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half *>(base), dims, strides, box, elem,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MTC_ERR_RUNTIME, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return MTC_OK;
+}
+
+template <bool A_MN, bool B_MN, Out MODE>
+int launch_product(const CUtensorMap &a, const CUtensorMap &b, const TileArgs &args, int sms, cudaStream_t stream) {
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_pair_product<A_MN, B_MN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kSmemBytes));
+    const int64_t units = (args.M + kTileRows - 1) / kTileRows * args.tiles_n * args.splits;
+    const int64_t pairs = units < sms / 2 ? units : sms / 2;
+    k_pair_product<A_MN, B_MN, MODE><<<static_cast<unsigned>(2 * pairs), kCtaThreads, kSmemBytes, stream>>>(a, b, args);
+    return check_launch("linear cross entropy (tensor-core product)");
+}
+
+// Splits of K so that the tiles of a product fill the pairs of SMs: the fewest whose
+// last wave is nearly full, each at least 512 of K.
+int choose_splits(int64_t tiles, int64_t K, int64_t pairs, size_t bytes) {
+    int best = 1;
+    double best_cost = 1e30;
+    for (int s = 1; s <= 16; ++s) {
+        if (s > 1 && (K / s < 512 || bytes * s > (size_t{1} << 30))) break;
+        const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
+        const double cost = waves / s * (1.0 + 0.01 * (s - 1));
+        if (cost < best_cost * 0.98) {
+            best_cost = cost;
+            best = s;
+        }
+    }
+    return best;
+}
+
+bool vector_source(const float *p, int64_t rs, int64_t cs, int64_t cols) {
+    return aligned16(p) && cs == 1 && rs % 4 == 0 && cols % 4 == 0;
+}
+
+}  // namespace
+
+int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
+    const int sms = sm_count(current_device());
+    const int64_t pairs = sms / 2;
+    const bool grads = p.dloss != nullptr && ((p.D > 0 && (p.dx != nullptr || p.dw != nullptr)) || p.db != nullptr);
+    const int64_t d_blocks = (p.D + kBlock - 1) / kBlock, v_blocks = (p.V + kBlock - 1) / kBlock;
+    const int64_t pitch = v_blocks * kBlock;
+    const int tiles_v = static_cast<int>((p.V + kTileCols - 1) / kTileCols);
+    const int tiles_d = static_cast<int>((p.D + kTileCols - 1) / kTileCols);
+    // rows at a time: the logits of a piece fill at most 2 GiB; without gradients only
+    // their statistics are kept, 8 bytes for 128 logits
+    const int64_t rows_all = (p.N + 255) / 256 * 256;
+    const int64_t row_bytes = grads ? pitch * 4 : static_cast<int64_t>(tiles_v) * 16;
+    int64_t piece = (int64_t{2} << 30) / row_bytes / 256 * 256;
+    if (piece < 256) piece = 256;
+    if (piece > (int64_t{1} << 21)) piece = int64_t{1} << 21;  // k_softmax_grad's grid
+    const int64_t pieces = (rows_all + piece - 1) / piece;
+    piece = ((rows_all + pieces - 1) / pieces + 255) / 256 * 256;
+    if (rows_all * d_blocks > (int64_t{1} << 40) || pitch > INT32_MAX)
+        return fail(MTC_ERR_UNSUPPORTED, "linear cross entropy: too large");
+
+    const int splits_dx = choose_splits(piece / 256 * tiles_d, p.V, pairs, static_cast<size_t>(piece) * p.D * 4);
+    const int splits_dw = choose_splits(static_cast<int64_t>(tiles_v) * tiles_d, piece, pairs,
+                                        static_cast<size_t>(p.V) * p.D * 4);
+    const size_t list = padded(static_cast<size_t>(p.N) * 4);
+    const size_t x_bytes = padded(static_cast<size_t>(rows_all) * d_blocks * 256);
+    const size_t w_bytes = padded(static_cast<size_t>(p.V) * d_blocks * 256);
+    const size_t stat = padded(static_cast<size_t>(piece) * 2 * tiles_v * 4);
+    const size_t row_stat = padded(static_cast<size_t>(piece) * 4);
+    const size_t z_bytes = grads ? padded(static_cast<size_t>(piece) * pitch * 4) : 0;
+    const size_t col_bytes = p.db != nullptr ? padded(static_cast<size_t>(piece / kGradRows) * pitch * 4) : 0;
+    const size_t split_dx = p.dx != nullptr && splits_dx > 1 ? static_cast<size_t>(splits_dx) * piece * p.D * 4 : 0;
+    const size_t split_dw = p.dw != nullptr && splits_dw > 1 ? static_cast<size_t>(splits_dw) * p.V * p.D * 4 : 0;
+    const size_t split_bytes = grads ? padded(split_dx > split_dw ? split_dx : split_dw) : 0;
+    Workspace ws;
+    MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 2 * row_stat + z_bytes + col_bytes + split_bytes,
+                        stream));
+    LiveRows live;
+    live.count = ws.take<int>(256);
+    live.row = ws.take<int>(list);
+    live.target = ws.take<int>(list);
+    live.dloss = ws.take<float>(list);
+    __half *xp = ws.take<__half>(x_bytes);
+    __half *wp = ws.take<__half>(w_bytes);
+    float *part_max = ws.take<float>(stat);
+    float *part_sum = ws.take<float>(stat);
+    float *z_target = ws.take<float>(row_stat);
+    float *lse_live = ws.take<float>(row_stat);
+    float *z = ws.take<float>(z_bytes);
+    float *columns = ws.take<float>(col_bytes);
+    float *split_ws = ws.take<float>(split_bytes);
+    unsigned long long *err = nullptr;
+    MTC_TRY(device_error_word(&err));
+    MTC_TRY(list_live_rows(p, live, stream));
+
+    PackArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.s[0] = PackSource{p.x, p.x_rs, p.x_cs, p.N, p.D, live.row, live.count, vector_source(p.x, p.x_rs, p.x_cs, p.D),
+                        xp, rows_all, live.count + 1};
+    k.s[1] = PackSource{p.w, p.w_rs, p.w_cs, p.V, p.D, nullptr, nullptr, vector_source(p.w, p.w_rs, p.w_cs, p.D),
+                        wp, p.V, live.count + 2};
+    if (grads) k.dloss = live.dloss;
+    k.dloss_amax = live.count + 3;
+    k.dloss_count = live.count;
+    // CTAs in proportion to the tensors' rows, eight to an SM in all
+    const int64_t most = static_cast<int64_t>(sms) * 8;
+    const int64_t share = most * p.N / (p.N + p.V);
+    k.first_of_second = share < 1 ? 1 : share > most - 1 ? most - 1 : share;
+    k_largest<<<static_cast<unsigned>(most), 256, 0, stream>>>(k);
+    MTC_TRY(check_launch("linear cross entropy (magnitudes)"));
+    if (p.D > 0) {
+        k_pack<<<static_cast<unsigned>(most), 256, 0, stream>>>(k);
+        MTC_TRY(check_launch("linear cross entropy (packing)"));
+    }
+
+    CUtensorMap x_k, w_k, w_mn, x_mn, g_k, g_mn;
+    const int64_t map_blocks = d_blocks > 0 ? d_blocks : 1;
+    for (int64_t first = 0; first < p.N; first += piece) {
+        const int64_t rows = p.N - first < piece ? p.N - first : piece;
+        const int64_t rows_up = (rows + 63) / 64 * 64;
+        const __half *xc = xp + first * d_blocks * 2 * kBlock;
+        MTC_TRY(operand_map(x_k, xc, rows_up, map_blocks, map_blocks, false));
+        MTC_TRY(operand_map(w_k, wp, p.V, map_blocks, map_blocks, false));
+        TileArgs t;
+        std::memset(&t, 0, sizeof(t));
+        t.M = rows;
+        t.N = p.V;
+        t.K = p.D;
+        t.live = live.count;
+        t.first = first;
+        t.tiles_n = tiles_v;
+        t.group = 16;
+        t.splits = 1;
+        t.amax_a = live.count + 1;
+        t.amax_b = live.count + 2;
+        t.err = err;
+        t.z = grads ? z : nullptr;
+        t.z_pitch = pitch;
+        t.bias = p.bias;
+        t.bias_s = p.b_s;
+        t.target = live.target;
+        t.part_max = part_max;
+        t.part_sum = part_sum;
+        t.z_target = z_target;
+        MTC_TRY((launch_product<false, false, Out::Logits>(x_k, w_k, t, sms, stream)));
+        // (a last tile of 128 columns or less has no second half)
+        const RowArgs ra{first, rows, live.count, static_cast<int>((p.V + 127) / 128), 2 * tiles_v, part_max, part_sum,
+                         z_target, live.row, lse_live, p.loss, p.lse, p.loss_s, p.lse_s};
+        k_row_loss<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(ra);
+        MTC_TRY(check_launch("linear cross entropy (loss)"));
+        if (!grads) continue;
+        const GradArgs ga{first, rows_up, live.count, p.V, z, pitch, lse_live, live.target, live.dloss, live.count + 3,
+                          p.db != nullptr ? columns : nullptr};
+        const dim3 grid(static_cast<unsigned>((pitch + 127) / 128), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
+        k_softmax_grad<<<grid, 256, 0, stream>>>(ga);
+        MTC_TRY(check_launch("linear cross entropy (gradient of the logits)"));
+        if (p.db != nullptr) {
+            k_bias_grad<<<static_cast<unsigned>((p.V + 255) / 256), 256, 0, stream>>>(ga, p.db, p.db_s, first > 0);
+            MTC_TRY(check_launch("linear cross entropy (bias gradient)"));
+        }
+        const __half *gp = reinterpret_cast<const __half *>(z);
+        if (p.dx != nullptr && p.D > 0) {
+            MTC_TRY(operand_map(g_k, gp, rows_up, v_blocks, v_blocks, false));
+            MTC_TRY(operand_map(w_mn, wp, p.V, d_blocks, d_blocks, true));
+            std::memset(&t, 0, sizeof(t));
+            t.M = rows;
+            t.N = p.D;
+            t.K = p.V;
+            t.live = live.count;
+            t.first = first;
+            t.tiles_n = tiles_d;
+            t.group = 16;
+            t.splits = splits_dx;
+            t.amax_a = live.count + 3;
+            t.amax_b = live.count + 2;
+            t.err = err;
+            t.out_rs = p.dx_rs;
+            t.out_cs = p.dx_cs;
+            t.out_map = live.row;
+            const bool vec = aligned16(p.dx) && p.dx_cs == 1 && p.dx_rs % 4 == 0 && p.D % 4 == 0;
+            t.out = splits_dx > 1 ? split_ws : p.dx;
+            t.vec = splits_dx > 1 ? p.D % 4 == 0 : vec;
+            MTC_TRY((launch_product<false, true, Out::Sum>(g_k, w_mn, t, sms, stream)));
+            if (splits_dx > 1) {
+                t.part_sum = split_ws;
+                t.out = p.dx;
+                t.vec = vec;
+                k_join_splits<<<static_cast<unsigned>(sms * 8), 256, 0, stream>>>(t);
+                MTC_TRY(check_launch("linear cross entropy (input gradient)"));
+            }
+        }
+        if (p.dw != nullptr && p.D > 0) {
+            MTC_TRY(operand_map(g_mn, gp, rows_up, v_blocks, v_blocks, true));
+            MTC_TRY(operand_map(x_mn, xc, rows_up, d_blocks, d_blocks, true));
+            std::memset(&t, 0, sizeof(t));
+            t.M = p.V;
+            t.N = p.D;
+            t.K = rows;
+            t.live = live.count;
+            t.live_k = true;
+            t.first = first;
+            t.tiles_n = tiles_d;
+            t.group = 16;
+            t.splits = splits_dw;
+            t.amax_a = live.count + 3;
+            t.amax_b = live.count + 1;
+            t.err = err;
+            t.out_rs = p.dw_rs;
+            t.out_cs = p.dw_cs;
+            t.add = first > 0;
+            const bool vec = aligned16(p.dw) && p.dw_cs == 1 && p.dw_rs % 4 == 0 && p.D % 4 == 0;
+            t.out = splits_dw > 1 ? split_ws : p.dw;
+            t.vec = splits_dw > 1 ? p.D % 4 == 0 : vec;
+            MTC_TRY((launch_product<true, true, Out::Sum>(g_mn, x_mn, t, sms, stream)));
+            if (splits_dw > 1) {
+                t.part_sum = split_ws;
+                t.out = p.dw;
+                t.vec = vec;
+                k_join_splits<<<static_cast<unsigned>(sms * 8), 256, 0, stream>>>(t);
+                MTC_TRY(check_launch("linear cross entropy (weight gradient)"));
+            }
+        }
+    }
+    return MTC_OK;
+}
+
+}  // namespace mtc
