@@ -11,10 +11,13 @@
 // MMAs run at twice the rate of the TF32 ones that a split in TF32 would need.
 //
 // The tensor core truncates its accumulator at every addition, which over a long K
-// costs a part in 2^24 each time, always towards zero.  So 64 values of K stay in
-// tensor memory at most: the epilogue warps read each piece of 64 and add it, rounded
+// costs a part in 2^24 each time, always towards zero.  So 128 values of K stay in
+// tensor memory at most: the epilogue warps read each piece of 128 and add it, rounded
 // to nearest, to sums in registers, while the next piece runs in the other half of
-// tensor memory.  (The scale of the cross terms needs a piece to end there too.)
+// tensor memory.  A piece is the cross terms of its two blocks of 64, then the hi.hi of
+// both.  (Pieces of 64 were 20 % slower: a piece's hand-over, from the MMAs' commit by
+// way of the epilogues of both CTAs to the next MMA, takes some 1500 clocks and the
+// reading 700, which two pieces of 1536 clocks do not cover and two of 3072 do.)
 //
 // All three products read the same packed operands, [row][64 columns][hi, lo], K-major
 // or MN-major by the matrix descriptors alone:
@@ -25,9 +28,13 @@
 // turns them into g' in place, 256 bytes of z into 128 of hi and 128 of lo.
 //
 // A pair of CTAs works on a 256 x 256 tile (tcgen05.mma.cta_group::2): each stages its
-// own 128 rows of A and 128 columns of B, 64 KB a stage for 1536 clocks of MMAs, three
-// stages deep.  Warp 0 loads (TMA), warp 1 of the leader issues, warps 2..9 are the
-// epilogue: two warps for each quarter of the tensor memory's lanes, 128 columns each.
+// own 128 rows of A and 128 columns of B, 64 KB for 1536 clocks of MMAs.  The lo halves
+// are free after a piece's cross terms, the hi halves only at its end, so each has a ring
+// of its own: four stages of hi, two of lo, 32 KB each.  Warp 0 loads (TMA), warp 1 of the leader issues, warps 4..11 are the
+// epilogue: two warps for each quarter of the tensor memory's lanes, 128 columns each,
+// with 208 registers a thread (128 sums, 64 of a load in flight) that the first four
+// warps give up.  Results leave through 4 KB of shared memory a warp, so that a store
+// covers whole lines of four rows and not 16 bytes of 32.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
@@ -42,11 +49,17 @@ namespace {
 
 constexpr int kBlock = 64;                       // columns of a packed block: 64 hi, 64 lo, 256 bytes
 constexpr int kTileRows = 256, kTileCols = 256;  // of a CTA pair
-constexpr int kOperandBytes = 32768;             // 128 rows (or columns) x 64 of K, hi and lo
-constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kStages = 3;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
-constexpr int kCtaThreads = 320;
+constexpr int kOperandBytes = 16384;             // 128 rows (or columns) x 64 of K, hi or lo
+constexpr int kStageBytes = 2 * kOperandBytes;   // A and B
+constexpr int kHiStages = 4, kLoStages = 2;
+constexpr int kStages = kHiStages + kLoStages;
+constexpr int kPieceBlocks = 2;                  // blocks of K that are summed in tensor memory
+constexpr int kStageOut = 4096;  // 32 rows x 32 columns of an epilogue warp
+constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStageOut + 1024 + 256;
+constexpr int kCtaThreads = 384;
+constexpr int kEpilogueRegs = 208, kOtherRegs = 88;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+static_assert(256 * kEpilogueRegs + 128 * kOtherRegs <= kCtaThreads * 168, "registers of the launch (168 a thread)");
 constexpr uint32_t kTmemCols = 512;
 
 // ---------------------------------------------------------------- packing --
@@ -238,11 +251,12 @@ struct TileArgs {
     int vec;          // float4 stores
 };
 
-__device__ __forceinline__ void tma_load_operand(void *dst, const CUtensorMap *map, uint32_t leader_bar, int row, int block) {
+__device__ __forceinline__ void tma_load_operand(void *dst, const CUtensorMap *map, uint32_t leader_bar, int row, int block,
+                                                 int lo) {
     asm volatile(
         "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
         "[%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(0), "r"(row), "r"(block), "r"(0)
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(0), "r"(row), "r"(block), "r"(lo)
         : "memory");
 }
 
@@ -322,78 +336,144 @@ __device__ __forceinline__ void unit_of(const TileArgs &a, const Extent &e, int6
     if (kb1 < kb0) kb1 = kb0;
 }
 
-// The logits' epilogue: this thread's row, 128 columns from col0 on.
-__device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float (&acc)[128], int64_t row, int64_t col0,
-                                             int part, float f0, float f1) {
-    if (row >= M || col0 >= a.N) return;
-    const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
-    const int target = a.target[a.first + row] - static_cast<int>(col0);
-    float top = -INFINITY, zt = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 128; ++j) {
-        float z = acc[j] * f0 * f1;
-        if (a.bias != nullptr && j < n) z += __ldg(a.bias + (col0 + j) * a.bias_s);
-        acc[j] = j < n ? z : -INFINITY;
-        top = fmaxf(top, acc[j]);
-        if (j == target) zt = z;
-    }
-    const float base = isinf(top) ? 0.0f : top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 128; ++j) sum += expf(acc[j] - base);
-    a.part_max[row * 2 * a.tiles_n + part] = top;
-    a.part_sum[row * 2 * a.tiles_n + part] = sum;
-    if (target >= 0 && target < n) a.z_target[row] = zt;
-    if (a.z == nullptr) return;
-    float4 *to = reinterpret_cast<float4 *>(a.z + row * a.z_pitch + col0);  // rows are padded to 64 columns
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-        if (4 * j < n) to[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&acc)[128], int64_t row, int64_t col0,
-                                          int split, float f0, float f1) {
-    if (row >= M || col0 >= a.N) return;
-    const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
+// A warp's 32 rows x n columns from the lanes' registers to memory, 32 columns at a time
+// through `stage`: written as 16-byte chunks XOR-swizzled by the row, read back as four
+// rows of 128 bytes (vec) or one row of 32 values at a time.  `to`: where this lane's row
+// begins, null for a row that is not stored.
+__device__ __forceinline__ void store_rows(float *stage, const float (&acc)[128], float *to, int n, int64_t cs, bool vec,
+                                           bool add) {
+    const int lane = threadIdx.x % 32;
+    float4 *s4 = reinterpret_cast<float4 *>(stage);
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(to);
 #pragma unroll
-    for (int j = 0; j < 128; ++j) acc[j] = acc[j] * f0 * f1;
-    float *to;
-    int64_t cs = 1;
-    if (a.splits > 1) {
-        to = a.out + (split * a.M + row) * a.N + col0;
-    } else {
-        cs = a.out_cs;
-        to = a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0 * cs;
-    }
-    const bool add = a.add && a.splits == 1;
-    if (a.vec) {
-        float4 *v = reinterpret_cast<float4 *>(to);
+    for (int c = 0; c < 4; ++c) {
+        if (c * 32 >= n) break;
+        __syncwarp();
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 4) {
-            float4 old[4];
-            if (add) {
+        for (int j = 0; j < 8; ++j)
+            s4[lane * 8 + (j ^ (lane & 7))] =
+                make_float4(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3]);
+        __syncwarp();
+        if (vec) {
+            const int j = lane % 8, col = c * 32 + 4 * j;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (4 * (j0 + j) < n) old[j] = v[j0 + j];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = 4 * (j0 + j);
-                float4 x = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + lane / 8;
+                float *row = reinterpret_cast<float *>(__shfl_sync(0xFFFFFFFFu, mine, r));
+                float4 x = s4[r * 8 + (j ^ (r & 7))];
+                if (row == nullptr || col >= n) continue;
+                float4 *p = reinterpret_cast<float4 *>(row + col);
                 if (add) {
-                    x.x += old[j].x;
-                    x.y += old[j].y;
-                    x.z += old[j].z;
-                    x.w += old[j].w;
+                    const float4 o = *p;
+                    x.x += o.x;
+                    x.y += o.y;
+                    x.z += o.z;
+                    x.w += o.w;
                 }
-                if (c < n) v[j0 + j] = x;
+                *p = x;
+            }
+        } else {
+            const int col = c * 32 + lane;
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+                float *row = reinterpret_cast<float *>(__shfl_sync(0xFFFFFFFFu, mine, r));
+                const float x = stage[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+                if (row == nullptr || col >= n) continue;
+                float *p = row + col * cs;
+                *p = add ? *p + x : x;
             }
         }
-    } else {
+    }
+}
+
+// x 2^e in place; e beyond float32's exponents takes a second factor.
+__device__ __forceinline__ void rescale(float (&acc)[128], float f0, float f1) {
+#pragma unroll
+    for (int j = 0; j < 128; ++j) acc[j] *= f0;
+    if (f1 != 1.0f) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j] *= f1;
+    }
+}
+
+// The logits' epilogue: this lane's row, 128 columns from col0 on.  What most tiles do
+// not need (a ragged end, a bias, the target) is kept out of the loops of the others.
+__device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float (&acc)[128], float *stage, int64_t row,
+                                             int64_t col0, int part, float f0, float f1) {
+    if (col0 >= a.N) return;
+    const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
+    const bool live = row < M;
+    rescale(acc, f0, f1);
+    if (a.bias != nullptr) {
 #pragma unroll
         for (int j = 0; j < 128; ++j)
-            if (j < n) to[j * cs] = add ? to[j * cs] + acc[j] : acc[j];
+            if (j < n) acc[j] += __ldg(a.bias + (col0 + j) * a.bias_s);
     }
+    if (n < 128) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+            if (j >= n) acc[j] = -INFINITY;
+    }
+    const int target = live ? a.target[a.first + row] - static_cast<int>(col0) : -1;
+    if (target >= 0 && target < n) {
+        float zt = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+            if (j == target) zt = acc[j];
+        a.z_target[row] = zt;
+    }
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 128; ++j) top[j % 4] = fmaxf(top[j % 4], acc[j]);
+    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    // exp by the hardware's 2^x (2^-22): its error and the product's weigh little in a sum
+    // whose largest terms have arguments near zero
+    const float base = isinf(top[0]) ? 0.0f : top[0];
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 128; ++j) sum[j % 4] += __expf(acc[j] - base);
+    if (live) {
+        a.part_max[row * 2 * a.tiles_n + part] = top[0];
+        a.part_sum[row * 2 * a.tiles_n + part] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+    if (a.z == nullptr) return;
+    // rows are padded to 64 columns: the last four of a ragged end may lie behind V
+    store_rows(stage, acc, live ? a.z + row * a.z_pitch + col0 : nullptr, n, 1, true, false);
+}
+
+__device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&acc)[128], float *stage, int64_t row,
+                                          int64_t col0, int split, float f0, float f1) {
+    if (col0 >= a.N) return;
+    const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
+    rescale(acc, f0, f1);
+    float *to = nullptr;
+    int64_t cs = 1;
+    if (a.splits > 1) {
+        if (row < M) to = a.out + (split * a.M + row) * a.N + col0;
+    } else {
+        cs = a.out_cs;
+        if (row < M) to = a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0 * cs;
+    }
+    store_rows(stage, acc, to, n, cs, a.vec, a.add && a.splits == 1);
 }
 
 template <bool A_MN, bool B_MN, Out MODE>
@@ -404,8 +484,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     // the same aligned offset in both CTAs (same dynamic size, same static layout)
     unsigned char *smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes);  // leader's: both CTAs' bytes
-    uint64_t *empty = full + kStages;    // each CTA's: the stage's MMAs are done
+    float *stage_out = reinterpret_cast<float *>(smem + kStages * kStageBytes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes + 8 * kStageOut);  // leader's: both CTAs' bytes
+    uint64_t *empty = full + kStages;    // each CTA's: the stage's MMAs are done (hi stages first, then lo)
     uint64_t *acc_full = empty + kStages;  // [2] each CTA's: a piece is in tensor memory
     uint64_t *acc_empty = acc_full + 2;    // [2] leader's: both epilogues have read it
     uint64_t *drain = acc_empty + 2;
@@ -443,82 +524,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            int64_t it = 0;
-            bool ok = true;
-            for (int64_t u = cluster; u < e.units && ok; u += clusters) {
-                int tm, tn, split, kb0, kb1;
-                unit_of(args, e, u, tm, tn, split, kb0, kb1);
-                const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
-                const int b0 = tn * kTileCols + static_cast<int>(rank) * 128;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = static_cast<int>(it % kStages);
-                    if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / kStages) & 1u) ^ 1u, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    unsigned char *st = smem + s * kStageBytes;
-                    if (leader) mbar_expect_tx(&full[s], 2 * kStageBytes);
-                    const uint32_t fb = peer_addr(&full[s], 0);
-                    tma_load_operand(st, &map_a, fb, A_MN ? kb * kBlock : a0, A_MN ? a0 / kBlock : kb);
-                    tma_load_operand(st + kOperandBytes, &map_b, fb, B_MN ? kb * kBlock : b0, B_MN ? b0 / kBlock : kb);
-                }
-            }
-            if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
-            if (leader) {  // every stage issued by the pair has landed before the cluster exits
-                for (int64_t d = it > kStages ? it - kStages : 0; d < it; ++d) {
-                    const uint32_t round = static_cast<uint32_t>(d / kStages);
-                    for (long long i = 0; i < kWaitLimit && !mbar_try_wait(&full[d % kStages], round & 1u); ++i) {
-                    }
-                }
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && leader) {
-            constexpr uint32_t idesc = instr_desc<A_MN, B_MN>();
-            constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
-            constexpr uint64_t lo = (kOperandBytes / 2) >> 4;
-            int64_t it = 0;
-            bool ok = true;
-            for (int64_t u = cluster; u < e.units && ok; u += clusters) {
-                int tm, tn, split, kb0, kb1;
-                unit_of(args, e, u, tm, tn, split, kb0, kb1);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = static_cast<int>(it % kStages);
-                    const int b = static_cast<int>(it & 1);
-                    if (!mbar_wait(&acc_empty[b], (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, abort_flag) ||
-                        !mbar_wait(&full[s], static_cast<uint32_t>(it / kStages) & 1u, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t d = tmem_base + static_cast<uint32_t>(b * kTileCols);
-                    const uint32_t st = smem_u32(smem + s * kStageBytes);
-                    const uint64_t da = operand_desc<A_MN>(st), db = operand_desc<B_MN>(st + kOperandBytes);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        mma_pair(d, da + k * a_step, db + lo + k * b_step, idesc, k > 0);
-                        mma_pair(d, da + lo + k * a_step, db + k * b_step, idesc, 1);
-                    }
-                    mma_pair_scaled(d, da, db, idesc);
-#pragma unroll
-                    for (int k = 1; k < 4; ++k) mma_pair(d, da + k * a_step, db + k * b_step, idesc, 1);
-                    umma_commit_both(&empty[s]);
-                    umma_commit_both(&acc_full[b]);
-                }
-            }
-            if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
-            umma_commit_pair_local(drain);  // all MMAs of the pair are done before either CTA frees tensor memory
-            for (long long i = 0; i < kWaitLimit && !mbar_try_wait(drain, 0u); ++i) {
-            }
-        }
-    } else {
-        const int quadrant = warp % 4, half = (warp - 2) / 4;
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
+        const int quadrant = warp % 4, half = (warp - 4) / 4;
+        float *stage = stage_out + (warp - 4) * (kStageOut / 4);
         const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
         const int scale = -(scale_exponent(*args.amax_a) + scale_exponent(*args.amax_b));
-        const float f0 = power_of_two(scale / 2), f1 = power_of_two(scale - scale / 2);
-        int64_t it = 0;
+        const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
+        const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
+        int64_t piece = 0;
         bool ok = true;
         for (int64_t u = cluster; u < e.units && ok; u += clusters) {
             int tm, tn, split, kb0, kb1;
@@ -526,9 +540,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int b = static_cast<int>(it & 1);
-                if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(it >> 1) & 1u, abort_flag)) {
+            for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
+                const int b = static_cast<int>(piece & 1);
+                if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(piece >> 1) & 1u, abort_flag)) {
                     ok = false;
                     break;
                 }
@@ -536,11 +550,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
                 const uint32_t at = tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16) +
                                     static_cast<uint32_t>(b * kTileCols + half * 128);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    tmem_ld32(at + static_cast<uint32_t>(c * 32), v);
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[64];
+                    tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[c * 32 + j] += v[j];
+                    for (int j = 0; j < 64; ++j) acc[c * 64 + j] += __uint_as_float(v[j]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -549,11 +563,109 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
             if (!ok) break;
             const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
             const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
-            if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, f0, f1);
-            else store_sum(args, e.M, acc, row, col0, split, f0, f1);
+            if (MODE == Out::Logits) store_logits(args, e.M, acc, stage, row, col0, tn * 2 + half, f0, f1);
+            else store_sum(args, e.M, acc, stage, row, col0, split, f0, f1);
             __syncwarp();
         }
         if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 0) {
+            if (lane == 0) {
+                int64_t it = 0;
+                bool ok = true;
+                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                    int tm, tn, split, kb0, kb1;
+                    unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                    const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
+                    const int b0 = tn * kTileCols + static_cast<int>(rank) * 128;
+                    for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+                        for (int lo = 0; lo < 2; ++lo) {
+                            const int depth = lo ? kLoStages : kHiStages;
+                            const int s = (lo ? kHiStages : 0) + static_cast<int>(it % depth);
+                            if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / depth) & 1u) ^ 1u, abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            unsigned char *st = smem + s * kStageBytes;
+                            if (leader) mbar_expect_tx(&full[s], 2 * kStageBytes);
+                            const uint32_t fb = peer_addr(&full[s], 0);
+                            tma_load_operand(st, &map_a, fb, A_MN ? kb * kBlock : a0, A_MN ? a0 / kBlock : kb, lo);
+                            tma_load_operand(st + kOperandBytes, &map_b, fb, B_MN ? kb * kBlock : b0,
+                                             B_MN ? b0 / kBlock : kb, lo);
+                        }
+                    }
+                }
+                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+                if (leader) {  // every stage issued by the pair has landed before the cluster exits
+                    for (int lo = 0; lo < 2; ++lo) {
+                        const int depth = lo ? kLoStages : kHiStages;
+                        for (int64_t d = it > depth ? it - depth : 0; d < it; ++d) {
+                            uint64_t *bar = &full[(lo ? kHiStages : 0) + d % depth];
+                            const uint32_t round = static_cast<uint32_t>(d / depth);
+                            for (long long i = 0; i < kWaitLimit && !mbar_try_wait(bar, round & 1u); ++i) {
+                            }
+                        }
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0 && leader) {
+                constexpr uint32_t idesc = instr_desc<A_MN, B_MN>();
+                constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
+                int64_t it = 0, piece = 0;
+                bool ok = true;
+                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                    int tm, tn, split, kb0, kb1;
+                    unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                    for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
+                        const int n = kb1 - kb < kPieceBlocks ? kb1 - kb : kPieceBlocks;
+                        const int b = static_cast<int>(piece & 1);
+                        if (!mbar_wait(&acc_empty[b], (static_cast<uint32_t>(piece >> 1) & 1u) ^ 1u, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t d = tmem_base + static_cast<uint32_t>(b * kTileCols);
+                        for (int j = 0; j < n; ++j) {
+                            const int sh = static_cast<int>((it + j) % kHiStages);
+                            const int sl = kHiStages + static_cast<int>((it + j) % kLoStages);
+                            if (!mbar_wait(&full[sh], static_cast<uint32_t>((it + j) / kHiStages) & 1u, abort_flag) ||
+                                !mbar_wait(&full[sl], static_cast<uint32_t>((it + j) / kLoStages) & 1u, abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            const uint32_t hi = smem_u32(smem + sh * kStageBytes), lo = smem_u32(smem + sl * kStageBytes);
+                            const uint64_t ah = operand_desc<A_MN>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
+                            const uint64_t al = operand_desc<A_MN>(lo), bl = operand_desc<B_MN>(lo + kOperandBytes);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                mma_pair(d, ah + k * a_step, bl + k * b_step, idesc, j > 0 || k > 0);
+                                mma_pair(d, al + k * a_step, bh + k * b_step, idesc, 1);
+                            }
+                            umma_commit_both(&empty[sl]);
+                        }
+                        if (!ok) break;
+                        for (int j = 0; j < n; ++j) {
+                            const int sh = static_cast<int>((it + j) % kHiStages);
+                            const uint32_t hi = smem_u32(smem + sh * kStageBytes);
+                            const uint64_t ah = operand_desc<A_MN>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
+                            if (j == 0) mma_pair_scaled(d, ah, bh, idesc);
+                            else mma_pair(d, ah, bh, idesc, 1);
+#pragma unroll
+                            for (int k = 1; k < 4; ++k) mma_pair(d, ah + k * a_step, bh + k * b_step, idesc, 1);
+                            umma_commit_both(&empty[sh]);
+                        }
+                        umma_commit_both(&acc_full[b]);
+                        it += n;
+                    }
+                }
+                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+                umma_commit_pair_local(drain);  // all MMAs of the pair are done before either CTA frees tensor memory
+                for (long long i = 0; i < kWaitLimit && !mbar_try_wait(drain, 0u); ++i) {
+                }
+            }
+        }
     }
 
     tc_fence_before();
@@ -749,7 +861,7 @@ int operand_map(CUtensorMap &map, const __half *base, int64_t rows, int64_t bloc
     if (enc == nullptr) return fail(MTC_ERR_RUNTIME, "cuTensorMapEncodeTiled is unavailable");
     const cuuint64_t dims[4] = {kBlock, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(blocks), 2};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(pitch_blocks) * 256, 256, 128};
-    const cuuint32_t box[4] = {kBlock, mn ? 64u : 128u, mn ? 2u : 1u, 2};
+    const cuuint32_t box[4] = {kBlock, mn ? 64u : 128u, mn ? 2u : 1u, 1};
     const cuuint32_t elem[4] = {1, 1, 1, 1};
     const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half *>(base), dims, strides, box, elem,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
