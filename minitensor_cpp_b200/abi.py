@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from dataclasses import dataclass
+import struct
 from pathlib import Path
 from typing import Sequence
 
@@ -50,6 +50,23 @@ class Desc(ctypes.Structure):
         ("shape", ctypes.c_int64 * MAX_RANK),
         ("strides", ctypes.c_int64 * MAX_RANK),
     ]
+
+
+_DESC = struct.Struct("@Pqqii8q8q")
+_PAD = [(0,) * (MAX_RANK - rank) for rank in range(MAX_RANK + 1)]
+assert _DESC.size == ctypes.sizeof(Desc)
+
+
+_DTYPES: dict = {}
+
+
+def _dtype_code(dtype) -> int:
+    import torch
+
+    _DTYPES.update({torch.float32: FLOAT32, torch.int64: INT64})
+    if dtype not in _DTYPES:
+        raise ValueError(f"{dtype} operands are not supported: Float32 or Int64")
+    return _DTYPES[dtype]
 
 
 class Instr(ctypes.Structure):
@@ -89,32 +106,61 @@ def contiguous_strides(shape: Sequence[int]) -> list[int]:
     return strides
 
 
-@dataclass
 class View:
     """A strided view of a flat storage tensor (torch tensor, on any device)."""
 
-    storage: "object"  # torch.Tensor, 1-D
-    shape: tuple
-    strides: tuple
-    offset: int = 0
+    __slots__ = ("_storage", "_tensor", "shape", "strides", "offset")
+
+    def __init__(self, storage, shape: tuple, strides: tuple, offset: int = 0):
+        self._storage = storage  # torch.Tensor, 1-D
+        self._tensor = None
+        self.shape = shape
+        self.strides = strides
+        self.offset = offset
+
+    def __repr__(self) -> str:
+        return f"View(shape={self.shape}, strides={self.strides}, offset={self.offset}, storage={self.storage!r})"
 
     @staticmethod
     def of(t) -> "View":
         """View of an existing torch tensor (shares its storage)."""
-        import torch
-
-        flat = torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
-        return View(flat, tuple(t.shape), tuple(t.stride()), t.storage_offset())
+        v = View(None, t.shape, t.stride(), t.storage_offset())
+        v._tensor = t
+        return v
 
     @staticmethod
     def contiguous(storage, shape, offset: int = 0) -> "View":
         return View(storage, tuple(shape), tuple(contiguous_strides(shape)), offset)
 
-    def desc(self) -> Desc:
-        import torch
+    @property
+    def storage(self):
+        if self._storage is None:
+            import torch
 
-        dt = INT64 if self.storage.dtype == torch.int64 else FLOAT32
-        return make_desc(self.storage.data_ptr(), self.storage.numel(), dt, self.shape, self.strides, self.offset)
+            t = self._tensor
+            self._storage = torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
+        return self._storage
+
+    def desc(self) -> Desc:
+        return Desc.from_buffer_copy(self.packed())
+
+    def packed(self) -> bytes:
+        """The view's descriptor as the bytes of an mtc_desc."""
+        t = self._storage if self._tensor is None else self._tensor
+        dtype = _DTYPES.get(t.dtype)
+        if dtype is None:
+            dtype = _dtype_code(t.dtype)
+        rank = len(self.shape)
+        if rank != len(self.strides) or rank > MAX_RANK:
+            raise ValueError("shape/strides rank mismatch or rank > 8")
+        if self._tensor is None:
+            ptr, capacity = t.data_ptr(), t.numel()
+        else:
+            s = t.untyped_storage()
+            ptr, capacity = s.data_ptr(), s.nbytes() // (8 if dtype == INT64 else 4)
+        pad = _PAD[rank]
+        # one pack of the whole structure: a call of small tensors costs what its descriptors do
+        return _DESC.pack(ptr, self.offset, capacity, dtype, rank, *self.shape, *pad, *self.strides, *pad)
 
     def tensor(self):
         """The same view as a torch tensor (for zero/positive strides)."""
@@ -130,16 +176,17 @@ _lib = None
 
 def lib():
     global _lib
-    if _lib is None:
-        path = LIB_DIR / "libmtcuda.so"
-        try:  # load PyTorch first so its CUDA runtime / NCCL are the process-wide copies
-            import torch  # noqa: F401
-        except ImportError:
-            pass
-        if not path.exists():
-            raise MtcError(f"libmtcuda.so is not built ({path}); run __graft_entry__.build()")
-        _lib = ctypes.CDLL(str(path), mode=os.RTLD_GLOBAL if hasattr(os, "RTLD_GLOBAL") else 0)
-        _declare(_lib)
+    if _lib is not None:
+        return _lib
+    path = LIB_DIR / "libmtcuda.so"
+    try:  # load PyTorch first so its CUDA runtime / NCCL are the process-wide copies
+        import torch  # noqa: F401
+    except ImportError:
+        pass
+    if not path.exists():
+        raise MtcError(f"libmtcuda.so is not built ({path}); run __graft_entry__.build()")
+    _lib = ctypes.CDLL(str(path), mode=os.RTLD_GLOBAL if hasattr(os, "RTLD_GLOBAL") else 0)
+    _declare(_lib)
     return _lib
 
 
@@ -191,12 +238,13 @@ def _declare(L):
         "mtc_gather": ([P(Desc), P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_gather_scatter_add": ([P(Desc), P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_gather_scatter_add_into": ([P(Desc), P(Desc), c_i64, P(Desc), c_vp], c_int),
-        "mtc_embedding": ([P(Desc), P(Desc), c_f, c_i64, P(Desc), c_vp], c_int),
-        "mtc_embedding_grad": ([P(Desc), P(Desc), c_f, c_i64, c_i32, P(Desc), c_vp], c_int),
-        "mtc_linear_cross_entropy": ([P(Desc)] * 4 + [c_i64, P(Desc), P(Desc), c_vp], c_int),
-        "mtc_linear_cross_entropy_grad": ([P(Desc)] * 4 + [c_i64] + [P(Desc)] * 6 + [c_vp], c_int),
-        "mtc_global_norm": ([P(Desc), c_i32, P(Desc), c_vp], c_int),
-        "mtc_clip_global_norm": ([P(Desc), c_i32, c_f, P(Desc), P(Desc), c_vp], c_int),
+        # descriptors as untyped pointers: the packed bytes of a view, or byref(Desc)
+        "mtc_embedding": ([c_vp, c_vp, c_f, c_i64, c_vp, c_vp], c_int),
+        "mtc_embedding_grad": ([c_vp, c_vp, c_f, c_i64, c_i32, c_vp, c_vp], c_int),
+        "mtc_linear_cross_entropy": ([c_vp] * 4 + [c_i64, c_vp, c_vp, c_vp], c_int),
+        "mtc_linear_cross_entropy_grad": ([c_vp] * 4 + [c_i64] + [c_vp] * 7, c_int),
+        "mtc_global_norm": ([c_vp, c_i32, c_vp, c_vp], c_int),
+        "mtc_clip_global_norm": ([c_vp, c_i32, c_f, c_vp, c_vp, c_vp], c_int),
         "mtc_reduce": ([c_i32, P(Desc), P(c_i64), c_i32, P(Desc), c_vp], c_int),
         "mtc_log_softmax": ([P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_matmul": ([P(Desc), P(Desc), P(Desc), c_i32, c_vp], c_int),
@@ -251,7 +299,8 @@ def _stream(stream):
     if stream is None:
         import torch
 
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        # the handle alone: a Stream object costs more than a small call's launch
+        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
     return ctypes.c_void_p(int(stream))
 
 
@@ -318,7 +367,7 @@ def gather_scatter_add(upd: View, idx: View, axis: int, out: View, stream=None, 
 
 
 def _ref(v: View | None):
-    return None if v is None else ctypes.byref(v.desc())
+    return None if v is None else v.packed()
 
 
 def _token(t: int | None) -> int:
@@ -359,17 +408,17 @@ def linear_cross_entropy_grad(x: View, weight: View, targets: View, dloss: View,
 
 def global_norm(tensors: Sequence[View], norm: View, stream=None, prepare: bool = False):
     """norm = sqrt of the sum of squares of all elements of all tensors."""
-    arr = (Desc * max(len(tensors), 1))(*[v.desc() for v in tensors])
+    arr = b"".join([v.packed() for v in tensors])
     return _run("mtc_global_norm", (arr, len(tensors), _ref(norm), _stream(stream)), "global_norm", prepare)
 
 
 def clip_global_norm(tensors: Sequence[View], max_norm: float, norm: View | None = None,
                      outs: Sequence[View] | None = None, stream=None, prepare: bool = False):
     """Scales the tensors by max_norm / norm where their global norm exceeds max_norm; into `outs`, or in place."""
-    arr = (Desc * max(len(tensors), 1))(*[v.desc() for v in tensors])
+    arr = b"".join([v.packed() for v in tensors])
     if outs is not None and len(outs) != len(tensors):
         raise ValueError(f"{len(outs)} outputs for {len(tensors)} tensors")
-    to = arr if outs is None else (Desc * max(len(outs), 1))(*[v.desc() for v in outs])
+    to = arr if outs is None else b"".join([v.packed() for v in outs])
     return _run("mtc_clip_global_norm", (arr, len(tensors), max_norm, to, _ref(norm), _stream(stream)),
                 "clip_global_norm", prepare)
 
