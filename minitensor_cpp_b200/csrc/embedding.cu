@@ -15,8 +15,12 @@
 // token), and the sorted list is cut into pieces of 32 positions, whatever the
 // tokens: one CTA adds a piece's runs in registers, writes the rows whose run
 // lies inside the piece, and leaves the run that came in from the piece before
-// and the one that goes on into the next as partial rows.  A second kernel joins
-// those.  Which sums are formed depends on the tokens alone.
+// and the one that goes on into the next as partial rows.  The last piece of a run
+// to finish adds its partial rows, in the order of the pieces: which sums are formed
+// depends on the tokens alone.  Rows without a position are cleared by further CTAs
+// of the same launch, 32 rows a bit mask.
+#include <cooperative_groups.h>
+
 #include <climits>
 #include <cstring>
 
@@ -107,80 +111,87 @@ __global__ void __launch_bounds__(kThreads) k_embedding(const LookupArgs a) {
 }
 
 // ---------------------------------------------------------------- the sort --
-// Least-significant-digit radix sort of (token, position), stable.  A tile is
-// 4096 keys of one CTA; a key of a position without a gradient is V, the
-// largest.  Each pass: count the digits of every tile, then place every tile
-// after the sum of the counts before it.  Eight warps own 512 consecutive keys
-// of the tile each and rank them 32 at a time with match_any, so equal digits
-// keep their order.
+// Least-significant-digit radix sort of (token, position), stable.  A key of a
+// position without a gradient is V, the largest.  A warp owns consecutive keys
+// and ranks them 32 at a time with match_any, so equal digits keep their order;
+// a key goes behind the smaller digits, the equal ones of the warps and CTAs
+// before, and its rank.
+//
+// Up to 65536 positions are sorted by one cluster of up to 16 CTAs in one launch:
+// 4096 keys a CTA in shared memory, counts read and keys sent over distributed
+// shared memory.  That is bound by latency alone (a launch, the token loads, four
+// cluster barriers): 16384 positions 10 us, against 75 us for the first version's
+// four launches, whose loads waited for one another.  More positions take two
+// launches a pass (three with many tiles).
 
 constexpr int kTile = 4096;
-constexpr int kWarpKeys = 512;  // kTile / 8 warps
 constexpr int kMaxBins = 1024;
+constexpr int kClusterTiles = 16;  // CTAs of the largest cluster
+constexpr int kClusterBins = 512;
+constexpr int kClusterThreads = 1024;
 
 struct SortArgs {
     Positions pos;
     long long vocab, padding;
     unsigned int n;
-    int shift, bits;
+    int shift, bits, passes;
     int tiles;
+    int last;                     // this launch writes the sorted list
     const unsigned int *keys_in;  // null: read the tokens
     const unsigned int *at_in;
     unsigned int *keys_out, *at_out;
-    unsigned int *counts;  // [tiles][bins]
-    unsigned int *before;  // [tiles][bins] sums over the tiles before, and [bins] totals behind them; null: few tiles
+    unsigned int *counts;   // [tiles][bins]
+    unsigned int *before;   // [tiles][bins] sums over the tiles before, and [bins] totals behind them; null: few tiles
+    unsigned int *present;  // a bit for each table row that has a position; null: not wanted
+    unsigned int *arrived;  // counters of the sums, to be zeroed
+    unsigned int n_arrived;
     unsigned long long *err;
 };
 
-__device__ __forceinline__ unsigned int key_of(const SortArgs &a, unsigned int i, bool report) {
-    if (a.keys_in != nullptr) return a.keys_in[i];
-    long long row;
-    const long long t = token_at(a.pos, i, row);
-    if (t == a.padding) return static_cast<unsigned int>(a.vocab);
-    if (t < 0 || t >= a.vocab) {
-        if (report) report_index(a.err, t);
-        return static_cast<unsigned int>(a.vocab);
-    }
-    return static_cast<unsigned int>(t);
-}
-
-__global__ void __launch_bounds__(kThreads) k_digit_count(const SortArgs a) {
-    __shared__ unsigned int count[kMaxBins];
-    const int bins = 1 << a.bits;
-    for (int b = threadIdx.x; b < bins; b += kThreads) count[b] = 0;
-    __syncthreads();
-    const unsigned int first = blockIdx.x * kTile;
-#pragma unroll 4
-    for (int j = 0; j < kTile / kThreads; ++j) {
-        const unsigned int i = first + j * kThreads + threadIdx.x;
-        if (i < a.n) atomicAdd(&count[(key_of(a, i, true) >> a.shift) & (bins - 1)], 1u);
-    }
-    __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kThreads) a.counts[blockIdx.x * bins + b] = count[b];
-}
-
-// Sums over the tiles before each tile, one thread a digit.
-__global__ void __launch_bounds__(kThreads) k_digit_scan(const SortArgs a) {
-    const int bins = 1 << a.bits;
-    const int b = blockIdx.x * kThreads + threadIdx.x;
-    if (b >= bins) return;
-    unsigned int sum = 0;
-    int t = 0;
-    for (; t + 8 <= a.tiles; t += 8) {
-        unsigned int c[8];
+// Keys of N indices of a thread, the loads all in flight at once.
+template <int N, class Index>
+__device__ __forceinline__ void load_keys(const SortArgs &a, unsigned int (&key)[N], Index index, bool report) {
+    if (a.keys_in != nullptr) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) c[u] = a.counts[(t + u) * bins + b];
+        for (int j = 0; j < N; ++j) key[j] = index(j) < a.n ? a.keys_in[index(j)] : 0u;
+        return;
+    }
+    long long t[N];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            a.before[(t + u) * bins + b] = sum;
-            sum += c[u];
+    for (int j = 0; j < N; ++j) {
+        long long row;
+        t[j] = index(j) < a.n ? token_at(a.pos, index(j), row) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        key[j] = static_cast<unsigned int>(t[j]);
+        if (t[j] == a.padding) {
+            key[j] = static_cast<unsigned int>(a.vocab);
+        } else if (t[j] < 0 || t[j] >= a.vocab) {
+            if (report) report_index(a.err, t[j]);
+            key[j] = static_cast<unsigned int>(a.vocab);
         }
     }
-    for (; t < a.tiles; ++t) {
-        a.before[t * bins + b] = sum;
-        sum += a.counts[t * bins + b];
-    }
-    a.before[a.tiles * bins + b] = sum;
+}
+
+// What the sort's launches and the sums count in, zeroed by the first of them.
+__device__ __forceinline__ void clear_flags(const SortArgs &a, unsigned int thread, unsigned int threads) {
+    if (a.present != nullptr)
+        for (long long i = thread; i < (a.vocab + 31) / 32; i += threads) a.present[i] = 0;
+    for (unsigned int i = thread; i < a.n_arrived; i += threads) a.arrived[i] = 0;
+}
+
+// Sets the bits of N keys' rows; a frequent token's word is read before it is written
+// to, so that its thousands of positions do not queue at one address.
+template <int N, class Live>
+__device__ __forceinline__ void mark_present(const SortArgs &a, const unsigned int (&key)[N], Live live) {
+    if (a.present == nullptr) return;
+    unsigned int word[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) word[j] = live(j) && key[j] < a.vocab ? __ldcg(a.present + key[j] / 32) : 0xFFFFFFFFu;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (!(word[j] >> (key[j] % 32) & 1)) atomicOr(&a.present[key[j] / 32], 1u << (key[j] % 32));
 }
 
 // Exclusive sum over the CTA of one value a thread.
@@ -195,18 +206,170 @@ __device__ __forceinline__ unsigned int block_exclusive(unsigned int v, unsigned
     __syncthreads();
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    unsigned int before = 0;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    return before + x - v;
+    const unsigned int mine = lane < warp ? warp_sums[lane] : 0;
+    return __reduce_add_sync(0xFFFFFFFFu, mine) + x - v;
+}
+
+// Ranks of a warp's keys among the equal digits of its keys before: seen[d] counts them.
+template <int N, class Live>
+__device__ __forceinline__ void rank_keys(const unsigned int (&key)[N], unsigned short (&rank)[N], Live live, int shift,
+                                          unsigned int mask, unsigned short *seen) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const unsigned int d = (key[j] >> shift) & mask;
+        const unsigned int same = __match_any_sync(0xFFFFFFFFu, live(j) ? d : 0xFFFFFFFFu);
+        rank[j] = 0;
+        if (live(j)) rank[j] = seen[d] + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (live(j) && (same >> lane) == 1u) seen[d] = rank[j] + 1;  // the last of the equal lanes
+        __syncwarp();
+    }
+}
+
+struct ClusterSort {
+    unsigned int key[kTile], at[kTile];
+    unsigned short seen[kClusterThreads / 32][kClusterBins];
+    unsigned int count[kClusterBins], place[kClusterBins];
+    unsigned int warp_sums[32];
+};
+
+__global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    ClusterSort &s = *reinterpret_cast<ClusterSort *>(raw);
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const unsigned int me = cluster.block_rank(), ctas = cluster.num_blocks();
+    constexpr int N = kTile / kClusterThreads;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int bins = 1 << a.bits;
+    const unsigned int first = me * kTile + warp * (32 * N) + lane;
+    auto index = [&](int j) { return first + j * 32; };
+    auto live = [&](int j) { return index(j) < a.n; };
+    clear_flags(a, me * kClusterThreads + threadIdx.x, ctas * kClusterThreads);
+    unsigned int key[N], at[N];
+    load_keys<N>(a, key, index, true);
+#pragma unroll
+    for (int j = 0; j < N; ++j) at[j] = index(j);
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int shift = pass * a.bits;
+        if (pass > 0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int i = warp * (32 * N) + j * 32 + lane;
+                key[j] = s.key[i];
+                at[j] = s.at[i];
+            }
+        }
+        for (int i = threadIdx.x; i < static_cast<int>(sizeof(s.seen) / 4); i += kClusterThreads)
+            reinterpret_cast<unsigned int *>(s.seen)[i] = 0;
+        __syncthreads();
+        unsigned short rank[N];
+        rank_keys<N>(key, rank, live, shift, bins - 1, s.seen[warp]);
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < bins) {
+            unsigned short c[kClusterThreads / 32];
+#pragma unroll
+            for (int w = 0; w < kClusterThreads / 32; ++w) c[w] = s.seen[w][threadIdx.x];
+            unsigned int sum = 0;
+#pragma unroll
+            for (int w = 0; w < kClusterThreads / 32; ++w) {
+                s.seen[w][threadIdx.x] = static_cast<unsigned short>(sum);
+                sum += c[w];
+            }
+            s.count[threadIdx.x] = sum;
+        }
+        cluster.sync();  // every CTA's counts, and its reading of the keys it had
+        unsigned int total = 0, before = 0;
+        if (static_cast<int>(threadIdx.x) < bins) {
+            unsigned int c[kClusterTiles];
+#pragma unroll
+            for (unsigned int r = 0; r < kClusterTiles; ++r)
+                c[r] = r < ctas ? cluster.map_shared_rank(s.count, r)[threadIdx.x] : 0;
+#pragma unroll
+            for (unsigned int r = 0; r < kClusterTiles; ++r) {
+                if (r < me) before += c[r];
+                total += c[r];
+            }
+        }
+        const unsigned int base = block_exclusive(total, s.warp_sums);
+        if (static_cast<int>(threadIdx.x) < bins) s.place[threadIdx.x] = base + before;
+        __syncthreads();
+        const bool last = pass == a.passes - 1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (!live(j)) continue;
+            const unsigned int d = (key[j] >> shift) & (bins - 1);
+            const unsigned int to = s.place[d] + s.seen[warp][d] + rank[j];
+            if (last) {
+                a.keys_out[to] = key[j];
+                a.at_out[to] = at[j];
+            } else {
+                cluster.map_shared_rank(s.key, to / kTile)[to % kTile] = key[j];
+                cluster.map_shared_rank(s.at, to / kTile)[to % kTile] = at[j];
+            }
+        }
+        if (last) mark_present<N>(a, key, live);
+        cluster.sync();  // the keys have arrived, and nobody reads the counts any more
+    }
+}
+
+constexpr int kTileKeys = kTile / kThreads;
+
+__global__ void __launch_bounds__(kThreads) k_digit_count(const SortArgs a) {
+    __shared__ unsigned int count[kMaxBins];
+    const int bins = 1 << a.bits;
+    for (int b = threadIdx.x; b < bins; b += kThreads) count[b] = 0;
+    if (a.keys_in == nullptr) clear_flags(a, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads);
+    __syncthreads();
+    const unsigned int first = blockIdx.x * kTile + threadIdx.x;
+    unsigned int key[kTileKeys];
+    auto index = [&](int j) { return first + j * kThreads; };
+    load_keys<kTileKeys>(a, key, index, true);
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j)
+        if (index(j) < a.n) atomicAdd(&count[(key[j] >> a.shift) & (bins - 1)], 1u);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kThreads) a.counts[blockIdx.x * bins + b] = count[b];
+}
+
+// Sums over the tiles before each tile, one thread a digit.
+__global__ void __launch_bounds__(kThreads) k_digit_scan(const SortArgs a) {
+    const int bins = 1 << a.bits;
+    const int b = blockIdx.x * kThreads + threadIdx.x;
+    if (b >= bins) return;
+    unsigned int sum = 0;
+    int t = 0;
+    for (; t + 8 <= a.tiles; t += 8) {
+        unsigned int c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c[u] = a.counts[static_cast<long long>(t + u) * bins + b];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            a.before[static_cast<long long>(t + u) * bins + b] = sum;
+            sum += c[u];
+        }
+    }
+    for (; t < a.tiles; ++t) {
+        a.before[static_cast<long long>(t) * bins + b] = sum;
+        sum += a.counts[static_cast<long long>(t) * bins + b];
+    }
+    a.before[static_cast<long long>(a.tiles) * bins + b] = sum;
 }
 
 __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
-    __shared__ unsigned int place[kMaxBins];           // where the tile's keys of a digit begin
-    __shared__ unsigned short seen[8][kMaxBins];       // keys of a digit each warp has ranked so far
+    __shared__ unsigned int place[kMaxBins];      // where the tile's keys of a digit begin
+    __shared__ unsigned short seen[8][kMaxBins];  // keys of a digit each warp has ranked so far
     __shared__ unsigned int warp_sums[8];
     const int bins = 1 << a.bits;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int b = threadIdx.x; b < 8 * kMaxBins / 2; b += kThreads) reinterpret_cast<unsigned int *>(seen)[b] = 0;
+    const unsigned int first = blockIdx.x * kTile + warp * (kTile / 8) + lane;
+    auto index = [&](int j) { return first + j * 32; };
+    auto live = [&](int j) { return index(j) < a.n; };
+    unsigned int key[kTileKeys];
+    unsigned short rank[kTileKeys];
+    load_keys<kTileKeys>(a, key, index, false);
     const int per_thread = (bins + kThreads - 1) / kThreads;
     unsigned int total[kMaxBins / kThreads], before[kMaxBins / kThreads], sum = 0;
 #pragma unroll
@@ -215,9 +378,10 @@ __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
         const int b = threadIdx.x * per_thread + j;
         if (j >= per_thread || b >= bins) continue;
         if (a.before != nullptr) {
-            before[j] = a.before[blockIdx.x * bins + b];
-            total[j] = a.before[a.tiles * bins + b];
+            before[j] = a.before[static_cast<long long>(blockIdx.x) * bins + b];
+            total[j] = a.before[static_cast<long long>(a.tiles) * bins + b];
         } else {
+#pragma unroll 8
             for (int t = 0; t < a.tiles; ++t) {
                 const unsigned int c = a.counts[t * bins + b];
                 if (t < static_cast<int>(blockIdx.x)) before[j] += c;
@@ -234,26 +398,7 @@ __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
         at += total[j];
     }
     __syncthreads();
-    // ranks within the warp's 512 keys
-    const unsigned int first = blockIdx.x * kTile + warp * kWarpKeys;
-    unsigned int key[kWarpKeys / 32];
-    unsigned short rank[kWarpKeys / 32];
-#pragma unroll
-    for (int j = 0; j < kWarpKeys / 32; ++j) {
-        const unsigned int i = first + j * 32 + lane;
-        key[j] = i < a.n ? key_of(a, i, false) : 0u;
-    }
-#pragma unroll
-    for (int j = 0; j < kWarpKeys / 32; ++j) {
-        const bool live = first + j * 32 + lane < a.n;
-        const unsigned int d = (key[j] >> a.shift) & (bins - 1);
-        const unsigned int same = __match_any_sync(0xFFFFFFFFu, live ? d : 0xFFFFFFFFu);
-        rank[j] = 0;
-        if (live) rank[j] = seen[warp][d] + __popc(same & ((1u << lane) - 1));
-        __syncwarp();
-        if (live && (same >> lane) == 1u) seen[warp][d] = rank[j] + 1;  // the last of the equal lanes
-        __syncwarp();
-    }
+    rank_keys<kTileKeys>(key, rank, live, a.shift, bins - 1, seen[warp]);
     __syncthreads();
     // counts of the warps before: seen becomes each warp's first rank
     for (int b = threadIdx.x; b < bins; b += kThreads) {
@@ -267,24 +412,25 @@ __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kWarpKeys / 32; ++j) {
-        const unsigned int i = first + j * 32 + lane;
-        if (i >= a.n) continue;
+    for (int j = 0; j < kTileKeys; ++j) {
+        if (!live(j)) continue;
         const unsigned int d = (key[j] >> a.shift) & (bins - 1);
         const unsigned int to = place[d] + seen[warp][d] + rank[j];
         a.keys_out[to] = key[j];
-        a.at_out[to] = a.at_in != nullptr ? a.at_in[i] : i;
+        a.at_out[to] = a.at_in != nullptr ? a.at_in[index(j)] : index(j);
     }
+    if (a.last) mark_present<kTileKeys>(a, key, live);
 }
 
 // ---------------------------------------------------------------- the sums --
 
 constexpr int kRun = 32;      // sorted positions of a piece
-constexpr int kZeroRows = 8;  // table rows a CTA checks for having no position
+constexpr int kZeroRows = 32;  // table rows a CTA checks for having no position
 
 struct SumArgs {
     Positions pos;
     const unsigned int *keys, *at;
+    const unsigned int *present;
     unsigned int n;
     unsigned int pieces;
     unsigned int slabs;      // column slabs of kThreads * VEC
@@ -294,6 +440,7 @@ struct SumArgs {
     long long dout_cs, table_rs, table_cs;
     long long vocab, dim;
     float *partial;          // [pieces][2][dim]: the run that came in, the run that goes on
+    unsigned int *arrived;   // [pieces][slabs] partial rows written of the run that begins in the piece
     float scale;
     int accumulate;
 };
@@ -318,6 +465,22 @@ __device__ __forceinline__ Row<VEC> load_row(const float *p) {
     return r;
 }
 
+// A row that another CTA has written: past this SM's L1.
+template <int VEC>
+__device__ __forceinline__ Row<VEC> load_shared_row(const float *p) {
+    Row<VEC> r;
+    if (VEC == 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
+        r.v[3 % VEC] = x.w;
+        r.v[2 % VEC] = x.z;
+        r.v[1 % VEC] = x.y;
+        r.v[0] = x.x;
+    } else {
+        r.v[0] = __ldcg(p);
+    }
+    return r;
+}
+
 template <int VEC>
 __device__ __forceinline__ void store_row(float *p, const Row<VEC> &r) {
     if (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(r.v[0], r.v[1 % VEC], r.v[2 % VEC], r.v[3 % VEC]);
@@ -336,14 +499,66 @@ __device__ __forceinline__ void finish_row(const SumArgs &a, float *p, Row<VEC> 
     store_row<VEC>(p, r);
 }
 
-__device__ __forceinline__ unsigned int lower_bound(const unsigned int *keys, unsigned int n, unsigned int v) {
-    unsigned int lo = 0, hi = n;
-    while (lo < hi) {
-        const unsigned int mid = (lo + hi) / 2;
-        if (keys[mid] < v) lo = mid + 1;
-        else hi = mid;
+// Called by every piece that holds a part of a run of several pieces, once its partial
+// row is written: the last of them adds the partial rows, in the order of the pieces,
+// eight loads ahead.  `k`: the run's key; `on`: it goes on behind this piece.  One warp
+// finds the run's first piece, another its last, 32 pieces a step.
+template <int VEC>
+__device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsigned int unit, bool on, long long col,
+                                         bool in) {
+    __shared__ unsigned int range[2];
+    __shared__ bool last_here;
+    __threadfence();
+    __syncthreads();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (warp == 0) {  // the piece is the first if its first key, or the one before it, is another
+        for (unsigned int p0 = unit;; p0 -= 32) {
+            const bool valid = p0 >= static_cast<unsigned int>(lane);
+            const unsigned int p = valid ? p0 - lane : 0;
+            const bool begins = p == 0 || a.keys[p * kRun] != k || a.keys[p * kRun - 1] != k;
+            const unsigned int found = __ballot_sync(0xFFFFFFFFu, valid && begins);
+            if (found != 0) {
+                if (lane == 0) range[0] = p0 - (__ffs(found) - 1);
+                break;
+            }
+        }
+    } else if (warp == 1) {  // the last piece whose first key is still k
+        unsigned int end = unit;
+        for (unsigned int p0 = unit + 1; on; p0 += 32) {
+            const unsigned int p = p0 + lane;
+            const unsigned int found = __ballot_sync(0xFFFFFFFFu, p >= a.pieces || a.keys[p * kRun] != k);
+            end = found != 0 ? p0 + __ffs(found) - 2 : p0 + 31;
+            if (found != 0) break;
+        }
+        if (lane == 0) range[1] = end;
     }
-    return lo;
+    __syncthreads();
+    const unsigned int begin = range[0];
+    const unsigned int end = range[1];
+    const unsigned int slab = blockIdx.x % a.slabs;
+    if (threadIdx.x == 0) {
+        last_here = atomicAdd(&a.arrived[begin * a.slabs + slab], 1u) == end - begin;
+    }
+    __syncthreads();
+    if (!last_here) return;
+    __threadfence();
+    if (!in) return;
+    Row<VEC> sum;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
+    for (unsigned int p0 = begin; p0 <= end; p0 += 8) {
+        Row<VEC> x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (p0 + u <= end) x[u] = load_shared_row<VEC>(a.partial + (2ll * (p0 + u) + (p0 + u == begin)) * a.dim + col);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (p0 + u <= end) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
+            }
+    }
+    finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
 }
 
 template <int VEC>
@@ -352,25 +567,17 @@ __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
     const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * kThreads + threadIdx.x) * VEC;
     if (unit >= a.pieces) {
         // rows without a position
-        __shared__ unsigned char empty[kZeroRows];
-        const long long v0 = static_cast<long long>(unit - a.pieces) * kZeroRows;
-        if (threadIdx.x < kZeroRows) {
-            const long long v = v0 + threadIdx.x;
-            bool none = v < a.vocab;
-            if (none) {
-                const unsigned int at = lower_bound(a.keys, a.n, static_cast<unsigned int>(v));
-                none = at >= a.n || a.keys[at] != static_cast<unsigned int>(v);
-            }
-            empty[threadIdx.x] = none;
-        }
-        __syncthreads();
+        const unsigned int group = unit - a.pieces;
+        const long long v0 = static_cast<long long>(group) * kZeroRows;
+        const unsigned int has = a.n > 0 ? a.present[group] : 0;
         if (col >= a.dim) return;
         Row<VEC> zero;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) zero.v[j] = 0.0f;
-#pragma unroll
+        float *to = a.dtable + v0 * a.table_rs + col * a.table_cs;
+#pragma unroll 8
         for (int r = 0; r < kZeroRows; ++r)
-            if (empty[r]) store_row<VEC>(a.dtable + (v0 + r) * a.table_rs + col * a.table_cs, zero);
+            if (v0 + r < a.vocab && !(has >> r & 1)) store_row<VEC>(to + r * a.table_rs, zero);
         return;
     }
     __shared__ unsigned int key[kRun + 2];   // with the neighbours' last and first
@@ -387,77 +594,42 @@ __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
         row[threadIdx.x] = r;
     }
     __syncthreads();
-    if (col >= a.dim) return;
+    const bool in = col < a.dim;
     const float *src = a.dout + col * a.dout_cs;
     Row<VEC> sum;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
-    bool came_in = key[0] == key[1];
-    for (int i0 = 0; i0 < count; i0 += 8) {
+    // positions without a gradient are the last: their keys are V
+    const bool comes_in = key[0] == key[1] && key[1] < a.vocab;
+    const bool goes_on = key[count + 1] == key[count] && key[count] < a.vocab;
+    bool head = comes_in;
+    for (int i0 = 0; i0 < count && key[1 + i0] < a.vocab; i0 += 8) {
         Row<VEC> x[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (i0 + u < count && key[1 + i0 + u] < a.vocab) x[u] = load_row<VEC>(src + row[i0 + u]);
+            if (in && i0 + u < count && key[1 + i0 + u] < a.vocab) x[u] = load_row<VEC>(src + row[i0 + u]);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int i = i0 + u;
-            if (i >= count) break;
+            if (i >= count || key[1 + i] >= a.vocab) break;
             const unsigned int k = key[1 + i];
-            if (k >= a.vocab) return;  // positions without a gradient are the last
 #pragma unroll
             for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
-            const bool goes_on = key[2 + i] == k;
-            if (goes_on && i + 1 < count) continue;
-            if (came_in) {
-                store_row<VEC>(a.partial + (2ll * unit) * a.dim + col, sum);
-            } else if (goes_on) {
-                store_row<VEC>(a.partial + (2ll * unit + 1) * a.dim + col, sum);
-            } else {
-                finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
+            const bool on = key[2 + i] == k;
+            if (on && i + 1 < count) continue;
+            if (in) {
+                if (head) store_row<VEC>(a.partial + (2ll * unit) * a.dim + col, sum);
+                else if (on) store_row<VEC>(a.partial + (2ll * unit + 1) * a.dim + col, sum);
+                else finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
             }
-            came_in = false;
+            head = false;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
         }
     }
-}
-
-// Joins the runs that cross pieces: the piece in which a run begins adds the
-// partial rows of the pieces after it, eight loads ahead.
-template <int VEC>
-__global__ void __launch_bounds__(kThreads) k_token_join(const SumArgs a) {
-    const unsigned int unit = blockIdx.x / a.slabs;
-    const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * kThreads + threadIdx.x) * VEC;
-    const unsigned int last = (unit + 1) * kRun - 1;  // the piece's last position; there is a piece after it
-    const unsigned int k = a.keys[last];
-    if (k >= a.vocab || a.keys[last + 1] != k) return;
-    const unsigned int first = unit * kRun;
-    if (first > 0 && a.keys[first] == k && a.keys[first - 1] == k) return;  // began before
-    unsigned int end = unit + 1;  // the last piece that the run reaches
-    {
-        unsigned int lo = unit + 1, hi = a.pieces - 1;
-        while (lo < hi) {  // its first key is still k
-            const unsigned int mid = (lo + hi + 1) / 2;
-            if (a.keys[mid * kRun] == k) lo = mid;
-            else hi = mid - 1;
-        }
-        end = lo;
-    }
-    if (col >= a.dim) return;
-    Row<VEC> sum = load_row<VEC>(a.partial + (2ll * unit + 1) * a.dim + col);
-    for (unsigned int p0 = unit + 1; p0 <= end; p0 += 8) {
-        Row<VEC> x[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (p0 + u <= end) x[u] = load_row<VEC>(a.partial + (2ll * (p0 + u)) * a.dim + col);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (p0 + u <= end) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
-            }
-    }
-    finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
+    const bool one_run = key[1] == key[count];  // (of a piece that goes on as it came in, the whole is the head)
+    if (comes_in) join_run<VEC>(a, key[1], unit, one_run && goes_on, col, in);
+    if (goes_on && !(comes_in && one_run)) join_run<VEC>(a, key[count], unit, true, col, in);
 }
 
 // ------------------------------------------------------------------- host --
@@ -549,47 +721,81 @@ struct Sorted {
     const unsigned int *at;
 };
 
-constexpr int kFewTiles = 32;  // tiles whose counts every CTA adds itself (one launch less)
+constexpr int kFewTiles = 32;      // tiles whose counts every CTA adds itself (one launch less)
 
-int digit_bits(int64_t vocab, int &passes) {
+int digit_bits(int64_t vocab, int most, int &passes) {
     int bits = 1;
     while ((int64_t{1} << bits) <= vocab) ++bits;  // keys 0..vocab
-    passes = (bits + 9) / 10;
+    passes = (bits + most - 1) / most;
     return (bits + passes - 1) / passes;
 }
 
-int sort_positions(const Positions &pos, int64_t vocab, int64_t padding, unsigned int *buffers, unsigned int *counts,
-                   unsigned int *before, cudaStream_t stream, Sorted &sorted) {
+int sort_in_cluster(SortArgs a, cudaStream_t stream) {
+    a.bits = digit_bits(a.vocab, 9, a.passes);
+    unsigned int ctas = 1;
+    while (ctas < static_cast<unsigned int>(a.tiles)) ctas *= 2;
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ClusterSort)));
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t config;
+    std::memset(&config, 0, sizeof(config));
+    config.gridDim = dim3(ctas);
+    config.blockDim = dim3(kClusterThreads);
+    config.dynamicSmemBytes = sizeof(ClusterSort);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    std::memset(&attr, 0, sizeof(attr));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    MTC_CUDA_TRY(cudaLaunchKernelEx(&config, k_sort_cluster, a));
+    return check_launch("token sort");
+}
+
+int sort_positions(const SumArgs &sums, int64_t padding, unsigned int *buffers, unsigned int *counts,
+                   unsigned int *before, unsigned int *present, cudaStream_t stream, Sorted &sorted) {
+    const Positions &pos = sums.pos;
     SortArgs a;
     std::memset(&a, 0, sizeof(a));
     a.pos = pos;
-    a.vocab = vocab;
+    a.vocab = sums.vocab;
     a.padding = padding;
-    a.n = static_cast<unsigned int>(pos.n);
+    a.n = sums.n;
     a.tiles = static_cast<int>((pos.n + kTile - 1) / kTile);
-    a.counts = counts;
-    a.before = a.tiles > kFewTiles ? before : nullptr;
+    a.present = present;
+    a.arrived = sums.arrived;
+    a.n_arrived = sums.pieces * sums.slabs;
     MTC_TRY(device_error_word(&a.err));
-    int passes;
-    a.bits = digit_bits(vocab, passes);
     unsigned int *from = nullptr, *to = buffers;
-    for (int p = 0; p < passes; ++p) {
-        a.shift = p * a.bits;
-        a.keys_in = from;
-        a.at_in = from != nullptr ? from + pos.n : nullptr;
+    if (a.tiles <= kClusterTiles) {
         a.keys_out = to;
         a.at_out = to + pos.n;
-        k_digit_count<<<a.tiles, kThreads, 0, stream>>>(a);
-        MTC_TRY(check_launch("token sort (count)"));
-        if (a.before != nullptr) {
-            k_digit_scan<<<((1 << a.bits) + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
-            MTC_TRY(check_launch("token sort (scan)"));
-        }
-        k_digit_place<<<a.tiles, kThreads, 0, stream>>>(a);
-        MTC_TRY(check_launch("token sort (place)"));
-        unsigned int *next = from != nullptr ? from : buffers + 2 * pos.n;
+        MTC_TRY(sort_in_cluster(a, stream));
         from = to;
-        to = next;
+    } else {
+        a.counts = counts;
+        a.before = a.tiles > kFewTiles ? before : nullptr;
+        a.bits = digit_bits(a.vocab, 10, a.passes);
+        for (int p = 0; p < a.passes; ++p) {
+            a.shift = p * a.bits;
+            a.last = p == a.passes - 1;
+            a.keys_in = from;
+            a.at_in = from != nullptr ? from + pos.n : nullptr;
+            a.keys_out = to;
+            a.at_out = to + pos.n;
+            k_digit_count<<<a.tiles, kThreads, 0, stream>>>(a);
+            MTC_TRY(check_launch("token sort (count)"));
+            if (a.before != nullptr) {
+                k_digit_scan<<<((1 << a.bits) + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
+                MTC_TRY(check_launch("token sort (scan)"));
+            }
+            k_digit_place<<<a.tiles, kThreads, 0, stream>>>(a);
+            MTC_TRY(check_launch("token sort (place)"));
+            unsigned int *next = from != nullptr ? from : buffers + 2 * pos.n;
+            from = to;
+            to = next;
+        }
     }
     sorted.keys = from;
     sorted.at = from + pos.n;
@@ -633,27 +839,27 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
     const size_t counts = padded(tiles * kMaxBins * sizeof(unsigned int));
     const size_t before = padded((tiles + 1) * kMaxBins * sizeof(unsigned int));
     const size_t partial = padded(static_cast<size_t>(a.pieces) * 2 * a.dim * sizeof(float));
+    const size_t present = padded(static_cast<size_t>((a.vocab + 31) / 32) * sizeof(unsigned int));
     Workspace ws;
+    const size_t arrived = padded(static_cast<size_t>(a.pieces) * a.slabs * sizeof(unsigned int));
     if (a.n > 0) {
-        MTC_TRY(ws.allocate(list + counts + before + partial, stream));
+        MTC_TRY(ws.allocate(list + counts + before + partial + arrived + present, stream));
         unsigned int *buffers = ws.take<unsigned int>(list);
         unsigned int *c = ws.take<unsigned int>(counts);
         unsigned int *b = ws.take<unsigned int>(before);
         a.partial = ws.take<float>(partial);
+        a.arrived = ws.take<unsigned int>(arrived);
+        unsigned int *rows = accumulate ? nullptr : ws.take<unsigned int>(present);
+        a.present = rows;
         Sorted sorted;
-        MTC_TRY(sort_positions(a.pos, a.vocab, padding, buffers, c, b, stream, sorted));
+        MTC_TRY(sort_positions(a, padding, buffers, c, b, rows, stream, sorted));
         a.keys = sorted.keys;
         a.at = sorted.at;
     }
     const unsigned int grid = (a.pieces + a.zero_units) * a.slabs;
     if (vec) k_token_sums<4><<<grid, kThreads, 0, stream>>>(a);
     else k_token_sums<1><<<grid, kThreads, 0, stream>>>(a);
-    MTC_TRY(check_launch("embedding gradient (sums)"));
-    if (a.pieces < 2) return MTC_OK;
-    const unsigned int joins = (a.pieces - 1) * a.slabs;
-    if (vec) k_token_join<4><<<joins, kThreads, 0, stream>>>(a);
-    else k_token_join<1><<<joins, kThreads, 0, stream>>>(a);
-    return check_launch("embedding gradient (join)");
+    return check_launch("embedding gradient (sums)");
 }
 
 }  // namespace

@@ -61,7 +61,7 @@ def make_tokens(n, vocab, seed, hot=0.3):
 
 
 EMB_SHAPES = [(1, 5, 1), (1, 1, 7), (7, 3, 4), (33, 10, 64), (257, 100, 65), (1000, 999, 128), (4097, 50, 36),
-              (5000, 70001, 20), (9000, 2000, 1100)]
+              (5000, 70001, 20), (9000, 2000, 1100), (65536, 1000, 8), (70001, 3000, 16), (200003, 300000, 5)]
 
 
 @pytest.mark.parametrize("n, vocab, dim", EMB_SHAPES)
