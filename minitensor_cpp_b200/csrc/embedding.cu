@@ -113,16 +113,13 @@ __global__ void __launch_bounds__(kThreads) k_embedding(const LookupArgs a) {
 // ---------------------------------------------------------------- the sort --
 // Least-significant-digit radix sort of (token, position), stable.  A key of a
 // position without a gradient is V, the largest.  A warp owns consecutive keys
-// and ranks them 32 at a time with match_any, so equal digits keep their order;
+// and ranks them 32 at a time by ballots, so equal digits keep their order;
 // a key goes behind the smaller digits, the equal ones of the warps and CTAs
 // before, and its rank.
 //
-// Up to 65536 positions are sorted by one cluster of up to 16 CTAs in one launch:
-// 4096 keys a CTA in shared memory, counts read and keys sent over distributed
-// shared memory.  That is bound by latency alone (a launch, the token loads, four
-// cluster barriers): 16384 positions 10 us, against 75 us for the first version's
-// four launches, whose loads waited for one another.  More positions take two
-// launches a pass (three with many tiles).
+// Up to 65536 positions are sorted by one cluster of up to 16 CTAs in one launch, the
+// keys in shared memory, counts read and keys sent over distributed shared memory.
+// More positions take two launches a pass (three with many tiles).
 
 constexpr int kTile = 4096;
 constexpr int kMaxBins = 1024;
@@ -137,9 +134,8 @@ struct SortArgs {
     int shift, bits, passes;
     int tiles;
     int last;                     // this launch writes the sorted list
-    const unsigned int *keys_in;  // null: read the tokens
-    const unsigned int *at_in;
-    unsigned int *keys_out, *at_out;
+    const uint2 *in;        // (token, position); null: read the tokens
+    uint2 *out;
     unsigned int *counts;   // [tiles][bins]
     unsigned int *before;   // [tiles][bins] sums over the tiles before, and [bins] totals behind them; null: few tiles
     unsigned int *present;  // a bit for each table row that has a position; null: not wanted
@@ -150,12 +146,19 @@ struct SortArgs {
 
 // Keys of N indices of a thread, the loads all in flight at once.
 template <int N, class Index>
-__device__ __forceinline__ void load_keys(const SortArgs &a, unsigned int (&key)[N], Index index, bool report) {
-    if (a.keys_in != nullptr) {
+__device__ __forceinline__ void load_keys(const SortArgs &a, unsigned int (&key)[N], unsigned int (&at)[N], Index index,
+                                          bool report) {
+    if (a.in != nullptr) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) key[j] = index(j) < a.n ? a.keys_in[index(j)] : 0u;
+        for (int j = 0; j < N; ++j) {
+            const uint2 x = index(j) < a.n ? a.in[index(j)] : make_uint2(0, 0);
+            key[j] = x.x;
+            at[j] = x.y;
+        }
         return;
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j) at[j] = index(j);
     long long t[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -211,61 +214,73 @@ __device__ __forceinline__ unsigned int block_exclusive(unsigned int v, unsigned
 }
 
 // Ranks of a warp's keys among the equal digits of its keys before: seen[d] counts them.
+// The lanes with an equal digit come from one ballot a bit.
 template <int N, class Live>
 __device__ __forceinline__ void rank_keys(const unsigned int (&key)[N], unsigned short (&rank)[N], Live live, int shift,
-                                          unsigned int mask, unsigned short *seen) {
+                                          int bits, unsigned short *seen) {
     const int lane = threadIdx.x % 32;
+    unsigned int same[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) same[j] = __ballot_sync(0xFFFFFFFFu, live(j));
+    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const bool one = (key[j] >> (shift + b)) & 1;
+            const unsigned int ones = __ballot_sync(0xFFFFFFFFu, one);
+            same[j] &= one ? ones : ~ones;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const unsigned int d = (key[j] >> shift) & mask;
-        const unsigned int same = __match_any_sync(0xFFFFFFFFu, live(j) ? d : 0xFFFFFFFFu);
+        const unsigned int d = (key[j] >> shift) & ((1u << bits) - 1);
         rank[j] = 0;
-        if (live(j)) rank[j] = seen[d] + __popc(same & ((1u << lane) - 1));
+        if (live(j)) rank[j] = seen[d] + __popc(same[j] & ((1u << lane) - 1));
         __syncwarp();
-        if (live(j) && (same >> lane) == 1u) seen[d] = rank[j] + 1;  // the last of the equal lanes
+        if (live(j) && (same[j] >> lane) == 1u) seen[d] = rank[j] + 1;  // the last of the equal lanes
         __syncwarp();
     }
 }
 
 struct ClusterSort {
-    unsigned int key[kTile], at[kTile];
+    uint2 key[kTile];  // (token, position)
     unsigned short seen[kClusterThreads / 32][kClusterBins];
     unsigned int count[kClusterBins], place[kClusterBins];
     unsigned int warp_sums[32];
 };
 
+// N keys a thread, 1024 N a CTA: a scatter costs a clock a key of its SM's, so the keys
+// are spread over as many CTAs as a cluster has.
+template <int N>
 __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
     ClusterSort &s = *reinterpret_cast<ClusterSort *>(raw);
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned int me = cluster.block_rank(), ctas = cluster.num_blocks();
-    constexpr int N = kTile / kClusterThreads;
+    constexpr int kKeys = kClusterThreads * N;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int bins = 1 << a.bits;
-    const unsigned int first = me * kTile + warp * (32 * N) + lane;
+    const unsigned int first = me * kKeys + warp * (32 * N) + lane;
     auto index = [&](int j) { return first + j * 32; };
     auto live = [&](int j) { return index(j) < a.n; };
     clear_flags(a, me * kClusterThreads + threadIdx.x, ctas * kClusterThreads);
     unsigned int key[N], at[N];
-    load_keys<N>(a, key, index, true);
-#pragma unroll
-    for (int j = 0; j < N; ++j) at[j] = index(j);
+    load_keys<N>(a, key, at, index, true);
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.bits;
         if (pass > 0) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const int i = warp * (32 * N) + j * 32 + lane;
-                key[j] = s.key[i];
-                at[j] = s.at[i];
+                const uint2 x = s.key[warp * (32 * N) + j * 32 + lane];
+                key[j] = x.x;
+                at[j] = x.y;
             }
         }
         for (int i = threadIdx.x; i < static_cast<int>(sizeof(s.seen) / 4); i += kClusterThreads)
             reinterpret_cast<unsigned int *>(s.seen)[i] = 0;
         __syncthreads();
         unsigned short rank[N];
-        rank_keys<N>(key, rank, live, shift, bins - 1, s.seen[warp]);
+        rank_keys<N>(key, rank, live, shift, a.bits, s.seen[warp]);
         __syncthreads();
         if (static_cast<int>(threadIdx.x) < bins) {
             unsigned short c[kClusterThreads / 32];
@@ -301,13 +316,8 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const SortA
             if (!live(j)) continue;
             const unsigned int d = (key[j] >> shift) & (bins - 1);
             const unsigned int to = s.place[d] + s.seen[warp][d] + rank[j];
-            if (last) {
-                a.keys_out[to] = key[j];
-                a.at_out[to] = at[j];
-            } else {
-                cluster.map_shared_rank(s.key, to / kTile)[to % kTile] = key[j];
-                cluster.map_shared_rank(s.at, to / kTile)[to % kTile] = at[j];
-            }
+            if (last) a.out[to] = make_uint2(key[j], at[j]);
+            else cluster.map_shared_rank(s.key, to / kKeys)[to % kKeys] = make_uint2(key[j], at[j]);
         }
         if (last) mark_present<N>(a, key, live);
         cluster.sync();  // the keys have arrived, and nobody reads the counts any more
@@ -320,12 +330,12 @@ __global__ void __launch_bounds__(kThreads) k_digit_count(const SortArgs a) {
     __shared__ unsigned int count[kMaxBins];
     const int bins = 1 << a.bits;
     for (int b = threadIdx.x; b < bins; b += kThreads) count[b] = 0;
-    if (a.keys_in == nullptr) clear_flags(a, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads);
+    if (a.in == nullptr) clear_flags(a, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads);
     __syncthreads();
     const unsigned int first = blockIdx.x * kTile + threadIdx.x;
-    unsigned int key[kTileKeys];
+    unsigned int key[kTileKeys], at[kTileKeys];
     auto index = [&](int j) { return first + j * kThreads; };
-    load_keys<kTileKeys>(a, key, index, true);
+    load_keys<kTileKeys>(a, key, at, index, true);
 #pragma unroll
     for (int j = 0; j < kTileKeys; ++j)
         if (index(j) < a.n) atomicAdd(&count[(key[j] >> a.shift) & (bins - 1)], 1u);
@@ -367,9 +377,9 @@ __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
     const unsigned int first = blockIdx.x * kTile + warp * (kTile / 8) + lane;
     auto index = [&](int j) { return first + j * 32; };
     auto live = [&](int j) { return index(j) < a.n; };
-    unsigned int key[kTileKeys];
+    unsigned int key[kTileKeys], at[kTileKeys];
     unsigned short rank[kTileKeys];
-    load_keys<kTileKeys>(a, key, index, false);
+    load_keys<kTileKeys>(a, key, at, index, false);
     const int per_thread = (bins + kThreads - 1) / kThreads;
     unsigned int total[kMaxBins / kThreads], before[kMaxBins / kThreads], sum = 0;
 #pragma unroll
@@ -390,15 +400,15 @@ __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
         }
         sum += total[j];
     }
-    unsigned int at = block_exclusive(sum, warp_sums);
+    unsigned int begin = block_exclusive(sum, warp_sums);
 #pragma unroll
     for (int j = 0; j < kMaxBins / kThreads; ++j) {
         const int b = threadIdx.x * per_thread + j;
-        if (j < per_thread && b < bins) place[b] = at + before[j];
-        at += total[j];
+        if (j < per_thread && b < bins) place[b] = begin + before[j];
+        begin += total[j];
     }
     __syncthreads();
-    rank_keys<kTileKeys>(key, rank, live, a.shift, bins - 1, seen[warp]);
+    rank_keys<kTileKeys>(key, rank, live, a.shift, a.bits, seen[warp]);
     __syncthreads();
     // counts of the warps before: seen becomes each warp's first rank
     for (int b = threadIdx.x; b < bins; b += kThreads) {
@@ -415,9 +425,7 @@ __global__ void __launch_bounds__(kThreads) k_digit_place(const SortArgs a) {
     for (int j = 0; j < kTileKeys; ++j) {
         if (!live(j)) continue;
         const unsigned int d = (key[j] >> a.shift) & (bins - 1);
-        const unsigned int to = place[d] + seen[warp][d] + rank[j];
-        a.keys_out[to] = key[j];
-        a.at_out[to] = a.at_in != nullptr ? a.at_in[index(j)] : index(j);
+        a.out[place[d] + seen[warp][d] + rank[j]] = make_uint2(key[j], at[j]);
     }
     if (a.last) mark_present<kTileKeys>(a, key, live);
 }
@@ -429,7 +437,7 @@ constexpr int kZeroRows = 32;  // table rows a CTA checks for having no position
 
 struct SumArgs {
     Positions pos;
-    const unsigned int *keys, *at;
+    const uint2 *list;       // (token, position), sorted
     const unsigned int *present;
     unsigned int n;
     unsigned int pieces;
@@ -515,7 +523,7 @@ __device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsig
         for (unsigned int p0 = unit;; p0 -= 32) {
             const bool valid = p0 >= static_cast<unsigned int>(lane);
             const unsigned int p = valid ? p0 - lane : 0;
-            const bool begins = p == 0 || a.keys[p * kRun] != k || a.keys[p * kRun - 1] != k;
+            const bool begins = p == 0 || a.list[p * kRun].x != k || a.list[p * kRun - 1].x != k;
             const unsigned int found = __ballot_sync(0xFFFFFFFFu, valid && begins);
             if (found != 0) {
                 if (lane == 0) range[0] = p0 - (__ffs(found) - 1);
@@ -526,7 +534,7 @@ __device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsig
         unsigned int end = unit;
         for (unsigned int p0 = unit + 1; on; p0 += 32) {
             const unsigned int p = p0 + lane;
-            const unsigned int found = __ballot_sync(0xFFFFFFFFu, p >= a.pieces || a.keys[p * kRun] != k);
+            const unsigned int found = __ballot_sync(0xFFFFFFFFu, p >= a.pieces || a.list[p * kRun].x != k);
             end = found != 0 ? p0 + __ffs(found) - 2 : p0 + 31;
             if (found != 0) break;
         }
@@ -586,11 +594,11 @@ __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
     const int count = static_cast<int>(a.n - first < kRun ? a.n - first : kRun);
     if (threadIdx.x < kRun + 2) {
         const long long i = static_cast<long long>(first) + threadIdx.x - 1;
-        key[threadIdx.x] = i >= 0 && i < a.n ? a.keys[i] : 0xFFFFFFFFu;
+        key[threadIdx.x] = i >= 0 && i < a.n ? a.list[i].x : 0xFFFFFFFFu;
     }
     if (threadIdx.x < count) {
         long long r;
-        (void)token_at(a.pos, a.at[first + threadIdx.x], r);
+        (void)token_at(a.pos, a.list[first + threadIdx.x].y, r);
         row[threadIdx.x] = r;
     }
     __syncthreads();
@@ -715,12 +723,6 @@ int run_embedding(const mtc_desc *table, const mtc_desc *tokens, float scale, in
     return MTC_OK;
 }
 
-// The positions in token order: keys and positions in two buffers of n each.
-struct Sorted {
-    const unsigned int *keys;
-    const unsigned int *at;
-};
-
 constexpr int kFewTiles = 32;      // tiles whose counts every CTA adds itself (one launch less)
 
 int digit_bits(int64_t vocab, int most, int &passes) {
@@ -730,12 +732,14 @@ int digit_bits(int64_t vocab, int most, int &passes) {
     return (bits + passes - 1) / passes;
 }
 
+template <int N>
 int sort_in_cluster(SortArgs a, cudaStream_t stream) {
     a.bits = digit_bits(a.vocab, 9, a.passes);
+    const unsigned int keys = kClusterThreads * N;
     unsigned int ctas = 1;
-    while (ctas < static_cast<unsigned int>(a.tiles)) ctas *= 2;
-    MTC_CUDA_TRY(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ClusterSort)));
-    MTC_CUDA_TRY(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    while (ctas * keys < a.n) ctas *= 2;
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_sort_cluster<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ClusterSort)));
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_sort_cluster<N>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t config;
     std::memset(&config, 0, sizeof(config));
     config.gridDim = dim3(ctas);
@@ -749,56 +753,47 @@ int sort_in_cluster(SortArgs a, cudaStream_t stream) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    MTC_CUDA_TRY(cudaLaunchKernelEx(&config, k_sort_cluster, a));
+    MTC_CUDA_TRY(cudaLaunchKernelEx(&config, k_sort_cluster<N>, a));
     return check_launch("token sort");
 }
 
-int sort_positions(const SumArgs &sums, int64_t padding, unsigned int *buffers, unsigned int *counts,
-                   unsigned int *before, unsigned int *present, cudaStream_t stream, Sorted &sorted) {
-    const Positions &pos = sums.pos;
+// Sorts the positions by token; `sums.list` becomes one of the two `buffers` of n.
+int sort_positions(SumArgs &sums, int64_t padding, uint2 *buffers, unsigned int *counts, unsigned int *before,
+                   unsigned int *present, cudaStream_t stream) {
     SortArgs a;
     std::memset(&a, 0, sizeof(a));
-    a.pos = pos;
+    a.pos = sums.pos;
     a.vocab = sums.vocab;
     a.padding = padding;
     a.n = sums.n;
-    a.tiles = static_cast<int>((pos.n + kTile - 1) / kTile);
+    a.tiles = static_cast<int>((sums.pos.n + kTile - 1) / kTile);
     a.present = present;
     a.arrived = sums.arrived;
     a.n_arrived = sums.pieces * sums.slabs;
     MTC_TRY(device_error_word(&a.err));
-    unsigned int *from = nullptr, *to = buffers;
-    if (a.tiles <= kClusterTiles) {
-        a.keys_out = to;
-        a.at_out = to + pos.n;
-        MTC_TRY(sort_in_cluster(a, stream));
-        from = to;
-    } else {
-        a.counts = counts;
-        a.before = a.tiles > kFewTiles ? before : nullptr;
-        a.bits = digit_bits(a.vocab, 10, a.passes);
-        for (int p = 0; p < a.passes; ++p) {
-            a.shift = p * a.bits;
-            a.last = p == a.passes - 1;
-            a.keys_in = from;
-            a.at_in = from != nullptr ? from + pos.n : nullptr;
-            a.keys_out = to;
-            a.at_out = to + pos.n;
-            k_digit_count<<<a.tiles, kThreads, 0, stream>>>(a);
-            MTC_TRY(check_launch("token sort (count)"));
-            if (a.before != nullptr) {
-                k_digit_scan<<<((1 << a.bits) + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
-                MTC_TRY(check_launch("token sort (scan)"));
-            }
-            k_digit_place<<<a.tiles, kThreads, 0, stream>>>(a);
-            MTC_TRY(check_launch("token sort (place)"));
-            unsigned int *next = from != nullptr ? from : buffers + 2 * pos.n;
-            from = to;
-            to = next;
+    a.out = buffers;
+    sums.list = a.out;
+    if (a.n <= kClusterThreads * kClusterTiles) return sort_in_cluster<1>(a, stream);
+    if (a.n <= kClusterThreads * kClusterTiles * 2) return sort_in_cluster<2>(a, stream);
+    if (a.n <= kClusterThreads * kClusterTiles * 4) return sort_in_cluster<4>(a, stream);
+    a.counts = counts;
+    a.before = a.tiles > kFewTiles ? before : nullptr;
+    a.bits = digit_bits(a.vocab, 10, a.passes);
+    for (int p = 0; p < a.passes; ++p) {
+        a.shift = p * a.bits;
+        a.last = p == a.passes - 1;
+        a.out = buffers + (p % 2) * static_cast<int64_t>(a.n);
+        k_digit_count<<<a.tiles, kThreads, 0, stream>>>(a);
+        MTC_TRY(check_launch("token sort (count)"));
+        if (a.before != nullptr) {
+            k_digit_scan<<<((1 << a.bits) + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
+            MTC_TRY(check_launch("token sort (scan)"));
         }
+        k_digit_place<<<a.tiles, kThreads, 0, stream>>>(a);
+        MTC_TRY(check_launch("token sort (place)"));
+        a.in = a.out;
     }
-    sorted.keys = from;
-    sorted.at = from + pos.n;
+    sums.list = a.in;
     return MTC_OK;
 }
 
@@ -834,7 +829,7 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
         return fail(MTC_ERR_UNSUPPORTED, "the embedding gradient is too large for one launch");
     a.zero_units = static_cast<unsigned int>(zero_units);
     if (a.pieces + a.zero_units == 0) return MTC_OK;
-    const size_t list = padded(4 * static_cast<size_t>(a.n) * sizeof(unsigned int));
+    const size_t list = padded(2 * static_cast<size_t>(a.n) * sizeof(uint2));
     const size_t tiles = (static_cast<size_t>(a.n) + kTile - 1) / kTile;
     const size_t counts = padded(tiles * kMaxBins * sizeof(unsigned int));
     const size_t before = padded((tiles + 1) * kMaxBins * sizeof(unsigned int));
@@ -844,17 +839,14 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
     const size_t arrived = padded(static_cast<size_t>(a.pieces) * a.slabs * sizeof(unsigned int));
     if (a.n > 0) {
         MTC_TRY(ws.allocate(list + counts + before + partial + arrived + present, stream));
-        unsigned int *buffers = ws.take<unsigned int>(list);
+        uint2 *buffers = ws.take<uint2>(list);
         unsigned int *c = ws.take<unsigned int>(counts);
         unsigned int *b = ws.take<unsigned int>(before);
         a.partial = ws.take<float>(partial);
         a.arrived = ws.take<unsigned int>(arrived);
         unsigned int *rows = accumulate ? nullptr : ws.take<unsigned int>(present);
         a.present = rows;
-        Sorted sorted;
-        MTC_TRY(sort_positions(a, padding, buffers, c, b, rows, stream, sorted));
-        a.keys = sorted.keys;
-        a.at = sorted.at;
+        MTC_TRY(sort_positions(a, padding, buffers, c, b, rows, stream));
     }
     const unsigned int grid = (a.pieces + a.zero_units) * a.slabs;
     if (vec) k_token_sums<4><<<grid, kThreads, 0, stream>>>(a);
