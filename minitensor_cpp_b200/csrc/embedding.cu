@@ -3,9 +3,7 @@
 //   out[i, :] = scale * table[tok_i, :]            dtable[v, :] = scale * sum_{i: tok_i = v} dout[i, :]
 //
 // The lookup reads each row once and writes 4 D bytes a position: bound by HBM
-// for many positions, by the launch for few.  Threads walk the flat space of
-// (position, four columns), four loads in flight each, so rows of any width
-// keep the CTA full and neighbouring threads stay on neighbouring addresses.
+// for many positions, by the launch for few.
 //
 // The gradient reads every dout row once and writes every table row once.
 // Atomics would add the rows of a frequent token one after the other at one
@@ -58,9 +56,10 @@ __device__ __forceinline__ long long token_at(const Positions &p, long long i, l
 
 struct LookupArgs {
     Positions pos;
-    long long first;      // position of the launch's first row
-    unsigned int total;   // vectors of the launch
-    FastDiv per_row;      // vectors a row
+    int lanes_log2;      // lanes that share a segment of a row
+    unsigned int segments;  // of a row, each kLookupLoads vectors a lane
+    long long groups;    // positions x segments
+    long long vectors;   // of a row
     const float *table;
     float *out;
     long long table_rs, table_cs, out_cs;
@@ -70,43 +69,54 @@ struct LookupArgs {
     unsigned long long *err;
 };
 
+constexpr int kLookupLoads = 4;
+
+// 2^lanes_log2 lanes take a segment of a row, one token for all of their four loads, and
+// fetch the token of their next segment before they wait for the row of this one.
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) k_embedding(const LookupArgs a) {
-    constexpr int U = 4;
-    const unsigned int base = blockIdx.x * (kThreads * U) + threadIdx.x;
-    float4 v[U];
-    float *dst[U];
+    constexpr int U = kLookupLoads;
+    const int lanes = 1 << a.lanes_log2;
+    const unsigned int thread = blockIdx.x * kThreads + threadIdx.x;
+    const int lane = static_cast<int>(thread) & (lanes - 1);
+    const long long stride = static_cast<long long>(gridDim.x) * kThreads >> a.lanes_log2;
+    long long g = thread >> a.lanes_log2;
+    if (g >= a.groups) return;
+    long long i = a.segments == 1 ? g : g / a.segments;
+    long long row;
+    long long t = token_at(a.pos, i, row);
+    while (true) {
+        const long long c0 = (g - i * a.segments) * (lanes * U) + lane;
+        float *dst = a.out + row + c0 * VEC * a.out_cs;
+        const bool zero = t == a.padding, valid = t >= 0 && t < a.vocab;
+        if (!zero && !valid && c0 == 0) report_index(a.err, t);
+        const float *src = a.table + (valid ? t : 0) * a.table_rs + c0 * VEC * a.table_cs;
+        float4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned int q = base + u * kThreads;
-        dst[u] = nullptr;
-        v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (q >= a.total) continue;
-        const unsigned int r = fastdiv(q, a.per_row);
-        const long long c = q - r * a.per_row.d;
-        long long row;
-        const long long t = token_at(a.pos, a.first + r, row);
-        if (t == a.padding) {
-            dst[u] = a.out + row + c * VEC * a.out_cs;
-            continue;
+        for (int u = 0; u < U; ++u) {
+            v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (!valid || zero || c0 + u * lanes >= a.vectors) continue;
+            if (VEC == 4) v[u] = __ldg(reinterpret_cast<const float4 *>(src) + u * lanes);
+            else v[u].x = __ldg(src + u * lanes * a.table_cs);
         }
-        if (t < 0 || t >= a.vocab) {
-            if (c == 0) report_index(a.err, t);
-            continue;
+        const long long next = g + stride;
+        if (next < a.groups) {
+            i = a.segments == 1 ? next : next / a.segments;
+            t = token_at(a.pos, i, row);
         }
-        dst[u] = a.out + row + c * VEC * a.out_cs;
-        const float *src = a.table + t * a.table_rs + c * VEC * a.table_cs;
-        if (VEC == 4) v[u] = __ldg(reinterpret_cast<const float4 *>(src));
-        else v[u].x = __ldg(src);
-    }
+        if (valid || zero) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (dst[u] == nullptr) continue;
-        if (VEC == 4)
-            *reinterpret_cast<float4 *>(dst[u]) =
-                make_float4(v[u].x * a.scale, v[u].y * a.scale, v[u].z * a.scale, v[u].w * a.scale);
-        else
-            *dst[u] = v[u].x * a.scale;
+            for (int u = 0; u < U; ++u) {
+                if (c0 + u * lanes >= a.vectors) continue;
+                if (VEC == 4)
+                    __stcs(reinterpret_cast<float4 *>(dst) + u * lanes,
+                           make_float4(v[u].x * a.scale, v[u].y * a.scale, v[u].z * a.scale, v[u].w * a.scale));
+                else
+                    dst[u * lanes * a.out_cs] = v[u].x * a.scale;
+            }
+        }
+        if (next >= a.groups) return;
+        g = next;
     }
 }
 
@@ -708,19 +718,18 @@ int run_embedding(const mtc_desc *table, const mtc_desc *tokens, float scale, in
     const long long table_rs = a.table_rs;
     const bool vec = vector_rows(a.table, dim, a.table_cs, &table_rs, 1) &&
                      vector_rows(a.out, dim, a.out_cs, a.pos.row_stride, a.pos.rank);
-    const int64_t per_row = vec ? dim / 4 : dim;
-    if (per_row >= (int64_t{1} << 31)) return fail(MTC_ERR_UNSUPPORTED, "embedding rows are too wide");
-    a.per_row = make_fastdiv(static_cast<uint32_t>(per_row));
-    const int64_t rows_a_launch = (int64_t{1} << 31) / per_row;
-    for (a.first = 0; a.first < a.pos.n; a.first += rows_a_launch) {
-        const int64_t rows = a.pos.n - a.first < rows_a_launch ? a.pos.n - a.first : rows_a_launch;
-        a.total = static_cast<unsigned int>(rows * per_row);
-        const unsigned int grid = static_cast<unsigned int>((static_cast<int64_t>(a.total) + kThreads * 4 - 1) / (kThreads * 4));
-        if (vec) k_embedding<4><<<grid, kThreads, 0, stream>>>(a);
-        else k_embedding<1><<<grid, kThreads, 0, stream>>>(a);
-        MTC_TRY(check_launch("embedding"));
-    }
-    return MTC_OK;
+    a.vectors = vec ? dim / 4 : dim;
+    while (a.lanes_log2 < 5 && (int64_t{kLookupLoads} << a.lanes_log2) < a.vectors) ++a.lanes_log2;
+    const int64_t segment = int64_t{kLookupLoads} << a.lanes_log2;
+    if (a.vectors / segment >= UINT32_MAX) return fail(MTC_ERR_UNSUPPORTED, "embedding rows are too wide");
+    a.segments = static_cast<unsigned int>((a.vectors + segment - 1) / segment);
+    a.groups = a.pos.n * a.segments;
+    const int64_t ctas = ((a.groups << a.lanes_log2) + kThreads - 1) / kThreads;
+    const int64_t most = static_cast<int64_t>(sm_count(current_device())) * 8;
+    const unsigned int grid = static_cast<unsigned int>(ctas < most ? ctas : most);
+    if (vec) k_embedding<4><<<grid, kThreads, 0, stream>>>(a);
+    else k_embedding<1><<<grid, kThreads, 0, stream>>>(a);
+    return check_launch("embedding");
 }
 
 constexpr int kFewTiles = 32;      // tiles whose counts every CTA adds itself (one launch less)

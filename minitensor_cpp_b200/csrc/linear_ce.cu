@@ -4,9 +4,10 @@
 //   g_nv = dloss_n (exp(z_nv - lse_n) - [v = t_n])
 //   dx = g W                 dW = g^T x                          db_v = sum_n g_nv
 //
-// Rows without a loss are left out before any product: one CTA lists the others
-// in order (k_live_rows), and everything below runs over that list, whose length
-// only the device knows.
+// Three paths.  Few rows (up to 16) read W once in float32, whatever its size; small
+// problems take a warp a row; the others run on the tensor cores (linear_ce_tc.cu), over
+// the rows that have a loss: one CTA lists them in order (k_live_rows), and only the device
+// knows how many there are.
 #include <cfloat>
 #include <climits>
 #include <cstring>
@@ -91,278 +92,556 @@ __global__ void __launch_bounds__(256) k_zero_dx(const LinearCe p) {
     }
 }
 
-// ------------------------------------------------------------- small problems --
-// Float32 products on the FMA units, 64 x 64 tiles of the result.
+// ------------------------------------------------------------ shared pieces --
 
-struct Mat {
-    const float *p;
-    int64_t rs, cs;
-    const int *map;  // rows of the operand by way of this list; null: as they are
+// A row's target, or -1 for a row without a loss; reports one outside the vocabulary.
+__device__ __forceinline__ int row_target(const LinearCe &p, int64_t n, unsigned long long *err, bool report) {
+    const int64_t t = p.targets[n * p.t_s];
+    if (t == p.ignore) return -1;
+    if (t < 0 || t >= p.V) {
+        if (report) report_index(err, t);
+        return -1;
+    }
+    return static_cast<int>(t);
+}
+
+// Running maximum and sum of exponentials relative to it.  Infinite maxima count from 0,
+// so that a row of +inf or -inf has its limit and not exp(inf - inf).
+struct Softmax {
+    float top, sum;
 };
 
-struct SimtArgs {
-    Mat a, b;  // C[m, n] = sum_k a(m, k) b(k, n)
-    float *c;
-    int64_t c_rs, c_cs;
-    const int *c_map;
-    const float *bias;  // added to column n
-    int64_t bias_s;
-    int64_t M, N, K;
-    const int *live;  // rows with a loss: bounds M (live_dim 0) or K (live_dim 1), first..first + extent
-    int live_dim;
-    int64_t first;
-    int64_t k_split;  // K of one blockIdx.z; partial results [z][M][N] in c with several
+__device__ __forceinline__ float softmax_base(float top) { return isinf(top) ? 0.0f : top; }
+
+__device__ __forceinline__ Softmax merge(Softmax a, Softmax b) {
+    Softmax r;
+    r.top = fmaxf(a.top, b.top);
+    const float base = softmax_base(r.top);
+    r.sum = (a.sum != 0.0f ? a.sum * expf(softmax_base(a.top) - base) : 0.0f) +
+            (b.sum != 0.0f ? b.sum * expf(softmax_base(b.top) - base) : 0.0f);
+    return r;
+}
+
+__device__ __forceinline__ Softmax merge_lanes(Softmax s, int from, int to) {
+    for (int o = from; o < to; o <<= 1) {
+        Softmax other;
+        other.top = __shfl_xor_sync(0xFFFFFFFFu, s.top, o);
+        other.sum = __shfl_xor_sync(0xFFFFFFFFu, s.sum, o);
+        s = merge(s, other);
+    }
+    return s;
+}
+
+__device__ __forceinline__ float softmax_grad(float z, float lse, float d, bool hot) {
+    const float x = z - lse;
+    return d * (hot ? expm1f(x) : expf(x));
+}
+
+// ----------------------------------------------------------------- few rows --
+// Up to 16 rows: bound by reading W, once for the loss (131 MB of a 32000 x 1024 layer at
+// ## us) and once more, next to the writing of dW, for the gradients.  Float32 products on
+// the FMA units: at 16 rows 16 FMAs for 4 bytes of W, still less than its reading takes.
+//
+// k_few_logits: a warp takes four rows of W at a time, 128 columns a step, against all rows
+// of x in shared memory; one lane for each of its 4 N logits keeps their softmax.
+// k_few_grad: a CTA takes 128 columns and a part of the vocabulary; x's columns and the sums
+// of dx stay in registers, g comes from the logits by one exponential a class and lane.
+
+constexpr int kFewRows = 16;
+constexpr int kFewThreads = 256;
+constexpr int kFewShared = 160 * 1024;
+
+struct FewArgs {
+    int vec;             // float4 loads of W
+    int d_pad;           // x's row in shared memory, a multiple of 128
+    float *z;            // [N][V], null: not wanted
+    Softmax *parts;      // [CTAs][R]
+    int n_parts;
+    float *z_target;     // [R]
+    float *dx_parts;     // [splits][N][D]
+    int splits;
+    int dw_vec;
+    unsigned long long *err;
 };
 
-__global__ void __launch_bounds__(256) k_simt_product(const SimtArgs g) {
-    constexpr int T = 64, KT = 16;
-    __shared__ float as[KT][T + 1], bs[KT][T + 1];
-    int64_t M = g.M, K = g.K;
-    if (g.live_dim == 0) M = live_extent(g.live, g.first, M);
-    else K = live_extent(g.live, g.first, K);
-    const int64_t m0 = static_cast<int64_t>(blockIdx.x) * T, n0 = static_cast<int64_t>(blockIdx.y) * T;
-    if (m0 >= M) return;
-    const int64_t k_begin = static_cast<int64_t>(blockIdx.z) * g.k_split;
-    const int64_t k_end = k_begin + g.k_split < K ? k_begin + g.k_split : K;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const bool a_by_k = g.a.cs == 1, b_by_k = g.b.rs == 1;
-    float acc[4][4] = {};
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += KT) {
+template <int R, bool VEC>
+__global__ void __launch_bounds__(kFewThreads) k_few_logits(const LinearCe p, const FewArgs a) {
+    extern __shared__ __align__(16) float xs[];  // [R][d_pad]
+    __shared__ int target[R];
+    __shared__ Softmax warps[kFewThreads / 32][R];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x < R) {
+        const int n = threadIdx.x;
+        target[n] = n < p.N ? row_target(p, n, a.err, blockIdx.x == 0) : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * a.d_pad; i += kFewThreads) {
+        const int n = i / a.d_pad, d = i - n * a.d_pad;
+        xs[i] = n < p.N && d < p.D && target[n] >= 0 ? p.x[n * p.x_rs + d * p.x_cs] : 0.0f;
+    }
+    __syncthreads();
+    constexpr int kMine = (4 * R + 31) / 32;  // logits of a lane: i = lane + 32 k is row i / 4 and class i % 4
+    Softmax mine[kMine];
 #pragma unroll
-        for (int j = 0; j < T * KT / 256; ++j) {
-            const int e = j * 256 + threadIdx.x;
-            const int am = a_by_k ? e / KT : e % T, ak = a_by_k ? e % KT : e / T;
-            float v = 0.0f;
-            if (m0 + am < M && k0 + ak < k_end) {
-                const int64_t m = g.a.map != nullptr ? g.a.map[g.first + m0 + am] : m0 + am;
-                v = g.a.p[m * g.a.rs + (k0 + ak) * g.a.cs];
+    for (int k = 0; k < kMine; ++k) mine[k] = Softmax{-INFINITY, 0.0f};
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kFewThreads / 32) * 4;
+    for (int64_t v0 = (static_cast<int64_t>(blockIdx.x) * (kFewThreads / 32) + warp) * 4; v0 < p.V; v0 += step) {
+        const float *w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = p.w + (v0 + j < p.V ? v0 + j : p.V - 1) * p.w_rs;
+        float acc[4][R];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int n = 0; n < R; ++n) acc[j][n] = 0.0f;
+        constexpr int S = R <= 4 ? 2 : 1;  // steps in flight
+#pragma unroll 1
+        for (int64_t c0 = 0; c0 < p.D; c0 += 128 * S) {
+            float4 x[S][4];
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const int64_t c = c0 + s * 128 + lane * 4;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[s][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (VEC) {
+                        if (c < p.D) x[s][j] = __ldcs(reinterpret_cast<const float4 *>(w[j] + c));
+                    } else {  // a lane's four columns 32 apart, so that a load is contiguous where W is
+                        const int64_t b = c0 + s * 128 + lane;
+                        if (b < p.D) x[s][j].x = __ldcs(w[j] + b * p.w_cs);
+                        if (b + 32 < p.D) x[s][j].y = __ldcs(w[j] + (b + 32) * p.w_cs);
+                        if (b + 64 < p.D) x[s][j].z = __ldcs(w[j] + (b + 64) * p.w_cs);
+                        if (b + 96 < p.D) x[s][j].w = __ldcs(w[j] + (b + 96) * p.w_cs);
+                    }
+                }
             }
-            as[ak][am] = v;
-            const int bn = b_by_k ? e / KT : e % T, bk = b_by_k ? e % KT : e / T;
-            v = 0.0f;
-            if (n0 + bn < g.N && k0 + bk < k_end) {
-                const int64_t k = g.b.map != nullptr ? g.b.map[g.first + k0 + bk] : k0 + bk;
-                v = g.b.p[k * g.b.rs + (n0 + bn) * g.b.cs];
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                if (c0 + s * 128 >= p.D) break;
+#pragma unroll
+                for (int n = 0; n < R; ++n) {
+                    const float *row = xs + n * a.d_pad + c0 + s * 128;
+                    float4 y;
+                    if (VEC) y = *reinterpret_cast<const float4 *>(row + lane * 4);
+                    else y = make_float4(row[lane], row[lane + 32], row[lane + 64], row[lane + 96]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        acc[j][n] = fmaf(x[s][j].x, y.x, acc[j][n]);
+                        acc[j][n] = fmaf(x[s][j].y, y.y, acc[j][n]);
+                        acc[j][n] = fmaf(x[s][j].z, y.z, acc[j][n]);
+                        acc[j][n] = fmaf(x[s][j].w, y.w, acc[j][n]);
+                    }
+                }
             }
-            bs[bk][bn] = v;
         }
+        float z[kMine];
+#pragma unroll
+        for (int n = 0; n < R; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v = acc[j][n];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+                if (lane == (4 * n + j) % 32) z[(4 * n + j) / 32] = v;
+            }
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int i = lane + 32 * k, n = i / 4;
+            const int64_t v = v0 + i % 4;
+            if (n >= R || n >= p.N || v >= p.V) continue;
+            float x = z[k];
+            if (p.bias != nullptr) x += __ldg(p.bias + v * p.b_s);
+            if (a.z != nullptr) a.z[n * p.V + v] = x;
+            if (v == target[n]) a.z_target[n] = x;
+            mine[k] = merge(mine[k], Softmax{x, isnan(x) ? x : isinf(x) ? (x > 0.0f ? x : 0.0f) : 1.0f});
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+        const Softmax s = merge_lanes(mine[k], 1, 4);
+        const int i = lane + 32 * k;
+        if (i % 4 == 0 && i / 4 < R) warps[warp][i / 4] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < R) {
+        Softmax s = warps[0][threadIdx.x];
+        for (int w = 1; w < kFewThreads / 32; ++w) s = merge(s, warps[w][threadIdx.x]);
+        a.parts[blockIdx.x * R + threadIdx.x] = s;
+    }
+}
+
+// lse of row n from the CTAs' parts; every lane of the warp gets it.
+__device__ __forceinline__ float few_lse(const FewArgs &a, int R, int n) {
+    Softmax s{-INFINITY, 0.0f};
+    for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) s = merge(s, a.parts[i * R + n]);
+    s = merge_lanes(s, 1, 32);
+    return softmax_base(s.top) + logf(s.sum);
+}
+
+__device__ __forceinline__ void store_loss(const LinearCe &p, const FewArgs &a, int n, int target, float lse) {
+    if (p.loss != nullptr) p.loss[n * p.loss_s] = target < 0 ? 0.0f : lse - a.z_target[n];
+    if (p.lse != nullptr) p.lse[n * p.lse_s] = target < 0 ? 0.0f : lse;
+}
+
+__global__ void __launch_bounds__(32 * kFewRows) k_few_loss(const LinearCe p, const FewArgs a, int R) {
+    const int n = threadIdx.x / 32;
+    if (n >= p.N) return;
+    const float lse = few_lse(a, R, n);
+    if (threadIdx.x % 32 == 0) store_loss(p, a, n, row_target(p, n, a.err, false), lse);
+}
+
+template <int R>
+__global__ void __launch_bounds__(kFewThreads) k_few_grad(const LinearCe p, const FewArgs a) {
+    __shared__ float lse[R], dloss[R];
+    __shared__ int target[R];
+    __shared__ float4 sums[kFewThreads / 32][32];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int n = warp; n < R; n += kFewThreads / 32) {
+        const int t = n < p.N ? row_target(p, n, a.err, false) : -1;
+        const float l = n < p.N ? few_lse(a, R, n) : 0.0f;
+        if (lane == 0) {
+            lse[n] = l;
+            target[n] = t;
+            dloss[n] = t >= 0 ? p.dloss[n * p.dl_s] : 0.0f;
+            if (n < p.N && blockIdx.x == 0 && blockIdx.y == 0) store_loss(p, a, n, t, l);
+        }
+    }
+    __syncthreads();
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + lane * 4;
+    const int cols = static_cast<int>(p.D - c < 0 ? 0 : p.D - c < 4 ? p.D - c : 4);
+    float4 x[R], dx[R];
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+        x[n] = dx[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (n >= p.N || target[n] < 0) continue;
+        const float *src = p.x + n * p.x_rs + c * p.x_cs;
+        if (cols > 0) x[n].x = src[0];
+        if (cols > 1) x[n].y = src[p.x_cs];
+        if (cols > 2) x[n].z = src[2 * p.x_cs];
+        if (cols > 3) x[n].w = src[3 * p.x_cs];
+    }
+    const int64_t step = static_cast<int64_t>(gridDim.y) * (kFewThreads / 32) * 32;
+    for (int64_t v0 = (static_cast<int64_t>(blockIdx.y) * (kFewThreads / 32) + warp) * 32; v0 < p.V; v0 += step) {
+        const int64_t v = v0 + lane;
+        float g[R], db = 0.0f;
+#pragma unroll
+        for (int n = 0; n < R; ++n) {
+            g[n] = 0.0f;
+            if (n < p.N && v < p.V && target[n] >= 0) g[n] = softmax_grad(a.z[n * p.V + v], lse[n], dloss[n], v == target[n]);
+            db += g[n];
+        }
+        if (p.db != nullptr && blockIdx.x == 0 && v < p.V) p.db[v * p.db_s] = db;
+        const int count = static_cast<int>(p.V - v0 < 32 ? p.V - v0 : 32);
+        constexpr int U = 4;
+        for (int j0 = 0; j0 < count; j0 += U) {
+            float4 w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                w[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (p.dx == nullptr || j0 + u >= count) continue;
+                const float *src = p.w + (v0 + j0 + u) * p.w_rs + c * p.w_cs;
+                if (a.vec) {
+                    if (cols > 0) w[u] = __ldcs(reinterpret_cast<const float4 *>(src));
+                } else {
+                    if (cols > 0) w[u].x = __ldcs(src);
+                    if (cols > 1) w[u].y = __ldcs(src + p.w_cs);
+                    if (cols > 2) w[u].z = __ldcs(src + 2 * p.w_cs);
+                    if (cols > 3) w[u].w = __ldcs(src + 3 * p.w_cs);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (j0 + u >= count) break;
+                float4 dw = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int n = 0; n < R; ++n) {
+                    const float gn = __shfl_sync(0xFFFFFFFFu, g[n], j0 + u);
+                    dx[n].x = fmaf(gn, w[u].x, dx[n].x);
+                    dx[n].y = fmaf(gn, w[u].y, dx[n].y);
+                    dx[n].z = fmaf(gn, w[u].z, dx[n].z);
+                    dx[n].w = fmaf(gn, w[u].w, dx[n].w);
+                    dw.x = fmaf(gn, x[n].x, dw.x);
+                    dw.y = fmaf(gn, x[n].y, dw.y);
+                    dw.z = fmaf(gn, x[n].z, dw.z);
+                    dw.w = fmaf(gn, x[n].w, dw.w);
+                }
+                if (p.dw == nullptr) continue;
+                float *to = p.dw + (v0 + j0 + u) * p.dw_rs + c * p.dw_cs;
+                if (a.dw_vec) {
+                    if (cols > 0) *reinterpret_cast<float4 *>(to) = dw;
+                } else {
+                    if (cols > 0) to[0] = dw.x;
+                    if (cols > 1) to[p.dw_cs] = dw.y;
+                    if (cols > 2) to[2 * p.dw_cs] = dw.z;
+                    if (cols > 3) to[3 * p.dw_cs] = dw.w;
+                }
+            }
+        }
+    }
+    if (p.dx == nullptr) return;
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+        if (n >= p.N) break;
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = as[k][ty + 16 * i];
-                b[i] = bs[k][tx + 16 * i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-        }
+        sums[warp][lane] = dx[n];
         __syncthreads();
-    }
-    float *c = g.c;
-    if (gridDim.z > 1) c += static_cast<int64_t>(blockIdx.z) * g.M * g.N;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t m = m0 + ty + 16 * i;
-        if (m >= M) continue;
-        const int64_t row = g.c_map != nullptr ? g.c_map[g.first + m] : m;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t n = n0 + tx + 16 * j;
-            if (n >= g.N) continue;
-            float v = acc[i][j];
-            if (g.bias != nullptr) v += g.bias[n * g.bias_s];
-            if (gridDim.z > 1) c[m * g.N + n] = v;
-            else c[row * g.c_rs + n * g.c_cs] = v;
+        if (warp != 0) continue;
+        float4 s = sums[0][lane];
+        for (int w = 1; w < kFewThreads / 32; ++w) {
+            s.x += sums[w][lane].x;
+            s.y += sums[w][lane].y;
+            s.z += sums[w][lane].z;
+            s.w += sums[w][lane].w;
         }
+        float *to = a.dx_parts + (blockIdx.y * p.N + n) * p.D + c;
+        if (cols > 0) to[0] = s.x;
+        if (cols > 1) to[1] = s.y;
+        if (cols > 2) to[2] = s.z;
+        if (cols > 3) to[3] = s.w;
     }
 }
 
-// Sums the K splits in order into C, adding to it where `add`.
-__global__ void __launch_bounds__(256) k_simt_join(const float *parts, int splits, int64_t M, int64_t N, float *c,
-                                                   int64_t c_rs, int64_t c_cs, int add) {
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < M * N;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
-        float sum = 0.0f;
-        for (int s = 0; s < splits; ++s) sum += parts[s * M * N + i];
-        float *to = c + (i / N) * c_rs + (i % N) * c_cs;
-        *to = add ? *to + sum : sum;
-    }
-}
-
-__device__ __forceinline__ float block_reduce(float v, bool take_max) {
-    __shared__ float part[32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        v = take_max ? fmaxf(v, y) : v + y;
-    }
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
-    __syncthreads();
-    const int warps = blockDim.x / 32;
-    v = static_cast<int>(threadIdx.x % 32) < warps ? part[threadIdx.x % 32] : take_max ? -INFINITY : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        v = take_max ? fmaxf(v, y) : v + y;
-    }
-    return v;
-}
-
-// One CTA a row of logits: lse and loss, then g in the place of z.
-__global__ void __launch_bounds__(256) k_softmax_rows(const LinearCe p, const LiveRows live, int64_t first, int64_t rows,
-                                                      float *z) {
-    const int64_t r = blockIdx.x;
-    if (r >= live_extent(live.count, first, rows)) return;
-    float *zr = z + r * p.V;
-    float top = -INFINITY;
-    bool nan = false;
-    for (int64_t v = threadIdx.x; v < p.V; v += 256) {
-        const float x = zr[v];
-        top = fmaxf(top, x);
-        nan |= isnan(x);
-    }
-    nan = __syncthreads_or(nan);
-    top = block_reduce(top, true);
-    if (nan) top = NAN;
+__global__ void __launch_bounds__(256) k_few_dx(const LinearCe p, const FewArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= p.N * p.D) return;
+    const int64_t n = i / p.D;
     float sum = 0.0f;
-    const float base = isinf(top) ? 0.0f : top;  // exp(inf - inf) would make a NaN of a row that has a limit
-    for (int64_t v = threadIdx.x; v < p.V; v += 256) sum += expf(zr[v] - base);
-    sum = block_reduce(sum, false);
-    const float lse = base + logf(sum);
-    const int t = live.target[first + r];
-    const int64_t n = live.row[first + r];
-    if (threadIdx.x == 0) {
-        if (p.lse != nullptr) p.lse[n * p.lse_s] = lse;
-        if (p.loss != nullptr) p.loss[n * p.loss_s] = lse - zr[t];
-    }
-    if (p.dloss == nullptr) return;
-    __syncthreads();
-    const float d = live.dloss[first + r];
-    for (int64_t v = threadIdx.x; v < p.V; v += 256) {
-        const float x = zr[v] - lse;
-        zr[v] = d * (v == t ? expm1f(x) : expf(x));
-    }
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) sum += a.dx_parts[s * p.N * p.D + i];
+    if (row_target(p, n, a.err, false) < 0) sum = 0.0f;
+    p.dx[n * p.dx_rs + (i - n * p.D) * p.dx_cs] = sum;
 }
 
-constexpr int64_t kSplitRows = 256;
-
-int simt_product(SimtArgs &g, cudaStream_t stream, int splits) {
-    const dim3 grid(static_cast<unsigned>((g.M + 63) / 64), static_cast<unsigned>((g.N + 63) / 64),
-                    static_cast<unsigned>(splits));
-    if ((g.N + 63) / 64 > 65535 || splits > 65535) return fail(MTC_ERR_UNSUPPORTED, "linear cross entropy: too many columns");
-    k_simt_product<<<grid, 256, 0, stream>>>(g);
-    return check_launch("linear cross entropy (product)");
-}
-
-// Column sums of g over the chunk's rows: a product with a row of ones.
-__global__ void __launch_bounds__(256) k_column_sums(const float *g, int64_t V, const int *live, int64_t first,
-                                                     int64_t rows, float *db, int64_t db_s, int add) {
-    const int64_t v = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
-    const int64_t n = live_extent(live, first, rows);
-    __shared__ float part[8][32];
-    float sum = 0.0f;
-    if (v < V)
-        for (int64_t r = threadIdx.x / 32; r < n; r += 8) sum += g[r * V + v];
-    part[threadIdx.x / 32][threadIdx.x % 32] = sum;
-    __syncthreads();
-    if (threadIdx.x >= 32 || v >= V) return;
-    sum = 0.0f;
-    for (int w = 0; w < 8; ++w) sum += part[w][threadIdx.x];
-    db[v * db_s] = add ? db[v * db_s] + sum : sum;
-}
-
-int simt_path(const LinearCe &p, cudaStream_t stream) {
-    int64_t chunk = (int64_t{1} << 28) / (p.V * 4);
-    if (chunk < 64) chunk = 64;
-    if (chunk > p.N) chunk = p.N;
-    const int splits = static_cast<int>((chunk + kSplitRows - 1) / kSplitRows);
-    const size_t list = padded(static_cast<size_t>(p.N) * 4);
-    const size_t zs = padded(static_cast<size_t>(chunk) * p.V * 4);
-    const size_t parts = p.dw != nullptr && splits > 1 ? padded(static_cast<size_t>(splits) * p.V * p.D * 4) : 0;
+template <int R>
+int few_path(const LinearCe &p, cudaStream_t stream) {
+    const int sms = sm_count(current_device());
+    const bool grads = p.dloss != nullptr && (p.dx != nullptr || p.dw != nullptr || p.db != nullptr);
+    FewArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.vec = aligned16(p.w) && p.w_cs == 1 && p.w_rs % 4 == 0 && p.D % 4 == 0;
+    a.dw_vec = aligned16(p.dw) && p.dw_cs == 1 && p.dw_rs % 4 == 0 && p.D % 4 == 0;
+    a.d_pad = static_cast<int>((p.D + 127) / 128 * 128);
+    const size_t shared = static_cast<size_t>(R) * a.d_pad * 4;
+    const int64_t wanted = (p.V + 31) / 32;  // CTAs of 8 warps, 4 classes each
+    const int64_t resident = static_cast<int64_t>(sms) * (shared > 72 * 1024 ? 1 : shared > 48 * 1024 ? 2 : 3);
+    a.n_parts = static_cast<int>(wanted < resident ? wanted : resident);
+    const int64_t slabs = (p.D + 127) / 128 > 0 ? (p.D + 127) / 128 : 1;
+    int64_t splits = (static_cast<int64_t>(sms) * 4 + slabs - 1) / slabs;
+    const int64_t most = (p.V + 255) / 256;  // 8 warps of 32 classes
+    a.splits = static_cast<int>(splits < most ? splits : most);
+    const size_t parts = padded(static_cast<size_t>(a.n_parts) * R * sizeof(Softmax));
+    const size_t zs = grads ? padded(static_cast<size_t>(p.N) * p.V * 4) : 0;
+    const size_t dxs = grads && p.dx != nullptr ? padded(static_cast<size_t>(a.splits) * p.N * p.D * 4) : 0;
     Workspace ws;
-    MTC_TRY(ws.allocate(256 + 3 * list + zs + parts, stream));
-    LiveRows live;
-    live.count = ws.take<int>(256);
-    live.row = ws.take<int>(list);
-    live.target = ws.take<int>(list);
-    live.dloss = ws.take<float>(list);
+    MTC_TRY(ws.allocate(256 + parts + zs + dxs, stream));
+    a.z_target = ws.take<float>(256);
+    a.parts = ws.take<Softmax>(parts);
     float *z = ws.take<float>(zs);
-    float *part = ws.take<float>(parts);
-    MTC_TRY(list_live_rows(p, live, stream));
-    for (int64_t first = 0; first < p.N; first += chunk) {
-        const int64_t rows = p.N - first < chunk ? p.N - first : chunk;
-        SimtArgs g;
-        std::memset(&g, 0, sizeof(g));
-        g.a = Mat{p.x, p.x_rs, p.x_cs, live.row};
-        g.b = Mat{p.w, p.w_cs, p.w_rs, nullptr};
-        g.c = z;
-        g.c_rs = p.V;
-        g.c_cs = 1;
-        g.bias = p.bias;
-        g.bias_s = p.b_s;
-        g.M = rows;
-        g.N = p.V;
-        g.K = g.k_split = p.D;
-        g.live = live.count;
-        g.first = first;
-        MTC_TRY(simt_product(g, stream, 1));
-        k_softmax_rows<<<static_cast<unsigned>(rows), 256, 0, stream>>>(p, live, first, rows, z);
-        MTC_TRY(check_launch("linear cross entropy (softmax)"));
-        if (p.dx != nullptr && p.D > 0) {
-            std::memset(&g, 0, sizeof(g));
-            g.a = Mat{z, p.V, 1, nullptr};
-            g.b = Mat{p.w, p.w_rs, p.w_cs, nullptr};
-            g.c = p.dx;
-            g.c_rs = p.dx_rs;
-            g.c_cs = p.dx_cs;
-            g.c_map = live.row;
-            g.M = rows;
-            g.N = p.D;
-            g.K = g.k_split = p.V;
-            g.live = live.count;
-            g.first = first;
-            MTC_TRY(simt_product(g, stream, 1));
+    a.dx_parts = ws.take<float>(dxs);
+    a.z = grads ? z : nullptr;
+    MTC_TRY(device_error_word(&a.err));
+    if (a.vec) {
+        MTC_CUDA_TRY(cudaFuncSetAttribute(k_few_logits<R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared));
+        k_few_logits<R, true><<<a.n_parts, kFewThreads, shared, stream>>>(p, a);
+    } else {
+        MTC_CUDA_TRY(cudaFuncSetAttribute(k_few_logits<R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared));
+        k_few_logits<R, false><<<a.n_parts, kFewThreads, shared, stream>>>(p, a);
+    }
+    MTC_TRY(check_launch("linear cross entropy (few rows)"));
+    if (!grads) {
+        k_few_loss<<<1, static_cast<unsigned>(32 * p.N), 0, stream>>>(p, a, R);
+        return check_launch("linear cross entropy (loss)");
+    }
+    k_few_grad<R><<<dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(a.splits)), kFewThreads, 0, stream>>>(p, a);
+    MTC_TRY(check_launch("linear cross entropy (few rows' gradients)"));
+    if (p.dx == nullptr || p.D == 0) return MTC_OK;
+    k_few_dx<<<static_cast<unsigned>((p.N * p.D + 255) / 256), 256, 0, stream>>>(p, a);
+    return check_launch("linear cross entropy (input gradient)");
+}
+
+// ------------------------------------------------------------- small problems --
+// Up to 256 classes and 2^22 products: bound by latency, so two launches.  k_small_rows: a
+// warp a row, its lanes over the classes (and over the columns where the classes are few),
+// loss, g and the row of dx.  k_small_weights: a thread an element of dW (or of db), 32 rows
+// a CTA; the last CTA of an element's to finish adds the parts in the order of the rows.
+
+constexpr int kSmallClasses = 256;
+constexpr int kSmallRows = 32;
+
+struct SmallArgs {
+    float *g;               // [N][V], null: no gradients
+    float *parts;           // [splits][V D + V]
+    unsigned int *arrived;  // [CTAs of one split]
+    unsigned int n_arrived;
+    int classes_log2;       // lanes over classes
+    unsigned long long *err;
+};
+
+__global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const SmallArgs a) {
+    if (a.g != nullptr)
+        for (unsigned int i = blockIdx.x * 256 + threadIdx.x; i < a.n_arrived; i += gridDim.x * 256) a.arrived[i] = 0;
+    const int lane = threadIdx.x % 32;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+    if (n >= p.N) return;
+    const int t = row_target(p, n, a.err, lane == 0);
+    if (t < 0) {
+        if (lane == 0) {
+            if (p.loss != nullptr) p.loss[n * p.loss_s] = 0.0f;
+            if (p.lse != nullptr) p.lse[n * p.lse_s] = 0.0f;
         }
-        if (p.dw != nullptr && p.D > 0) {
-            std::memset(&g, 0, sizeof(g));
-            g.a = Mat{z, 1, p.V, nullptr};
-            g.b = Mat{p.x, p.x_rs, p.x_cs, live.row};
-            g.c = part;
-            g.M = p.V;
-            g.N = p.D;
-            g.K = rows;
-            g.live = live.count;
-            g.live_dim = 1;
-            g.first = first;
-            const int s = static_cast<int>((rows + kSplitRows - 1) / kSplitRows);
-            g.k_split = kSplitRows;
-            if (s == 1 && first == 0) {
-                g.c = p.dw;
-                g.c_rs = p.dw_rs;
-                g.c_cs = p.dw_cs;
-                MTC_TRY(simt_product(g, stream, 1));
-            } else {
-                g.c_rs = p.D;
-                g.c_cs = 1;
-                MTC_TRY(simt_product(g, stream, s));
-                const int64_t blocks = (p.V * p.D + 255) / 256;
-                k_simt_join<<<static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(
-                    part, s, p.V, p.D, p.dw, p.dw_rs, p.dw_cs, first > 0);
-                MTC_TRY(check_launch("linear cross entropy (weight gradient)"));
+        if (a.g == nullptr) return;
+        for (int64_t v = lane; v < p.V; v += 32) a.g[n * p.V + v] = 0.0f;
+        if (p.dx != nullptr)
+            for (int64_t d = lane; d < p.D; d += 32) p.dx[n * p.dx_rs + d * p.dx_cs] = 0.0f;
+        return;
+    }
+    const int C = 1 << a.classes_log2, L = 32 / C;  // L lanes share a class
+    const int sub = lane % L;
+    const float *x = p.x + n * p.x_rs;
+    constexpr int kMost = kSmallClasses / 32;
+    float z[kMost];
+    Softmax s{-INFINITY, 0.0f};
+    float zt = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        z[i] = 0.0f;
+        if (i * C >= p.V) continue;
+        const int v = i * C + lane / L;
+        const float *w = p.w + (v < p.V ? v : 0) * p.w_rs;
+        float sum = 0.0f;
+        int64_t d = sub;
+        for (; d + 15 * L < p.D; d += 16 * L) {
+            float xv[16], wv[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                xv[u] = __ldg(x + (d + u * L) * p.x_cs);
+                wv[u] = __ldg(w + (d + u * L) * p.w_cs);
+            }
+#pragma unroll
+            for (int u = 0; u < 16; ++u) sum = fmaf(xv[u], wv[u], sum);
+        }
+        for (; d < p.D; d += L) sum = fmaf(__ldg(x + d * p.x_cs), __ldg(w + d * p.w_cs), sum);
+        for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (v >= p.V) {
+            z[i] = -INFINITY;
+            continue;
+        }
+        if (p.bias != nullptr) sum += __ldg(p.bias + v * p.b_s);
+        z[i] = sum;
+        if (v == t) zt = sum;
+        if (sub == 0) s = merge(s, Softmax{sum, isnan(sum) ? sum : isinf(sum) ? (sum > 0.0f ? sum : 0.0f) : 1.0f});
+    }
+    s = merge_lanes(s, 1, 32);
+    const float lse = softmax_base(s.top) + logf(s.sum);
+    zt = __shfl_sync(0xFFFFFFFFu, zt, t % C * L);
+    if (lane == 0) {
+        if (p.loss != nullptr) p.loss[n * p.loss_s] = lse - zt;
+        if (p.lse != nullptr) p.lse[n * p.lse_s] = lse;
+    }
+    if (a.g == nullptr) return;
+    const float dl = p.dloss[n * p.dl_s];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int v = i * C + lane / L;
+        if (i * C >= p.V || v >= p.V) {
+            z[i] = 0.0f;
+            continue;
+        }
+        z[i] = softmax_grad(z[i], lse, dl, v == t);
+        if (sub == 0) a.g[n * p.V + v] = z[i];
+    }
+    if (p.dx == nullptr) return;
+    for (int64_t d0 = 0; d0 < p.D; d0 += 128) {
+        float dx[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) {
+            if (i * C >= p.V) break;
+            const int classes = static_cast<int>(p.V - i * C < C ? p.V - i * C : C);
+#pragma unroll 4
+            for (int c = 0; c < classes; ++c) {
+                const float g = __shfl_sync(0xFFFFFFFFu, z[i], c * L);
+                const float *w = p.w + static_cast<int64_t>(i * C + c) * p.w_rs;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t d = d0 + u * 32 + lane;
+                    if (d < p.D) dx[u] = fmaf(g, __ldg(w + d * p.w_cs), dx[u]);
+                }
             }
         }
-        if (p.db != nullptr) {
-            k_column_sums<<<static_cast<unsigned>((p.V + 31) / 32), 256, 0, stream>>>(z, p.V, live.count, first, rows,
-                                                                                     p.db, p.db_s, first > 0);
-            MTC_TRY(check_launch("linear cross entropy (bias gradient)"));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t d = d0 + u * 32 + lane;
+            if (d < p.D) p.dx[n * p.dx_rs + d * p.dx_cs] = dx[u];
         }
     }
-    return MTC_OK;
+}
+
+__global__ void __launch_bounds__(256) k_small_weights(const LinearCe p, const SmallArgs a) {
+    const int64_t weights = p.V * p.D, total = weights + p.V;
+    const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t v = e < weights ? e / p.D : e - weights, d = e - v * p.D;
+    float sum = 0.0f;
+    if (e < total) {
+        const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kSmallRows;
+        const int rows = static_cast<int>(p.N - r0 < kSmallRows ? p.N - r0 : kSmallRows);
+        const float *g = a.g + r0 * p.V + v, *x = p.x + r0 * p.x_rs + d * p.x_cs;
+        for (int j0 = 0; j0 < rows; j0 += 16) {
+            float gv[16], xv[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                gv[u] = j0 + u < rows ? g[(j0 + u) * p.V] : 0.0f;
+                xv[u] = e >= weights || j0 + u >= rows ? 1.0f : __ldg(x + (j0 + u) * p.x_rs);
+            }
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+                if (gv[u] != 0.0f) sum = fmaf(gv[u], xv[u], sum);  // a row without a loss may hold anything
+        }
+    }
+    if (gridDim.y > 1) {
+        __shared__ bool last;
+        if (e < total) a.parts[blockIdx.y * total + e] = sum;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) last = atomicAdd(&a.arrived[blockIdx.x], 1u) == gridDim.y - 1;
+        __syncthreads();
+        if (!last) return;
+        __threadfence();
+        if (e >= total) return;
+        sum = 0.0f;
+#pragma unroll 8
+        for (unsigned int s = 0; s < gridDim.y; ++s) sum += __ldcg(a.parts + s * total + e);
+    }
+    if (e < weights) {
+        if (p.dw != nullptr) p.dw[v * p.dw_rs + d * p.dw_cs] = sum;
+    } else if (e < total && p.db != nullptr) {
+        p.db[v * p.db_s] = sum;
+    }
+}
+
+int small_path(const LinearCe &p, cudaStream_t stream) {
+    const bool grads = p.dloss != nullptr && (p.dx != nullptr || p.dw != nullptr || p.db != nullptr);
+    SmallArgs a;
+    std::memset(&a, 0, sizeof(a));
+    while (a.classes_log2 < 5 && (1 << a.classes_log2) < p.V) ++a.classes_log2;
+    const int64_t total = p.V * p.D + p.V;
+    const int64_t splits = (p.N + kSmallRows - 1) / kSmallRows;
+    a.n_arrived = static_cast<unsigned int>((total + 255) / 256);
+    MTC_TRY(device_error_word(&a.err));
+    Workspace ws;
+    if (grads) {
+        const size_t gs = padded(static_cast<size_t>(p.N) * p.V * 4);
+        const size_t parts = splits > 1 ? padded(static_cast<size_t>(splits) * total * 4) : 0;
+        const size_t arrived = padded(static_cast<size_t>(a.n_arrived) * 4);
+        MTC_TRY(ws.allocate(gs + parts + arrived, stream));
+        a.g = ws.take<float>(gs);
+        a.parts = ws.take<float>(parts);
+        a.arrived = ws.take<unsigned int>(arrived);
+    }
+    k_small_rows<<<static_cast<unsigned>((p.N + 7) / 8), 256, 0, stream>>>(p, a);
+    MTC_TRY(check_launch("linear cross entropy (small)"));
+    if (!grads || (p.dw == nullptr && p.db == nullptr)) return MTC_OK;
+    k_small_weights<<<dim3(a.n_arrived, static_cast<unsigned>(splits)), 256, 0, stream>>>(p, a);
+    return check_launch("linear cross entropy (small, weight gradient)");
 }
 
 // ------------------------------------------------------------------- host --
@@ -450,8 +729,16 @@ int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bia
         MTC_TRY(zero_view(dw, stream));
         return zero_view(db, stream);
     }
-    // Small problems stay on the FMA units.
-    if (p.N * p.V < (int64_t{1} << 22) / (p.D + 1)) return simt_path(p, stream);
+    if (p.V <= kSmallClasses && p.N < (int64_t{1} << 21) && p.N * p.V < (int64_t{1} << 22) / (p.D + 1))
+        return small_path(p, stream);
+    if (p.N <= kFewRows) {
+        const int64_t row = (p.D + 127) / 128 * 512;
+        if (p.N == 1 && row <= kFewShared) return few_path<1>(p, stream);
+        if (p.N <= 2 && 2 * row <= kFewShared) return few_path<2>(p, stream);
+        if (p.N <= 4 && 4 * row <= kFewShared) return few_path<4>(p, stream);
+        if (p.N <= 8 && 8 * row <= kFewShared) return few_path<8>(p, stream);
+        if (16 * row <= kFewShared) return few_path<16>(p, stream);
+    }
     return linear_ce_tensor(p, stream);
 }
 

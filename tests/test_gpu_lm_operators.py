@@ -700,8 +700,9 @@ def test_a_foreign_capture_is_refused(cuda):
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     views = [view(v) for v in (x, w, t, loss, grad, out, norm)]
+    dl = view(dloss)
     with torch.cuda.graph(graph, capture_error_mode="relaxed"):
-        for call in (lambda: abi.linear_cross_entropy(views[0], views[1], views[2], views[3]),
+        for call in (lambda: abi.linear_cross_entropy_grad(views[0], views[1], views[2], dl, dweight=views[4]),
                      lambda: abi.embedding_grad(views[0], views[2], views[4]),
                      lambda: abi.global_norm([views[1]], views[6]),
                      lambda: abi.clip_global_norm([views[1]], 1.0)):
