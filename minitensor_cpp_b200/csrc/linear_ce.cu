@@ -6,8 +6,10 @@
 //
 // Three paths.  Few rows (up to 16) read W once in float32, whatever its size; small
 // problems take a warp a row; the others run on the tensor cores (linear_ce_tc.cu), over
-// the rows that have a loss: one CTA lists them in order (k_live_rows), and only the device
-// knows how many there are.
+// the rows that have a loss: k_live_rows lists them in order, and only the device knows how
+// many there are.
+#include <cooperative_groups.h>
+
 #include <cfloat>
 #include <climits>
 #include <cstring>
@@ -16,6 +18,8 @@
 
 namespace mtc {
 namespace {
+
+constexpr int kListThreads = 1024, kListRows = 4, kListCtas = 16;
 
 __device__ __forceinline__ int block_exclusive(int v, int *warp_sums, int &total) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -28,68 +32,88 @@ __device__ __forceinline__ int block_exclusive(int v, int *warp_sums, int &total
     __syncthreads();
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x / 32); ++w) {
-        if (w < warp) before += warp_sums[w];
-        total += warp_sums[w];
-    }
-    return before + x - v;
+    const int w = warp_sums[lane];
+    total = __reduce_add_sync(0xFFFFFFFFu, w);
+    return __reduce_add_sync(0xFFFFFFFFu, lane < warp ? w : 0) + x - v;
 }
 
-// The rows with a loss, in order; zero loss, lse and dx count for the others.
-__global__ void __launch_bounds__(1024) k_live_rows(const LinearCe p, const LiveRows live, unsigned long long *err) {
+// The rows with a loss, in order, and from the end of the list backwards those without;
+// zero loss and lse of the latter.  One cluster: each CTA counts its part of the rows, the
+// counts before it tell where its rows go.
+__global__ void __launch_bounds__(kListThreads) k_live_rows(const LinearCe p, const LiveRows live,
+                                                            unsigned long long *err) {
     __shared__ int warp_sums[32];
-    constexpr int U = 4;
-    int first = 0;
-    for (int64_t n0 = 0; n0 < p.N; n0 += 1024 * U) {
-        int64_t t[U];
-        bool has[U];
+    __shared__ int counted;
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int me = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+    constexpr int kTile = kListThreads * kListRows;
+    const int64_t tiles = (p.N + kTile - 1) / kTile;
+    const int64_t begin = tiles * me / ctas * kTile, end_tile = tiles * (me + 1) / ctas * kTile;
+    const int64_t end = end_tile < p.N ? end_tile : p.N;
+    int64_t t[kListRows];
+    auto load = [&](int64_t n0, bool report) {  // targets of the tile at n0; how many have a loss
+#pragma unroll
+        for (int u = 0; u < kListRows; ++u) {
+            const int64_t n = n0 + static_cast<int64_t>(threadIdx.x) * kListRows + u;
+            t[u] = n < end ? p.targets[n * p.t_s] : p.ignore;
+        }
         int mine = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t n = n0 + static_cast<int64_t>(threadIdx.x) * U + u;
-            has[u] = false;
-            t[u] = 0;
-            if (n >= p.N) continue;
-            t[u] = p.targets[n * p.t_s];
-            has[u] = t[u] != p.ignore;
-            if (has[u] && (t[u] < 0 || t[u] >= p.V)) {
-                report_index(err, t[u]);
-                has[u] = false;
+        for (int u = 0; u < kListRows; ++u) {
+            if (t[u] == p.ignore) {
+                t[u] = -1;
+            } else if (t[u] < 0 || t[u] >= p.V) {
+                if (report) report_index(err, t[u]);
+                t[u] = -1;
             }
-            mine += has[u];
-            if (!has[u]) {
+            mine += t[u] >= 0;
+        }
+        return mine;
+    };
+    int mine = 0;
+    for (int64_t n0 = begin; n0 < end; n0 += kTile) mine += load(n0, true);
+    int count;
+    (void)block_exclusive(mine, warp_sums, count);
+    if (threadIdx.x == 0) counted = count;
+    cluster.sync();
+    int first = 0, all = 0;
+    for (int r = 0; r < ctas; ++r) {
+        const int c = *cluster.map_shared_rank(&counted, r);
+        if (r < me) first += c;
+        all += c;
+    }
+    int64_t dead = p.N - 1 - (begin - first);  // where the next row without a loss goes
+    for (int64_t n0 = begin; n0 < end; n0 += kTile) {
+        const int has = load(n0, false);
+        int total;
+        int at = block_exclusive(has, warp_sums, total);
+        const int64_t n1 = n0 + static_cast<int64_t>(threadIdx.x) * kListRows;
+        int64_t none = dead - (static_cast<int64_t>(threadIdx.x) * kListRows - at);
+        at += first;
+#pragma unroll
+        for (int u = 0; u < kListRows; ++u) {
+            const int64_t n = n1 + u;
+            if (n >= end) break;
+            if (t[u] >= 0) {
+                live.row[at] = static_cast<int>(n);
+                live.target[at] = static_cast<int>(t[u]);
+                if (p.dloss != nullptr) live.dloss[at] = p.dloss[n * p.dl_s];
+                ++at;
+            } else {
+                live.row[none--] = static_cast<int>(n);
                 if (p.loss != nullptr) p.loss[n * p.loss_s] = 0.0f;
                 if (p.lse != nullptr) p.lse[n * p.lse_s] = 0.0f;
             }
         }
-        int total;
-        int at = first + block_exclusive(mine, warp_sums, total);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (!has[u]) continue;
-            const int64_t n = n0 + static_cast<int64_t>(threadIdx.x) * U + u;
-            live.row[at] = static_cast<int>(n);
-            live.target[at] = static_cast<int>(t[u]);
-            if (p.dloss != nullptr) live.dloss[at] = p.dloss[n * p.dl_s];
-            ++at;
-        }
         first += total;
+        dead -= kTile - total;
     }
-    if (threadIdx.x == 0) {
-        live.count[0] = first;
+    if (me == 0 && threadIdx.x == 0) {
+        live.count[0] = all;
         live.count[1] = live.count[2] = live.count[3] = 0;
     }
-}
-
-// dx rows without a loss.
-__global__ void __launch_bounds__(256) k_zero_dx(const LinearCe p) {
-    for (int64_t n = blockIdx.x; n < p.N; n += gridDim.x) {
-        const int64_t t = p.targets[n * p.t_s];
-        if (t != p.ignore && t >= 0 && t < p.V) continue;
-        for (int64_t d = threadIdx.x; d < p.D; d += 256) p.dx[n * p.dx_rs + d * p.dx_cs] = 0.0f;
-    }
+    cluster.sync();  // nobody leaves while its count is read
 }
 
 // ------------------------------------------------------------ shared pieces --
@@ -808,11 +832,24 @@ int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bia
 int list_live_rows(const LinearCe &p, const LiveRows &live, cudaStream_t stream) {
     unsigned long long *err = nullptr;
     MTC_TRY(device_error_word(&err));
-    k_live_rows<<<1, 1024, 0, stream>>>(p, live, err);
-    MTC_TRY(check_launch("linear cross entropy (rows)"));
-    if (p.dx == nullptr || p.D == 0) return MTC_OK;
-    k_zero_dx<<<static_cast<unsigned>(p.N < 1184 ? p.N : 1184), 256, 0, stream>>>(p);
-    return check_launch("linear cross entropy (zero rows)");
+    const int64_t tiles = (p.N + kListThreads * kListRows - 1) / (kListThreads * kListRows);
+    unsigned int ctas = 1;
+    while (ctas < kListCtas && ctas < tiles) ctas *= 2;
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_live_rows, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t config;
+    std::memset(&config, 0, sizeof(config));
+    config.gridDim = dim3(ctas);
+    config.blockDim = dim3(kListThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    std::memset(&attr, 0, sizeof(attr));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    MTC_CUDA_TRY(cudaLaunchKernelEx(&config, k_live_rows, p, live, err));
+    return check_launch("linear cross entropy (rows)");
 }
 
 }  // namespace mtc

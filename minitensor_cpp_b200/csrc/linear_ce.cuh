@@ -28,13 +28,12 @@ struct LinearCe {
 // What the device knows about the rows that have a loss.
 struct LiveRows {
     int *count;      // [1], and behind it the largest finite |x|, |weight| and |dloss| as bits [3], zeroed with it
-    int *row;        // [N] the row of x
+    int *row;        // [N] the row of x; behind them, from the end backwards, the rows without a loss
     int *target;     // [N]
     float *dloss;    // [N]
 };
 
-// Lists the rows with a loss; writes the zero loss and lse of the others and the
-// zero rows of dx.
+// Lists the rows with a loss; writes the zero loss and lse of the others.
 int list_live_rows(const LinearCe &p, const LiveRows &live, cudaStream_t stream);
 
 // Tensor-core path (any sizes).

@@ -100,6 +100,9 @@ struct PackArgs {
     const float *dloss;       // its largest magnitude too; null: none
     int *dloss_amax;
     const int *dloss_count;
+    float *dx;                // its rows without a loss become zero; null: not wanted
+    int64_t dx_rs, dx_cs;
+    int dx_vec;
 };
 
 __device__ __forceinline__ void keep_max(float v, int *to) {
@@ -128,8 +131,8 @@ __device__ __forceinline__ const float *source_row(const PackSource &s, int64_t 
     return s.p + (s.map != nullptr ? s.map[r] : r) * s.rs;
 }
 
-// Largest finite magnitudes of x (rows with a loss), weight and dloss.  Each warp
-// takes rows in turn, four 16-byte loads in flight a lane.
+// Largest finite magnitudes of x (rows with a loss), weight and dloss, and the zero rows of
+// dx.  Each warp takes rows in turn, four 16-byte loads in flight a lane, or sixteen of 4.
 __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
@@ -160,11 +163,38 @@ __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
                 m1 = fmaxf(m1, fmaxf(finite_abs(v.z), finite_abs(v.w)));
             }
         } else {
-#pragma unroll 4
-            for (int64_t c = lane; c < s.cols; c += 32) m0 = fmaxf(m0, finite_abs(__ldg(src + c * s.cs)));
+            int64_t c = lane;
+            for (; c + 480 < s.cols; c += 512) {
+                float v[16];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) v[u] = __ldg(src + (c + 32 * u) * s.cs);
+#pragma unroll
+                for (int u = 0; u < 16; u += 2) {
+                    m0 = fmaxf(m0, finite_abs(v[u]));
+                    m1 = fmaxf(m1, finite_abs(v[u + 1]));
+                }
+            }
+            float v[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v[u] = c + 32 * u < s.cols ? __ldg(src + (c + 32 * u) * s.cs) : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 16; ++u) m0 = fmaxf(m0, finite_abs(v[u]));
         }
     }
     keep_max(fmaxf(m0, m1), s.amax);
+    if (a.dx != nullptr) {
+        const PackSource &x = a.s[0];
+        const int64_t dead = x.rows - source_rows(x);
+        const int64_t warp = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+        for (int64_t i = warp; i < dead; i += static_cast<int64_t>(gridDim.x) * 8) {
+            float *to = a.dx + x.map[x.rows - 1 - i] * a.dx_rs;
+            if (a.dx_vec) {
+                for (int64_t c = lane; c < x.cols / 4; c += 32) reinterpret_cast<float4 *>(to)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            } else {
+                for (int64_t c = lane; c < x.cols; c += 32) to[c * a.dx_cs] = 0.0f;
+            }
+        }
+    }
     if (a.dloss != nullptr && blockIdx.x == 0) {
         float m = 0.0f;
         for (int i = threadIdx.x; i < *a.dloss_count; i += 256) m = fmaxf(m, finite_abs(a.dloss[i]));
@@ -800,9 +830,9 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
             lse[j] = d[j] = 0.0f;
             t[j] = -1;
             if (r < live) {
-                if (in) z[j] = *reinterpret_cast<const float4 *>(a.z + r * a.pitch + c);
+                if (in) z[j] = __ldcs(reinterpret_cast<const float4 *>(a.z + r * a.pitch + c));
                 lse[j] = a.lse_live[r];
-                d[j] = a.dloss[a.first + r];
+                d[j] = a.dloss[a.first + r] * f0 * f1;  // scaled by a power of two, exactly
                 t[j] = a.target[a.first + r];
             }
         }
@@ -810,13 +840,16 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t r = r0 + (j0 + j) * 8 + warp;
-            float g[4] = {z[j].x, z[j].y, z[j].z, z[j].w};
+            float g[4] = {z[j].x - lse[j], z[j].y - lse[j], z[j].z - lse[j], z[j].w - lse[j]};
             __half h[4], l[4];
+            const int hot = t[j] - static_cast<int>(c);
+            float at_hot = 0.0f;
+            if (hot >= 0 && hot < 4) at_hot = d[j] * expm1f(hot == 0 ? g[0] : hot == 1 ? g[1] : hot == 2 ? g[2] : g[3]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float x = g[k] - lse[j];
-                g[k] = c + k < a.V && r < live ? d[j] * (c + k == t[j] ? expm1f(x) : expf(x)) : 0.0f;
-                split_pair(g[k] * f0 * f1, h[k], l[k]);
+                g[k] = hot == k ? at_hot : d[j] * expf(g[k]);
+                if (c + k >= a.V || r >= live) g[k] = 0.0f;
+                split_pair(g[k], h[k], l[k]);
             }
             column.x += g[0];
             column.y += g[1];
@@ -840,16 +873,25 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
         column.z += sums[w][lane].z;
         column.w += sums[w][lane].w;
     }
-    *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) = column;
+    const float u0 = power_of_two(-(e / 2)), u1 = power_of_two(-(e - e / 2));
+    *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) =
+        make_float4(column.x * u0 * u1, column.y * u0 * u1, column.z * u0 * u1, column.w * u0 * u1);
 }
 
+// A CTA takes 32 columns; its eight warps take the row blocks in turn.
 __global__ void __launch_bounds__(256) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
-    const int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (v >= a.V) return;
+    __shared__ float sums[8][32];
+    const int64_t v = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
     const int blocks = static_cast<int>((live_extent(a.live, a.first, a.rows) + kGradRows - 1) / kGradRows);
     float sum = 0.0f;
+    if (v < a.V) {
 #pragma unroll 8
-    for (int b = 0; b < blocks; ++b) sum += a.column_parts[b * a.pitch + v];
+        for (int b = threadIdx.x / 32; b < blocks; b += 8) sum += a.column_parts[b * a.pitch + v];
+    }
+    sums[threadIdx.x / 32][threadIdx.x % 32] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 32 || v >= a.V) return;
+    for (int w = 1; w < 8; ++w) sum += sums[w][threadIdx.x];
     db[v * db_s] = add ? db[v * db_s] + sum : sum;
 }
 
@@ -911,11 +953,12 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const int64_t pitch = v_blocks * kBlock;
     const int tiles_v = static_cast<int>((p.V + kTileCols - 1) / kTileCols);
     const int tiles_d = static_cast<int>((p.D + kTileCols - 1) / kTileCols);
-    // rows at a time: the logits of a piece fill at most 2 GiB; without gradients only
+    // rows at a time: the logits of a piece fill at most 4 GiB (a piece more reads and writes
+    // dweight once more); without gradients only
     // their statistics are kept, 8 bytes for 128 logits
     const int64_t rows_all = (p.N + 255) / 256 * 256;
     const int64_t row_bytes = grads ? pitch * 4 : static_cast<int64_t>(tiles_v) * 16;
-    int64_t piece = (int64_t{2} << 30) / row_bytes / 256 * 256;
+    int64_t piece = (int64_t{4} << 30) / row_bytes / 256 * 256;
     if (piece < 256) piece = 256;
     if (piece > (int64_t{1} << 21)) piece = int64_t{1} << 21;  // k_softmax_grad's grid
     const int64_t pieces = (rows_all + piece - 1) / piece;
@@ -964,6 +1007,10 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     k.s[1] = PackSource{p.w, p.w_rs, p.w_cs, p.V, p.D, nullptr, nullptr, vector_source(p.w, p.w_rs, p.w_cs, p.D),
                         wp, p.V, live.count + 2};
     if (grads) k.dloss = live.dloss;
+    if (p.dx != nullptr && p.D > 0) k.dx = p.dx;
+    k.dx_rs = p.dx_rs;
+    k.dx_cs = p.dx_cs;
+    k.dx_vec = vector_source(p.dx, p.dx_rs, p.dx_cs, p.D);
     k.dloss_amax = live.count + 3;
     k.dloss_count = live.count;
     // CTAs in proportion to the tensors' rows, eight to an SM in all
@@ -1019,7 +1066,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         k_softmax_grad<<<grid, 256, 0, stream>>>(ga);
         MTC_TRY(check_launch("linear cross entropy (gradient of the logits)"));
         if (p.db != nullptr) {
-            k_bias_grad<<<static_cast<unsigned>((p.V + 255) / 256), 256, 0, stream>>>(ga, p.db, p.db_s, first > 0);
+            k_bias_grad<<<static_cast<unsigned>((p.V + 31) / 32), 256, 0, stream>>>(ga, p.db, p.db_s, first > 0);
             MTC_TRY(check_launch("linear cross entropy (bias gradient)"));
         }
         const __half *gp = reinterpret_cast<const __half *>(z);
