@@ -109,14 +109,14 @@ def contiguous_strides(shape: Sequence[int]) -> list[int]:
 class View:
     """A strided view of a flat storage tensor (torch tensor, on any device)."""
 
-    __slots__ = ("_storage", "_tensor", "shape", "strides", "offset")
+    __slots__ = ("_tensor", "_storage", "_shape", "_strides", "_offset")
 
     def __init__(self, storage, shape: tuple, strides: tuple, offset: int = 0):
-        self._storage = storage  # torch.Tensor, 1-D
         self._tensor = None
-        self.shape = shape
-        self.strides = strides
-        self.offset = offset
+        self._storage = storage  # torch.Tensor, 1-D
+        self._shape = shape
+        self._strides = strides
+        self._offset = offset
 
     def __repr__(self) -> str:
         return f"View(shape={self.shape}, strides={self.strides}, offset={self.offset}, storage={self.storage!r})"
@@ -124,7 +124,7 @@ class View:
     @staticmethod
     def of(t) -> "View":
         """View of an existing torch tensor (shares its storage)."""
-        v = View(None, t.shape, t.stride(), t.storage_offset())
+        v = _new_view(View)
         v._tensor = t
         return v
 
@@ -133,38 +133,65 @@ class View:
         return View(storage, tuple(shape), tuple(contiguous_strides(shape)), offset)
 
     @property
-    def storage(self):
-        if self._storage is None:
-            import torch
+    def shape(self) -> tuple:
+        return self._shape if self._tensor is None else tuple(self._tensor.shape)
 
-            t = self._tensor
-            self._storage = torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
-        return self._storage
+    @property
+    def strides(self) -> tuple:
+        return self._strides if self._tensor is None else self._tensor.stride()
+
+    @property
+    def offset(self) -> int:
+        return self._offset if self._tensor is None else self._tensor.storage_offset()
+
+    @property
+    def storage(self):
+        if self._tensor is None:
+            return self._storage
+        import torch
+
+        t = self._tensor
+        return torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
 
     def desc(self) -> Desc:
         return Desc.from_buffer_copy(self.packed())
 
     def packed(self) -> bytes:
-        """The view's descriptor as the bytes of an mtc_desc."""
-        t = self._storage if self._tensor is None else self._tensor
+        """The view's descriptor as the bytes of an mtc_desc, in one pack: a call of small
+        tensors costs what its descriptors do."""
+        t = self._tensor
+        if t is not None:
+            dtype = _DTYPES.get(t.dtype)
+            if dtype is None:
+                dtype = _dtype_code(t.dtype)
+            shape = t.shape
+            rank = len(shape)
+            if rank > MAX_RANK:
+                raise ValueError("shape/strides rank mismatch or rank > 8")
+            pad = _PAD[rank]
+            if t.is_contiguous():  # its own elements are all that the view reaches
+                return _DESC.pack(t.data_ptr(), 0, t.numel(), dtype, rank, *shape, *pad, *t.stride(), *pad)
+            s = t.untyped_storage()
+            return _DESC.pack(s.data_ptr(), t.storage_offset(), s.nbytes() // (8 if dtype == INT64 else 4), dtype, rank,
+                              *shape, *pad, *t.stride(), *pad)
+        t = self._storage
         dtype = _DTYPES.get(t.dtype)
         if dtype is None:
             dtype = _dtype_code(t.dtype)
-        rank = len(self.shape)
-        if rank != len(self.strides) or rank > MAX_RANK:
+        rank = len(self._shape)
+        if rank != len(self._strides) or rank > MAX_RANK:
             raise ValueError("shape/strides rank mismatch or rank > 8")
-        if self._tensor is None:
-            ptr, capacity = t.data_ptr(), t.numel()
-        else:
-            s = t.untyped_storage()
-            ptr, capacity = s.data_ptr(), s.nbytes() // (8 if dtype == INT64 else 4)
         pad = _PAD[rank]
-        # one pack of the whole structure: a call of small tensors costs what its descriptors do
-        return _DESC.pack(ptr, self.offset, capacity, dtype, rank, *self.shape, *pad, *self.strides, *pad)
+        return _DESC.pack(t.data_ptr(), self._offset, t.numel(), dtype, rank, *self._shape, *pad, *self._strides, *pad)
 
     def tensor(self):
         """The same view as a torch tensor (for zero/positive strides)."""
+        if self._tensor is not None:
+            return self._tensor
         return self.storage.as_strided(self.shape, self.strides, self.offset)
+
+
+_new_view = object.__new__
 
 
 class MtcError(RuntimeError):
@@ -300,7 +327,9 @@ def _stream(stream):
         import torch
 
         # the handle alone: a Stream object costs more than a small call's launch
-        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        if not torch.cuda.is_initialized():
+            torch.cuda.init()
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     return ctypes.c_void_p(int(stream))
 
 

@@ -461,6 +461,7 @@ struct SumArgs {
     unsigned int *arrived;   // [pieces][slabs] partial rows written of the run that begins in the piece
     float scale;
     int accumulate;
+    int flat;                // the table's rows are contiguous and back to back, at an odd width
 };
 
 template <int VEC>
@@ -475,6 +476,10 @@ __device__ __forceinline__ Row<VEC> load_row(const float *p) {
         const float4 x = *reinterpret_cast<const float4 *>(p);
         r.v[3 % VEC] = x.w;
         r.v[2 % VEC] = x.z;
+        r.v[1 % VEC] = x.y;
+        r.v[0] = x.x;
+    } else if (VEC == 2) {
+        const float2 x = *reinterpret_cast<const float2 *>(p);
         r.v[1 % VEC] = x.y;
         r.v[0] = x.x;
     } else {
@@ -493,6 +498,10 @@ __device__ __forceinline__ Row<VEC> load_shared_row(const float *p) {
         r.v[2 % VEC] = x.z;
         r.v[1 % VEC] = x.y;
         r.v[0] = x.x;
+    } else if (VEC == 2) {
+        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
+        r.v[1 % VEC] = x.y;
+        r.v[0] = x.x;
     } else {
         r.v[0] = __ldcg(p);
     }
@@ -502,6 +511,7 @@ __device__ __forceinline__ Row<VEC> load_shared_row(const float *p) {
 template <int VEC>
 __device__ __forceinline__ void store_row(float *p, const Row<VEC> &r) {
     if (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(r.v[0], r.v[1 % VEC], r.v[2 % VEC], r.v[3 % VEC]);
+    else if (VEC == 2) *reinterpret_cast<float2 *>(p) = make_float2(r.v[0], r.v[1 % VEC]);
     else *p = r.v[0];
 }
 
@@ -515,6 +525,41 @@ __device__ __forceinline__ void finish_row(const SumArgs &a, float *p, Row<VEC> 
         for (int j = 0; j < VEC; ++j) r.v[j] += old.v[j];
     }
     store_row<VEC>(p, r);
+}
+
+// Clears those of the table's rows v0 .. v0 + 31 that `has` has no bit for: this CTA's slab of
+// their columns, or, where the rows lie back to back at an odd width, its share of the whole
+// in 16-byte pieces.
+template <int VEC>
+__device__ __forceinline__ void clear_rows(const SumArgs &a, long long v0, unsigned int has, unsigned int slab) {
+    const int rows = static_cast<int>(a.vocab - v0 < kZeroRows ? a.vocab - v0 : kZeroRows);
+    if (a.flat) {
+        float *base = a.dtable + v0 * a.table_rs;
+        const unsigned int total = static_cast<unsigned int>(rows * a.dim), dim = static_cast<unsigned int>(a.dim);
+        const unsigned int head = static_cast<unsigned int>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) / 4) & 3;
+        auto clear = [&](unsigned int e) {
+            if (e < total && !(has >> (e / dim) & 1)) base[e] = 0.0f;
+        };
+        if (slab == 0 && threadIdx.x < head) clear(threadIdx.x);
+        for (unsigned int e = head + 4 * (slab * blockDim.x + threadIdx.x); e < total; e += 4 * a.slabs * blockDim.x) {
+            const unsigned int r0 = e / dim, r1 = (e + 3) / dim;
+            if (e + 3 < total && !(has >> r0 & 1) && !(has >> r1 & 1) && r1 <= r0 + 1) {
+                *reinterpret_cast<float4 *>(base + e) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            } else {
+                for (int j = 0; j < 4; ++j) clear(e + j);
+            }
+        }
+        return;
+    }
+    const long long col = (static_cast<long long>(slab) * blockDim.x + threadIdx.x) * VEC;
+    if (col >= a.dim) return;
+    Row<VEC> zero;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) zero.v[j] = 0.0f;
+    float *to = a.dtable + v0 * a.table_rs + col * a.table_cs;
+#pragma unroll 8
+    for (int r = 0; r < kZeroRows; ++r)
+        if (r < rows && !(has >> r & 1)) store_row<VEC>(to + r * a.table_rs, zero);
 }
 
 // Called by every piece that holds a part of a run of several pieces, once its partial
@@ -582,20 +627,12 @@ __device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsig
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
     const unsigned int unit = blockIdx.x / a.slabs;
-    const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * kThreads + threadIdx.x) * VEC;
+    const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * blockDim.x + threadIdx.x) * VEC;
     if (unit >= a.pieces) {
         // rows without a position
         const unsigned int group = unit - a.pieces;
-        const long long v0 = static_cast<long long>(group) * kZeroRows;
-        const unsigned int has = a.n > 0 ? a.present[group] : 0;
-        if (col >= a.dim) return;
-        Row<VEC> zero;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) zero.v[j] = 0.0f;
-        float *to = a.dtable + v0 * a.table_rs + col * a.table_cs;
-#pragma unroll 8
-        for (int r = 0; r < kZeroRows; ++r)
-            if (v0 + r < a.vocab && !(has >> r & 1)) store_row<VEC>(to + r * a.table_rs, zero);
+        clear_rows<VEC>(a, static_cast<long long>(group) * kZeroRows, a.n > 0 ? a.present[group] : 0,
+                        blockIdx.x - unit * a.slabs);
         return;
     }
     __shared__ unsigned int key[kRun + 2];   // with the neighbours' last and first
@@ -650,6 +687,73 @@ __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
     if (goes_on && !(comes_in && one_run)) join_run<VEC>(a, key[count], unit, true, col, in);
 }
 
+// Up to 256 positions need no sort: every CTA reads all tokens, the one of a token's first
+// position adds the rows of all its positions, and the CTAs of the table's rows see which of
+// them have none.  One launch instead of two.
+constexpr int kFewPositions = kThreads;
+
+template <int VEC>
+__global__ void __launch_bounds__(kThreads) k_token_few(const SumArgs a, long long padding, unsigned long long *err) {
+    __shared__ unsigned int key[kFewPositions];
+    __shared__ long long row[kFewPositions];
+    __shared__ unsigned short list[kFewPositions];
+    __shared__ int before[kThreads / 32 + 1];
+    __shared__ unsigned int has;
+    const unsigned int unit = blockIdx.x / a.slabs;
+    const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * kThreads + threadIdx.x) * VEC;
+    const unsigned int i = threadIdx.x;
+    key[i] = 0xFFFFFFFFu;
+    if (i == 0) has = 0;
+    if (i < a.n) {
+        long long r;
+        const long long t = token_at(a.pos, i, r);
+        if (t != padding && t >= 0 && t < a.vocab) key[i] = static_cast<unsigned int>(t);
+        else if (t != padding && blockIdx.x == 0) report_index(err, t);
+        row[i] = r;
+    }
+    __syncthreads();
+    if (unit >= a.n) {
+        const long long v0 = static_cast<long long>(unit - a.n) * kZeroRows;
+        if (key[i] >= v0 && key[i] < v0 + kZeroRows) atomicOr(&has, 1u << (key[i] - v0));
+        __syncthreads();
+        clear_rows<VEC>(a, v0, has, blockIdx.x - unit * a.slabs);
+        return;
+    }
+    const unsigned int k = key[unit];
+    if (k == 0xFFFFFFFFu) return;
+    if (__syncthreads_or(i < unit && key[i] == k)) return;
+    const unsigned int same = __ballot_sync(0xFFFFFFFFu, key[i] == k);
+    if (i % 32 == 0) before[i / 32 + 1] = __popc(same);
+    if (i == 0) before[0] = 0;
+    __syncthreads();
+    int first = 0, count = 0;
+#pragma unroll
+    for (int w = 1; w <= kThreads / 32; ++w) {
+        if (w <= static_cast<int>(i / 32)) first += before[w];
+        count += before[w];
+    }
+    if (key[i] == k) list[first + __popc(same & ((1u << (i % 32)) - 1))] = static_cast<unsigned short>(i);
+    __syncthreads();
+    if (col >= a.dim) return;
+    const float *src = a.dout + col * a.dout_cs;
+    Row<VEC> sum;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
+    for (int i0 = 0; i0 < count; i0 += 8) {
+        Row<VEC> x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u < count) x[u] = load_row<VEC>(src + row[list[i0 + u]]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u < count) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
+            }
+    }
+    finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
+}
+
 // ------------------------------------------------------------------- host --
 
 // Checks tokens against rows [tokens.shape + [D]] and a table [V, D], and folds
@@ -687,11 +791,12 @@ int positions(const mtc_desc &table, const mtc_desc &tokens, const mtc_desc &row
     return MTC_OK;
 }
 
-// Whether the columns of a row can be moved four at a time: contiguous, a
-// multiple of four, every row on a 16-byte boundary.
-bool vector_rows(const float *base, int64_t dim, int64_t col_stride, const long long *row_strides, int n_strides) {
-    bool ok = aligned16(base) && dim % 4 == 0 && col_stride == 1;
-    for (int i = 0; i < n_strides && ok; ++i) ok = row_strides[i] % 4 == 0;
+// Whether the columns of a row can be moved `vec` at a time: contiguous, a
+// multiple of it, every row on a boundary of it.
+bool vector_rows(int vec, const float *base, int64_t dim, int64_t col_stride, const long long *row_strides,
+                 int n_strides) {
+    bool ok = reinterpret_cast<uintptr_t>(base) % (4 * vec) == 0 && dim % vec == 0 && col_stride == 1;
+    for (int i = 0; i < n_strides && ok; ++i) ok = row_strides[i] % vec == 0;
     return ok;
 }
 
@@ -716,8 +821,8 @@ int run_embedding(const mtc_desc *table, const mtc_desc *tokens, float scale, in
     a.scale = scale;
     MTC_TRY(device_error_word(&a.err));
     const long long table_rs = a.table_rs;
-    const bool vec = vector_rows(a.table, dim, a.table_cs, &table_rs, 1) &&
-                     vector_rows(a.out, dim, a.out_cs, a.pos.row_stride, a.pos.rank);
+    const bool vec = vector_rows(4, a.table, dim, a.table_cs, &table_rs, 1) &&
+                     vector_rows(4, a.out, dim, a.out_cs, a.pos.row_stride, a.pos.rank);
     a.vectors = vec ? dim / 4 : dim;
     while (a.lanes_log2 < 5 && (int64_t{kLookupLoads} << a.lanes_log2) < a.vectors) ++a.lanes_log2;
     const int64_t segment = int64_t{kLookupLoads} << a.lanes_log2;
@@ -829,15 +934,32 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
     a.scale = scale;
     a.accumulate = accumulate != 0;
     const long long table_rs = a.table_rs;
-    const bool vec = vector_rows(a.dtable, a.dim, a.table_cs, &table_rs, 1) &&
-                     (a.n == 0 || vector_rows(a.dout, a.dim, a.dout_cs, a.pos.row_stride, a.pos.rank));
-    const int64_t slab = kThreads * (vec ? 4 : 1);
+    auto fits = [&](int v) {
+        return vector_rows(v, a.dtable, a.dim, a.table_cs, &table_rs, 1) &&
+               (a.n == 0 || vector_rows(v, a.dout, a.dim, a.dout_cs, a.pos.row_stride, a.pos.rank));
+    };
+    const int vec = fits(4) ? 4 : fits(2) ? 2 : 1;
+    // narrow rows take smaller CTAs (of two warps at least), so that their threads have columns
+    const bool few = a.n > 0 && a.n <= kFewPositions;
+    const int64_t lanes = (a.dim / vec + 31) / 32 * 32;
+    const int threads = few || lanes > kThreads ? kThreads : lanes < 64 ? 64 : static_cast<int>(lanes);
+    const int64_t slab = static_cast<int64_t>(threads) * vec;
     a.slabs = static_cast<unsigned int>((a.dim + slab - 1) / slab);
+    a.flat = vec < 4 && a.table_cs == 1 && a.table_rs == a.dim && a.dim < (int64_t{1} << 26);
     const int64_t zero_units = accumulate ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
-    if ((zero_units + a.pieces) * static_cast<int64_t>(a.slabs) > INT32_MAX)
+    if ((zero_units + a.pieces + kFewPositions) * static_cast<int64_t>(a.slabs) > INT32_MAX)
         return fail(MTC_ERR_UNSUPPORTED, "the embedding gradient is too large for one launch");
     a.zero_units = static_cast<unsigned int>(zero_units);
     if (a.pieces + a.zero_units == 0) return MTC_OK;
+    if (few) {
+        unsigned long long *err = nullptr;
+        MTC_TRY(device_error_word(&err));
+        const unsigned int ctas = (a.n + a.zero_units) * a.slabs;
+        if (vec == 4) k_token_few<4><<<ctas, kThreads, 0, stream>>>(a, padding, err);
+        else if (vec == 2) k_token_few<2><<<ctas, kThreads, 0, stream>>>(a, padding, err);
+        else k_token_few<1><<<ctas, kThreads, 0, stream>>>(a, padding, err);
+        return check_launch("embedding gradient (few positions)");
+    }
     const size_t list = padded(2 * static_cast<size_t>(a.n) * sizeof(uint2));
     const size_t tiles = (static_cast<size_t>(a.n) + kTile - 1) / kTile;
     const size_t counts = padded(tiles * kMaxBins * sizeof(unsigned int));
@@ -858,8 +980,9 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
         MTC_TRY(sort_positions(a, padding, buffers, c, b, rows, stream));
     }
     const unsigned int grid = (a.pieces + a.zero_units) * a.slabs;
-    if (vec) k_token_sums<4><<<grid, kThreads, 0, stream>>>(a);
-    else k_token_sums<1><<<grid, kThreads, 0, stream>>>(a);
+    if (vec == 4) k_token_sums<4><<<grid, threads, 0, stream>>>(a);
+    else if (vec == 2) k_token_sums<2><<<grid, threads, 0, stream>>>(a);
+    else k_token_sums<1><<<grid, threads, 0, stream>>>(a);
     return check_launch("embedding gradient (sums)");
 }
 

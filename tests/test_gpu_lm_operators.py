@@ -60,7 +60,7 @@ def make_tokens(n, vocab, seed, hot=0.3):
     return t.cuda()
 
 
-EMB_SHAPES = [(1, 5, 1), (1, 1, 7), (7, 3, 4), (33, 10, 64), (257, 100, 65), (1000, 999, 128), (4097, 50, 36),
+EMB_SHAPES = [(1, 5, 1), (1, 1, 7), (7, 3, 4), (33, 10, 64), (256, 30, 48), (257, 100, 65), (300, 77, 30), (60, 500, 142), (1000, 999, 128), (4097, 50, 36),
               (5000, 70001, 20), (9000, 2000, 1100), (65536, 1000, 8), (70001, 3000, 16), (200003, 300000, 5)]
 
 
@@ -701,9 +701,11 @@ def test_a_foreign_capture_is_refused(cuda):
     graph = torch.cuda.CUDAGraph()
     views = [view(v) for v in (x, w, t, loss, grad, out, norm)]
     dl = view(dloss)
+    many, repeated = view(x.repeat(20, 1)), view(t.repeat(20))  # few positions need no workspace
+    torch.cuda.synchronize()
     with torch.cuda.graph(graph, capture_error_mode="relaxed"):
         for call in (lambda: abi.linear_cross_entropy_grad(views[0], views[1], views[2], dl, dweight=views[4]),
-                     lambda: abi.embedding_grad(views[0], views[2], views[4]),
+                     lambda: abi.embedding_grad(many, repeated, views[4]),
                      lambda: abi.global_norm([views[1]], views[6]),
                      lambda: abi.clip_global_norm([views[1]], 1.0)):
             with pytest.raises(abi.MtcError, match="mtc_capture_begin"):
