@@ -464,73 +464,91 @@ struct SumArgs {
     int flat;                // the table's rows are contiguous and back to back, at an odd width
 };
 
-template <int VEC>
-struct Row {
+// A thread's columns of a row: VEC neighbouring ones moved at once, or, SPREAD, four that
+// lie a CTA's width apart, for rows whose width, strides or address allow no vectors.
+template <int VEC, bool SPREAD>
+struct Columns {
     float v[VEC];
 };
 
-template <int VEC>
-__device__ __forceinline__ Row<VEC> load_row(const float *p) {
-    Row<VEC> r;
-    if (VEC == 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(p);
-        r.v[3 % VEC] = x.w;
-        r.v[2 % VEC] = x.z;
-        r.v[1 % VEC] = x.y;
-        r.v[0] = x.x;
-    } else if (VEC == 2) {
-        const float2 x = *reinterpret_cast<const float2 *>(p);
-        r.v[1 % VEC] = x.y;
-        r.v[0] = x.x;
-    } else {
-        r.v[0] = *p;
+template <int VEC, bool SPREAD>
+struct Place {
+    using Values = Columns<VEC, SPREAD>;
+    long long col;
+    int count;  // columns that the row has; 0: none
+
+    __device__ __forceinline__ Place(unsigned int slab, long long dim) {
+        const long long first = static_cast<long long>(slab) * blockDim.x * VEC;
+        if (SPREAD) {
+            col = first + threadIdx.x;
+            const long long left = dim - col + blockDim.x - 1;
+            count = left <= 0 ? 0 : left / blockDim.x < VEC ? static_cast<int>(left / blockDim.x) : VEC;
+        } else {
+            col = first + static_cast<long long>(threadIdx.x) * VEC;
+            count = col < dim ? VEC : 0;
+        }
     }
-    return r;
-}
-
-// A row that another CTA has written: past this SM's L1.
-template <int VEC>
-__device__ __forceinline__ Row<VEC> load_shared_row(const float *p) {
-    Row<VEC> r;
-    if (VEC == 4) {
-        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
-        r.v[3 % VEC] = x.w;
-        r.v[2 % VEC] = x.z;
-        r.v[1 % VEC] = x.y;
-        r.v[0] = x.x;
-    } else if (VEC == 2) {
-        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
-        r.v[1 % VEC] = x.y;
-        r.v[0] = x.x;
-    } else {
-        r.v[0] = __ldcg(p);
-    }
-    return r;
-}
-
-template <int VEC>
-__device__ __forceinline__ void store_row(float *p, const Row<VEC> &r) {
-    if (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(r.v[0], r.v[1 % VEC], r.v[2 % VEC], r.v[3 % VEC]);
-    else if (VEC == 2) *reinterpret_cast<float2 *>(p) = make_float2(r.v[0], r.v[1 % VEC]);
-    else *p = r.v[0];
-}
-
-template <int VEC>
-__device__ __forceinline__ void finish_row(const SumArgs &a, float *p, Row<VEC> r) {
+    __device__ __forceinline__ Values zero() const {
+        Values r;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) r.v[j] *= a.scale;
-    if (a.accumulate) {
-        const Row<VEC> old = load_row<VEC>(p);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) r.v[j] += old.v[j];
+        for (int j = 0; j < VEC; ++j) r.v[j] = 0.0f;
+        return r;
     }
-    store_row<VEC>(p, r);
-}
+    template <bool SHARED = false>  // SHARED: another CTA has written it, past this SM's L1
+    __device__ __forceinline__ Values load(const float *row, long long cs) const {
+        Values r = zero();
+        const float *p = row + col * cs;
+        if (SPREAD) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (j < count) r.v[j] = SHARED ? __ldcg(p + j * static_cast<long long>(blockDim.x) * cs)
+                                               : p[j * static_cast<long long>(blockDim.x) * cs];
+        } else if (count > 0) {
+            if (VEC == 4) {
+                const float4 *q = reinterpret_cast<const float4 *>(p);
+                const float4 x = SHARED ? __ldcg(q) : *q;
+                r.v[3 % VEC] = x.w;
+                r.v[2 % VEC] = x.z;
+                r.v[1] = x.y;
+                r.v[0] = x.x;
+            } else {
+                const float2 *q = reinterpret_cast<const float2 *>(p);
+                const float2 x = SHARED ? __ldcg(q) : *q;
+                r.v[1] = x.y;
+                r.v[0] = x.x;
+            }
+        }
+        return r;
+    }
+    __device__ __forceinline__ void store(float *row, long long cs, const Values &r) const {
+        float *p = row + col * cs;
+        if (SPREAD) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (j < count) p[j * static_cast<long long>(blockDim.x) * cs] = r.v[j];
+        } else if (count > 0) {
+            if (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(r.v[0], r.v[1], r.v[2 % VEC], r.v[3 % VEC]);
+            else *reinterpret_cast<float2 *>(p) = make_float2(r.v[0], r.v[1]);
+        }
+    }
+    // scale * sum into a row of the table
+    __device__ __forceinline__ void finish(const SumArgs &a, unsigned int k, Values r) const {
+        float *row = a.dtable + k * a.table_rs;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) r.v[j] *= a.scale;
+        if (a.accumulate) add(r, load(row, a.table_cs));
+        store(row, a.table_cs, r);
+    }
+    static __device__ __forceinline__ void add(Values &a, const Values &b) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a.v[j] += b.v[j];
+    }
+};
 
 // Clears those of the table's rows v0 .. v0 + 31 that `has` has no bit for: this CTA's slab of
 // their columns, or, where the rows lie back to back at an odd width, its share of the whole
 // in 16-byte pieces.
-template <int VEC>
+template <class P>
 __device__ __forceinline__ void clear_rows(const SumArgs &a, long long v0, unsigned int has, unsigned int slab) {
     const int rows = static_cast<int>(a.vocab - v0 < kZeroRows ? a.vocab - v0 : kZeroRows);
     if (a.flat) {
@@ -551,24 +569,19 @@ __device__ __forceinline__ void clear_rows(const SumArgs &a, long long v0, unsig
         }
         return;
     }
-    const long long col = (static_cast<long long>(slab) * blockDim.x + threadIdx.x) * VEC;
-    if (col >= a.dim) return;
-    Row<VEC> zero;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) zero.v[j] = 0.0f;
-    float *to = a.dtable + v0 * a.table_rs + col * a.table_cs;
+    const P at(slab, a.dim);
+    float *to = a.dtable + v0 * a.table_rs;
 #pragma unroll 8
     for (int r = 0; r < kZeroRows; ++r)
-        if (r < rows && !(has >> r & 1)) store_row<VEC>(to + r * a.table_rs, zero);
+        if (r < rows && !(has >> r & 1)) at.store(to + r * a.table_rs, a.table_cs, at.zero());
 }
 
 // Called by every piece that holds a part of a run of several pieces, once its partial
 // row is written: the last of them adds the partial rows, in the order of the pieces,
 // eight loads ahead.  `k`: the run's key; `on`: it goes on behind this piece.  One warp
 // finds the run's first piece, another its last, 32 pieces a step.
-template <int VEC>
-__device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsigned int unit, bool on, long long col,
-                                         bool in) {
+template <class P>
+__device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsigned int unit, bool on, const P &at) {
     __shared__ unsigned int range[2];
     __shared__ bool last_here;
     __threadfence();
@@ -605,33 +618,27 @@ __device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsig
     __syncthreads();
     if (!last_here) return;
     __threadfence();
-    if (!in) return;
-    Row<VEC> sum;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
+    typename P::Values sum = at.zero();
     for (unsigned int p0 = begin; p0 <= end; p0 += 8) {
-        Row<VEC> x[8];
+        typename P::Values x[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (p0 + u <= end) x[u] = load_shared_row<VEC>(a.partial + (2ll * (p0 + u) + (p0 + u == begin)) * a.dim + col);
+            if (p0 + u <= end)
+                x[u] = at.template load<true>(a.partial + (2ll * (p0 + u) + (p0 + u == begin)) * a.dim, 1);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (p0 + u <= end) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
-            }
+            if (p0 + u <= end) P::add(sum, x[u]);
     }
-    finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
+    at.finish(a, k, sum);
 }
 
-template <int VEC>
+template <class P>
 __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
     const unsigned int unit = blockIdx.x / a.slabs;
-    const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * blockDim.x + threadIdx.x) * VEC;
     if (unit >= a.pieces) {
         // rows without a position
         const unsigned int group = unit - a.pieces;
-        clear_rows<VEC>(a, static_cast<long long>(group) * kZeroRows, a.n > 0 ? a.present[group] : 0,
+        clear_rows<P>(a, static_cast<long long>(group) * kZeroRows, a.n > 0 ? a.present[group] : 0,
                         blockIdx.x - unit * a.slabs);
         return;
     }
@@ -649,42 +656,35 @@ __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
         row[threadIdx.x] = r;
     }
     __syncthreads();
-    const bool in = col < a.dim;
-    const float *src = a.dout + col * a.dout_cs;
-    Row<VEC> sum;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
+    const P at(blockIdx.x - unit * a.slabs, a.dim);
+    typename P::Values sum = at.zero();
     // positions without a gradient are the last: their keys are V
     const bool comes_in = key[0] == key[1] && key[1] < a.vocab;
     const bool goes_on = key[count + 1] == key[count] && key[count] < a.vocab;
     bool head = comes_in;
     for (int i0 = 0; i0 < count && key[1 + i0] < a.vocab; i0 += 8) {
-        Row<VEC> x[8];
+        typename P::Values x[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (in && i0 + u < count && key[1 + i0 + u] < a.vocab) x[u] = load_row<VEC>(src + row[i0 + u]);
+            if (i0 + u < count && key[1 + i0 + u] < a.vocab) x[u] = at.load(a.dout + row[i0 + u], a.dout_cs);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int i = i0 + u;
             if (i >= count || key[1 + i] >= a.vocab) break;
             const unsigned int k = key[1 + i];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
+            P::add(sum, x[u]);
             const bool on = key[2 + i] == k;
             if (on && i + 1 < count) continue;
-            if (in) {
-                if (head) store_row<VEC>(a.partial + (2ll * unit) * a.dim + col, sum);
-                else if (on) store_row<VEC>(a.partial + (2ll * unit + 1) * a.dim + col, sum);
-                else finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
-            }
+            if (head) at.store(a.partial + (2ll * unit) * a.dim, 1, sum);
+            else if (on) at.store(a.partial + (2ll * unit + 1) * a.dim, 1, sum);
+            else at.finish(a, k, sum);
             head = false;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
+            sum = at.zero();
         }
     }
     const bool one_run = key[1] == key[count];  // (of a piece that goes on as it came in, the whole is the head)
-    if (comes_in) join_run<VEC>(a, key[1], unit, one_run && goes_on, col, in);
-    if (goes_on && !(comes_in && one_run)) join_run<VEC>(a, key[count], unit, true, col, in);
+    if (comes_in) join_run(a, key[1], unit, one_run && goes_on, at);
+    if (goes_on && !(comes_in && one_run)) join_run(a, key[count], unit, true, at);
 }
 
 // Up to 256 positions need no sort: every CTA reads all tokens, the one of a token's first
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
 // them have none.  One launch instead of two.
 constexpr int kFewPositions = kThreads;
 
-template <int VEC>
+template <class P>
 __global__ void __launch_bounds__(kThreads) k_token_few(const SumArgs a, long long padding, unsigned long long *err) {
     __shared__ unsigned int key[kFewPositions];
     __shared__ long long row[kFewPositions];
@@ -700,7 +700,6 @@ __global__ void __launch_bounds__(kThreads) k_token_few(const SumArgs a, long lo
     __shared__ int before[kThreads / 32 + 1];
     __shared__ unsigned int has;
     const unsigned int unit = blockIdx.x / a.slabs;
-    const long long col = (static_cast<long long>(blockIdx.x - unit * a.slabs) * kThreads + threadIdx.x) * VEC;
     const unsigned int i = threadIdx.x;
     key[i] = 0xFFFFFFFFu;
     if (i == 0) has = 0;
@@ -716,7 +715,7 @@ __global__ void __launch_bounds__(kThreads) k_token_few(const SumArgs a, long lo
         const long long v0 = static_cast<long long>(unit - a.n) * kZeroRows;
         if (key[i] >= v0 && key[i] < v0 + kZeroRows) atomicOr(&has, 1u << (key[i] - v0));
         __syncthreads();
-        clear_rows<VEC>(a, v0, has, blockIdx.x - unit * a.slabs);
+        clear_rows<P>(a, v0, has, blockIdx.x - unit * a.slabs);
         return;
     }
     const unsigned int k = key[unit];
@@ -734,25 +733,23 @@ __global__ void __launch_bounds__(kThreads) k_token_few(const SumArgs a, long lo
     }
     if (key[i] == k) list[first + __popc(same & ((1u << (i % 32)) - 1))] = static_cast<unsigned short>(i);
     __syncthreads();
-    if (col >= a.dim) return;
-    const float *src = a.dout + col * a.dout_cs;
-    Row<VEC> sum;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.v[j] = 0.0f;
+    const P at(blockIdx.x - unit * a.slabs, a.dim);
+    typename P::Values sum = at.zero();
     for (int i0 = 0; i0 < count; i0 += 8) {
-        Row<VEC> x[8];
+        typename P::Values x[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (i0 + u < count) x[u] = load_row<VEC>(src + row[list[i0 + u]]);
+            if (i0 + u < count) x[u] = at.load(a.dout + row[list[i0 + u]], a.dout_cs);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (i0 + u < count) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) sum.v[j] += x[u].v[j];
-            }
+            if (i0 + u < count) P::add(sum, x[u]);
     }
-    finish_row<VEC>(a, a.dtable + k * a.table_rs + col * a.table_cs, sum);
+    at.finish(a, k, sum);
 }
+
+using Vectors4 = Place<4, false>;
+using Vectors2 = Place<2, false>;
+using Spread4 = Place<4, true>;
 
 // ------------------------------------------------------------------- host --
 
@@ -941,9 +938,10 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
     const int vec = fits(4) ? 4 : fits(2) ? 2 : 1;
     // narrow rows take smaller CTAs (of two warps at least), so that their threads have columns
     const bool few = a.n > 0 && a.n <= kFewPositions;
-    const int64_t lanes = (a.dim / vec + 31) / 32 * 32;
+    const int columns = vec == 2 ? 2 : 4;  // of a thread
+    const int64_t lanes = ((a.dim + columns - 1) / columns + 31) / 32 * 32;
     const int threads = few || lanes > kThreads ? kThreads : lanes < 64 ? 64 : static_cast<int>(lanes);
-    const int64_t slab = static_cast<int64_t>(threads) * vec;
+    const int64_t slab = static_cast<int64_t>(threads) * columns;
     a.slabs = static_cast<unsigned int>((a.dim + slab - 1) / slab);
     a.flat = vec < 4 && a.table_cs == 1 && a.table_rs == a.dim && a.dim < (int64_t{1} << 26);
     const int64_t zero_units = accumulate ? 0 : (a.vocab + kZeroRows - 1) / kZeroRows;
@@ -955,9 +953,9 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
         unsigned long long *err = nullptr;
         MTC_TRY(device_error_word(&err));
         const unsigned int ctas = (a.n + a.zero_units) * a.slabs;
-        if (vec == 4) k_token_few<4><<<ctas, kThreads, 0, stream>>>(a, padding, err);
-        else if (vec == 2) k_token_few<2><<<ctas, kThreads, 0, stream>>>(a, padding, err);
-        else k_token_few<1><<<ctas, kThreads, 0, stream>>>(a, padding, err);
+        if (vec == 4) k_token_few<Vectors4><<<ctas, kThreads, 0, stream>>>(a, padding, err);
+        else if (vec == 2) k_token_few<Vectors2><<<ctas, kThreads, 0, stream>>>(a, padding, err);
+        else k_token_few<Spread4><<<ctas, kThreads, 0, stream>>>(a, padding, err);
         return check_launch("embedding gradient (few positions)");
     }
     const size_t list = padded(2 * static_cast<size_t>(a.n) * sizeof(uint2));
@@ -980,9 +978,9 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
         MTC_TRY(sort_positions(a, padding, buffers, c, b, rows, stream));
     }
     const unsigned int grid = (a.pieces + a.zero_units) * a.slabs;
-    if (vec == 4) k_token_sums<4><<<grid, threads, 0, stream>>>(a);
-    else if (vec == 2) k_token_sums<2><<<grid, threads, 0, stream>>>(a);
-    else k_token_sums<1><<<grid, threads, 0, stream>>>(a);
+    if (vec == 4) k_token_sums<Vectors4><<<grid, threads, 0, stream>>>(a);
+    else if (vec == 2) k_token_sums<Vectors2><<<grid, threads, 0, stream>>>(a);
+    else k_token_sums<Spread4><<<grid, threads, 0, stream>>>(a);
     return check_launch("embedding gradient (sums)");
 }
 
