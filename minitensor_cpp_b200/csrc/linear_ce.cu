@@ -4,8 +4,8 @@
 //   g_nv = dloss_n (exp(z_nv - lse_n) - [v = t_n])
 //   dx = g W                 dW = g^T x                          db_v = sum_n g_nv
 //
-// Three paths.  Few rows (up to 16) read W once in float32, whatever its size; small
-// problems take a warp a row; the others run on the tensor cores (linear_ce_tc.cu), over
+// Small problems take a warp a row (here), few rows or few classes stream the other operand
+// past them (linear_ce_few.cu), and the rest runs on the tensor cores (linear_ce_tc.cu) over
 // the rows that have a loss: k_live_rows lists them in order, and only the device knows how
 // many there are.
 #include <cooperative_groups.h>
@@ -116,434 +116,6 @@ __global__ void __launch_bounds__(kListThreads) k_live_rows(const LinearCe p, co
     cluster.sync();  // nobody leaves while its count is read
 }
 
-// ------------------------------------------------------------ shared pieces --
-
-// A row's target, or -1 for a row without a loss; reports one outside the vocabulary.
-__device__ __forceinline__ int row_target(const LinearCe &p, int64_t n, unsigned long long *err, bool report) {
-    const int64_t t = p.targets[n * p.t_s];
-    if (t == p.ignore) return -1;
-    if (t < 0 || t >= p.V) {
-        if (report) report_index(err, t);
-        return -1;
-    }
-    return static_cast<int>(t);
-}
-
-// Running maximum and sum of exponentials relative to it.  Infinite maxima count from 0,
-// so that a row of +inf or -inf has its limit and not exp(inf - inf).
-struct Softmax {
-    float top, sum;
-};
-
-__device__ __forceinline__ float softmax_base(float top) { return isinf(top) ? 0.0f : top; }
-
-__device__ __forceinline__ Softmax merge(Softmax a, Softmax b) {
-    Softmax r;
-    r.top = fmaxf(a.top, b.top);
-    const float base = softmax_base(r.top);
-    r.sum = (a.sum != 0.0f ? a.sum * expf(softmax_base(a.top) - base) : 0.0f) +
-            (b.sum != 0.0f ? b.sum * expf(softmax_base(b.top) - base) : 0.0f);
-    return r;
-}
-
-__device__ __forceinline__ Softmax merge_lanes(Softmax s, int from, int to) {
-    for (int o = from; o < to; o <<= 1) {
-        Softmax other;
-        other.top = __shfl_xor_sync(0xFFFFFFFFu, s.top, o);
-        other.sum = __shfl_xor_sync(0xFFFFFFFFu, s.sum, o);
-        s = merge(s, other);
-    }
-    return s;
-}
-
-__device__ __forceinline__ float softmax_grad(float z, float lse, float d, bool hot) {
-    const float x = z - lse;
-    return d * (hot ? expm1f(x) : expf(x));
-}
-
-// ----------------------------------------------------------------- few rows --
-// Up to 16 rows: bound by reading W, once for the loss (131 MB of a 32000 x 1024 layer at
-// ## us) and once more, next to the writing of dW, for the gradients.  Float32 products on
-// the FMA units: at 16 rows 16 FMAs for 4 bytes of W, still less than its reading takes.
-//
-// k_few_logits: a warp takes four rows of W at a time, 128 columns a step, against all rows
-// of x in shared memory; one lane for each of its 4 N logits keeps their softmax.
-// k_few_grad: a CTA takes 128 (64) columns and a part of the vocabulary; x's columns and the
-// sums of dx stay in registers, g comes from the logits by one exponential a class and lane.
-
-constexpr int kFewRows = 16;
-constexpr int kFewThreads = 256;
-constexpr int kFewShared = 160 * 1024;
-
-struct FewArgs {
-    int vec;             // float4 loads of W
-    int d_pad;           // x's row in shared memory, a multiple of 128
-    float *z;            // [N][V], null: not wanted
-    Softmax *parts;      // [CTAs][R]
-    int n_parts;
-    float *z_target;     // [R]
-    float *dx_parts;     // [splits][N][D]
-    int splits;
-    int dw_vec;
-    unsigned long long *err;
-};
-
-// Sums over the warp of COUNT values a lane at once (COUNT a power of two up to 32): each
-// step halves the list, a lane keeping the half its number has the bit for, so that lane l
-// ends with the sum of value l % COUNT after COUNT - 1 shuffles and not 5 COUNT.
-template <int COUNT>
-__device__ __forceinline__ float warp_sums(const float *a) {
-    const int lane = threadIdx.x % 32;
-    float v[COUNT];
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) v[i] = a[i];
-    int o = 1;
-#pragma unroll
-    for (int left = COUNT / 2; left > 0; left /= 2, o *= 2) {
-#pragma unroll
-        for (int i = 0; i < left; ++i) {
-            const bool odd = (lane & o) != 0;
-            const float keep = odd ? v[2 * i + 1] : v[2 * i], give = odd ? v[2 * i] : v[2 * i + 1];
-            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
-        }
-    }
-    for (; o < 32; o *= 2) v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
-    return v[0];
-}
-
-// One step of a warp: 128 S columns of four rows of W.  Without VEC a lane's four columns
-// are 32 apart, so that a load is contiguous where W is.
-template <int S, bool VEC>
-__device__ __forceinline__ void load_step(const LinearCe &p, int64_t v0, int64_t c0, float4 (&x)[S][4]) {
-    const int lane = threadIdx.x % 32;
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float *w = p.w + (v0 + j < p.V ? v0 + j : p.V - 1) * p.w_rs;
-            x[s][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (VEC) {
-                const int64_t c = c0 + s * 128 + lane * 4;
-                if (c < p.D) x[s][j] = __ldcs(reinterpret_cast<const float4 *>(w + c));
-            } else {
-                const int64_t c = c0 + s * 128 + lane;
-                if (c < p.D) x[s][j].x = __ldcs(w + c * p.w_cs);
-                if (c + 32 < p.D) x[s][j].y = __ldcs(w + (c + 32) * p.w_cs);
-                if (c + 64 < p.D) x[s][j].z = __ldcs(w + (c + 64) * p.w_cs);
-                if (c + 96 < p.D) x[s][j].w = __ldcs(w + (c + 96) * p.w_cs);
-            }
-        }
-}
-
-// CTAs an SM holds, by registers: with one or two rows the loads in flight decide, and those
-// come from warps.
-constexpr int few_resident(int R) { return R <= 2 ? 4 : R <= 4 ? 3 : 2; }
-
-template <int R, bool VEC>
-__global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(const LinearCe p, const FewArgs a) {
-    extern __shared__ __align__(16) float xs[];  // [R][d_pad]
-    __shared__ int target[R];
-    __shared__ Softmax warps[kFewThreads / 32][R];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    constexpr int S = 1;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kFewThreads / 32) * 4;
-    int64_t v0 = (static_cast<int64_t>(blockIdx.x) * (kFewThreads / 32) + warp) * 4, c0 = 0;
-    float4 w[S][4], next[S][4];
-    if (v0 < p.V) load_step<S, VEC>(p, v0, c0, w);  // under way while x arrives
-    if (threadIdx.x < R) target[threadIdx.x] = threadIdx.x < p.N ? row_target(p, threadIdx.x, a.err, blockIdx.x == 0) : -1;
-    for (int n = 0; n < R; ++n)
-        for (int d = threadIdx.x; d < a.d_pad; d += kFewThreads)
-            xs[n * a.d_pad + d] = n < p.N && d < p.D ? p.x[n * p.x_rs + d * p.x_cs] : 0.0f;
-    __syncthreads();
-    for (int n = 0; n < R; ++n)
-        if (target[n] < 0)
-            for (int d = threadIdx.x; d < a.d_pad; d += kFewThreads) xs[n * a.d_pad + d] = 0.0f;
-    __syncthreads();
-    constexpr int kMine = (4 * R + 31) / 32;  // logits of a lane: i = lane + 32 k is row i / 4 and class i % 4
-    Softmax mine[kMine];
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) mine[k] = Softmax{-INFINITY, 0.0f};
-    float acc[4 * R];
-#pragma unroll
-    for (int i = 0; i < 4 * R; ++i) acc[i] = 0.0f;
-    while (v0 < p.V) {
-        int64_t v1 = v0, c1 = c0 + 128 * S;
-        if (c1 >= p.D) {
-            c1 = 0;
-            v1 += step;
-        }
-        if (v1 < p.V) load_step<S, VEC>(p, v1, c1, next);
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            if (c0 + s * 128 >= p.D) break;
-#pragma unroll
-            for (int n = 0; n < R; ++n) {
-                const float *row = xs + n * a.d_pad + c0 + s * 128;
-                float4 y;
-                if (VEC) y = *reinterpret_cast<const float4 *>(row + lane * 4);
-                else y = make_float4(row[lane], row[lane + 32], row[lane + 64], row[lane + 96]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float &c = acc[4 * n + j];
-                    c = fmaf(w[s][j].x, y.x, c);
-                    c = fmaf(w[s][j].y, y.y, c);
-                    c = fmaf(w[s][j].z, y.z, c);
-                    c = fmaf(w[s][j].w, y.w, c);
-                }
-            }
-        }
-        if (v1 != v0) {
-#pragma unroll
-            for (int k = 0; k < kMine; ++k) {
-                float x = warp_sums<(4 * R < 32 ? 4 * R : 32)>(acc + 32 * k);
-                const int i = lane + 32 * k, n = i / 4;
-                const int64_t v = v0 + i % 4;
-                if (n >= R || n >= p.N || v >= p.V) continue;
-                if (p.bias != nullptr) x += __ldg(p.bias + v * p.b_s);
-                if (a.z != nullptr) a.z[n * p.V + v] = x;
-                if (v == target[n]) a.z_target[n] = x;
-                mine[k] = merge(mine[k], Softmax{x, isnan(x) ? x : isinf(x) ? (x > 0.0f ? x : 0.0f) : 1.0f});
-            }
-#pragma unroll
-            for (int i = 0; i < 4 * R; ++i) acc[i] = 0.0f;
-        }
-        v0 = v1;
-        c0 = c1;
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[s][j] = next[s][j];
-    }
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-        const Softmax s = merge_lanes(mine[k], 1, 4);
-        const int i = lane + 32 * k;
-        if (i % 4 == 0 && i / 4 < R) warps[warp][i / 4] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x < R) {
-        Softmax s = warps[0][threadIdx.x];
-        for (int w = 1; w < kFewThreads / 32; ++w) s = merge(s, warps[w][threadIdx.x]);
-        a.parts[blockIdx.x * R + threadIdx.x] = s;
-    }
-}
-
-// lse of row n from the CTAs' parts; every lane of the warp gets it.
-__device__ __forceinline__ float few_lse(const FewArgs &a, int R, int n) {
-    Softmax s{-INFINITY, 0.0f};
-    const Softmax *parts = a.parts + n;
-#pragma unroll 8
-    for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) s.top = fmaxf(s.top, parts[i * R].top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s.top = fmaxf(s.top, __shfl_xor_sync(0xFFFFFFFFu, s.top, o));
-    const float base = softmax_base(s.top);
-#pragma unroll 8
-    for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) {
-        const Softmax x = parts[i * R];
-        if (x.sum != 0.0f) s.sum += x.sum * expf(softmax_base(x.top) - base);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s.sum += __shfl_xor_sync(0xFFFFFFFFu, s.sum, o);
-    return softmax_base(s.top) + logf(s.sum);
-}
-
-__device__ __forceinline__ void store_loss(const LinearCe &p, const FewArgs &a, int n, int target, float lse) {
-    if (p.loss != nullptr) p.loss[n * p.loss_s] = target < 0 ? 0.0f : lse - a.z_target[n];
-    if (p.lse != nullptr) p.lse[n * p.lse_s] = target < 0 ? 0.0f : lse;
-}
-
-__global__ void __launch_bounds__(32 * kFewRows) k_few_loss(const LinearCe p, const FewArgs a, int R) {
-    const int n = threadIdx.x / 32;
-    if (n >= p.N) return;
-    const float lse = few_lse(a, R, n);
-    if (threadIdx.x % 32 == 0) store_loss(p, a, n, row_target(p, n, a.err, false), lse);
-}
-
-// C columns a lane, 32 C a CTA.
-template <int R, int C>
-__global__ void __launch_bounds__(kFewThreads) k_few_grad(const LinearCe p, const FewArgs a) {
-    __shared__ float lse[R], dloss[R];
-    __shared__ int target[R];
-    __shared__ float sums[kFewThreads / 32][32 * C];
-    __shared__ __align__(16) float gs[kFewThreads / 32][32][R];  // a warp's 32 classes
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    for (int n = warp; n < R; n += kFewThreads / 32) {
-        const int t = n < p.N ? row_target(p, n, a.err, false) : -1;
-        const float l = n < p.N ? few_lse(a, R, n) : 0.0f;
-        if (lane == 0) {
-            lse[n] = l;
-            target[n] = t;
-            dloss[n] = t >= 0 ? p.dloss[n * p.dl_s] : 0.0f;
-            if (n < p.N && blockIdx.x == 0 && blockIdx.y == 0) store_loss(p, a, n, t, l);
-        }
-    }
-    __syncthreads();
-    const int64_t c0 = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * C;
-    const int cols = static_cast<int>(p.D - c0 < 0 ? 0 : p.D - c0 < C ? p.D - c0 : C);
-    float x[R][C], dx[R][C];
-#pragma unroll
-    for (int n = 0; n < R; ++n)
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            dx[n][c] = 0.0f;
-            x[n][c] = n < p.N && c < cols && target[n] >= 0 ? p.x[n * p.x_rs + (c0 + c) * p.x_cs] : 0.0f;
-        }
-    const int64_t step = static_cast<int64_t>(gridDim.y) * (kFewThreads / 32) * 32;
-    for (int64_t v0 = (static_cast<int64_t>(blockIdx.y) * (kFewThreads / 32) + warp) * 32; v0 < p.V; v0 += step) {
-        const int64_t v = v0 + lane;
-        float db = 0.0f;
-        __syncwarp();
-#pragma unroll
-        for (int n = 0; n < R; ++n) {
-            float g = 0.0f;
-            if (n < p.N && v < p.V && target[n] >= 0) g = softmax_grad(a.z[n * p.V + v], lse[n], dloss[n], v == target[n]);
-            gs[warp][lane][n] = g;
-            db += g;
-        }
-        __syncwarp();
-        if (p.db != nullptr && blockIdx.x == 0 && v < p.V) p.db[v * p.db_s] = db;
-        const int count = static_cast<int>(p.V - v0 < 32 ? p.V - v0 : 32);
-        constexpr int U = 8;
-        for (int j0 = 0; j0 < count; j0 += U) {
-            float w[U][C];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-#pragma unroll
-                for (int c = 0; c < C; ++c) w[u][c] = 0.0f;
-                if (p.dx == nullptr || j0 + u >= count) continue;
-                const float *src = p.w + (v0 + j0 + u) * p.w_rs + c0 * p.w_cs;
-                if (a.vec) {
-                    if (cols <= 0) continue;
-                    if (C == 4) {
-                        const float4 y = __ldcs(reinterpret_cast<const float4 *>(src));
-                        w[u][C - 1] = y.w;
-                        w[u][2 % C] = y.z;
-                        w[u][1] = y.y;
-                        w[u][0] = y.x;
-                    } else {
-                        const float2 y = __ldcs(reinterpret_cast<const float2 *>(src));
-                        w[u][0] = y.x;
-                        w[u][1] = y.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        if (c < cols) w[u][c] = __ldcs(src + c * p.w_cs);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (j0 + u >= count) break;
-                float dw[C];
-#pragma unroll
-                for (int c = 0; c < C; ++c) dw[c] = 0.0f;
-#pragma unroll
-                for (int n = 0; n < R; ++n) {
-                    const float gn = gs[warp][j0 + u][n];
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        dx[n][c] = fmaf(gn, w[u][c], dx[n][c]);
-                        dw[c] = fmaf(gn, x[n][c], dw[c]);
-                    }
-                }
-                if (p.dw == nullptr) continue;
-                float *to = p.dw + (v0 + j0 + u) * p.dw_rs + c0 * p.dw_cs;
-                if (a.dw_vec) {
-                    if (cols <= 0) continue;
-                    if (C == 4) *reinterpret_cast<float4 *>(to) = make_float4(dw[0], dw[1], dw[2 % C], dw[3 % C]);
-                    else *reinterpret_cast<float2 *>(to) = make_float2(dw[0], dw[1]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        if (c < cols) to[c * p.dw_cs] = dw[c];
-                }
-            }
-        }
-    }
-    if (p.dx == nullptr) return;
-#pragma unroll
-    for (int n = 0; n < R; ++n) {
-        if (n >= p.N) break;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < C; ++c) sums[warp][lane * C + c] = dx[n][c];
-        __syncthreads();
-        if (static_cast<int>(threadIdx.x) >= 32 * C) continue;
-        const int64_t d = static_cast<int64_t>(blockIdx.x) * 32 * C + threadIdx.x;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kFewThreads / 32; ++w) s += sums[w][threadIdx.x];
-        if (d < p.D) a.dx_parts[(blockIdx.y * p.N + n) * p.D + d] = s;
-    }
-}
-
-// Eight warps take the parts of 32 elements in turn.
-__global__ void __launch_bounds__(256) k_few_dx(const LinearCe p, const FewArgs a) {
-    __shared__ float sums[8][32];
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
-    const int64_t n = i / p.D;
-    float sum = 0.0f;
-    if (i < p.N * p.D) {
-#pragma unroll 8
-        for (int s = threadIdx.x / 32; s < a.splits; s += 8) sum += a.dx_parts[s * p.N * p.D + i];
-    }
-    sums[threadIdx.x / 32][threadIdx.x % 32] = sum;
-    __syncthreads();
-    if (threadIdx.x >= 32 || i >= p.N * p.D) return;
-    for (int w = 1; w < 8; ++w) sum += sums[w][threadIdx.x];
-    if (row_target(p, n, a.err, false) < 0) sum = 0.0f;
-    p.dx[n * p.dx_rs + (i - n * p.D) * p.dx_cs] = sum;
-}
-
-template <int R>
-int few_path(const LinearCe &p, cudaStream_t stream) {
-    const int sms = sm_count(current_device());
-    const bool grads = p.dloss != nullptr && (p.dx != nullptr || p.dw != nullptr || p.db != nullptr);
-    FewArgs a;
-    std::memset(&a, 0, sizeof(a));
-    a.vec = aligned16(p.w) && p.w_cs == 1 && p.w_rs % 4 == 0 && p.D % 4 == 0;
-    a.dw_vec = aligned16(p.dw) && p.dw_cs == 1 && p.dw_rs % 4 == 0 && p.D % 4 == 0;
-    a.d_pad = static_cast<int>((p.D + 127) / 128 * 128);
-    const size_t shared = static_cast<size_t>(R) * a.d_pad * 4;
-    const int64_t wanted = (p.V + 31) / 32;  // CTAs of 8 warps, 4 classes each
-    const int64_t most_ctas = static_cast<int64_t>(sms) * (shared > 72 * 1024 ? 1 : shared > 48 * 1024 ? 2 : few_resident(R));
-    const int64_t rounds = (wanted + most_ctas - 1) / most_ctas;  // even ones: a CTA loads x once
-    a.n_parts = static_cast<int>((wanted + rounds - 1) / rounds);
-    constexpr int C = R <= 8 ? 4 : 2;  // columns a lane of k_few_grad: 2 R C values in registers
-    const int64_t slabs = p.D > 0 ? (p.D + 32 * C - 1) / (32 * C) : 1;
-    const int64_t splits = (static_cast<int64_t>(sms) * 4 + slabs - 1) / slabs;
-    const int64_t most = (p.V + 255) / 256;  // 8 warps of 32 classes
-    a.splits = static_cast<int>(splits < most ? splits : most);
-    const size_t parts = padded(static_cast<size_t>(a.n_parts) * R * sizeof(Softmax));
-    const size_t zs = grads ? padded(static_cast<size_t>(p.N) * p.V * 4) : 0;
-    const size_t dxs = grads && p.dx != nullptr ? padded(static_cast<size_t>(a.splits) * p.N * p.D * 4) : 0;
-    Workspace ws;
-    MTC_TRY(ws.allocate(256 + parts + zs + dxs, stream));
-    a.z_target = ws.take<float>(256);
-    a.parts = ws.take<Softmax>(parts);
-    float *z = ws.take<float>(zs);
-    a.dx_parts = ws.take<float>(dxs);
-    a.z = grads ? z : nullptr;
-    MTC_TRY(device_error_word(&a.err));
-    if (a.vec) {
-        MTC_CUDA_TRY(cudaFuncSetAttribute(k_few_logits<R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared));
-        k_few_logits<R, true><<<a.n_parts, kFewThreads, shared, stream>>>(p, a);
-    } else {
-        MTC_CUDA_TRY(cudaFuncSetAttribute(k_few_logits<R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared));
-        k_few_logits<R, false><<<a.n_parts, kFewThreads, shared, stream>>>(p, a);
-    }
-    MTC_TRY(check_launch("linear cross entropy (few rows)"));
-    if (!grads) {
-        k_few_loss<<<1, static_cast<unsigned>(32 * p.N), 0, stream>>>(p, a, R);
-        return check_launch("linear cross entropy (loss)");
-    }
-    k_few_grad<R, C><<<dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(a.splits)), kFewThreads, 0, stream>>>(p, a);
-    MTC_TRY(check_launch("linear cross entropy (few rows' gradients)"));
-    if (p.dx == nullptr || p.D == 0) return MTC_OK;
-    k_few_dx<<<static_cast<unsigned>((p.N * p.D + 31) / 32), 256, 0, stream>>>(p, a);
-    return check_launch("linear cross entropy (input gradient)");
-}
-
 // ------------------------------------------------------------- small problems --
 // Up to 256 classes and 2^22 products: bound by latency, so two launches.  k_small_rows: a
 // warp a row, its lanes over the classes (and over the columns where the classes are few),
@@ -614,7 +186,7 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
         if (p.bias != nullptr) sum += __ldg(p.bias + v * p.b_s);
         z[i] = sum;
         if (v == t) zt = sum;
-        if (sub == 0) s = merge(s, Softmax{sum, isnan(sum) ? sum : isinf(sum) ? (sum > 0.0f ? sum : 0.0f) : 1.0f});
+        if (sub == 0) s = merge(s, one_logit(sum));
     }
     s = merge_lanes(s, 1, 32);
     const float lse = softmax_base(s.top) + logf(s.sum);
@@ -816,14 +388,8 @@ int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bia
     }
     if (p.V <= kSmallClasses && p.N < (int64_t{1} << 21) && p.N * p.V < (int64_t{1} << 22) / (p.D + 1))
         return small_path(p, stream);
-    if (p.N <= kFewRows) {
-        const int64_t row = (p.D + 127) / 128 * 512;
-        if (p.N == 1 && row <= kFewShared) return few_path<1>(p, stream);
-        if (p.N <= 2 && 2 * row <= kFewShared) return few_path<2>(p, stream);
-        if (p.N <= 4 && 4 * row <= kFewShared) return few_path<4>(p, stream);
-        if (p.N <= 8 && 8 * row <= kFewShared) return few_path<8>(p, stream);
-        if (16 * row <= kFewShared) return few_path<16>(p, stream);
-    }
+    if (few_rows(p)) return linear_ce_few(p, false, stream);
+    if (few_classes(p)) return linear_ce_few(p, true, stream);
     return linear_ce_tensor(p, stream);
 }
 

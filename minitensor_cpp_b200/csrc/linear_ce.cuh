@@ -39,7 +39,63 @@ int list_live_rows(const LinearCe &p, const LiveRows &live, cudaStream_t stream)
 // Tensor-core path (any sizes).
 int linear_ce_tensor(const LinearCe &p, cudaStream_t stream);
 
+// Up to kFewRows rows, or up to as many classes: float32 products that read W, or x, once for
+// the loss and once more for the gradients (linear_ce_few.cu).  Whether one of the two holds
+// and its rows fit in shared memory.
+constexpr int kFewRows = 16;
+bool few_rows(const LinearCe &p);
+bool few_classes(const LinearCe &p);
+int linear_ce_few(const LinearCe &p, bool classes, cudaStream_t stream);
+
 #ifdef __CUDACC__
+// A row's target, or -1 for a row without a loss; reports one outside the vocabulary.
+__device__ __forceinline__ int row_target(const LinearCe &p, int64_t n, unsigned long long *err, bool report) {
+    const int64_t t = p.targets[n * p.t_s];
+    if (t == p.ignore) return -1;
+    if (t < 0 || t >= p.V) {
+        if (report) report_index(err, t);
+        return -1;
+    }
+    return static_cast<int>(t);
+}
+
+// Running maximum and sum of exponentials relative to it.  Infinite maxima count from 0,
+// so that a row of +inf or -inf has its limit and not exp(inf - inf).
+struct Softmax {
+    float top, sum;
+};
+
+// (of one logit: a NaN or an infinity makes the sum what it is)
+__device__ __forceinline__ Softmax one_logit(float z) {
+    return Softmax{z, isnan(z) ? z : isinf(z) ? (z > 0.0f ? z : 0.0f) : 1.0f};
+}
+
+__device__ __forceinline__ float softmax_base(float top) { return isinf(top) ? 0.0f : top; }
+
+__device__ __forceinline__ Softmax merge(Softmax a, Softmax b) {
+    Softmax r;
+    r.top = fmaxf(a.top, b.top);
+    const float base = softmax_base(r.top);
+    r.sum = (a.sum != 0.0f ? a.sum * expf(softmax_base(a.top) - base) : 0.0f) +
+            (b.sum != 0.0f ? b.sum * expf(softmax_base(b.top) - base) : 0.0f);
+    return r;
+}
+
+__device__ __forceinline__ Softmax merge_lanes(Softmax s, int from, int to) {
+    for (int o = from; o < to; o <<= 1) {
+        Softmax other;
+        other.top = __shfl_xor_sync(0xFFFFFFFFu, s.top, o);
+        other.sum = __shfl_xor_sync(0xFFFFFFFFu, s.sum, o);
+        s = merge(s, other);
+    }
+    return s;
+}
+
+__device__ __forceinline__ float softmax_grad(float z, float lse, float d, bool hot) {
+    const float x = z - lse;
+    return d * (hot ? expm1f(x) : expf(x));
+}
+
 // How many of `extent` rows from `first` on have a loss.
 __device__ __forceinline__ int64_t live_extent(const int *live, int64_t first, int64_t extent) {
     const int64_t left = *live - first;

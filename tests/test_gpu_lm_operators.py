@@ -290,7 +290,9 @@ def check_ce(x, w, b, t, dloss):
 # one in each direction; more rows than a piece of the logits holds
 CE_SHAPES = [(1, 1, 1), (1, 2, 1), (1, 1000, 64), (2, 3, 5), (5, 257, 63), (64, 64, 64), (65, 63, 66), (127, 129, 128),
              (128, 256, 64), (129, 255, 200), (300, 3, 64), (256, 512, 256), (257, 513, 129), (1000, 1000, 96),
-             (513, 5003, 77), (2300, 301, 320), (33, 20011, 257), (4096, 40, 1024), (700, 1500, 1)]
+             (513, 5003, 77), (2300, 301, 320), (33, 20011, 257), (4096, 40, 1024), (700, 1500, 1),
+             (5000, 3, 300), (3000, 16, 130), (9001, 7, 97), (300, 1, 20000), (70000, 2, 33), (2000, 11, 256),
+             (16, 700, 515), (13, 3001, 640), (3, 5000, 1100), (1, 90001, 50), (17, 900, 400)]
 
 
 @pytest.mark.parametrize("n, vocab, dim", CE_SHAPES)
@@ -309,7 +311,7 @@ def test_linear_cross_entropy_and_gradients(cuda, n, vocab, dim):
         assert torch.equal(grads[k], again[k]), f"{k} differs from run to run"
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(6, 40, 16), (300, 1000, 80), (1500, 3000, 64)])
+@pytest.mark.parametrize("n, vocab, dim", [(6, 40, 16), (300, 1000, 80), (1500, 3000, 64), (4000, 6, 200), (9, 3000, 170)])
 def test_linear_cross_entropy_takes_views_of_any_layout(cuda, n, vocab, dim):
     """Transposed and padded operands, odd offsets, a broadcast dloss, every second
     target; what lies beside the outputs stays."""
@@ -339,7 +341,7 @@ def test_linear_cross_entropy_takes_views_of_any_layout(cuda, n, vocab, dim):
     assert (lo[0] == 55).all() and (lo[:, 1] == 55).all() and (db[:, 0] == 55).all() and (db[:, 2] == 55).all()
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(40, 30, 20), (600, 1000, 96), (1100, 2048, 256)])
+@pytest.mark.parametrize("n, vocab, dim", [(40, 30, 20), (600, 1000, 96), (1100, 2048, 256), (3000, 10, 150), (12, 4000, 200)])
 def test_ignored_rows_may_hold_anything(cuda, n, vocab, dim):
     """NaN and infinities in rows without a loss reach no output; with all rows
     ignored every gradient is zero."""
@@ -363,7 +365,7 @@ def test_ignored_rows_may_hold_anything(cuda, n, vocab, dim):
     check_ce(x2, w, b, one, torch.ones(n, device=cuda))
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(40, 30, 20), (600, 1000, 96)])
+@pytest.mark.parametrize("n, vocab, dim", [(40, 30, 20), (600, 1000, 96), (3000, 13, 150), (15, 4000, 100)])
 def test_targets_outside_the_vocabulary_are_reported(cuda, n, vocab, dim):
     import torch
 
@@ -382,7 +384,7 @@ def test_targets_outside_the_vocabulary_are_reported(cuda, n, vocab, dim):
             assert torch.equal(got[k], want[k]), k
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(30, 50, 24), (520, 1030, 72)])
+@pytest.mark.parametrize("n, vocab, dim", [(30, 50, 24), (520, 1030, 72), (2200, 12, 170), (10, 3000, 150)])
 def test_non_finite_rows_stay_rows(cuda, n, vocab, dim):
     """NaN and infinite x: that row's loss and dx are not finite, the others are as before."""
     import torch
@@ -399,7 +401,7 @@ def test_non_finite_rows_stay_rows(cuda, n, vocab, dim):
     assert not got["dw"].isfinite().any()
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(50, 70, 33), (400, 900, 130)])
+@pytest.mark.parametrize("n, vocab, dim", [(50, 70, 33), (400, 900, 130), (3000, 9, 160), (7, 2000, 330)])
 @pytest.mark.parametrize("sx, sw", [(1e-30, 1.0), (1e25, 1e-25), (1.0, 1e-38), (3e-42, 1.0), (1e30, 1e-38)])
 def test_scales_far_from_one(cuda, n, vocab, dim, sx, sw):
     """Operands near the ends of float32's range; the products stay in it."""
@@ -408,7 +410,7 @@ def test_scales_far_from_one(cuda, n, vocab, dim, sx, sw):
     check_ce(x, w, b, t, dloss * 1e-30)
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(40, 60, 16), (520, 1300, 100)])
+@pytest.mark.parametrize("n, vocab, dim", [(40, 60, 16), (520, 1300, 100), (3000, 8, 200), (6, 4000, 200)])
 def test_confident_rows_keep_small_gradients(cuda, n, vocab, dim):
     """Logits so far apart that p is 1 - 1e-9 at the target and 1e-30 elsewhere: the
     gradient's entries span 30 decades and stay inside their bounds."""
@@ -420,7 +422,7 @@ def test_confident_rows_keep_small_gradients(cuda, n, vocab, dim):
     assert got["loss"].min() >= 0
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(37, 53, 29), (530, 700, 120)])
+@pytest.mark.parametrize("n, vocab, dim", [(37, 53, 29), (530, 700, 120), (3000, 15, 120), (5, 5000, 180)])
 def test_rare_classes_keep_their_precision(cuda, n, vocab, dim):
     """A class of probability 1e-9 in every row: its weight gradient is 1e9 times
     smaller than the others' and still accurate to 1e-4 of itself, as the float32
@@ -480,7 +482,7 @@ def test_each_gradient_alone_equals_all_together(cuda):
     """Outputs that are not asked for are not written, and the others do not change."""
     import torch
 
-    for n, vocab, dim in ((40, 60, 16), (300, 900, 70)):
+    for n, vocab, dim in ((40, 60, 16), (300, 900, 70), (3000, 14, 110), (11, 2500, 170)):
         x, w, b, t, dloss = ce_data(n, vocab, dim, 21, ignored=0.2)
         all_ = run_ce(x, w, b, t, dloss)
         for name, shape in (("dx", x.shape), ("dw", w.shape), ("db", b.shape), ("loss", t.shape), ("lse", t.shape)):
