@@ -32,6 +32,7 @@ template <int N>
 struct DenseTable {
     int count;
     int pieces;
+    int in_place;  // every dst is its src
     int first_piece[N];
     const float *src[N];
     float *dst[N];
@@ -140,16 +141,17 @@ __global__ void __launch_bounds__(kThreads) k_square_sum(const __grid_constant__
 template <int N>
 __global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ DenseTable<N> t, const double *partials,
                                                     int n_partials, float max_norm, float *norm_out) {
+    wait_for_previous();
     const double norm = sqrt(sum_partials(partials, n_partials));
     const float c = clip_factor(norm, max_norm);
     if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(norm);
+    if (c == 1.0f && t.in_place) return;
     for (int p = t.pieces - 1 - static_cast<int>(blockIdx.x); p >= 0; p -= gridDim.x) {
         long long begin, end;
         int head;
         const int k = find_piece(t, p, begin, end, head);
         const float *src = t.src[k];
         float *dst = t.dst[k];
-        if (c == 1.0f && src == dst) continue;
         long long at = begin;
         if (begin == 0 && head > 0) {
             at = head < end ? head : end;
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(kThreads) k_square_sum_strided(const StridedTe
 
 __global__ void __launch_bounds__(kThreads) k_scale_strided(const StridedTensor t, const double *partials,
                                                             int n_partials, float max_norm) {
+    wait_for_previous();
     const float c = clip_factor(sqrt(sum_partials(partials, n_partials)), max_norm);
     for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < t.numel;
          i += static_cast<long long>(gridDim.x) * kThreads) {
@@ -312,12 +315,14 @@ int pieces_of(const Dense &d) {
 template <int N>
 void fill_table(DenseTable<N> &t, const Dense *d, int count) {
     t.count = count;
+    t.in_place = 1;
     int p = 0;
     for (int i = 0; i < count; ++i) {
         t.first_piece[i] = p;
         t.src[i] = d[i].src;
         t.dst[i] = d[i].dst;
         t.n[i] = d[i].n;
+        t.in_place &= d[i].src == d[i].dst;
         p += pieces_of(d[i]);
     }
     t.pieces = p;
@@ -380,14 +385,16 @@ struct Launcher {
     int scale(float max_norm, float *norm) {
         float *write = norm;  // by the first launch alone
         MTC_TRY(tables([&](const auto &t) {
-            k_scale<<<grid(t.pieces), kThreads, 0, stream>>>(t, partials, n_partials, max_norm, write);
+            constexpr int N = sizeof(t.n) / sizeof(t.n[0]);
+            float *once = write;
             write = nullptr;
-            return check_launch("gradient clipping");
+            return launch_dependent("gradient clipping", k_scale<N>, grid(t.pieces), kThreads, 0, stream, t, partials,
+                                    n_partials, max_norm, once);
         }));
         for (const StridedTensor &t : plan.strided) {
-            k_scale_strided<<<grid((t.numel + kThreads - 1) / kThreads), kThreads, 0, stream>>>(t, partials, n_partials,
-                                                                                               max_norm);
-            MTC_TRY(check_launch("gradient clipping (strided)"));
+            MTC_TRY(launch_dependent("gradient clipping (strided)", k_scale_strided,
+                                     grid((t.numel + kThreads - 1) / kThreads), kThreads, 0, stream, t, partials,
+                                     n_partials, max_norm));
         }
         if (write != nullptr) return write_norm(write);
         return MTC_OK;

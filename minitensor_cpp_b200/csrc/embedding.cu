@@ -634,6 +634,7 @@ __device__ __forceinline__ void join_run(const SumArgs &a, unsigned int k, unsig
 
 template <class P>
 __global__ void __launch_bounds__(kThreads) k_token_sums(const SumArgs a) {
+    wait_for_previous();
     const unsigned int unit = blockIdx.x / a.slabs;
     if (unit >= a.pieces) {
         // rows without a position
@@ -978,9 +979,9 @@ int run_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
         MTC_TRY(sort_positions(a, padding, buffers, c, b, rows, stream));
     }
     const unsigned int grid = (a.pieces + a.zero_units) * a.slabs;
-    if (vec == 4) k_token_sums<Vectors4><<<grid, threads, 0, stream>>>(a);
-    else if (vec == 2) k_token_sums<Vectors2><<<grid, threads, 0, stream>>>(a);
-    else k_token_sums<Spread4><<<grid, threads, 0, stream>>>(a);
+    auto sums = vec == 4 ? k_token_sums<Vectors4> : vec == 2 ? k_token_sums<Vectors2> : k_token_sums<Spread4>;
+    if (a.n > 0) return launch_dependent("embedding gradient (sums)", sums, grid, threads, 0, stream, a);
+    sums<<<grid, threads, 0, stream>>>(a);  // nothing but rows to clear: the call's first launch
     return check_launch("embedding gradient (sums)");
 }
 

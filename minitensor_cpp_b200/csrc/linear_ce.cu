@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
 }
 
 __global__ void __launch_bounds__(256) k_small_weights(const LinearCe p, const SmallArgs a) {
+    wait_for_previous();
     const int64_t weights = p.V * p.D, total = weights + p.V;
     const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int64_t v = e < weights ? e / p.D : e - weights, d = e - v * p.D;
@@ -297,8 +298,7 @@ int small_path(const LinearCe &p, cudaStream_t stream) {
     k_small_rows<<<static_cast<unsigned>((p.N + 7) / 8), 256, 0, stream>>>(p, a);
     MTC_TRY(check_launch("linear cross entropy (small)"));
     if (!grads || (p.dw == nullptr && p.db == nullptr)) return MTC_OK;
-    k_small_weights<<<dim3(a.n_arrived, static_cast<unsigned>(splits)), 256, 0, stream>>>(p, a);
-    return check_launch("linear cross entropy (small, weight gradient)");
+    return launch_dependent("linear cross entropy (small, weight gradient)", k_small_weights, dim3(a.n_arrived, static_cast<unsigned>(splits)), 256, 0, stream, p, a);
 }
 
 // ------------------------------------------------------------------- host --

@@ -247,6 +247,7 @@ __device__ __forceinline__ void store_loss(const LinearCe &p, const FewArgs &a, 
 }
 
 __global__ void __launch_bounds__(32 * kFewRows) k_few_loss(const LinearCe p, const FewArgs a, int R) {
+    wait_for_previous();
     const int n = threadIdx.x / 32;
     if (n >= p.N) return;
     const float lse = few_lse(a, R, n);
@@ -256,6 +257,7 @@ __global__ void __launch_bounds__(32 * kFewRows) k_few_loss(const LinearCe p, co
 // C columns a lane, 32 C a CTA.
 template <int R, int C, bool CLASSES>
 __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const LinearCe p, const FewArgs a) {
+    wait_for_previous();
     __shared__ float lse[R], dloss[R];
     __shared__ int target[R];
     __shared__ float sums[kFewThreads / 32][32 * C];
@@ -408,6 +410,7 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const 
 // The gradient of the few: eight warps take the parts of 32 elements in turn.
 template <bool CLASSES>
 __global__ void __launch_bounds__(256) k_few_join(const LinearCe p, const FewArgs a) {
+    wait_for_previous();
     __shared__ float sums[8][32];
     const int64_t width = p.D + 1, total = a.few.rows * width;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
@@ -472,14 +475,11 @@ int few_path(const LinearCe &p, FewArgs a, cudaStream_t stream) {
     MTC_TRY(check_launch("linear cross entropy (few)"));
     if (!grads) {
         if (CLASSES) return MTC_OK;
-        k_few_loss<<<1, static_cast<unsigned>(32 * p.N), 0, stream>>>(p, a, R);
-        return check_launch("linear cross entropy (loss)");
+        return launch_dependent("linear cross entropy (loss)", k_few_loss, 1, static_cast<unsigned>(32 * p.N), 0, stream, p, a, R);
     }
-    k_few_grad<R, C, CLASSES><<<dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(a.splits)), kFewThreads, 0, stream>>>(p, a);
-    MTC_TRY(check_launch("linear cross entropy (few, gradients)"));
+    MTC_TRY((launch_dependent("linear cross entropy (few, gradients)", k_few_grad<R, C, CLASSES>, dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(a.splits)), kFewThreads, 0, stream, p, a)));
     if (!few_grad) return MTC_OK;
-    k_few_join<CLASSES><<<static_cast<unsigned>((a.few.rows * (p.D + 1) + 31) / 32), 256, 0, stream>>>(p, a);
-    return check_launch("linear cross entropy (few, join)");
+    return launch_dependent("linear cross entropy (few, join)", k_few_join<CLASSES>, static_cast<unsigned>((a.few.rows * (p.D + 1) + 31) / 32), 256, 0, stream, p, a);
 }
 
 template <bool CLASSES>

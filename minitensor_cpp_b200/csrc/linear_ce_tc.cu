@@ -134,6 +134,7 @@ __device__ __forceinline__ const float *source_row(const PackSource &s, int64_t 
 // Largest finite magnitudes of x (rows with a loss), weight and dloss, and the zero rows of
 // dx.  Each warp takes rows in turn, four 16-byte loads in flight a lane, or sixteen of 4.
 __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
+    wait_for_previous();
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
     const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
 
 // Each half-warp packs one block of 64 columns at a time: a lane four columns.
 __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
+    wait_for_previous();
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
     const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
@@ -527,7 +529,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
     const int64_t cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
-    const Extent e = extent_of(args);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -553,6 +554,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    wait_for_previous();
+    const Extent e = extent_of(args);
 
     if (warp >= 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
@@ -710,6 +713,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
 
 // The splits' partial results in order, into the rows of the result.
 __global__ void __launch_bounds__(256) k_join_splits(const TileArgs a) {
+    wait_for_previous();
     int64_t M = a.M;
     if (a.live != nullptr && !a.live_k) M = live_extent(a.live, a.first, M);
     if (a.live_k && a.first > 0 && live_extent(a.live, a.first, a.K) == 0) return;
@@ -767,6 +771,7 @@ struct RowArgs {
 
 // One warp a row: the statistics of its tiles make lse and the loss.
 __global__ void __launch_bounds__(256) k_row_loss(const RowArgs a) {
+    wait_for_previous();
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     if (r >= live_extent(a.live, a.first, a.rows)) return;
@@ -809,6 +814,7 @@ constexpr int kGradRows = 64;  // rows of a CTA
 // z -> g' in place.  A CTA takes 128 columns of 64 rows, a warp eight of the rows, a lane
 // four columns: 512 bytes of z a load, two blocks of 128 + 128 bytes a store.
 __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
+    wait_for_previous();
     const int64_t live = live_extent(a.live, a.first, a.rows);
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kGradRows;
     if (r0 >= (live + 63) / 64 * 64) return;
@@ -880,6 +886,7 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
 
 // A CTA takes 32 columns; its eight warps take the row blocks in turn.
 __global__ void __launch_bounds__(256) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
+    wait_for_previous();
     __shared__ float sums[8][32];
     const int64_t v = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
     const int blocks = static_cast<int>((live_extent(a.live, a.first, a.rows) + kGradRows - 1) / kGradRows);
@@ -918,8 +925,8 @@ int launch_product(const CUtensorMap &a, const CUtensorMap &b, const TileArgs &a
                                       kSmemBytes));
     const int64_t units = (args.M + kTileRows - 1) / kTileRows * args.tiles_n * args.splits;
     const int64_t pairs = units < sms / 2 ? units : sms / 2;
-    k_pair_product<A_MN, B_MN, MODE><<<static_cast<unsigned>(2 * pairs), kCtaThreads, kSmemBytes, stream>>>(a, b, args);
-    return check_launch("linear cross entropy (tensor-core product)");
+    return launch_dependent("linear cross entropy (tensor-core product)", k_pair_product<A_MN, B_MN, MODE>,
+                            static_cast<unsigned>(2 * pairs), kCtaThreads, kSmemBytes, stream, a, b, args);
 }
 
 // Splits of K so that the tiles of a product fill the pairs of SMs: the fewest whose
@@ -1017,11 +1024,9 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const int64_t most = static_cast<int64_t>(sms) * 8;
     const int64_t share = most * p.N / (p.N + p.V);
     k.first_of_second = share < 1 ? 1 : share > most - 1 ? most - 1 : share;
-    k_largest<<<static_cast<unsigned>(most), 256, 0, stream>>>(k);
-    MTC_TRY(check_launch("linear cross entropy (magnitudes)"));
+    MTC_TRY((launch_dependent("linear cross entropy (magnitudes)", k_largest, static_cast<unsigned>(most), 256, 0, stream, k)));
     if (p.D > 0) {
-        k_pack<<<static_cast<unsigned>(most), 256, 0, stream>>>(k);
-        MTC_TRY(check_launch("linear cross entropy (packing)"));
+        MTC_TRY((launch_dependent("linear cross entropy (packing)", k_pack, static_cast<unsigned>(most), 256, 0, stream, k)));
     }
 
     CUtensorMap x_k, w_k, w_mn, x_mn, g_k, g_mn;
@@ -1057,17 +1062,14 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         // (a last tile of 128 columns or less has no second half)
         const RowArgs ra{first, rows, live.count, static_cast<int>((p.V + 127) / 128), 2 * tiles_v, part_max, part_sum,
                          z_target, live.row, lse_live, p.loss, p.lse, p.loss_s, p.lse_s};
-        k_row_loss<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(ra);
-        MTC_TRY(check_launch("linear cross entropy (loss)"));
+        MTC_TRY((launch_dependent("linear cross entropy (loss)", k_row_loss, static_cast<unsigned>((rows + 7) / 8), 256, 0, stream, ra)));
         if (!grads) continue;
         const GradArgs ga{first, rows_up, live.count, p.V, z, pitch, lse_live, live.target, live.dloss, live.count + 3,
                           p.db != nullptr ? columns : nullptr};
         const dim3 grid(static_cast<unsigned>((pitch + 127) / 128), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
-        k_softmax_grad<<<grid, 256, 0, stream>>>(ga);
-        MTC_TRY(check_launch("linear cross entropy (gradient of the logits)"));
+        MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, 256, 0, stream, ga)));
         if (p.db != nullptr) {
-            k_bias_grad<<<static_cast<unsigned>((p.V + 31) / 32), 256, 0, stream>>>(ga, p.db, p.db_s, first > 0);
-            MTC_TRY(check_launch("linear cross entropy (bias gradient)"));
+            MTC_TRY((launch_dependent("linear cross entropy (bias gradient)", k_bias_grad, static_cast<unsigned>((p.V + 31) / 32), 256, 0, stream, ga, p.db, p.db_s, first > 0)));
         }
         const __half *gp = reinterpret_cast<const __half *>(z);
         if (p.dx != nullptr && p.D > 0) {
@@ -1096,8 +1098,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
                 t.part_sum = split_ws;
                 t.out = p.dx;
                 t.vec = vec;
-                k_join_splits<<<static_cast<unsigned>(sms * 8), 256, 0, stream>>>(t);
-                MTC_TRY(check_launch("linear cross entropy (input gradient)"));
+                MTC_TRY((launch_dependent("linear cross entropy (input gradient)", k_join_splits, static_cast<unsigned>(sms * 8), 256, 0, stream, t)));
             }
         }
         if (p.dw != nullptr && p.D > 0) {
@@ -1127,8 +1128,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
                 t.part_sum = split_ws;
                 t.out = p.dw;
                 t.vec = vec;
-                k_join_splits<<<static_cast<unsigned>(sms * 8), 256, 0, stream>>>(t);
-                MTC_TRY(check_launch("linear cross entropy (weight gradient)"));
+                MTC_TRY((launch_dependent("linear cross entropy (weight gradient)", k_join_splits, static_cast<unsigned>(sms * 8), 256, 0, stream, t)));
             }
         }
     }

@@ -2,6 +2,8 @@
 // workspaces for the time of a call, argument checks and device-side helpers.
 #pragma once
 
+#include <cstring>
+
 #include "common.cuh"
 #include "graph.cuh"
 
@@ -93,6 +95,31 @@ inline float *float_at(const mtc_desc *d) { return static_cast<float *>(d->data)
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 #ifdef __CUDACC__
+// Launches a kernel that calls wait_for_previous() first: its CTAs may take their places while
+// the kernel before it on the stream runs out, which hides most of the launch.  Only for the
+// second and later kernels of a call; each of them waits for the one before, so all earlier
+// ones are done as well.
+template <class... P, class... A>
+int launch_dependent(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
+                     A &&...args) {
+    cudaLaunchAttribute attr;
+    std::memset(&attr, 0, sizeof(attr));
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config;
+    std::memset(&config, 0, sizeof(config));
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    MTC_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
+    return check_launch(what);
+}
+
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void report_index(unsigned long long *err, long long index) {
     if (atomicCAS(&err[0], 0ull, static_cast<unsigned long long>(MTC_ERR_OUT_OF_RANGE)) == 0ull)
         atomicExch(&err[1], static_cast<unsigned long long>(index));
