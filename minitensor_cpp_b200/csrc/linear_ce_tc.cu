@@ -34,7 +34,8 @@
 // epilogue: two warps for each quarter of the tensor memory's lanes, 128 columns each,
 // with 208 registers a thread (128 sums, 64 of a load in flight) that the first four
 // warps give up.  Results leave through 4 KB of shared memory a warp, so that a store
-// covers whole lines of four rows and not 16 bytes of 32.
+// covers whole lines of four rows and not 16 bytes of 32; results whose rows allow no such
+// stores go by way of a padded workspace.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
@@ -276,11 +277,12 @@ struct TileArgs {
     float *part_max, *part_sum;  // [M][2 tiles_n]
     float *z_target;             // [M]
     // Sum
-    float *out;       // final, or with splits the partial results [splits][M][N]
-    int64_t out_rs, out_cs;
+    float *out;       // rows that float4 stores fit
+    int64_t out_rs;
     const int *out_map;
     int add;
-    int vec;          // float4 stores
+    float *parts;     // the splits' partial results [splits][M][parts_pitch]; null: straight to out
+    int64_t parts_pitch;
 };
 
 __device__ __forceinline__ void tma_load_operand(void *dst, const CUtensorMap *map, uint32_t leader_bar, int row, int block,
@@ -389,10 +391,9 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
 
 // A warp's 32 rows x n columns from the lanes' registers to memory, 32 columns at a time
 // through `stage`: written as 16-byte chunks XOR-swizzled by the row, read back as four
-// rows of 128 bytes (vec) or one row of 32 values at a time.  `to`: where this lane's row
-// begins, null for a row that is not stored.
-__device__ __forceinline__ void store_rows(float *stage, const float (&acc)[128], float *to, int n, int64_t cs, bool vec,
-                                           bool add) {
+// rows of 128 bytes, so that a store covers whole lines.  `to`: where this lane's row begins,
+// null for a row that is not stored.
+__device__ __forceinline__ void store_rows(float *stage, const float (&acc)[128], float *to, int n, bool add) {
     const int lane = threadIdx.x % 32;
     float4 *s4 = reinterpret_cast<float4 *>(stage);
     const unsigned long long mine = reinterpret_cast<unsigned long long>(to);
@@ -405,34 +406,22 @@ __device__ __forceinline__ void store_rows(float *stage, const float (&acc)[128]
             s4[lane * 8 + (j ^ (lane & 7))] =
                 make_float4(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3]);
         __syncwarp();
-        if (vec) {
-            const int j = lane % 8, col = c * 32 + 4 * j;
+        const int j = lane % 8, col = c * 32 + 4 * j;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + lane / 8;
-                float *row = reinterpret_cast<float *>(__shfl_sync(0xFFFFFFFFu, mine, r));
-                float4 x = s4[r * 8 + (j ^ (r & 7))];
-                if (row == nullptr || col >= n) continue;
-                float4 *p = reinterpret_cast<float4 *>(row + col);
-                if (add) {
-                    const float4 o = *p;
-                    x.x += o.x;
-                    x.y += o.y;
-                    x.z += o.z;
-                    x.w += o.w;
-                }
-                *p = x;
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + lane / 8;
+            float *row = reinterpret_cast<float *>(__shfl_sync(0xFFFFFFFFu, mine, r));
+            float4 x = s4[r * 8 + (j ^ (r & 7))];
+            if (row == nullptr || col >= n) continue;
+            float4 *p = reinterpret_cast<float4 *>(row + col);
+            if (add) {
+                const float4 o = *p;
+                x.x += o.x;
+                x.y += o.y;
+                x.z += o.z;
+                x.w += o.w;
             }
-        } else {
-            const int col = c * 32 + lane;
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-                float *row = reinterpret_cast<float *>(__shfl_sync(0xFFFFFFFFu, mine, r));
-                const float x = stage[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
-                if (row == nullptr || col >= n) continue;
-                float *p = row + col * cs;
-                *p = add ? *p + x : x;
-            }
+            *p = x;
         }
     }
 }
@@ -489,7 +478,7 @@ __device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float
     }
     if (a.z == nullptr) return;
     // rows are padded to 64 columns: the last four of a ragged end may lie behind V
-    store_rows(stage, acc, live ? a.z + row * a.z_pitch + col0 : nullptr, n, 1, true, false);
+    store_rows(stage, acc, live ? a.z + row * a.z_pitch + col0 : nullptr, n, false);
 }
 
 __device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&acc)[128], float *stage, int64_t row,
@@ -498,14 +487,10 @@ __device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&
     const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
     rescale(acc, f0, f1);
     float *to = nullptr;
-    int64_t cs = 1;
-    if (a.splits > 1) {
-        if (row < M) to = a.out + (split * a.M + row) * a.N + col0;
-    } else {
-        cs = a.out_cs;
-        if (row < M) to = a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0 * cs;
-    }
-    store_rows(stage, acc, to, n, cs, a.vec, a.add && a.splits == 1);
+    if (row < M)
+        to = a.parts != nullptr ? a.parts + (split * a.M + row) * a.parts_pitch + col0
+                                : a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0;
+    store_rows(stage, acc, to, n, a.add && a.parts == nullptr);
 }
 
 template <bool A_MN, bool B_MN, Out MODE>
@@ -711,20 +696,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     }
 }
 
-// The splits' partial results in order, into the rows of the result.
-__global__ void __launch_bounds__(256) k_join_splits(const TileArgs a) {
+// The splits' partial results in order, into the rows of the result, whatever their layout.
+__global__ void __launch_bounds__(256) k_join_splits(const TileArgs a, int64_t out_cs, int vec) {
     wait_for_previous();
     int64_t M = a.M;
     if (a.live != nullptr && !a.live_k) M = live_extent(a.live, a.first, M);
     if (a.live_k && a.first > 0 && live_extent(a.live, a.first, a.K) == 0) return;
-    const float *parts = a.part_sum;
-    const int64_t plane = a.M * a.N;
-    if (a.vec) {
+    const int64_t plane = a.M * a.parts_pitch;
+    if (vec) {
         const int64_t per_row = a.N / 4;
         for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < M * per_row;
              i += static_cast<int64_t>(gridDim.x) * 256) {
             const int64_t r = i / per_row, c = (i - r * per_row) * 4;
-            const float *src = parts + r * a.N + c;
+            const float *src = a.parts + r * a.parts_pitch + c;
             float4 sum = *reinterpret_cast<const float4 *>(src);
             for (int s = 1; s < a.splits; ++s) {
                 const float4 v = *reinterpret_cast<const float4 *>(src + s * plane);
@@ -746,13 +730,27 @@ __global__ void __launch_bounds__(256) k_join_splits(const TileArgs a) {
         }
         return;
     }
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < M * a.N;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / a.N, c = i - r * a.N;
-        float sum = parts[i];
-        for (int s = 1; s < a.splits; ++s) sum += parts[s * plane + i];
-        float *to = a.out + (a.out_map != nullptr ? a.out_map[a.first + r] : r) * a.out_rs + c * a.out_cs;
-        *to = a.add ? *to + sum : sum;
+    // a warp a row, eight columns of a lane in flight
+    const int lane = threadIdx.x % 32;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; r < M;
+         r += static_cast<int64_t>(gridDim.x) * 8) {
+        const float *src = a.parts + r * a.parts_pitch;
+        float *to = a.out + (a.out_map != nullptr ? a.out_map[a.first + r] : r) * a.out_rs;
+        for (int64_t c0 = lane; c0 < a.N; c0 += 256) {
+            float sum[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) sum[u] = c0 + 32 * u < a.N ? src[c0 + 32 * u] : 0.0f;
+            for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (c0 + 32 * u < a.N) sum[u] += src[s * plane + c0 + 32 * u];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (c0 + 32 * u >= a.N) break;
+                float *p = to + (c0 + 32 * u) * out_cs;
+                *p = a.add ? *p + sum[u] : sum[u];
+            }
+        }
     }
 }
 
@@ -983,8 +981,11 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t row_stat = padded(static_cast<size_t>(piece) * 4);
     const size_t z_bytes = grads ? padded(static_cast<size_t>(piece) * pitch * 4) : 0;
     const size_t col_bytes = p.db != nullptr ? padded(static_cast<size_t>(piece / kGradRows) * pitch * 4) : 0;
-    const size_t split_dx = p.dx != nullptr && splits_dx > 1 ? static_cast<size_t>(splits_dx) * piece * p.D * 4 : 0;
-    const size_t split_dw = p.dw != nullptr && splits_dw > 1 ? static_cast<size_t>(splits_dw) * p.V * p.D * 4 : 0;
+    const int64_t parts_pitch = (p.D + 3) / 4 * 4;
+    const bool parts_dx = splits_dx > 1 || !vector_source(p.dx, p.dx_rs, p.dx_cs, p.D);
+    const bool parts_dw = splits_dw > 1 || !vector_source(p.dw, p.dw_rs, p.dw_cs, p.D);
+    const size_t split_dx = p.dx != nullptr && parts_dx ? static_cast<size_t>(splits_dx) * piece * parts_pitch * 4 : 0;
+    const size_t split_dw = p.dw != nullptr && parts_dw ? static_cast<size_t>(splits_dw) * p.V * parts_pitch * 4 : 0;
     const size_t split_bytes = grads ? padded(split_dx > split_dw ? split_dx : split_dw) : 0;
     Workspace ws;
     MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 2 * row_stat + z_bytes + col_bytes + split_bytes,
@@ -1087,19 +1088,16 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.amax_a = live.count + 3;
             t.amax_b = live.count + 2;
             t.err = err;
+            t.out = p.dx;
             t.out_rs = p.dx_rs;
-            t.out_cs = p.dx_cs;
             t.out_map = live.row;
-            const bool vec = aligned16(p.dx) && p.dx_cs == 1 && p.dx_rs % 4 == 0 && p.D % 4 == 0;
-            t.out = splits_dx > 1 ? split_ws : p.dx;
-            t.vec = splits_dx > 1 ? p.D % 4 == 0 : vec;
+            t.parts = parts_dx ? split_ws : nullptr;
+            t.parts_pitch = parts_pitch;
             MTC_TRY((launch_product<false, true, Out::Sum>(g_k, w_mn, t, sms, stream)));
-            if (splits_dx > 1) {
-                t.part_sum = split_ws;
-                t.out = p.dx;
-                t.vec = vec;
-                MTC_TRY((launch_dependent("linear cross entropy (input gradient)", k_join_splits, static_cast<unsigned>(sms * 8), 256, 0, stream, t)));
-            }
+            if (parts_dx)
+                MTC_TRY(launch_dependent("linear cross entropy (input gradient)", k_join_splits,
+                                         static_cast<unsigned>(sms * 8), 256, 0, stream, t, p.dx_cs,
+                                         vector_source(p.dx, p.dx_rs, p.dx_cs, p.D)));
         }
         if (p.dw != nullptr && p.D > 0) {
             MTC_TRY(operand_map(g_mn, gp, rows_up, v_blocks, v_blocks, true));
@@ -1117,19 +1115,16 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.amax_a = live.count + 3;
             t.amax_b = live.count + 1;
             t.err = err;
+            t.out = p.dw;
             t.out_rs = p.dw_rs;
-            t.out_cs = p.dw_cs;
             t.add = first > 0;
-            const bool vec = aligned16(p.dw) && p.dw_cs == 1 && p.dw_rs % 4 == 0 && p.D % 4 == 0;
-            t.out = splits_dw > 1 ? split_ws : p.dw;
-            t.vec = splits_dw > 1 ? p.D % 4 == 0 : vec;
+            t.parts = parts_dw ? split_ws : nullptr;
+            t.parts_pitch = parts_pitch;
             MTC_TRY((launch_product<true, true, Out::Sum>(g_mn, x_mn, t, sms, stream)));
-            if (splits_dw > 1) {
-                t.part_sum = split_ws;
-                t.out = p.dw;
-                t.vec = vec;
-                MTC_TRY((launch_dependent("linear cross entropy (weight gradient)", k_join_splits, static_cast<unsigned>(sms * 8), 256, 0, stream, t)));
-            }
+            if (parts_dw)
+                MTC_TRY(launch_dependent("linear cross entropy (weight gradient)", k_join_splits,
+                                         static_cast<unsigned>(sms * 8), 256, 0, stream, t, p.dw_cs,
+                                         vector_source(p.dw, p.dw_rs, p.dw_cs, p.D)));
         }
     }
     return MTC_OK;
