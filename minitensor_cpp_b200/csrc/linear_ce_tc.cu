@@ -11,13 +11,15 @@
 // MMAs run at twice the rate of the TF32 ones that a split in TF32 would need.
 //
 // The tensor core truncates its accumulator at every addition, which over a long K
-// costs a part in 2^24 each time, always towards zero.  So 128 values of K stay in
-// tensor memory at most: the epilogue warps read each piece of 128 and add it, rounded
+// costs a part in 2^24 each time, always towards zero.  So 256 values of K stay in
+// tensor memory at most: the epilogue warps read each piece of 256 and add it, rounded
 // to nearest, to sums in registers, while the next piece runs in the other half of
-// tensor memory.  A piece is the cross terms of its two blocks of 64, then the hi.hi of
-// both.  (Pieces of 64 were 20 % slower: a piece's hand-over, from the MMAs' commit by
-// way of the epilogues of both CTAs to the next MMA, takes some 1500 clocks and the
-// reading 700, which two pieces of 1536 clocks do not cover and two of 3072 do.)
+// tensor memory.  A piece is the cross terms of its four blocks of 64, then the hi.hi of
+// all four.  (Pieces of 64 were 20 % slower than of 128: a piece's hand-over, from the MMAs'
+// commit by way of the epilogues of both CTAs to the next MMA, takes some 1500 clocks and the
+// reading 1900, which two pieces of 1536 clocks do not cover.  Pieces of 256 gain another 5 %:
+// the reads of tensor memory share it with the MMAs, and under the power limit their energy
+// is taken from the MMAs' clock.)
 //
 // All three products read the same packed operands, [row][64 columns][hi, lo], K-major
 // or MN-major by the matrix descriptors alone:
@@ -30,12 +32,13 @@
 // A pair of CTAs works on a 256 x 256 tile (tcgen05.mma.cta_group::2): each stages its
 // own 128 rows of A and 128 columns of B, 64 KB for 1536 clocks of MMAs.  The lo halves
 // are free after a piece's cross terms, the hi halves only at its end, so each has a ring
-// of its own: four stages of hi, two of lo, 32 KB each.  Warp 0 loads (TMA), warp 1 of the leader issues, warps 4..11 are the
-// epilogue: two warps for each quarter of the tensor memory's lanes, 128 columns each,
-// with 208 registers a thread (128 sums, 64 of a load in flight) that the first four
-// warps give up.  Results leave through 4 KB of shared memory a warp, so that a store
-// covers whole lines of four rows and not 16 bytes of 32; results whose rows allow no such
-// stores go by way of a padded workspace.
+// of its own: five stages of hi, two of lo, 32 KB each.  Warp 0 loads (TMA), warp 1 of the
+// leader issues, warps 4..11 are the epilogue: two warps for each quarter of the tensor
+// memory's lanes, 128 columns each, with 208 registers a thread (128 sums, 64 of a load in
+// flight) that the first four warps give up.  A lane holds a row and stores it itself, a
+// 32-byte sector at a time: the 32 KB of shared memory that would make whole lines of it are
+// worth more as a stage.  Results whose rows allow no such stores go by way of a padded
+// workspace.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
@@ -52,11 +55,10 @@ constexpr int kBlock = 64;                       // columns of a packed block: 6
 constexpr int kTileRows = 256, kTileCols = 256;  // of a CTA pair
 constexpr int kOperandBytes = 16384;             // 128 rows (or columns) x 64 of K, hi or lo
 constexpr int kStageBytes = 2 * kOperandBytes;   // A and B
-constexpr int kHiStages = 4, kLoStages = 2;
+constexpr int kHiStages = 5, kLoStages = 2;
 constexpr int kStages = kHiStages + kLoStages;
-constexpr int kPieceBlocks = 2;                  // blocks of K that are summed in tensor memory
-constexpr int kStageOut = 4096;  // 32 rows x 32 columns of an epilogue warp
-constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStageOut + 1024 + 256;
+constexpr int kPieceBlocks = 4;                  // blocks of K that are summed in tensor memory
+constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
 constexpr int kCtaThreads = 384;
 constexpr int kEpilogueRegs = 208, kOtherRegs = 88;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
@@ -277,7 +279,7 @@ struct TileArgs {
     float *part_max, *part_sum;  // [M][2 tiles_n]
     float *z_target;             // [M]
     // Sum
-    float *out;       // rows that float4 stores fit
+    float *out;       // rows of 32-byte sectors
     int64_t out_rs;
     const int *out_map;
     int add;
@@ -389,40 +391,31 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// A warp's 32 rows x n columns from the lanes' registers to memory, 32 columns at a time
-// through `stage`: written as 16-byte chunks XOR-swizzled by the row, read back as four
-// rows of 128 bytes, so that a store covers whole lines.  `to`: where this lane's row begins,
-// null for a row that is not stored.
-__device__ __forceinline__ void store_rows(float *stage, const float (&acc)[128], float *to, int n, bool add) {
-    const int lane = threadIdx.x % 32;
-    float4 *s4 = reinterpret_cast<float4 *>(stage);
-    const unsigned long long mine = reinterpret_cast<unsigned long long>(to);
+__device__ __forceinline__ void store8(float *to, const float *v) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ void load8(const float *from, float (&v)[8]) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(from)
+                 : "memory");
+}
+
+// The first n of a lane's 128 columns to its row, whole sectors.
+__device__ __forceinline__ void store_row(float *to, float (&acc)[128], int n, bool add) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        if (c * 32 >= n) break;
-        __syncwarp();
+    for (int j = 0; j < 128; j += 8) {
+        if (j >= n) break;
+        if (add) {
+            float old[8];
+            load8(to + j, old);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            s4[lane * 8 + (j ^ (lane & 7))] =
-                make_float4(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3]);
-        __syncwarp();
-        const int j = lane % 8, col = c * 32 + 4 * j;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + lane / 8;
-            float *row = reinterpret_cast<float *>(__shfl_sync(0xFFFFFFFFu, mine, r));
-            float4 x = s4[r * 8 + (j ^ (r & 7))];
-            if (row == nullptr || col >= n) continue;
-            float4 *p = reinterpret_cast<float4 *>(row + col);
-            if (add) {
-                const float4 o = *p;
-                x.x += o.x;
-                x.y += o.y;
-                x.z += o.z;
-                x.w += o.w;
-            }
-            *p = x;
+            for (int k = 0; k < 8; ++k) acc[j + k] += old[k];
         }
+        store8(to + j, acc + j);
     }
 }
 
@@ -438,8 +431,8 @@ __device__ __forceinline__ void rescale(float (&acc)[128], float f0, float f1) {
 
 // The logits' epilogue: this lane's row, 128 columns from col0 on.  What most tiles do
 // not need (a ragged end, a bias, the target) is kept out of the loops of the others.
-__device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float (&acc)[128], float *stage, int64_t row,
-                                             int64_t col0, int part, float f0, float f1) {
+__device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float (&acc)[128], int64_t row, int64_t col0,
+                                             int part, float f0, float f1) {
     if (col0 >= a.N) return;
     const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
     const bool live = row < M;
@@ -476,21 +469,17 @@ __device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float
         a.part_max[row * 2 * a.tiles_n + part] = top[0];
         a.part_sum[row * 2 * a.tiles_n + part] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    if (a.z == nullptr) return;
-    // rows are padded to 64 columns: the last four of a ragged end may lie behind V
-    store_rows(stage, acc, live ? a.z + row * a.z_pitch + col0 : nullptr, n, false);
+    // rows are padded to 64 columns: the last sector of a ragged end may reach behind V
+    if (a.z != nullptr && live) store_row(a.z + row * a.z_pitch + col0, acc, n, false);
 }
 
-__device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&acc)[128], float *stage, int64_t row,
-                                          int64_t col0, int split, float f0, float f1) {
-    if (col0 >= a.N) return;
+__device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&acc)[128], int64_t row, int64_t col0,
+                                          int split, float f0, float f1) {
+    if (row >= M || col0 >= a.N) return;
     const int n = static_cast<int>(a.N - col0 < 128 ? a.N - col0 : 128);
     rescale(acc, f0, f1);
-    float *to = nullptr;
-    if (row < M)
-        to = a.parts != nullptr ? a.parts + (split * a.M + row) * a.parts_pitch + col0
-                                : a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0;
-    store_rows(stage, acc, to, n, a.add && a.parts == nullptr);
+    if (a.parts != nullptr) store_row(a.parts + (split * a.M + row) * a.parts_pitch + col0, acc, n, false);
+    else store_row(a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0, acc, n, a.add);
 }
 
 template <bool A_MN, bool B_MN, Out MODE>
@@ -501,8 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     // the same aligned offset in both CTAs (same dynamic size, same static layout)
     unsigned char *smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float *stage_out = reinterpret_cast<float *>(smem + kStages * kStageBytes);
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes + 8 * kStageOut);  // leader's: both CTAs' bytes
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes);  // leader's: both CTAs' bytes
     uint64_t *empty = full + kStages;    // each CTA's: the stage's MMAs are done (hi stages first, then lo)
     uint64_t *acc_full = empty + kStages;  // [2] each CTA's: a piece is in tensor memory
     uint64_t *acc_empty = acc_full + 2;    // [2] leader's: both epilogues have read it
@@ -545,7 +533,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     if (warp >= 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const int quadrant = warp % 4, half = (warp - 4) / 4;
-        float *stage = stage_out + (warp - 4) * (kStageOut / 4);
         const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
         const int scale = -(scale_exponent(*args.amax_a) + scale_exponent(*args.amax_b));
         const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
@@ -581,8 +568,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
             if (!ok) break;
             const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
             const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
-            if (MODE == Out::Logits) store_logits(args, e.M, acc, stage, row, col0, tn * 2 + half, f0, f1);
-            else store_sum(args, e.M, acc, stage, row, col0, split, f0, f1);
+            if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, f0, f1);
+            else store_sum(args, e.M, acc, row, col0, split, f0, f1);
             __syncwarp();
         }
         if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
@@ -944,6 +931,11 @@ int choose_splits(int64_t tiles, int64_t K, int64_t pairs, size_t bytes) {
     return best;
 }
 
+// Whether rows can be stored a 32-byte sector a time.
+bool sector_rows(const float *p, int64_t rs, int64_t cs, int64_t cols) {
+    return reinterpret_cast<uintptr_t>(p) % 32 == 0 && cs == 1 && rs % 8 == 0 && cols % 8 == 0;
+}
+
 bool vector_source(const float *p, int64_t rs, int64_t cs, int64_t cols) {
     return aligned16(p) && cs == 1 && rs % 4 == 0 && cols % 4 == 0;
 }
@@ -981,9 +973,9 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t row_stat = padded(static_cast<size_t>(piece) * 4);
     const size_t z_bytes = grads ? padded(static_cast<size_t>(piece) * pitch * 4) : 0;
     const size_t col_bytes = p.db != nullptr ? padded(static_cast<size_t>(piece / kGradRows) * pitch * 4) : 0;
-    const int64_t parts_pitch = (p.D + 3) / 4 * 4;
-    const bool parts_dx = splits_dx > 1 || !vector_source(p.dx, p.dx_rs, p.dx_cs, p.D);
-    const bool parts_dw = splits_dw > 1 || !vector_source(p.dw, p.dw_rs, p.dw_cs, p.D);
+    const int64_t parts_pitch = (p.D + 7) / 8 * 8;
+    const bool parts_dx = splits_dx > 1 || !sector_rows(p.dx, p.dx_rs, p.dx_cs, p.D);
+    const bool parts_dw = splits_dw > 1 || !sector_rows(p.dw, p.dw_rs, p.dw_cs, p.D);
     const size_t split_dx = p.dx != nullptr && parts_dx ? static_cast<size_t>(splits_dx) * piece * parts_pitch * 4 : 0;
     const size_t split_dw = p.dw != nullptr && parts_dw ? static_cast<size_t>(splits_dw) * p.V * parts_pitch * 4 : 0;
     const size_t split_bytes = grads ? padded(split_dx > split_dw ? split_dx : split_dw) : 0;

@@ -191,6 +191,40 @@ def test_embedding_gradient_of_a_single_token_and_of_nothing(cuda):
     assert (got == 3.0).all()
 
 
+def test_embedding_beyond_32_bits(cuda):
+    """A table of 4.7e9 elements: rows behind 2^32 elements are read, summed and cleared."""
+    import torch
+
+    vocab, dim = 2300000, 2048
+    table = torch.zeros(vocab, dim, device=cuda)
+    high = torch.tensor([vocab - 1, 5, vocab - 2, 2 ** 21, 2 ** 21 + 1, vocab - 1], device=cuda)
+    table[high] = torch.randn(6, dim, device=cuda)
+    out = torch.empty(6, dim, device=cuda)
+    abi.embedding(view(table), view(high), view(out), scale=2.0)
+    assert torch.equal(out, table[high] * 2.0)
+    for tok in (high, high.repeat(60)):  # with and without the sort
+        d = torch.randn(tok.numel(), dim, device=cuda)
+        table.fill_(3.0)
+        abi.embedding_grad(view(d), view(tok), view(table))
+        abi.check_device_errors(0)
+        for v in high.unique().tolist():
+            mine = d[tok == v].double()
+            within(table[v], mine.sum(0), (mine.shape[0] + 1) * U * 1.01 * mine.abs().sum(0) + 1e-45, f"row {v}")
+            table[v] = 0.0
+        assert not table.any()
+
+
+def test_embedding_of_one_scalar_token(cuda):
+    import torch
+
+    table, tok, out = torch.randn(9, 33, device=cuda), torch.tensor(4, device=cuda), torch.empty(33, device=cuda)
+    abi.embedding(view(table), view(tok), view(out), scale=0.5)
+    assert torch.equal(out, table[4] * 0.5)
+    grad = torch.empty(9, 33, device=cuda)
+    abi.embedding_grad(view(out), view(tok), view(grad), scale=2.0)
+    assert torch.equal(grad[4], out * 2.0) and grad.count_nonzero() == out.count_nonzero()
+
+
 def test_embedding_keeps_infinities_and_nan_to_their_rows(cuda):
     import torch
 
@@ -490,6 +524,74 @@ def test_each_gradient_alone_equals_all_together(cuda):
             kw = {{"dw": "dweight", "db": "dbias"}.get(name, name): view(out)}
             abi.linear_cross_entropy_grad(view(x), view(w), view(t), view(dloss), bias=view(b), ignore_target=IGNORE, **kw)
             assert torch.equal(out, all_[name]), name
+
+
+@pytest.mark.parametrize("n, vocab, dim", [(40, 90, 16), (6, 3000, 150), (3000, 12, 130), (400, 1700, 96)])
+@pytest.mark.parametrize("low", [-math.inf, -3.4028234663852886e38])
+def test_classes_masked_by_the_bias(cuda, n, vocab, dim, low):
+    """A bias of -inf, or of the type's lowest value, takes classes out, whole tiles of
+    them too: the results are those of the other classes alone, and the masked classes'
+    gradients are exact zeros."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 19, ignored=0.1)
+    masked = torch.rand(vocab, device=cuda) < 0.4
+    masked[: vocab // 2] = True
+    masked[vocab - 1] = False
+    rest = (~masked).nonzero().flatten()
+    pick = rest[torch.randint(0, rest.numel(), (n,), device=cuda)]
+    t = torch.where(t == IGNORE, t, pick)
+    bm = torch.where(masked, low, b)
+    got = run_ce(x, w, bm, t, dloss)
+    index = torch.full((vocab,), IGNORE, device=cuda)
+    index[rest] = torch.arange(rest.numel(), device=cuda)
+    tr = torch.where(t == IGNORE, t, index[t.clamp(min=0)])
+    want = ce_reference(x, w[rest], b[rest], tr, dloss)
+    extra = (vocab / 256 + 32) * 2 * U  # the sums run over all classes
+    for k in ("loss", "lse", "dx"):
+        scale = 1.0 if k != "dx" else (dloss.abs().max().double() * w.abs().max().double() * vocab)
+        within(got[k], want[k][0], want[k][1] + extra * scale, k)
+    within(got["dw"][rest], want["dw"][0], want["dw"][1] + extra * x.abs().sum(0).double() * dloss.abs().max(), "dw")
+    within(got["db"][rest], want["db"][0], want["db"][1] + extra * dloss.abs().sum(), "db")
+    assert (got["dw"][masked] == 0).all() and (got["db"][masked] == 0).all()
+
+
+def test_linear_cross_entropy_without_columns(cuda):
+    """D = 0: the logits are the bias."""
+    import torch
+
+    for n, vocab in ((30, 40), (3, 700), (500, 3000), (5000, 7)):
+        x, w, b, t, dloss = ce_data(n, vocab, 0, 23, ignored=0.1)
+        check_ce(x, w, b, t, dloss)
+        check_ce(x, w, None, t, None)
+
+
+def test_linear_cross_entropy_beyond_32_bits(cuda):
+    """A weight of 2.2e9 elements: the loss and sampled rows of its gradient against
+    float64, on classes at the end of the vocabulary."""
+    import torch
+
+    n, vocab, dim = 260, 700000, 3200
+    g = torch.Generator(device="cuda").manual_seed(70)
+    w = torch.randn(vocab, dim, device=cuda, generator=g).mul_(0.02)
+    x = torch.randn(n, dim, device=cuda, generator=g)
+    t = torch.randint(vocab - 3000, vocab, (n,), device=cuda, generator=g)
+    dloss = torch.full((n,), 1.0 / n, device=cuda)
+    loss, dw = torch.empty(n, device=cuda), torch.empty_like(w)
+    abi.linear_cross_entropy_grad(view(x), view(w), view(t), view(dloss), dweight=view(dw), loss=view(loss))
+    abi.check_device_errors(0)
+    z = torch.cat([x.double() @ w[i: i + 50000].double().t() for i in range(0, vocab, 50000)], 1)
+    lse = torch.logsumexp(z, 1)
+    want = lse - z.gather(1, t.unsqueeze(1)).squeeze(1)
+    size = (x.double().abs() @ w[t].double().abs().t()).max() * 1.5  # sums of |x||w| vary little
+    bound = 2 * product_bound(dim, size) + (vocab / 256 + 32) * 2 * U + 30 * U
+    within(loss, want, torch.full_like(want, float(bound)), "loss")
+    rows = torch.cat([t[:20], torch.tensor([0, vocab // 2, vocab - 1], device=cuda)])
+    p = torch.exp(z[:, rows] - lse.unsqueeze(1)) - (t.unsqueeze(1) == rows).double()
+    ref = (p * dloss.unsqueeze(1).double()).t() @ x.double()
+    tol = ((p.abs() * (2 * float(bound) + 16 * U) + 2.0 ** -40) * dloss.unsqueeze(1).double()).t() @ x.double().abs()
+    tol = tol + product_bound(n, (p.abs() * dloss.unsqueeze(1).double()).t() @ x.double().abs())
+    within(dw[rows], ref, tol, "dw")
 
 
 # ------------------------------------------------------------------ clipping --
