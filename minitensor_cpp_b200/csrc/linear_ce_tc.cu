@@ -95,6 +95,7 @@ struct PackSource {
     __half *to;       // [rows_out][blocks][2][64]
     int64_t rows_out; // with zero rows behind the live ones, up to a multiple of 64
     int *amax;
+    FastDiv blocks;   // of a row
 };
 
 struct PackArgs {
@@ -221,6 +222,7 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     const int lane = threadIdx.x % 16;
     constexpr int U = 4;
     const int64_t total = rows_out * blocks;
+    const bool narrow = total < (int64_t{1} << 32);  // a 64-bit division a block costs as much as its bytes
     for (int64_t i0 = block * 16 * U + threadIdx.x / 16; i0 < total; i0 += grid * 16 * U) {
         float4 v[U];
 #pragma unroll
@@ -228,7 +230,8 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
             const int64_t i = i0 + u * 16;
             v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (i >= total) continue;
-            const int64_t r = i / blocks, c = (i - r * blocks) * kBlock + lane * 4;
+            const int64_t r = narrow ? fastdiv(static_cast<uint32_t>(i), s.blocks) : i / blocks;
+            const int64_t c = (i - r * blocks) * kBlock + lane * 4;
             if (r >= rows || c >= s.cols) continue;
             const float *src = source_row(s, r);
             if (s.vec) {
@@ -1006,6 +1009,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
                         xp, rows_all, live.count + 1};
     k.s[1] = PackSource{p.w, p.w_rs, p.w_cs, p.V, p.D, nullptr, nullptr, vector_source(p.w, p.w_rs, p.w_cs, p.D),
                         wp, p.V, live.count + 2};
+    k.s[0].blocks = k.s[1].blocks = make_fastdiv(static_cast<uint32_t>(d_blocks > 0 ? d_blocks : 1));
     if (grads) k.dloss = live.dloss;
     if (p.dx != nullptr && p.D > 0) k.dx = p.dx;
     k.dx_rs = p.dx_rs;
