@@ -37,7 +37,8 @@ struct FewArgs {
     Side few, many;
     int vec, grad_vec;   // float4 access to the many, to their gradient
     int d_pad;           // a row of the few in shared memory, a multiple of 128
-    float *z;            // few rows: the logits [N][V]; few classes: g [N][R]; null: not wanted
+    float *z;            // few rows: the logits [N][V]; null: not wanted
+    float *g;            // [many][R]
     Softmax *parts;      // [CTAs][R]
     int n_parts;
     float *z_target;     // [R]
@@ -178,12 +179,12 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
                     if (p.loss != nullptr) p.loss[n * p.loss_s] = t < 0 ? 0.0f : lse - zt;
                     if (p.lse != nullptr) p.lse[n * p.lse_s] = t < 0 ? 0.0f : lse;
                 }
-                if (a.z != nullptr && in) {
+                if (a.g != nullptr && in) {
                     const float d = t < 0 ? 0.0f : p.dloss[n * p.dl_s];
 #pragma unroll
                     for (int k = 0; k < kMine; ++k) {
                         const int v = lane / 4 + 8 * k;
-                        if (v < R) a.z[n * R + v] = t < 0 || v >= p.V ? 0.0f : softmax_grad(z[k], lse, d, v == t);
+                        if (v < R) a.g[n * R + v] = t < 0 || v >= p.V ? 0.0f : softmax_grad(z[k], lse, d, v == t);
                     }
                 }
             } else {
@@ -254,25 +255,66 @@ __global__ void __launch_bounds__(32 * kFewRows) k_few_loss(const LinearCe p, co
     if (threadIdx.x % 32 == 0) store_loss(p, a, n, row_target(p, n, a.err, false), lse);
 }
 
-// C columns a lane, 32 C a CTA.
+// With eight rows or more the exponentials are worth a pass of their own: z [N][V] -> g [V][R],
+// instead of once for each slab of columns in k_few_grad.  The loss and the bias gradient with it.
+constexpr bool g_before(int R, bool classes) { return classes || R >= 8; }
+
+template <int R>
+__global__ void __launch_bounds__(kFewThreads) k_few_g(const LinearCe p, const FewArgs a) {
+    wait_for_previous();
+    __shared__ float lse[R], dloss[R];
+    __shared__ int target[R];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int n = warp; n < R; n += kFewThreads / 32) {
+        const int t = n < p.N ? row_target(p, n, a.err, false) : -1;
+        const float l = n < p.N ? few_lse(a, R, n) : 0.0f;
+        if (lane == 0) {
+            lse[n] = l;
+            target[n] = t;
+            dloss[n] = t >= 0 ? p.dloss[n * p.dl_s] : 0.0f;
+            if (n < p.N && blockIdx.x == 0) store_loss(p, a, n, t, l);
+        }
+    }
+    __syncthreads();
+    for (int64_t v = static_cast<int64_t>(blockIdx.x) * kFewThreads + threadIdx.x; v < p.V;
+         v += static_cast<int64_t>(gridDim.x) * kFewThreads) {
+        float g[R], sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < R; ++n) g[n] = n < p.N ? a.z[n * p.V + v] : 0.0f;
+#pragma unroll
+        for (int n = 0; n < R; ++n) {
+            g[n] = target[n] >= 0 ? softmax_grad(g[n], lse[n], dloss[n], v == target[n]) : 0.0f;
+            sum += g[n];
+        }
+        if (p.db != nullptr) p.db[v * p.db_s] = sum;
+#pragma unroll
+        for (int n = 0; n < R; ++n) a.g[v * R + n] = g[n];
+    }
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+// C columns a lane, 32 C a CTA.  Two columns a multiply-add (FFMA2); g lies in shared memory
+// twice over, as its operand wants it.
 template <int R, int C, bool CLASSES>
 __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const LinearCe p, const FewArgs a) {
     wait_for_previous();
     __shared__ float lse[R], dloss[R];
     __shared__ int target[R];
-    __shared__ float sums[kFewThreads / 32][32 * C];
-    __shared__ __align__(16) float gs[kFewThreads / 32][32][R];  // of a warp's 32 of the many
+    __shared__ __align__(16) float sums[kFewThreads / 32][32 * C];
+    __shared__ __align__(16) float2 gs[kFewThreads / 32][32][R + 2];  // of a warp's 32 of the many; a lane's row off the banks of the next
     __shared__ bool live[kFewThreads / 32][32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    constexpr bool kBefore = g_before(R, CLASSES);
     if (!CLASSES) {
         for (int n = warp; n < R; n += kFewThreads / 32) {
             const int t = n < p.N ? row_target(p, n, a.err, false) : -1;
-            const float l = n < p.N ? few_lse(a, R, n) : 0.0f;
+            const float l = !kBefore && n < p.N ? few_lse(a, R, n) : 0.0f;
             if (lane == 0) {
                 lse[n] = l;
                 target[n] = t;
                 dloss[n] = t >= 0 ? p.dloss[n * p.dl_s] : 0.0f;
-                if (n < p.N && blockIdx.x == 0 && blockIdx.y == 0) store_loss(p, a, n, t, l);
+                if (!kBefore && n < p.N && blockIdx.x == 0 && blockIdx.y == 0) store_loss(p, a, n, t, l);
             }
         }
         __syncthreads();
@@ -281,15 +323,18 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const 
     const int64_t c0 = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * C;
     const int cols = static_cast<int>(p.D - c0 < 0 ? 0 : p.D - c0 < C ? p.D - c0 : C);
     const bool few_grad = a.few_parts != nullptr;
-    float x[R][C], dx[R][C], db[R];
+    float2 x[R][C / 2], dx[R][C / 2];
+    float db[R];
 #pragma unroll
     for (int n = 0; n < R; ++n) {
         db[n] = 0.0f;
+        const float *row = a.few.p + n * a.few.rs + c0 * a.few.cs;
+        const bool has = n < a.few.rows && (CLASSES || target[n] >= 0);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            dx[n][c] = 0.0f;
-            x[n][c] = n < a.few.rows && c < cols && (CLASSES || target[n] >= 0)
-                          ? a.few.p[n * a.few.rs + (c0 + c) * a.few.cs] : 0.0f;
+        for (int c = 0; c < C / 2; ++c) {
+            dx[n][c] = make_float2(0.0f, 0.0f);
+            x[n][c].x = has && 2 * c < cols ? row[2 * c * a.few.cs] : 0.0f;
+            x[n][c].y = has && 2 * c + 1 < cols ? row[(2 * c + 1) * a.few.cs] : 0.0f;
         }
     }
     const int64_t step = static_cast<int64_t>(gridDim.y) * (kFewThreads / 32) * 32;
@@ -301,77 +346,77 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const 
 #pragma unroll
         for (int n = 0; n < R; ++n) {
             float g = 0.0f;
-            if (CLASSES) {
-                if (v < m.rows) g = a.z[v * R + n];
+            if (kBefore) {
+                if (v < m.rows) g = a.g[v * R + n];
                 any |= g != 0.0f;
-                db[n] += g;
+                if (CLASSES) db[n] += g;
             } else {
                 if (n < p.N && v < p.V && target[n] >= 0) g = softmax_grad(a.z[n * p.V + v], lse[n], dloss[n], v == target[n]);
                 sum += g;
             }
-            gs[warp][lane][n] = g;
+            gs[warp][lane][n] = make_float2(g, g);
         }
         if (CLASSES) live[warp][lane] = any;
         __syncwarp();
-        if (!CLASSES && p.db != nullptr && blockIdx.x == 0 && v < p.V) p.db[v * p.db_s] = sum;
+        if (!kBefore && p.db != nullptr && blockIdx.x == 0 && v < p.V) p.db[v * p.db_s] = sum;
         const int count = static_cast<int>(m.rows - v0 < 32 ? m.rows - v0 : 32);
-        constexpr int U = 8;
+        constexpr int U = R <= 4 ? 8 : 4;
         for (int j0 = 0; j0 < count; j0 += U) {
-            float w[U][C];
+            float2 w[U][C / 2];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) w[u][c] = 0.0f;
+                for (int c = 0; c < C / 2; ++c) w[u][c] = make_float2(0.0f, 0.0f);
                 if (!few_grad || j0 + u >= count || (CLASSES && !live[warp][j0 + u])) continue;
                 const float *src = m.p + (v0 + j0 + u) * m.rs + c0 * m.cs;
                 if (a.vec) {
                     if (cols <= 0) continue;
                     if (C == 4) {
                         const float4 y = __ldcs(reinterpret_cast<const float4 *>(src));
-                        w[u][C - 1] = y.w;
-                        w[u][2 % C] = y.z;
-                        w[u][1] = y.y;
-                        w[u][0] = y.x;
+                        w[u][C / 2 - 1] = make_float2(y.z, y.w);
+                        w[u][0] = make_float2(y.x, y.y);
                     } else {
-                        const float2 y = __ldcs(reinterpret_cast<const float2 *>(src));
-                        w[u][0] = y.x;
-                        w[u][1] = y.y;
+                        w[u][0] = __ldcs(reinterpret_cast<const float2 *>(src));
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        if (c < cols) w[u][c] = __ldcs(src + c * m.cs);
+                    for (int c = 0; c < C / 2; ++c) {
+                        if (2 * c < cols) w[u][c].x = __ldcs(src + 2 * c * m.cs);
+                        if (2 * c + 1 < cols) w[u][c].y = __ldcs(src + (2 * c + 1) * m.cs);
+                    }
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (j0 + u >= count) break;
-                float dm[C];
+                float2 dm[C / 2];
 #pragma unroll
-                for (int c = 0; c < C; ++c) dm[c] = 0.0f;
+                for (int c = 0; c < C / 2; ++c) dm[c] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int n = 0; n < R; ++n) {
-                    const float gn = gs[warp][j0 + u][n];
+                    const float2 gn = gs[warp][j0 + u][n];
 #pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        dx[n][c] = fmaf(gn, w[u][c], dx[n][c]);
-                        dm[c] = fmaf(gn, x[n][c], dm[c]);
+                    for (int c = 0; c < C / 2; ++c) {
+                        dx[n][c] = fma2(gn, w[u][c], dx[n][c]);
+                        dm[c] = fma2(gn, x[n][c], dm[c]);
                     }
                 }
                 if (m.grad == nullptr) continue;
                 if (CLASSES && !live[warp][j0 + u]) {  // W may hold infinities; the row has no loss
 #pragma unroll
-                    for (int c = 0; c < C; ++c) dm[c] = 0.0f;
+                    for (int c = 0; c < C / 2; ++c) dm[c] = make_float2(0.0f, 0.0f);
                 }
                 float *to = m.grad + (v0 + j0 + u) * m.g_rs + c0 * m.g_cs;
                 if (a.grad_vec) {
                     if (cols <= 0) continue;
-                    if (C == 4) *reinterpret_cast<float4 *>(to) = make_float4(dm[0], dm[1], dm[2 % C], dm[3 % C]);
-                    else *reinterpret_cast<float2 *>(to) = make_float2(dm[0], dm[1]);
+                    if (C == 4) *reinterpret_cast<float4 *>(to) = make_float4(dm[0].x, dm[0].y, dm[C / 2 - 1].x, dm[C / 2 - 1].y);
+                    else *reinterpret_cast<float2 *>(to) = dm[0];
                 } else {
 #pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        if (c < cols) to[c * m.g_cs] = dm[c];
+                    for (int c = 0; c < C / 2; ++c) {
+                        if (2 * c < cols) to[2 * c * m.g_cs] = dm[c].x;
+                        if (2 * c + 1 < cols) to[(2 * c + 1) * m.g_cs] = dm[c].y;
+                    }
                 }
             }
         }
@@ -382,7 +427,7 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const 
         if (n >= a.few.rows) break;
         __syncthreads();
 #pragma unroll
-        for (int c = 0; c < C; ++c) sums[warp][lane * C + c] = dx[n][c];
+        for (int c = 0; c < C / 2; ++c) *reinterpret_cast<float2 *>(&sums[warp][lane * C + 2 * c]) = dx[n][c];
         __syncthreads();
         float *part = a.few_parts + (blockIdx.y * a.few.rows + n) * (p.D + 1);
         if (static_cast<int>(threadIdx.x) < 32 * C) {
@@ -447,22 +492,26 @@ int few_path(const LinearCe &p, FewArgs a, cudaStream_t stream) {
     a.n_parts = static_cast<int>(wanted < most_ctas ? wanted : most_ctas);  // every SM as many: a CTA loads the few once
     constexpr int C = R <= 8 ? 4 : 2;  // columns a lane of k_few_grad: 2 R C values in registers
     const int64_t slabs = p.D > 0 ? (p.D + 32 * C - 1) / (32 * C) : 1;
-    const int64_t splits = (static_cast<int64_t>(sms) * 4 + slabs - 1) / slabs;
+    // two full waves of CTAs, two of which fill an SM
+    const int64_t splits = static_cast<int64_t>(sms) * 4 / slabs > 0 ? static_cast<int64_t>(sms) * 4 / slabs : 1;
     const int64_t most = (m.rows + 255) / 256;  // 8 warps of 32
     a.splits = static_cast<int>(splits < most ? splits : most);
     const bool few_grad = grads && (a.few.grad != nullptr || (CLASSES && p.db != nullptr));
     const size_t parts = padded(static_cast<size_t>(a.n_parts) * R * sizeof(Softmax));
-    const size_t zs = grads ? padded(static_cast<size_t>(m.rows) * (CLASSES ? R : p.N) * 4) : 0;
+    const size_t zs = grads && !CLASSES ? padded(static_cast<size_t>(m.rows) * p.N * 4) : 0;
+    const size_t gs = grads && g_before(R, CLASSES) ? padded(static_cast<size_t>(m.rows) * R * 4) : 0;
     const size_t fs = few_grad ? padded(static_cast<size_t>(a.splits) * a.few.rows * (p.D + 1) * 4) : 0;
     MTC_TRY(device_error_word(&a.err));
     Workspace ws;
     if (!CLASSES || grads) {
-        MTC_TRY(ws.allocate(256 + parts + zs + fs, stream));
+        MTC_TRY(ws.allocate(256 + parts + zs + gs + fs, stream));
         a.z_target = ws.take<float>(256);
         a.parts = ws.take<Softmax>(parts);
         float *z = ws.take<float>(zs);
+        float *g = ws.take<float>(gs);
         float *f = ws.take<float>(fs);
-        a.z = grads ? z : nullptr;
+        a.z = zs > 0 ? z : nullptr;
+        a.g = gs > 0 ? g : nullptr;
         a.few_parts = few_grad ? f : nullptr;
     }
     if (a.vec) {
@@ -475,11 +524,20 @@ int few_path(const LinearCe &p, FewArgs a, cudaStream_t stream) {
     MTC_TRY(check_launch("linear cross entropy (few)"));
     if (!grads) {
         if (CLASSES) return MTC_OK;
-        return launch_dependent("linear cross entropy (loss)", k_few_loss, 1, static_cast<unsigned>(32 * p.N), 0, stream, p, a, R);
+        return launch_dependent("linear cross entropy (loss)", k_few_loss, 1, static_cast<unsigned>(32 * p.N), 0, stream,
+                                p, a, R);
     }
-    MTC_TRY((launch_dependent("linear cross entropy (few, gradients)", k_few_grad<R, C, CLASSES>, dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(a.splits)), kFewThreads, 0, stream, p, a)));
+    if constexpr (!CLASSES && g_before(R, CLASSES)) {
+        const int64_t ctas = (p.V + kFewThreads - 1) / kFewThreads;
+        MTC_TRY(launch_dependent("linear cross entropy (few, gradient of the logits)", k_few_g<R>,
+                                 static_cast<unsigned>(ctas < sms * 4 ? ctas : sms * 4), kFewThreads, 0, stream, p, a));
+    }
+    const dim3 grid(static_cast<unsigned>(slabs), static_cast<unsigned>(a.splits));
+    MTC_TRY((launch_dependent("linear cross entropy (few, gradients)", k_few_grad<R, C, CLASSES>, grid, kFewThreads, 0,
+                              stream, p, a)));
     if (!few_grad) return MTC_OK;
-    return launch_dependent("linear cross entropy (few, join)", k_few_join<CLASSES>, static_cast<unsigned>((a.few.rows * (p.D + 1) + 31) / 32), 256, 0, stream, p, a);
+    return launch_dependent("linear cross entropy (few, join)", k_few_join<CLASSES>,
+                            static_cast<unsigned>((a.few.rows * (p.D + 1) + 31) / 32), 256, 0, stream, p, a);
 }
 
 template <bool CLASSES>
