@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kListThreads) k_live_rows(const LinearCe p, co
     }
     if (me == 0 && threadIdx.x == 0) {
         live.count[0] = all;
-        live.count[1] = live.count[2] = live.count[3] = 0;
+        for (int i = 1; i < kLiveKnown; ++i) live.count[i] = 0;
     }
     cluster.sync();  // nobody leaves while its count is read
 }

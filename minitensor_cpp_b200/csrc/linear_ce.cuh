@@ -26,8 +26,9 @@ struct LinearCe {
 };
 
 // What the device knows about the rows that have a loss.
+constexpr int kLiveKnown = 9;
 struct LiveRows {
-    int *count;      // [1], and behind it the largest finite |x|, |weight| and |dloss| as bits [3], zeroed with it
+    int *count;      // [1], and behind it what the tensor-core path learns of the magnitudes, zeroed with it
     int *row;        // [N] the row of x; behind them, from the end backwards, the rows without a loss
     int *target;     // [N]
     float *dloss;    // [N]

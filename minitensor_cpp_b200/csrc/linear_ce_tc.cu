@@ -1,10 +1,17 @@
 // Linear cross entropy on the tensor cores, with float32 accuracy.
 //
 // A float32 operand becomes a pair of 16-bit floats.  Scaled by a power of two that
-// brings the largest finite magnitude of its tensor to [2^14, 2^15), x is kept as
+// brings the largest finite magnitude of its tensor to [2^8, 2^15), x is kept as
 //   hi = f16(x),  lo = f16((x - hi) * 2^11),   x = hi + lo * 2^-11 within 2^-22 |x|
-// for every |x| down to 2^-29 of the largest, and within 2^-51 of the largest below
+// for every |x| down to 2^-23 of the largest, and within 2^-45 of the largest below
 // (f16 ends at 2^-24, so an unscaled lo would end there; scaled, lo reaches 2^-35).
+// The scale comes from a sample of the rows with 2^6 to spare, so that the packing reads
+// the tensor once; it finds the largest magnitude on its way, and where that does not fit
+// after all, a second packing with its own scale follows (k_pack<true>, which otherwise
+// returns at once).  Against a pass of its own for the maximum: 64 rows, 131072 columns
+// of length 2048: 839 -> 684 us for the loss; 16384 rows, 32000 columns of length 1024:
+// 2636 -> 2585 us; within the noise where the products take most of the time.  Up to 1184
+// rows of either tensor are all in the sample, which then is the largest magnitude.
 // A product is three MMAs, hi.lo + lo.hi first and then hi.hi:
 //   a.b = hi.hi + 2^-11 (hi.lo + lo.hi)          (lo.lo is below 2^-22)
 // with the 2^-11 applied by the MMA itself (scale-input-d) when hi.hi is added.  f16
@@ -85,6 +92,10 @@ __device__ __forceinline__ void split_pair(float x, __half &hi, __half &lo) {
     lo = __float2half_rn((x - __half2float(hi)) * 2048.0f);
 }
 
+// What the device knows of the scales, behind the count of the live rows.
+enum Known { kLargest = 1, kSampled = 4, kExponent = 6 };  // of x, weight (and of dloss: kLargest, kExponent)
+static_assert(kExponent + 3 == kLiveKnown, "zeroed with the count");
+
 struct PackSource {
     const float *p;
     int64_t rs, cs;
@@ -94,16 +105,16 @@ struct PackSource {
     int vec;          // float4 loads
     __half *to;       // [rows_out][blocks][2][64]
     int64_t rows_out; // with zero rows behind the live ones, up to a multiple of 64
-    int *amax;
+    int which;        // 0: x, 1: weight
     FastDiv blocks;   // of a row
 };
 
 struct PackArgs {
     PackSource s[2];
     int64_t first_of_second;  // blocks of the grid before the second tensor
+    int *known;               // the live rows' count and what follows it
+    int headroom;             // powers of two above the sample; 0: it is the whole
     const float *dloss;       // its largest magnitude too; null: none
-    int *dloss_amax;
-    const int *dloss_count;
     float *dx;                // its rows without a loss become zero; null: not wanted
     int64_t dx_rs, dx_cs;
     int dx_vec;
@@ -135,9 +146,24 @@ __device__ __forceinline__ const float *source_row(const PackSource &s, int64_t 
     return s.p + (s.map != nullptr ? s.map[r] : r) * s.rs;
 }
 
-// Largest finite magnitudes of x (rows with a loss), weight and dloss, and the zero rows of
-// dx.  Each warp takes rows in turn, four 16-byte loads in flight a lane, or sixteen of 4.
-__global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
+// The scale of the first packing: the sampled maximum to [2^8, 2^9).
+__device__ __forceinline__ int first_exponent(const PackArgs &a, int which) {
+    const int sampled = a.known[kSampled + which];
+    return sampled == 0 ? 0 : scale_exponent(sampled) - a.headroom;
+}
+
+// And the one that counts: the same, unless the largest magnitude needs a smaller one (or
+// the sample was all zeros).
+__device__ __forceinline__ int last_exponent(const PackArgs &a, int which) {
+    const int exact = scale_exponent(a.known[kLargest + which]);
+    if (a.known[kSampled + which] == 0) return exact;
+    const int first = first_exponent(a, which);
+    return first < exact ? first : exact;
+}
+
+// Largest finite magnitudes of x (rows with a loss) and weight over a sample of the rows, one
+// a warp, and of dloss; the zero rows of dx.
+__global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     wait_for_previous();
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
@@ -146,8 +172,9 @@ __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
     const int lane = threadIdx.x % 32;
     float m0 = 0.0f, m1 = 0.0f;
     const int64_t rows = source_rows(s);
-    for (int64_t r = block * 8 + threadIdx.x / 32; r < rows; r += blocks * 8) {
-        const float *src = source_row(s, r);
+    const int64_t warp_at = block * 8 + threadIdx.x / 32, warps = blocks * 8;
+    if (warp_at < rows) {
+        const float *src = source_row(s, rows > warps ? warp_at * rows / warps : warp_at);
         if (s.vec) {
             const float4 *v4 = reinterpret_cast<const float4 *>(src);
             const int n4 = static_cast<int>(s.cols / 4);
@@ -186,7 +213,7 @@ __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
             for (int u = 0; u < 16; ++u) m0 = fmaxf(m0, finite_abs(v[u]));
         }
     }
-    keep_max(fmaxf(m0, m1), s.amax);
+    keep_max(fmaxf(m0, m1), a.known + kSampled + s.which);
     if (a.dx != nullptr) {
         const PackSource &x = a.s[0];
         const int64_t dead = x.rows - source_rows(x);
@@ -202,14 +229,20 @@ __global__ void __launch_bounds__(256) k_largest(const PackArgs a) {
     }
     if (a.dloss != nullptr && blockIdx.x == 0) {
         float m = 0.0f;
-        for (int i = threadIdx.x; i < *a.dloss_count; i += 256) m = fmaxf(m, finite_abs(a.dloss[i]));
-        keep_max(m, a.dloss_amax);
+        for (int i = threadIdx.x; i < a.known[0]; i += 256) m = fmaxf(m, finite_abs(a.dloss[i]));
+        keep_max(m, a.known + kLargest + 2);
     }
 }
 
-// Each half-warp packs one block of 64 columns at a time: a lane four columns.
+// Each half-warp packs one block of 64 columns at a time: a lane four columns.  AGAIN: only
+// the tensors whose scale was wrong; and the exponents are written down.
+template <bool AGAIN>
 __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     wait_for_previous();
+    if ((AGAIN || a.headroom == 0) && blockIdx.x == 0 && threadIdx.x < 3)
+        a.known[kExponent + threadIdx.x] = threadIdx.x == 2 ? scale_exponent(a.known[kLargest + 2])
+                                           : AGAIN          ? last_exponent(a, threadIdx.x)
+                                                            : first_exponent(a, threadIdx.x);
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
     const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
@@ -217,9 +250,11 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     const int64_t blocks = (s.cols + kBlock - 1) / kBlock;
     const int64_t rows = source_rows(s);
     const int64_t rows_out = s.live != nullptr && (rows + 63) / 64 * 64 < s.rows_out ? (rows + 63) / 64 * 64 : s.rows_out;
-    const int e = scale_exponent(*s.amax);
+    const int e = AGAIN ? last_exponent(a, s.which) : first_exponent(a, s.which);
+    if (AGAIN && (e == first_exponent(a, s.which) || a.known[kLargest + s.which] == 0)) return;
     const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
     const int lane = threadIdx.x % 16;
+    float largest = 0.0f;
     constexpr int U = 4;
     const int64_t total = rows_out * blocks;
     const bool narrow = total < (int64_t{1} << 32);  // a 64-bit division a block costs as much as its bytes
@@ -247,6 +282,9 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
         for (int u = 0; u < U; ++u) {
             const int64_t i = i0 + u * 16;
             if (i >= total) continue;
+            if (!AGAIN && a.headroom != 0)
+                largest = fmaxf(largest, fmaxf(fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)),
+                                               fmaxf(finite_abs(v[u].z), finite_abs(v[u].w))));
             __half h[4], l[4];
             split_pair(v[u].x * f0 * f1, h[0], l[0]);
             split_pair(v[u].y * f0 * f1, h[1], l[1]);
@@ -257,6 +295,7 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
             *reinterpret_cast<uint2 *>(to + kBlock) = *reinterpret_cast<const uint2 *>(l);
         }
     }
+    if (!AGAIN && a.headroom != 0) keep_max(largest, a.known + kLargest + s.which);
 }
 
 // ---------------------------------------------------------------- products --
@@ -271,7 +310,7 @@ struct TileArgs {
     int tiles_n;
     int group;        // row tiles that share a sweep of the columns
     int splits;       // of K
-    const int *amax_a, *amax_b;
+    const int *exp_a, *exp_b;  // exponents of the operands' scales
     unsigned long long *err;
     // Logits
     float *z;         // [M][z_pitch], null: statistics alone
@@ -537,7 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const int quadrant = warp % 4, half = (warp - 4) / 4;
         const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
-        const int scale = -(scale_exponent(*args.amax_a) + scale_exponent(*args.amax_b));
+        const int scale = -(*args.exp_a + *args.exp_b);
         const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
         const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
         int64_t piece = 0;
@@ -793,7 +832,7 @@ struct GradArgs {
     const float *lse_live;
     const int *target;
     const float *dloss;
-    const int *amax;     // of dloss
+    const int *exponent; // of the scale of g'
     float *column_parts; // [row blocks][pitch] column sums of g; null: not wanted
 };
 
@@ -809,7 +848,7 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + lane * 4;
     const bool in = c < a.pitch;
-    const int e = scale_exponent(*a.amax);
+    const int e = *a.exponent;
     const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
     float4 column = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -1006,25 +1045,31 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     PackArgs k;
     std::memset(&k, 0, sizeof(k));
     k.s[0] = PackSource{p.x, p.x_rs, p.x_cs, p.N, p.D, live.row, live.count, vector_source(p.x, p.x_rs, p.x_cs, p.D),
-                        xp, rows_all, live.count + 1};
+                        xp, rows_all, 0, {}};
     k.s[1] = PackSource{p.w, p.w_rs, p.w_cs, p.V, p.D, nullptr, nullptr, vector_source(p.w, p.w_rs, p.w_cs, p.D),
-                        wp, p.V, live.count + 2};
+                        wp, p.V, 1, {}};
     k.s[0].blocks = k.s[1].blocks = make_fastdiv(static_cast<uint32_t>(d_blocks > 0 ? d_blocks : 1));
     if (grads) k.dloss = live.dloss;
     if (p.dx != nullptr && p.D > 0) k.dx = p.dx;
     k.dx_rs = p.dx_rs;
     k.dx_cs = p.dx_cs;
     k.dx_vec = vector_source(p.dx, p.dx_rs, p.dx_cs, p.D);
-    k.dloss_amax = live.count + 3;
-    k.dloss_count = live.count;
+    k.known = live.count;
     // CTAs in proportion to the tensors' rows, eight to an SM in all
     const int64_t most = static_cast<int64_t>(sms) * 8;
     const int64_t share = most * p.N / (p.N + p.V);
     k.first_of_second = share < 1 ? 1 : share > most - 1 ? most - 1 : share;
-    MTC_TRY((launch_dependent("linear cross entropy (magnitudes)", k_largest, static_cast<unsigned>(most), 256, 0, stream, k)));
-    if (p.D > 0) {
-        MTC_TRY((launch_dependent("linear cross entropy (packing)", k_pack, static_cast<unsigned>(most), 256, 0, stream, k)));
+    const unsigned ctas = static_cast<unsigned>(most);
+    {
+        PackArgs few = k;  // a quarter of the CTAs, half of them each
+        few.first_of_second = sms;
+        MTC_TRY(launch_dependent("linear cross entropy (sample)", k_sample, static_cast<unsigned>(2 * sms), 256, 0, stream, few));
     }
+    const int64_t sample = 8 * sms;
+    k.headroom = p.N <= sample && p.V <= sample ? 0 : 6;
+    MTC_TRY(launch_dependent("linear cross entropy (packing)", k_pack<false>, ctas, 256, 0, stream, k));
+    if (k.headroom != 0)
+        MTC_TRY(launch_dependent("linear cross entropy (packing again)", k_pack<true>, ctas, 256, 0, stream, k));
 
     CUtensorMap x_k, w_k, w_mn, x_mn, g_k, g_mn;
     const int64_t map_blocks = d_blocks > 0 ? d_blocks : 1;
@@ -1044,8 +1089,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         t.tiles_n = tiles_v;
         t.group = 16;
         t.splits = 1;
-        t.amax_a = live.count + 1;
-        t.amax_b = live.count + 2;
+        t.exp_a = live.count + kExponent;
+        t.exp_b = live.count + kExponent + 1;
         t.err = err;
         t.z = grads ? z : nullptr;
         t.z_pitch = pitch;
@@ -1061,7 +1106,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
                          z_target, live.row, lse_live, p.loss, p.lse, p.loss_s, p.lse_s};
         MTC_TRY((launch_dependent("linear cross entropy (loss)", k_row_loss, static_cast<unsigned>((rows + 7) / 8), 256, 0, stream, ra)));
         if (!grads) continue;
-        const GradArgs ga{first, rows_up, live.count, p.V, z, pitch, lse_live, live.target, live.dloss, live.count + 3,
+        const GradArgs ga{first, rows_up, live.count, p.V, z, pitch, lse_live, live.target, live.dloss, live.count + kExponent + 2,
                           p.db != nullptr ? columns : nullptr};
         const dim3 grid(static_cast<unsigned>((pitch + 127) / 128), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
         MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, 256, 0, stream, ga)));
@@ -1081,8 +1126,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.tiles_n = tiles_d;
             t.group = 16;
             t.splits = splits_dx;
-            t.amax_a = live.count + 3;
-            t.amax_b = live.count + 2;
+            t.exp_a = live.count + kExponent + 2;
+            t.exp_b = live.count + kExponent + 1;
             t.err = err;
             t.out = p.dx;
             t.out_rs = p.dx_rs;
@@ -1108,8 +1153,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.tiles_n = tiles_d;
             t.group = 16;
             t.splits = splits_dw;
-            t.amax_a = live.count + 3;
-            t.amax_b = live.count + 1;
+            t.exp_a = live.count + kExponent + 2;
+            t.exp_b = live.count + kExponent;
             t.err = err;
             t.out = p.dw;
             t.out_rs = p.dw_rs;

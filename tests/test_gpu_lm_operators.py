@@ -444,6 +444,22 @@ def test_scales_far_from_one(cuda, n, vocab, dim, sx, sw):
     check_ce(x, w, b, t, dloss * 1e-30)
 
 
+def test_scales_that_a_sample_misses(cuda):
+    """A few rows far larger than the others, or all others zero: the scale of the 16-bit
+    pairs is that of the largest all the same."""
+    x, w, b, t, dloss = ce_data(3000, 2500, 80, 24)
+    big = x.clone()
+    big[1] *= 3e4
+    check_ce(big * 1e-3, w, b, t, dloss)
+    wide = w.clone()
+    wide[3], wide[2401] = wide[3] * 1e3, wide[2401] * 300.0
+    check_ce(x * 1e-2, wide, b, t, dloss)
+    lone = x * 0.0
+    lone[1], lone[2] = x[1], x[2] * 1e-4
+    check_ce(lone, w, b, t, dloss)
+    check_ce(lone * 0.0, w * 0.0, b, t, dloss)
+
+
 @pytest.mark.parametrize("n, vocab, dim", [(40, 60, 16), (520, 1300, 100), (3000, 8, 200), (6, 4000, 200)])
 def test_confident_rows_keep_small_gradients(cuda, n, vocab, dim):
     """Logits so far apart that p is 1 - 1e-9 at the target and 1e-30 elsewhere: the
