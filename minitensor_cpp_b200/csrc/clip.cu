@@ -356,12 +356,14 @@ struct Launcher {
     }
 
     int count_partials() {
-        n_partials = 0;
+        long long n = 0;
         MTC_TRY(tables([&](const auto &t) {
-            n_partials += grid(t.pieces);
+            n += grid(t.pieces);
             return MTC_OK;
         }));
-        for (const StridedTensor &t : plan.strided) n_partials += grid((t.numel + kThreads - 1) / kThreads);
+        for (const StridedTensor &t : plan.strided) n += grid((t.numel + kThreads - 1) / kThreads);
+        if (n > INT_MAX) return fail(MTC_ERR_UNSUPPORTED, "too many tensors");
+        n_partials = static_cast<int>(n);
         return MTC_OK;
     }
 
@@ -435,6 +437,9 @@ int run_norm(const mtc_desc *tensors, int32_t n, bool clip, float max_norm, cons
     }
     Plan plan;
     for (int i = 0; i < n; ++i) MTC_TRY(plan_tensor(tensors[i], outs[i], plan));
+    // pieces are counted in 32 bits, the first and the last of a tensor apart
+    if (plan.dense_total / kPiece + 2ll * n > (int64_t{1} << 30))
+        return fail(MTC_ERR_UNSUPPORTED, "the tensors have too many elements");
     float *norm_ptr = norm != nullptr ? float_at(norm) : nullptr;
     Launcher l{plan, stream, sm_count(current_device())};
     MTC_TRY(l.count_partials());

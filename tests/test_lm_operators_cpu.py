@@ -137,6 +137,13 @@ def test_clipping_refuses(call):
     assert call() == abi.ERR_INVALID_ARGUMENT
 
 
+def test_clipping_refuses_more_elements_than_its_counters_hold():
+    huge = desc([2 ** 41])
+    assert norm([huge] * 5, desc([])) == abi.ERR_UNSUPPORTED
+    assert norm([desc([2 ** 43])], desc([])) == abi.ERR_UNSUPPORTED
+    assert clip([huge] * 5, [desc([2 ** 41], ptr=P * (i + 1) * 2 ** 32) for i in range(5)]) == abi.ERR_UNSUPPORTED
+
+
 def test_clipping_nothing_is_a_call_without_work():
     assert clip([], []) == abi.OK
     assert clip([desc([0, 5])], [desc([0, 5])]) == abi.OK
