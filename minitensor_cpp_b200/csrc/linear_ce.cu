@@ -156,16 +156,16 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
     const int sub = lane % L;
     const float *x = p.x + n * p.x_rs;
     constexpr int kMost = kSmallClasses / 32;
-    float z[kMost];
-    Softmax s{-INFINITY, 0.0f};
-    float zt = 0.0f;
+    // the logits in float64, which a latency-bound kernel has time for: of a few rows, each
+    // rounding of one shows in the gradients
+    double z[kMost], zt = 0.0, top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
-        z[i] = 0.0f;
+        z[i] = 0.0;
         if (i * C >= p.V) continue;
         const int v = i * C + lane / L;
         const float *w = p.w + (v < p.V ? v : 0) * p.w_rs;
-        float sum = 0.0f;
+        double sum = 0.0;
         int64_t d = sub;
         for (; d + 15 * L < p.D; d += 16 * L) {
             float xv[16], wv[16];
@@ -175,9 +175,10 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
                 wv[u] = __ldg(w + (d + u * L) * p.w_cs);
             }
 #pragma unroll
-            for (int u = 0; u < 16; ++u) sum = fmaf(xv[u], wv[u], sum);
+            for (int u = 0; u < 16; ++u) sum = fma(static_cast<double>(xv[u]), static_cast<double>(wv[u]), sum);
         }
-        for (; d < p.D; d += L) sum = fmaf(__ldg(x + d * p.x_cs), __ldg(w + d * p.w_cs), sum);
+        for (; d < p.D; d += L)
+            sum = fma(static_cast<double>(__ldg(x + d * p.x_cs)), static_cast<double>(__ldg(w + d * p.w_cs)), sum);
         for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         if (v >= p.V) {
             z[i] = -INFINITY;
@@ -186,26 +187,33 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
         if (p.bias != nullptr) sum += __ldg(p.bias + v * p.b_s);
         z[i] = sum;
         if (v == t) zt = sum;
-        if (sub == 0) s = merge(s, one_logit(sum));
+        top = fmax(top, sum);
     }
-    s = merge_lanes(s, 1, 32);
-    const float lse = softmax_base(s.top) + logf(s.sum);
+    for (int o = 1; o < 32; o <<= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const double base = isinf(top) ? 0.0 : top;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+        if (i * C < p.V && sub == 0) sum += expf(static_cast<float>(z[i] - base));
+    for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const float beyond = static_cast<float>(log(sum));  // lse = base + beyond
     zt = __shfl_sync(0xFFFFFFFFu, zt, t % C * L);
     if (lane == 0) {
-        if (p.loss != nullptr) p.loss[n * p.loss_s] = lse - zt;
-        if (p.lse != nullptr) p.lse[n * p.lse_s] = lse;
+        if (p.loss != nullptr) p.loss[n * p.loss_s] = static_cast<float>(base - zt) + beyond;
+        if (p.lse != nullptr) p.lse[n * p.lse_s] = static_cast<float>(base + beyond);
     }
     if (a.g == nullptr) return;
+    float g[kMost];
     const float dl = p.dloss[n * p.dl_s];
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
         const int v = i * C + lane / L;
         if (i * C >= p.V || v >= p.V) {
-            z[i] = 0.0f;
+            g[i] = 0.0f;
             continue;
         }
-        z[i] = softmax_grad(z[i], lse, dl, v == t);
-        if (sub == 0) a.g[n * p.V + v] = z[i];
+        g[i] = softmax_grad(static_cast<float>(z[i] - base) - beyond, dl, v == t);
+        if (sub == 0) a.g[n * p.V + v] = g[i];
     }
     if (p.dx == nullptr) return;
     for (int64_t d0 = 0; d0 < p.D; d0 += 128) {
@@ -216,12 +224,12 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
             const int classes = static_cast<int>(p.V - i * C < C ? p.V - i * C : C);
 #pragma unroll 4
             for (int c = 0; c < classes; ++c) {
-                const float g = __shfl_sync(0xFFFFFFFFu, z[i], c * L);
+                const float gc = __shfl_sync(0xFFFFFFFFu, g[i], c * L);
                 const float *w = p.w + static_cast<int64_t>(i * C + c) * p.w_rs;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int64_t d = d0 + u * 32 + lane;
-                    if (d < p.D) dx[u] = fmaf(g, __ldg(w + d * p.w_cs), dx[u]);
+                    if (d < p.D) dx[u] = fmaf(gc, __ldg(w + d * p.w_cs), dx[u]);
                 }
             }
         }
@@ -386,7 +394,7 @@ int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bia
         MTC_TRY(zero_view(dw, stream));
         return zero_view(db, stream);
     }
-    if (p.V <= kSmallClasses && p.N < (int64_t{1} << 21) && p.N * p.V < (int64_t{1} << 22) / (p.D + 1))
+    if (p.V <= kSmallClasses && p.N < (int64_t{1} << 20) && p.N * p.V < (int64_t{1} << 22) / (p.D + 1))
         return small_path(p, stream);
     if (few_rows(p)) return linear_ce_few(p, false, stream);
     if (few_classes(p)) return linear_ce_few(p, true, stream);

@@ -61,14 +61,16 @@ __device__ __forceinline__ int row_target(const LinearCe &p, int64_t n, unsigned
 }
 
 // Running maximum and sum of exponentials relative to it.  Infinite maxima count from 0,
-// so that a row of +inf or -inf has its limit and not exp(inf - inf).
+// so that a row of +inf or -inf has its limit and not exp(inf - inf).  The sum in float64:
+// of a row that is sure of its class it is 1 and little more, and that little is the gradient.
 struct Softmax {
-    float top, sum;
+    float top;
+    double sum;
 };
 
 // (of one logit: a NaN or an infinity makes the sum what it is)
 __device__ __forceinline__ Softmax one_logit(float z) {
-    return Softmax{z, isnan(z) ? z : isinf(z) ? (z > 0.0f ? z : 0.0f) : 1.0f};
+    return Softmax{z, isnan(z) ? z : isinf(z) ? (z > 0.0f ? z : 0.0f) : 1.0};
 }
 
 __device__ __forceinline__ float softmax_base(float top) { return isinf(top) ? 0.0f : top; }
@@ -77,8 +79,8 @@ __device__ __forceinline__ Softmax merge(Softmax a, Softmax b) {
     Softmax r;
     r.top = fmaxf(a.top, b.top);
     const float base = softmax_base(r.top);
-    r.sum = (a.sum != 0.0f ? a.sum * expf(softmax_base(a.top) - base) : 0.0f) +
-            (b.sum != 0.0f ? b.sum * expf(softmax_base(b.top) - base) : 0.0f);
+    r.sum = (a.sum != 0.0 ? a.sum * expf(softmax_base(a.top) - base) : 0.0) +
+            (b.sum != 0.0 ? b.sum * expf(softmax_base(b.top) - base) : 0.0);
     return r;
 }
 
@@ -92,9 +94,20 @@ __device__ __forceinline__ Softmax merge_lanes(Softmax s, int from, int to) {
     return s;
 }
 
-__device__ __forceinline__ float softmax_grad(float z, float lse, float d, bool hot) {
-    const float x = z - lse;
-    return d * (hot ? expm1f(x) : expf(x));
+// lse in two parts: base + log rounds to the base's places, (z - base) - log does not.
+struct LogSum {
+    float base, log;
+    __device__ __forceinline__ float lse() const { return base + log; }
+    __device__ __forceinline__ float of(float z) const { return (z - base) - log; }  // log of the class's probability
+    __device__ __forceinline__ float loss(float z) const { return log - (z - base); }
+};
+
+__device__ __forceinline__ LogSum log_sum(float top, double sum) {
+    return LogSum{softmax_base(top), static_cast<float>(log(sum))};
+}
+
+__device__ __forceinline__ float softmax_grad(float log_p, float d, bool hot) {
+    return d * (hot ? expm1f(log_p) : expf(log_p));
 }
 
 // How many of `extent` rows from `first` on have a loss.

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
     constexpr int kMine = (4 * R + 31) / 32;  // logits of a lane: i = lane + 32 k is few i / 4 and many i % 4
     Softmax mine[kMine];
 #pragma unroll
-    for (int k = 0; k < kMine; ++k) mine[k] = Softmax{-INFINITY, 0.0f};
+    for (int k = 0; k < kMine; ++k) mine[k] = Softmax{-INFINITY, 0.0};
     float acc[4 * R];
 #pragma unroll
     for (int i = 0; i < 4 * R; ++i) acc[i] = 0.0f;
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
                 const int64_t n = v0 + lane % 4;  // the lanes of a row: its classes, lane / 4 apart
                 const bool in = n < many && (R >= 8 || lane < 4 * R);
                 const int t = n < many ? row_target(p, n, a.err, lane < 4) : -1;
-                Softmax s{-INFINITY, 0.0f};
+                Softmax s{-INFINITY, 0.0};
                 float zt = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < kMine; ++k) {
@@ -174,17 +174,17 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
                     const float other = __shfl_xor_sync(0xFFFFFFFFu, zt, o);
                     if (zt == -INFINITY) zt = other;
                 }
-                const float lse = softmax_base(s.top) + logf(s.sum);
+                const LogSum l = log_sum(s.top, s.sum);
                 if (lane < 4 && n < many) {
-                    if (p.loss != nullptr) p.loss[n * p.loss_s] = t < 0 ? 0.0f : lse - zt;
-                    if (p.lse != nullptr) p.lse[n * p.lse_s] = t < 0 ? 0.0f : lse;
+                    if (p.loss != nullptr) p.loss[n * p.loss_s] = t < 0 ? 0.0f : l.loss(zt);
+                    if (p.lse != nullptr) p.lse[n * p.lse_s] = t < 0 ? 0.0f : l.lse();
                 }
                 if (a.g != nullptr && in) {
                     const float d = t < 0 ? 0.0f : p.dloss[n * p.dl_s];
 #pragma unroll
                     for (int k = 0; k < kMine; ++k) {
                         const int v = lane / 4 + 8 * k;
-                        if (v < R) a.g[n * R + v] = t < 0 || v >= p.V ? 0.0f : softmax_grad(z[k], lse, d, v == t);
+                        if (v < R) a.g[n * R + v] = t < 0 || v >= p.V ? 0.0f : softmax_grad(l.of(z[k]), d, v == t);
                     }
                 }
             } else {
@@ -224,8 +224,8 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
 }
 
 // lse of row n from the CTAs' parts; every lane of the warp gets it.
-__device__ __forceinline__ float few_lse(const FewArgs &a, int R, int n) {
-    Softmax s{-INFINITY, 0.0f};
+__device__ __forceinline__ LogSum few_lse(const FewArgs &a, int R, int n) {
+    Softmax s{-INFINITY, 0.0};
     const Softmax *parts = a.parts + n;
 #pragma unroll 8
     for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) s.top = fmaxf(s.top, parts[i * R].top);
@@ -235,24 +235,24 @@ __device__ __forceinline__ float few_lse(const FewArgs &a, int R, int n) {
 #pragma unroll 8
     for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) {
         const Softmax x = parts[i * R];
-        if (x.sum != 0.0f) s.sum += x.sum * expf(softmax_base(x.top) - base);
+        if (x.sum != 0.0) s.sum += x.sum * expf(softmax_base(x.top) - base);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s.sum += __shfl_xor_sync(0xFFFFFFFFu, s.sum, o);
-    return softmax_base(s.top) + logf(s.sum);
+    return log_sum(s.top, s.sum);
 }
 
-__device__ __forceinline__ void store_loss(const LinearCe &p, const FewArgs &a, int n, int target, float lse) {
-    if (p.loss != nullptr) p.loss[n * p.loss_s] = target < 0 ? 0.0f : lse - a.z_target[n];
-    if (p.lse != nullptr) p.lse[n * p.lse_s] = target < 0 ? 0.0f : lse;
+__device__ __forceinline__ void store_loss(const LinearCe &p, const FewArgs &a, int n, int target, LogSum l) {
+    if (p.loss != nullptr) p.loss[n * p.loss_s] = target < 0 ? 0.0f : l.loss(a.z_target[n]);
+    if (p.lse != nullptr) p.lse[n * p.lse_s] = target < 0 ? 0.0f : l.lse();
 }
 
 __global__ void __launch_bounds__(32 * kFewRows) k_few_loss(const LinearCe p, const FewArgs a, int R) {
     wait_for_previous();
     const int n = threadIdx.x / 32;
     if (n >= p.N) return;
-    const float lse = few_lse(a, R, n);
-    if (threadIdx.x % 32 == 0) store_loss(p, a, n, row_target(p, n, a.err, false), lse);
+    const LogSum l = few_lse(a, R, n);
+    if (threadIdx.x % 32 == 0) store_loss(p, a, n, row_target(p, n, a.err, false), l);
 }
 
 // With eight rows or more the exponentials are worth a pass of their own: z [N][V] -> g [V][R],
@@ -262,12 +262,13 @@ constexpr bool g_before(int R, bool classes) { return classes || R >= 8; }
 template <int R>
 __global__ void __launch_bounds__(kFewThreads) k_few_g(const LinearCe p, const FewArgs a) {
     wait_for_previous();
-    __shared__ float lse[R], dloss[R];
+    __shared__ LogSum lse[R];
+    __shared__ float dloss[R];
     __shared__ int target[R];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int n = warp; n < R; n += kFewThreads / 32) {
         const int t = n < p.N ? row_target(p, n, a.err, false) : -1;
-        const float l = n < p.N ? few_lse(a, R, n) : 0.0f;
+        const LogSum l = n < p.N ? few_lse(a, R, n) : LogSum{0.0f, 0.0f};
         if (lane == 0) {
             lse[n] = l;
             target[n] = t;
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kFewThreads) k_few_g(const LinearCe p, const F
         for (int n = 0; n < R; ++n) g[n] = n < p.N ? a.z[n * p.V + v] : 0.0f;
 #pragma unroll
         for (int n = 0; n < R; ++n) {
-            g[n] = target[n] >= 0 ? softmax_grad(g[n], lse[n], dloss[n], v == target[n]) : 0.0f;
+            g[n] = target[n] >= 0 ? softmax_grad(lse[n].of(g[n]), dloss[n], v == target[n]) : 0.0f;
             sum += g[n];
         }
         if (p.db != nullptr) p.db[v * p.db_s] = sum;
@@ -299,7 +300,8 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __
 template <int R, int C, bool CLASSES>
 __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const LinearCe p, const FewArgs a) {
     wait_for_previous();
-    __shared__ float lse[R], dloss[R];
+    __shared__ LogSum lse[R];
+    __shared__ float dloss[R];
     __shared__ int target[R];
     __shared__ __align__(16) float sums[kFewThreads / 32][32 * C];
     __shared__ __align__(16) float2 gs[kFewThreads / 32][32][R + 2];  // of a warp's 32 of the many; a lane's row off the banks of the next
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const 
     if (!CLASSES) {
         for (int n = warp; n < R; n += kFewThreads / 32) {
             const int t = n < p.N ? row_target(p, n, a.err, false) : -1;
-            const float l = !kBefore && n < p.N ? few_lse(a, R, n) : 0.0f;
+            const LogSum l = !kBefore && n < p.N ? few_lse(a, R, n) : LogSum{0.0f, 0.0f};
             if (lane == 0) {
                 lse[n] = l;
                 target[n] = t;
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 3 : 2) k_few_grad(const 
                 any |= g != 0.0f;
                 if (CLASSES) db[n] += g;
             } else {
-                if (n < p.N && v < p.V && target[n] >= 0) g = softmax_grad(a.z[n * p.V + v], lse[n], dloss[n], v == target[n]);
+                if (n < p.N && v < p.V && target[n] >= 0) g = softmax_grad(lse[n].of(a.z[n * p.V + v]), dloss[n], v == target[n]);
                 sum += g;
             }
             gs[warp][lane][n] = make_float2(g, g);

@@ -791,7 +791,7 @@ struct RowArgs {
     int parts, part_pitch;  // of a row
     const float *part_max, *part_sum, *z_target;
     const int *row;       // of x
-    float *lse_live;      // [rows]
+    LogSum *lse_live;     // [rows]
     float *loss, *lse;
     int64_t loss_s, lse_s;
 };
@@ -808,19 +808,19 @@ __global__ void __launch_bounds__(256) k_row_loss(const RowArgs a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float base = isinf(top) ? 0.0f : top;
-    float sum = 0.0f;
+    double sum = 0.0;
     for (int j = lane; j < a.parts; j += 32) {
         const float mj = isinf(m[j]) ? 0.0f : m[j];
-        if (s[j] != 0.0f) sum += s[j] * expf(mj - base);
+        if (s[j] != 0.0f) sum += static_cast<double>(s[j]) * expf(mj - base);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane != 0) return;
-    const float lse = base + logf(sum);
-    a.lse_live[r] = lse;
+    const LogSum l = log_sum(top, sum);
+    a.lse_live[r] = l;
     const int64_t n = a.row[a.first + r];
-    if (a.lse != nullptr) a.lse[n * a.lse_s] = lse;
-    if (a.loss != nullptr) a.loss[n * a.loss_s] = lse - a.z_target[r];
+    if (a.lse != nullptr) a.lse[n * a.lse_s] = l.lse();
+    if (a.loss != nullptr) a.loss[n * a.loss_s] = l.loss(a.z_target[r]);
 }
 
 struct GradArgs {
@@ -829,7 +829,7 @@ struct GradArgs {
     int64_t V;
     float *z;            // [rows][pitch], becomes g'
     int64_t pitch;
-    const float *lse_live;
+    const LogSum *lse_live;
     const int *target;
     const float *dloss;
     const int *exponent; // of the scale of g'
@@ -854,13 +854,15 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
 #pragma unroll
     for (int j0 = 0; j0 < kGradRows / 8; j0 += 4) {
         float4 z[4];
-        float lse[4], d[4];
+        LogSum lse[4];
+        float d[4];
         int t[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t r = r0 + (j0 + j) * 8 + warp;
             z[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            lse[j] = d[j] = 0.0f;
+            lse[j] = LogSum{0.0f, 0.0f};
+            d[j] = 0.0f;
             t[j] = -1;
             if (r < live) {
                 if (in) z[j] = __ldcs(reinterpret_cast<const float4 *>(a.z + r * a.pitch + c));
@@ -873,7 +875,7 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t r = r0 + (j0 + j) * 8 + warp;
-            float g[4] = {z[j].x - lse[j], z[j].y - lse[j], z[j].z - lse[j], z[j].w - lse[j]};
+            float g[4] = {lse[j].of(z[j].x), lse[j].of(z[j].y), lse[j].of(z[j].z), lse[j].of(z[j].w)};
             __half h[4], l[4];
             const int hot = t[j] - static_cast<int>(c);
             float at_hot = 0.0f;
@@ -1022,7 +1024,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t split_dw = p.dw != nullptr && parts_dw ? static_cast<size_t>(splits_dw) * p.V * parts_pitch * 4 : 0;
     const size_t split_bytes = grads ? padded(split_dx > split_dw ? split_dx : split_dw) : 0;
     Workspace ws;
-    MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 2 * row_stat + z_bytes + col_bytes + split_bytes,
+    MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 3 * row_stat + z_bytes + col_bytes + split_bytes,
                         stream));
     LiveRows live;
     live.count = ws.take<int>(256);
@@ -1034,7 +1036,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     float *part_max = ws.take<float>(stat);
     float *part_sum = ws.take<float>(stat);
     float *z_target = ws.take<float>(row_stat);
-    float *lse_live = ws.take<float>(row_stat);
+    LogSum *lse_live = ws.take<LogSum>(2 * row_stat);
     float *z = ws.take<float>(z_bytes);
     float *columns = ws.take<float>(col_bytes);
     float *split_ws = ws.take<float>(split_bytes);

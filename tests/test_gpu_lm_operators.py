@@ -582,6 +582,45 @@ def test_linear_cross_entropy_without_columns(cuda):
         check_ce(x, w, None, t, None)
 
 
+@pytest.mark.parametrize("n, vocab, dim", [(1, 4, 450), (5, 200, 64), (1, 3000, 515), (3, 1000, 64), (16, 700, 128),
+                                           (4000, 6, 1024), (9001, 16, 64)])
+@pytest.mark.parametrize("gap", [3.0, 11.5, 18.0, 40.0])
+def test_rows_sure_of_their_class_keep_the_digits_of_what_is_left(cuda, n, vocab, dim, gap):
+    """Logits that float32 holds exactly, one far above the others: 1 - p is lost in 1, and is
+    the gradient.  The logarithm of a probability is rounded once beside its value, and an
+    exponential is off by that and two units more."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 26)
+    steps = torch.round(w[:, :1] * 8).clamp(-16, 16) / 8
+    x, w = torch.zeros_like(x), torch.zeros_like(w)
+    x[:, 0], w[:, :1] = 1.0, steps
+    w[vocab // 2, 0] = 3.0 + gap
+    t = torch.full_like(t, vocab // 2)
+    dloss = torch.ones_like(dloss)
+    got = run_ce(x, w, None, t, dloss)
+    z = w[:, 0].double()
+    logp = z - torch.logsumexp(z, 0)
+    others = torch.arange(vocab, device=cuda) != vocab // 2
+    rest = torch.logsumexp(z[others], 0) - torch.logsumexp(z, 0)  # log(1 - p), without the difference
+    g = torch.where(others, logp.exp(), -rest.exp())
+    rel = 2 * U * (logp.abs().max() + 10)
+    loss = -torch.log1p(-rest.exp())
+    # The sum of exponentials lies in [1, 2) and is a float64: each of its at most `vocab`
+    # additions rounds by half a step, 2^-53, at most, and the logarithm of 1 + r is within r.
+    # (A gap of 40 leaves 1 - p below the first step.)
+    step = vocab * 2.0 ** -53 * 1.01
+    within(got["loss"], loss.expand(n), (rel * loss + step).expand(n), "loss")
+    within(got["db"], n * g, (rel + 2 * U * n) * n * g.abs() + n * step, "db")
+    within(got["dw"][:, 0], n * g, (rel + 2 * U * n) * n * g.abs() + n * step, "dw")
+
+
+@pytest.mark.parametrize("n, vocab, dim", [(2 ** 21 - 1, 1, 1), (2 ** 21 - 1, 2, 0), (2 ** 20, 3, 0), (2 ** 20 - 1, 3, 0)])
+def test_more_rows_than_a_grid_has_parts(cuda, n, vocab, dim):
+    """Where 32 rows a CTA would be more than the 65535 parts of a launch's second axis."""
+    check_ce(*ce_data(n, vocab, dim, 25, ignored=0.1))
+
+
 def test_linear_cross_entropy_beyond_32_bits(cuda):
     """A weight of 2.2e9 elements: the loss and sampled rows of its gradient against
     float64, on classes at the end of the vocabulary."""
