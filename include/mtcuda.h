@@ -289,7 +289,8 @@ int mtc_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale
  * outside [0, V), which also sets the device error word.  Products have float32
  * accuracy (each operand as a pair of 16-bit floats, or float32 for small
  * problems).  A non-finite x makes its own row's loss NaN or infinite, a
- * non-finite weight or bias every row's. */
+ * non-finite weight or bias every row's.  On the tensor cores the call takes
+ * 4 bytes of workspace an element of x and weight and 8 a row and 128 classes. */
 int mtc_linear_cross_entropy(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias, const mtc_desc *targets,
                              int64_t ignore_target, const mtc_desc *loss, const mtc_desc *lse, void *stream);
 
@@ -299,7 +300,9 @@ int mtc_linear_cross_entropy(const mtc_desc *x, const mtc_desc *weight, const mt
  * in one call (three products; the logits of a piece of the rows at a time).
  * dloss [N] may be a broadcast view.  loss, lse, dx, dweight and dbias may each
  * be NULL.  dx rows of ignored targets are zero.  dx, dweight and dbias are
- * overwritten. */
+ * overwritten.  The workspace also holds the logits of a piece of the rows, up
+ * to 4 GiB, and partial sums of dx or dweight where these have few tiles of
+ * 256 x 256, or rows without 32-byte alignment. */
 int mtc_linear_cross_entropy_grad(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias,
                                   const mtc_desc *targets, int64_t ignore_target, const mtc_desc *dloss,
                                   const mtc_desc *loss, const mtc_desc *lse, const mtc_desc *dx,

@@ -6,8 +6,8 @@
 //
 // Small problems take a warp a row (here), few rows or few classes stream the other operand
 // past them (linear_ce_few.cu), and the rest runs on the tensor cores (linear_ce_tc.cu) over
-// the rows that have a loss: k_live_rows lists them in order, and only the device knows how
-// many there are.
+// the rows that have a loss: k_live_rows lists them in order (8 us for 1031 rows, 13 us for
+// 65536), and only the device knows how many there are.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -117,12 +117,18 @@ __global__ void __launch_bounds__(kListThreads) k_live_rows(const LinearCe p, co
 }
 
 // ------------------------------------------------------------- small problems --
-// Up to 256 classes and 2^22 products: bound by latency, so two launches.  k_small_rows: a
-// warp a row, its lanes over the classes (and over the columns where the classes are few),
-// loss, g and the row of dx.  k_small_weights: a thread an element of dW (or of db), 32 rows
-// a CTA; the last CTA of an element's to finish adds the parts in the order of the rows.
+// Up to 256 classes, 4096 products a row and 2^22 in all: bound by latency, so two launches.
+// k_small_rows: a warp a row, its lanes over the classes (and over the columns where the classes
+// are few), loss, g and the row of dx.  A warp's time goes with the products of a row: 300 rows
+// take 21 us for 1280 and 38 for 5120 for the loss and its gradients, where the tensor cores take
+// 51 and 57, but 32 rows 111 us for 20480, where they take 59; 8 rows 21 us for 1280 and 33 for
+// 5120, where the path of few rows takes 26 and 27, so that those leave at 2048.
+// k_small_weights: a thread an element of dW (or of db), 32 rows a CTA; the last CTA of an
+// element's to finish adds the parts in the order of the rows.
+// 300 rows of 64 columns, 3 classes: 26 us a call with its checks, most of it the host's.
 
 constexpr int kSmallClasses = 256;
+constexpr int64_t kSmallRow = 4096, kSmallFewRow = 2048;  // products of a row
 constexpr int kSmallRows = 32;
 
 struct SmallArgs {
@@ -394,7 +400,9 @@ int run_linear_ce(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bia
         MTC_TRY(zero_view(dw, stream));
         return zero_view(db, stream);
     }
-    if (p.V <= kSmallClasses && p.N < (int64_t{1} << 20) && p.N * p.V < (int64_t{1} << 22) / (p.D + 1))
+    const bool few = few_rows(p) || few_classes(p);
+    if (p.V <= kSmallClasses && p.V * p.D <= (few ? kSmallFewRow : kSmallRow) && p.N < (int64_t{1} << 20) &&
+        p.N * p.V < (int64_t{1} << 22) / (p.D + 1))
         return small_path(p, stream);
     if (few_rows(p)) return linear_ce_few(p, false, stream);
     if (few_classes(p)) return linear_ce_few(p, true, stream);

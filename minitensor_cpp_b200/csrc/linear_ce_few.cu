@@ -12,7 +12,10 @@
 // keeps the softmax of its logits, joined over the CTAs afterwards; over few classes a row's
 // logits are all in one warp, which writes the loss and g at once.
 // k_few_grad: a CTA takes 128 (64) columns and a part of the many; the columns of the few and
-// of their gradient stay in registers, the gradient of the many is written as it goes.
+// of their gradient stay in registers, the gradient of the many is written as it goes: 4 rows
+// against 131072 x 2048 take 566 us for the loss and all gradients, where reading W twice and
+// writing dW takes 492 us at the rate of a copy; 16 rows 1267 us, bound by the FMAs.  (The tensor
+// path takes 1264 us for 17 rows, which is where the limit of 16 comes from.)
 #include <cfloat>
 #include <climits>
 #include <cstring>

@@ -46,6 +46,9 @@
 // 32-byte sector at a time: the 32 KB of shared memory that would make whole lines of it are
 // worth more as a stage.  Results whose rows allow no such stores go by way of a padded
 // workspace.
+// Bound by the MMAs and, in long calls, by the power limit: 4096 x 32000 x 2048 takes 1176 us
+// for the logits and 1106 and 1135 us for dx and dweight, 457 to 485 TFLOP/s of products
+// (three times that of MMAs) with the tensor pipe active in 79, 88 and 87 % of the cycles.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
@@ -162,7 +165,8 @@ __device__ __forceinline__ int last_exponent(const PackArgs &a, int which) {
 }
 
 // Largest finite magnitudes of x (rows with a loss) and weight over a sample of the rows, one
-// a warp, and of dloss; the zero rows of dx.
+// a warp, and of dloss; the zero rows of dx.  7 to 30 us for 1184 rows of 1024 to 8192 columns,
+// a warp's latency.
 __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     wait_for_previous();
     const bool second = blockIdx.x >= a.first_of_second;
@@ -235,7 +239,8 @@ __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
 }
 
 // Each half-warp packs one block of 64 columns at a time: a lane four columns.  AGAIN: only
-// the tensors whose scale was wrong; and the exponents are written down.
+// the tensors whose scale was wrong; and the exponents are written down.  Bound by HBM, 8
+// bytes an element: 36096 rows of 2048 in 103 us (5.7 TB/s).
 template <bool AGAIN>
 __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     wait_for_previous();
@@ -726,6 +731,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
 }
 
 // The splits' partial results in order, into the rows of the result, whatever their layout.
+// Bound by HBM, 4 bytes an element and split and 4 more.
 __global__ void __launch_bounds__(256) k_join_splits(const TileArgs a, int64_t out_cs, int vec) {
     wait_for_previous();
     int64_t M = a.M;
@@ -796,7 +802,8 @@ struct RowArgs {
     int64_t loss_s, lse_s;
 };
 
-// One warp a row: the statistics of its tiles make lse and the loss.
+// One warp a row: the statistics of its tiles make lse and the loss (8 bytes for 128 logits:
+// 7 us for 4096 x 32000).
 __global__ void __launch_bounds__(256) k_row_loss(const RowArgs a) {
     wait_for_previous();
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
@@ -839,7 +846,8 @@ struct GradArgs {
 constexpr int kGradRows = 64;  // rows of a CTA
 
 // z -> g' in place.  A CTA takes 128 columns of 64 rows, a warp eight of the rows, a lane
-// four columns: 512 bytes of z a load, two blocks of 128 + 128 bytes a store.
+// four columns: 512 bytes of z a load, two blocks of 128 + 128 bytes a store.  Bound by HBM,
+// 8 bytes a logit: 4096 x 32000 in 212 us (4.7 TB/s).
 __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
     wait_for_previous();
     const int64_t live = live_extent(a.live, a.first, a.rows);
@@ -913,7 +921,8 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
         make_float4(column.x * u0 * u1, column.y * u0 * u1, column.z * u0 * u1, column.w * u0 * u1);
 }
 
-// A CTA takes 32 columns; its eight warps take the row blocks in turn.
+// A CTA takes 32 columns; its eight warps take the row blocks in turn (4 bytes for 64 rows of
+// a column: 6 us for 928 x 50003).
 __global__ void __launch_bounds__(256) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
     wait_for_previous();
     __shared__ float sums[8][32];
