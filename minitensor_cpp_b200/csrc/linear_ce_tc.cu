@@ -30,7 +30,8 @@
 //
 // All three products read the same packed operands, [row][64 columns][hi, lo], K-major
 // or MN-major by the matrix descriptors alone:
-//   logits   z  = x' w'^T   A = x' K-major,  B = w' K-major      softmax statistics in the epilogue
+//   logits   z  = x' w'^T   A = x' K-major,  B = w' K-major      softmax statistics in the epilogue,
+//                                                                split along D when the tiles are few
 //   dx       dx = g' w'     A = g' K-major,  B = w' MN-major     split along V when the tiles are few
 //   dweight  dw = g'^T x'   A = g' MN-major, B = x' MN-major     added up over the pieces of the rows
 // The logits of one piece of the rows are written once, as float32; k_softmax_grad
@@ -789,6 +790,56 @@ __global__ void __launch_bounds__(256) k_join_splits(const TileArgs a, int64_t o
     }
 }
 
+// The logits of few tiles, split along the columns of x: their partial sums added in order, and
+// what store_logits does with them.  A warp takes 128 classes of a row.
+__global__ void __launch_bounds__(256) k_join_logits(const TileArgs a) {
+    wait_for_previous();
+    const int lane = threadIdx.x % 32;
+    const int64_t M = live_extent(a.live, a.first, a.M), chunks = (a.N + 127) / 128, plane = a.M * a.parts_pitch;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; i < M * chunks;
+         i += static_cast<int64_t>(gridDim.x) * 8) {
+        const int64_t r = i / chunks, k = i - r * chunks, c = k * 128 + lane * 4;
+        float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (c < a.parts_pitch) {
+            const float *src = a.parts + r * a.parts_pitch + c;
+#pragma unroll 4
+            for (int s = 0; s < a.splits; ++s) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + s * plane);
+                z[0] += v.x;
+                z[1] += v.y;
+                z[2] += v.z;
+                z[3] += v.w;
+            }
+        }
+        const int64_t target = a.target[a.first + r];
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j >= a.N) {
+                z[j] = -INFINITY;
+                continue;
+            }
+            if (a.bias != nullptr) z[j] += __ldg(a.bias + (c + j) * a.bias_s);
+            if (c + j == target) a.z_target[r] = z[j];
+            top = fmaxf(top, z[j]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float base = isinf(top) ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += expf(z[j] - base);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (lane == 0) {
+            a.part_max[r * 2 * a.tiles_n + k] = top;
+            a.part_sum[r * 2 * a.tiles_n + k] = sum;
+        }
+        if (a.z != nullptr && c < a.z_pitch)
+            *reinterpret_cast<float4 *>(a.z + r * a.z_pitch + c) = make_float4(z[0], z[1], z[2], z[3]);
+    }
+}
+
 // ----------------------------------------------------------------- softmax --
 
 struct RowArgs {
@@ -968,12 +1019,15 @@ int launch_product(const CUtensorMap &a, const CUtensorMap &b, const TileArgs &a
 }
 
 // Splits of K so that the tiles of a product fill the pairs of SMs: the fewest whose
-// last wave is nearly full, each at least 512 of K.
+// last wave is nearly full, each at least 512 of K, or 256 (a piece) where half of the GPU
+// would idle: there the partial results are small (17 x 1000 x 4096: 78 -> 68 us for the loss
+// and its gradients, against 249 -> 287 us for 4096 x 2500 x 1024).
 int choose_splits(int64_t tiles, int64_t K, int64_t pairs, size_t bytes) {
     int best = 1;
     double best_cost = 1e30;
+    const int64_t least = 2 * tiles <= pairs ? 256 : 512;
     for (int s = 1; s <= 16; ++s) {
-        if (s > 1 && (K / s < 512 || bytes * s > (size_t{1} << 30))) break;
+        if (s > 1 && (K / s < least || bytes * s > (size_t{1} << 30))) break;
         const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
         const double cost = waves / s * (1.0 + 0.01 * (s - 1));
         if (cost < best_cost * 0.98) {
@@ -1019,6 +1073,10 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const int splits_dx = choose_splits(piece / 256 * tiles_d, p.V, pairs, static_cast<size_t>(piece) * p.D * 4);
     const int splits_dw = choose_splits(static_cast<int64_t>(tiles_v) * tiles_d, piece, pairs,
                                         static_cast<size_t>(p.V) * p.D * 4);
+    // A tile of logits takes 13 ns a column of x, however few there are of them: split where they
+    // leave half of the GPU idle.  (60 rows, 200 classes of length 4096: 90 -> 38 us for the loss.)
+    const int64_t tiles_z = piece / 256 * tiles_v;
+    const int splits_z = 2 * tiles_z <= pairs ? choose_splits(tiles_z, p.D, pairs, static_cast<size_t>(piece) * pitch * 4) : 1;
     const size_t list = padded(static_cast<size_t>(p.N) * 4);
     const size_t x_bytes = padded(static_cast<size_t>(rows_all) * d_blocks * 256);
     const size_t w_bytes = padded(static_cast<size_t>(p.V) * d_blocks * 256);
@@ -1031,7 +1089,9 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const bool parts_dw = splits_dw > 1 || !sector_rows(p.dw, p.dw_rs, p.dw_cs, p.D);
     const size_t split_dx = p.dx != nullptr && parts_dx ? static_cast<size_t>(splits_dx) * piece * parts_pitch * 4 : 0;
     const size_t split_dw = p.dw != nullptr && parts_dw ? static_cast<size_t>(splits_dw) * p.V * parts_pitch * 4 : 0;
-    const size_t split_bytes = grads ? padded(split_dx > split_dw ? split_dx : split_dw) : 0;
+    const size_t split_z = splits_z > 1 ? static_cast<size_t>(splits_z) * piece * pitch * 4 : 0;
+    const size_t split_grad = !grads ? 0 : split_dx > split_dw ? split_dx : split_dw;
+    const size_t split_bytes = padded(split_z > split_grad ? split_z : split_grad);
     Workspace ws;
     MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 3 * row_stat + z_bytes + col_bytes + split_bytes,
                         stream));
@@ -1099,7 +1159,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         t.first = first;
         t.tiles_n = tiles_v;
         t.group = 16;
-        t.splits = 1;
+        t.splits = splits_z;
         t.exp_a = live.count + kExponent;
         t.exp_b = live.count + kExponent + 1;
         t.err = err;
@@ -1111,7 +1171,16 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         t.part_max = part_max;
         t.part_sum = part_sum;
         t.z_target = z_target;
-        MTC_TRY((launch_product<false, false, Out::Logits>(x_k, w_k, t, sms, stream)));
+        if (splits_z > 1) {
+            t.parts = split_ws;
+            t.parts_pitch = pitch;
+            MTC_TRY((launch_product<false, false, Out::Sum>(x_k, w_k, t, sms, stream)));
+            const int64_t ctas = (rows * ((p.V + 127) / 128) + 7) / 8;
+            MTC_TRY(launch_dependent("linear cross entropy (logits)", k_join_logits,
+                                     static_cast<unsigned>(ctas < sms * 8 ? ctas : sms * 8), 256, 0, stream, t));
+        } else {
+            MTC_TRY((launch_product<false, false, Out::Logits>(x_k, w_k, t, sms, stream)));
+        }
         // (a last tile of 128 columns or less has no second half)
         const RowArgs ra{first, rows, live.count, static_cast<int>((p.V + 127) / 128), 2 * tiles_v, part_max, part_sum,
                          z_target, live.row, lse_live, p.loss, p.lse, p.loss_s, p.lse_s};

@@ -326,7 +326,8 @@ CE_SHAPES = [(1, 1, 1), (1, 2, 1), (1, 1000, 64), (2, 3, 5), (5, 257, 63), (64, 
              (128, 256, 64), (129, 255, 200), (300, 3, 64), (256, 512, 256), (257, 513, 129), (1000, 1000, 96),
              (513, 5003, 77), (2300, 301, 320), (33, 20011, 257), (4096, 40, 1024), (700, 1500, 1),
              (5000, 3, 300), (3000, 16, 130), (9001, 7, 97), (300, 1, 20000), (70000, 2, 33), (2000, 11, 256),
-             (600, 400, 128), (500, 385, 385), (520, 384, 290), (300, 2000, 771), (16, 700, 515), (13, 3001, 640), (3, 5000, 1100), (1, 90001, 50), (17, 900, 400)]
+             (600, 400, 128), (500, 385, 385), (520, 384, 290), (300, 2000, 771), (16, 700, 515), (13, 3001, 640), (3, 5000, 1100), (1, 90001, 50), (17, 900, 400),
+             (60, 200, 4096), (17, 17, 5000), (700, 900, 2047), (1300, 1025, 1100), (19, 3000, 1024)]
 
 
 @pytest.mark.parametrize("n, vocab, dim", CE_SHAPES)
