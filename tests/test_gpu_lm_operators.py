@@ -61,7 +61,8 @@ def make_tokens(n, vocab, seed, hot=0.3):
 
 
 EMB_SHAPES = [(1, 5, 1), (1, 1, 7), (7, 3, 4), (33, 10, 64), (256, 30, 48), (257, 100, 65), (300, 77, 30), (60, 500, 142), (1000, 999, 128), (4097, 50, 36),
-              (5000, 70001, 20), (9000, 2000, 1100), (65536, 1000, 8), (70001, 3000, 16), (200003, 300000, 5)]
+              (5000, 70001, 20), (9000, 2000, 1100), (65536, 1000, 8), (70001, 3000, 16), (200003, 300000, 5), (2048, 70000, 24), (2049, 3000, 24),
+              (700, 1 << 24, 1)]
 
 
 @pytest.mark.parametrize("n, vocab, dim", EMB_SHAPES)
