@@ -322,7 +322,7 @@ def check_ce(x, w, b, t, dloss):
 
 
 # one row and one class; tiles of 64, 128 and 256 met, missed by one and passed by
-# one in each direction; more rows than a piece of the logits holds
+# one in each direction
 CE_SHAPES = [(1, 1, 1), (1, 2, 1), (1, 1000, 64), (2, 3, 5), (5, 257, 63), (64, 64, 64), (65, 63, 66), (127, 129, 128),
              (128, 256, 64), (129, 255, 200), (300, 3, 64), (256, 512, 256), (257, 513, 129), (1000, 1000, 96),
              (513, 5003, 77), (2300, 301, 320), (33, 20011, 257), (4096, 40, 1024), (700, 1500, 1),
@@ -621,6 +621,34 @@ def test_rows_sure_of_their_class_keep_the_digits_of_what_is_left(cuda, n, vocab
 def test_more_rows_than_a_grid_has_parts(cuda, n, vocab, dim):
     """Where 32 rows a CTA would be more than the 65535 parts of a launch's second axis."""
     check_ce(*ce_data(n, vocab, dim, 25, ignored=0.1))
+
+
+def test_more_rows_than_a_piece_of_the_logits_holds(cuda):
+    """4.7 GB of logits: the rows go in two pieces, and dweight and dbias add up over them.  The
+    reference takes a thousand rows at a time; its bounds for dweight and dbias grow by the
+    ratio of the lengths of the sums."""
+    import torch
+
+    n, vocab, dim, step = 9000, 131100, 40, 1000
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 27, ignored=0.1)
+    t[4000:5000] = IGNORE
+    got = run_ce(x, w, b, t, dloss)
+    abi.check_device_errors(0)
+    dw, dw_tol, db, db_tol = (torch.zeros(s, dtype=torch.float64, device=cuda) for s in (w.shape, w.shape, b.shape, b.shape))
+    for i in range(0, n, step):
+        rows = slice(i, i + step)
+        want = ce_reference(x[rows], w, b, t[rows], dloss[rows])
+        for name in ("loss", "lse", "dx"):
+            within(got[name][rows], want[name][0], want[name][1] + 2.0 ** -40 * dloss.abs().max() * w.double().abs().sum(0) + 1e-42
+                   if name == "dx" else want[name][1] + 1e-42, f"{name} of rows {i}")
+        dw += want["dw"][0]
+        db += want["db"][0]
+        # (a gradient's smallest part goes by the largest |dloss| of all rows, not of these)
+        dw_tol += want["dw"][1] + 2.0 ** -40 * dloss.abs().max() * x[rows].double().abs().sum(0)
+        db_tol += want["db"][1] + 2.0 ** -40 * dloss.abs().max() * step
+    longer = (n + 16) / (step + 16)
+    within(got["dw"], dw, dw_tol * longer, "dw")
+    within(got["db"], db, db_tol * longer, "db")
 
 
 def test_linear_cross_entropy_beyond_32_bits(cuda):
