@@ -972,22 +972,23 @@ __global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
         make_float4(column.x * u0 * u1, column.y * u0 * u1, column.z * u0 * u1, column.w * u0 * u1);
 }
 
-// A CTA takes 32 columns; its eight warps take the row blocks in turn (4 bytes for 64 rows of
-// a column: 6 us for 928 x 50003).
-__global__ void __launch_bounds__(256) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
+// A CTA takes 32 columns; its warps, up to 32, take the row blocks in turn (4 bytes for 64 rows
+// of a column: 8 us for 928 x 50003, 18 us for 65536 x 1000, where 8 warps a CTA take 61 us).
+__global__ void __launch_bounds__(1024) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
     wait_for_previous();
-    __shared__ float sums[8][32];
+    __shared__ float sums[32][32];
+    const int warps = blockDim.x / 32;
     const int64_t v = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;
     const int blocks = static_cast<int>((live_extent(a.live, a.first, a.rows) + kGradRows - 1) / kGradRows);
     float sum = 0.0f;
     if (v < a.V) {
 #pragma unroll 8
-        for (int b = threadIdx.x / 32; b < blocks; b += 8) sum += a.column_parts[b * a.pitch + v];
+        for (int b = threadIdx.x / 32; b < blocks; b += warps) sum += a.column_parts[b * a.pitch + v];
     }
     sums[threadIdx.x / 32][threadIdx.x % 32] = sum;
     __syncthreads();
     if (threadIdx.x >= 32 || v >= a.V) return;
-    for (int w = 1; w < 8; ++w) sum += sums[w][threadIdx.x];
+    for (int w = 1; w < warps; ++w) sum += sums[w][threadIdx.x];
     db[v * db_s] = add ? db[v * db_s] + sum : sum;
 }
 
@@ -1191,7 +1192,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         const dim3 grid(static_cast<unsigned>((pitch + 127) / 128), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
         MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, 256, 0, stream, ga)));
         if (p.db != nullptr) {
-            MTC_TRY((launch_dependent("linear cross entropy (bias gradient)", k_bias_grad, static_cast<unsigned>((p.V + 31) / 32), 256, 0, stream, ga, p.db, p.db_s, first > 0)));
+            MTC_TRY((launch_dependent("linear cross entropy (bias gradient)", k_bias_grad, static_cast<unsigned>((p.V + 31) / 32), piece > 64 * kGradRows ? 1024 : 256, 0, stream, ga, p.db, p.db_s, first > 0)));
         }
         const __half *gp = reinterpret_cast<const __half *>(z);
         if (p.dx != nullptr && p.D > 0) {
