@@ -132,33 +132,39 @@ class View:
     def contiguous(storage, shape, offset: int = 0) -> "View":
         return View(storage, tuple(shape), tuple(contiguous_strides(shape)), offset)
 
-    @property
-    def shape(self) -> tuple:
-        return self._shape if self._tensor is None else tuple(self._tensor.shape)
-
-    @property
-    def strides(self) -> tuple:
-        return self._strides if self._tensor is None else self._tensor.stride()
-
-    @property
-    def offset(self) -> int:
-        return self._offset if self._tensor is None else self._tensor.storage_offset()
-
-    @property
-    def storage(self):
-        if self._tensor is None:
-            return self._storage
-        import torch
-
+    def _unbind(self) -> "View":
+        """Takes the fields over from the tensor that the view was made of."""
         t = self._tensor
-        return torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
+        if t is not None:
+            import torch
+
+            self._storage = torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
+            self._shape, self._strides, self._offset = tuple(t.shape), tuple(t.stride()), t.storage_offset()
+            self._tensor = None
+        return self
+
+    def _field(name):
+        return property(lambda self: getattr(self._unbind(), name), lambda self, value: setattr(self._unbind(), name, value))
+
+    storage, shape, strides, offset = _field("_storage"), _field("_shape"), _field("_strides"), _field("_offset")
+    del _field
+
+    def __eq__(self, other) -> bool:
+        if not isinstance(other, View):
+            return NotImplemented
+        return (self.storage, self.shape, self.strides, self.offset) == (other.storage, other.shape, other.strides, other.offset)
+
+    __hash__ = None
 
     def desc(self) -> Desc:
-        return Desc.from_buffer_copy(self.packed())
+        import torch
+
+        dt = INT64 if self.storage.dtype == torch.int64 else FLOAT32
+        return make_desc(self.storage.data_ptr(), self.storage.numel(), dt, self.shape, self.strides, self.offset)
 
     def packed(self) -> bytes:
         """The view's descriptor as the bytes of an mtc_desc, in one pack: a call of small
-        tensors costs what its descriptors do."""
+        tensors costs what its descriptors do.  Float32 and Int64 alone."""
         t = self._tensor
         if t is not None:
             dtype = _DTYPES.get(t.dtype)
@@ -186,8 +192,6 @@ class View:
 
     def tensor(self):
         """The same view as a torch tensor (for zero/positive strides)."""
-        if self._tensor is not None:
-            return self._tensor
         return self.storage.as_strided(self.shape, self.strides, self.offset)
 
 

@@ -162,3 +162,24 @@ def test_python_wrapper_turns_refusals_into_exceptions():
         abi.clip_global_norm([v(3)], 1.0, outs=[], stream=0)
     with pytest.raises(ValueError, match="max_norm"):
         abi.clip_global_norm([v(3)], -1.0, stream=0)
+
+
+def test_views_of_tensors_keep_their_fields():
+    """A view made of a tensor has the fields of one made of a storage, which can be set."""
+    import torch
+
+    t = torch.arange(12.0).reshape(3, 4)[1:, ::2]
+    v = abi.View.of(t)
+    bound = v.packed()
+    assert (v.shape, v.strides, v.offset) == ((2, 2), (4, 2), 4) and v.storage.numel() == 12
+    assert v.packed() == bound and bytes(v.desc()) == bound
+    assert torch.equal(v.tensor(), t)
+    v.offset = 1
+    assert v.tensor().tolist() == [[1.0, 3.0], [5.0, 7.0]]
+    s = torch.zeros(6)
+    assert abi.View(s, (2, 3), (3, 1)) == abi.View.contiguous(s, (2, 3))
+    assert abi.View.of(torch.ones(2, requires_grad=True)).tensor().requires_grad is False
+    words = abi.View.of(torch.zeros(3, dtype=torch.int32))  # 4-byte words, as the bitwise copies take them
+    assert words.desc().dtype == abi.FLOAT32
+    with pytest.raises(ValueError, match="int32"):
+        words.packed()
