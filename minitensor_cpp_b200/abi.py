@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+from dataclasses import dataclass, field
 from pathlib import Path
 from typing import Sequence
 
@@ -52,21 +53,20 @@ class Desc(ctypes.Structure):
     ]
 
 
-_DESC = struct.Struct("@Pqqii8q8q")
-_PAD = [(0,) * (MAX_RANK - rank) for rank in range(MAX_RANK + 1)]
-assert _DESC.size == ctypes.sizeof(Desc)
+# mtc_desc by rank: the unused extents and strides are padding (zeros)
+_DESC = [struct.Struct(f"@Pqqii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x") for r in range(MAX_RANK + 1)]
+assert all(s.size == ctypes.sizeof(Desc) for s in _DESC)
 
 
 _DTYPES: dict = {}
 
 
-def _dtype_code(dtype) -> int:
-    import torch
+def _dtypes() -> dict:
+    if not _DTYPES:
+        import torch
 
-    _DTYPES.update({torch.float32: FLOAT32, torch.int64: INT64})
-    if dtype not in _DTYPES:
-        raise ValueError(f"{dtype} operands are not supported: Float32 or Int64")
-    return _DTYPES[dtype]
+        _DTYPES.update({torch.float32: FLOAT32, torch.int64: INT64})
+    return _DTYPES
 
 
 class Instr(ctypes.Structure):
@@ -106,55 +106,59 @@ def contiguous_strides(shape: Sequence[int]) -> list[int]:
     return strides
 
 
+def _flat(memory, dtype):
+    """A storage as a flat tensor."""
+    import torch
+
+    return torch.empty(0, dtype=dtype, device=memory.device).set_(memory)
+
+
+@dataclass
 class View:
     """A strided view of a flat storage tensor (torch tensor, on any device)."""
 
-    __slots__ = ("_tensor", "_storage", "_shape", "_strides", "_offset")
-
-    def __init__(self, storage, shape: tuple, strides: tuple, offset: int = 0):
-        self._tensor = None
-        self._storage = storage  # torch.Tensor, 1-D
-        self._shape = shape
-        self._strides = strides
-        self._offset = offset
-
-    def __repr__(self) -> str:
-        return f"View(shape={self.shape}, strides={self.strides}, offset={self.offset}, storage={self.storage!r})"
+    storage: "object"  # torch.Tensor, 1-D
+    shape: tuple
+    strides: tuple
+    offset: int = field(default_factory=int)
 
     @staticmethod
     def of(t) -> "View":
-        """View of an existing torch tensor (shares its storage)."""
+        """View of an existing torch tensor as it is now (shares its storage)."""
+        memory, dtype, shape = t.untyped_storage(), t.dtype, t.shape
+        rank, strides, offset = len(shape), t.stride(), t.storage_offset()
+        code = (_DTYPES or _dtypes()).get(dtype)
+        if code is None or rank > MAX_RANK:
+            return View(_flat(memory, dtype), tuple(shape), strides, offset)
+        # The descriptor is packed at once, and the fields and the flat tensor are made when they
+        # are asked for: that one tensor costs as much as a small call's launch.
+        ptr = memory.data_ptr()
         v = _new_view(View)
-        v._tensor = t
+        v.__dict__["_of"] = (ptr, memory, _DESC[rank].pack(ptr, offset, memory.nbytes() >> (3 if code == INT64 else 2),
+                                                           code, rank, *shape, *strides), dtype, rank)
         return v
+
+    def __getattr__(self, name):
+        fields = self.__dict__
+        if name not in ("storage", "shape", "strides", "offset") or "_of" not in fields:
+            raise AttributeError(f"{type(self).__name__!r} object has no attribute {name!r}")
+        _, memory, packed, dtype, rank = fields["_of"]
+        if name == "storage":
+            fields["storage"] = _flat(memory, dtype)
+        else:
+            _, fields["offset"], _, _, _, *axes = _DESC[rank].unpack(packed)
+            fields["shape"], fields["strides"] = tuple(axes[:rank]), tuple(axes[rank:])
+        return fields[name]
+
+    def __setattr__(self, name, value):
+        if "_of" in self.__dict__:
+            self.storage, self.shape  # the fields that are not set stay what the view was made with
+            del self.__dict__["_of"]
+        object.__setattr__(self, name, value)
 
     @staticmethod
     def contiguous(storage, shape, offset: int = 0) -> "View":
         return View(storage, tuple(shape), tuple(contiguous_strides(shape)), offset)
-
-    def _unbind(self) -> "View":
-        """Takes the fields over from the tensor that the view was made of."""
-        t = self._tensor
-        if t is not None:
-            import torch
-
-            self._storage = torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage())
-            self._shape, self._strides, self._offset = tuple(t.shape), tuple(t.stride()), t.storage_offset()
-            self._tensor = None
-        return self
-
-    def _field(name):
-        return property(lambda self: getattr(self._unbind(), name), lambda self, value: setattr(self._unbind(), name, value))
-
-    storage, shape, strides, offset = _field("_storage"), _field("_shape"), _field("_strides"), _field("_offset")
-    del _field
-
-    def __eq__(self, other) -> bool:
-        if not isinstance(other, View):
-            return NotImplemented
-        return (self.storage, self.shape, self.strides, self.offset) == (other.storage, other.shape, other.strides, other.offset)
-
-    __hash__ = None
 
     def desc(self) -> Desc:
         import torch
@@ -165,30 +169,19 @@ class View:
     def packed(self) -> bytes:
         """The view's descriptor as the bytes of an mtc_desc, in one pack: a call of small
         tensors costs what its descriptors do.  Float32 and Int64 alone."""
-        t = self._tensor
-        if t is not None:
-            dtype = _DTYPES.get(t.dtype)
-            if dtype is None:
-                dtype = _dtype_code(t.dtype)
-            shape = t.shape
-            rank = len(shape)
-            if rank > MAX_RANK:
-                raise ValueError("shape/strides rank mismatch or rank > 8")
-            pad = _PAD[rank]
-            if t.is_contiguous():  # its own elements are all that the view reaches
-                return _DESC.pack(t.data_ptr(), 0, t.numel(), dtype, rank, *shape, *pad, *t.stride(), *pad)
-            s = t.untyped_storage()
-            return _DESC.pack(s.data_ptr(), t.storage_offset(), s.nbytes() // (8 if dtype == INT64 else 4), dtype, rank,
-                              *shape, *pad, *t.stride(), *pad)
-        t = self._storage
-        dtype = _DTYPES.get(t.dtype)
-        if dtype is None:
-            dtype = _dtype_code(t.dtype)
-        rank = len(self._shape)
-        if rank != len(self._strides) or rank > MAX_RANK:
+        of = self.__dict__.get("_of")
+        if of is not None:
+            if of[1].data_ptr() == of[0]:  # (a storage that was resized since lies elsewhere)
+                return of[2]
+        storage = self.storage
+        rank = len(self.shape)
+        if rank != len(self.strides) or rank > MAX_RANK:
             raise ValueError("shape/strides rank mismatch or rank > 8")
-        pad = _PAD[rank]
-        return _DESC.pack(t.data_ptr(), self._offset, t.numel(), dtype, rank, *self._shape, *pad, *self._strides, *pad)
+        code = _dtypes().get(storage.dtype)
+        if code is None:
+            raise ValueError(f"{storage.dtype} operands are not supported: Float32 or Int64")
+        return _DESC[rank].pack(storage.data_ptr(), self.offset, storage.numel(), code, rank, *self.shape,
+                                *self.strides)
 
     def tensor(self):
         """The same view as a torch tensor (for zero/positive strides)."""
@@ -330,10 +323,12 @@ def _stream(stream):
     if stream is None:
         import torch
 
-        # the handle alone: a Stream object costs more than a small call's launch
-        if not torch.cuda.is_initialized():
-            torch.cuda.init()
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        # the handle alone, where this torch has a function for it: a Stream object costs more
+        # than a small call's launch
+        handle = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if handle is None:
+            return torch.cuda.current_stream().cuda_stream
+        return handle(torch.cuda.current_device())
     return ctypes.c_void_p(int(stream))
 
 
@@ -342,13 +337,20 @@ def _stream(stream):
 # with its ctypes arguments converted once: repeated calls then cost one ctypes
 # dispatch, so back-to-back launches keep the GPU busy in timing loops.
 
+_FUNCTIONS: dict = {}
+
+
 def _run(name: str, args: tuple, what: str, prepare: bool):
-    fn = getattr(lib(), name)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(lib(), name)
     if prepare:
         def call() -> None:
             check(fn(*args), what)
         return call
-    check(fn(*args), what)
+    rc = fn(*args)
+    if rc != OK:
+        check(rc, what)
     return None
 
 
@@ -417,8 +419,8 @@ def embedding(table: View, tokens: View, out: View, scale: float = 1.0, padding_
 def embedding_grad(dout: View, tokens: View, dtable: View, scale: float = 1.0, padding_token: int | None = None,
                    accumulate: bool = False, stream=None, prepare: bool = False):
     """dtable[v, :] = scale * the sum of dout over v's positions (added to dtable with `accumulate`)."""
-    return _run("mtc_embedding_grad", (_ref(dout), _ref(tokens), scale, _token(padding_token), int(accumulate),
-                                       _ref(dtable), _stream(stream)), "embedding_grad", prepare)
+    return _run("mtc_embedding_grad", (d_ref(out), _ref(tokens), scale, _token(padding_token), int(accumulate),
+                                       d_ref(table), _stream(stream)), "embedding_grad", prepare)
 
 
 def linear_cross_entropy(x: View, weight: View, targets: View, loss: View, bias: View | None = None,
@@ -435,7 +437,7 @@ def linear_cross_entropy_grad(x: View, weight: View, targets: View, dloss: View,
                               stream=None, prepare: bool = False):
     """linear_cross_entropy with the gradients of sum(dloss * loss) for x, weight and bias."""
     return _run("mtc_linear_cross_entropy_grad",
-                (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target), _ref(dloss), _ref(loss),
+                (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target), d_ref(loss), _ref(loss),
                  _ref(lse), _ref(dx), _ref(dweight), _ref(dbias), _stream(stream)), "linear_cross_entropy_grad", prepare)
 
 

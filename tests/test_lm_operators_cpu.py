@@ -183,3 +183,46 @@ def test_views_of_tensors_keep_their_fields():
     assert words.desc().dtype == abi.FLOAT32
     with pytest.raises(ValueError, match="int32"):
         words.packed()
+
+
+def test_views_of_tensors_are_made_when_they_are_made():
+    """What is done to the tensor afterwards is not done to the view: its shape, strides and
+    offset are the tensor's at the time, and it holds the memory but no autograd graph."""
+    import dataclasses
+    import gc
+    import weakref
+
+    import torch
+
+    def fields(v):
+        return v.offset, v.shape, v.strides, v.storage.data_ptr(), v.storage.numel()
+
+    t = torch.arange(12.0).reshape(3, 4)[1:, 1:]
+    want = (5, (2, 3), (4, 1), t.data_ptr() - 20, 12)
+    first, v = abi.View.of(t), abi.View.of(t)
+    before = first.packed()
+    assert abi.View.of(t).offset == 5  # the first field that is asked for
+    t.t_()
+    assert v.packed() == before and fields(v) == want
+    t.resize_(2)
+    assert first.packed() == before and fields(first) == want
+    other = abi.View.of(t)
+    t.set_(torch.zeros(7))
+    assert other.shape == (2,) and other.storage.numel() == 12
+    moved = torch.zeros(3)
+    held = abi.View.of(moved)
+    moved.resize_(100)  # the same storage, elsewhere by now: the view goes with it
+    assert held.packed() == bytes(held.desc()) and held.storage.data_ptr() == moved.data_ptr()
+    x = torch.ones(4, requires_grad=True)
+    y = x * 2
+    graph = weakref.ref(y)
+    v = abi.View.of(y)
+    del y
+    gc.collect()
+    assert graph() is None and v.tensor().tolist() == [2.0] * 4
+    assert dataclasses.is_dataclass(v) and [f.name for f in dataclasses.fields(v)] == ["storage", "shape", "strides", "offset"]
+    assert dataclasses.replace(v, offset=1, shape=(3,)).tensor().tolist() == [2.0] * 3
+    v.note = "as any object"
+    assert v.note == "as any object" and v.packed() == bytes(v.desc())
+    with pytest.raises(AttributeError, match="stride"):
+        v.stride
