@@ -419,8 +419,8 @@ def embedding(table: View, tokens: View, out: View, scale: float = 1.0, padding_
 def embedding_grad(dout: View, tokens: View, dtable: View, scale: float = 1.0, padding_token: int | None = None,
                    accumulate: bool = False, stream=None, prepare: bool = False):
     """dtable[v, :] = scale * the sum of dout over v's positions (added to dtable with `accumulate`)."""
-    return _run("mtc_embedding_grad", (d_ref(out), _ref(tokens), scale, _token(padding_token), int(accumulate),
-                                       d_ref(table), _stream(stream)), "embedding_grad", prepare)
+    return _run("mtc_embedding_grad", (_ref(dout), _ref(tokens), scale, _token(padding_token), int(accumulate),
+                                       _ref(dtable), _stream(stream)), "embedding_grad", prepare)
 
 
 def linear_cross_entropy(x: View, weight: View, targets: View, loss: View, bias: View | None = None,
@@ -437,7 +437,7 @@ def linear_cross_entropy_grad(x: View, weight: View, targets: View, dloss: View,
                               stream=None, prepare: bool = False):
     """linear_cross_entropy with the gradients of sum(dloss * loss) for x, weight and bias."""
     return _run("mtc_linear_cross_entropy_grad",
-                (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target), d_ref(loss), _ref(loss),
+                (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target), _ref(dloss), _ref(loss),
                  _ref(lse), _ref(dx), _ref(dweight), _ref(dbias), _stream(stream)), "linear_cross_entropy_grad", prepare)
 
 

@@ -226,3 +226,29 @@ def test_views_of_tensors_are_made_when_they_are_made():
     assert v.note == "as any object" and v.packed() == bytes(v.desc())
     with pytest.raises(AttributeError, match="stride"):
         v.stride
+
+
+def test_python_wrappers_hand_every_operand_over():
+    """Calls without work: each wrapper's operands arrive in their places."""
+    import torch
+
+    v = lambda *s: abi.View.of(torch.zeros(*s))
+    t = lambda *s: abi.View.of(torch.zeros(*s, dtype=torch.int64))
+    abi.embedding(v(4, 3), t(0), v(0, 3), stream=0)
+    abi.embedding_grad(v(5, 0), t(5), v(4, 0), stream=0)
+    abi.linear_cross_entropy(v(0, 3), v(4, 3), t(0), v(0), bias=v(4), lse=v(0), stream=0)
+    abi.linear_cross_entropy_grad(v(0, 3), v(0, 3), t(0), v(0), dx=v(0, 3), dweight=v(0, 3), bias=v(0), dbias=v(0),
+                                  loss=v(0), lse=v(0), stream=0)
+    abi.clip_global_norm([v(0)], 1.0, stream=0)
+    for bad in ({"bias": v(3)}, {"lse": v(1)}):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            abi.linear_cross_entropy(v(0, 3), v(4, 3), t(0), v(0), stream=0, **bad)
+    for name in ("dx", "dweight", "dbias", "bias", "loss", "lse"):
+        with pytest.raises(ValueError, match=name):
+            abi.linear_cross_entropy_grad(v(0, 3), v(4, 3), t(0), v(0), stream=0, **{name: v(7)})
+    with pytest.raises(ValueError, match="dloss"):
+        abi.linear_cross_entropy_grad(v(0, 3), v(4, 3), t(0), v(1), stream=0)
+    with pytest.raises(ValueError, match="norm"):
+        abi.global_norm([v(3)], v(2), stream=0)
+    with pytest.raises(ValueError, match="null"):
+        abi.embedding_grad(None, t(5), v(4, 3), stream=0)
