@@ -40,7 +40,9 @@ std::vector<DeviceState> g_devices;
 // order instead of going to the driver: a block freed on stream S is handed to
 // the next request on S at once (everything that used it is queued before
 // anything that will), and a block freed on another stream becomes reusable by
-// every stream when an event recorded at the free has completed.  Requests of
+// every stream when an event recorded at the free has completed.  The handle of
+// the default stream is null: the blocks of any stream have a key of their own.
+// Requests of
 // 1 MiB or less are rounded to 512 bytes, larger ones to 2 MiB; the best fit
 // whose size is within 1/8 (at least 2 MiB) of the request is reused whole.
 // cudaMalloc is called only when nothing fits; when it fails, the unused cached
@@ -52,6 +54,9 @@ struct Block {
     cudaStream_t stream = nullptr;  // stream of the last owner
 };
 
+// Key of the blocks that no queued work uses; no stream's handle.
+const cudaStream_t kAnyStream = reinterpret_cast<cudaStream_t>(~uintptr_t(0));
+
 struct PendingFree {
     Block block;
     cudaEvent_t done = nullptr;
@@ -60,7 +65,7 @@ struct PendingFree {
 struct DevicePool {
     using FreeList = std::multimap<size_t, Block>;
     std::mutex mu;
-    // free blocks reusable by one stream (stream order) or, key nullptr, by any stream
+    // free blocks reusable by one stream (stream order) or, key kAnyStream, by any stream
     std::vector<std::pair<cudaStream_t, std::unique_ptr<FreeList>>> free_lists;
     // every free block by address, for taking one back by address (graph replay)
     std::unordered_map<void *, std::pair<FreeList *, FreeList::iterator>> free_at;
@@ -125,8 +130,8 @@ void collect_pending(DevicePool &pool) {
         PendingFree &pf = pool.pending[i];
         if (cudaEventQuery(pf.done) == cudaSuccess) {
             Block b = pf.block;
-            b.stream = nullptr;
-            pool.put_free(nullptr, b);
+            b.stream = kAnyStream;
+            pool.put_free(kAnyStream, b);
             pool.spare_events.push_back(pf.done);
             pool.pending[i] = pool.pending.back();
             pool.pending.pop_back();
@@ -164,7 +169,7 @@ int pool_alloc(int device, size_t bytes, cudaStream_t stream, void **ptr) {
     if (!pool.pending.empty()) collect_pending(pool);
     Block b;
     bool hit = take_fit(pool, stream, want, b);
-    if (!hit) hit = take_fit(pool, nullptr, want, b);
+    if (!hit) hit = take_fit(pool, kAnyStream, want, b);
     if (hit) {
         pool.cached -= b.size;
     } else {
@@ -234,8 +239,8 @@ int take_locked(DevicePool &pool, int device, void *ptr, size_t bytes, cudaStrea
     if (f == pool.free_at.end()) return fail(MTC_ERR_UNSUPPORTED, "device %d: %p is not a free block", device, ptr);
     DevicePool::FreeList *fl = f->second.first;
     auto it = f->second.second;
-    const bool usable = fl == &pool.list_for(stream) || fl == &pool.list_for(nullptr) ||
-                        (fl == &pool.parked && (it->second.stream == stream || it->second.stream == nullptr));
+    const bool usable = fl == &pool.list_for(stream) || fl == &pool.list_for(kAnyStream) ||
+                        (fl == &pool.parked && (it->second.stream == stream || it->second.stream == kAnyStream));
     if (!usable) return fail(MTC_ERR_UNSUPPORTED, "device %d: %p was released on another stream", device, ptr);
     Block b = it->second;
     if (b.size < want) return fail(MTC_ERR_UNSUPPORTED, "device %d: the block at %p is too small", device, ptr);

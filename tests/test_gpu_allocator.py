@@ -101,3 +101,22 @@ def test_freeing_an_unknown_pointer_is_an_error(cuda):
     with pytest.raises(ValueError):
         _free(a + 512, s)
     _free(a, s)
+
+
+def test_blocks_of_the_default_stream_are_not_any_streams(cuda):
+    """The default stream's handle is null.  A block freed on it is the default stream's alone
+    until that stream has passed the free: a stream that does not wait for the default one
+    gets other memory, or both would work in the same block at once."""
+    import torch
+
+    other = torch.cuda.Stream().cuda_stream
+    abi.check(abi.lib().mtc_pool_trim(0), "trim")
+    a = _alloc(8 << 20, None)
+    _free(a, None)
+    b = _alloc(8 << 20, other)
+    assert b != a
+    c = _alloc(8 << 20, None)
+    assert c == a
+    _free(b, other)
+    _free(c, None)
+    abi.check(abi.lib().mtc_pool_trim(0), "trim")
