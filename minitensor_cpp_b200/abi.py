@@ -55,17 +55,18 @@ class Desc(ctypes.Structure):
 
 # mtc_desc by rank: the unused extents and strides are padding (zeros)
 _DESC = [struct.Struct(f"@Pqqii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x") for r in range(MAX_RANK + 1)]
+_PACK = [s.pack for s in _DESC]
 assert all(s.size == ctypes.sizeof(Desc) for s in _DESC)
 
 
-_DTYPES: dict = {}
+_DTYPES: dict = {}  # torch dtype -> (code, binary logarithm of its size)
 
 
 def _dtypes() -> dict:
     if not _DTYPES:
         import torch
 
-        _DTYPES.update({torch.float32: FLOAT32, torch.int64: INT64})
+        _DTYPES.update({torch.float32: (FLOAT32, 2), torch.int64: (INT64, 3)})
     return _DTYPES
 
 
@@ -113,8 +114,14 @@ def _flat(memory, dtype):
     return torch.empty(0, dtype=dtype, device=memory.device).set_(memory)
 
 
+class _OfTensor:
+    """What a view made of a tensor was made of, beside its fields."""
+
+    __slots__ = ("_of",)
+
+
 @dataclass
-class View:
+class View(_OfTensor):
     """A strided view of a flat storage tensor (torch tensor, on any device)."""
 
     storage: "object"  # torch.Tensor, 1-D
@@ -126,23 +133,26 @@ class View:
     def of(t) -> "View":
         """View of an existing torch tensor as it is now (shares its storage)."""
         memory, dtype, shape = t.untyped_storage(), t.dtype, t.shape
-        rank, strides, offset = len(shape), t.stride(), t.storage_offset()
+        rank = len(shape)
         code = (_DTYPES or _dtypes()).get(dtype)
         if code is None or rank > MAX_RANK:
-            return View(_flat(memory, dtype), tuple(shape), strides, offset)
+            return View(_flat(memory, dtype), tuple(shape), t.stride(), t.storage_offset())
         # The descriptor is packed at once, and the fields and the flat tensor are made when they
         # are asked for: that one tensor costs as much as a small call's launch.
         ptr = memory.data_ptr()
         v = _new_view(View)
-        v.__dict__["_of"] = (ptr, memory, _DESC[rank].pack(ptr, offset, memory.nbytes() >> (3 if code == INT64 else 2),
-                                                           code, rank, *shape, *strides), dtype, rank)
+        _set_of(v, (ptr, memory, _PACK[rank](ptr, t.storage_offset(), memory.nbytes() >> code[1], code[0], rank, *shape,
+                                             *t.stride()), dtype, rank))
         return v
 
     def __getattr__(self, name):
-        fields = self.__dict__
-        if name not in ("storage", "shape", "strides", "offset") or "_of" not in fields:
+        if name == "_of":
+            return None
+        of = self._of
+        if of is None or name not in ("storage", "shape", "strides", "offset"):
             raise AttributeError(f"{type(self).__name__!r} object has no attribute {name!r}")
-        _, memory, packed, dtype, rank = fields["_of"]
+        _, memory, packed, dtype, rank = of
+        fields = self.__dict__
         if name == "storage":
             fields["storage"] = _flat(memory, dtype)
         else:
@@ -151,9 +161,9 @@ class View:
         return fields[name]
 
     def __setattr__(self, name, value):
-        if "_of" in self.__dict__:
+        if self._of is not None:
             self.storage, self.shape  # the fields that are not set stay what the view was made with
-            del self.__dict__["_of"]
+            _set_of(self, None)
         object.__setattr__(self, name, value)
 
     @staticmethod
@@ -169,10 +179,9 @@ class View:
     def packed(self) -> bytes:
         """The view's descriptor as the bytes of an mtc_desc, in one pack: a call of small
         tensors costs what its descriptors do.  Float32 and Int64 alone."""
-        of = self.__dict__.get("_of")
-        if of is not None:
-            if of[1].data_ptr() == of[0]:  # (a storage that was resized since lies elsewhere)
-                return of[2]
+        of = self._of
+        if of is not None and of[1].data_ptr() == of[0]:  # (a storage that was resized since lies elsewhere)
+            return of[2]
         storage = self.storage
         rank = len(self.shape)
         if rank != len(self.strides) or rank > MAX_RANK:
@@ -180,15 +189,14 @@ class View:
         code = _dtypes().get(storage.dtype)
         if code is None:
             raise ValueError(f"{storage.dtype} operands are not supported: Float32 or Int64")
-        return _DESC[rank].pack(storage.data_ptr(), self.offset, storage.numel(), code, rank, *self.shape,
-                                *self.strides)
+        return _PACK[rank](storage.data_ptr(), self.offset, storage.numel(), code[0], rank, *self.shape, *self.strides)
 
     def tensor(self):
         """The same view as a torch tensor (for zero/positive strides)."""
         return self.storage.as_strided(self.shape, self.strides, self.offset)
 
 
-_new_view = object.__new__
+_new_view, _set_of = object.__new__, _OfTensor._of.__set__
 
 
 class MtcError(RuntimeError):
@@ -405,6 +413,11 @@ def _ref(v: View | None):
     return None if v is None else v.packed()
 
 
+def _packed_all(views: Sequence[View]) -> bytes:
+    # (as View.packed does it, without a call for each of many tensors)
+    return b"".join([of[2] if (of := v._of) is not None and of[1].data_ptr() == of[0] else v.packed() for v in views])
+
+
 def _token(t: int | None) -> int:
     return NO_TOKEN if t is None else int(t)
 
@@ -443,17 +456,17 @@ def linear_cross_entropy_grad(x: View, weight: View, targets: View, dloss: View,
 
 def global_norm(tensors: Sequence[View], norm: View, stream=None, prepare: bool = False):
     """norm = sqrt of the sum of squares of all elements of all tensors."""
-    arr = b"".join([v.packed() for v in tensors])
+    arr = _packed_all(tensors)
     return _run("mtc_global_norm", (arr, len(tensors), _ref(norm), _stream(stream)), "global_norm", prepare)
 
 
 def clip_global_norm(tensors: Sequence[View], max_norm: float, norm: View | None = None,
                      outs: Sequence[View] | None = None, stream=None, prepare: bool = False):
     """Scales the tensors by max_norm / norm where their global norm exceeds max_norm; into `outs`, or in place."""
-    arr = b"".join([v.packed() for v in tensors])
+    arr = _packed_all(tensors)
     if outs is not None and len(outs) != len(tensors):
         raise ValueError(f"{len(outs)} outputs for {len(tensors)} tensors")
-    to = arr if outs is None else b"".join([v.packed() for v in outs])
+    to = arr if outs is None else _packed_all(outs)
     return _run("mtc_clip_global_norm", (arr, len(tensors), max_norm, to, _ref(norm), _stream(stream)),
                 "clip_global_norm", prepare)
 
