@@ -617,6 +617,45 @@ def test_rows_sure_of_their_class_keep_the_digits_of_what_is_left(cuda, n, vocab
     within(got["dw"][:, 0], n * g, (rel + 2 * U * n) * n * g.abs() + n * step, "dw")
 
 
+@pytest.mark.parametrize("n, vocab, dim", [(300, 100, 512), (300, 128, 512), (600, 1000, 96), (60, 200, 4096), (17, 900, 400)])
+@pytest.mark.parametrize("gap", [3.0, 11.5, 18.0])
+def test_rows_sure_of_their_class_on_the_tensor_cores(cuda, n, vocab, dim, gap):
+    """The same where the sums of exponentials are taken 128 classes at a time, logits split along
+    the columns among them: the digits of what is left come from a sum that the largest logit's 1
+    is not part of.
+
+    The logits are exact, and so are their differences.  An exponential, 2^x by the hardware within
+    2^-22 (4u) of an argument that two roundings put off by u |x| each, is within (2 |x| + 4) u; 36
+    additions of positive terms are within 36u, the joining exponential within 4u: the sum of the
+    others is within (2 |x| + 46) u of itself, its log1p and exponentials of it within 6u more.
+    (From an eighth of the largest on, the others may share a sum with it: the 36u of 1 + rest are
+    9 times as much of the rest.)
+    The gradient's pairs hold 2^-22 of it and 2^-48 of the largest |dloss|."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 28)
+    steps = torch.round(w[:, :1] * 8).clamp(-16, 16) / 8
+    x, w = torch.zeros_like(x), torch.zeros_like(w)
+    x[:, 0], w[:, :1] = 1.0, steps
+    w[vocab // 2, 0] = 3.0 + gap
+    t = torch.full_like(t, vocab // 2)
+    dloss = torch.ones_like(dloss)
+    got = run_ce(x, w, None, t, dloss)
+    alone = run_ce(x, w, None, t, None)
+    assert torch.equal(alone["loss"], got["loss"]) and torch.equal(alone["lse"], got["lse"])
+    z = w[:, 0].double()
+    logp = z - torch.logsumexp(z, 0)
+    others = torch.arange(vocab, device=cuda) != vocab // 2
+    rest = torch.logsumexp(z[others], 0) - torch.logsumexp(z, 0)
+    g = torch.where(others, logp.exp(), -rest.exp())
+    shared = 36 * 8 if rest.exp() / (1 - rest.exp()) > 0.12 else 0
+    rel = U * (2 * logp.abs().max() + 52 + 4 * 4 + shared)
+    loss = -torch.log1p(-rest.exp())
+    within(got["loss"], loss.expand(n), (rel * loss).expand(n), "loss")
+    within(got["db"], n * g, (rel + 2 * U * n) * n * g.abs(), "db")
+    within(got["dw"][:, 0], n * g, (rel + 2 * U * (n + 16)) * n * g.abs() + n * 2.0 ** -48, "dw")
+
+
 @pytest.mark.parametrize("n, vocab, dim", [(2 ** 21 - 1, 1, 1), (2 ** 21 - 1, 2, 0), (2 ** 20, 3, 0), (2 ** 20 - 1, 3, 0)])
 def test_more_rows_than_a_grid_has_parts(cuda, n, vocab, dim):
     """Where 32 rows a CTA would be more than the 65535 parts of a launch's second axis."""
