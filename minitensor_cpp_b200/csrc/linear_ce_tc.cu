@@ -35,7 +35,8 @@
 //   dx       dx = g' w'     A = g' K-major,  B = w' MN-major     split along V when the tiles are few
 //   dweight  dw = g'^T x'   A = g' MN-major, B = x' MN-major     added up over the pieces of the rows
 // The logits of one piece of the rows are written once, as float32; k_softmax_grad
-// turns them into g' in place, 256 bytes of z into 128 of hi and 128 of lo.
+// turns them into g', 256 bytes of z into 128 of hi and 128 of lo, on one scale a row for dx and
+// on one a class and 256 rows for dweight.
 //
 // A pair of CTAs works on a 256 x 256 tile (tcgen05.mma.cta_group::2): each stages its
 // own 128 rows of A and 128 columns of B, 64 KB for 1536 clocks of MMAs.  The lo halves
@@ -96,9 +97,9 @@ __device__ __forceinline__ void split_pair(float x, __half &hi, __half &lo) {
     lo = __float2half_rn((x - __half2float(hi)) * 2048.0f);
 }
 
-// What the device knows of the scales, behind the count of the live rows.
-enum Known { kLargest = 1, kSampled = 4, kExponent = 6 };  // of x, weight (and of dloss: kLargest, kExponent)
-static_assert(kExponent + 3 == kLiveKnown, "zeroed with the count");
+// What the device knows of the scales of x and weight, behind the count of the live rows.
+enum Known { kLargest = 1, kSampled = 3, kExponent = 5 };
+static_assert(kExponent + 2 == kLiveKnown, "zeroed with the count");
 
 struct PackSource {
     const float *p;
@@ -118,7 +119,6 @@ struct PackArgs {
     int64_t first_of_second;  // blocks of the grid before the second tensor
     int *known;               // the live rows' count and what follows it
     int headroom;             // powers of two above the sample; 0: it is the whole
-    const float *dloss;       // its largest magnitude too; null: none
     float *dx;                // its rows without a loss become zero; null: not wanted
     int64_t dx_rs, dx_cs;
     int dx_vec;
@@ -166,7 +166,7 @@ __device__ __forceinline__ int last_exponent(const PackArgs &a, int which) {
 }
 
 // Largest finite magnitudes of x (rows with a loss) and weight over a sample of the rows, one
-// a warp, and of dloss; the zero rows of dx.  7 to 30 us for 1184 rows of 1024 to 8192 columns,
+// a warp; the zero rows of dx.  7 to 30 us for 1184 rows of 1024 to 8192 columns,
 // a warp's latency.
 __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     wait_for_previous();
@@ -232,11 +232,6 @@ __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
             }
         }
     }
-    if (a.dloss != nullptr && blockIdx.x == 0) {
-        float m = 0.0f;
-        for (int i = threadIdx.x; i < a.known[0]; i += 256) m = fmaxf(m, finite_abs(a.dloss[i]));
-        keep_max(m, a.known + kLargest + 2);
-    }
 }
 
 // Each half-warp packs one block of 64 columns at a time: a lane four columns.  AGAIN: only
@@ -245,10 +240,8 @@ __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
 template <bool AGAIN>
 __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     wait_for_previous();
-    if ((AGAIN || a.headroom == 0) && blockIdx.x == 0 && threadIdx.x < 3)
-        a.known[kExponent + threadIdx.x] = threadIdx.x == 2 ? scale_exponent(a.known[kLargest + 2])
-                                           : AGAIN          ? last_exponent(a, threadIdx.x)
-                                                            : first_exponent(a, threadIdx.x);
+    if ((AGAIN || a.headroom == 0) && blockIdx.x == 0 && threadIdx.x < 2)
+        a.known[kExponent + threadIdx.x] = AGAIN ? last_exponent(a, threadIdx.x) : first_exponent(a, threadIdx.x);
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
     const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
@@ -316,7 +309,10 @@ struct TileArgs {
     int tiles_n;
     int group;        // row tiles that share a sweep of the columns
     int splits;       // of K
-    const int *exp_a, *exp_b;  // exponents of the operands' scales
+    // Exponents of the operands' scales: one for a packed tensor, and of g' one a row as the rows
+    // of dx, or one a class and piece of K as the rows of dweight.
+    const int *exp_a, *exp_b;
+    int64_t exp_pitch;  // [pieces][exp_pitch]
     unsigned long long *err;
     // Logits
     float *z;         // [M][z_pitch], null: statistics alone
@@ -399,6 +395,7 @@ __device__ __forceinline__ Extent extent_of(const TileArgs &a) {
     e.units = e.tiles * a.splits;
     if (a.live_k && K == 0 && a.first > 0) e.units = 0;  // nothing left to add
     e.per_split = (e.kblocks + a.splits - 1) / a.splits;
+    if (a.live_k) e.per_split = (e.per_split + kPieceBlocks - 1) / kPieceBlocks * kPieceBlocks;  // the pieces of g'
     return e;
 }
 
@@ -622,19 +619,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const int quadrant = warp % 4, half = (warp - 4) / 4;
         const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
-        const int scale = -(*args.exp_a + *args.exp_b);
-        const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
-        const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
+        const int exp_b = *args.exp_b;
         int64_t piece = 0;
         bool ok = true;
         for (int64_t u = cluster; u < e.units && ok; u += clusters) {
             int tm, tn, split, kb0, kb1;
             unit_of(args, e, u, tm, tn, split, kb0, kb1);
+            const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
             for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
                 const int b = static_cast<int>(piece & 1);
+                float unscale = 1.0f;  // of a class's row in this piece
+                if (A_MN && row < e.M)
+                    unscale = power_of_two(-args.exp_a[static_cast<int64_t>(kb / kPieceBlocks) * args.exp_pitch + row]);
                 if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(piece >> 1) & 1u, abort_flag)) {
                     ok = false;
                     break;
@@ -647,14 +646,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
                     uint32_t v[64];
                     tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) acc[c * 64 + j] += __uint_as_float(v[j]);
+                    for (int j = 0; j < 64; ++j)
+                        acc[c * 64 + j] = A_MN ? fmaf(__uint_as_float(v[j]), unscale, acc[c * 64 + j])
+                                               : acc[c * 64 + j] + __uint_as_float(v[j]);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_remote(release[b]);
             }
             if (!ok) break;
-            const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
+            const int scale = -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
+            const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
+            const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
             const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
             if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, f0, f1);
             else store_sum(args, e.M, acc, row, col0, split, f0, f1);
@@ -894,6 +897,8 @@ struct RowArgs {
     const float *part_max, *part_rest, *z_target;
     const int *row;       // of x
     LogSum *lse_live;     // [rows]
+    const float *dloss;   // null: no gradients
+    int *row_exp;         // [rows] exponent of the scale of g' as the rows of dx
     float *loss, *lse;
     int64_t loss_s, lse_s;
 };
@@ -914,104 +919,148 @@ __global__ void __launch_bounds__(256) k_row_loss(const RowArgs a) {
     if (lane != 0) return;
     const LogSum l = log_sum(all);
     a.lse_live[r] = l;
+    // the largest |g| of a row is that of its target, to which all others add up
+    if (a.dloss != nullptr)
+        a.row_exp[r] = scale_exponent(__float_as_int(finite_abs(a.dloss[a.first + r] * expm1f(l.of(a.z_target[r])))));
     const int64_t n = a.row[a.first + r];
     if (a.lse != nullptr) a.lse[n * a.lse_s] = l.lse();
     if (a.loss != nullptr) a.loss[n * a.loss_s] = l.loss(a.z_target[r]);
 }
 
 struct GradArgs {
-    int64_t first, rows;
+    int64_t first;
     const int *live;
+    int64_t rows;
     int64_t V;
-    float *z;            // [rows][pitch], becomes g'
+    float *z;            // [rows][pitch], becomes g' as the rows of dx (of dweight, where there is no dx)
     int64_t pitch;
     const LogSum *lse_live;
     const int *target;
     const float *dloss;
-    const int *exponent; // of the scale of g'
+    const int *row_exp;  // [rows] exponents of the scales of g' as the rows of dx; null: not wanted
+    int *class_exp;      // [row blocks][pitch] of g' as the rows of dweight; null: not wanted
+    __half *by_class;    // [rows][pitch][2], that g'
     float *column_parts; // [row blocks][pitch] column sums of g; null: not wanted
 };
 
-constexpr int kGradRows = 64;  // rows of a CTA
+constexpr int kGradRows = kPieceBlocks * kBlock;  // rows of a CTA: a piece of dweight's K
 
-// z -> g' in place.  A CTA takes 128 columns of 64 rows, a warp eight of the rows, a lane
-// four columns: 512 bytes of z a load, two blocks of 128 + 128 bytes a store.  Bound by HBM,
-// 8 bytes a logit: 4096 x 32000 in 212 us (4.7 TB/s).
-__global__ void __launch_bounds__(256) k_softmax_grad(const GradArgs a) {
-    wait_for_previous();
-    const int64_t live = live_extent(a.live, a.first, a.rows);
-    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kGradRows;
-    if (r0 >= (live + 63) / 64 * 64) return;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + lane * 4;
-    const bool in = c < a.pitch;
-    const int e = *a.exponent;
-    const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
-    float4 column = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+// Scales x by 2^e, exactly, and stores it as a pair: four columns of a packed block.
+__device__ __forceinline__ void store_pairs(__half *to, const float (&x)[4], const int (&e)[4]) {
+    __half h[4], l[4];
 #pragma unroll
-    for (int j0 = 0; j0 < kGradRows / 8; j0 += 4) {
-        float4 z[4];
-        LogSum lse[4];
-        float d[4];
-        int t[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = r0 + (j0 + j) * 8 + warp;
-            z[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            lse[j] = LogSum{0.0f, 0.0f};
-            d[j] = 0.0f;
-            t[j] = -1;
-            if (r < live) {
-                if (in) z[j] = __ldcs(reinterpret_cast<const float4 *>(a.z + r * a.pitch + c));
-                lse[j] = a.lse_live[r];
-                d[j] = a.dloss[a.first + r] * f0 * f1;  // scaled by a power of two, exactly
-                t[j] = a.target[a.first + r];
-            }
-        }
-        __syncwarp();  // the whole block is read before any lane overwrites it
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = r0 + (j0 + j) * 8 + warp;
-            float g[4] = {lse[j].of(z[j].x), lse[j].of(z[j].y), lse[j].of(z[j].z), lse[j].of(z[j].w)};
-            __half h[4], l[4];
-            const int hot = t[j] - static_cast<int>(c);
-            float at_hot = 0.0f;
-            if (hot >= 0 && hot < 4) at_hot = d[j] * expm1f(hot == 0 ? g[0] : hot == 1 ? g[1] : hot == 2 ? g[2] : g[3]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                g[k] = hot == k ? at_hot : d[j] * expf(g[k]);
-                if (c + k >= a.V || r >= live) g[k] = 0.0f;
-                split_pair(g[k], h[k], l[k]);
-            }
-            column.x += g[0];
-            column.y += g[1];
-            column.z += g[2];
-            column.w += g[3];
-            if (in && r < a.rows) {
-                __half *to = reinterpret_cast<__half *>(a.z + r * a.pitch + c / kBlock * kBlock) + c % kBlock;
-                *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
-                *reinterpret_cast<uint2 *>(to + kBlock) = *reinterpret_cast<const uint2 *>(l);
-            }
-        }
-    }
-    if (a.column_parts == nullptr) return;
-    __shared__ float4 sums[8][32];
-    sums[warp][lane] = column;
-    __syncthreads();
-    if (warp != 0 || !in) return;
-    for (int w = 1; w < 8; ++w) {
-        column.x += sums[w][lane].x;
-        column.y += sums[w][lane].y;
-        column.z += sums[w][lane].z;
-        column.w += sums[w][lane].w;
-    }
-    const float u0 = power_of_two(-(e / 2)), u1 = power_of_two(-(e - e / 2));
-    *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) =
-        make_float4(column.x * u0 * u1, column.y * u0 * u1, column.z * u0 * u1, column.w * u0 * u1);
+    for (int k = 0; k < 4; ++k) split_pair(x[k] * power_of_two(e[k] / 2) * power_of_two(e[k] - e[k] / 2), h[k], l[k]);
+    *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
+    *reinterpret_cast<uint2 *>(to + kBlock) = *reinterpret_cast<const uint2 *>(l);
 }
 
-// A CTA takes 32 columns; its warps, up to 32, take the row blocks in turn (4 bytes for 64 rows
-// of a column: 8 us for 928 x 50003, 18 us for 65536 x 1000, where 8 warps a CTA take 61 us).
+// z -> g'.  The two products want g on scales of their own, or the small ones among its entries
+// lose their digits next to the large ones: dx takes each row to its largest entry (rows whose
+// dloss is small, rows sure of their class), dweight each class to its largest in a piece of K
+// (classes that are improbable everywhere).  So g goes out twice, once in the place of z.
+// A CTA takes 64 columns of 256 rows, a thread four columns of 16 of the rows, in registers;
+// everything is read before anything is written.  Bound by HBM, 12 bytes a logit.
+__global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
+    wait_for_previous();
+    __shared__ LogSum lse[kGradRows];
+    __shared__ float dloss[kGradRows];
+    __shared__ int target[kGradRows], row_exp[kGradRows];
+    __shared__ float4 sums[8][16], tops[8][16];
+    const int64_t live = live_extent(a.live, a.first, a.rows), packed = (live + 63) / 64 * 64;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kGradRows;
+    if (r0 >= packed) return;
+    constexpr int kMine = kGradRows / 16;
+    const int group = threadIdx.x / 16, warp = threadIdx.x / 32, quad = threadIdx.x % 16;
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kBlock, c = c0 + quad * 4;
+    float g[kMine][4];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+        const int64_t r = r0 + j * 16 + group;
+        const float4 z = r < live ? __ldcs(reinterpret_cast<const float4 *>(a.z + r * a.pitch + c))
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        g[j][0] = z.x;
+        g[j][1] = z.y;
+        g[j][2] = z.z;
+        g[j][3] = z.w;
+    }
+    {
+        const int64_t r = r0 + threadIdx.x;
+        lse[threadIdx.x] = r < live ? a.lse_live[r] : LogSum{0.0f, 0.0f};
+        dloss[threadIdx.x] = r < live ? a.dloss[a.first + r] : 0.0f;
+        target[threadIdx.x] = r < live ? a.target[a.first + r] : -1;
+        row_exp[threadIdx.x] = r < live && a.row_exp != nullptr ? a.row_exp[r] : 0;
+    }
+    __syncthreads();
+    float4 column = make_float4(0.0f, 0.0f, 0.0f, 0.0f), top = column;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+        const int at = j * 16 + group;
+        const LogSum l = lse[at];
+        const float d = dloss[at];
+        const int hot = target[at] - static_cast<int>(c);
+        float at_hot = 0.0f;
+        if (hot >= 0 && hot < 4) at_hot = d * expm1f(l.of(hot == 0 ? g[j][0] : hot == 1 ? g[j][1] : hot == 2 ? g[j][2] : g[j][3]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            g[j][k] = hot == k ? at_hot : d * expf(l.of(g[j][k]));
+            if (c + k >= a.V || r0 + at >= live) g[j][k] = 0.0f;
+        }
+        column.x += g[j][0];
+        column.y += g[j][1];
+        column.z += g[j][2];
+        column.w += g[j][3];
+        top.x = fmaxf(top.x, finite_abs(g[j][0]));
+        top.y = fmaxf(top.y, finite_abs(g[j][1]));
+        top.z = fmaxf(top.z, finite_abs(g[j][2]));
+        top.w = fmaxf(top.w, finite_abs(g[j][3]));
+    }
+    if (a.column_parts != nullptr || a.class_exp != nullptr) {
+        auto other = [](float4 v) {
+            return make_float4(__shfl_xor_sync(0xFFFFFFFFu, v.x, 16), __shfl_xor_sync(0xFFFFFFFFu, v.y, 16),
+                               __shfl_xor_sync(0xFFFFFFFFu, v.z, 16), __shfl_xor_sync(0xFFFFFFFFu, v.w, 16));
+        };
+        auto add = [](float4 &x, float4 y) { x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); };
+        auto max = [](float4 &x, float4 y) {
+            x = make_float4(fmaxf(x.x, y.x), fmaxf(x.y, y.y), fmaxf(x.z, y.z), fmaxf(x.w, y.w));
+        };
+        add(column, other(column));
+        max(top, other(top));
+        if (threadIdx.x % 32 < 16) {
+            sums[warp][quad] = column;
+            tops[warp][quad] = top;
+        }
+        __syncthreads();
+        top = tops[0][quad];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) max(top, tops[w][quad]);
+        if (threadIdx.x < 16 && a.column_parts != nullptr) {
+            for (int w = 1; w < 8; ++w) add(column, sums[w][quad]);
+            *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) = column;
+        }
+    }
+    if (a.row_exp != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int64_t r = r0 + j * 16 + group;
+            const int e = row_exp[j * 16 + group];
+            if (r < packed) store_pairs(reinterpret_cast<__half *>(a.z + r * a.pitch + c0) + quad * 4, g[j], {e, e, e, e});
+        }
+    }
+    if (a.class_exp != nullptr) {
+        const int e[4] = {scale_exponent(__float_as_int(top.x)), scale_exponent(__float_as_int(top.y)),
+                          scale_exponent(__float_as_int(top.z)), scale_exponent(__float_as_int(top.w))};
+        if (threadIdx.x < 16)
+            *reinterpret_cast<int4 *>(a.class_exp + blockIdx.y * a.pitch + c) = make_int4(e[0], e[1], e[2], e[3]);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int64_t r = r0 + j * 16 + group;
+            if (r < packed) store_pairs(a.by_class + 2 * (r * a.pitch + c0) + quad * 4, g[j], e);
+        }
+    }
+}
+
+// A CTA takes 32 columns; its warps, up to 32, take the row blocks in turn (4 bytes for 256 rows
+// of a column).
 __global__ void __launch_bounds__(1024) k_bias_grad(const GradArgs a, float *db, int64_t db_s, int add) {
     wait_for_previous();
     __shared__ float sums[32][32];
@@ -1096,11 +1145,12 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const int64_t pitch = v_blocks * kBlock;
     const int tiles_v = static_cast<int>((p.V + kTileCols - 1) / kTileCols);
     const int tiles_d = static_cast<int>((p.D + kTileCols - 1) / kTileCols);
-    // rows at a time: the logits of a piece fill at most 4 GiB (a piece more reads and writes
-    // dweight once more); without gradients only
-    // their statistics are kept, 8 bytes for 128 logits
+    // rows at a time: the logits of a piece, and the second g' of both products, fill at most
+    // 4 GiB (a piece more reads and writes dweight once more); without gradients only their
+    // statistics are kept, 8 bytes for 128 logits
     const int64_t rows_all = (p.N + 255) / 256 * 256;
-    const int64_t row_bytes = grads ? pitch * 4 : static_cast<int64_t>(tiles_v) * 16;
+    const bool two = p.dx != nullptr && p.dw != nullptr && p.D > 0;
+    const int64_t row_bytes = grads ? pitch * (two ? 8 : 4) : static_cast<int64_t>(tiles_v) * 16;
     int64_t piece = (int64_t{4} << 30) / row_bytes / 256 * 256;
     if (piece < 256) piece = 256;
     if (piece > (int64_t{1} << 21)) piece = int64_t{1} << 21;  // k_softmax_grad's grid
@@ -1122,7 +1172,10 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t stat = padded(static_cast<size_t>(piece) * 2 * tiles_v * 4);
     const size_t row_stat = padded(static_cast<size_t>(piece) * 4);
     const size_t z_bytes = grads ? padded(static_cast<size_t>(piece) * pitch * 4) : 0;
-    const size_t col_bytes = p.db != nullptr ? padded(static_cast<size_t>(piece / kGradRows) * pitch * 4) : 0;
+    const size_t by_class_bytes = grads && two ? z_bytes : 0;
+    const size_t col_bytes = padded(static_cast<size_t>(piece / kGradRows) * pitch * 4);
+    const size_t db_bytes = grads && p.db != nullptr ? col_bytes : 0;
+    const size_t exp_bytes = grads && p.dw != nullptr ? col_bytes : 0;
     const int64_t parts_pitch = (p.D + 7) / 8 * 8;
     const bool parts_dx = splits_dx > 1 || !sector_rows(p.dx, p.dx_rs, p.dx_cs, p.D);
     const bool parts_dw = splits_dw > 1 || !sector_rows(p.dw, p.dw_rs, p.dw_cs, p.D);
@@ -1132,7 +1185,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t split_grad = !grads ? 0 : split_dx > split_dw ? split_dx : split_dw;
     const size_t split_bytes = padded(split_z > split_grad ? split_z : split_grad);
     Workspace ws;
-    MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 3 * row_stat + z_bytes + col_bytes + split_bytes,
+    MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 4 * row_stat + z_bytes + by_class_bytes + db_bytes +
+                            exp_bytes + split_bytes,
                         stream));
     LiveRows live;
     live.count = ws.take<int>(256);
@@ -1145,8 +1199,11 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     float *part_rest = ws.take<float>(stat);
     float *z_target = ws.take<float>(row_stat);
     LogSum *lse_live = ws.take<LogSum>(2 * row_stat);
+    int *row_exp = ws.take<int>(row_stat);
     float *z = ws.take<float>(z_bytes);
-    float *columns = ws.take<float>(col_bytes);
+    __half *by_class = two ? ws.take<__half>(by_class_bytes) : reinterpret_cast<__half *>(z);
+    float *columns = ws.take<float>(db_bytes);
+    int *class_exp = ws.take<int>(exp_bytes);
     float *split_ws = ws.take<float>(split_bytes);
     unsigned long long *err = nullptr;
     MTC_TRY(device_error_word(&err));
@@ -1159,7 +1216,6 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     k.s[1] = PackSource{p.w, p.w_rs, p.w_cs, p.V, p.D, nullptr, nullptr, vector_source(p.w, p.w_rs, p.w_cs, p.D),
                         wp, p.V, 1, {}};
     k.s[0].blocks = k.s[1].blocks = make_fastdiv(static_cast<uint32_t>(d_blocks > 0 ? d_blocks : 1));
-    if (grads) k.dloss = live.dloss;
     if (p.dx != nullptr && p.D > 0) k.dx = p.dx;
     k.dx_rs = p.dx_rs;
     k.dx_cs = p.dx_cs;
@@ -1222,19 +1278,19 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         }
         // (a last tile of 128 columns or less has no second half)
         const RowArgs ra{first, rows, live.count, static_cast<int>((p.V + 127) / 128), 2 * tiles_v, part_max, part_rest,
-                         z_target, live.row, lse_live, p.loss, p.lse, p.loss_s, p.lse_s};
+                         z_target, live.row, lse_live, grads ? live.dloss : nullptr, row_exp, p.loss, p.lse, p.loss_s, p.lse_s};
         MTC_TRY((launch_dependent("linear cross entropy (loss)", k_row_loss, static_cast<unsigned>((rows + 7) / 8), 256, 0, stream, ra)));
         if (!grads) continue;
-        const GradArgs ga{first, rows_up, live.count, p.V, z, pitch, lse_live, live.target, live.dloss, live.count + kExponent + 2,
-                          p.db != nullptr ? columns : nullptr};
-        const dim3 grid(static_cast<unsigned>((pitch + 127) / 128), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
+        const bool dx = p.dx != nullptr && p.D > 0, dw = p.dw != nullptr && p.D > 0;
+        const GradArgs ga{first, live.count, rows_up, p.V, z, pitch, lse_live, live.target, live.dloss,
+                          dx ? row_exp : nullptr, dw ? class_exp : nullptr, by_class, p.db != nullptr ? columns : nullptr};
+        const dim3 grid(static_cast<unsigned>(v_blocks), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
         MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, 256, 0, stream, ga)));
         if (p.db != nullptr) {
-            MTC_TRY((launch_dependent("linear cross entropy (bias gradient)", k_bias_grad, static_cast<unsigned>((p.V + 31) / 32), piece > 64 * kGradRows ? 1024 : 256, 0, stream, ga, p.db, p.db_s, first > 0)));
+            MTC_TRY((launch_dependent("linear cross entropy (bias gradient)", k_bias_grad, static_cast<unsigned>((p.V + 31) / 32), piece > 16 * kGradRows ? 1024 : 256, 0, stream, ga, p.db, p.db_s, first > 0)));
         }
-        const __half *gp = reinterpret_cast<const __half *>(z);
-        if (p.dx != nullptr && p.D > 0) {
-            MTC_TRY(operand_map(g_k, gp, rows_up, v_blocks, v_blocks, false));
+        if (dx) {
+            MTC_TRY(operand_map(g_k, reinterpret_cast<const __half *>(z), rows_up, v_blocks, v_blocks, false));
             MTC_TRY(operand_map(w_mn, wp, p.V, d_blocks, d_blocks, true));
             std::memset(&t, 0, sizeof(t));
             t.M = rows;
@@ -1245,7 +1301,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.tiles_n = tiles_d;
             t.group = 16;
             t.splits = splits_dx;
-            t.exp_a = live.count + kExponent + 2;
+            t.exp_a = row_exp;
             t.exp_b = live.count + kExponent + 1;
             t.err = err;
             t.out = p.dx;
@@ -1259,8 +1315,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
                                          static_cast<unsigned>(sms * 8), 256, 0, stream, t, p.dx_cs,
                                          vector_source(p.dx, p.dx_rs, p.dx_cs, p.D)));
         }
-        if (p.dw != nullptr && p.D > 0) {
-            MTC_TRY(operand_map(g_mn, gp, rows_up, v_blocks, v_blocks, true));
+        if (dw) {
+            MTC_TRY(operand_map(g_mn, by_class, rows_up, v_blocks, v_blocks, true));
             MTC_TRY(operand_map(x_mn, xc, rows_up, d_blocks, d_blocks, true));
             std::memset(&t, 0, sizeof(t));
             t.M = p.V;
@@ -1272,7 +1328,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.tiles_n = tiles_d;
             t.group = 16;
             t.splits = splits_dw;
-            t.exp_a = live.count + kExponent + 2;
+            t.exp_a = class_exp;
+            t.exp_pitch = pitch;
             t.exp_b = live.count + kExponent;
             t.err = err;
             t.out = p.dw;

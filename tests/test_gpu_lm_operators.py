@@ -656,6 +656,113 @@ def test_rows_sure_of_their_class_on_the_tensor_cores(cuda, n, vocab, dim, gap):
     within(got["dw"][:, 0], n * g, (rel + 2 * U * (n + 16)) * n * g.abs() + n * 2.0 ** -48, "dw")
 
 
+def own_bounds(x, w, b, t, dloss):
+    """(dx, dw, db) in float64 and bounds by each row's and each class's own size: an entry of g is
+    off by its rounding errors, relative to itself, and by its pair of 16-bit floats, 2^-22 of itself
+    and 2^-48 of the largest entry of its row (dx) or class (dw)."""
+    import torch
+
+    live = (t != IGNORE).unsqueeze(1)
+    xd, wd = torch.where(live, x.double(), 0.0), w.double()
+    z = xd @ wd.t() + b.double()
+    dz = product_bound(x.shape[1], xd.abs() @ wd.abs().t()) + 2 * U * (z.abs() + b.double().abs())
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    at = torch.where(live, t.unsqueeze(1), 0)
+    p = torch.exp(z - lse)
+    dlse = (p * dz).sum(1, keepdim=True) * (1 + 1e-3) + (w.shape[0] / 256 + 32) * 2 * U + 4 * U * lse.abs()
+    others = torch.ones_like(p).scatter_(1, at, 0.0)
+    left = (p * others).sum(1, keepdim=True)  # 1 - p of the target, without the difference
+    d = torch.where(live, dloss.double().unsqueeze(1), 0.0)
+    g = d * (p * others - left * (1.0 - others))
+    e = dz + dlse + 2 * U * (z.abs() + lse.abs())
+    e = e * others + (1.0 - others) * ((p * others * e).sum(1, keepdim=True) / left + e)
+    dg = g.abs() * (torch.expm1(e) + 16 * U)
+    ag, ax, aw = g.abs(), xd.abs(), wd.abs()
+    by_row, by_class = 2.0 ** -48 * ag.amax(1, keepdim=True), 2.0 ** -48 * ag.amax(0, keepdim=True)
+    return {"dx": (g @ wd, (dg + by_row) @ aw + product_bound(w.shape[0], ag @ aw)),
+            "dw": (g.t() @ xd, (dg + by_class * live).t() @ ax + product_bound(x.shape[0], ag.t() @ ax)),
+            "db": (g.sum(0), dg.sum(0) + product_bound(x.shape[0], ag.sum(0)))}
+
+
+def check_own(x, w, b, t, dloss):
+    got = run_ce(x, w, b, t, dloss)
+    abi.check_device_errors(0)
+    for name, (value, tol) in own_bounds(x, w, b, t, dloss).items():
+        within(got[name], value, tol + 1e-42, name)
+    return got
+
+
+GRADIENT_SHAPES = [(37, 53, 29), (530, 700, 120), (1031, 903, 65), (3000, 15, 120), (5, 5000, 180), (17, 900, 400)]
+
+
+@pytest.mark.parametrize("n, vocab, dim", GRADIENT_SHAPES)
+def test_gradients_of_classes_improbable_everywhere(cuda, n, vocab, dim):
+    """Classes of probabilities down to 1e-35 in every row: their rows of dweight are held to their
+    own size, not to that of the other classes'."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 33, ignored=0.1, spread=0.5)
+    t = torch.where(t == IGNORE, t, t % (vocab - 8))
+    b = b.clone()
+    b[vocab - 8:] = -torch.arange(10.0, 81.0, 10.0, device=cuda)
+    got = check_own(x, w, b, t, torch.ones(n, device=cuda))
+    assert (got["dw"][vocab - 8:] != 0).any(1).all() and got["dw"][-1].abs().max() < 1e-25
+
+
+@pytest.mark.parametrize("n, vocab, dim", GRADIENT_SHAPES)
+def test_gradients_of_rows_with_a_small_share_of_the_loss(cuda, n, vocab, dim):
+    """dloss over thirty decades, in no order: each row of dx is held to its own size."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 34, ignored=0.1)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    share = 10.0 ** -torch.linspace(0, 30, n, device=cuda)[torch.randperm(n, device=cuda, generator=g)]
+    got = check_own(x, w, b, t, dloss.sign() * share)
+    assert (got["dx"][t != IGNORE] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("n, vocab, dim", [(530, 700, 120), (1031, 903, 65), (17, 900, 400), (60, 200, 4095)])
+def test_gradients_of_rows_sure_of_their_class(cuda, n, vocab, dim):
+    """Rows sure of their class to 1e-3 and to 1e-30, side by side, on the tensor cores."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 35, ignored=0.1, spread=0.25)
+    at = torch.where(t == IGNORE, 0, t)
+    w = torch.cat([w, torch.zeros(vocab, 1, device=cuda)], 1)
+    w[:, -1] = torch.where(torch.arange(vocab, device=cuda) == vocab // 2, 1.0, 0.0)
+    lift = torch.linspace(8, 70, n, device=cuda).unsqueeze(1)
+    t = torch.where(t == IGNORE, t, vocab // 2)
+    check_own(torch.cat([x, lift], 1), w, b * 0.1, t, torch.ones(n, device=cuda))
+
+
+@pytest.mark.parametrize("n, vocab, dim", [(300, 100, 512), (300, 128, 512), (600, 1000, 96), (60, 200, 4096), (17, 900, 400)])
+@pytest.mark.parametrize("gap", [40.0, 75.0])
+def test_gradients_below_the_first_step_of_one(cuda, n, vocab, dim, gap):
+    """What is left next to a probability that float64 too holds as 1, by the bounds of
+    test_rows_sure_of_their_class_on_the_tensor_cores without the share of the largest |dloss|."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 28)
+    steps = torch.round(w[:, :1] * 8).clamp(-16, 16) / 8
+    x, w = torch.zeros_like(x), torch.zeros_like(w)
+    x[:, 0], w[:, :1] = 1.0, steps
+    w[vocab // 2, 0] = 3.0 + gap
+    t = torch.full_like(t, vocab // 2)
+    got = run_ce(x, w, None, t, torch.ones_like(dloss))
+    z = w[:, 0].double()
+    logp = z - torch.logsumexp(z, 0)
+    others = torch.arange(vocab, device=cuda) != vocab // 2
+    rest = torch.logsumexp(z[others], 0) - torch.logsumexp(z, 0)
+    g = torch.where(others, logp.exp(), -rest.exp())
+    rel = U * (2 * logp.abs().max() + 52 + 4 * 4)
+    within(got["loss"], rest.exp().expand(n), (rel * rest.exp()).expand(n), "loss")
+    within(got["db"], n * g, (rel + 2 * U * n) * n * g.abs(), "db")
+    within(got["dw"][:, 0], n * g, (rel + 2 * U * (n + 16)) * n * g.abs(), "dw")
+    # p of the other classes is the same in every row: dx is their logits' mean less the target's
+    dx = (g * z).sum()
+    within(got["dx"][:, 0], dx.expand(n), ((rel + 2 * U * (vocab + 16)) * (g * z).abs().sum()).expand(n), "dx")
+
+
 @pytest.mark.parametrize("n, vocab, dim", [(2 ** 21 - 1, 1, 1), (2 ** 21 - 1, 2, 0), (2 ** 20, 3, 0), (2 ** 20 - 1, 3, 0)])
 def test_more_rows_than_a_grid_has_parts(cuda, n, vocab, dim):
     """Where 32 rows a CTA would be more than the 65535 parts of a launch's second axis."""
