@@ -26,7 +26,7 @@ struct LinearCe {
 };
 
 // What the device knows about the rows that have a loss.
-constexpr int kLiveKnown = 7;
+constexpr int kLiveKnown = 10;
 struct LiveRows {
     int *count;      // [1], and behind it what the tensor-core path learns of the magnitudes, zeroed with it
     int *row;        // [N] the row of x; behind them, from the end backwards, the rows without a loss

@@ -105,8 +105,21 @@ __device__ __forceinline__ void store_pairs(__half *to, float x0, float x1, floa
 }
 
 // What the device knows of the scales of x and weight, behind the count of the live rows.
-enum Known { kLargest = 1, kSampled = 3, kExponent = 5 };
-static_assert(kExponent + 2 == kLiveKnown, "zeroed with the count");
+// kWide: the pairs would not hold x and weight; kArrived counts CTAs.
+enum Known { kLargest = 1, kSampled = 3, kExponent = 5, kWide = 7, kArrived = 8 };
+static_assert(kArrived + 2 == kLiveKnown, "zeroed with the count");
+
+// Whether the pairs hold a tensor.  With a scaled x off by 2^-36 at most, a row or a column is
+// held to 2^-24 of its largest element, as float32 would round that one, where an element of it
+// reaches 2^-12.  Beside the largest of the tensor, scaled to 2^8 at least, such a row may be
+// smaller by 2^20.  A byte each says whether the row (column) has an element that large and
+// whether it has any at all that is finite and not zero: one that has but the latter makes the
+// products go by float32 (plain_sum).
+constexpr float kHeld = 0x1p-12f;
+struct Held {
+    unsigned char *row_ok, *row_some, *col_ok, *col_some;
+    int64_t rows16, cols16;  // their lengths in 16 bytes
+};
 
 struct PackSource {
     const float *p;
@@ -118,13 +131,15 @@ struct PackSource {
     __half *to;       // [rows_out][blocks][2][64]
     int64_t rows_out; // with zero rows behind the live ones, up to a multiple of 64
     int which;        // 0: x, 1: weight
-    FastDiv blocks;   // of a row
+    Held held[2];     // by the first packing, and by the second
 };
 
 struct PackArgs {
     PackSource s[2];
     int64_t first_of_second;  // blocks of the grid before the second tensor
     int *known;               // the live rows' count and what follows it
+    uint4 *flags;             // all of Held's bytes, to be zeroed
+    int64_t flags16;
     int headroom;             // powers of two above the sample; 0: it is the whole
     float *dx;                // its rows without a loss become zero; null: not wanted
     int64_t dx_rs, dx_cs;
@@ -173,7 +188,7 @@ __device__ __forceinline__ int last_exponent(const PackArgs &a, int which) {
 }
 
 // Largest finite magnitudes of x (rows with a loss) and weight over a sample of the rows, one
-// a warp; the zero rows of dx.  7 to 30 us for 1184 rows of 1024 to 8192 columns,
+// a warp; the zero rows of dx, and Held's zeroes.  7 to 30 us for 1184 rows of 1024 to 8192 columns,
 // a warp's latency.
 __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     wait_for_previous();
@@ -182,6 +197,8 @@ __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
     const int64_t blocks = second ? gridDim.x - a.first_of_second : a.first_of_second;
     const int lane = threadIdx.x % 32;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < a.flags16; i += gridDim.x * 256)
+        a.flags[i] = make_uint4(0, 0, 0, 0);
     float m0 = 0.0f, m1 = 0.0f;
     const int64_t rows = source_rows(s);
     const int64_t warp_at = block * 8 + threadIdx.x / 32, warps = blocks * 8;
@@ -241,9 +258,31 @@ __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     }
 }
 
-// Each half-warp packs one block of 64 columns at a time: a lane four columns.  AGAIN: only
-// the tensors whose scale was wrong; and the exponents are written down.  Bound by HBM, 8
-// bytes an element: 36096 rows of 2048 in 103 us (5.7 TB/s).
+// Looks the bytes over, 16 at a time, a share of them a thread.
+__device__ __forceinline__ void judge(const Held &h, int64_t at, int64_t step, int *wide) {
+    bool bad = false;
+    auto look = [&](const unsigned char *ok, const unsigned char *some, int64_t n) {
+        for (int64_t i = at; i < n; i += step) {
+            const uint4 o = __ldcg(reinterpret_cast<const uint4 *>(ok) + i), m = __ldcg(reinterpret_cast<const uint4 *>(some) + i);
+            bad |= ((m.x & ~o.x) | (m.y & ~o.y) | (m.z & ~o.z) | (m.w & ~o.w)) != 0;
+        }
+    };
+    look(h.row_ok, h.row_some, h.rows16);
+    look(h.col_ok, h.col_some, h.cols16);
+    if (bad) atomicOr(wide, 1);
+}
+
+// Sets the bytes of four columns; most are set already.
+__device__ __forceinline__ void mark_columns(unsigned char *to, unsigned int four) {
+    const unsigned int has = __ldcg(reinterpret_cast<const unsigned int *>(to));
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if ((four >> k & 1) && !(has >> (8 * k) & 1)) to[k] = 1;
+}
+
+// Each half-warp packs one block of 64 columns of every so many rows: a lane four columns.
+// AGAIN: only the tensors whose scale was wrong; and the exponents are written down.  Bound by
+// HBM, 8 bytes an element: 36096 rows of 2048 in 103 us (5.7 TB/s).
 template <bool AGAIN>
 __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     wait_for_previous();
@@ -251,56 +290,102 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
         a.known[kExponent + threadIdx.x] = AGAIN ? last_exponent(a, threadIdx.x) : first_exponent(a, threadIdx.x);
     const bool second = blockIdx.x >= a.first_of_second;
     const PackSource &s = a.s[second];
-    const int64_t block = second ? blockIdx.x - a.first_of_second : blockIdx.x;
-    const int64_t grid = second ? gridDim.x - a.first_of_second : a.first_of_second;
+    const int block = static_cast<int>(second ? blockIdx.x - a.first_of_second : blockIdx.x);
+    const int grid = static_cast<int>(second ? gridDim.x - a.first_of_second : a.first_of_second);
     const int64_t blocks = (s.cols + kBlock - 1) / kBlock;
     const int64_t rows = source_rows(s);
     const int64_t rows_out = s.live != nullptr && (rows + 63) / 64 * 64 < s.rows_out ? (rows + 63) / 64 * 64 : s.rows_out;
     const int e = AGAIN ? last_exponent(a, s.which) : first_exponent(a, s.which);
-    if (AGAIN && (e == first_exponent(a, s.which) || a.known[kLargest + s.which] == 0)) return;
+    if (AGAIN && (e == first_exponent(a, s.which) || a.known[kLargest + s.which] == 0)) {
+        judge(s.held[0], static_cast<int64_t>(block) * 256 + threadIdx.x, static_cast<int64_t>(grid) * 256, a.known + kWide);
+        return;
+    }
+    const Held &held = s.held[AGAIN];
     const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
     const int lane = threadIdx.x % 16;
+    const unsigned int mates = 0xFFFFu << (threadIdx.x & 16);
     float largest = 0.0f;
     constexpr int U = 4;
-    const int64_t total = rows_out * blocks;
-    const bool narrow = total < (int64_t{1} << 32);  // a 64-bit division a block costs as much as its bytes
-    for (int64_t i0 = block * 16 * U + threadIdx.x / 16; i0 < total; i0 += grid * 16 * U) {
-        float4 v[U];
+    const int halves = grid * 16;
+    const int abreast = blocks < halves ? static_cast<int>(blocks) : halves;  // half-warps along a row
+    const int step = abreast > 0 ? halves / abreast : 0;                      // rows at a time
+    const int half = block * 16 + threadIdx.x / 16;
+    const int at = abreast > 0 ? half % abreast : 0, r_first = abreast > 0 ? half / abreast : 0;
+    for (int64_t b0 = 0; b0 < blocks; b0 += abreast) {
+        const int64_t b = b0 + at, c = b * kBlock + lane * 4;
+        const bool mine = b < blocks && r_first < step;
+        unsigned int col_ok = 0, col_some = 0;
+        for (int64_t r0 = 0; r0 < rows_out; r0 += static_cast<int64_t>(step) * U) {
+            float4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = i0 + u * 16;
-            v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i >= total) continue;
-            const int64_t r = narrow ? fastdiv(static_cast<uint32_t>(i), s.blocks) : i / blocks;
-            const int64_t c = (i - r * blocks) * kBlock + lane * 4;
-            if (r >= rows || c >= s.cols) continue;
-            const float *src = source_row(s, r);
-            if (s.vec) {
-                v[u] = __ldg(reinterpret_cast<const float4 *>(src + c));
-            } else {
-                v[u].x = __ldg(src + c * s.cs);
-                if (c + 1 < s.cols) v[u].y = __ldg(src + (c + 1) * s.cs);
-                if (c + 2 < s.cols) v[u].z = __ldg(src + (c + 2) * s.cs);
-                if (c + 3 < s.cols) v[u].w = __ldg(src + (c + 3) * s.cs);
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + static_cast<int64_t>(u) * step + r_first;
+                v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (!mine || r >= rows || c >= s.cols) continue;
+                const float *src = source_row(s, r);
+                if (s.vec) {
+                    v[u] = __ldg(reinterpret_cast<const float4 *>(src + c));
+                } else {
+                    v[u].x = __ldg(src + c * s.cs);
+                    if (c + 1 < s.cols) v[u].y = __ldg(src + (c + 1) * s.cs);
+                    if (c + 2 < s.cols) v[u].z = __ldg(src + (c + 2) * s.cs);
+                    if (c + 3 < s.cols) v[u].w = __ldg(src + (c + 3) * s.cs);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + static_cast<int64_t>(u) * step + r_first;
+                if (!AGAIN && a.headroom != 0)
+                    largest = fmaxf(largest, fmaxf(fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)),
+                                                   fmaxf(finite_abs(v[u].z), finite_abs(v[u].w))));
+                const float x[4] = {v[u].x * f0 * f1, v[u].y * f0 * f1, v[u].z * f0 * f1, v[u].w * f0 * f1};
+                const float raw[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                unsigned int ok = 0, some = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool finite = fabsf(x[k]) <= 3.402823466e38f;
+                    ok |= static_cast<unsigned int>(finite && fabsf(x[k]) >= kHeld) << k;
+                    some |= static_cast<unsigned int>(finite && raw[k] != 0.0f) << k;
+                }
+                col_ok |= ok;
+                col_some |= some;
+                const unsigned int row_ok = __ballot_sync(0xFFFFFFFFu, ok != 0), row_some = __ballot_sync(0xFFFFFFFFu, some != 0);
+                if (!mine || r >= rows_out) continue;
+                if (lane == 0 && (row_ok & mates)) held.row_ok[r] = 1;
+                else if (lane == 0 && (row_some & mates)) held.row_some[r] = 1;
+                store_pairs(s.to + (r * blocks + b) * 2 * kBlock + lane * 4, x[0], x[1], x[2], x[3]);
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = i0 + u * 16;
-            if (i >= total) continue;
-            if (!AGAIN && a.headroom != 0)
-                largest = fmaxf(largest, fmaxf(fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)),
-                                               fmaxf(finite_abs(v[u].z), finite_abs(v[u].w))));
-            store_pairs(s.to + i * 2 * kBlock + lane * 4, v[u].x * f0 * f1, v[u].y * f0 * f1, v[u].z * f0 * f1,
-                        v[u].w * f0 * f1);
+        if (mine) {
+            mark_columns(held.col_ok + c, col_ok);
+            mark_columns(held.col_some + c, col_some);
         }
     }
-    if (!AGAIN && a.headroom != 0) keep_max(largest, a.known + kLargest + s.which);
+    if (!AGAIN && a.headroom != 0) {
+        keep_max(largest, a.known + kLargest + s.which);
+        return;
+    }
+    // nothing after this launch but the products: the tensor's last CTA looks it over
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(&a.known[kArrived + s.which], 1) == grid - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    judge(held, threadIdx.x, 256, a.known + kWide);
 }
 
 // ---------------------------------------------------------------- products --
 
 enum class Out { Logits, Sum };
+
+// An operand as float32, wherever it lies: element k of row r at map[r] rs + map[k] ks.
+struct Plain {
+    const float *p;
+    int64_t rs, ks;
+    const int *rows, *ks_map;  // null: as they are
+};
 
 struct TileArgs {
     int64_t M, N, K;  // M or K: of the piece, of which the first live ones count
@@ -314,6 +399,8 @@ struct TileArgs {
     // of dx, or one a class and piece of K as the rows of dweight.
     const int *exp_a, *exp_b;
     int64_t exp_pitch;  // [pieces][exp_pitch]
+    const int *wide;    // set: float32 products of the operands themselves
+    Plain a, b;
     unsigned long long *err;
     // Logits
     float *z;         // [M][z_pitch], null: statistics alone
@@ -379,7 +466,7 @@ __device__ __forceinline__ void mma_pair_scaled(uint32_t d, uint64_t a, uint64_t
 struct Extent {
     int64_t tiles_m, tiles, units;
     int kblocks, per_split;
-    int64_t M;
+    int64_t M, K;
 };
 
 __device__ __forceinline__ Extent extent_of(const TileArgs &a) {
@@ -390,6 +477,7 @@ __device__ __forceinline__ Extent extent_of(const TileArgs &a) {
         if (a.live_k) K = live_extent(a.live, a.first, K);
         else e.M = live_extent(a.live, a.first, e.M);
     }
+    e.K = K;
     e.kblocks = static_cast<int>((K + kBlock - 1) / kBlock);
     e.tiles_m = (e.M + kTileRows - 1) / kTileRows;
     e.tiles = e.tiles_m * a.tiles_n;
@@ -568,6 +656,55 @@ __device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&
     else store_row(a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0, acc, n, a.add);
 }
 
+// ROWS rows of 32 columns of an operand into shared memory, the columns `pitch` apart; zeros
+// beyond its ends.  256 threads, next to one another where the operand's elements are.
+template <int ROWS>
+__device__ __forceinline__ void stage_plain(const Plain &o, int64_t row0, int64_t rows, int64_t k0, int64_t k1, float *to,
+                                            int pitch, int thread) {
+    const bool along_k = o.ks == 1 || o.rs != 1;
+#pragma unroll 4
+    for (int i = thread; i < ROWS * 32; i += 256) {
+        const int r = along_k ? i / 32 : i % ROWS, k = along_k ? i % 32 : i / ROWS;
+        const int64_t row = row0 + r, col = k0 + k;
+        float v = 0.0f;
+        if (row < rows && col < k1)
+            v = __ldg(o.p + (o.rows != nullptr ? o.rows[row] : row) * o.rs + (o.ks_map != nullptr ? o.ks_map[col] : col) * o.ks);
+        to[k * pitch + r] = v;
+    }
+}
+
+// The sums of this lane's row and 128 columns in float32, on the FMA units, for operands whose
+// rows or columns are of so unlike size that pairs on one scale lose the small ones.  A lane's 128
+// products take one element of A and, all lanes alike, 32 vectors of B from shared memory: bound by
+// the FMAs.
+__device__ __forceinline__ void plain_sum(const TileArgs &a, const Extent &e, float *as, int tm, int tn, int rank, int kb0,
+                                          int kb1, float (&acc)[128]) {
+    constexpr int kPitchA = 132, kPitchB = 260;
+    float *bs = as + 32 * kPitchA;
+    const int thread = threadIdx.x - 128, quadrant = (threadIdx.x / 32) % 4, half = thread / 128;
+    const int64_t k_end = static_cast<int64_t>(kb1) * kBlock < e.K ? static_cast<int64_t>(kb1) * kBlock : e.K;
+    const float *mine = as + quadrant * 32 + threadIdx.x % 32;
+    for (int64_t k0 = static_cast<int64_t>(kb0) * kBlock; k0 < k_end; k0 += 32) {
+        stage_plain<128>(a.a, static_cast<int64_t>(tm) * kTileRows + rank * 128, e.M, k0, k_end, as, kPitchA, thread);
+        stage_plain<256>(a.b, static_cast<int64_t>(tn) * kTileCols, a.N, k0, k_end, bs, kPitchB, thread);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the epilogue warps alone
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k) {
+            const float x = mine[k * kPitchA];
+            const float4 *row = reinterpret_cast<const float4 *>(bs + k * kPitchB + half * 128);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float4 y = row[j];
+                acc[4 * j] = fmaf(x, y.x, acc[4 * j]);
+                acc[4 * j + 1] = fmaf(x, y.y, acc[4 * j + 1]);
+                acc[4 * j + 2] = fmaf(x, y.z, acc[4 * j + 2]);
+                acc[4 * j + 3] = fmaf(x, y.w, acc[4 * j + 3]);
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+}
+
 template <bool A_MN, bool B_MN, Out MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     k_pair_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -615,6 +752,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     wait_for_previous();
     const Extent e = extent_of(args);
+    const bool wide = *args.wide != 0;
+    const int64_t first_unit = wide ? e.units : cluster;  // of the tensor core's warps
 
     if (warp >= 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
@@ -630,7 +769,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-            for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
+            if (wide) plain_sum(args, e, reinterpret_cast<float *>(smem), tm, tn, static_cast<int>(rank), kb0, kb1, acc);
+            for (int kb = wide ? kb1 : kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
                 const int b = static_cast<int>(piece & 1);
                 float unscale = 1.0f;  // of a class's row in this piece
                 if (A_MN && row < e.M)
@@ -656,7 +796,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
                 if (lane == 0) mbar_arrive_remote(release[b]);
             }
             if (!ok) break;
-            const int scale = -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
+            const int scale = wide ? 0 : -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
             const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
             const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
             const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
@@ -671,7 +811,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
             if (lane == 0) {
                 int64_t it = 0;
                 bool ok = true;
-                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                for (int64_t u = first_unit; u < e.units && ok; u += clusters) {
                     int tm, tn, split, kb0, kb1;
                     unit_of(args, e, u, tm, tn, split, kb0, kb1);
                     const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
@@ -712,7 +852,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
                 constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
                 int64_t it = 0, piece = 0;
                 bool ok = true;
-                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                for (int64_t u = first_unit; u < e.units && ok; u += clusters) {
                     int tm, tn, split, kb0, kb1;
                     unit_of(args, e, u, tm, tn, split, kb0, kb1);
                     for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
@@ -942,6 +1082,7 @@ struct GradArgs {
     int *class_exp;      // [row blocks][pitch] of g' as the rows of dweight; null: not wanted
     __half *by_class;    // [rows][pitch][2], that g'
     float *column_parts; // [row blocks][pitch] column sums of g; null: not wanted
+    const int *wide;     // set: z becomes g, as float32, for both
 };
 
 constexpr int kGradRows = kPieceBlocks * kBlock;  // rows of a CTA: a piece of dweight's K
@@ -1030,6 +1171,15 @@ __global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
             for (int w = 1; w < 8; ++w) add(column, sums[w][quad]);
             *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) = column;
         }
+    }
+    if (*a.wide != 0) {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int64_t r = r0 + j * 16 + group;
+            if (r < live)
+                *reinterpret_cast<float4 *>(a.z + r * a.pitch + c) = make_float4(g[j][0], g[j][1], g[j][2], g[j][3]);
+        }
+        return;
     }
     if (a.row_exp != nullptr) {
 #pragma unroll
@@ -1188,8 +1338,12 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t split_z = splits_z > 1 ? static_cast<size_t>(splits_z) * piece * pitch * 4 : 0;
     const size_t split_grad = !grads ? 0 : split_dx > split_dw ? split_dx : split_dw;
     const size_t split_bytes = padded(split_z > split_grad ? split_z : split_grad);
+    // a byte a row and one a column of either tensor, four times: see Held
+    const int64_t d_pad = d_blocks * kBlock;
+    const size_t held_x = padded(static_cast<size_t>(rows_all)), held_w = padded(static_cast<size_t>(p.V));
+    const size_t held_d = padded(static_cast<size_t>(d_pad)), held = 4 * (held_x + held_w + 2 * held_d);
     Workspace ws;
-    MTC_TRY(ws.allocate(256 + 3 * list + x_bytes + w_bytes + 2 * stat + 4 * row_stat + z_bytes + by_class_bytes + db_bytes +
+    MTC_TRY(ws.allocate(256 + held + 3 * list + x_bytes + w_bytes + 2 * stat + 4 * row_stat + z_bytes + by_class_bytes + db_bytes +
                             exp_bytes + split_bytes,
                         stream));
     LiveRows live;
@@ -1197,6 +1351,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     live.row = ws.take<int>(list);
     live.target = ws.take<int>(list);
     live.dloss = ws.take<float>(list);
+    unsigned char *flags = ws.take<unsigned char>(held);
     __half *xp = ws.take<__half>(x_bytes);
     __half *wp = ws.take<__half>(w_bytes);
     float *part_max = ws.take<float>(stat);
@@ -1219,7 +1374,16 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
                         xp, rows_all, 0, {}};
     k.s[1] = PackSource{p.w, p.w_rs, p.w_cs, p.V, p.D, nullptr, nullptr, vector_source(p.w, p.w_rs, p.w_cs, p.D),
                         wp, p.V, 1, {}};
-    k.s[0].blocks = k.s[1].blocks = make_fastdiv(static_cast<uint32_t>(d_blocks > 0 ? d_blocks : 1));
+    k.flags = reinterpret_cast<uint4 *>(flags);
+    k.flags16 = static_cast<int64_t>(held / 16);
+    for (PackSource &s : k.s) {
+        const size_t rows = s.which == 0 ? held_x : held_w;
+        for (Held &h : s.held) {
+            h = Held{flags, flags + rows, flags + 2 * rows, flags + 2 * rows + held_d, static_cast<int64_t>(rows / 16),
+                     static_cast<int64_t>(held_d / 16)};
+            flags += 2 * (rows + held_d);
+        }
+    }
     if (p.dx != nullptr && p.D > 0) k.dx = p.dx;
     k.dx_rs = p.dx_rs;
     k.dx_cs = p.dx_cs;
@@ -1261,6 +1425,9 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         t.splits = splits_z;
         t.exp_a = live.count + kExponent;
         t.exp_b = live.count + kExponent + 1;
+        t.wide = live.count + kWide;
+        t.a = Plain{p.x, p.x_rs, p.x_cs, live.row + first, nullptr};
+        t.b = Plain{p.w, p.w_rs, p.w_cs, nullptr, nullptr};
         t.err = err;
         t.z = grads ? z : nullptr;
         t.z_pitch = pitch;
@@ -1287,7 +1454,8 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         if (!grads) continue;
         const bool dx = p.dx != nullptr && p.D > 0, dw = p.dw != nullptr && p.D > 0;
         const GradArgs ga{first, live.count, rows_up, p.V, z, pitch, lse_live, live.target, live.dloss,
-                          dx ? row_exp : nullptr, dw ? class_exp : nullptr, by_class, p.db != nullptr ? columns : nullptr};
+                          dx ? row_exp : nullptr, dw ? class_exp : nullptr, by_class, p.db != nullptr ? columns : nullptr,
+                          live.count + kWide};
         const dim3 grid(static_cast<unsigned>(v_blocks), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
         MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, 256, 0, stream, ga)));
         if (p.db != nullptr) {
@@ -1307,6 +1475,9 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.splits = splits_dx;
             t.exp_a = row_exp;
             t.exp_b = live.count + kExponent + 1;
+            t.wide = live.count + kWide;
+            t.a = Plain{z, pitch, 1, nullptr, nullptr};
+            t.b = Plain{p.w, p.w_cs, p.w_rs, nullptr, nullptr};
             t.err = err;
             t.out = p.dx;
             t.out_rs = p.dx_rs;
@@ -1335,6 +1506,9 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
             t.exp_a = class_exp;
             t.exp_pitch = pitch;
             t.exp_b = live.count + kExponent;
+            t.wide = live.count + kWide;
+            t.a = Plain{z, 1, pitch, nullptr, nullptr};
+            t.b = Plain{p.x, p.x_cs, p.x_rs, nullptr, live.row + first};
             t.err = err;
             t.out = p.dw;
             t.out_rs = p.dw_rs;

@@ -675,8 +675,9 @@ def own_bounds(x, w, b, t, dloss):
     d = torch.where(live, dloss.double().unsqueeze(1), 0.0)
     g = d * (p * others - left * (1.0 - others))
     e = dz + dlse + 2 * U * (z.abs() + lse.abs())
-    e = e * others + (1.0 - others) * ((p * others * e).sum(1, keepdim=True) / left + e)
-    dg = g.abs() * (torch.expm1(e) + 16 * U)
+    up = (torch.exp((z - lse + e).clamp(max=0.0)) - p) * others  # p at the end of its exponent's range
+    up = up + up.sum(1, keepdim=True).clamp(max=1.0) * (1.0 - others)  # and what is left of the target's
+    dg = d.abs() * up + 16 * U * g.abs()
     ag, ax, aw = g.abs(), xd.abs(), wd.abs()
     by_row, by_class = 2.0 ** -48 * ag.amax(1, keepdim=True), 2.0 ** -48 * ag.amax(0, keepdim=True)
     return {"dx": (g @ wd, (dg + by_row) @ aw + product_bound(w.shape[0], ag @ aw)),
@@ -687,7 +688,8 @@ def own_bounds(x, w, b, t, dloss):
 def check_own(x, w, b, t, dloss):
     got = run_ce(x, w, b, t, dloss)
     abi.check_device_errors(0)
-    for name, (value, tol) in own_bounds(x, w, b, t, dloss).items():
+    want = {**ce_reference(x, w, b, t, None), **own_bounds(x, w, b, t, dloss)}
+    for name, (value, tol) in want.items():
         within(got[name], value, tol + 1e-42, name)
     return got
 
@@ -761,6 +763,85 @@ def test_gradients_below_the_first_step_of_one(cuda, n, vocab, dim, gap):
     # p of the other classes is the same in every row: dx is their logits' mean less the target's
     dx = (g * z).sum()
     within(got["dx"][:, 0], dx.expand(n), ((rel + 2 * U * (vocab + 16)) * (g * z).abs().sum()).expand(n), "dx")
+
+
+# float32 path of few rows, one piece and several, logits split along the columns, a scale from a
+# sample of the rows, and neither dimension a multiple of anything
+UNLIKE_SHAPES = [(16, 700, 120), (300, 2000, 256), (520, 1300, 100), (60, 200, 4096), (3000, 2500, 80), (1301, 1999, 131)]
+
+
+@pytest.mark.parametrize("n, vocab, dim", UNLIKE_SHAPES)
+@pytest.mark.parametrize("size", [1e8, 1e12, 1e15, 1e25])
+def test_a_large_row_leaves_the_others_their_digits(cuda, n, vocab, dim, size):
+    """A row of x, or of the weight, far larger than the others: each other row's loss and dx, and
+    each class's dweight, stay within what the sums of their own products allow."""
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 36, ignored=0.1)
+    t[0] = t[7] = vocab // 2
+    for at in (0, 7):
+        big = x.clone()
+        big[at] *= size
+        check_own(big, w, b, t, dloss)
+    for at in (3, vocab - 1):
+        big = w.clone()
+        big[at] *= size
+        check_own(x, big, b, t, dloss)
+
+
+@pytest.mark.parametrize("n, vocab, dim", UNLIKE_SHAPES)
+def test_rows_and_columns_of_unlike_size(cuda, n, vocab, dim):
+    """Rows of x over 25 decades, rows of the weight over 20, columns over 30 (of x and, the other
+    way round, of the weight), and columns of either alone: features in units of their own."""
+    import torch
+
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 37, ignored=0.1)
+    g = torch.Generator(device="cuda").manual_seed(2)
+
+    def decades(low, high, count):
+        order = torch.randperm(count, device=cuda, generator=g)
+        return 10.0 ** torch.linspace(low, high, count, device=cuda)[order]
+
+    check_own(x * decades(-22, 3, n).unsqueeze(1), w, b, t, dloss)
+    check_own(x, w * decades(-18, 2, vocab).unsqueeze(1), b, t, dloss)
+    both = decades(-15, 15, dim)
+    check_own(x * both, w / both, b, t, dloss)
+    check_own(x * decades(-20, 0, dim), w, b, t, dloss)
+    check_own(x, w * decades(-20, 0, dim), b, t, dloss)
+    rare = x.clone()
+    rare[:, 1] *= 1e-12
+    check_own(rare, w, b, t, dloss)
+
+
+def test_operands_of_unlike_size_through_views_of_any_layout(cuda):
+    """As test_linear_cross_entropy_takes_views_of_any_layout, with rows and columns that the pairs
+    do not hold; NaN in rows without a loss; each gradient alone."""
+    import torch
+
+    n, vocab, dim = 523, 1111, 139
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 38, ignored=0.2)
+    x[5] *= 1e13
+    w[:, 3] *= 1e-14
+    t[5] = 4
+    xt = x.t().contiguous().t()
+    ws = torch.randn(vocab, dim + 3, device=cuda)
+    ws[:, 1:1 + dim] = w
+    bs = torch.stack([b, b + 1], 1)
+    xn = xt.clone()
+    xn[t == IGNORE] = float("nan")
+    want = {**ce_reference(x, w, b, t, None), **own_bounds(x, w, b, t, dloss)}
+    out = {"dx": torch.full((n, dim + 2), 55.0, device=cuda)[:, 1:1 + dim],
+           "dw": torch.full((dim, vocab + 1), 55.0, device=cuda)[:, 1:].t(),
+           "db": torch.full((vocab, 3), 55.0, device=cuda)[:, 1], "loss": torch.full((n,), 55.0, device=cuda)}
+    names = {"dw": "dweight", "db": "dbias"}
+    args = view(xn), view(ws[:, 1:1 + dim]), view(t), view(dloss)
+    abi.linear_cross_entropy_grad(*args, bias=view(bs[:, 0]), ignore_target=IGNORE,
+                                  **{names.get(k, k): view(v) for k, v in out.items()})
+    abi.check_device_errors(0)
+    for k, v in out.items():
+        within(v, want[k][0], want[k][1] + 1e-42, k)
+    for k, v in out.items():
+        alone = torch.full(v.shape, 44.0, device=cuda)
+        abi.linear_cross_entropy_grad(*args, bias=view(bs[:, 0]), ignore_target=IGNORE, **{names.get(k, k): view(alone)})
+        assert torch.equal(alone, v), k
 
 
 @pytest.mark.parametrize("n, vocab, dim", [(2 ** 21 - 1, 1, 1), (2 ** 21 - 1, 2, 0), (2 ** 20, 3, 0), (2 ** 20 - 1, 3, 0)])
