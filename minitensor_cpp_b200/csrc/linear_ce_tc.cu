@@ -272,17 +272,17 @@ __device__ __forceinline__ void judge(const Held &h, int64_t at, int64_t step, i
     if (bad) atomicOr(wide, 1);
 }
 
-// Sets the bytes of four columns; most are set already.
-__device__ __forceinline__ void mark_columns(unsigned char *to, unsigned int four) {
+// Sets the bytes of those of four columns that reach `least`; most are set already.
+__device__ __forceinline__ void mark_columns(unsigned char *to, const float (&largest)[4], float least) {
     const unsigned int has = __ldcg(reinterpret_cast<const unsigned int *>(to));
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        if ((four >> k & 1) && !(has >> (8 * k) & 1)) to[k] = 1;
+        if (largest[k] >= least && !(has >> (8 * k) & 1)) to[k] = 1;
 }
 
-// Each half-warp packs one block of 64 columns of every so many rows: a lane four columns.
+// Each half-warp packs one block of 64 columns of four rows in every so many: a lane four columns.
 // AGAIN: only the tensors whose scale was wrong; and the exponents are written down.  Bound by
-// HBM, 8 bytes an element: 36096 rows of 2048 in 103 us (5.7 TB/s).
+// HBM, 8 bytes an element: 36096 rows of 2048 in 96 us (6.2 TB/s).
 template <bool AGAIN>
 __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     wait_for_previous();
@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     }
     const Held &held = s.held[AGAIN];
     const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
+    const float enough = kHeld * power_of_two(-(e / 2)) * power_of_two(-(e - e / 2));  // of an element as it is
     const int lane = threadIdx.x % 16;
     const unsigned int mates = 0xFFFFu << (threadIdx.x & 16);
     float largest = 0.0f;
@@ -313,15 +314,16 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     const int at = abreast > 0 ? half % abreast : 0, r_first = abreast > 0 ? half / abreast : 0;
     for (int64_t b0 = 0; b0 < blocks; b0 += abreast) {
         const int64_t b = b0 + at, c = b * kBlock + lane * 4;
-        const bool mine = b < blocks && r_first < step;
-        unsigned int col_ok = 0, col_some = 0;
+        const bool mine = b < blocks && r_first < step, reads = mine && c < s.cols;
+        float col[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int64_t r0 = 0; r0 < rows_out; r0 += static_cast<int64_t>(step) * U) {
             float4 v[U];
+            unsigned int rows_ok = 0;  // a byte a row, of the half-warp's
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t r = r0 + static_cast<int64_t>(u) * step + r_first;
+                const int64_t r = r0 + r_first * U + u;
                 v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (!mine || r >= rows || c >= s.cols) continue;
+                if (!reads || r >= rows) continue;
                 const float *src = source_row(s, r);
                 if (s.vec) {
                     v[u] = __ldg(reinterpret_cast<const float4 *>(src + c));
@@ -334,32 +336,40 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t r = r0 + static_cast<int64_t>(u) * step + r_first;
-                if (!AGAIN && a.headroom != 0)
-                    largest = fmaxf(largest, fmaxf(fmaxf(finite_abs(v[u].x), finite_abs(v[u].y)),
-                                                   fmaxf(finite_abs(v[u].z), finite_abs(v[u].w))));
-                const float x[4] = {v[u].x * f0 * f1, v[u].y * f0 * f1, v[u].z * f0 * f1, v[u].w * f0 * f1};
-                const float raw[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-                unsigned int ok = 0, some = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool finite = fabsf(x[k]) <= 3.402823466e38f;
-                    ok |= static_cast<unsigned int>(finite && fabsf(x[k]) >= kHeld) << k;
-                    some |= static_cast<unsigned int>(finite && raw[k] != 0.0f) << k;
+                const int64_t r = r0 + r_first * U + u;
+                float4 m = v[u];  // its magnitudes: a maximum passes NaN over, and infinities are taken out
+                float top = fmaxf(fmaxf(fabsf(m.x), fabsf(m.y)), fmaxf(fabsf(m.z), fabsf(m.w)));
+                if (isinf(top)) {
+                    m = make_float4(finite_abs(m.x), finite_abs(m.y), finite_abs(m.z), finite_abs(m.w));
+                    top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
                 }
-                col_ok |= ok;
-                col_some |= some;
-                const unsigned int row_ok = __ballot_sync(0xFFFFFFFFu, ok != 0), row_some = __ballot_sync(0xFFFFFFFFu, some != 0);
+                col[0] = fmaxf(col[0], fabsf(m.x));
+                col[1] = fmaxf(col[1], fabsf(m.y));
+                col[2] = fmaxf(col[2], fabsf(m.z));
+                col[3] = fmaxf(col[3], fabsf(m.w));
+                const unsigned int ok = __ballot_sync(0xFFFFFFFFu, top >= enough) & mates;
+                const unsigned int some = __ballot_sync(0xFFFFFFFFu, top > 0.0f) & mates;
+                rows_ok |= (ok != 0 ? 1u : 0u) << (8 * u);
                 if (!mine || r >= rows_out) continue;
-                if (lane == 0 && (row_ok & mates)) held.row_ok[r] = 1;
-                else if (lane == 0 && (row_some & mates)) held.row_some[r] = 1;
-                store_pairs(s.to + (r * blocks + b) * 2 * kBlock + lane * 4, x[0], x[1], x[2], x[3]);
+                if (lane == 0 && some != 0 && ok == 0) held.row_some[r] = 1;
+                store_pairs(s.to + (r * blocks + b) * 2 * kBlock + lane * 4, v[u].x * f0 * f1, v[u].y * f0 * f1,
+                            v[u].z * f0 * f1, v[u].w * f0 * f1);
+            }
+            // (bytes that are not set stay as another half-warp may have set them)
+            const int64_t r = r0 + r_first * U;
+            if (lane == 0 && rows_ok == 0x01010101u) {
+                *reinterpret_cast<unsigned int *>(held.row_ok + r) = rows_ok;
+            } else if (lane == 0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (rows_ok >> (8 * u) & 1) held.row_ok[r + u] = 1;
             }
         }
         if (mine) {
-            mark_columns(held.col_ok + c, col_ok);
-            mark_columns(held.col_some + c, col_some);
+            mark_columns(held.col_ok + c, col, enough);
+            mark_columns(held.col_some + c, col, 1e-45f);
         }
+        largest = fmaxf(largest, fmaxf(fmaxf(col[0], col[1]), fmaxf(col[2], col[3])));
     }
     if (!AGAIN && a.headroom != 0) {
         keep_max(largest, a.known + kLargest + s.which);
@@ -1389,13 +1399,13 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     k.dx_cs = p.dx_cs;
     k.dx_vec = vector_source(p.dx, p.dx_rs, p.dx_cs, p.D);
     k.known = live.count;
-    // CTAs in proportion to the tensors' rows, eight to an SM in all
-    const int64_t most = static_cast<int64_t>(sms) * 8;
+    // CTAs in proportion to the tensors' rows, four to an SM in all
+    const int64_t most = static_cast<int64_t>(sms) * 4;
     const int64_t share = most * p.N / (p.N + p.V);
     k.first_of_second = share < 1 ? 1 : share > most - 1 ? most - 1 : share;
     const unsigned ctas = static_cast<unsigned>(most);
     {
-        PackArgs few = k;  // a quarter of the CTAs, half of them each
+        PackArgs few = k;  // half of the CTAs, a quarter for each
         few.first_of_second = sms;
         MTC_TRY(launch_dependent("linear cross entropy (sample)", k_sample, static_cast<unsigned>(2 * sms), 256, 0, stream, few));
     }
