@@ -8,7 +8,9 @@
 // 1e154, and at 64 DFMA a clock and SM far from the bound), per thread, then
 // per CTA in a fixed tree, then over the CTAs in index order, so the same
 // tensors give the same bits.  No third launch joins the CTAs' sums: every CTA
-// of the scaling adds the few hundred partial sums itself, in the same order.
+// of the scaling adds the up to 1184 partial sums of a launch itself, in the
+// same order.  Of many launches (views with gaps) there are too many for that,
+// and one CTA adds them first.
 //
 // All tensors that are dense in memory go through one launch per pass: their
 // addresses and sizes travel in the kernel's parameters (28 bytes each, up to
@@ -67,6 +69,7 @@ __device__ __forceinline__ double block_sum(double v) {
 // Sum of the CTAs' partial sums; every thread of every CTA gets the same value.
 __device__ __forceinline__ double sum_partials(const double *partials, int n) {
     double v = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < n; i += blockDim.x) v += partials[i];
     return block_sum(v);
 }
@@ -221,7 +224,19 @@ __global__ void __launch_bounds__(kThreads) k_write_norm(const double *partials,
     if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(sum));
 }
 
+// One partial sum in the place behind all others, in their stead.
+__global__ void __launch_bounds__(kThreads) k_total(double *partials, int n_partials) {
+    wait_for_previous();
+    const double sum = sum_partials(partials, n_partials);
+    if (threadIdx.x == 0) partials[n_partials] = sum;
+}
+
 // ------------------------------------------------------------------- host --
+
+// Partial sums that every CTA of the scaling adds itself: those of three launches at most.  Each
+// CTA of each launch reads them, which is quadratic in the number of views with gaps (of 1000 x 1022
+// each: 4 take 91 us so and 82 with their sum taken first, 100 18.0 and 2.3 ms).
+constexpr int kOwnPartials = 4096;
 
 struct Dense {
     const float *src;
@@ -386,6 +401,11 @@ struct Launcher {
     }
 
     int scale(float max_norm, float *norm) {
+        if (n_partials > kOwnPartials) {
+            MTC_TRY(launch_dependent("global norm (total)", k_total, 1, kThreads, 0, stream, partials, n_partials));
+            partials += n_partials;
+            n_partials = 1;
+        }
         float *write = norm;  // by the first launch alone
         MTC_TRY(tables([&](const auto &t) {
             constexpr int N = sizeof(t.n) / sizeof(t.n[0]);

@@ -970,6 +970,25 @@ def test_clipping_of_views_with_gaps(cuda):
     assert_clipped(ref[:2], outs, norm, 1.5)
 
 
+@pytest.mark.parametrize("views, rows", [(3, 700), (4, 700), (60, 700), (200, 3)])
+def test_clipping_of_many_views_with_gaps(cuda, views, rows):
+    """So many partial sums that they are added before the scaling, and as many as are not."""
+    import torch
+
+    torch.manual_seed(views)
+    store = torch.randn(views, rows, 512, device=cuda)
+    tensors = [s[:, 1:-1] for s in store] + [torch.randn(1000, device=cuda)]
+    ref = [t.clone() for t in tensors]
+    rest = store[:, :, 0].clone()
+    norm, alone = torch.empty(1, device=cuda), torch.empty(1, device=cuda)
+    abi.global_norm([view(t) for t in tensors], view(alone))
+    for max_norm in (1e30, 2.0):
+        abi.clip_global_norm([view(t) for t in tensors], max_norm, view(norm))
+        assert torch.equal(alone, norm)
+        assert_clipped(ref, tensors, norm, max_norm)
+    assert torch.equal(store[:, :, 0], rest)
+
+
 def test_norms_beyond_the_range_of_float32_squares(cuda):
     import torch
 
