@@ -1299,9 +1299,8 @@ bool vector_source(const float *p, int64_t rs, int64_t cs, int64_t cols) {
     return aligned16(p) && cs == 1 && rs % 4 == 0 && cols % 4 == 0;
 }
 
-}  // namespace
-
-int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
+// `most_rows`: of a piece, a multiple of 256.
+int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
     const int sms = sm_count(current_device());
     const int64_t pairs = sms / 2;
     const bool grads = p.dloss != nullptr && ((p.D > 0 && (p.dx != nullptr || p.dw != nullptr)) || p.db != nullptr);
@@ -1317,7 +1316,7 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const int64_t row_bytes = grads ? pitch * (two ? 8 : 4) : static_cast<int64_t>(tiles_v) * 16;
     int64_t piece = (int64_t{4} << 30) / row_bytes / 256 * 256;
     if (piece < 256) piece = 256;
-    if (piece > (int64_t{1} << 21)) piece = int64_t{1} << 21;  // k_softmax_grad's grid
+    if (piece > most_rows) piece = most_rows;
     const int64_t pieces = (rows_all + piece - 1) / piece;
     piece = ((rows_all + pieces - 1) / pieces + 255) / 256 * 256;
     if (rows_all * d_blocks > (int64_t{1} << 40) || pitch > INT32_MAX)
@@ -1353,9 +1352,15 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
     const size_t held_x = padded(static_cast<size_t>(rows_all)), held_w = padded(static_cast<size_t>(p.V));
     const size_t held_d = padded(static_cast<size_t>(d_pad)), held = 4 * (held_x + held_w + 2 * held_d);
     Workspace ws;
-    MTC_TRY(ws.allocate(256 + held + 3 * list + x_bytes + w_bytes + 2 * stat + 4 * row_stat + z_bytes + by_class_bytes + db_bytes +
-                            exp_bytes + split_bytes,
-                        stream));
+    const int allocated = ws.allocate(256 + held + 3 * list + x_bytes + w_bytes + 2 * stat + 4 * row_stat + z_bytes +
+                                          by_class_bytes + db_bytes + exp_bytes + split_bytes,
+                                      stream);
+    if (allocated == MTC_ERR_RUNTIME && piece > 256) {  // no memory for that: in smaller pieces
+        MTC_TRY(in_pieces(p, stream, piece / 2 / 256 * 256));
+        clear_error();
+        return MTC_OK;
+    }
+    MTC_TRY(allocated);
     LiveRows live;
     live.count = ws.take<int>(256);
     live.row = ws.take<int>(list);
@@ -1533,6 +1538,12 @@ int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
         }
     }
     return MTC_OK;
+}
+
+}  // namespace
+
+int linear_ce_tensor(const LinearCe &p, cudaStream_t stream) {
+    return in_pieces(p, stream, int64_t{1} << 21);  // k_softmax_grad's grid
 }
 
 }  // namespace mtc

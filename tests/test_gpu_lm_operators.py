@@ -878,6 +878,42 @@ def test_more_rows_than_a_piece_of_the_logits_holds(cuda):
     within(got["db"], db, db_tol * longer, "db")
 
 
+def test_little_memory_makes_smaller_pieces(cuda):
+    """Of a workspace of 1.7 GB, 1.2 can be had: the rows go in two pieces instead of one."""
+    import torch
+
+    lib = abi.lib()
+    x, w, b, t, dloss = ce_data(1500, 131072, 24, 39, ignored=0.1)
+    want = ce_reference(x, w, b, t, dloss)
+    whole = run_ce(x, w, b, t, dloss)
+    torch.cuda.synchronize()
+    outs = run_ce(x, w, b, t, dloss)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    abi.check(lib.mtc_pool_trim(0), "trim")
+    free = torch.cuda.mem_get_info()[0]
+    hold = torch.empty(free - (1200 << 20), dtype=torch.uint8, device=cuda)
+    for o in outs.values():
+        o.fill_(7.0)
+    try:
+        abi.linear_cross_entropy_grad(view(x), view(w), view(t), view(dloss), dx=view(outs["dx"]), dweight=view(outs["dw"]),
+                                      bias=view(b), dbias=view(outs["db"]), loss=view(outs["loss"]), lse=view(outs["lse"]),
+                                      ignore_target=IGNORE)
+        torch.cuda.synchronize()
+        used, cached = ctypes.c_uint64(), ctypes.c_uint64()
+        abi.check(lib.mtc_pool_stats(0, ctypes.byref(used), ctypes.byref(cached)), "pool stats")
+        assert 0 < used.value < 1200 << 20  # it did run in less
+    finally:
+        del hold
+        abi.check(lib.mtc_pool_trim(0), "trim")
+    abi.check_device_errors(0)
+    assert torch.equal(outs["loss"], whole["loss"]) and torch.equal(outs["lse"], whole["lse"])
+    for name in ("dx", "dw", "db"):
+        within(outs[name], want[name][0], want[name][1] + 1e-42, name)
+    del want, whole, outs, x, w, b
+    torch.cuda.empty_cache()  # the reference's, for what comes next
+
+
 def test_linear_cross_entropy_beyond_32_bits(cuda):
     """A weight of 2.2e9 elements: the loss and sampled rows of its gradient against
     float64, on classes at the end of the vocabulary."""
