@@ -197,12 +197,17 @@ __global__ void __launch_bounds__(256) k_small_rows(const LinearCe p, const Smal
     }
     for (int o = 1; o < 32; o <<= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const double base = isinf(top) ? 0.0 : top;
-    double sum = 0.0;
+    double rest = 0.0;  // the others' exponentials, as in Softmax
+    int same = 0;
 #pragma unroll
-    for (int i = 0; i < kMost; ++i)
-        if (i * C < p.V && sub == 0) sum += expf(static_cast<float>(z[i] - base));
-    for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const float beyond = static_cast<float>(log(sum));  // lse = base + beyond
+    for (int i = 0; i < kMost; ++i) {
+        if (i * C >= p.V || sub != 0) continue;
+        if (z[i] == top) ++same;
+        else rest += expf(static_cast<float>(z[i] - base));
+    }
+    for (int o = 1; o < 32; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
+    rest += static_cast<double>(static_cast<int>(__reduce_add_sync(0xFFFFFFFFu, same)) - 1);
+    const float beyond = static_cast<float>(!isinf(top) ? log1p(rest) : isnan(rest) ? rest : top);  // lse = base + beyond
     zt = __shfl_sync(0xFFFFFFFFu, zt, t % C * L);
     if (lane == 0) {
         if (p.loss != nullptr) p.loss[n * p.loss_s] = static_cast<float>(base - zt) + beyond;

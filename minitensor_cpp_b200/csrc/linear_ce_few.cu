@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
     constexpr int kMine = (4 * R + 31) / 32;  // logits of a lane: i = lane + 32 k is few i / 4 and many i % 4
     Softmax mine[kMine];
 #pragma unroll
-    for (int k = 0; k < kMine; ++k) mine[k] = Softmax{-INFINITY, 0.0};
+    for (int k = 0; k < kMine; ++k) mine[k] = no_logits();
     float acc[4 * R];
 #pragma unroll
     for (int i = 0; i < 4 * R; ++i) acc[i] = 0.0f;
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
                 const int64_t n = v0 + lane % 4;  // the lanes of a row: its classes, lane / 4 apart
                 const bool in = n < many && (R >= 8 || lane < 4 * R);
                 const int t = n < many ? row_target(p, n, a.err, lane < 4) : -1;
-                Softmax s{-INFINITY, 0.0};
+                Softmax s = no_logits();
                 float zt = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < kMine; ++k) {
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
                     const float other = __shfl_xor_sync(0xFFFFFFFFu, zt, o);
                     if (zt == -INFINITY) zt = other;
                 }
-                const LogSum l = log_sum(s.top, s.sum);
+                const LogSum l = s.log_sum();
                 if (lane < 4 && n < many) {
                     if (p.loss != nullptr) p.loss[n * p.loss_s] = t < 0 ? 0.0f : l.loss(zt);
                     if (p.lse != nullptr) p.lse[n * p.lse_s] = t < 0 ? 0.0f : l.lse();
@@ -228,21 +228,11 @@ __global__ void __launch_bounds__(kFewThreads, few_resident(R)) k_few_logits(con
 
 // lse of row n from the CTAs' parts; every lane of the warp gets it.
 __device__ __forceinline__ LogSum few_lse(const FewArgs &a, int R, int n) {
-    Softmax s{-INFINITY, 0.0};
+    Softmax s = no_logits();
     const Softmax *parts = a.parts + n;
 #pragma unroll 8
-    for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) s.top = fmaxf(s.top, parts[i * R].top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s.top = fmaxf(s.top, __shfl_xor_sync(0xFFFFFFFFu, s.top, o));
-    const float base = softmax_base(s.top);
-#pragma unroll 8
-    for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) {
-        const Softmax x = parts[i * R];
-        if (x.sum != 0.0) s.sum += x.sum * expf(softmax_base(x.top) - base);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s.sum += __shfl_xor_sync(0xFFFFFFFFu, s.sum, o);
-    return log_sum(s.top, s.sum);
+    for (int i = threadIdx.x % 32; i < a.n_parts; i += 32) s = merge(s, parts[i * R]);
+    return merge_lanes(s, 1, 32).log_sum();
 }
 
 __device__ __forceinline__ void store_loss(const LinearCe &p, const FewArgs &a, int n, int target, LogSum l) {

@@ -418,7 +418,7 @@ struct TileArgs {
     const float *bias;
     int64_t bias_s;
     const int *target;
-    float *part_max, *part_rest;  // [M][2 tiles_n], see Rest
+    float *part_max, *part_rest;  // [M][2 tiles_n], see Softmax
     float *z_target;              // [M]
     // Sum
     float *out;       // rows of 32-byte sectors
@@ -571,32 +571,6 @@ __device__ __forceinline__ void rescale(float (&acc)[128], float f0, float f1) {
 #pragma unroll
         for (int j = 0; j < 128; ++j) acc[j] *= f1;
     }
-}
-
-// The largest of some logits, and the exponentials of the others relative to it, in float32 and
-// without one occurrence of the largest: next to its 1 they would lose the digits that are the
-// gradient of a row sure of its class.  (300 rows, 100 classes, the target's logit 16 above the
-// others: with the 1 in the sum the target's gradient is off by 6e-3 of itself.)  1 + rest is the
-// sum; no logits at all: -inf and -1.
-struct Rest {
-    float top;
-    double rest;
-};
-
-__device__ __forceinline__ Rest merge(Rest a, Rest b) {
-    if (b.top > a.top) {
-        const Rest c = a;
-        a = b;
-        b = c;
-    }
-    // equal infinities: a factor of 1, so that -inf adds 1 - 1 and NaN stays
-    a.rest += (1.0 + b.rest) * (a.top == b.top ? 1.0f : expf(b.top - a.top));
-    return a;
-}
-
-__device__ __forceinline__ LogSum log_sum(Rest s) {
-    if (isinf(s.top)) return LogSum{0.0f, isnan(s.rest) ? static_cast<float>(s.rest) : s.top};
-    return LogSum{s.top, static_cast<float>(log1p(s.rest))};
 }
 
 // The logits' epilogue: this lane's row, 128 columns from col0 on.  What most tiles do
@@ -1062,13 +1036,11 @@ __global__ void __launch_bounds__(256) k_row_loss(const RowArgs a) {
     const int lane = threadIdx.x % 32;
     if (r >= live_extent(a.live, a.first, a.rows)) return;
     const float *m = a.part_max + r * a.part_pitch, *s = a.part_rest + r * a.part_pitch;
-    Rest all{-INFINITY, -1.0};
-    for (int j = lane; j < a.parts; j += 32) all = merge(all, Rest{m[j], s[j]});
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        all = merge(all, Rest{__shfl_xor_sync(0xFFFFFFFFu, all.top, o), __shfl_xor_sync(0xFFFFFFFFu, all.rest, o)});
+    Softmax all = no_logits();
+    for (int j = lane; j < a.parts; j += 32) all = merge(all, Softmax{m[j], s[j]});
+    all = merge_lanes(all, 1, 32);
     if (lane != 0) return;
-    const LogSum l = log_sum(all);
+    const LogSum l = all.log_sum();
     a.lse_live[r] = l;
     // the largest |g| of a row is that of its target, to which all others add up
     if (a.dloss != nullptr)

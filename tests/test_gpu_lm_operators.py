@@ -737,7 +737,9 @@ def test_gradients_of_rows_sure_of_their_class(cuda, n, vocab, dim):
     check_own(torch.cat([x, lift], 1), w, b * 0.1, t, torch.ones(n, device=cuda))
 
 
-@pytest.mark.parametrize("n, vocab, dim", [(300, 100, 512), (300, 128, 512), (600, 1000, 96), (60, 200, 4096), (17, 900, 400)])
+@pytest.mark.parametrize("n, vocab, dim", [(300, 100, 512), (300, 128, 512), (600, 1000, 96), (60, 200, 4096), (17, 900, 400),
+                                           (1, 4, 450), (5, 200, 64), (1, 3000, 515), (3, 1000, 64), (16, 700, 128),
+                                           (4000, 6, 1024), (9001, 16, 64), (300, 3, 64), (40, 90, 16)])
 @pytest.mark.parametrize("gap", [40.0, 75.0])
 def test_gradients_below_the_first_step_of_one(cuda, n, vocab, dim, gap):
     """What is left next to a probability that float64 too holds as 1, by the bounds of
