@@ -114,7 +114,7 @@ static_assert(kArrived + 2 == kLiveKnown, "zeroed with the count");
 // reaches 2^-12.  Beside the largest of the tensor, scaled to 2^8 at least, such a row may be
 // smaller by 2^20.  A byte each says whether the row (column) has an element that large and
 // whether it has any at all that is finite and not zero: one that has but the latter makes the
-// products go by float32 (plain_sum).
+// products go by float32 (plain_sums).
 constexpr float kHeld = 0x1p-12f;
 struct Held {
     unsigned char *row_ok, *row_some, *col_ok, *col_some;
@@ -606,22 +606,30 @@ __device__ __forceinline__ void store_logits(const TileArgs &a, int64_t M, float
     // exp by the hardware's 2^x (2^-22): its error and the product's weigh little in a sum
     // whose largest terms have arguments near zero
     const float base = isinf(top[0]) ? 0.0f : top[0];
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 128; ++j) sum[j % 4] += __expf(acc[j] - base);
-    float rest = (sum[0] + sum[1]) + (sum[2] + sum[3]) - 1.0f;
-    // The 1 costs the others digits where they are little next to it: then they are summed
-    // again, without the one logit that is the largest.  (4096 x 32000 x 1024, a quarter of the
-    // rows without loss: 599 us with that choice made for every logit, 573 so.)
-    if (rest < 0.125f && !isinf(top[0])) {
+    for (int j = 0; j < 128; ++j) sum[j % 8] += __expf(acc[j] - base);
+    auto total = [&] { return ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7])); };
+    float rest = total() - 1.0f;
+    // The 1 costs the others of its eighth digits where they are little next to it: then these are
+    // summed again, without the one logit that is the largest.  (Every tile waits for the slowest of
+    // its 16 warps.  3000 x 32000 x 1024, logits of deviation 2, which leaves 1 of 1700 rows of 128 so:
+    // 501 us for the logits; 534 from 1/8 on and with all eighths summed again; 485 not at all.)
+    if (rest < 0.0625f && !isinf(top[0])) {
         float again = base;
         asm volatile("" : "+f"(again));  // or the first sum's exponentials are kept, in memory
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] = 0.0f;
+        for (int k = 0; k < 8; ++k) {
+            bool here = false;
 #pragma unroll
-        for (int j = 0; j < 128; ++j)
-            if (acc[j] != again) sum[j % 4] += __expf(acc[j] - again);
-        rest = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            for (int j = k; j < 128; j += 8) here |= acc[j] == again;
+            if (!here) continue;
+            sum[k] = 0.0f;
+#pragma unroll
+            for (int j = k; j < 128; j += 8)
+                if (acc[j] != again) sum[k] += __expf(acc[j] - again);
+        }
+        rest = total();
     }
     if (live) {
         a.part_max[row * 2 * a.tiles_n + part] = top[0];
@@ -640,52 +648,111 @@ __device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&
     else store_row(a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0, acc, n, a.add);
 }
 
-// ROWS rows of 32 columns of an operand into shared memory, the columns `pitch` apart; zeros
-// beyond its ends.  256 threads, next to one another where the operand's elements are.
+// The products in float32, on the FMA units, for operands whose rows or columns are of so unlike
+// size that pairs on one scale lose the small ones.  The first four warps stage 16 columns of K at
+// a time in one of two buffers while the epilogue's eight work on the other, 8 x 16 sums a thread,
+// and hand them over, a row of 128 to a lane, by way of shared memory.  Bound by the FMAs and the
+// waits of two warps a scheduler: 4096 x 32000 x 1024 in 12.1 ms for the loss and 35.0 with dx and
+// dweight, 22 to 23 TFLOP/s, where pairs take 0.64 and 2.2 ms.
+constexpr int kPlainK = 16, kPlainPitchA = 132, kPlainPitchB = 260;
+constexpr int kPlainBuffer = kPlainK * (kPlainPitchA + kPlainPitchB);  // floats
+static_assert((2 * kPlainBuffer + 128 * kPlainPitchB) * 4 <= kStages * kStageBytes, "two buffers and the sums of a CTA");
+
+__device__ __forceinline__ void plain_barrier() { asm volatile("bar.sync 1, 384;" ::: "memory"); }
+
+struct PlainRange {
+    int64_t begin, end;  // of K
+    __device__ __forceinline__ PlainRange(const Extent &e, int kb0, int kb1) {
+        begin = static_cast<int64_t>(kb0) * kBlock;
+        end = static_cast<int64_t>(kb1) * kBlock < e.K ? static_cast<int64_t>(kb1) * kBlock : e.K;
+    }
+};
+
+// ROWS rows of 16 columns of an operand; zeros beyond its ends.  128 threads, next to one another
+// where the operand's elements are.
 template <int ROWS>
 __device__ __forceinline__ void stage_plain(const Plain &o, int64_t row0, int64_t rows, int64_t k0, int64_t k1, float *to,
-                                            int pitch, int thread) {
+                                            int pitch) {
     const bool along_k = o.ks == 1 || o.rs != 1;
-#pragma unroll 4
-    for (int i = thread; i < ROWS * 32; i += 256) {
-        const int r = along_k ? i / 32 : i % ROWS, k = along_k ? i % 32 : i / ROWS;
+    const int thread = threadIdx.x;
+#pragma unroll 8
+    for (int i = 0; i < ROWS / 8; ++i) {
+        const int r = along_k ? thread / kPlainK + 8 * i : thread + 128 * (i % (ROWS / 128));
+        const int k = along_k ? thread % kPlainK : i / (ROWS / 128);
         const int64_t row = row0 + r, col = k0 + k;
-        float v = 0.0f;
-        if (row < rows && col < k1)
-            v = __ldg(o.p + (o.rows != nullptr ? o.rows[row] : row) * o.rs + (o.ks_map != nullptr ? o.ks_map[col] : col) * o.ks);
-        to[k * pitch + r] = v;
+        const float *from = o.p;
+        int bytes = 0;  // none: a zero
+        if (row < rows && col < k1) {
+            from += (o.rows != nullptr ? o.rows[row] : row) * o.rs + (o.ks_map != nullptr ? o.ks_map[col] : col) * o.ks;
+            bytes = 4;
+        }
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to + k * pitch + r)), "l"(from), "r"(bytes)
+                     : "memory");
     }
 }
 
-// The sums of this lane's row and 128 columns in float32, on the FMA units, for operands whose
-// rows or columns are of so unlike size that pairs on one scale lose the small ones.  A lane's 128
-// products take one element of A and, all lanes alike, 32 vectors of B from shared memory: bound by
-// the FMAs.
-__device__ __forceinline__ void plain_sum(const TileArgs &a, const Extent &e, float *as, int tm, int tn, int rank, int kb0,
-                                          int kb1, float (&acc)[128]) {
-    constexpr int kPitchA = 132, kPitchB = 260;
-    float *bs = as + 32 * kPitchA;
-    const int thread = threadIdx.x - 128, quadrant = (threadIdx.x / 32) % 4, half = thread / 128;
-    const int64_t k_end = static_cast<int64_t>(kb1) * kBlock < e.K ? static_cast<int64_t>(kb1) * kBlock : e.K;
-    const float *mine = as + quadrant * 32 + threadIdx.x % 32;
-    for (int64_t k0 = static_cast<int64_t>(kb0) * kBlock; k0 < k_end; k0 += 32) {
-        stage_plain<128>(a.a, static_cast<int64_t>(tm) * kTileRows + rank * 128, e.M, k0, k_end, as, kPitchA, thread);
-        stage_plain<256>(a.b, static_cast<int64_t>(tn) * kTileCols, a.N, k0, k_end, bs, kPitchB, thread);
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the epilogue warps alone
-#pragma unroll 1
-        for (int k = 0; k < 32; ++k) {
-            const float x = mine[k * kPitchA];
-            const float4 *row = reinterpret_cast<const float4 *>(bs + k * kPitchB + half * 128);
+// `turn` counts the buffers filled (emptied) so far.  A buffer is filled again after the barrier
+// behind which the other one is read, so after it has been read.
+__device__ __forceinline__ void plain_stages(const TileArgs &a, const Extent &e, float *smem, int tm, int tn, int rank,
+                                             PlainRange k, int &turn) {
+    for (int64_t k0 = k.begin; k0 < k.end; k0 += kPlainK, ++turn) {
+        float *as = smem + (turn & 1) * kPlainBuffer;
+        stage_plain<128>(a.a, static_cast<int64_t>(tm) * kTileRows + rank * 128, e.M, k0, k.end, as, kPlainPitchA);
+        stage_plain<256>(a.b, static_cast<int64_t>(tn) * kTileCols, a.N, k0, k.end, as + kPlainK * kPlainPitchA, kPlainPitchB);
+        cp_async_wait_all();
+        plain_barrier();
+    }
+}
+
+__device__ __forceinline__ void plain_sums(float *smem, PlainRange k, int &turn, float (&acc)[128]) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float4 y = row[j];
-                acc[4 * j] = fmaf(x, y.x, acc[4 * j]);
-                acc[4 * j + 1] = fmaf(x, y.y, acc[4 * j + 1]);
-                acc[4 * j + 2] = fmaf(x, y.z, acc[4 * j + 2]);
-                acc[4 * j + 3] = fmaf(x, y.w, acc[4 * j + 3]);
+    for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+    if (k.begin >= k.end) return;
+    const int thread = threadIdx.x - 128, ty = thread / 16, tx = thread % 16;
+    float2 two[8][8];  // rows, pairs of columns: two of a multiply-add (FFMA2)
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) two[r][q] = make_float2(0.0f, 0.0f);
+    for (int64_t k0 = k.begin; k0 < k.end; k0 += kPlainK, ++turn) {
+        plain_barrier();
+        const float *as = smem + (turn & 1) * kPlainBuffer + ty * 8;
+        const float *bs = smem + (turn & 1) * kPlainBuffer + kPlainK * kPlainPitchA + tx * 4;
+#pragma unroll 2
+        for (int i = 0; i < kPlainK; ++i) {
+            const float4 x0 = *reinterpret_cast<const float4 *>(as + i * kPlainPitchA);
+            const float4 x1 = *reinterpret_cast<const float4 *>(as + i * kPlainPitchA + 4);
+            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            float4 y[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const float4 *>(bs + i * kPlainPitchB + 64 * q);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float2 xx = make_float2(x[r], x[r]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    two[r][2 * q] = __ffma2_rn(xx, make_float2(y[q].x, y[q].y), two[r][2 * q]);
+                    two[r][2 * q + 1] = __ffma2_rn(xx, make_float2(y[q].z, y[q].w), two[r][2 * q + 1]);
+                }
             }
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    float *sums = smem + 2 * kPlainBuffer;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4 *>(sums + (ty * 8 + r) * kPlainPitchB + tx * 4 + 64 * q) =
+                make_float4(two[r][2 * q].x, two[r][2 * q].y, two[r][2 * q + 1].x, two[r][2 * q + 1].y);
+    asm volatile("bar.sync 2, 256;" ::: "memory");  // the epilogue's warps alone
+    const float *mine = sums + (thread % 128) * kPlainPitchB + thread / 128 * 128;
+#pragma unroll
+    for (int j = 0; j < 128; j += 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(mine + j);
+        acc[j] = v.x;
+        acc[j + 1] = v.y;
+        acc[j + 2] = v.z;
+        acc[j + 3] = v.w;
     }
 }
 
@@ -737,7 +804,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
     wait_for_previous();
     const Extent e = extent_of(args);
     const bool wide = *args.wide != 0;
-    const int64_t first_unit = wide ? e.units : cluster;  // of the tensor core's warps
 
     if (warp >= 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
@@ -746,15 +812,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
         const int exp_b = *args.exp_b;
         int64_t piece = 0;
         bool ok = true;
-        for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+        if (wide) {  // apart from the other loop, whose registers it would take
+            int turn = 0;
+            for (int64_t u = cluster; u < e.units; u += clusters) {
+                int tm, tn, split, kb0, kb1;
+                unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                float acc[128];
+                plain_sums(reinterpret_cast<float *>(smem), PlainRange(e, kb0, kb1), turn, acc);
+                const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
+                const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
+                if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, 1.0f, 1.0f);
+                else store_sum(args, e.M, acc, row, col0, split, 1.0f, 1.0f);
+            }
+        }
+        for (int64_t u = wide ? e.units : cluster; u < e.units && ok; u += clusters) {
             int tm, tn, split, kb0, kb1;
             unit_of(args, e, u, tm, tn, split, kb0, kb1);
             const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-            if (wide) plain_sum(args, e, reinterpret_cast<float *>(smem), tm, tn, static_cast<int>(rank), kb0, kb1, acc);
-            for (int kb = wide ? kb1 : kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
+            for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
                 const int b = static_cast<int>(piece & 1);
                 float unscale = 1.0f;  // of a class's row in this piece
                 if (A_MN && row < e.M)
@@ -780,7 +858,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
                 if (lane == 0) mbar_arrive_remote(release[b]);
             }
             if (!ok) break;
-            const int scale = wide ? 0 : -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
+            const int scale = -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
             const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
             const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
             const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
@@ -791,11 +869,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
         if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == 0) {
+        if (wide) {
+            int turn = 0;
+            for (int64_t u = cluster; u < e.units; u += clusters) {
+                int tm, tn, split, kb0, kb1;
+                unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                plain_stages(args, e, reinterpret_cast<float *>(smem), tm, tn, static_cast<int>(rank), PlainRange(e, kb0, kb1), turn);
+            }
+        } else if (warp == 0) {
             if (lane == 0) {
                 int64_t it = 0;
                 bool ok = true;
-                for (int64_t u = first_unit; u < e.units && ok; u += clusters) {
+                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
                     int tm, tn, split, kb0, kb1;
                     unit_of(args, e, u, tm, tn, split, kb0, kb1);
                     const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
@@ -836,7 +921,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
                 constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
                 int64_t it = 0, piece = 0;
                 bool ok = true;
-                for (int64_t u = first_unit; u < e.units && ok; u += clusters) {
+                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
                     int tm, tn, split, kb0, kb1;
                     unit_of(args, e, u, tm, tn, split, kb0, kb1);
                     for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
