@@ -1217,3 +1217,64 @@ def test_two_streams_at_once(cuda):
             assert torch.equal(got_e[k], want_e[k])
             for name in want[k]:
                 assert torch.equal(got[k][name], want[k][name]), name
+
+
+def test_the_default_stream_and_another_at_once(cuda):
+    """A call on the default stream and one on a stream that does not wait for it."""
+    import torch
+
+    data = [ce_data(900, 2100, 160, s, ignored=0.1) for s in (62, 63)]
+    want = [run_ce(*d) for d in data]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    for _ in range(8):
+        got = [run_ce(*data[0])]
+        with torch.cuda.stream(stream):
+            got.append(run_ce(*data[1]))
+        got.append(run_ce(*data[0]))
+        torch.cuda.synchronize()
+        for k, g in enumerate(got):
+            for name in g:
+                assert torch.equal(g[name], want[k % 2][name]), name
+
+
+def test_a_recorded_call_follows_its_operands(cuda):
+    """What the call finds out about its operands it finds out again at every replay: rows of like
+    and of unlike size, a scale that the sample of the rows misses, rows without a loss."""
+    import torch
+
+    lib = abi.lib()
+    n, vocab, dim = 1500, 2300, 96
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 64, ignored=0.1)
+    variants = [(x, w, t)]
+    big = x.clone()
+    big[5] *= 1e13
+    variants.append((big, w, t))
+    missed = x * 1e-3
+    missed[1] *= 2e5
+    variants.append((missed, w * 0.5, t))
+    thin = w.clone()
+    thin[:, 7] *= 1e-15
+    variants.append((x, thin, torch.where(torch.arange(n, device=cuda) % 3 == 0, t, IGNORE)))
+    variants.append((x * 0.0, w, torch.full_like(t, IGNORE)))
+    want = [run_ce(xx, ww, b, tt, dloss) for xx, ww, tt in variants]
+    xs, ws, ts = x.clone(), w.clone(), t.clone()
+    torch.cuda.set_device(0)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        run_ce(xs, ws, b, ts, dloss)
+        torch.cuda.synchronize()
+        abi.check(lib.mtc_capture_begin(0, ctypes.c_void_p(stream.cuda_stream)), "capture")
+        got = run_ce(xs, ws, b, ts, dloss)
+        g = ctypes.c_void_p()
+        abi.check(lib.mtc_capture_end(1, ctypes.byref(g)), "capture end")
+    for k in (0, 1, 0, 2, 3, 1, 4, 0):
+        for to, source in zip((xs, ws, ts), variants[k]):
+            to.copy_(source)
+        torch.cuda.synchronize()
+        abi.check(lib.mtc_graph_launch(g), "replay")
+        torch.cuda.synchronize()
+        for name in got:
+            assert torch.equal(got[name], want[k][name]), (k, name)
+    abi.check_device_errors(0)
+    abi.check(lib.mtc_graph_destroy(g), "destroy")
