@@ -439,7 +439,7 @@ def embedding_grad(dout: View, tokens: View, dtable: View, scale: float = 1.0, p
 def linear_cross_entropy(x: View, weight: View, targets: View, loss: View, bias: View | None = None,
                          lse: View | None = None, ignore_target: int | None = None, stream=None,
                          prepare: bool = False):
-    """loss[n] = logsumexp(z[n]) - z[n, targets[n]] with z = x . weight^T + bias, the logits never stored."""
+    """loss[n] = logsumexp(z[n]) - z[n, targets[n]] with z = x . weight^T + bias, whose logits the caller never holds."""
     return _run("mtc_linear_cross_entropy", (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target),
                                              _ref(loss), _ref(lse), _stream(stream)), "linear_cross_entropy", prepare)
 

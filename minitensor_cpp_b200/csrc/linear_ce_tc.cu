@@ -105,9 +105,9 @@ __device__ __forceinline__ void store_pairs(__half *to, float x0, float x1, floa
 }
 
 // What the device knows of the scales of x and weight, behind the count of the live rows.
-// kWide: the pairs would not hold x and weight; kArrived counts CTAs.
-enum Known { kLargest = 1, kSampled = 3, kExponent = 5, kWide = 7, kArrived = 8 };
-static_assert(kArrived + 2 == kLiveKnown, "zeroed with the count");
+// kWide: the pairs would not hold x and weight; kRepacked: the second packing counts.
+enum Known { kLargest = 1, kSampled = 3, kExponent = 5, kWide = 7, kRepacked = 8 };
+static_assert(kRepacked + 2 == kLiveKnown, "zeroed with the count");
 
 // Whether the pairs hold a tensor.  With a scaled x off by 2^-36 at most, a row or a column is
 // held to 2^-24 of its largest element, as float32 would round that one, where an element of it
@@ -258,26 +258,19 @@ __global__ void __launch_bounds__(256) k_sample(const PackArgs a) {
     }
 }
 
-// Looks the bytes over, 16 at a time, a share of them a thread.
-__device__ __forceinline__ void judge(const Held &h, int64_t at, int64_t step, int *wide) {
-    bool bad = false;
-    auto look = [&](const unsigned char *ok, const unsigned char *some, int64_t n) {
-        for (int64_t i = at; i < n; i += step) {
-            const uint4 o = __ldcg(reinterpret_cast<const uint4 *>(ok) + i), m = __ldcg(reinterpret_cast<const uint4 *>(some) + i);
-            bad |= ((m.x & ~o.x) | (m.y & ~o.y) | (m.z & ~o.z) | (m.w & ~o.w)) != 0;
-        }
-    };
-    look(h.row_ok, h.row_some, h.rows16);
-    look(h.col_ok, h.col_some, h.cols16);
-    if (bad) atomicOr(wide, 1);
-}
-
 // Sets the bytes of those of four columns that reach `least`; most are set already.
-__device__ __forceinline__ void mark_columns(unsigned char *to, const float (&largest)[4], float least) {
-    const unsigned int has = __ldcg(reinterpret_cast<const unsigned int *>(to));
+__device__ __forceinline__ void mark_columns(unsigned char *to, float4 largest, float least) {
+    const unsigned int set = (largest.x >= least ? 1u : 0u) | (largest.y >= least ? 0x100u : 0u) |
+                             (largest.z >= least ? 0x10000u : 0u) | (largest.w >= least ? 0x1000000u : 0u);
+    const unsigned int left = set & ~__ldcg(reinterpret_cast<const unsigned int *>(to));
+    if (left == 0) return;
+    if (set == 0x01010101u) {
+        *reinterpret_cast<unsigned int *>(to) = set;
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        if (largest[k] >= least && !(has >> (8 * k) & 1)) to[k] = 1;
+        if (left >> (8 * k) & 1) to[k] = 1;
 }
 
 // Each half-warp packs one block of 64 columns of four rows in every so many: a lane four columns.
@@ -297,9 +290,9 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     const int64_t rows_out = s.live != nullptr && (rows + 63) / 64 * 64 < s.rows_out ? (rows + 63) / 64 * 64 : s.rows_out;
     const int e = AGAIN ? last_exponent(a, s.which) : first_exponent(a, s.which);
     if (AGAIN && (e == first_exponent(a, s.which) || a.known[kLargest + s.which] == 0)) {
-        judge(s.held[0], static_cast<int64_t>(block) * 256 + threadIdx.x, static_cast<int64_t>(grid) * 256, a.known + kWide);
         return;
     }
+    if (AGAIN && block == 0 && threadIdx.x == 0) a.known[kRepacked + s.which] = 1;
     const Held &held = s.held[AGAIN];
     const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
     const float enough = kHeld * power_of_two(-(e / 2)) * power_of_two(-(e - e / 2));  // of an element as it is
@@ -365,25 +358,25 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
                     if (rows_ok >> (8 * u) & 1) held.row_ok[r + u] = 1;
             }
         }
-        if (mine) {
-            mark_columns(held.col_ok + c, col, enough);
-            mark_columns(held.col_some + c, col, 1e-45f);
-        }
         largest = fmaxf(largest, fmaxf(fmaxf(col[0], col[1]), fmaxf(col[2], col[3])));
+        // of half-warps of this CTA that have the same columns the first speaks for all
+        __shared__ float4 columns[16][16];
+        const int group = threadIdx.x / 16;
+        float4 all = make_float4(col[0], col[1], col[2], col[3]);
+        if (abreast < 16) {
+            columns[group][lane] = mine ? all : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            __syncthreads();
+            for (int o = group + abreast; group < abreast && o < 16; o += abreast) {
+                const float4 x = columns[o][lane];
+                all = make_float4(fmaxf(all.x, x.x), fmaxf(all.y, x.y), fmaxf(all.z, x.z), fmaxf(all.w, x.w));
+            }
+        }
+        if (mine && group < abreast) {
+            mark_columns(held.col_ok + c, all, enough);
+            mark_columns(held.col_some + c, all, 1e-45f);
+        }
     }
-    if (!AGAIN && a.headroom != 0) {
-        keep_max(largest, a.known + kLargest + s.which);
-        return;
-    }
-    // nothing after this launch but the products: the tensor's last CTA looks it over
-    __shared__ bool last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(&a.known[kArrived + s.which], 1) == grid - 1;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    judge(held, threadIdx.x, 256, a.known + kWide);
+    if (!AGAIN && a.headroom != 0) keep_max(largest, a.known + kLargest + s.which);
 }
 
 // ---------------------------------------------------------------- products --
@@ -409,7 +402,10 @@ struct TileArgs {
     // of dx, or one a class and piece of K as the rows of dweight.
     const int *exp_a, *exp_b;
     int64_t exp_pitch;  // [pieces][exp_pitch]
-    const int *wide;    // set: float32 products of the operands themselves
+    int *wide;          // set: float32 products of the operands themselves
+    bool judges;        // whether that is so is found out in this launch, next to the products
+    Held held[2][2];    // by x and weight, and by the packing
+    const int *repacked;  // [2]
     Plain a, b;
     unsigned long long *err;
     // Logits
@@ -648,15 +644,247 @@ __device__ __forceinline__ void store_sum(const TileArgs &a, int64_t M, float (&
     else store_row(a.out + (a.out_map != nullptr ? a.out_map[a.first + row] : row) * a.out_rs + col0, acc, n, a.add);
 }
 
+// Looks the bytes over, 16 at a time, a share of them a thread.
+__device__ __forceinline__ void judge(const Held &h, int64_t at, int64_t step, int *wide) {
+    bool bad = false;
+    auto look = [&](const unsigned char *ok, const unsigned char *some, int64_t n) {
+        for (int64_t i = at; i < n; i += step) {
+            const uint4 o = __ldcg(reinterpret_cast<const uint4 *>(ok) + i), m = __ldcg(reinterpret_cast<const uint4 *>(some) + i);
+            bad |= ((m.x & ~o.x) | (m.y & ~o.y) | (m.z & ~o.z) | (m.w & ~o.w)) != 0;
+        }
+    };
+    look(h.row_ok, h.row_some, h.rows16);
+    look(h.col_ok, h.col_some, h.cols16);
+    if (bad) atomicOr(wide, 1);
+}
+
+template <bool A_MN, bool B_MN, Out MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
+    k_pair_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const TileArgs args) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    // the same aligned offset in both CTAs (same dynamic size, same static layout)
+    unsigned char *smem =
+        reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes);  // leader's: both CTAs' bytes
+    uint64_t *empty = full + kStages;    // each CTA's: the stage's MMAs are done (hi stages first, then lo)
+    uint64_t *acc_full = empty + kStages;  // [2] each CTA's: a piece is in tensor memory
+    uint64_t *acc_empty = acc_full + 2;    // [2] leader's: both epilogues have read it
+    uint64_t *drain = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int64_t cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 16);  // 8 epilogue warps x 2 CTAs
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    wait_for_previous();
+    Extent e = extent_of(args);
+    if (!args.judges && *args.wide != 0) e.units = 0;  // k_plain_products'
+
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
+        const int quadrant = warp % 4, half = (warp - 4) / 4;
+        const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
+        const int exp_b = *args.exp_b;
+        int64_t piece = 0;
+        bool ok = true;
+        for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+            int tm, tn, split, kb0, kb1;
+            unit_of(args, e, u, tm, tn, split, kb0, kb1);
+            const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+            for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
+                const int b = static_cast<int>(piece & 1);
+                float unscale = 1.0f;  // of a class's row in this piece
+                if (A_MN && row < e.M)
+                    unscale = power_of_two(-args.exp_a[static_cast<int64_t>(kb / kPieceBlocks) * args.exp_pitch + row]);
+                if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(piece >> 1) & 1u, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t at = tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16) +
+                                    static_cast<uint32_t>(b * kTileCols + half * 128);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[64];
+                    tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        acc[c * 64 + j] = A_MN ? fmaf(__uint_as_float(v[j]), unscale, acc[c * 64 + j])
+                                               : acc[c * 64 + j] + __uint_as_float(v[j]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(release[b]);
+            }
+            if (!ok) break;
+            const int scale = -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
+            const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
+            const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
+            const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
+            if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, f0, f1);
+            else store_sum(args, e.M, acc, row, col0, split, f0, f1);
+            __syncwarp();
+        }
+        if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 0) {
+            if (lane == 0) {
+                int64_t it = 0;
+                bool ok = true;
+                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                    int tm, tn, split, kb0, kb1;
+                    unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                    const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
+                    const int b0 = tn * kTileCols + static_cast<int>(rank) * 128;
+                    for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+                        for (int lo = 0; lo < 2; ++lo) {
+                            const int depth = lo ? kLoStages : kHiStages;
+                            const int s = (lo ? kHiStages : 0) + static_cast<int>(it % depth);
+                            if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / depth) & 1u) ^ 1u, abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            unsigned char *st = smem + s * kStageBytes;
+                            if (leader) mbar_expect_tx(&full[s], 2 * kStageBytes);
+                            const uint32_t fb = peer_addr(&full[s], 0);
+                            tma_load_operand(st, &map_a, fb, A_MN ? kb * kBlock : a0, A_MN ? a0 / kBlock : kb, lo);
+                            tma_load_operand(st + kOperandBytes, &map_b, fb, B_MN ? kb * kBlock : b0,
+                                             B_MN ? b0 / kBlock : kb, lo);
+                        }
+                    }
+                }
+                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+                if (leader) {  // every stage issued by the pair has landed before the cluster exits
+                    for (int lo = 0; lo < 2; ++lo) {
+                        const int depth = lo ? kLoStages : kHiStages;
+                        for (int64_t d = it > depth ? it - depth : 0; d < it; ++d) {
+                            uint64_t *bar = &full[(lo ? kHiStages : 0) + d % depth];
+                            const uint32_t round = static_cast<uint32_t>(d / depth);
+                            for (long long i = 0; i < kWaitLimit && !mbar_try_wait(bar, round & 1u); ++i) {
+                            }
+                        }
+                    }
+                }
+            }
+        } else if (warp >= 2) {
+            if (!A_MN && !B_MN && args.judges) {
+                const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x - 64, step = static_cast<int64_t>(gridDim.x) * 64;
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which)
+                    judge(args.repacked[which] ? args.held[which][1] : args.held[which][0], at, step, args.wide);
+            }
+        } else if (warp == 1) {
+            if (lane == 0 && leader) {
+                constexpr uint32_t idesc = instr_desc<A_MN, B_MN>();
+                constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
+                int64_t it = 0, piece = 0;
+                bool ok = true;
+                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
+                    int tm, tn, split, kb0, kb1;
+                    unit_of(args, e, u, tm, tn, split, kb0, kb1);
+                    for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
+                        const int n = kb1 - kb < kPieceBlocks ? kb1 - kb : kPieceBlocks;
+                        const int b = static_cast<int>(piece & 1);
+                        if (!mbar_wait(&acc_empty[b], (static_cast<uint32_t>(piece >> 1) & 1u) ^ 1u, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t d = tmem_base + static_cast<uint32_t>(b * kTileCols);
+                        for (int j = 0; j < n; ++j) {
+                            const int sh = static_cast<int>((it + j) % kHiStages);
+                            const int sl = kHiStages + static_cast<int>((it + j) % kLoStages);
+                            if (!mbar_wait(&full[sh], static_cast<uint32_t>((it + j) / kHiStages) & 1u, abort_flag) ||
+                                !mbar_wait(&full[sl], static_cast<uint32_t>((it + j) / kLoStages) & 1u, abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            const uint32_t hi = smem_u32(smem + sh * kStageBytes), lo = smem_u32(smem + sl * kStageBytes);
+                            const uint64_t ah = operand_desc<A_MN>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
+                            const uint64_t al = operand_desc<A_MN>(lo), bl = operand_desc<B_MN>(lo + kOperandBytes);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                mma_pair(d, ah + k * a_step, bl + k * b_step, idesc, j > 0 || k > 0);
+                                mma_pair(d, al + k * a_step, bh + k * b_step, idesc, 1);
+                            }
+                            umma_commit_both(&empty[sl]);
+                        }
+                        if (!ok) break;
+                        for (int j = 0; j < n; ++j) {
+                            const int sh = static_cast<int>((it + j) % kHiStages);
+                            const uint32_t hi = smem_u32(smem + sh * kStageBytes);
+                            const uint64_t ah = operand_desc<A_MN>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
+                            if (j == 0) mma_pair_scaled(d, ah, bh, idesc);
+                            else mma_pair(d, ah, bh, idesc, 1);
+#pragma unroll
+                            for (int k = 1; k < 4; ++k) mma_pair(d, ah + k * a_step, bh + k * b_step, idesc, 1);
+                            umma_commit_both(&empty[sh]);
+                        }
+                        umma_commit_both(&acc_full[b]);
+                        it += n;
+                    }
+                }
+                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+                umma_commit_pair_local(drain);  // all MMAs of the pair are done before either CTA frees tensor memory
+                for (long long i = 0; i < kWaitLimit && !mbar_try_wait(drain, 0u); ++i) {
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the leader's MMAs into this CTA's tensor memory have drained
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols));
+    }
+}
+
 // The products in float32, on the FMA units, for operands whose rows or columns are of so unlike
-// size that pairs on one scale lose the small ones.  The first four warps stage 16 columns of K at
-// a time in one of two buffers while the epilogue's eight work on the other, 8 x 16 sums a thread,
-// and hand them over, a row of 128 to a lane, by way of shared memory.  Bound by the FMAs and the
+// size that pairs on one scale lose the small ones: k_plain_products follows the logits' launch and
+// the two gradients', and returns at once where the pairs hold (2 us; as a part of the same kernel
+// it took 5 % of the tensor cores' time away).  The tiles, splits and results are the same.  The
+// first four warps stage 16 columns of K at a time in one of two buffers while eight work on the
+// other, 8 x 16 sums a thread, and make of them a row of 128 a lane by way of shared memory.  Bound by the FMAs and the
 // waits of two warps a scheduler: 4096 x 32000 x 1024 in 12.1 ms for the loss and 35.0 with dx and
 // dweight, 22 to 23 TFLOP/s, where pairs take 0.64 and 2.2 ms.
 constexpr int kPlainK = 16, kPlainPitchA = 132, kPlainPitchB = 260;
 constexpr int kPlainBuffer = kPlainK * (kPlainPitchA + kPlainPitchB);  // floats
-static_assert((2 * kPlainBuffer + 128 * kPlainPitchB) * 4 <= kStages * kStageBytes, "two buffers and the sums of a CTA");
+constexpr int kPlainSmem = (2 * kPlainBuffer + 128 * kPlainPitchB) * 4;  // two buffers and the sums of a CTA
+static_assert(kPlainSmem <= 227 * 1024, "shared memory per CTA");
 
 __device__ __forceinline__ void plain_barrier() { asm volatile("bar.sync 1, 384;" ::: "memory"); }
 
@@ -744,7 +972,7 @@ __device__ __forceinline__ void plain_sums(float *smem, PlainRange k, int &turn,
         for (int q = 0; q < 4; ++q)
             *reinterpret_cast<float4 *>(sums + (ty * 8 + r) * kPlainPitchB + tx * 4 + 64 * q) =
                 make_float4(two[r][2 * q].x, two[r][2 * q].y, two[r][2 * q + 1].x, two[r][2 * q + 1].y);
-    asm volatile("bar.sync 2, 256;" ::: "memory");  // the epilogue's warps alone
+    asm volatile("bar.sync 2, 256;" ::: "memory");  // the eight warps alone
     const float *mine = sums + (thread % 128) * kPlainPitchB + thread / 128 * 128;
 #pragma unroll
     for (int j = 0; j < 128; j += 4) {
@@ -756,232 +984,35 @@ __device__ __forceinline__ void plain_sums(float *smem, PlainRange k, int &turn,
     }
 }
 
-template <bool A_MN, bool B_MN, Out MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
-    k_pair_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const TileArgs args) {
-    extern __shared__ __align__(1024) unsigned char smem_raw[];
-    // the same aligned offset in both CTAs (same dynamic size, same static layout)
-    unsigned char *smem =
-        reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes);  // leader's: both CTAs' bytes
-    uint64_t *empty = full + kStages;    // each CTA's: the stage's MMAs are done (hi stages first, then lo)
-    uint64_t *acc_full = empty + kStages;  // [2] each CTA's: a piece is in tensor memory
-    uint64_t *acc_empty = acc_full + 2;    // [2] leader's: both epilogues have read it
-    uint64_t *drain = acc_empty + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t rank = cluster_rank();
-    const bool leader = rank == 0;
-    const int64_t cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 16);  // 8 epilogue warps x 2 CTAs
-        }
-        mbar_init(drain, 1);
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-    }
-    tc_fence_before();
-    __syncthreads();
-    cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-    wait_for_previous();
+template <Out MODE>
+__device__ __forceinline__ void plain_product(const TileArgs &args, float *smem, int &turn) {
     const Extent e = extent_of(args);
-    const bool wide = *args.wide != 0;
-
-    if (warp >= 4) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
-        const int quadrant = warp % 4, half = (warp - 4) / 4;
-        const uint32_t release[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
-        const int exp_b = *args.exp_b;
-        int64_t piece = 0;
-        bool ok = true;
-        if (wide) {  // apart from the other loop, whose registers it would take
-            int turn = 0;
-            for (int64_t u = cluster; u < e.units; u += clusters) {
-                int tm, tn, split, kb0, kb1;
-                unit_of(args, e, u, tm, tn, split, kb0, kb1);
-                float acc[128];
-                plain_sums(reinterpret_cast<float *>(smem), PlainRange(e, kb0, kb1), turn, acc);
-                const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
-                const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
-                if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, 1.0f, 1.0f);
-                else store_sum(args, e.M, acc, row, col0, split, 1.0f, 1.0f);
-            }
+    const int warp = threadIdx.x / 32, half = (warp - 4) / 4, rank = blockIdx.x % 2;
+    for (int64_t u = blockIdx.x / 2; u < e.units; u += gridDim.x / 2) {
+        int tm, tn, split, kb0, kb1;
+        unit_of(args, e, u, tm, tn, split, kb0, kb1);
+        if (warp < 4) {
+            plain_stages(args, e, smem, tm, tn, rank, PlainRange(e, kb0, kb1), turn);
+            continue;
         }
-        for (int64_t u = wide ? e.units : cluster; u < e.units && ok; u += clusters) {
-            int tm, tn, split, kb0, kb1;
-            unit_of(args, e, u, tm, tn, split, kb0, kb1);
-            const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + quadrant * 32 + lane;
-            float acc[128];
-#pragma unroll
-            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-            for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
-                const int b = static_cast<int>(piece & 1);
-                float unscale = 1.0f;  // of a class's row in this piece
-                if (A_MN && row < e.M)
-                    unscale = power_of_two(-args.exp_a[static_cast<int64_t>(kb / kPieceBlocks) * args.exp_pitch + row]);
-                if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(piece >> 1) & 1u, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t at = tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16) +
-                                    static_cast<uint32_t>(b * kTileCols + half * 128);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t v[64];
-                    tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
-#pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        acc[c * 64 + j] = A_MN ? fmaf(__uint_as_float(v[j]), unscale, acc[c * 64 + j])
-                                               : acc[c * 64 + j] + __uint_as_float(v[j]);
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_remote(release[b]);
-            }
-            if (!ok) break;
-            const int scale = -exp_b - (A_MN ? 0 : B_MN ? args.exp_a[row < e.M ? row : 0] : *args.exp_a);
-            const int most = scale < -126 ? -126 : scale > 126 ? 126 : scale;
-            const float f0 = power_of_two(most), f1 = power_of_two(scale - most);
-            const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
-            if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, f0, f1);
-            else store_sum(args, e.M, acc, row, col0, split, f0, f1);
-            __syncwarp();
-        }
-        if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (wide) {
-            int turn = 0;
-            for (int64_t u = cluster; u < e.units; u += clusters) {
-                int tm, tn, split, kb0, kb1;
-                unit_of(args, e, u, tm, tn, split, kb0, kb1);
-                plain_stages(args, e, reinterpret_cast<float *>(smem), tm, tn, static_cast<int>(rank), PlainRange(e, kb0, kb1), turn);
-            }
-        } else if (warp == 0) {
-            if (lane == 0) {
-                int64_t it = 0;
-                bool ok = true;
-                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
-                    int tm, tn, split, kb0, kb1;
-                    unit_of(args, e, u, tm, tn, split, kb0, kb1);
-                    const int a0 = tm * kTileRows + static_cast<int>(rank) * 128;
-                    const int b0 = tn * kTileCols + static_cast<int>(rank) * 128;
-                    for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
-                        for (int lo = 0; lo < 2; ++lo) {
-                            const int depth = lo ? kLoStages : kHiStages;
-                            const int s = (lo ? kHiStages : 0) + static_cast<int>(it % depth);
-                            if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / depth) & 1u) ^ 1u, abort_flag)) {
-                                ok = false;
-                                break;
-                            }
-                            unsigned char *st = smem + s * kStageBytes;
-                            if (leader) mbar_expect_tx(&full[s], 2 * kStageBytes);
-                            const uint32_t fb = peer_addr(&full[s], 0);
-                            tma_load_operand(st, &map_a, fb, A_MN ? kb * kBlock : a0, A_MN ? a0 / kBlock : kb, lo);
-                            tma_load_operand(st + kOperandBytes, &map_b, fb, B_MN ? kb * kBlock : b0,
-                                             B_MN ? b0 / kBlock : kb, lo);
-                        }
-                    }
-                }
-                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
-                if (leader) {  // every stage issued by the pair has landed before the cluster exits
-                    for (int lo = 0; lo < 2; ++lo) {
-                        const int depth = lo ? kLoStages : kHiStages;
-                        for (int64_t d = it > depth ? it - depth : 0; d < it; ++d) {
-                            uint64_t *bar = &full[(lo ? kHiStages : 0) + d % depth];
-                            const uint32_t round = static_cast<uint32_t>(d / depth);
-                            for (long long i = 0; i < kWaitLimit && !mbar_try_wait(bar, round & 1u); ++i) {
-                            }
-                        }
-                    }
-                }
-            }
-        } else if (warp == 1) {
-            if (lane == 0 && leader) {
-                constexpr uint32_t idesc = instr_desc<A_MN, B_MN>();
-                constexpr uint64_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
-                int64_t it = 0, piece = 0;
-                bool ok = true;
-                for (int64_t u = cluster; u < e.units && ok; u += clusters) {
-                    int tm, tn, split, kb0, kb1;
-                    unit_of(args, e, u, tm, tn, split, kb0, kb1);
-                    for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
-                        const int n = kb1 - kb < kPieceBlocks ? kb1 - kb : kPieceBlocks;
-                        const int b = static_cast<int>(piece & 1);
-                        if (!mbar_wait(&acc_empty[b], (static_cast<uint32_t>(piece >> 1) & 1u) ^ 1u, abort_flag)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t d = tmem_base + static_cast<uint32_t>(b * kTileCols);
-                        for (int j = 0; j < n; ++j) {
-                            const int sh = static_cast<int>((it + j) % kHiStages);
-                            const int sl = kHiStages + static_cast<int>((it + j) % kLoStages);
-                            if (!mbar_wait(&full[sh], static_cast<uint32_t>((it + j) / kHiStages) & 1u, abort_flag) ||
-                                !mbar_wait(&full[sl], static_cast<uint32_t>((it + j) / kLoStages) & 1u, abort_flag)) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                            const uint32_t hi = smem_u32(smem + sh * kStageBytes), lo = smem_u32(smem + sl * kStageBytes);
-                            const uint64_t ah = operand_desc<A_MN>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
-                            const uint64_t al = operand_desc<A_MN>(lo), bl = operand_desc<B_MN>(lo + kOperandBytes);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                mma_pair(d, ah + k * a_step, bl + k * b_step, idesc, j > 0 || k > 0);
-                                mma_pair(d, al + k * a_step, bh + k * b_step, idesc, 1);
-                            }
-                            umma_commit_both(&empty[sl]);
-                        }
-                        if (!ok) break;
-                        for (int j = 0; j < n; ++j) {
-                            const int sh = static_cast<int>((it + j) % kHiStages);
-                            const uint32_t hi = smem_u32(smem + sh * kStageBytes);
-                            const uint64_t ah = operand_desc<A_MN>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
-                            if (j == 0) mma_pair_scaled(d, ah, bh, idesc);
-                            else mma_pair(d, ah, bh, idesc, 1);
-#pragma unroll
-                            for (int k = 1; k < 4; ++k) mma_pair(d, ah + k * a_step, bh + k * b_step, idesc, 1);
-                            umma_commit_both(&empty[sh]);
-                        }
-                        umma_commit_both(&acc_full[b]);
-                        it += n;
-                    }
-                }
-                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
-                umma_commit_pair_local(drain);  // all MMAs of the pair are done before either CTA frees tensor memory
-                for (long long i = 0; i < kWaitLimit && !mbar_try_wait(drain, 0u); ++i) {
-                }
-            }
-        }
+        float acc[128];
+        plain_sums(smem, PlainRange(e, kb0, kb1), turn, acc);
+        const int64_t row = static_cast<int64_t>(tm) * kTileRows + rank * 128 + warp % 4 * 32 + threadIdx.x % 32;
+        const int64_t col0 = static_cast<int64_t>(tn) * kTileCols + half * 128;
+        if (MODE == Out::Logits) store_logits(args, e.M, acc, row, col0, tn * 2 + half, 1.0f, 1.0f);
+        else store_sum(args, e.M, acc, row, col0, split, 1.0f, 1.0f);
     }
+}
 
-    tc_fence_before();
-    __syncthreads();
-    cluster_sync_all();  // the leader's MMAs into this CTA's tensor memory have drained
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols));
-    }
+template <Out MODE>
+__global__ void __launch_bounds__(kCtaThreads, 1) k_plain_products(const __grid_constant__ TileArgs args0,
+                                                                   const __grid_constant__ TileArgs args1, int n) {
+    extern __shared__ __align__(16) float plain_smem[];
+    wait_for_previous();
+    if (*args0.wide == 0) return;
+    int turn = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) plain_product<MODE>(i == 0 ? args0 : args1, plain_smem, turn);
 }
 
 // The splits' partial results in order, into the rows of the result, whatever their layout.
@@ -1153,30 +1184,31 @@ struct GradArgs {
 };
 
 constexpr int kGradRows = kPieceBlocks * kBlock;  // rows of a CTA: a piece of dweight's K
+constexpr int kGradThreads = 512, kGradWarps = kGradThreads / 32;
 
 // z -> g'.  The two products want g on scales of their own, or the small ones among its entries
 // lose their digits next to the large ones: dx takes each row to its largest entry (rows whose
 // dloss is small, rows sure of their class), dweight each class to its largest in a piece of K
 // (classes that are improbable everywhere).  So g goes out twice, once in the place of z.
-// A CTA takes 64 columns of 256 rows, a thread four columns of 16 of the rows, in registers;
+// A CTA takes 64 columns of 256 rows, a thread four columns of 8 of the rows, in registers;
 // everything is read before anything is written.  Bound by HBM, 12 bytes a logit: 4096 x 32000
 // in 335 us (4.7 TB/s; 218 us for the 8 bytes of one g').
-__global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, 2) k_softmax_grad(const GradArgs a) {
     wait_for_previous();
     __shared__ LogSum lse[kGradRows];
     __shared__ float dloss[kGradRows];
     __shared__ int target[kGradRows], row_exp[kGradRows];
-    __shared__ float4 sums[8][16], tops[8][16];
+    __shared__ float4 sums[kGradWarps][16], tops[kGradWarps][16];
     const int64_t live = live_extent(a.live, a.first, a.rows), packed = (live + 63) / 64 * 64;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kGradRows;
     if (r0 >= packed) return;
-    constexpr int kMine = kGradRows / 16;
+    constexpr int kGroups = kGradThreads / 16, kMine = kGradRows / kGroups;
     const int group = threadIdx.x / 16, warp = threadIdx.x / 32, quad = threadIdx.x % 16;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kBlock, c = c0 + quad * 4;
     float g[kMine][4];
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-        const int64_t r = r0 + j * 16 + group;
+        const int64_t r = r0 + j * kGroups + group;
         const float4 z = r < live ? __ldcs(reinterpret_cast<const float4 *>(a.z + r * a.pitch + c))
                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         g[j][0] = z.x;
@@ -1184,7 +1216,7 @@ __global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
         g[j][2] = z.z;
         g[j][3] = z.w;
     }
-    {
+    if (threadIdx.x < kGradRows) {
         const int64_t r = r0 + threadIdx.x;
         lse[threadIdx.x] = r < live ? a.lse_live[r] : LogSum{0.0f, 0.0f};
         dloss[threadIdx.x] = r < live ? a.dloss[a.first + r] : 0.0f;
@@ -1195,7 +1227,7 @@ __global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
     float4 column = make_float4(0.0f, 0.0f, 0.0f, 0.0f), top = column;
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
-        const int at = j * 16 + group;
+        const int at = j * kGroups + group;
         const LogSum l = lse[at];
         const float d = dloss[at];
         const int hot = target[at] - static_cast<int>(c);
@@ -1233,16 +1265,16 @@ __global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
         __syncthreads();
         top = tops[0][quad];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) max(top, tops[w][quad]);
+        for (int w = 1; w < kGradWarps; ++w) max(top, tops[w][quad]);
         if (threadIdx.x < 16 && a.column_parts != nullptr) {
-            for (int w = 1; w < 8; ++w) add(column, sums[w][quad]);
+            for (int w = 1; w < kGradWarps; ++w) add(column, sums[w][quad]);
             *reinterpret_cast<float4 *>(a.column_parts + blockIdx.y * a.pitch + c) = column;
         }
     }
     if (*a.wide != 0) {
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-            const int64_t r = r0 + j * 16 + group;
+            const int64_t r = r0 + j * kGroups + group;
             if (r < live)
                 *reinterpret_cast<float4 *>(a.z + r * a.pitch + c) = make_float4(g[j][0], g[j][1], g[j][2], g[j][3]);
         }
@@ -1251,8 +1283,8 @@ __global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
     if (a.row_exp != nullptr) {
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-            const int64_t r = r0 + j * 16 + group;
-            const int e = row_exp[j * 16 + group];
+            const int64_t r = r0 + j * kGroups + group;
+            const int e = row_exp[j * kGroups + group];
             const float f0 = power_of_two(e / 2), f1 = power_of_two(e - e / 2);
             if (r < packed)
                 store_pairs(reinterpret_cast<__half *>(a.z + r * a.pitch + c0) + quad * 4, g[j][0] * f0 * f1,
@@ -1272,7 +1304,7 @@ __global__ void __launch_bounds__(256, 2) k_softmax_grad(const GradArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-            const int64_t r = r0 + j * 16 + group;
+            const int64_t r = r0 + j * kGroups + group;
             if (r < packed)
                 store_pairs(a.by_class + 2 * (r * a.pitch + c0) + quad * 4, g[j][0] * f0[0] * f1[0],
                             g[j][1] * f0[1] * f1[1], g[j][2] * f0[2] * f1[2], g[j][3] * f0[3] * f1[3]);
@@ -1325,6 +1357,14 @@ int launch_product(const CUtensorMap &a, const CUtensorMap &b, const TileArgs &a
     const int64_t pairs = units < sms / 2 ? units : sms / 2;
     return launch_dependent("linear cross entropy (tensor-core product)", k_pair_product<A_MN, B_MN, MODE>,
                             static_cast<unsigned>(2 * pairs), kCtaThreads, kSmemBytes, stream, a, b, args);
+}
+
+// The float32 products in their stead, of one or of both gradients.
+template <Out MODE>
+int launch_plain(const TileArgs *args, int n, int sms, cudaStream_t stream) {
+    MTC_CUDA_TRY(cudaFuncSetAttribute(k_plain_products<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlainSmem));
+    return launch_dependent("linear cross entropy (float32 products)", k_plain_products<MODE>,
+                            static_cast<unsigned>(sms / 2 * 2), kCtaThreads, kPlainSmem, stream, args[0], args[n - 1], n);
 }
 
 // Splits of K so that the tiles of a product fill the pairs of SMs: the fewest whose
@@ -1402,8 +1442,8 @@ int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
     const size_t split_dx = p.dx != nullptr && parts_dx ? static_cast<size_t>(splits_dx) * piece * parts_pitch * 4 : 0;
     const size_t split_dw = p.dw != nullptr && parts_dw ? static_cast<size_t>(splits_dw) * p.V * parts_pitch * 4 : 0;
     const size_t split_z = splits_z > 1 ? static_cast<size_t>(splits_z) * piece * pitch * 4 : 0;
-    const size_t split_grad = !grads ? 0 : split_dx > split_dw ? split_dx : split_dw;
-    const size_t split_bytes = padded(split_z > split_grad ? split_z : split_grad);
+    const size_t split_grad = !grads ? 0 : padded(split_dx) + padded(split_dw);
+    const size_t split_bytes = padded(split_z) > split_grad ? padded(split_z) : split_grad;
     // a byte a row and one a column of either tensor, four times: see Held
     const int64_t d_pad = d_blocks * kBlock;
     const size_t held_x = padded(static_cast<size_t>(rows_all)), held_w = padded(static_cast<size_t>(p.V));
@@ -1498,6 +1538,10 @@ int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
         t.exp_a = live.count + kExponent;
         t.exp_b = live.count + kExponent + 1;
         t.wide = live.count + kWide;
+        t.judges = first == 0;
+        std::memcpy(t.held[0], k.s[0].held, sizeof(t.held[0]));
+        std::memcpy(t.held[1], k.s[1].held, sizeof(t.held[1]));
+        t.repacked = live.count + kRepacked;
         t.a = Plain{p.x, p.x_rs, p.x_cs, live.row + first, nullptr};
         t.b = Plain{p.w, p.w_rs, p.w_cs, nullptr, nullptr};
         t.err = err;
@@ -1513,11 +1557,13 @@ int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
             t.parts = split_ws;
             t.parts_pitch = pitch;
             MTC_TRY((launch_product<false, false, Out::Sum>(x_k, w_k, t, sms, stream)));
+            MTC_TRY(launch_plain<Out::Sum>(&t, 1, sms, stream));
             const int64_t ctas = (rows * ((p.V + 127) / 128) + 7) / 8;
             MTC_TRY(launch_dependent("linear cross entropy (logits)", k_join_logits,
                                      static_cast<unsigned>(ctas < sms * 8 ? ctas : sms * 8), 256, 0, stream, t));
         } else {
             MTC_TRY((launch_product<false, false, Out::Logits>(x_k, w_k, t, sms, stream)));
+            MTC_TRY(launch_plain<Out::Logits>(&t, 1, sms, stream));
         }
         // (a last tile of 128 columns or less has no second half)
         const RowArgs ra{first, rows, live.count, static_cast<int>((p.V + 127) / 128), 2 * tiles_v, part_max, part_rest,
@@ -1529,11 +1575,14 @@ int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
                           dx ? row_exp : nullptr, dw ? class_exp : nullptr, by_class, p.db != nullptr ? columns : nullptr,
                           live.count + kWide};
         const dim3 grid(static_cast<unsigned>(v_blocks), static_cast<unsigned>((rows_up + kGradRows - 1) / kGradRows));
-        MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, 256, 0, stream, ga)));
+        MTC_TRY((launch_dependent("linear cross entropy (gradient of the logits)", k_softmax_grad, grid, kGradThreads, 0, stream, ga)));
         if (p.db != nullptr) {
             MTC_TRY((launch_dependent("linear cross entropy (bias gradient)", k_bias_grad, static_cast<unsigned>((p.V + 31) / 32), piece > 16 * kGradRows ? 1024 : 256, 0, stream, ga, p.db, p.db_s, first > 0)));
         }
+        TileArgs of[2];
+        int n = 0;
         if (dx) {
+            TileArgs &t = of[n++];
             MTC_TRY(operand_map(g_k, reinterpret_cast<const __half *>(z), rows_up, v_blocks, v_blocks, false));
             MTC_TRY(operand_map(w_mn, wp, p.V, d_blocks, d_blocks, true));
             std::memset(&t, 0, sizeof(t));
@@ -1557,12 +1606,9 @@ int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
             t.parts = parts_dx ? split_ws : nullptr;
             t.parts_pitch = parts_pitch;
             MTC_TRY((launch_product<false, true, Out::Sum>(g_k, w_mn, t, sms, stream)));
-            if (parts_dx)
-                MTC_TRY(launch_dependent("linear cross entropy (input gradient)", k_join_splits,
-                                         static_cast<unsigned>(sms * 8), 256, 0, stream, t, p.dx_cs,
-                                         vector_source(p.dx, p.dx_rs, p.dx_cs, p.D)));
         }
         if (dw) {
+            TileArgs &t = of[n++];
             MTC_TRY(operand_map(g_mn, by_class, rows_up, v_blocks, v_blocks, true));
             MTC_TRY(operand_map(x_mn, xc, rows_up, d_blocks, d_blocks, true));
             std::memset(&t, 0, sizeof(t));
@@ -1585,14 +1631,18 @@ int in_pieces(const LinearCe &p, cudaStream_t stream, int64_t most_rows) {
             t.out = p.dw;
             t.out_rs = p.dw_rs;
             t.add = first > 0;
-            t.parts = parts_dw ? split_ws : nullptr;
+            t.parts = parts_dw ? split_ws + padded(split_dx) / sizeof(float) : nullptr;
             t.parts_pitch = parts_pitch;
             MTC_TRY((launch_product<true, true, Out::Sum>(g_mn, x_mn, t, sms, stream)));
-            if (parts_dw)
-                MTC_TRY(launch_dependent("linear cross entropy (weight gradient)", k_join_splits,
-                                         static_cast<unsigned>(sms * 8), 256, 0, stream, t, p.dw_cs,
-                                         vector_source(p.dw, p.dw_rs, p.dw_cs, p.D)));
         }
+        if (n == 0) continue;
+        MTC_TRY(launch_plain<Out::Sum>(of, n, sms, stream));
+        if (dx && parts_dx)
+            MTC_TRY(launch_dependent("linear cross entropy (input gradient)", k_join_splits, static_cast<unsigned>(sms * 8),
+                                     256, 0, stream, of[0], p.dx_cs, vector_source(p.dx, p.dx_rs, p.dx_cs, p.D)));
+        if (dw && parts_dw)
+            MTC_TRY(launch_dependent("linear cross entropy (weight gradient)", k_join_splits, static_cast<unsigned>(sms * 8),
+                                     256, 0, stream, of[n - 1], p.dw_cs, vector_source(p.dw, p.dw_rs, p.dw_cs, p.D)));
     }
     return MTC_OK;
 }
