@@ -281,16 +281,30 @@ int mtc_embedding(const mtc_desc *table, const mtc_desc *tokens, float scale, in
 int mtc_embedding_grad(const mtc_desc *dout, const mtc_desc *tokens, float scale, int64_t padding_token,
                        int32_t accumulate, const mtc_desc *dtable, void *stream);
 
-/* Softmax cross entropy of a linear layer, without keeping the logits:
+/* Softmax cross entropy of a linear layer, whose logits the caller never holds:
  *   z = x . weight^T + bias,  lse[n] = log sum_v exp z[n,v],  loss[n] = lse[n] - z[n, targets[n]]
  * x [N, D], weight [V, D] (the layout of Linear), bias [V] or NULL, targets
  * Int64 [N], loss [N], lse [N] or NULL.  A row whose target is `ignore_target`
  * has loss 0 and lse 0, whatever x holds there; so does a row whose target lies
- * outside [0, V), which also sets the device error word.  Products have float32
- * accuracy (each operand as a pair of 16-bit floats, or float32 for small
- * problems).  A non-finite x makes its own row's loss NaN or infinite, a
- * non-finite weight or bias every row's.  On the tensor cores the call takes
- * 4 bytes of workspace an element of x and weight and 8 a row and 128 classes. */
+ * outside [0, V), which also sets the device error word.  A non-finite x makes
+ * its own row's loss NaN or infinite, a non-finite weight or bias every row's.
+ *
+ * Products have float32 accuracy.  Up to 16 rows or 16 classes, and in small
+ * problems, they are float32 (float64) products.  Else an operand's element is a
+ * pair of 16-bit floats: held to 2^-22 of itself or, if it is small beside them,
+ * to 2^-24 of the largest element of its row and of its column, whichever is
+ * less.  A row or a column of x or weight whose elements are all below 2^-20 of
+ * the tensor's largest cannot be held so; where there is one (zeros and rows
+ * without a loss apart), all products of the call are float32 products, which
+ * take about 20 times as long.
+ *
+ * Workspace (but for up to 16 rows or classes and small problems): 256 bytes for
+ * 64 columns of a row of x (the rows up to a multiple of 256) and of weight; 16
+ * bytes a row, 4 a class and 8 a column; of a piece of the rows, up to 2^21, 16
+ * bytes a row and 256 classes and 16 a row; and, for logits of so few tiles of
+ * 256 x 256 that they are split along the columns, up to 16 partial sums of them,
+ * 1 GiB at most.  Where the pool cannot give that, the rows go in smaller pieces,
+ * down to 256 rows (sums over the rows are then rounded in another order). */
 int mtc_linear_cross_entropy(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias, const mtc_desc *targets,
                              int64_t ignore_target, const mtc_desc *loss, const mtc_desc *lse, void *stream);
 
@@ -300,9 +314,14 @@ int mtc_linear_cross_entropy(const mtc_desc *x, const mtc_desc *weight, const mt
  * in one call (three products; the logits of a piece of the rows at a time).
  * dloss [N] may be a broadcast view.  loss, lse, dx, dweight and dbias may each
  * be NULL.  dx rows of ignored targets are zero.  dx, dweight and dbias are
- * overwritten.  The workspace also holds the logits of a piece of the rows, up
- * to 4 GiB, and partial sums of dx or dweight where these have few tiles of
- * 256 x 256, or rows without 32-byte alignment. */
+ * overwritten.  An element of g is held to 2^-22 of itself or, if it is small
+ * beside it, to 2^-50 of the largest of its row (for dx) or of its class in 256
+ * rows (for dweight).
+ * The workspace also holds the logits of a piece of the rows, 4 bytes each or,
+ * where both dx and dweight are wanted, 8: up to 4 GiB, but for 256 rows at
+ * least; 4 bytes a class and 256 rows of a piece for each of dweight and dbias;
+ * and partial sums of dx or dweight where these have few tiles of 256 x 256 (1
+ * GiB at most) or rows without 32-byte alignment. */
 int mtc_linear_cross_entropy_grad(const mtc_desc *x, const mtc_desc *weight, const mtc_desc *bias,
                                   const mtc_desc *targets, int64_t ignore_target, const mtc_desc *dloss,
                                   const mtc_desc *loss, const mtc_desc *lse, const mtc_desc *dx,

@@ -15,7 +15,7 @@
 // of their gradient stay in registers, the gradient of the many is written as it goes: 4 rows
 // against 131072 x 2048 take 566 us for the loss and all gradients, where reading W twice and
 // writing dW takes 492 us at the rate of a copy; 16 rows 1267 us, bound by the FMAs.  (The tensor
-// path takes 1264 us for 17 rows, which is where the limit of 16 comes from.)
+// path takes 1267 us for 17 rows, which is where the limit of 16 comes from.)
 #include <cfloat>
 #include <climits>
 #include <cstring>

@@ -2,9 +2,13 @@
 //
 // A float32 operand becomes a pair of 16-bit floats.  Scaled by a power of two that
 // brings the largest finite magnitude of its tensor to [2^8, 2^15), x is kept as
-//   hi = f16(x),  lo = f16((x - hi) * 2^11),   x = hi + lo * 2^-11 within 2^-22 |x|
-// for every |x| down to 2^-23 of the largest, and within 2^-45 of the largest below
-// (f16 ends at 2^-24, so an unscaled lo would end there; scaled, lo reaches 2^-35).
+//   hi = f16(x),  lo = f16((x - hi) * 2^11),   x = hi + lo * 2^-11 within 2^-22 |x| or 2^-36
+// (f16 ends at 2^-24, so an unscaled lo would end there; scaled, lo reaches 2^-35).  That
+// holds a row or a column to 2^-24 of its largest element where that is 2^-12 at least, scaled.
+// Of x and weight each row and each column is looked at while they are packed, and where one
+// is not held so, beside others 2^20 times as large, the products of the call are float32
+// products of the operands as they are (k_plain_products).  The logits' gradient, whose rows
+// and classes do differ so much, has a scale a row (dx) or a class (dweight).
 // The scale comes from a sample of the rows with 2^6 to spare, so that the packing reads
 // the tensor once; it finds the largest magnitude on its way, and where that does not fit
 // after all, a second packing with its own scale follows (k_pack<true>, which otherwise
@@ -48,9 +52,9 @@
 // 32-byte sector at a time: the 32 KB of shared memory that would make whole lines of it are
 // worth more as a stage.  Results whose rows allow no such stores go by way of a padded
 // workspace.
-// Bound by the MMAs and, in long calls, by the power limit: 4096 x 32000 x 2048 takes 1176 us
-// for the logits and 1106 and 1135 us for dx and dweight, 457 to 485 TFLOP/s of products
-// (three times that of MMAs) with the tensor pipe active in 79, 88 and 87 % of the cycles.
+// Bound by the MMAs and, in long calls, by the power limit: 4096 x 32000 x 2048 takes 1183 us
+// for the logits (1265 with a bias) and 1131 and 1153 us for dx and dweight, 454 to 475 TFLOP/s
+// of products (three times that of MMAs) with the tensor pipe active in 75, 84 and 82 % of the time.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
@@ -873,8 +877,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCtaThreads, 1)
 // it took 5 % of the tensor cores' time away).  The tiles, splits and results are the same.  The
 // first four warps stage 16 columns of K at a time in one of two buffers while eight work on the
 // other, 8 x 16 sums a thread, and make of them a row of 128 a lane by way of shared memory.  Bound by the FMAs and the
-// waits of two warps a scheduler: 4096 x 32000 x 1024 in 12.1 ms for the loss and 35.0 with dx and
-// dweight, 22 to 23 TFLOP/s, where pairs take 0.64 and 2.2 ms.
+// waits of two warps a scheduler: 4096 x 32000 x 1024 in 11.9 ms for the loss and 34.7 with dx and
+// dweight, 23 TFLOP/s, where pairs take 0.62 and 2.1 ms.
 constexpr int kPlainK = 16, kPlainPitchA = 132, kPlainPitchB = 260;
 constexpr int kPlainBuffer = kPlainK * (kPlainPitchA + kPlainPitchB);  // floats
 constexpr int kPlainSmem = (2 * kPlainBuffer + 128 * kPlainPitchB) * 4;  // two buffers and the sums of a CTA
