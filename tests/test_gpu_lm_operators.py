@@ -880,6 +880,34 @@ def test_more_rows_than_a_piece_of_the_logits_holds(cuda):
     within(got["db"], db, db_tol * longer, "db")
 
 
+def test_pieces_of_rows_of_unlike_size(cuda):
+    """The same in float32 products: a large row in the second piece.  Each chunk's bounds are its
+    own, and those of dweight and dbias grow by the ratio of the lengths of the sums."""
+    import torch
+
+    n, vocab, dim, step = 9000, 131100, 24, 1000
+    x, w, b, t, dloss = ce_data(n, vocab, dim, 40, ignored=0.1)
+    t[4000:5000] = IGNORE
+    x[6007] *= 1e13
+    t[6007] = 77
+    got = run_ce(x, w, b, t, dloss)
+    abi.check_device_errors(0)
+    dw, dw_tol, db, db_tol = (torch.zeros(s, dtype=torch.float64, device=cuda) for s in (w.shape, w.shape, b.shape, b.shape))
+    for i in range(0, n, step):
+        rows = slice(i, i + step)
+        want = {**ce_reference(x[rows], w, b, t[rows], None), **own_bounds(x[rows], w, b, t[rows], dloss[rows])}
+        for name in ("loss", "lse", "dx"):
+            within(got[name][rows], want[name][0], want[name][1] + 1e-42, f"{name} of rows {i}")
+        for total, tol, name in ((dw, dw_tol, "dw"), (db, db_tol, "db")):
+            total += want[name][0]
+            tol += want[name][1]
+    longer = (n + 16) / (step + 16)
+    within(got["dw"], dw, dw_tol * longer, "dw")
+    within(got["db"], db, db_tol * longer, "db")
+    del want
+    torch.cuda.empty_cache()
+
+
 def test_little_memory_makes_smaller_pieces(cuda):
     """Of a workspace of 1.7 GB, 1.2 can be had: the rows go in two pieces instead of one."""
     import torch
