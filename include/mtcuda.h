@@ -327,6 +327,36 @@ int mtc_linear_cross_entropy_grad(const mtc_desc *x, const mtc_desc *weight, con
                                   const mtc_desc *loss, const mtc_desc *lse, const mtc_desc *dx,
                                   const mtc_desc *dweight, const mtc_desc *dbias, void *stream);
 
+/* Log probabilities of given tokens under z = scale * logits, with the entropy of
+ * each distribution and its likeliest alternatives:
+ *   log_probs[i..] = z[i.., tokens[i..]] - lse[i..],  lse = log sum_v exp z[i.., v]
+ *   entropy[i..] = -sum_v p log p
+ *   top_tokens[i.., 0..k), top_log_probs: the k largest logits, largest first, the
+ *   lowest index first where they are equal, and their log probabilities
+ * logits [.., V] Float32, tokens Int64 and log_probs, lse, entropy Float32 of the
+ * leading shape, top_log_probs Float32 and top_tokens Int64 with an axis of k behind
+ * it, 1 <= k <= 32 and k <= V.  Every operand but the logits may be NULL; log_probs
+ * needs tokens.  0 < scale <= 2^100.
+ * A row whose token is `ignore_token` is not read: its floats are 0, its top_tokens
+ * -1; so are those of a token outside [0, V), which also sets the device error word.
+ * Logits of -inf have probability 0.  A row of nothing else has lse, log_probs and
+ * top_log_probs -inf and entropy 0.  A NaN or +inf in a row makes its floats NaN; a
+ * NaN counts as the largest logit.  Needs no workspace. */
+int mtc_token_log_probs(const mtc_desc *logits, const mtc_desc *tokens, float scale, int64_t ignore_token,
+                        const mtc_desc *log_probs, const mtc_desc *lse, const mtc_desc *entropy,
+                        const mtc_desc *top_log_probs, const mtc_desc *top_tokens, void *stream);
+
+/* The gradient of sum_i dlog_probs[i] * log_probs[i] + dentropy[i] * entropy[i]:
+ *   dlogits[i.., v] = scale * (dlog_probs * ([v = tokens] - p) - dentropy * p * (log p + entropy))
+ * dlog_probs (needs tokens) and dentropy, of the leading shape, may be broadcast views;
+ * one of them may be NULL.  dlogits is overwritten and may be the same view as the
+ * logits.  Rows that are not scored and rows of nothing but -inf get zeros, a row with
+ * NaN or +inf NaN.  The statistics are taken from the logits again, which loses
+ * nothing where p is close to 1.  Needs no workspace. */
+int mtc_token_log_probs_grad(const mtc_desc *logits, const mtc_desc *tokens, float scale, int64_t ignore_token,
+                             const mtc_desc *dlog_probs, const mtc_desc *dentropy, const mtc_desc *dlogits,
+                             void *stream);
+
 /* norm (Float32, one element) = sqrt of the sum of squares over all `n` Float32
  * tensors, summed in float64 in a fixed order. */
 int mtc_global_norm(const mtc_desc *tensors, int32_t n, const mtc_desc *norm, void *stream);

@@ -34,7 +34,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
 CU_SOURCES = ["runtime.cu", "graph.cu", "elementwise.cu", "fused.cu", "copy.cu", "random.cu", "reduce.cu", "gemm.cu",
-              "gemm_tc.cu", "embedding.cu", "linear_ce.cu", "linear_ce_few.cu", "linear_ce_tc.cu", "clip.cu", "comm.cu"]
+              "gemm_tc.cu", "embedding.cu", "linear_ce.cu", "linear_ce_few.cu", "linear_ce_tc.cu", "clip.cu", "log_probs.cu",
+              "comm.cu"]
 
 
 def _newer(target: Path, deps) -> bool:

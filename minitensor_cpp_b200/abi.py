@@ -275,6 +275,8 @@ def _declare(L):
         "mtc_embedding_grad": ([c_vp, c_vp, c_f, c_i64, c_i32, c_vp, c_vp], c_int),
         "mtc_linear_cross_entropy": ([c_vp] * 4 + [c_i64, c_vp, c_vp, c_vp], c_int),
         "mtc_linear_cross_entropy_grad": ([c_vp] * 4 + [c_i64] + [c_vp] * 7, c_int),
+        "mtc_token_log_probs": ([c_vp, c_vp, c_f, c_i64] + [c_vp] * 6, c_int),
+        "mtc_token_log_probs_grad": ([c_vp, c_vp, c_f, c_i64] + [c_vp] * 4, c_int),
         "mtc_global_norm": ([c_vp, c_i32, c_vp, c_vp], c_int),
         "mtc_clip_global_norm": ([c_vp, c_i32, c_f, c_vp, c_vp, c_vp], c_int),
         "mtc_reduce": ([c_i32, P(Desc), P(c_i64), c_i32, P(Desc), c_vp], c_int),
@@ -308,7 +310,7 @@ EXPORTED = (
     "mtc_stream_wait_event", "mtc_event_create_timed", "mtc_event_elapsed", "mtc_pool_take", "mtc_pool_take_many", "mtc_pool_protect", "mtc_capture_begin", "mtc_capture_end", "mtc_capture_fused_count", "mtc_graph_launch",
     "mtc_graph_set_constants", "mtc_graph_launches", "mtc_graph_destroy",
     "mtc_check_device_errors", "mtc_watch_device_errors", "mtc_poll_device_errors", "mtc_selftest_bounded_wait", "mtc_unary", "mtc_binary", "mtc_fused", "mtc_copy", "mtc_concat", "mtc_index_scatter",
-    "mtc_gather", "mtc_gather_scatter_add", "mtc_gather_scatter_add_into", "mtc_embedding", "mtc_embedding_grad", "mtc_linear_cross_entropy", "mtc_linear_cross_entropy_grad", "mtc_global_norm", "mtc_clip_global_norm", "mtc_reduce", "mtc_log_softmax", "mtc_matmul", "mtc_fill", "mtc_uniform",
+    "mtc_gather", "mtc_gather_scatter_add", "mtc_gather_scatter_add_into", "mtc_embedding", "mtc_embedding_grad", "mtc_linear_cross_entropy", "mtc_linear_cross_entropy_grad", "mtc_token_log_probs", "mtc_token_log_probs_grad", "mtc_global_norm", "mtc_clip_global_norm", "mtc_reduce", "mtc_log_softmax", "mtc_matmul", "mtc_fill", "mtc_uniform",
     "mtc_normal", "mtc_launch_count", "mtc_profile_enable", "mtc_profile_gemm", "mtc_gemm_path_counts", "mtc_comm_unique_id", "mtc_comm_init", "mtc_comm_allreduce_f32", "mtc_comm_allreduce_f32_async", "mtc_comm_wait", "mtc_comm_destroy",
 )
 
@@ -452,6 +454,25 @@ def linear_cross_entropy_grad(x: View, weight: View, targets: View, dloss: View,
     return _run("mtc_linear_cross_entropy_grad",
                 (_ref(x), _ref(weight), _ref(bias), _ref(targets), _token(ignore_target), _ref(dloss), _ref(loss),
                  _ref(lse), _ref(dx), _ref(dweight), _ref(dbias), _stream(stream)), "linear_cross_entropy_grad", prepare)
+
+
+def token_log_probs(logits: View, tokens: View | None = None, log_probs: View | None = None, lse: View | None = None,
+                    entropy: View | None = None, top_log_probs: View | None = None, top_tokens: View | None = None,
+                    scale: float = 1.0, ignore_token: int | None = None, stream=None, prepare: bool = False):
+    """log_probs[i..] = z[i.., tokens[i..]] - logsumexp(z[i..]) with z = scale * logits, the entropy of softmax(z)
+    and its likeliest alternatives."""
+    return _run("mtc_token_log_probs",
+                (_ref(logits), _ref(tokens), scale, _token(ignore_token), _ref(log_probs), _ref(lse), _ref(entropy),
+                 _ref(top_log_probs), _ref(top_tokens), _stream(stream)), "token_log_probs", prepare)
+
+
+def token_log_probs_grad(logits: View, dlogits: View, tokens: View | None = None, dlog_probs: View | None = None,
+                         dentropy: View | None = None, scale: float = 1.0, ignore_token: int | None = None,
+                         stream=None, prepare: bool = False):
+    """dlogits = the gradient of sum(dlog_probs * log_probs) + sum(dentropy * entropy); in place where it is logits."""
+    return _run("mtc_token_log_probs_grad",
+                (_ref(logits), _ref(tokens), scale, _token(ignore_token), _ref(dlog_probs), _ref(dentropy),
+                 _ref(dlogits), _stream(stream)), "token_log_probs_grad", prepare)
 
 
 def global_norm(tensors: Sequence[View], norm: View, stream=None, prepare: bool = False):
