@@ -370,6 +370,28 @@ int mtc_global_norm(const mtc_desc *tensors, int32_t n, const mtc_desc *norm, vo
 int mtc_clip_global_norm(const mtc_desc *tensors, int32_t n, float max_norm, const mtc_desc *outs,
                          const mtc_desc *norm, void *stream);
 
+/* Updates of weight matrices made orthogonal by Newton-Schulz products (the singular
+ * values of each are brought close to one another, its directions stay):
+ *   X = T / (|T|_F + eps), then in step k with (a, b, c) = coefficients[3 k ..]
+ *   S = X X^T,  X <- a X + (b S + c S^2) X          (on the shorter side of T)
+ * for each matrix T of `n` Float32 tensors [.., M, N]; leading axes are a batch of
+ * matrices.  `coefficients` lies in host memory; 1 <= steps <= 32; eps >= 0.
+ * Coefficients that let singular values of [0, 1] grow beyond 2^20 (b S + c S^2
+ * beyond 2^40) are refused.  A matrix of zeros stays one; a NaN or an infinity makes its whole
+ * matrix NaN.  outs[k] has tensors[k]'s shape and may be the same view (in place);
+ * other overlaps are not allowed.
+ *
+ * Products have float32 accuracy: small matrices are worked on in float32, others
+ * as pairs of 16-bit floats, which hold an element of X, S or of the polynomial to
+ * 2^-22 of itself or to 2^-49 of the largest it could be, whichever is more.
+ *
+ * Workspace (but for small matrices): 8 bytes an element and 8 for each element of S,
+ * sides padded to a multiple of 256 (of 128 where the shorter one is 128 or less),
+ * for as many matrices at a time as take 4 GiB together, one at least; where the
+ * pool cannot give that, for fewer. */
+int mtc_orthogonalize(const mtc_desc *tensors, int32_t n, const float *coefficients, int32_t steps, float eps,
+                      const mtc_desc *outs, void *stream);
+
 /* -------------------------------------------------------- reductions (A8, A9) -- */
 
 /* Reduce `in` over `axes` (normalised, distinct).  `out` is contiguous and holds the

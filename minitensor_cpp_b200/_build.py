@@ -35,7 +35,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-r
 
 CU_SOURCES = ["runtime.cu", "graph.cu", "elementwise.cu", "fused.cu", "copy.cu", "random.cu", "reduce.cu", "gemm.cu",
               "gemm_tc.cu", "embedding.cu", "linear_ce.cu", "linear_ce_few.cu", "linear_ce_tc.cu", "clip.cu", "log_probs.cu",
-              "comm.cu"]
+              "orthogonalize.cu", "orthogonalize_tc.cu", "comm.cu"]
 
 
 def _newer(target: Path, deps) -> bool:

@@ -279,6 +279,7 @@ def _declare(L):
         "mtc_token_log_probs_grad": ([c_vp, c_vp, c_f, c_i64] + [c_vp] * 4, c_int),
         "mtc_global_norm": ([c_vp, c_i32, c_vp, c_vp], c_int),
         "mtc_clip_global_norm": ([c_vp, c_i32, c_f, c_vp, c_vp, c_vp], c_int),
+        "mtc_orthogonalize": ([c_vp, c_i32, c_vp, c_i32, c_f, c_vp, c_vp], c_int),
         "mtc_reduce": ([c_i32, P(Desc), P(c_i64), c_i32, P(Desc), c_vp], c_int),
         "mtc_log_softmax": ([P(Desc), c_i64, P(Desc), c_vp], c_int),
         "mtc_matmul": ([P(Desc), P(Desc), P(Desc), c_i32, c_vp], c_int),
@@ -310,7 +311,7 @@ EXPORTED = (
     "mtc_stream_wait_event", "mtc_event_create_timed", "mtc_event_elapsed", "mtc_pool_take", "mtc_pool_take_many", "mtc_pool_protect", "mtc_capture_begin", "mtc_capture_end", "mtc_capture_fused_count", "mtc_graph_launch",
     "mtc_graph_set_constants", "mtc_graph_launches", "mtc_graph_destroy",
     "mtc_check_device_errors", "mtc_watch_device_errors", "mtc_poll_device_errors", "mtc_selftest_bounded_wait", "mtc_unary", "mtc_binary", "mtc_fused", "mtc_copy", "mtc_concat", "mtc_index_scatter",
-    "mtc_gather", "mtc_gather_scatter_add", "mtc_gather_scatter_add_into", "mtc_embedding", "mtc_embedding_grad", "mtc_linear_cross_entropy", "mtc_linear_cross_entropy_grad", "mtc_token_log_probs", "mtc_token_log_probs_grad", "mtc_global_norm", "mtc_clip_global_norm", "mtc_reduce", "mtc_log_softmax", "mtc_matmul", "mtc_fill", "mtc_uniform",
+    "mtc_gather", "mtc_gather_scatter_add", "mtc_gather_scatter_add_into", "mtc_embedding", "mtc_embedding_grad", "mtc_linear_cross_entropy", "mtc_linear_cross_entropy_grad", "mtc_token_log_probs", "mtc_token_log_probs_grad", "mtc_global_norm", "mtc_clip_global_norm", "mtc_orthogonalize", "mtc_reduce", "mtc_log_softmax", "mtc_matmul", "mtc_fill", "mtc_uniform",
     "mtc_normal", "mtc_launch_count", "mtc_profile_enable", "mtc_profile_gemm", "mtc_gemm_path_counts", "mtc_comm_unique_id", "mtc_comm_init", "mtc_comm_allreduce_f32", "mtc_comm_allreduce_f32_async", "mtc_comm_wait", "mtc_comm_destroy",
 )
 
@@ -490,6 +491,27 @@ def clip_global_norm(tensors: Sequence[View], max_norm: float, norm: View | None
     to = arr if outs is None else _packed_all(outs)
     return _run("mtc_clip_global_norm", (arr, len(tensors), max_norm, to, _ref(norm), _stream(stream)),
                 "clip_global_norm", prepare)
+
+
+# (a, b, c) of a step that takes singular values of [0.01, 1] to about [0.7, 1.2] in five
+QUINTIC = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(tensors: Sequence[View], outs: Sequence[View] | None = None,
+                  coefficients: Sequence[Sequence[float]] = (QUINTIC,) * 5, eps: float = 1e-7, stream=None,
+                  prepare: bool = False):
+    """X = T / (|T| + eps), then X <- a X + (b S + c S^2) X with S = X X^T for each (a, b, c), of every matrix T of
+    the tensors (their last two axes, on the shorter side); into `outs`, or in place."""
+    arr = _packed_all(tensors)
+    if outs is not None and len(outs) != len(tensors):
+        raise ValueError(f"{len(outs)} outputs for {len(tensors)} tensors")
+    to = arr if outs is None else _packed_all(outs)
+    flat = [float(v) for step in coefficients for v in step]
+    if len(flat) != 3 * len(coefficients):
+        raise ValueError("coefficients are not of three numbers a step")
+    table = (ctypes.c_float * max(len(flat), 1))(*flat)
+    return _run("mtc_orthogonalize", (arr, len(tensors), table, len(coefficients), eps, to, _stream(stream)),
+                "orthogonalize", prepare)
 
 
 def reduce(op: int, x: View, axes: Sequence[int], out: View, stream=None, prepare: bool = False):

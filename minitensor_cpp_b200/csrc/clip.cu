@@ -296,29 +296,6 @@ int plan_tensor(const mtc_desc &in, const mtc_desc &out, Plan &plan) {
     return MTC_OK;
 }
 
-// Outputs that share memory would be scaled twice, or by two CTAs at once.
-int need_apart(const mtc_desc *outs, int n) {
-    std::vector<std::pair<const float *, const float *>> spans;  // lowest and highest element of dense outputs
-    std::vector<const float *> lowest;
-    for (int i = 0; i < n; ++i) {
-        const mtc_desc &d = outs[i];
-        if (numel_of(d) == 0) continue;
-        const float *lo = float_at(&d), *hi = lo;
-        for (int a = 0; a < d.rank; ++a) {
-            const int64_t span = d.strides[a] * (d.shape[a] - 1);
-            if (span < 0) lo += span;
-            else hi += span;
-        }
-        lowest.push_back(lo);
-        if (hi - lo + 1 == numel_of(d)) spans.emplace_back(lo, hi);
-    }
-    std::sort(lowest.begin(), lowest.end());
-    std::sort(spans.begin(), spans.end());
-    bool ok = std::adjacent_find(lowest.begin(), lowest.end()) == lowest.end();
-    for (size_t i = 1; i < spans.size() && ok; ++i) ok = spans[i].first > spans[i - 1].second;
-    return ok ? MTC_OK : fail(MTC_ERR_INVALID_ARGUMENT, "two outputs share memory");
-}
-
 constexpr int kSmallTable = 64, kLargeTable = 1024;
 
 int pieces_of(const Dense &d) {

@@ -1,8 +1,12 @@
-// What the language-model operators (embedding.cu, linear_ce.cu, clip.cu) share:
+// What the language-model operators (embedding.cu, linear_ce.cu, log_probs.cu, clip.cu,
+// orthogonalize.cu) share:
 // workspaces for the time of a call, argument checks and device-side helpers.
 #pragma once
 
+#include <algorithm>
 #include <cstring>
+#include <utility>
+#include <vector>
 
 #include "common.cuh"
 #include "graph.cuh"
@@ -91,6 +95,29 @@ inline int need_distinct(const mtc_desc *d, const char *name) {
 }
 
 inline float *float_at(const mtc_desc *d) { return static_cast<float *>(d->data) + d->offset; }
+
+// Outputs that share memory would be written twice, in place with what the first write left.
+inline int need_apart(const mtc_desc *outs, int n) {
+    std::vector<std::pair<const float *, const float *>> spans;  // lowest and highest element of dense outputs
+    std::vector<const float *> lowest;
+    for (int i = 0; i < n; ++i) {
+        const mtc_desc &d = outs[i];
+        if (numel_of(d) == 0) continue;
+        const float *lo = float_at(&d), *hi = lo;
+        for (int a = 0; a < d.rank; ++a) {
+            const int64_t span = d.strides[a] * (d.shape[a] - 1);
+            if (span < 0) lo += span;
+            else hi += span;
+        }
+        lowest.push_back(lo);
+        if (hi - lo + 1 == numel_of(d)) spans.emplace_back(lo, hi);
+    }
+    std::sort(lowest.begin(), lowest.end());
+    std::sort(spans.begin(), spans.end());
+    bool ok = std::adjacent_find(lowest.begin(), lowest.end()) == lowest.end();
+    for (size_t i = 1; i < spans.size() && ok; ++i) ok = spans[i].first > spans[i - 1].second;
+    return ok ? MTC_OK : fail(MTC_ERR_INVALID_ARGUMENT, "two outputs share memory");
+}
 
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
