@@ -382,7 +382,7 @@ int run_small(const std::vector<Matrix> &all, const std::vector<Step> &steps, fl
 
 size_t packed_bytes(const Matrix &m) {
     const int64_t tile = tile_of(m.m), rows = pad_to(m.m, tile);
-    return static_cast<size_t>(4 * (2 * rows * pad_to(m.n, tile) + 2 * rows * rows));
+    return static_cast<size_t>(4 * (2 * rows * pad_to(m.n, tile) + 2 * rows * rows + 2 * rows));
 }
 
 constexpr size_t kGroupBytes = size_t{4} << 30;  // of packed operands at a time
@@ -410,7 +410,9 @@ int run_group(Matrix *m, int count, const std::vector<Step> &steps, float eps, c
         x.x[1] = x.x[0] + of_x;
         x.s = x.x[1] + of_x;
         x.b = x.s + of_s;
-        position = x.b + of_s;
+        x.s_diagonal = x.b + of_s;
+        x.b_diagonal = x.s_diagonal + static_cast<int>(rows / 32);
+        position = x.b_diagonal + static_cast<int>(rows / 32);
         x.part = parts;
         x.parts = static_cast<int>(std::min<int64_t>(std::min<int64_t>(mine, share), 1024));
         parts += x.parts;

@@ -18,7 +18,8 @@ struct Matrix {
     // shared memory (a row 128 bytes, its 16-byte chunks permuted as the 128-byte swizzle does).
     // Positions are counted in rows of 128 bytes.
     int x_blocks, s_blocks;  // blocks of 64 columns of X (n) and of X X^T (m)
-    int x[2], s, b;          // X before and after a step, X X^T, and b X X^T + c (X X^T)^2
+    int x[2], s, b;          // X before and after a step, S = X X^T, and B = b S + c S S
+    int s_diagonal, b_diagonal;  // float32; s and b hold zeros there
     int part, parts;         // partial sums of squares
 };
 

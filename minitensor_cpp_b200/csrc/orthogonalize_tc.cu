@@ -6,13 +6,22 @@
 // and a product three MMAs, hi.lo + lo.hi first and then hi.hi, the 2^-11 applied by the MMA
 // itself (scale-input-d) when hi.hi is added.  The tensor core truncates its accumulator at every
 // addition, so 256 values of K stay in tensor memory at most; the epilogue warps add each such
-// piece, rounded to nearest, to sums in registers.
+// piece, rounded to nearest, to sums in registers.  What truncation takes is not noise: pieces of
+// 256 lost 4 (products of both signs) to 13 (of one sign) 2^-24 of themselves, 64 2 to 3, so a
+// piece counts as 1 + 2^-23 for each 64.  (S S X of 1024 x 4096: 1.9e-6 off, with it 1.4e-7.)
+//
+// Nor is it noise that small products lose when they are added to a large one, which the
+// diagonals of S and B make of every sum as X nears orthogonality (1024 x 4096 after five steps:
+// 5.5e-6 off, with the diagonals apart 7.4e-7, in float32 3.4e-6).  So S = D + R and B = E + Q with the diagonals D and E apart, in float32, and
+// zeros in their place:
+//   S S = D^2 + D R + R D + R R,   B X = E X + Q X
+// whose first terms are the epilogues'.
 //
 // Three products a step, all from packed operands to packed operands:
-//   S = X X^T             A = X, B = X, both K-major
-//   B = b S + c S S       A = S, B = S (symmetric), both K-major; S is read again as it is
-//   X = a X + B X         A = B K-major, B = X MN-major
-// S and B are symmetric, so only tiles on and above the diagonal are computed, and their
+//   D + R = X X^T             operands X and X, both K-major
+//   E + Q = b S + c S S       operands R and R (symmetric), both K-major; R is read again as it is
+//   X = (a + E) X + Q X       operands Q, K-major, and X, MN-major
+// R and Q are symmetric, so only tiles on and above the diagonal are computed, and their
 // epilogue writes a tile and its mirror image.
 //
 // A CTA works on a tile of 128 x 128, a pair of CTAs (tcgen05.mma.cta_group::2) on one of 256 x
@@ -42,6 +51,7 @@ constexpr int kHiStages = 5, kLoStages = 2, kStages = kHiStages + kLoStages;
 constexpr int kPieceBlocks = 4;                  // blocks of K that are summed in tensor memory
 constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
 constexpr int kCtaThreads = 384;
+constexpr float kCutOff = 0x1p-23f;              // what a sum loses a block, see above
 constexpr int kEpilogueRegs = 208, kOtherRegs = 88;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
 static_assert(256 * kEpilogueRegs + 128 * kOtherRegs <= kCtaThreads * 168, "registers of the launch (168 a thread)");
@@ -56,7 +66,9 @@ struct Args {
     int units;
     int from;           // kSymmetric: S from X (0), or B from S (1); kApply: from X 0 or 1
     int last;           // kApply: to the outputs
-    float p, q;         // result = p old + q product
+    float q;            // of the sums of products
+    float p, r;         // kSymmetric: R times p + r (D_i + D_j); kApply: X times p (r + E_i)
+    float b, c, unit;   // of the diagonals: D = unit sums, E = b D + c D^2 + unit sums
     char *workspace;
     unsigned long long *err;
 };
@@ -254,15 +266,31 @@ __device__ __forceinline__ void store_pairs(char *to, const uint32_t (&w)[8]) {
 // Eight columns, from `col` on, of a warp's 32 neighbouring rows: this lane's sums of products.
 template <Product PRODUCT, int N>
 __device__ __forceinline__ void finish(const Args<N> &a, const Matrix &mt, int row, int col, bool mirror, float (&v)[8]) {
+    float *const d = reinterpret_cast<float *>(a.workspace + static_cast<int64_t>(mt.s_diagonal) * 128);
+    float *const e = reinterpret_cast<float *>(a.workspace + static_cast<int64_t>(mt.b_diagonal) * 128);
     if (PRODUCT == kSymmetric) {
+        float on = 0.0f;
+        const bool own = row >= col && row < col + 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (row == col + j) on = v[j] * a.unit;
         if (a.from == 0) {
+            if (own) d[row] = on;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] *= a.q;
         } else {
             float old[8];
             load_pairs(a.workspace + chunk_at(mt.s, mt.s_blocks, row, col), old);
+            const float4 d0 = *reinterpret_cast<const float4 *>(d + col), d1 = *reinterpret_cast<const float4 *>(d + col + 4);
+            const float dj[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w}, di = d[row];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fmaf(a.p, old[j], a.q * v[j]);
+            for (int j = 0; j < 8; ++j) v[j] = fmaf(fmaf(a.r, di + dj[j], a.p), old[j], a.q * v[j]);
+            if (own) e[row] = fmaf(fmaf(a.c, di, a.b), di, on);
+        }
+        if (own) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (row == col + j) v[j] = 0.0f;
         }
         uint32_t w[8];
         to_pairs(v, w);
@@ -284,8 +312,9 @@ __device__ __forceinline__ void finish(const Args<N> &a, const Matrix &mt, int r
     }
     float old[8];
     load_pairs(a.workspace + chunk_at(mt.x[a.from], mt.x_blocks, row, col), old);
+    const float factor = a.p * (a.r + e[row]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fmaf(a.p, old[j], a.q * v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = fmaf(factor, old[j], a.q * v[j]);
     if (!a.last) {
         uint32_t w[8];
         to_pairs(v, w);
@@ -394,6 +423,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
                     break;
                 }
                 tc_fence_after();
+                const float whole = 1.0f + (kb1 - kb < kPieceBlocks ? kb1 - kb : kPieceBlocks) * kCutOff;
                 const uint32_t at = tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16) +
                                     static_cast<uint32_t>(b * kTile + half * kColumns);
 #pragma unroll
@@ -401,7 +431,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
                     uint32_t v[64];
                     tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) acc[c * 64 + j] += __uint_as_float(v[j]);
+                    for (int j = 0; j < 64; ++j) acc[c * 64 + j] = fmaf(__uint_as_float(v[j]), whole, acc[c * 64 + j]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -676,18 +706,23 @@ int all_steps(Args<N> &args, const CUtensorMap &map, const Step *steps, int n, c
         const Step &s = steps[k];
         args.from = 0;
         args.last = k % 2;  // (which X it is)
-        args.p = 0.0f;
         args.q = static_cast<float>(two(s.s - 2 * s.x));
+        args.unit = static_cast<float>(two(-2 * s.x));
         MTC_TRY((launch_product<kSymmetric, N>(map, args, stream)));
         args.from = 1;
-        args.p = static_cast<float>(s.b * two(s.b_exp - s.s));
         args.q = static_cast<float>(s.c * two(s.b_exp - 2 * s.s));
+        args.p = static_cast<float>(s.b * two(s.b_exp - s.s));
+        args.r = static_cast<float>(s.c * two(s.b_exp - s.s));
+        args.b = s.b;
+        args.c = s.c;
+        args.unit = static_cast<float>(s.c * two(-2 * s.s));
         MTC_TRY((launch_product<kSymmetric, N>(map, args, stream)));
         const int to = k == n - 1 ? 0 : s.x_after;
         args.from = k % 2;
         args.last = k == n - 1;
-        args.p = static_cast<float>(s.a * two(to - s.x));
         args.q = static_cast<float>(two(to - s.b_exp - s.x));
+        args.p = static_cast<float>(two(to - s.x));
+        args.r = s.a;
         MTC_TRY((launch_product<kApply, N>(map, args, stream)));
     }
     return MTC_OK;
