@@ -11,21 +11,25 @@
 // what is left.  The gradient takes its statistics from the row anew instead of from the
 // caller: a log-sum-exp rounded to float32 would cost them.
 //
-// Bound by HBM: 4 bytes an element, and for the gradient 8.  Up to 1024 classes a warp holds
-// a row in its registers.  Beyond, a CTA streams it once: a thread keeps the maximum of what it
-// has seen and sums relative to it, rescaled where a batch raises the maximum.  The gradient
-// reads the row a second time, last elements first, out of L2.
+// Bound by HBM: 4 bytes an element, and for the gradient 8.  Up to 1024 classes (2048 without
+// gradient) a warp holds a row in its registers.  Beyond, a CTA streams it once: a thread keeps
+// the maximum of what it has seen and sums relative to it, rescaled where a batch raises the
+// maximum.  The gradient reads the row a second time, last elements first, out of L2.  (A cluster a
+// row, a thread's elements in registers, was slower: 2^28 logits of 131072 classes 478 us at best
+// against 500, of 16000 420 against 401, of 50003 538 against 464: its CTAs wait for one another.)
 //
 // The k likeliest (k <= 32) need no second pass over the row.  Of 32 groups of threads each has
-// a maximum, and the k-th largest of these is a bound that k threads' maxima reach; the k-th
-// largest of those threads' maxima, told apart by their index where they are equal, is the
-// next; exactly k threads reach that one, and only what these have read is looked at again.
-// What is found is ranked by counting.  Elements that crowd in a few threads overflow the
-// list and cost k passes over the row instead.
+// a maximum, and the k-th largest of these is a bound that k elements reach; of the others few
+// do.  Only what the threads whose maximum reaches it have read is looked at again, and what is
+// found is ranked by counting.  Where too many elements are equal for the list, the k-th largest
+// of those threads' maxima, told apart by their index, is the next bound; exactly k threads reach
+// that one.  Elements that crowd in a few threads overflow the list again and cost k passes over
+// the row.
 #include <climits>
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <type_traits>
 
 #include "operators.cuh"
 
@@ -33,7 +37,7 @@ namespace mtc {
 namespace {
 
 constexpr int kMostTop = 32;
-constexpr int kWarpVocab = 1024;
+constexpr int kWarps = 8;  // of a CTA that takes a row a warp
 
 enum Operand { kLogits, kTokens, kLogProbs, kLse, kEntropy, kTopLogProbs, kTopTokens, kDLogProbs, kDEntropy, kDLogits, kOperands };
 
@@ -72,6 +76,7 @@ __device__ __forceinline__ int64_t at(const RowArgs &a, Operand o, int64_t row) 
 
 // -------------------------------------------------------------- statistics --
 
+constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kFloor = -200.0f;  // exponents below it are zeros of float32, of base 2 and of base e
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -80,10 +85,30 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ float exp2_full(float x) {  // with subnormal results
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+template <int N>
+__device__ __forceinline__ float largest_of(const float (&x)[N]) {
+    float y = x[0];
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2) y = max_nan(y, x[i], x[i + 1]);
+    return N % 2 == 0 && N > 1 ? max_nan(y, x[N - 1]) : y;
 }
 
 // Floats as whole numbers that order as they do: NaN the largest, -0 as 0.
@@ -96,12 +121,12 @@ constexpr int kNothing = INT_MIN;  // below all of them
 
 __device__ __forceinline__ float from_ordered(int o) { return __int_as_float(o < 0 ? o ^ INT_MAX : o); }
 
-// With the index, the lower the larger: no two are equal.
+// With the index, the lower the larger: no two are equal, and none is 0 or ~0.
 __device__ __forceinline__ unsigned long long key_of(int o, int index) {
     return (static_cast<unsigned long long>(static_cast<unsigned int>(o) ^ 0x80000000u) << 32) |
-           (0xFFFFFFFFu - static_cast<unsigned int>(index));
+           static_cast<unsigned int>(INT_MAX - index);
 }
-__device__ __forceinline__ int key_index(unsigned long long k) { return static_cast<int>(0xFFFFFFFFu - static_cast<unsigned int>(k)); }
+__device__ __forceinline__ int key_index(unsigned long long k) { return INT_MAX - static_cast<int>(k); }
 __device__ __forceinline__ float key_value(unsigned long long k) {
     return from_ordered(static_cast<int>(static_cast<unsigned int>(k >> 32) ^ 0x80000000u));
 }
@@ -140,11 +165,33 @@ struct Stats {
         }
     }
 
+    // The same where m is at hand already, without a look for it: n + r and e alone.
+    template <int N>
+    __device__ __forceinline__ void add_all(const float (&x)[N], float scale2) {
+        float r1 = 0.0f, e1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float u = fmaxf((x[i] - m) * scale2, kFloor), y = exp2_fast(u);
+            r += y;
+            e = fmaf(y, u, e);
+            if (i + 1 < N) {
+                const float v = fmaxf((x[i + 1] - m) * scale2, kFloor), z = exp2_fast(v);
+                r1 += z;
+                e1 = fmaf(z, v, e1);
+            }
+        }
+        r += r1;
+        e += e1;
+    }
+
     // Of a warp's lanes together, the same in all.
     __device__ __forceinline__ void join_warp(float scale2) {
         bad = __any_sync(0xFFFFFFFFu, bad);
         const float top = from_ordered(__reduce_max_sync(0xFFFFFFFFu, ordered(m)));
         if (top > m) rise(top, scale2);
+        sum_warp();
+    }
+    __device__ __forceinline__ void sum_warp() {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
@@ -160,12 +207,11 @@ struct Row {
     bool bad, empty;
 
     __device__ __forceinline__ Row(const Stats &s) {
-        constexpr float ln2 = 0.69314718055994531f;
         m = s.m;
         others = s.n - 1.0f + s.r;
         total = s.n + s.r;
         log_total = log1pf(others);
-        spread = -ln2 * s.e / total;
+        spread = -kLn2 * s.e / total;
         bad = s.bad;
         empty = s.n == 0.0f;
     }
@@ -207,11 +253,15 @@ __device__ __forceinline__ void write_skipped(const RowArgs &a, int64_t row, int
     }
 }
 
-// The row's token, or -1 without tokens; false: the row is not scored.
-__device__ __forceinline__ bool token_of(const RowArgs &a, int64_t row, bool report, int &token) {
+// The row's token as it is: loaded a row ahead, so that nothing waits for it.
+__device__ __forceinline__ long long token_at(const RowArgs &a, int64_t row) {
+    return a.tokens != nullptr && row < a.rows ? a.tokens[at(a, kTokens, row)] : 0;
+}
+
+// Its index, or -1 without tokens; false: the row is not scored.
+__device__ __forceinline__ bool token_of(const RowArgs &a, long long t, bool report, int &token) {
     token = -1;
     if (a.tokens == nullptr) return true;
-    const long long t = a.tokens[at(a, kTokens, row)];
     if (t == a.ignore) return false;
     if (t < 0 || t >= a.vocab) {
         if (report) report_index(a.err, t);
@@ -221,32 +271,41 @@ __device__ __forceinline__ bool token_of(const RowArgs &a, int64_t row, bool rep
     return true;
 }
 
-// One element of the gradient.
+// The gradient of a row: -p (by_entropy u + shift) with d = u ln 2, and of the token's element
+// apart.
 struct Slope {
-    Row s;
-    float by_prob, by_entropy, scale, inverse;
-    int token;
+    float m, scale2, by_entropy, shift, inverse, by_prob, spread, others;
+    bool whole;  // else every element is `fill`
+    float fill;
 
-    __device__ __forceinline__ Slope(const RowArgs &a, int64_t row, const Row &stats, int t) : s(stats), token(t) {
-        scale = a.scale;
-        by_prob = a.dlog_probs != nullptr ? a.dlog_probs[at(a, kDLogProbs, row)] * scale : 0.0f;
-        by_entropy = a.dentropy != nullptr ? a.dentropy[at(a, kDEntropy, row)] * scale : 0.0f;
+    __device__ __forceinline__ Slope(const RowArgs &a, int64_t row, const Row &s) {
+        m = s.m;
+        asm volatile("" : "+f"(m));  // or the sums' exponents are kept for it, in memory
+        scale2 = a.scale2;
+        by_prob = a.dlog_probs != nullptr ? a.dlog_probs[at(a, kDLogProbs, row)] * a.scale : 0.0f;
+        by_entropy = a.dentropy != nullptr ? a.dentropy[at(a, kDEntropy, row)] * a.scale : 0.0f;
+        spread = s.spread;
+        shift = fmaf(by_entropy, spread, by_prob);
+        by_entropy *= kLn2;
         inverse = 1.0f / s.total;
+        others = s.others;
+        whole = !s.bad && !s.empty;
+        fill = s.bad ? __int_as_float(0x7FC00000) : 0.0f;
     }
-    __device__ __forceinline__ float operator()(float x, int v) const {
-        if (s.bad) return __int_as_float(0x7FC00000);
-        if (s.empty) return 0.0f;
-        const float d = fmaxf((x - s.m) * scale, kFloor);
-        const float p = expf(d) * inverse;
-        const float by_own = by_entropy * (d + s.spread);
-        if (v == token) return by_prob * (x == s.m ? s.others * inverse : 1.0f - p) - p * by_own;
-        return -p * (by_prob + by_own);
+    __device__ __forceinline__ float operator()(float x) const {
+        const float u = fmaxf((x - m) * scale2, kFloor);
+        return -(exp2_full(u) * inverse) * fmaf(by_entropy, u, shift);
+    }
+    __device__ __forceinline__ float of_token(float x) const {
+        const float u = fmaxf((x - m) * scale2, kFloor), p = exp2_full(u) * inverse;
+        return by_prob * (x == m ? others * inverse : 1.0f - p) - p * fmaf(by_entropy, u, shift - by_prob);
     }
 };
 
 // ------------------------------------------------------------ a warp a row --
 
-__device__ __forceinline__ int sorted_falling(int v) {
+// The k-th largest of the lanes' values.
+__device__ __forceinline__ int kth_of_warp(int v, int k) {
     const int lane = threadIdx.x % 32;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
@@ -256,7 +315,7 @@ __device__ __forceinline__ int sorted_falling(int v) {
             const bool larger = ((lane & o) == 0) == ((lane & size) == 0);
             v = larger ? max(v, w) : min(v, w);
         }
-    return v;
+    return __shfl_sync(0xFFFFFFFFu, v, k - 1);
 }
 
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
@@ -268,59 +327,113 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
 
 constexpr int kWarpList = 64;
 
-// R elements a lane, the 32 lanes side by side.
-template <int R, bool GRAD>
-__global__ void __launch_bounds__(256) k_warp_rows(const RowArgs a) {
-    __shared__ unsigned long long lists[8][kWarpList];
+// R elements a lane: the 32 lanes side by side, or in vectors of four, 32 vectors side by side.
+enum Lanes { kApart, kUnit, kVectors };
+
+template <int R, Lanes LANES, bool GRAD>
+__global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_warp_rows(const RowArgs a) {
+    __shared__ unsigned long long lists[kWarps][kWarpList];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp; row < a.rows; row += static_cast<int64_t>(gridDim.x) * 8) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    long long next = token_at(a, row);
+    for (; row < a.rows; row += step) {
+        const long long given = next;
+        next = token_at(a, row + step);
         int token;
-        if (!token_of(a, row, lane == 0, token)) {
+        if (!token_of(a, given, lane == 0, token)) {
             write_skipped(a, row, lane, 32);
             continue;
         }
         const float *src = a.logits + at(a, kLogits, row);
+        const int64_t cs = LANES != kApart ? 1 : a.cs;
+        auto index = [&](int j) { return LANES == kVectors ? 4 * (lane + 32 * (j / 4)) + j % 4 : lane + 32 * j; };
         float x[R];
+        if (LANES == kVectors) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) x[j] = lane + 32 * j < a.vocab ? src[(lane + 32 * j) * a.cs] : -INFINITY;
-        float largest = x[0];
+            for (int j = 0; j < R; j += 4) {
+                float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (index(j) < a.vocab) v = *reinterpret_cast<const float4 *>(src + index(j));
+                x[j] = v.x;
+                x[j + 1 < R ? j + 1 : j] = v.y;
+                x[j + 2 < R ? j + 2 : j] = v.z;
+                x[j + 3 < R ? j + 3 : j] = v.w;
+            }
+        } else {
 #pragma unroll
-        for (int j = 1; j < R; ++j) largest = max_nan(largest, x[j]);
-        const int mine = lane < a.vocab ? ordered(largest) : kNothing;
+            for (int j = 0; j < R; ++j) x[j] = index(j) < a.vocab ? src[index(j) * cs] : -INFINITY;
+        }
+        const float largest = largest_of(x);
+        const int mine = index(0) < a.vocab ? ordered(largest) : kNothing;
         const float top = from_ordered(__reduce_max_sync(0xFFFFFFFFu, mine));
         Stats st;
-        st.add(x, top, a.scale2);
-        if (!st.bad) {
+        if (!(top < INFINITY)) {
+            st.bad = true;
+        } else if (top > -INFINITY) {
+            // Sums with the largest logit's 1 among them, unless the others are little next to it: 4
+            // instructions an element instead of 8.
             st.m = top;
-            st.join_warp(a.scale2);
+            st.add_all(x, a.scale2);
+            st.sum_warp();
+            if (st.r < 1.0625f) {
+                st = Stats();
+                st.m = top;
+#pragma unroll 4
+                for (int v = lane; v < a.vocab; v += 32) {
+                    const float one[1] = {src[v * cs]};
+                    st.add(one, one[0], a.scale2);
+                }
+                st.sum_warp();
+            } else {
+                st.n = 1.0f;
+                st.r -= 1.0f;
+            }
         }
         const Row s(st);
         if (GRAD) {
-            const Slope slope(a, row, s, token);
+            const Slope slope(a, row, s);
             float *to = a.dlogits + at(a, kDLogits, row);
+            auto of = [&](int j) { return !slope.whole ? slope.fill : index(j) == token ? slope.of_token(x[j]) : slope(x[j]); };
+            if (LANES == kVectors && a.dcs == 1 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
 #pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (lane + 32 * j < a.vocab) to[(lane + 32 * j) * a.dcs] = slope(x[j], lane + 32 * j);
+                for (int j = 0; j < R; j += 4)
+                    if (index(j) < a.vocab)
+                        __stcs(reinterpret_cast<float4 *>(to + index(j)), make_float4(of(j), of(j + 1 < R ? j + 1 : j),
+                                                                                      of(j + 2 < R ? j + 2 : j), of(j + 3 < R ? j + 3 : j)));
+            } else {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (index(j) < a.vocab) to[index(j) * a.dcs] = of(j);
+            }
             continue;
         }
         if (lane == 0) write_row(a, row, s, token >= 0 ? src[token * a.cs] : 0.0f);
         if (a.top == 0) continue;
         // the k-th largest of the lanes' maxima: k elements reach it
-        const int bound = __shfl_sync(0xFFFFFFFFu, sorted_falling(mine), a.top - 1);
+        const float bound = from_ordered(kth_of_warp(mine, a.top));
+        using Hits = typename std::conditional<(R > 32), unsigned long long, unsigned int>::type;
         unsigned long long *list = lists[warp];
-        int found = 0;
+        Hits hits = 0;
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const int o = lane + 32 * j < a.vocab ? ordered(x[j]) : kNothing;
-            const bool hit = o >= bound && o != kNothing;
-            const unsigned int hits = __ballot_sync(0xFFFFFFFFu, hit);
-            if (hits == 0) continue;
-            const int to = found + __popc(hits & ((1u << lane) - 1));
-            if (hit && to < kWarpList) list[to] = key_of(o, lane + 32 * j);
-            found += __popc(hits);
+        for (int j = 0; j < R; ++j) hits |= static_cast<Hits>(x[j] >= bound ? 1 : 0) << j;
+        if (index(R - 1) >= a.vocab) {  // (what is no element)
+            const int n = LANES == kVectors ? 4 * ((a.vocab / 4 - lane + 31) / 32) : (a.vocab - lane + 31) / 32;
+            hits &= (static_cast<Hits>(1) << n) - 1;
         }
-        __syncwarp();
+        int found = __reduce_add_sync(0xFFFFFFFFu, R > 32 ? __popcll(hits) : __popc(hits));
+        if (found < a.top || s.bad) found = kWarpList + 1;  // NaN, or fewer lanes than k have an element
         if (found <= kWarpList) {
+            int base = 0;
+            for (;; hits &= hits - 1) {
+                const unsigned int any = __ballot_sync(0xFFFFFFFFu, hits != 0);
+                if (any == 0) break;
+                if (hits != 0) {
+                    const int v = index((R > 32 ? __ffsll(hits) : __ffs(hits)) - 1);
+                    list[base + __popc(any & ((1u << lane) - 1))] = key_of(ordered(src[v * cs]), v);
+                }
+                base += __popc(any);
+            }
+            __syncwarp();
             for (int i = lane; i < found; i += 32) {
                 const unsigned long long k = list[i];
                 int rank = 0;
@@ -335,7 +448,7 @@ __global__ void __launch_bounds__(256) k_warp_rows(const RowArgs a) {
             unsigned long long best = 0;
 #pragma unroll
             for (int j = 0; j < R; ++j) {
-                const unsigned long long k = lane + 32 * j < a.vocab ? key_of(ordered(x[j]), lane + 32 * j) : 0;
+                const unsigned long long k = index(j) < a.vocab ? key_of(ordered(x[j]), index(j)) : 0;
                 if (k < last && k > best) best = k;
             }
             last = warp_max(best);
@@ -348,6 +461,7 @@ __global__ void __launch_bounds__(256) k_warp_rows(const RowArgs a) {
 
 constexpr int kBatch = 8;      // vectors of four that a thread has in flight
 constexpr int kList = 512;
+constexpr int kThreadsOfSm = 1024;  // 64 registers each
 
 // A row in vectors of four that start on 16-byte boundaries, and up to three elements before
 // and behind them.  With gaps between the elements, a vector is four loads.
@@ -374,9 +488,22 @@ struct Source {
     __device__ __forceinline__ int tail_at() const { return head + 4 * vecs; }
 };
 
+// A thread's vectors of a batch: j, j + step, ...
+template <bool VEC>
+__device__ __forceinline__ void read_batch(const Source<VEC> &src, int j, int step, float (&x)[4 * kBatch]) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const float4 v = j + step * u < src.vecs ? src.vec(j + step * u) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        x[4 * u] = v.x;
+        x[4 * u + 1] = v.y;
+        x[4 * u + 2] = v.z;
+        x[4 * u + 3] = v.w;
+    }
+}
+
 template <int T>
 __device__ __forceinline__ void join_block(Stats &s, float scale2, float4 *parts) {
-    static_assert(T >= 64 && T <= 1024, "warps");
+    static_assert(T >= 32 && T <= 1024, "warps");
     constexpr int W = T / 32;
     s.join_warp(scale2);
     if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = make_float4(s.bad ? INFINITY : s.m, s.n, s.r, s.e);
@@ -396,11 +523,12 @@ __device__ __forceinline__ void join_block(Stats &s, float scale2, float4 *parts
     s = all;
 }
 
+template <int T>
 struct TopShared {
     int group[32];
     int found, listed;
     unsigned long long bound;
-    unsigned long long maxima[1024];
+    unsigned long long maxima[T];
     unsigned long long list[kList];
     unsigned long long warps[32];
 };
@@ -411,7 +539,7 @@ constexpr int kHead = -1, kTail = -2;
 
 template <int T, bool VEC>
 __device__ __forceinline__ void find_top(const RowArgs &a, int64_t row, const Source<VEC> &src, const Row &s, int best,
-                                         int where, TopShared &sh) {
+                                         int where, TopShared<T> &sh) {
     constexpr int G = T / 32;
     const int thread = threadIdx.x, lane = thread % 32;
     int m = best;
@@ -420,9 +548,69 @@ __device__ __forceinline__ void find_top(const RowArgs &a, int64_t row, const So
     if (thread % G == 0) sh.group[thread / G] = m;
     if (thread == 0) sh.found = sh.listed = 0;
     __syncthreads();
-    const int first = __shfl_sync(0xFFFFFFFFu, sorted_falling(sh.group[lane]), a.top - 1);
+    const int first = kth_of_warp(sh.group[lane], a.top);
+    // What the threads that reach it have read, and is as large: some 2 k elements, unless many
+    // are equal or crowd.
+    const bool reaches = best >= first;
+    auto scan = [&](bool mine, auto &&look) {
+        for (unsigned int of = __ballot_sync(0xFFFFFFFFu, mine); of != 0;) {
+            int of_thread[2];  // (T: none)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                of_thread[q] = of != 0 ? thread - lane + __ffs(of) - 1 : T;
+                of &= of - 1;
+            }
+            for (int at = T * lane; at < src.vecs; at += T * 32) {
+                float4 v[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    v[q] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (of_thread[q] < T && at + of_thread[q] < src.vecs) v[q] = src.vec(at + of_thread[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (of_thread[q] < T && at + of_thread[q] < src.vecs) look(v[q], src.head + 4 * (at + of_thread[q]), 4);
+            }
+            if (lane < 2) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int v = lane == 0 ? of_thread[q] : src.tail_at() + of_thread[q];
+                    if (of_thread[q] < (lane == 0 ? src.head : src.tail)) look(make_float4(src.one(v), 0.0f, 0.0f, 0.0f), v, 1);
+                }
+            }
+        }
+    };
+    auto list = [&](unsigned long long k) {
+        const int to = atomicAdd(&sh.listed, 1);
+        if (to < kList) sh.list[to] = k;
+    };
+    auto rank_list = [&](int n) {
+        for (int i = thread; i < n; i += T) {
+            const unsigned long long k = sh.list[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) rank += sh.list[j] > k;
+            if (rank < a.top) write_top(a, row, s, rank, k);
+        }
+    };
+    const float least = from_ordered(first);
+    if (!s.bad && least > -INFINITY) {
+        scan(reaches, [&](const float4 &v, int i, int n) {
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < n && x[k] >= least && sh.listed < kList) list(key_of(ordered(x[k]), i + k));
+        });
+        __syncthreads();
+        if (sh.listed < kList) {
+            rank_list(sh.listed);
+            return;
+        }
+        __syncthreads();
+        if (thread == 0) sh.listed = 0;
+    }
     unsigned long long mine = 0;
-    if (best >= first) {
+    if (reaches) {
         int index = where == kHead ? thread : src.tail_at() + thread;
         if (where >= 0) {
             for (int u = kBatch - 1; u >= 0; --u) {
@@ -449,34 +637,17 @@ __device__ __forceinline__ void find_top(const RowArgs &a, int64_t row, const So
     }
     __syncthreads();
     const unsigned long long bound = sh.bound;
-    auto look = [&](float x, int index) {
-        const unsigned long long k = key_of(ordered(x), index);
-        if (k < bound) return;
-        const int to = atomicAdd(&sh.listed, 1);
-        if (to < kList) sh.list[to] = k;
-    };
-    for (unsigned int of = __ballot_sync(0xFFFFFFFFu, mine >= bound); of != 0; of &= of - 1) {
-        const int other = thread - lane + __ffs(of) - 1;
-        for (int j = other + T * lane; j < src.vecs; j += T * 32) {
-            const float4 v = src.vec(j);
-            const int i = src.head + 4 * j;
-            look(v.x, i);
-            look(v.y, i + 1);
-            look(v.z, i + 2);
-            look(v.w, i + 3);
+    scan(mine >= bound, [&](const float4 &v, int i, int n) {
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned long long key = key_of(ordered(x[k]), i + k);
+            if (k < n && key >= bound) list(key);
         }
-        if (lane == 0 && other < src.head) look(src.one(other), other);
-        if (lane == 1 && other < src.tail) look(src.one(src.tail_at() + other), src.tail_at() + other);
-    }
+    });
     __syncthreads();
-    const int listed = sh.listed;
-    if (listed <= kList) {
-        for (int i = thread; i < listed; i += T) {
-            const unsigned long long k = sh.list[i];
-            int rank = 0;
-            for (int j = 0; j < listed; ++j) rank += sh.list[j] > k;
-            if (rank < a.top) write_top(a, row, s, rank, k);
-        }
+    if (sh.listed <= kList) {
+        rank_list(sh.listed);
         return;
     }
     unsigned long long last = ~0ull;
@@ -496,18 +667,21 @@ __device__ __forceinline__ void find_top(const RowArgs &a, int64_t row, const So
 }
 
 template <int T, bool VEC, bool GRAD>
-__global__ void __launch_bounds__(T) k_cta_rows(const RowArgs a) {
+__global__ void __launch_bounds__(T, kThreadsOfSm / T) k_cta_rows(const RowArgs a) {
     __shared__ float4 parts[32];
-    __shared__ TopShared sh;
+    __shared__ TopShared<T> sh;
     const int thread = threadIdx.x;
+    long long next = token_at(a, blockIdx.x);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const long long given = next;
+        next = token_at(a, row + gridDim.x);
         int token;
-        if (!token_of(a, row, thread == 0, token)) {
+        if (!token_of(a, given, thread == 0, token)) {
             write_skipped(a, row, thread, T);
             continue;
         }
         const Source<VEC> src(a, row);
-        const float x_token = !GRAD && token >= 0 ? src.one(token) : 0.0f;
+        const float x_token = token >= 0 ? src.one(token) : 0.0f;
         Stats st;
         int best = kNothing, where = 0;
         auto keep = [&](float largest, int at) {
@@ -526,18 +700,8 @@ __global__ void __launch_bounds__(T) k_cta_rows(const RowArgs a) {
         const int batches = (src.vecs + T * kBatch - 1) / (T * kBatch);
         for (int b = 0; b < batches; ++b) {
             float x[4 * kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int j = thread + T * (b * kBatch + u);
-                const float4 v = j < src.vecs ? src.vec(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                x[4 * u] = v.x;
-                x[4 * u + 1] = v.y;
-                x[4 * u + 2] = v.z;
-                x[4 * u + 3] = v.w;
-            }
-            float largest = x[0];
-#pragma unroll
-            for (int i = 1; i < 4 * kBatch; ++i) largest = max_nan(largest, x[i]);
+            read_batch(src, thread + T * kBatch * b, T, x);
+            const float largest = largest_of(x);
             if (thread + T * b * kBatch < src.vecs) keep(largest, b);
             st.add(x, largest, a.scale2);
         }
@@ -548,36 +712,47 @@ __global__ void __launch_bounds__(T) k_cta_rows(const RowArgs a) {
         }
         join_block<T>(st, a.scale2, parts);
         const Row s(st);
-        if (GRAD) {
-            const Slope slope(a, row, s, token);
-            float *to = a.dlogits + at(a, kDLogits, row);
-            const bool whole = VEC && a.dcs == 1 && ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(src.p)) & 15) == 0;
-            for (int b = batches - 1; b >= 0; --b) {
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int j = thread + T * (b * kBatch + u);
-                    if (j >= src.vecs) continue;
-                    const float4 v = src.vec(j);
-                    const int i = src.head + 4 * j;
-                    const float4 g = make_float4(slope(v.x, i), slope(v.y, i + 1), slope(v.z, i + 2), slope(v.w, i + 3));
-                    if (whole) {
-                        *reinterpret_cast<float4 *>(to + i) = g;
-                    } else {
-                        to[i * a.dcs] = g.x;
-                        to[(i + 1) * a.dcs] = g.y;
-                        to[(i + 2) * a.dcs] = g.z;
-                        to[(i + 3) * a.dcs] = g.w;
-                    }
-                }
-            }
-            if (thread < src.head) to[thread * a.dcs] = slope(src.one(thread), thread);
-            if (thread < src.tail) {
-                const int i = src.tail_at() + thread;
-                to[i * a.dcs] = slope(src.one(i), i);
-            }
-        } else {
+        if (!GRAD) {
             if (thread == 0) write_row(a, row, s, x_token);
             if (a.top > 0) find_top<T, VEC>(a, row, src, s, best, where, sh);
+            __syncthreads();
+            continue;
+        }
+        const Slope slope(a, row, s);
+        float *to = a.dlogits + at(a, kDLogits, row);
+        if (!slope.whole) {
+            for (int v = thread; v < a.vocab; v += T) to[v * a.dcs] = slope.fill;
+            __syncthreads();
+            continue;
+        }
+        const bool whole = VEC && a.dcs == 1 && ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(src.p)) & 15) == 0;
+        for (int b = batches - 1; b >= 0; --b) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int j = thread + T * (b * kBatch + u);
+                if (j >= src.vecs) continue;
+                const float4 v = src.vec(j);
+                const int i = src.head + 4 * j;
+                const float4 g = make_float4(slope(v.x), slope(v.y), slope(v.z), slope(v.w));
+                if (whole) {
+                    __stcs(reinterpret_cast<float4 *>(to + i), g);
+                } else {
+                    to[i * a.dcs] = g.x;
+                    to[(i + 1) * a.dcs] = g.y;
+                    to[(i + 2) * a.dcs] = g.z;
+                    to[(i + 3) * a.dcs] = g.w;
+                }
+            }
+        }
+        if (thread < src.head) to[thread * a.dcs] = slope(src.one(thread));
+        if (thread < src.tail) {
+            const int i = src.tail_at() + thread;
+            to[i * a.dcs] = slope(src.one(i));
+        }
+        if (token >= 0) {  // by the thread that has just written it
+            const int j = token - src.head;
+            const int owner = j < 0 ? token : token >= src.tail_at() ? token - src.tail_at() : j / 4 % T;
+            if (thread == owner) to[token * a.dcs] = slope.of_token(x_token);
         }
         __syncthreads();
     }
@@ -587,27 +762,69 @@ __global__ void __launch_bounds__(T) k_cta_rows(const RowArgs a) {
 
 template <int R, bool GRAD>
 int launch_warps(const RowArgs &a, cudaStream_t stream) {
-    const int64_t ctas = (a.rows + 7) / 8, most = static_cast<int64_t>(sm_count(current_device())) * 64;
-    k_warp_rows<R, GRAD><<<static_cast<unsigned>(ctas < most ? ctas : most), 256, 0, stream>>>(a);
+    const int64_t ctas = (a.rows + kWarps - 1) / (kWarps), most = static_cast<int64_t>(sm_count(current_device())) * 64;
+    const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
+    // (by the logits alone: the same logits give the same bits, wherever the gradient goes)
+    bool vectors = R >= 4 && a.cs == 1 && a.vocab % 4 == 0 && aligned16(a.logits);
+    for (int i = 0; i < a.rank; ++i) vectors = vectors && a.stride[kLogits][i] % 4 == 0;
+    if (vectors) k_warp_rows<R, R >= 4 ? kVectors : kUnit, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
+    else if (a.cs == 1) k_warp_rows<R, kUnit, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
+    else k_warp_rows<R, kApart, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
     return check_launch("log probabilities (warps)");
 }
 
 template <int T, bool GRAD>
 int launch_ctas(const RowArgs &a, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(a.rows < INT_MAX ? a.rows : INT_MAX);
+    const int64_t most = static_cast<int64_t>(sm_count(current_device())) * (kThreadsOfSm / T) * 8;
+    const unsigned grid = static_cast<unsigned>(std::min(a.rows, most));
     if (a.cs == 1) k_cta_rows<T, true, GRAD><<<grid, T, 0, stream>>>(a);
     else k_cta_rows<T, false, GRAD><<<grid, T, 0, stream>>>(a);
     return check_launch("log probabilities");
 }
 
-template <bool GRAD>
-int launch(const RowArgs &a, cudaStream_t stream) {
-    if (a.vocab <= 32) return launch_warps<1, GRAD>(a, stream);
-    if (a.vocab <= 128) return launch_warps<4, GRAD>(a, stream);
-    if (a.vocab <= 512) return launch_warps<16, GRAD>(a, stream);
-    if (a.vocab <= kWarpVocab) return launch_warps<32, GRAD>(a, stream);
-    if (a.vocab <= 8192) return launch_ctas<256, GRAD>(a, stream);
-    return launch_ctas<512, GRAD>(a, stream);
+// The number of threads goes by the classes alone, so that a row's results are the same to the
+// bit whatever other rows the call has.  (For few rows more would be a little faster: of 32000
+// classes one row with 20 alternatives takes 12.4 us by 512 threads and 15.4 by 256.)
+// Times of 2^28 logits, without alternatives, with 5 and with 20:
+//   1500 classes  64 elements a lane 222, 363, 463 us;  a CTA of 32 238, 432, 811
+//   3000          CTAs of 32 211, 297, 525;  of 64 223, 367, 617
+//   8000          of 64 162, 205, 310;  of 128 177, 250, 377
+//   16000         of 128 164, 193, 261;  of 256 183, 242, 326
+//   32000         of 256 164, 189, 236;  of 128 164, 193, 279;  of 512 193, 247, 305
+//   131072        of 512 162, 183, 213;  of 256 168, 193, 273
+int launch_forward(const RowArgs &a, cudaStream_t stream) {
+    if (a.vocab <= 32) return launch_warps<1, false>(a, stream);
+    if (a.vocab <= 128) return launch_warps<4, false>(a, stream);
+    if (a.vocab <= 512) return launch_warps<16, false>(a, stream);
+    if (a.vocab <= 1024) return launch_warps<32, false>(a, stream);
+    if (a.vocab <= 2048) return launch_warps<64, false>(a, stream);
+    if (a.vocab <= 4000) return launch_ctas<32, false>(a, stream);
+    if (a.vocab <= 12000) return launch_ctas<64, false>(a, stream);
+    if (a.vocab <= 24000) return launch_ctas<128, false>(a, stream);
+    if (a.vocab <= 100000) return launch_ctas<256, false>(a, stream);
+    return launch_ctas<512, false>(a, stream);
+}
+
+// Some 64 elements a thread, two batches, so that the rows at work are few enough for L2 (126 MB,
+// half of which is another die's) when they are read again.  2^28 logits:
+//   1500 classes  CTAs of 32 435 us;  64 elements a lane of a warp 561
+//   4000          of 64 396;  of 32 461
+//   8000          of 128 396;  of 64 447, of 256 439
+//   16000         of 256 401;  of 128 449, of 512 453
+//   32000         of 512 412;  of 256 453
+//   50003         of 1024 464;  of 512 471
+//   131072        of 1024 500;  of 512 545
+int launch_gradient(const RowArgs &a, cudaStream_t stream) {
+    if (a.vocab <= 32) return launch_warps<1, true>(a, stream);
+    if (a.vocab <= 128) return launch_warps<4, true>(a, stream);
+    if (a.vocab <= 512) return launch_warps<16, true>(a, stream);
+    if (a.vocab <= 1024) return launch_warps<32, true>(a, stream);
+    if (a.vocab <= 3500) return launch_ctas<32, true>(a, stream);
+    if (a.vocab <= 6000) return launch_ctas<64, true>(a, stream);
+    if (a.vocab <= 12000) return launch_ctas<128, true>(a, stream);
+    if (a.vocab <= 24000) return launch_ctas<256, true>(a, stream);
+    if (a.vocab <= 48000) return launch_ctas<512, true>(a, stream);
+    return launch_ctas<1024, true>(a, stream);
 }
 
 // One operand over the leading axes of the logits; `extra` axes follow them.
@@ -718,7 +935,7 @@ int mtc_token_log_probs(const mtc_desc *logits, const mtc_desc *tokens, float sc
     if (log_probs != nullptr && tokens == nullptr) return fail(MTC_ERR_INVALID_ARGUMENT, "log_probs without tokens");
     if (a.rows == 0) return MTC_OK;
     MTC_TRY(device_error_word(&a.err));
-    return launch<false>(a, static_cast<cudaStream_t>(stream));
+    return launch_forward(a, static_cast<cudaStream_t>(stream));
 }
 
 int mtc_token_log_probs_grad(const mtc_desc *logits, const mtc_desc *tokens, float scale, int64_t ignore_token,
@@ -740,7 +957,7 @@ int mtc_token_log_probs_grad(const mtc_desc *logits, const mtc_desc *tokens, flo
     if (dlog_probs != nullptr && tokens == nullptr) return fail(MTC_ERR_INVALID_ARGUMENT, "dlog_probs without tokens");
     if (a.rows == 0) return MTC_OK;
     MTC_TRY(device_error_word(&a.err));
-    return launch<true>(a, static_cast<cudaStream_t>(stream));
+    return launch_gradient(a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
