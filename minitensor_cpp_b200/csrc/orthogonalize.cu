@@ -175,74 +175,77 @@ __global__ void __launch_bounds__(kThreads) k_small(const __grid_constant__ Tabl
 
 // ----------------------------------------------------------------- packing --
 
-// Blocks of 128 x 64 of a matrix, by way of shared memory: read along the axis whose elements
-// lie next to each other.
-struct Block {
+// A unit is 32 rows of a block of 64 columns, eight elements a thread: read along the axis whose
+// elements lie next to each other.
+constexpr int kUnitRows = 32;
+
+struct Unit {
     int r0, c0;
 };
 
 template <class F>
-__device__ __forceinline__ void read_block(const Matrix &mt, Block at, F &&take) {
+__device__ __forceinline__ void read_unit(const Matrix &mt, Unit at, F &&take) {
     const bool along = mt.cs == 1 || mt.rs != 1;
-    float v[32];
+    const int r0 = along ? threadIdx.x / 64 : threadIdx.x % kUnitRows, c0 = along ? threadIdx.x % 64 : threadIdx.x / kUnitRows;
+    const int dr = along ? kThreads / 64 : 0, dc = along ? 0 : kThreads / kUnitRows;
+    const float *src = mt.src + (at.r0 + r0) * mt.rs + (at.c0 + c0) * mt.cs;
+    const int64_t step = dr * mt.rs + dc * mt.cs;
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const int e = i * kThreads + threadIdx.x;
-        const int r = at.r0 + (along ? e / 64 : e % 128), c = at.c0 + (along ? e % 64 : e / 128);
-        v[i] = r < mt.m && c < mt.n ? mt.src[r * mt.rs + c * mt.cs] : 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        const bool in = at.r0 + r0 + i * dr < mt.m && at.c0 + c0 + i * dc < mt.n;
+        v[i] = in ? src[i * step] : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const int e = i * kThreads + threadIdx.x;
-        take(along ? e / 64 : e % 128, along ? e % 64 : e / 128, v[i]);
-    }
+    for (int i = 0; i < 8; ++i) take(r0 + i * dr, c0 + i * dc, v[i]);
 }
 
 template <int N>
 __global__ void __launch_bounds__(kThreads) k_squares(const __grid_constant__ Table<N> table, double *partials) {
     const int k = find_matrix(table, blockIdx.x);
     const Matrix &mt = table.matrix[k];
-    const int rows = (mt.m + 127) / 128, cols = (mt.n + 63) / 64;
+    const int cols = (mt.n + 63) / 64;
+    const int64_t units = static_cast<int64_t>((mt.m + kUnitRows - 1) / kUnitRows) * cols;
     double acc = 0.0;
-    for (int64_t i = static_cast<int>(blockIdx.x) - table.first[k]; i < static_cast<int64_t>(rows) * cols; i += mt.parts) {
-        const Block at{static_cast<int>(i / cols) * 128, static_cast<int>(i % cols) * 64};
-        read_block(mt, at, [&](int, int, float v) { acc += static_cast<double>(v) * v; });
+    for (int64_t i = static_cast<int>(blockIdx.x) - table.first[k]; i < units; i += mt.parts) {
+        const Unit at{static_cast<int>(i / cols) * kUnitRows, static_cast<int>(i % cols) * 64};
+        read_unit(mt, at, [&](int, int, float v) { acc += static_cast<double>(v) * v; });
     }
     acc = block_sum(acc);
     if (threadIdx.x == 0) partials[mt.part + static_cast<int>(blockIdx.x) - table.first[k]] = acc;
 }
 
-// A unit is a block of the padded matrix.
+// Units of the padded matrix.  The factor is a float32 in [1, 2) and a power of two in two parts,
+// which neither the largest nor the smallest norms take out of float32.
 template <int N>
 __global__ void __launch_bounds__(kThreads) k_pack_matrices(const __grid_constant__ Table<N> table, const double *partials,
-                                                            float eps, float scale, char *workspace) {
-    __shared__ float tile[128 * 65];
+                                                            float eps, int scale, char *workspace) {
+    __shared__ float tile[kUnitRows * 65];
     wait_for_previous();
     const int k = find_matrix(table, blockIdx.x);
     const Matrix &mt = table.matrix[k];
     double squares = 0.0;
     for (int i = threadIdx.x; i < mt.parts; i += kThreads) squares += partials[mt.part + i];
-    const double inverse = inverse_norm(block_sum(squares), eps);
+    int e = 0;
+    const float factor = 2.0f * static_cast<float>(frexp(inverse_norm(block_sum(squares), eps), &e));
+    e += scale - 1;
+    const float f0 = exp2f(static_cast<float>(e / 2)), f1 = exp2f(static_cast<float>(e - e / 2));
     const int u = static_cast<int>(blockIdx.x) - table.first[k];
-    const Block at{u / mt.x_blocks * 128, u % mt.x_blocks * 64};
-    read_block(mt, at, [&](int r, int c, float v) { tile[r * 65 + c] = static_cast<float>(v * inverse) * scale; });
+    const Unit at{u / mt.x_blocks * kUnitRows, u % mt.x_blocks * 64};
+    read_unit(mt, at, [&](int r, int c, float v) { tile[r * 65 + c] = v * f0 * factor * f1; });
     __syncthreads();
-    const int r = threadIdx.x % 128;
+    const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 8;  // a row's eight chunks side by side
+    __half2 hi[4], lo[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = (threadIdx.x / 128 * 4 + i) * 8;
-        __half2 hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float v0 = tile[r * 65 + c + 2 * j], v1 = tile[r * 65 + c + 2 * j + 1];
-            hi[j] = __floats2half2_rn(v0, v1);
-            const float2 f = __half22float2(hi[j]);
-            lo[j] = __floats2half2_rn((v0 - f.x) * 2048.0f, (v1 - f.y) * 2048.0f);
-        }
-        char *to = workspace + chunk_at(mt.x[0], mt.x_blocks, at.r0 + r, at.c0 + c);
-        *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(hi);
-        *reinterpret_cast<uint4 *>(to + 16384) = *reinterpret_cast<const uint4 *>(lo);
+    for (int j = 0; j < 4; ++j) {
+        const float v0 = tile[r * 65 + c + 2 * j], v1 = tile[r * 65 + c + 2 * j + 1];
+        hi[j] = __floats2half2_rn(v0, v1);
+        const float2 f = __half22float2(hi[j]);
+        lo[j] = __floats2half2_rn((v0 - f.x) * 2048.0f, (v1 - f.y) * 2048.0f);
     }
+    char *to = workspace + chunk_at(mt.x[0], mt.x_blocks, at.r0 + r, at.c0 + c);
+    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(hi);
+    *reinterpret_cast<uint4 *>(to + 16384) = *reinterpret_cast<const uint4 *>(lo);
 }
 
 // ------------------------------------------------------------------- host --
@@ -392,16 +395,16 @@ int run_group(Matrix *m, int count, const std::vector<Step> &steps, float eps, c
     int64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
         bytes += packed_bytes(m[i]);
-        blocks += pad_to(m[i].m, 128) / 128 * (pad_to(m[i].n, 64) / 64);
+        blocks += pad_to(m[i].m, kUnitRows) / kUnitRows * (pad_to(m[i].n, 64) / 64);
     }
     // positions are counted in 32 bits
     if (bytes / 128 > INT_MAX) return fail(MTC_ERR_UNSUPPORTED, "a matrix of %d x %d is too large", m[0].m, m[0].n);
-    const int64_t ctas = static_cast<int64_t>(sm_count(current_device())) * 4;
+    const int64_t ctas = static_cast<int64_t>(sm_count(current_device())) * 8;
     int parts = 0, position = 0;
     for (int i = 0; i < count; ++i) {
         Matrix &x = m[i];
         const int64_t tile = tile_of(x.m), rows = pad_to(x.m, tile), cols = pad_to(x.n, tile);
-        const int64_t mine = pad_to(x.m, 128) / 128 * (pad_to(x.n, 64) / 64);
+        const int64_t mine = pad_to(x.m, kUnitRows) / kUnitRows * (pad_to(x.n, 64) / 64);
         const int64_t share = std::max<int64_t>(1, ctas * mine / blocks);
         x.x_blocks = static_cast<int>(cols / 64);
         x.s_blocks = static_cast<int>(rows / 64);
@@ -436,11 +439,12 @@ int run_group(Matrix *m, int count, const std::vector<Step> &steps, float eps, c
         MTC_TRY(check_launch("orthogonalize (norms)"));
         int64_t units = 0;
         for (int i = 0; i < count; ++i) {
-            units += pad_to(m[i].m, tile_of(m[i].m)) / 128 * m[i].x_blocks;
+            units += pad_to(m[i].m, tile_of(m[i].m)) / kUnitRows * m[i].x_blocks;
+            if (units > INT_MAX) return fail(MTC_ERR_UNSUPPORTED, "a matrix of %d x %d is too large", m[0].m, m[0].n);
             t.first[i + 1] = static_cast<int>(units);
         }
         return launch_dependent("orthogonalize (packing)", k_pack_matrices<N>, static_cast<unsigned>(units), kThreads, 0,
-                                stream, t, partials, eps, static_cast<float>(std::ldexp(1.0, steps[0].x)), packed);
+                                stream, t, partials, eps, steps[0].x, packed);
     }));
     return products(m, count, steps.data(), static_cast<int>(steps.size()), packed, bytes, stream);
 }

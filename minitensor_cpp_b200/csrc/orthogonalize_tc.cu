@@ -25,13 +25,16 @@
 // epilogue writes a tile and its mirror image.
 //
 // A CTA works on a tile of 128 x 128, a pair of CTAs (tcgen05.mma.cta_group::2) on one of 256 x
-// 256; either way a CTA stages 128 rows of A and 128 columns of B, 64 KB for 64 of K: rings of
-// five stages of hi (free at the end of a piece) and two of lo (free after its cross terms), 32
-// KB each.  Warp 0 loads (TMA: the workspace is one tensor of rows of 128 bytes), warp 1 issues,
+// 256; either way a CTA stages 128 rows of A and 128 columns of B, 64 KB for 64 of K.  A pair has
+// rings of five stages of hi (free at the end of a piece) and two of lo (free after its cross
+// terms), 32 KB each.  A single CTA keeps the cross terms in columns of their own of the tensor
+// memory, which its smaller tiles leave, and has one ring of six: its blocks take half the time,
+// and two stages of lo would not cover a load.  Warp 0 loads (TMA: the workspace is one tensor of rows of 128 bytes), warp 1 issues,
 // warps 4..11 are the epilogue, two for each quarter of the tensor memory's lanes.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -47,7 +50,8 @@ constexpr int kBlock = 64;
 constexpr int kHalfBytes = 8192;                 // 64 rows of 128 bytes: a TMA box
 constexpr int kOperandBytes = 2 * kHalfBytes;
 constexpr int kStageBytes = 2 * kOperandBytes;   // A and B, hi or lo
-constexpr int kHiStages = 5, kLoStages = 2, kStages = kHiStages + kLoStages;
+constexpr int kHiStages = 5, kLoStages = 2, kStages = kHiStages + kLoStages;  // of a pair
+constexpr int kRing = 6;                         // of a single CTA; the epilogue warps have the seventh
 constexpr int kPieceBlocks = 4;                  // blocks of K that are summed in tensor memory
 constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
 constexpr int kCtaThreads = 384;
@@ -56,7 +60,9 @@ constexpr int kEpilogueRegs = 208, kOtherRegs = 88;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
 static_assert(256 * kEpilogueRegs + 128 * kOtherRegs <= kCtaThreads * 168, "registers of the launch (168 a thread)");
 constexpr int kSumPitch = 132;                   // of a CTA's sums in shared memory, which the stages have left
-static_assert(128 * kSumPitch * 4 <= kStages * kStageBytes, "sums");
+static_assert(128 * kSumPitch * 4 <= kRing * kStageBytes, "sums");
+static_assert(kRing % 2 == 0, "hi and lo in turn");
+static_assert(8 * 4096 <= kStageBytes, "the epilogue warps' rows");
 
 enum Product { kSymmetric, kApply };
 
@@ -73,11 +79,10 @@ struct Args {
     unsigned long long *err;
 };
 
-__device__ __forceinline__ void load_half(void *dst, const CUtensorMap *map, uint64_t *bar, int row) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row)
-        : "memory");
+__device__ __forceinline__ void load_rows(void *dst, const char *src, uint64_t *bar, int bytes) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
 }
 
 __device__ __forceinline__ void load_half_pair(void *dst, const CUtensorMap *map, uint32_t leader_bar, int row) {
@@ -171,6 +176,39 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The loader and the issuer run their loops with all lanes of their warps and values that the
+// compiler can tell are the same in all, so that these stay in uniform registers, which the
+// instructions that one lane of them issues want; a lone lane's loop moves each of them there
+// first, and a block of 128 x 128 x 64 took twice the time of its MMAs.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+__device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
+}
+
+// Where a block's hi or lo is staged, and the parity of its barriers, from block to block.  (Kept:
+// a division for each costs a lone thread more than the MMAs of a block.)
+template <bool PAIR>
+struct Stages {
+    int at[2] = {0, PAIR ? kHiStages : 1};
+    uint32_t parity[2] = {0, 0};
+
+    __device__ __forceinline__ void next() {
+#pragma unroll
+        for (int lo = 0; lo < 2; ++lo) {
+            at[lo] += PAIR ? 1 : 2;
+            const int end = !PAIR ? kRing : lo ? kStages : kHiStages;
+            if (at[lo] < end) continue;
+            at[lo] = PAIR && lo ? kHiStages : lo;
+            parity[lo] ^= 1;
+        }
+    }
+};
+
 // A unit of work: a tile of one matrix.
 struct Unit {
     int matrix, tm, tn;
@@ -237,8 +275,7 @@ __device__ __forceinline__ void to_pairs(const float (&v)[8], uint32_t (&w)[8]) 
     }
 }
 
-__device__ __forceinline__ void load_pairs(const char *from, float (&v)[8]) {
-    const uint4 h = *reinterpret_cast<const uint4 *>(from), l = *reinterpret_cast<const uint4 *>(from + kOperandBytes);
+__device__ __forceinline__ void from_pairs(const uint4 &h, const uint4 &l, float (&v)[8]) {
     const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -249,8 +286,7 @@ __device__ __forceinline__ void load_pairs(const char *from, float (&v)[8]) {
     }
 }
 
-__device__ __forceinline__ void store_pairs(char *to, const uint32_t (&w)[8]) {
-    uint4 h, l;
+__device__ __forceinline__ void split_pairs(const uint32_t (&w)[8], uint4 &h, uint4 &l) {
     h.x = __byte_perm(w[0], w[1], 0x5410);
     h.y = __byte_perm(w[2], w[3], 0x5410);
     h.z = __byte_perm(w[4], w[5], 0x5410);
@@ -259,88 +295,264 @@ __device__ __forceinline__ void store_pairs(char *to, const uint32_t (&w)[8]) {
     l.y = __byte_perm(w[2], w[3], 0x7632);
     l.z = __byte_perm(w[4], w[5], 0x7632);
     l.w = __byte_perm(w[6], w[7], 0x7632);
-    *reinterpret_cast<uint4 *>(to) = h;
-    *reinterpret_cast<uint4 *>(to + kOperandBytes) = l;
 }
 
-// Eight columns, from `col` on, of a warp's 32 neighbouring rows: this lane's sums of products.
-template <Product PRODUCT, int N>
-__device__ __forceinline__ void finish(const Args<N> &a, const Matrix &mt, int row, int col, bool mirror, float (&v)[8]) {
-    float *const d = reinterpret_cast<float *>(a.workspace + static_cast<int64_t>(mt.s_diagonal) * 128);
-    float *const e = reinterpret_cast<float *>(a.workspace + static_cast<int64_t>(mt.b_diagonal) * 128);
-    if (PRODUCT == kSymmetric) {
-        float on = 0.0f;
-        const bool own = row >= col && row < col + 8;
+// Two chunks of a row that share a sector; in odd rows the swizzle has them the other way round.
+template <int N>
+__device__ __forceinline__ void load_sector(const char *from, int swapped, uint4 (&v)[N]) {
+    uint4 a, b;
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(from)
+                 : "memory");
+    v[0] = swapped ? b : a;
+    v[N - 1] = swapped ? a : b;
+}
+
+template <int N>
+__device__ __forceinline__ void store_sector(char *to, int swapped, const uint4 (&v)[N]) {
+    const uint4 a = swapped ? v[N - 1] : v[0], b = swapped ? v[0] : v[N - 1];
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(to), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+
+// What is left of `chunks` chunks of eight columns, from `col` (of whole chunks) on, of a warp's 32
+// neighbouring rows, once their sums are there.  What they are added to is asked for early: kAhead
+// chunks at a time.
+template <bool PAIR, Product PRODUCT, int N>
+struct Finish {
+    // A pair takes two chunks at a time: the 32 bytes of a sector, which the swizzle keeps together.
+    static constexpr int kStep = PAIR ? 2 : 1, kAhead = PAIR ? 0 : 4, kHeld = PAIR ? 4 : 2;
+    const Args<N> &a;
+    const Matrix &mt;
+    int row, col, chunks;
+    bool with_old, mirror;
+    const char *old;
+    char *to, *image;
+    float factor;           // kSymmetric: D of the row; kApply: p (r + E of the row)
+    float held[kHeld];      // kSymmetric: D of the columns, 32 a register
+    uint4 hi[PAIR ? 1 : kAhead][kStep], lo[PAIR ? 1 : kAhead][kStep];
+
+    __device__ __forceinline__ Finish(const Args<N> &args, const Matrix &m, int r, int c, int n, bool image_too)
+        : a(args), mt(m), row(r), col(c), chunks(n), mirror(image_too) {
+        const int lane = threadIdx.x % 32;
+        with_old = PRODUCT == kApply || a.from == 1;
+        const int blocks = PRODUCT == kApply ? mt.x_blocks : mt.s_blocks;
+        const int64_t at = static_cast<int64_t>(row / 128 * blocks + col / 64) * 256 + row % 128;
+        const int from = PRODUCT == kApply ? mt.x[a.from] : mt.s;
+        const int into = PRODUCT == kApply ? mt.x[a.from ^ 1] : a.from == 0 ? mt.s : mt.b;
+        old = a.workspace + (from + at) * 128;
+        to = a.workspace + (into + at) * 128;
+        if (PRODUCT == kSymmetric)
+            image = a.workspace + (into + static_cast<int64_t>(col / 128 * blocks + row / 64) * 256 + col % 128) * 128;
+        if (!with_old) return;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (row == col + j) on = v[j] * a.unit;
-        if (a.from == 0) {
-            if (own) d[row] = on;
+        for (int i = 0; i < kAhead; ++i) ask(i * kStep, i);
+        const float *d = reinterpret_cast<const float *>(a.workspace + static_cast<int64_t>(mt.s_diagonal) * 128);
+        if (PRODUCT == kSymmetric) {
+            factor = d[row];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= a.q;
+            for (int i = 0; i < kHeld; ++i) {  // (within the padded diagonal)
+                const int at_col = col + 32 * i + lane;
+                held[i] = at_col < mt.s_blocks * 64 ? d[at_col] : 0.0f;
+            }
         } else {
-            float old[8];
-            load_pairs(a.workspace + chunk_at(mt.s, mt.s_blocks, row, col), old);
-            const float4 d0 = *reinterpret_cast<const float4 *>(d + col), d1 = *reinterpret_cast<const float4 *>(d + col + 4);
-            const float dj[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w}, di = d[row];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fmaf(fmaf(a.r, di + dj[j], a.p), old[j], a.q * v[j]);
-            if (own) e[row] = fmaf(fmaf(a.c, di, a.b), di, on);
+            factor = a.p * (a.r + reinterpret_cast<const float *>(a.workspace + static_cast<int64_t>(mt.b_diagonal) * 128)[row]);
         }
+    }
+
+    __device__ __forceinline__ int offset(int c) const {  // of chunk c in this row
+        const int k = col / 8 % 8 + c;
+        return k / 8 * 2 * kOperandBytes + ((k ^ row) & 7) * 16;
+    }
+
+    __device__ __forceinline__ void ask(int c, int slot) {
+        if (c >= chunks) return;
+        if (PAIR) {
+            load_sector(old + (offset(c) & ~31), row & 1, hi[slot]);
+            load_sector(old + (offset(c) & ~31) + kOperandBytes, row & 1, lo[slot]);
+        } else {
+            hi[slot][0] = *reinterpret_cast<const uint4 *>(old + offset(c));
+            lo[slot][0] = *reinterpret_cast<const uint4 *>(old + offset(c) + kOperandBytes);
+        }
+    }
+
+    // Sums and old values of chunk c to what comes of them.
+    __device__ __forceinline__ void combine(int c, const float (&x)[8], float (&v)[8]) {
+        if (PRODUCT == kApply) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = fmaf(factor, x[j], a.q * v[j]);
+            return;
+        }
+        const int first = col + 8 * c;
+        const bool own = row >= first && row < first + 8;
+        float on = 0.0f;
         if (own) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (row == col + j) v[j] = 0.0f;
+                if (row == first + j) on = v[j] * a.unit;
         }
-        uint32_t w[8];
-        to_pairs(v, w);
-        const int to = a.from == 0 ? mt.s : mt.b;
-        store_pairs(a.workspace + chunk_at(to, mt.s_blocks, row, col), w);
-        if (!mirror) return;
-        // Rows become columns: of two neighbouring lanes and columns each lane gets two neighbours
-        // of one row of the image.
+        if (!with_old) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= a.q;
+        } else {
+            float d = held[0];
+#pragma unroll
+            for (int i = 1; i < kHeld; ++i)
+                if (c / 4 == i) d = held[i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float dj = __shfl_sync(0xFFFFFFFFu, d, c % 4 * 8 + j);
+                v[j] = fmaf(fmaf(a.r, factor + dj, a.p), x[j], a.q * v[j]);
+            }
+        }
+        if (own) {
+            const int diagonal = a.from == 0 ? mt.s_diagonal : mt.b_diagonal;
+            reinterpret_cast<float *>(a.workspace + static_cast<int64_t>(diagonal) * 128)[row] =
+                with_old ? fmaf(fmaf(a.c, factor, a.b), factor, on) : on;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (row == first + j) v[j] = 0.0f;
+        }
+    }
+
+    // Rows become columns: of two neighbouring lanes and columns each lane gets two neighbours of
+    // one row of the image.
+    __device__ __forceinline__ void store_image(int c, const uint32_t (&w)[8]) {
         const int odd = row & 1;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[j] : w[j + 1], 1);
             const uint32_t left = odd ? other : w[j], right = odd ? w[j + 1] : other;
-            char *at = a.workspace + chunk_at(to, mt.s_blocks, col + j + odd, row & ~7) + (row & 6) * 2;
+            const int r = 8 * c + j + odd;  // from the image's first row on, a multiple of 8 in its block
+            char *at = image + r * 128 + (((row / 8) ^ r) & 7) * 16 + (row & 6) * 2;
             *reinterpret_cast<uint32_t *>(at) = __byte_perm(left, right, 0x5410);
             *reinterpret_cast<uint32_t *>(at + kOperandBytes) = __byte_perm(left, right, 0x7632);
         }
-        return;
     }
-    float old[8];
-    load_pairs(a.workspace + chunk_at(mt.x[a.from], mt.x_blocks, row, col), old);
-    const float factor = a.p * (a.r + e[row]);
+
+    __device__ __forceinline__ void operator()(int c, float (&v)[kStep][8]) {
+        uint4 h[kStep], l[kStep];
+        if (with_old) {
+            if (kAhead == 0) ask(c, 0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fmaf(factor, old[j], a.q * v[j]);
-    if (!a.last) {
-        uint32_t w[8];
-        to_pairs(v, w);
-        store_pairs(a.workspace + chunk_at(mt.x[a.from ^ 1], mt.x_blocks, row, col), w);
-        return;
-    }
-    if (row >= mt.m || col >= mt.n) return;
-    float *to = mt.dst + row * mt.out_rs + col * mt.out_cs;
-    if (mt.out_cs == 1 && col + 8 <= mt.n && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
-        reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        return;
-    }
+            for (int i = 0; i < kStep; ++i) {
+                h[i] = hi[0][i];
+                l[i] = lo[0][i];
+            }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (col + j < mt.n) to[j * mt.out_cs] = v[j];
+            for (int i = 0; i + 1 < kAhead; ++i)
+#pragma unroll
+                for (int k = 0; k < kStep; ++k) {
+                    hi[i][k] = hi[i + 1][k];
+                    lo[i][k] = lo[i + 1][k];
+                }
+            if (kAhead > 0) ask(c + kAhead * kStep, kAhead > 0 ? kAhead - 1 : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+            float x[8];
+            if (with_old) from_pairs(h[i], l[i], x);
+            combine(c + i, x, v[i]);
+        }
+        if (PRODUCT == kApply && a.last) {
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) store_output(col + 8 * (c + i), v[i]);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+            uint32_t w[8];
+            to_pairs(v[i], w);
+            split_pairs(w, h[i], l[i]);
+            if (PRODUCT == kSymmetric && mirror) store_image(c + i, w);
+        }
+        if (PAIR) {
+            store_sector(to + (offset(c) & ~31), row & 1, h);
+            store_sector(to + (offset(c) & ~31) + kOperandBytes, row & 1, l);
+        } else {
+            *reinterpret_cast<uint4 *>(to + offset(c)) = h[0];
+            *reinterpret_cast<uint4 *>(to + offset(c) + kOperandBytes) = l[0];
+        }
+    }
+
+    __device__ __forceinline__ void store_output(int first, const float (&v)[8]) const {
+        if (row >= mt.m || first >= mt.n) return;
+        float *out = mt.dst + row * mt.out_rs + first * mt.out_cs;
+        if (mt.out_cs == 1 && first + 8 <= mt.n && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+            reinterpret_cast<float4 *>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (first + j < mt.n) out[j * mt.out_cs] = v[j];
+    }
+};
+
+// A warp's 32 rows of a block of 64 columns, which are 4 KB in a row of the workspace, hi or lo, by
+// way of its 4 KB of shared memory: a lane reads and writes chunks of one row, but 16 bytes of each
+// of 32 rows at a time are 32 times the work of 512 bytes for the load and store units (a tile of
+// 128 x 128 read and written so took 5.1 us, which is most of a small product).
+__device__ __forceinline__ void rows_to_lanes(const char *from, char *buffer, uint4 (&v)[8]) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4 *>(from + k * 512 + lane * 16);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4 *>(buffer + k * 512 + lane * 16) = v[k];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4 *>(buffer + lane * 128 + ((k ^ lane) & 7) * 16);
 }
 
-// Without PAIR, the CTAs of a cluster share the K of one tile and add their sums by way of their
-// shared memory, each an equal share of the columns, in the order of the CTAs.
+__device__ __forceinline__ void lanes_to_rows(const uint4 (&v)[8], char *buffer, char *to) {
+    const int lane = threadIdx.x % 32;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4 *>(buffer + lane * 128 + ((k ^ lane) & 7) * 16) = v[k];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<uint4 *>(to + k * 512 + lane * 16) = *reinterpret_cast<const uint4 *>(buffer + k * 512 + lane * 16);
+}
+
+// The same for 32 of the outputs' columns, next to one another.
+__device__ __forceinline__ void lanes_to_output(const float *v, char *buffer, const Matrix &mt, int row0, int col) {
+    const int lane = threadIdx.x % 32;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<float4 *>(buffer + lane * 128 + ((k ^ lane) & 7) * 16) =
+            make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int r = 4 * k + lane / 8, c = col + lane % 8 * 4;
+        const float4 x = *reinterpret_cast<const float4 *>(buffer + r * 128 + ((lane ^ r) & 7) * 16);
+        if (row0 + r >= mt.m) continue;
+        float *out = mt.dst + (row0 + r) * mt.out_rs + c;
+        if (c + 4 <= mt.n && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+            *reinterpret_cast<float4 *>(out) = x;
+        } else {
+            if (c < mt.n) out[0] = x.x;
+            if (c + 1 < mt.n) out[1] = x.y;
+            if (c + 2 < mt.n) out[2] = x.z;
+            if (c + 3 < mt.n) out[3] = x.w;
+        }
+    }
+}
+
+// Without PAIR, the CTAs of a cluster share the K of one tile, a cluster a tile, and add their sums
+// by way of their shared memory, each an equal share of the columns, in the order of the CTAs.
 template <bool PAIR, Product PRODUCT, int N>
 __global__ void __launch_bounds__(kCtaThreads, 1)
     k_step_product(const __grid_constant__ CUtensorMap map, const __grid_constant__ Args<N> args) {
     constexpr bool B_MN = PRODUCT == kApply;
     constexpr int kTile = PAIR ? 256 : 128, kColumns = kTile / 2;  // of an epilogue thread
-    constexpr uint32_t kTmemCols = 2 * kTile;
+    constexpr uint32_t kTmemCols = 512;
+    constexpr int kSums = PAIR ? kTile : 2 * kTile;  // columns of a piece in tensor memory
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // the same aligned offset in all CTAs of a cluster (same dynamic size, same static layout)
     unsigned char *smem =
@@ -353,7 +565,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x / 32), 0), lane = threadIdx.x % 32;
     uint32_t cluster_size;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(cluster_size));
     const int rank = static_cast<int>(cluster_rank());
@@ -362,7 +574,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     const int pair_rank = PAIR ? rank : 0;
     const bool leader = pair_rank == 0;
 
-    if (threadIdx.x == 0) {
+    if (PAIR && threadIdx.x == 96) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
+    if (threadIdx.x == 64) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -391,7 +604,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     __syncthreads();
     if (cluster_size > 1) cluster_sync_all();  // the peers' barriers are initialised before any remote arrive
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     wait_for_previous();
 
     // K blocks of a unit that are this CTA's
@@ -406,55 +619,137 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const int quadrant = warp % 4, half = (warp - 4) / 4;
         const uint32_t release[2] = {peer_addr(&acc_empty[0], PAIR ? 0 : rank), peer_addr(&acc_empty[1], PAIR ? 0 : rank)};
-        int64_t piece = 0;
+        uint32_t piece = 0;
         bool ok = true;
         for (int u = group; u < args.units && ok; u += groups) {
             const Unit unit = unit_of<PRODUCT>(args, u, kTile);
             const Matrix &mt = args.table.matrix[unit.matrix];
             int kb0, kb1;
             k_range(mt, kb0, kb1);
+            const int row0 = quadrant * 32 + lane;
+            const bool whole_unit = PAIR || splits == 1;
+            // (of a shared tile the sums alone are worked out here)
+            Finish<PAIR, PRODUCT, N> finish(args, mt, unit.tm * kTile + pair_rank * 128 + row0,
+                                            unit.tn * kTile + half * kColumns, PAIR ? kColumns / 8 : 0,
+                                            PRODUCT == kSymmetric && unit.tm != unit.tn);
+            char *const buffer = reinterpret_cast<char *>(smem) + kRing * kStageBytes + (warp - 4) * 4096;
+            const int64_t lane_rows = lane * 128;  // from the warp's first row on
+            uint4 old_hi[8], old_lo[8];
+            if (!PAIR && whole_unit && finish.with_old) {
+                rows_to_lanes(finish.old - lane_rows, buffer, old_hi);
+                rows_to_lanes(finish.old - lane_rows + kOperandBytes, buffer, old_lo);
+            }
             float acc[kColumns];
 #pragma unroll
             for (int j = 0; j < kColumns; ++j) acc[j] = 0.0f;
             for (int kb = kb0; kb < kb1; kb += kPieceBlocks, ++piece) {
                 const int b = static_cast<int>(piece & 1);
-                if (!mbar_wait(&acc_full[b], static_cast<uint32_t>(piece >> 1) & 1u, abort_flag)) {
+                if (!mbar_wait(&acc_full[b], (piece >> 1) & 1u, abort_flag)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const float whole = 1.0f + (kb1 - kb < kPieceBlocks ? kb1 - kb : kPieceBlocks) * kCutOff;
                 const uint32_t at = tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16) +
-                                    static_cast<uint32_t>(b * kTile + half * kColumns);
+                                    static_cast<uint32_t>(b * kSums + half * kColumns);
+                if (PAIR) {
 #pragma unroll
-                for (int c = 0; c < kColumns / 64; ++c) {
-                    uint32_t v[64];
-                    tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
+                    for (int c = 0; c < kColumns / 64; ++c) {
+                        uint32_t v[64];
+                        tmem_ld64(at + static_cast<uint32_t>(c * 64), v);
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) acc[c * 64 + j] = fmaf(__uint_as_float(v[j]), whole, acc[c * 64 + j]);
+                        for (int j = 0; j < 64; ++j) acc[c * 64 + j] = fmaf(__uint_as_float(v[j]), whole, acc[c * 64 + j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2 * kColumns / 32; ++c) {  // hi.hi, and then the cross terms
+                        const bool cross = c >= kColumns / 32;
+                        const int first = c % (kColumns / 32) * 32;
+                        float v[32];
+                        tmem_ld32(at + static_cast<uint32_t>((cross ? kTile : 0) + first), v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) acc[first + j] = fmaf(v[j], cross ? 0x1p-11f : whole, acc[first + j]);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_remote(release[b]);
             }
-            const int row0 = quadrant * 32 + lane;
-            if (!PAIR && splits > 1) {
+            if (!whole_unit) {
                 // All MMAs of this CTA are done (and with them its loads): the stages hold the sums now.
                 float *sums = reinterpret_cast<float *>(smem) + row0 * kSumPitch + half * kColumns;
 #pragma unroll
                 for (int j = 0; j < kColumns; j += 4)
                     *reinterpret_cast<float4 *>(sums + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                // An equal share of the columns for each CTA, and of that for each half of the warps.
+                const int share = 64 / splits, col0 = rank * 2 * share + half * share;
+                Finish<PAIR, PRODUCT, N> finish_share(args, mt, unit.tm * kTile + row0, unit.tn * kTile + col0, share / 8,
+                                                      PRODUCT == kSymmetric && unit.tm != unit.tn);
+                cluster_sync_all();
+                const float *mine = reinterpret_cast<const float *>(smem) + row0 * kSumPitch + col0;
+#pragma unroll 1
+                for (int c = 0; c < share / 8; ++c) {
+                    float v[Finish<PAIR, PRODUCT, N>::kStep][8] = {};
+#pragma unroll 4
+                    for (int s = 0; s < splits; ++s) {
+                        const uint32_t from = peer_addr(mine + 8 * c, static_cast<uint32_t>(s));
+                        float x[8];
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(from) : "memory");
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "r"(from + 16) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[0][i] += x[i];
+                    }
+                    finish_share(c, v);
+                }
                 break;  // one unit a cluster
             }
             if (!ok) break;
-            const int row = unit.tm * kTile + pair_rank * 128 + row0, col = unit.tn * kTile + half * kColumns;
-            const bool mirror = PRODUCT == kSymmetric && unit.tm != unit.tn;
+            if (!PAIR) {
+                const bool floats = PRODUCT == kApply && args.last != 0;
+                uint4 out_hi[8], out_lo[8];
 #pragma unroll
-            for (int j = 0; j < kColumns; j += 8) {
-                float v[8];
+                for (int c = 0; c < 8; ++c) {
+                    float x[8], v[8];
+                    if (finish.with_old) from_pairs(old_hi[c], old_lo[c], x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = acc[j + i];
-                finish<PRODUCT>(args, mt, row, col + j, mirror, v);
+                    for (int i = 0; i < 8; ++i) v[i] = acc[8 * c + i];
+                    finish.combine(c, x, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[8 * c + i] = v[i];
+                    if (floats) continue;
+                    uint32_t w[8];
+                    to_pairs(v, w);
+                    split_pairs(w, out_hi[c], out_lo[c]);
+                    if (PRODUCT == kSymmetric && finish.mirror) finish.store_image(c, w);
+                }
+                if (!floats) {
+                    lanes_to_rows(out_hi, buffer, finish.to - lane_rows);
+                    lanes_to_rows(out_lo, buffer, finish.to - lane_rows + kOperandBytes);
+                } else if (mt.out_cs == 1) {
+                    lanes_to_output(acc, buffer, mt, finish.row - lane, finish.col);
+                    lanes_to_output(acc + 32, buffer, mt, finish.row - lane, finish.col + 32);
+                } else if (finish.row < mt.m) {
+                    float *out = mt.dst + finish.row * mt.out_rs + finish.col * mt.out_cs;
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (finish.col + j < mt.n) out[j * mt.out_cs] = acc[j];
+                }
+                __syncwarp();
+                continue;
+            }
+            // A rolled loop, the sums moved up by sixteen each time.
+#pragma unroll 1
+            for (int c = 0; c < kColumns / 8; c += 2) {
+                float v[Finish<PAIR, PRODUCT, N>::kStep][8];
+#pragma unroll
+                for (int k = 0; k < Finish<PAIR, PRODUCT, N>::kStep; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[k][i] = acc[8 * k + i];
+#pragma unroll
+                for (int i = 0; i + 16 < kColumns; ++i) acc[i] = acc[i + 16];
+                finish(c, v);
             }
             __syncwarp();
         }
@@ -462,66 +757,77 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == 0) {
-            if (lane == 0) {
-                int64_t it = 0;
-                bool ok = true;
-                for (int u = group; u < args.units && ok; u += groups) {
-                    const Unit unit = unit_of<PRODUCT>(args, u, kTile);
-                    const Matrix &mt = args.table.matrix[unit.matrix];
-                    int kb0, kb1;
-                    k_range(mt, kb0, kb1);
-                    const int ta = unit.tm * (kTile / 128) + pair_rank, tb = unit.tn * (kTile / 128) + pair_rank;
-                    const bool of_x = PRODUCT == kSymmetric && args.from == 0;
-                    const int a_at = PRODUCT == kApply ? mt.b : of_x ? mt.x[args.last] : mt.s;
-                    const int a_blocks = of_x ? mt.x_blocks : mt.s_blocks;
-                    const int b_at = PRODUCT == kApply ? mt.x[args.from] : a_at;
-                    const int b_blocks = PRODUCT == kApply ? mt.x_blocks : a_blocks;
-                    for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
-                        for (int lo = 0; lo < 2; ++lo) {
-                            const int depth = lo ? kLoStages : kHiStages;
-                            const int s = (lo ? kHiStages : 0) + static_cast<int>(it % depth);
-                            if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / depth) & 1u) ^ 1u, abort_flag)) {
-                                ok = false;
-                                break;
-                            }
-                            unsigned char *st = smem + s * kStageBytes;
-                            if (leader) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * kStageBytes);
-                            const uint32_t fb = peer_addr(&full[s], 0);
+            const bool elected = elect_one();
+            Stages<PAIR> stages;
+            int64_t it = 0;
+            bool ok = true;
+            for (int u = group; u < args.units && ok; u += groups) {
+                const Unit unit = unit_of<PRODUCT>(args, u, kTile);
+                const Matrix &mt = args.table.matrix[unit.matrix];
+                int kb0, kb1;
+                k_range(mt, kb0, kb1);
+                const int ta = unit.tm * (kTile / 128) + pair_rank, tb = unit.tn * (kTile / 128) + pair_rank;
+                const bool of_x = PRODUCT == kSymmetric && args.from == 0;
+                const int a_at = PRODUCT == kApply ? mt.b : of_x ? mt.x[args.last] : mt.s;
+                const int a_blocks = of_x ? mt.x_blocks : mt.s_blocks;
+                const int b_at = PRODUCT == kApply ? mt.x[args.from] : a_at;
+                const int b_blocks = PRODUCT == kApply ? mt.x_blocks : a_blocks;
+                for (int kb = kb0; kb < kb1 && ok; ++kb, ++it, stages.next()) {
+#pragma unroll
+                    for (int lo = 0; lo < 2; ++lo) {
+                        const int s = stages.at[lo];
+                        if (!wait_all(&empty[s], stages.parity[lo] ^ 1u, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        unsigned char *st = smem + s * kStageBytes;
+                        if (!elected) continue;
+                        if (leader) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * kStageBytes);
+                        const uint32_t fb = peer_addr(&full[s], 0);
+                        const int a_row = a_at + ((ta * a_blocks + kb) * 2 + lo) * 128;
+                        const int b_row = B_MN ? b_at + ((kb / 2 * b_blocks + tb * 2) * 2 + lo) * 128 + kb % 2 * 64
+                                               : b_at + ((tb * b_blocks + kb) * 2 + lo) * 128;
+                        constexpr int b_step = B_MN ? 256 : 64;  // to the second half
+                        if (PAIR) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const int a_row = a_at + ((ta * a_blocks + kb) * 2 + lo) * 128 + h * 64;
-                                const int b_row = B_MN ? b_at + ((kb / 2 * b_blocks + tb * 2 + h) * 2 + lo) * 128 + kb % 2 * 64
-                                                       : b_at + ((tb * b_blocks + kb) * 2 + lo) * 128 + h * 64;
-                                if (PAIR) {
-                                    load_half_pair(st + h * kHalfBytes, &map, fb, a_row);
-                                    load_half_pair(st + kOperandBytes + h * kHalfBytes, &map, fb, b_row);
-                                } else {
-                                    load_half(st + h * kHalfBytes, &map, &full[s], a_row);
-                                    load_half(st + kOperandBytes + h * kHalfBytes, &map, &full[s], b_row);
-                                }
+                                load_half_pair(st + h * kHalfBytes, &map, fb, a_row + h * 64);
+                                load_half_pair(st + kOperandBytes + h * kHalfBytes, &map, fb, b_row + h * b_step);
+                            }
+                        } else {
+                            const char *a_src = args.workspace + static_cast<int64_t>(a_row) * 128;
+                            const char *b_src = args.workspace + static_cast<int64_t>(b_row) * 128;
+                            load_rows(st, a_src, &full[s], kOperandBytes);
+                            if (B_MN) {
+                                load_rows(st + kOperandBytes, b_src, &full[s], kHalfBytes);
+                                load_rows(st + kOperandBytes + kHalfBytes, b_src + b_step * 128, &full[s], kHalfBytes);
+                            } else {
+                                load_rows(st + kOperandBytes, b_src, &full[s], kOperandBytes);
                             }
                         }
                     }
-                    if (!PAIR && splits > 1) break;
                 }
-                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
-                if (leader) {  // every stage issued has landed before the cluster exits
+                if (!PAIR && splits > 1) break;
+            }
+            if (!ok && elected) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+            if (leader && elected) {  // every stage issued has landed before the cluster exits
+                // (the last filling of each: of those that were filled, the one before the next)
+                for (int64_t d = it > kHiStages ? it - kHiStages : 0; d < it; ++d)
                     for (int lo = 0; lo < 2; ++lo) {
-                        const int depth = lo ? kLoStages : kHiStages;
-                        for (int64_t d = it > depth ? it - depth : 0; d < it; ++d) {
-                            uint64_t *bar = &full[(lo ? kHiStages : 0) + d % depth];
-                            const uint32_t round = static_cast<uint32_t>(d / depth);
-                            for (long long i = 0; i < kWaitLimit && !mbar_try_wait(bar, round & 1u); ++i) {
-                            }
+                        const int64_t depth = !PAIR ? kRing : lo ? kLoStages : kHiStages, n = PAIR ? d : 2 * d + lo;
+                        if (n + depth < (PAIR ? it : 2 * it)) continue;  // filled again since
+                        const int s = static_cast<int>(n % depth) + (PAIR && lo ? kHiStages : 0);
+                        for (long long i = 0; i < kWaitLimit && !mbar_try_wait(&full[s], static_cast<uint32_t>(n / depth) & 1u); ++i) {
                         }
                     }
-                }
             }
         } else if (warp == 1) {
-            if (lane == 0 && leader) {
+            if (leader) {
+                const bool elected = elect_one();
                 constexpr uint32_t idesc = instr_desc<PAIR, B_MN>();
                 constexpr uint64_t a_step = 32 >> 4, b_step = (B_MN ? 2048 : 32) >> 4;  // 16 of K
-                int64_t it = 0, piece = 0;
+                Stages<PAIR> stages;  // of the next block
+                uint32_t piece = 0;
                 bool ok = true;
                 for (int u = group; u < args.units && ok; u += groups) {
                     const Unit unit = unit_of<PRODUCT>(args, u, kTile);
@@ -530,33 +836,39 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
                     for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
                         const int n = kb1 - kb < kPieceBlocks ? kb1 - kb : kPieceBlocks;
                         const int b = static_cast<int>(piece & 1);
-                        if (!mbar_wait(&acc_empty[b], (static_cast<uint32_t>(piece >> 1) & 1u) ^ 1u, abort_flag)) {
+                        if (!wait_all(&acc_empty[b], ((piece >> 1) & 1u) ^ 1u, abort_flag)) {
                             ok = false;
                             break;
                         }
-                        const uint32_t d = tmem_base + static_cast<uint32_t>(b * kTile);
-                        for (int j = 0; j < n; ++j) {
-                            const int sh = static_cast<int>((it + j) % kHiStages);
-                            const int sl = kHiStages + static_cast<int>((it + j) % kLoStages);
-                            if (!mbar_wait(&full[sh], static_cast<uint32_t>((it + j) / kHiStages) & 1u, abort_flag) ||
-                                !mbar_wait(&full[sl], static_cast<uint32_t>((it + j) / kLoStages) & 1u, abort_flag)) {
+                        const uint32_t d = tmem_base + static_cast<uint32_t>(b * kSums);
+                        const uint32_t cross = PAIR ? d : d + kTile;
+                        int hi_stage = stages.at[0];
+                        for (int j = 0; j < n; ++j, stages.next()) {
+                            const int sh = stages.at[0], sl = stages.at[1];
+                            if (!wait_all(&full[sh], stages.parity[0], abort_flag) ||
+                                !wait_all(&full[sl], stages.parity[1], abort_flag)) {
                                 ok = false;
                                 break;
                             }
                             tc_fence_after();
+                            if (!elected) continue;
                             const uint32_t hi = smem_u32(smem + sh * kStageBytes), lo = smem_u32(smem + sl * kStageBytes);
                             const uint64_t ah = operand_desc<false>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
                             const uint64_t al = operand_desc<false>(lo), bl = operand_desc<B_MN>(lo + kOperandBytes);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                mma<PAIR>(d, ah + k * a_step, bl + k * b_step, idesc, j > 0 || k > 0);
-                                mma<PAIR>(d, al + k * a_step, bh + k * b_step, idesc, 1);
+                                mma<PAIR>(cross, ah + k * a_step, bl + k * b_step, idesc, j > 0 || k > 0);
+                                if (!PAIR) mma<PAIR>(d, ah + k * a_step, bh + k * b_step, idesc, j > 0 || k > 0);
+                                mma<PAIR>(cross, al + k * a_step, bh + k * b_step, idesc, 1);
                             }
                             commit<PAIR>(&empty[sl]);
+                            if (!PAIR) commit<PAIR>(&empty[sh]);
                         }
                         if (!ok) break;
-                        for (int j = 0; j < n; ++j) {
-                            const int sh = static_cast<int>((it + j) % kHiStages);
+                        for (int j = 0; PAIR && j < n; ++j) {
+                            const int sh = hi_stage;
+                            hi_stage = hi_stage + 1 < kHiStages ? hi_stage + 1 : 0;
+                            if (!elected) continue;
                             const uint32_t hi = smem_u32(smem + sh * kStageBytes);
                             const uint64_t ah = operand_desc<false>(hi), bh = operand_desc<B_MN>(hi + kOperandBytes);
                             if (j == 0) mma_scaled<PAIR>(d, ah, bh, idesc);
@@ -565,50 +877,27 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
                             for (int k = 1; k < 4; ++k) mma<PAIR>(d, ah + k * a_step, bh + k * b_step, idesc, 1);
                             commit<PAIR>(&empty[sh]);
                         }
-                        commit<PAIR>(&acc_full[b]);
-                        it += n;
+                        if (elected) commit<PAIR>(&acc_full[b]);
                     }
                     if (!PAIR && splits > 1) break;
                 }
-                if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+                if (!ok && elected) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
                 // all MMAs are done before a CTA frees its tensor memory
-                if (PAIR) umma_commit_pair_local(drain);
-                else commit<false>(drain);
+                if (elected) {
+                    if (PAIR) umma_commit_pair_local(drain);
+                    else commit<false>(drain);
+                }
                 for (long long i = 0; i < kWaitLimit && !mbar_try_wait(drain, 0u); ++i) {
                 }
             }
         }
+        __syncwarp();
+        if (!PAIR && splits > 1) cluster_sync_all();  // with the epilogue warps: the sums are in shared memory
     }
 
     tc_fence_before();
     __syncthreads();
-    if (cluster_size > 1) cluster_sync_all();  // the leader's MMAs have drained; all sums are in shared memory
-    if (!PAIR && splits > 1) {
-        if (warp >= 4 && group < args.units) {
-            const Unit unit = unit_of<PRODUCT>(args, group, kTile);
-            const Matrix &mt = args.table.matrix[unit.matrix];
-            const int quadrant = warp % 4, half = (warp - 4) / 4, share = 64 / splits;
-            const int row0 = quadrant * 32 + lane, col0 = rank * 2 * share + half * share;
-            const bool mirror = PRODUCT == kSymmetric && unit.tm != unit.tn;
-            const float *mine = reinterpret_cast<const float *>(smem) + row0 * kSumPitch + col0;
-            for (int j = 0; j < share; j += 8) {
-                float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-                for (int s = 0; s < splits; ++s) {
-                    const uint32_t from = peer_addr(mine + j, static_cast<uint32_t>(s));
-                    float x[8];
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(from) : "memory");
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                 : "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "r"(from + 16) : "memory");
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] += x[i];
-                }
-                finish<PRODUCT>(args, mt, unit.tm * kTile + row0, unit.tn * kTile + col0 + j, mirror, v);
-            }
-        }
-        cluster_sync_all();  // the sums have been read
-    }
+    if (cluster_size > 1) cluster_sync_all();  // a pair's MMAs have drained; the sums of a shared tile have been read
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -671,61 +960,76 @@ int64_t count_units(Table<N> &t, Product product, int tile) {
     return units;
 }
 
-template <Product PRODUCT, int N>
-int launch_product(const CUtensorMap &map, Args<N> &args, cudaStream_t stream) {
-    const int sms = sm_count(current_device());
-    bool pairs = true;
-    int64_t blocks = INT_MAX;  // of K, of the matrix with the fewest
-    for (int i = 0; i < args.table.count; ++i) {
-        const Matrix &m = args.table.matrix[i];
-        const int64_t k = ((PRODUCT == kSymmetric && args.from == 0 ? m.n : m.m) + kBlock - 1) / kBlock;
-        pairs = pairs && tile_of(m.m) == 256;
-        blocks = k < blocks ? k : blocks;
+int blocks_of(const Matrix &m, bool of_x) { return ((of_x ? m.n : m.m) + kBlock - 1) / kBlock; }
+
+struct Shape {
+    bool pairs;
+    int cluster, ctas;
+};
+
+// Microseconds of a launch whose units, those of most blocks first, go to `at_once` of them in
+// turn: `begin` and `end` of the launch, and for a unit of n blocks `block` times n / splits, or
+// the epilogue where that is longer.
+template <int N>
+double estimate(const Table<N> &t, bool of_x, int64_t units, int at_once, int splits, double begin, double block,
+                double epilogue, double end) {
+    double sum = begin + end;
+    int64_t u = 0;
+    for (int k = 0; k < 64 && u < units; ++k, u += at_once) {
+        const int n = (blocks_of(t.matrix[find_matrix(t, static_cast<int>(u))], of_x) + splits - 1) / splits;
+        sum += block * n > epilogue ? block * n : epilogue;
     }
-    if (pairs) {
-        const int64_t units = count_units(args.table, PRODUCT, 256);
-        if (units >= sms / 2) {
-            if (units >= INT_MAX) return fail(MTC_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
-            args.units = static_cast<int>(units);
-            return launch<true, PRODUCT, N>(map, args, 2, sms / 2 * 2, stream);
-        }
-    }
-    const int64_t units = count_units(args.table, PRODUCT, 128);
-    if (units >= INT_MAX) return fail(MTC_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
-    args.units = static_cast<int>(units);
-    int splits = 1;
-    while (splits < 8 && units * splits * 2 <= sms && blocks >= splits * 4) splits *= 2;
-    const int64_t ctas = splits > 1 ? units * splits : units < sms ? units : sms;
-    return launch<false, PRODUCT, N>(map, args, splits, static_cast<int>(ctas), stream);
+    return u < units ? sum * static_cast<double>(units) / static_cast<double>(u) : sum;
 }
 
+// Pairs on tiles of 256, single CTAs on tiles of 128, or these in clusters that share K: whatever
+// takes the shortest, by what the parts of a launch were seen to take (timers in the kernel).  A
+// block of 64 of K takes a pair 0.83 us, all pairs together 1.05 (L2 gives some 9 TB/s), a single
+// CTA 0.65 and all together 1.0, for a quarter of the products; a launch begins for 3 to 5 us,
+// and the last epilogues take 10 and 4; a cluster ends with its exchange, and its next unit is
+// launched anew.  (2048 x 2048, B X: 64 pairs 49 us, 256 single tiles 62; 1024 x 1024, X X^T: 36
+// clusters of 2 16 us, of 4 34, 10 pairs 30.)
 template <int N>
-int all_steps(Args<N> &args, const CUtensorMap &map, const Step *steps, int n, cudaStream_t stream) {
-    auto two = [](int e) { return std::ldexp(1.0, e); };
-    for (int k = 0; k < n; ++k) {
-        const Step &s = steps[k];
-        args.from = 0;
-        args.last = k % 2;  // (which X it is)
-        args.q = static_cast<float>(two(s.s - 2 * s.x));
-        args.unit = static_cast<float>(two(-2 * s.x));
-        MTC_TRY((launch_product<kSymmetric, N>(map, args, stream)));
-        args.from = 1;
-        args.q = static_cast<float>(s.c * two(s.b_exp - 2 * s.s));
-        args.p = static_cast<float>(s.b * two(s.b_exp - s.s));
-        args.r = static_cast<float>(s.c * two(s.b_exp - s.s));
-        args.b = s.b;
-        args.c = s.c;
-        args.unit = static_cast<float>(s.c * two(-2 * s.s));
-        MTC_TRY((launch_product<kSymmetric, N>(map, args, stream)));
-        const int to = k == n - 1 ? 0 : s.x_after;
-        args.from = k % 2;
-        args.last = k == n - 1;
-        args.q = static_cast<float>(two(to - s.b_exp - s.x));
-        args.p = static_cast<float>(two(to - s.x));
-        args.r = s.a;
-        MTC_TRY((launch_product<kApply, N>(map, args, stream)));
+int choose_shape(Args<N> &args, Product product, bool of_x, Shape &shape) {
+    Table<N> &t = args.table;
+    std::stable_sort(t.matrix, t.matrix + t.count,
+                     [&](const Matrix &a, const Matrix &b) { return blocks_of(a, of_x) > blocks_of(b, of_x); });
+    const int sms = sm_count(current_device());
+    double best = 1e30;
+    bool pairs = true;
+    for (int i = 0; i < t.count; ++i) pairs = pairs && tile_of(t.matrix[i].m) == 256;
+    if (pairs) {
+        const int64_t units = count_units(t, product, 256);
+        if (units < INT_MAX) {
+            const int at_once = static_cast<int>(units < sms / 2 ? units : sms / 2);
+            best = estimate(t, of_x, units, at_once, 1, 5.0, at_once * 3 < sms ? 0.83 : 1.05, 10.0, 10.0);
+            shape = Shape{true, 2, 2 * at_once};
+        }
     }
+    const int64_t units = count_units(t, product, 128);
+    if (units >= INT_MAX && !(best < 1e30)) return fail(MTC_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
+    // clusters that an SM's whole shared memory a CTA leaves room for, of 148 SMs
+    const int room[4] = {sms, sms / 2, sms * 33 / 148, sms * 15 / 148};
+    for (int i = 0, splits = 1; units < INT_MAX && i < 4; ++i, splits *= 2) {
+        if (splits > 1 && units * splits > INT_MAX / 2) break;
+        const int at_once = static_cast<int>(units < room[i] ? units : room[i]);
+        if (at_once < 1) break;
+        const double block = at_once * splits * 2 <= sms ? 0.65 : 1.0;
+        const double time = splits == 1 ? estimate(t, of_x, units, at_once, 1, 3.0, block, 4.0, 4.0)
+                                        : estimate(t, of_x, units, at_once, splits, 0.0, block, 0.0, 0.0) +
+                                              11.0 * static_cast<double>((units + at_once - 1) / at_once);
+        if (time >= best) continue;
+        best = time;
+        shape = Shape{false, splits, static_cast<int>(splits > 1 ? units * splits : at_once)};
+    }
+    args.units = static_cast<int>(count_units(t, product, shape.pairs ? 256 : 128));
     return MTC_OK;
+}
+
+template <Product PRODUCT, int N>
+int launch_product(const CUtensorMap &map, const Args<N> &args, const Shape &shape, cudaStream_t stream) {
+    return shape.pairs ? launch<true, PRODUCT, N>(map, args, shape.cluster, shape.ctas, stream)
+                       : launch<false, PRODUCT, N>(map, args, shape.cluster, shape.ctas, stream);
 }
 
 template <int N>
@@ -733,13 +1037,42 @@ int run_products(const Matrix *matrices, int count, const Step *steps, int n, ch
                  cudaStream_t stream) {
     CUtensorMap map;
     MTC_TRY(workspace_map(map, workspace, bytes));
-    Args<N> args;
-    std::memset(&args, 0, sizeof(args));
-    args.table.count = count;
-    for (int i = 0; i < count; ++i) args.table.matrix[i] = matrices[i];
-    args.workspace = workspace;
-    MTC_TRY(device_error_word(&args.err));
-    return all_steps(args, map, steps, n, stream);
+    Args<N> gram;
+    std::memset(&gram, 0, sizeof(gram));
+    gram.table.count = count;
+    for (int i = 0; i < count; ++i) gram.table.matrix[i] = matrices[i];
+    gram.workspace = workspace;
+    MTC_TRY(device_error_word(&gram.err));
+    Args<N> square = gram, apply = gram;
+    Shape gram_shape, square_shape, apply_shape;
+    MTC_TRY(choose_shape(gram, kSymmetric, true, gram_shape));
+    MTC_TRY(choose_shape(square, kSymmetric, false, square_shape));
+    MTC_TRY(choose_shape(apply, kApply, false, apply_shape));
+    auto two = [](int e) { return std::ldexp(1.0, e); };
+    for (int k = 0; k < n; ++k) {
+        const Step &s = steps[k];
+        gram.from = 0;
+        gram.last = k % 2;  // (which X it is)
+        gram.q = static_cast<float>(two(s.s - 2 * s.x));
+        gram.unit = static_cast<float>(two(-2 * s.x));
+        MTC_TRY((launch_product<kSymmetric, N>(map, gram, gram_shape, stream)));
+        square.from = 1;
+        square.q = static_cast<float>(s.c * two(s.b_exp - 2 * s.s));
+        square.p = static_cast<float>(s.b * two(s.b_exp - s.s));
+        square.r = static_cast<float>(s.c * two(s.b_exp - s.s));
+        square.b = s.b;
+        square.c = s.c;
+        square.unit = static_cast<float>(s.c * two(-2 * s.s));
+        MTC_TRY((launch_product<kSymmetric, N>(map, square, square_shape, stream)));
+        const int to = k == n - 1 ? 0 : s.x_after;
+        apply.from = k % 2;
+        apply.last = k == n - 1;
+        apply.q = static_cast<float>(two(to - s.b_exp - s.x));
+        apply.p = static_cast<float>(two(to - s.x));
+        apply.r = s.a;
+        MTC_TRY((launch_product<kApply, N>(map, apply, apply_shape, stream)));
+    }
+    return MTC_OK;
 }
 
 }  // namespace
