@@ -176,6 +176,28 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// Two blocks of 32 columns, waited for once.
+__device__ __forceinline__ void tmem_ld32_two(uint32_t from_v, uint32_t from_w, float (&v)[32], float (&w)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+          "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7]),
+          "=f"(w[8]), "=f"(w[9]), "=f"(w[10]), "=f"(w[11]), "=f"(w[12]), "=f"(w[13]), "=f"(w[14]), "=f"(w[15]),
+          "=f"(w[16]), "=f"(w[17]), "=f"(w[18]), "=f"(w[19]), "=f"(w[20]), "=f"(w[21]), "=f"(w[22]), "=f"(w[23]),
+          "=f"(w[24]), "=f"(w[25]), "=f"(w[26]), "=f"(w[27]), "=f"(w[28]), "=f"(w[29]), "=f"(w[30]), "=f"(w[31])
+        : "r"(from_v), "r"(from_w)
+        : "memory");
+}
+
 // The loader and the issuer run their loops with all lanes of their warps and values that the
 // compiler can tell are the same in all, so that these stay in uniform registers, which the
 // instructions that one lane of them issues want; a lone lane's loop moves each of them there
@@ -491,6 +513,12 @@ struct Finish {
     }
 };
 
+// The warp's buffer is free: the copies out of it that lane 0 has begun have read it.
+__device__ __forceinline__ void rows_are_read() {
+    if (threadIdx.x % 32 == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+}
+
 // A warp's 32 rows of a block of 64 columns, which are 4 KB in a row of the workspace, hi or lo, by
 // way of its 4 KB of shared memory: a lane reads and writes chunks of one row, but 16 bytes of each
 // of 32 rows at a time are 32 times the work of 512 bytes for the load and store units (a tile of
@@ -499,7 +527,7 @@ __device__ __forceinline__ void rows_to_lanes(const char *from, char *buffer, ui
     const int lane = threadIdx.x % 32;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4 *>(from + k * 512 + lane * 16);
-    __syncwarp();
+    rows_are_read();
 #pragma unroll
     for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4 *>(buffer + k * 512 + lane * 16) = v[k];
     __syncwarp();
@@ -509,19 +537,21 @@ __device__ __forceinline__ void rows_to_lanes(const char *from, char *buffer, ui
 
 __device__ __forceinline__ void lanes_to_rows(const uint4 (&v)[8], char *buffer, char *to) {
     const int lane = threadIdx.x % 32;
-    __syncwarp();
+    rows_are_read();
 #pragma unroll
     for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4 *>(buffer + lane * 128 + ((k ^ lane) & 7) * 16) = v[k];
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        *reinterpret_cast<uint4 *>(to + k * 512 + lane * 16) = *reinterpret_cast<const uint4 *>(buffer + k * 512 + lane * 16);
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], 4096;" ::"l"(to), "r"(smem_u32(buffer)) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
 }
 
 // The same for 32 of the outputs' columns, next to one another.
 __device__ __forceinline__ void lanes_to_output(const float *v, char *buffer, const Matrix &mt, int row0, int col) {
     const int lane = threadIdx.x % 32;
-    __syncwarp();
+    rows_are_read();
 #pragma unroll
     for (int k = 0; k < 8; ++k)
         *reinterpret_cast<float4 *>(buffer + lane * 128 + ((k ^ lane) & 7) * 16) =
@@ -574,6 +604,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     const int pair_rank = PAIR ? rank : 0;
     const bool leader = pair_rank == 0;
 
+    // The first unit, which the parameters' way from memory makes the longest part of a launch's
+    // beginning, while the barriers and the tensor memory are set up.
+    const Unit first_unit = unit_of<PRODUCT>(args, group < args.units ? group : 0, kTile);
     if (PAIR && threadIdx.x == 96) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
     if (threadIdx.x == 64) {
         for (int s = 0; s < kStages; ++s) {
@@ -622,7 +655,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         uint32_t piece = 0;
         bool ok = true;
         for (int u = group; u < args.units && ok; u += groups) {
-            const Unit unit = unit_of<PRODUCT>(args, u, kTile);
+            const Unit unit = u == group ? first_unit : unit_of<PRODUCT>(args, u, kTile);
             const Matrix &mt = args.table.matrix[unit.matrix];
             int kb0, kb1;
             k_range(mt, kb0, kb1);
@@ -662,13 +695,12 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < 2 * kColumns / 32; ++c) {  // hi.hi, and then the cross terms
-                        const bool cross = c >= kColumns / 32;
-                        const int first = c % (kColumns / 32) * 32;
-                        float v[32];
-                        tmem_ld32(at + static_cast<uint32_t>((cross ? kTile : 0) + first), v);
+                    for (int c = 0; c < kColumns / 32; ++c) {
+                        float v[32], w[32];
+                        tmem_ld32_two(at + static_cast<uint32_t>(c * 32), at + static_cast<uint32_t>(kTile + c * 32), v, w);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) acc[first + j] = fmaf(v[j], cross ? 0x1p-11f : whole, acc[first + j]);
+                        for (int j = 0; j < 32; ++j)
+                            acc[c * 32 + j] = fmaf(v[j], whole, fmaf(w[j], 0x1p-11f, acc[c * 32 + j]));
                     }
                 }
                 tc_fence_before();
@@ -754,6 +786,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             __syncwarp();
         }
         if (!ok) atomicCAS(args.err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+        if (!PAIR && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // written, before the next launch
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == 0) {
@@ -762,7 +795,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             int64_t it = 0;
             bool ok = true;
             for (int u = group; u < args.units && ok; u += groups) {
-                const Unit unit = unit_of<PRODUCT>(args, u, kTile);
+                const Unit unit = u == group ? first_unit : unit_of<PRODUCT>(args, u, kTile);
                 const Matrix &mt = args.table.matrix[unit.matrix];
                 int kb0, kb1;
                 k_range(mt, kb0, kb1);
@@ -830,7 +863,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
                 uint32_t piece = 0;
                 bool ok = true;
                 for (int u = group; u < args.units && ok; u += groups) {
-                    const Unit unit = unit_of<PRODUCT>(args, u, kTile);
+                    const Unit unit = u == group ? first_unit : unit_of<PRODUCT>(args, u, kTile);
                     int kb0, kb1;
                     k_range(args.table.matrix[unit.matrix], kb0, kb1);
                     for (int kb = kb0; kb < kb1 && ok; kb += kPieceBlocks, ++piece) {
@@ -985,10 +1018,11 @@ double estimate(const Table<N> &t, bool of_x, int64_t units, int at_once, int sp
 // Pairs on tiles of 256, single CTAs on tiles of 128, or these in clusters that share K: whatever
 // takes the shortest, by what the parts of a launch were seen to take (timers in the kernel).  A
 // block of 64 of K takes a pair 0.83 us, all pairs together 1.05 (L2 gives some 9 TB/s), a single
-// CTA 0.65 and all together 1.0, for a quarter of the products; a launch begins for 3 to 5 us,
-// and the last epilogues take 10 and 4; a cluster ends with its exchange, and its next unit is
-// launched anew.  (2048 x 2048, B X: 64 pairs 49 us, 256 single tiles 62; 1024 x 1024, X X^T: 36
-// clusters of 2 16 us, of 4 34, 10 pairs 30.)
+// CTA 0.67 (what an SM takes in) and all together 1.05, for a quarter of the products.  A launch
+// begins and ends for 9.5 us on single tiles, 16 to 28 on pairs' (the epilogue of a symmetric
+// product writes its image too), 14 to 19 on shared ones, which are launched anew for each that
+// an SM takes.  (2048 x 2048, B X: 64 pairs 49 us, 256 single tiles 62; 1024 x 1024, X X^T: 36
+// clusters of 2 19 us, of 4 34, 10 pairs 30; 512 x 512: 10 single tiles 15, clusters of 8 20.)
 template <int N>
 int choose_shape(Args<N> &args, Product product, bool of_x, Shape &shape) {
     Table<N> &t = args.table;
@@ -1002,7 +1036,7 @@ int choose_shape(Args<N> &args, Product product, bool of_x, Shape &shape) {
         const int64_t units = count_units(t, product, 256);
         if (units < INT_MAX) {
             const int at_once = static_cast<int>(units < sms / 2 ? units : sms / 2);
-            best = estimate(t, of_x, units, at_once, 1, 5.0, at_once * 3 < sms ? 0.83 : 1.05, 10.0, 10.0);
+            best = estimate(t, of_x, units, at_once, 1, 6.0, at_once * 3 < sms ? 0.83 : 1.05, 10.0, product == kSymmetric ? 22.0 : 10.0);
             shape = Shape{true, 2, 2 * at_once};
         }
     }
@@ -1014,10 +1048,11 @@ int choose_shape(Args<N> &args, Product product, bool of_x, Shape &shape) {
         if (splits > 1 && units * splits > INT_MAX / 2) break;
         const int at_once = static_cast<int>(units < room[i] ? units : room[i]);
         if (at_once < 1) break;
-        const double block = at_once * splits * 2 <= sms ? 0.65 : 1.0;
-        const double time = splits == 1 ? estimate(t, of_x, units, at_once, 1, 3.0, block, 4.0, 4.0)
+        const double block = at_once * splits * 2 <= sms ? 0.67 : 1.05;
+        const double shared[4] = {0.0, 14.0, 15.0, 19.0};
+        const double time = splits == 1 ? estimate(t, of_x, units, at_once, 1, 4.5, block, 4.0, 5.0)
                                         : estimate(t, of_x, units, at_once, splits, 0.0, block, 0.0, 0.0) +
-                                              11.0 * static_cast<double>((units + at_once - 1) / at_once);
+                                              shared[i] * static_cast<double>((units + at_once - 1) / at_once);
         if (time >= best) continue;
         best = time;
         shape = Shape{false, splits, static_cast<int>(splits > 1 ? units * splits : at_once)};
