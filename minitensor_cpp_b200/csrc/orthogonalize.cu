@@ -7,9 +7,10 @@
 // the elements of X, S and B are below it and its polynomials, which gives the packed operands
 // of the tensor cores fixed scales: nothing is looked at while the products run.
 //
-// Small matrices are worked on by a CTA each, in shared memory, in float32 (k_small).  All
-// others are packed into pairs of 16-bit floats once and then stay so, from one product's
-// epilogue to the next one's operands (orthogonalize_tc.cu).
+// Small matrices are worked on by a CTA each, in shared memory: in float32 (k_small), or on the
+// tensor cores where both sides are 128 or less and the products are enough.  All others are
+// packed into pairs of 16-bit floats once and then stay so, from one product's epilogue to the
+// next one's operands (orthogonalize_tc.cu).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -40,17 +41,7 @@ __device__ __forceinline__ double block_sum(double v) {
     return v;
 }
 
-// What the elements are multiplied by: zeros stay zeros whatever eps is, and one element that is
-// not finite makes all of them NaN.
-__device__ __forceinline__ double inverse_norm(double squares, float eps) {
-    if (squares == 0.0) return 0.0;
-    const double norm = sqrt(squares);
-    return isfinite(norm) ? 1.0 / (norm + static_cast<double>(eps)) : nan("");
-}
-
 // ---------------------------------------------------------- small matrices --
-
-constexpr int kMostSteps = 32;
 
 struct SmallSteps {
     int n;
@@ -215,8 +206,7 @@ __global__ void __launch_bounds__(kThreads) k_squares(const __grid_constant__ Ta
     if (threadIdx.x == 0) partials[mt.part + static_cast<int>(blockIdx.x) - table.first[k]] = acc;
 }
 
-// Units of the padded matrix.  The factor is a float32 in [1, 2) and a power of two in two parts,
-// which neither the largest nor the smallest norms take out of float32.
+// Units of the padded matrix.
 template <int N>
 __global__ void __launch_bounds__(kThreads) k_pack_matrices(const __grid_constant__ Table<N> table, const double *partials,
                                                             float eps, int scale, char *workspace) {
@@ -226,13 +216,10 @@ __global__ void __launch_bounds__(kThreads) k_pack_matrices(const __grid_constan
     const Matrix &mt = table.matrix[k];
     double squares = 0.0;
     for (int i = threadIdx.x; i < mt.parts; i += kThreads) squares += partials[mt.part + i];
-    int e = 0;
-    const float factor = 2.0f * static_cast<float>(frexp(inverse_norm(block_sum(squares), eps), &e));
-    e += scale - 1;
-    const float f0 = exp2f(static_cast<float>(e / 2)), f1 = exp2f(static_cast<float>(e - e / 2));
+    const Factor factor(inverse_norm(block_sum(squares), eps), scale);
     const int u = static_cast<int>(blockIdx.x) - table.first[k];
     const Unit at{u / mt.x_blocks * kUnitRows, u % mt.x_blocks * 64};
-    read_unit(mt, at, [&](int r, int c, float v) { tile[r * 65 + c] = v * f0 * factor * f1; });
+    read_unit(mt, at, [&](int r, int c, float v) { tile[r * 65 + c] = factor(v); });
     __syncthreads();
     const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 8;  // a row's eight chunks side by side
     __half2 hi[4], lo[4];
@@ -336,28 +323,16 @@ void add_matrices(const mtc_desc &in, const mtc_desc &out, std::vector<Matrix> &
     }
 }
 
-// A CTA's matrix: in shared memory, and up to about 64 x 64 x 64 of products.
+// A CTA's matrix in float32: in shared memory, and of few products.  Up to 128 columns the other way
+// is a CTA with the tensor cores (48 x 48: 38 us here, 47 there; 64 x 64: 50 and 48.5), beyond 17
+// launches (64 x 100: 160 us there, and in proportion to its products some 70 here).
 bool is_small(const Matrix &mt) {
     const int64_t m = mt.m, n = mt.n;
-    return 2 * m * m * n + m * m * m <= 3 * 64 * 64 * 64 && small_bytes(mt.m, mt.n) <= 200 * 1024;
+    return 2 * m * m * n + m * m * m <= (n <= 128 ? 3 * 60 * 60 * 60 : 9 * 64 * 64 * 64) &&
+           small_bytes(mt.m, mt.n) <= 200 * 1024;
 }
 
-// Calls f with a table of the matrices at hand: a small one where they are few.
-template <class F>
-int with_table(const Matrix *m, int count, F &&f) {
-    auto fill = [&](auto &t) {
-        std::memset(&t, 0, sizeof(t));
-        t.count = count;
-        for (int i = 0; i < count; ++i) t.matrix[i] = m[i];
-        return f(t);
-    };
-    if (count <= 8) {
-        Table<8> t;
-        return fill(t);
-    }
-    Table<kMostMatrices> t;
-    return fill(t);
-}
+bool is_whole(const Matrix &mt) { return mt.n <= 128; }
 
 int run_small(const std::vector<Matrix> &all, const std::vector<Step> &steps, float eps, cudaStream_t stream) {
     SmallSteps s;
@@ -472,9 +447,9 @@ int run(const mtc_desc *tensors, int32_t n, const float *coefficients, int32_t n
     MTC_TRY(check_lists(tensors, n, outs));
     std::vector<Step> steps;
     MTC_TRY(follow_steps(coefficients, n_steps, steps));
-    std::vector<Matrix> all, small, low, large;  // low: one row of tiles, of 128
+    std::vector<Matrix> all, small, whole, low, large;  // low: one row of tiles, of 128
     for (int i = 0; i < n; ++i) add_matrices(tensors[i], outs[i], all);
-    for (const Matrix &m : all) (is_small(m) ? small : tile_of(m.m) == 128 ? low : large).push_back(m);
+    for (const Matrix &m : all) (is_small(m) ? small : is_whole(m) ? whole : tile_of(m.m) == 128 ? low : large).push_back(m);
     for (std::vector<Matrix> *list : {&large, &low}) {
         for (size_t at = 0; at < list->size();) {
             size_t end = at, bytes = 0;
@@ -484,6 +459,17 @@ int run(const mtc_desc *tensors, int32_t n, const float *coefficients, int32_t n
             MTC_TRY(run_group(list->data() + at, static_cast<int>(end - at), steps, eps, stream));
             at = end;
         }
+    }
+    if (!whole.empty()) {  // small ones along with them, on other SMs, not after them
+        for (size_t i = 0; i < small.size();) {
+            if (!is_whole(small[i])) {
+                ++i;
+                continue;
+            }
+            whole.push_back(small[i]);
+            small.erase(small.begin() + static_cast<std::ptrdiff_t>(i));
+        }
+        MTC_TRY(whole_matrices(whole.data(), static_cast<int>(whole.size()), steps.data(), static_cast<int>(steps.size()), eps, stream));
     }
     return small.empty() ? MTC_OK : run_small(small, steps, eps, stream);
 }

@@ -2,6 +2,8 @@
 // and orthogonalize_tc.cu (products on the tensor cores).
 #pragma once
 
+#include <cmath>
+
 #include "operators.cuh"
 
 namespace mtc {
@@ -36,6 +38,33 @@ inline int64_t pad_to(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // All products of all steps over `count` matrices, packed at x[0] of each.
 int products(const Matrix *matrices, int count, const Step *steps, int n_steps, char *workspace, size_t bytes, cudaStream_t stream);
 
+constexpr int kMostSteps = 32;
+
+// What the elements are multiplied by: zeros stay zeros whatever eps is, and one element that is
+// not finite makes all of them NaN.
+__host__ __device__ inline double inverse_norm(double squares, float eps) {
+    if (squares == 0.0) return 0.0;
+    const double norm = sqrt(squares);
+    return isfinite(norm) ? 1.0 / (norm + static_cast<double>(eps)) : nan("");
+}
+
+// That and a scale as a float32 in [1, 2) and a power of two in two parts, which neither the
+// largest nor the smallest norms take out of float32.
+struct Factor {
+    float f, two0, two1;
+    __host__ __device__ Factor(double inverse, int scale) {
+        int e = 0;
+        f = 2.0f * static_cast<float>(frexp(inverse, &e));
+        e += scale - 1;
+        two0 = exp2f(static_cast<float>(e / 2));
+        two1 = exp2f(static_cast<float>(e - e / 2));
+    }
+    __host__ __device__ float operator()(float v) const { return v * two0 * f * two1; }
+};
+
+// All steps over matrices of up to 128 x 128, a CTA each (one launch for each kMostMatrices).
+int whole_matrices(const Matrix *matrices, int count, const Step *steps, int n_steps, float eps, cudaStream_t stream);
+
 constexpr int kMostMatrices = 128;  // of a launch: they travel in its parameters
 
 template <int N>
@@ -44,6 +73,23 @@ struct Table {
     int first[N + 1];  // unit of the launch's work that a matrix begins with
     Matrix matrix[N];
 };
+
+// Calls f with a table of the matrices at hand: a small one where they are few.
+template <class F>
+int with_table(const Matrix *m, int count, F &&f) {
+    auto fill = [&](auto &t) {
+        std::memset(&t, 0, sizeof(t));
+        t.count = count;
+        for (int i = 0; i < count; ++i) t.matrix[i] = m[i];
+        return f(t);
+    };
+    if (count <= 8) {
+        Table<8> t;
+        return fill(t);
+    }
+    Table<kMostMatrices> t;
+    return fill(t);
+}
 
 // The matrix that unit u belongs to.
 template <int N>

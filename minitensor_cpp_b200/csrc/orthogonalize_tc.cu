@@ -941,6 +941,216 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     }
 }
 
+// --------------------------------------------------- matrices of one tile --
+//
+// Up to 128 x 128: a CTA has X, R and Q in shared memory as blocks' images, 64 KB each, and goes
+// through all products of all steps: the MMAs of one, then its sums out of tensor memory, worked
+// out and written to the next one's operand by all threads.  Bound by that chain's latency, 3 to
+// 4.5 us a product: five steps of 64 x 64 in 48 us, of 128 x 128 in 69 (by launches of their own,
+// 145), 64 of these in 78 (164).
+
+constexpr int kWholeThreads = 256, kImage = 4 * kOperandBytes;  // two blocks, hi and lo
+constexpr int kTilePitch = 129;                                 // of X as float32, in the place of R and Q
+constexpr int kWholeBytes = 3 * kImage + 1024 + 2 * 128 * 4 + 64;
+static_assert(kWholeBytes <= 227 * 1024 && 128 * kTilePitch * 4 <= 2 * kImage, "shared memory");
+
+struct WholeSteps {
+    int n;
+    float eps;
+    Step step[kMostSteps];
+};
+
+__device__ __forceinline__ double whole_sum(double v, double *part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWholeThreads / 32; ++i) v += part[i];
+    return v;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kWholeThreads, 1)
+    k_whole(const __grid_constant__ Table<N> table, const __grid_constant__ WholeSteps steps, unsigned long long *err) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ double part[kWholeThreads / 32];
+    char *const x = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    char *const r = x + kImage, *const q = r + kImage;
+    float *const d = reinterpret_cast<float *>(q + kImage), *const e = d + 128;
+    uint64_t *const bar = reinterpret_cast<uint64_t *>(e + 128);
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(bar + 1);
+    volatile int *const abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x / 32), 0), lane = threadIdx.x % 32;
+    const Matrix &mt = table.matrix[blockIdx.x];
+    if (threadIdx.x == 64) {
+        mbar_init(bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // X as it is, and its norm
+    float *const tile = reinterpret_cast<float *>(r);
+    const bool along = mt.cs == 1 || mt.rs != 1;
+    double squares = 0.0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < 128 * 128; i += kWholeThreads) {
+        const int row = along ? i / 128 : i % 128, col = along ? i % 128 : i / 128;
+        const float v = row < mt.m && col < mt.n ? mt.src[row * mt.rs + col * mt.cs] : 0.0f;
+        squares += static_cast<double>(v) * v;
+        tile[row * kTilePitch + col] = v;
+    }
+    tc_fence_before();
+    const Factor factor(inverse_norm(whole_sum(squares, part), steps.eps), steps.step[0].x);
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    // a thread's row and the first of its 64 columns, which are one block
+    const int row = warp % 4 * 32 + lane, col0 = warp / 4 * 64;
+    const int at = warp / 4 * 2 * kOperandBytes + row * 128;
+    auto chunk = [&](char *image, int c) { return image + at + ((c ^ row) & 7) * 16; };
+    auto put = [&](char *image, int c, const float (&v)[8]) {
+        uint32_t w[8];
+        uint4 h, l;
+        to_pairs(v, w);
+        split_pairs(w, h, l);
+        *reinterpret_cast<uint4 *>(chunk(image, c)) = h;
+        *reinterpret_cast<uint4 *>(chunk(image, c) + kOperandBytes) = l;
+    };
+    auto get = [&](char *image, int c, float (&v)[8]) {
+        from_pairs(*reinterpret_cast<const uint4 *>(chunk(image, c)),
+                   *reinterpret_cast<const uint4 *>(chunk(image, c) + kOperandBytes), v);
+    };
+#pragma unroll 2
+    for (int c = 0; c < 8; ++c) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = factor(tile[row * kTilePitch + col0 + 8 * c + j]);
+        put(x, c, v);
+    }
+    uint32_t phase = 0;
+    float acc[64];
+    // The sums of a product over `blocks` blocks of K, A K-major and B either way.  Warps without a
+    // row or a column of the result leave it be; of R and Q, whose columns are K after that, rows
+    // count up to a whole block.
+    auto product = [&](char *a, char *b, bool mn, int blocks, bool here) {
+        tc_fence_before();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();  // the operands are written, and the last sums read
+        if (warp == 0 && elect_one()) {
+            tc_fence_after();
+            const uint32_t idesc = mn ? instr_desc<false, true>() : instr_desc<false, false>();
+            for (int k = 0; k < 4 * blocks; ++k) {
+                const uint32_t block = static_cast<uint32_t>(k / 4 * 2 * kOperandBytes + k % 4 * 32);
+                const uint64_t ah = operand_desc<false>(smem_u32(a) + block);
+                const uint64_t al = operand_desc<false>(smem_u32(a) + block + kOperandBytes);
+                // of 16 rows of X, the next 64 columns a block on
+                const uint64_t far = static_cast<uint64_t>((2 * kOperandBytes - 8192) >> 4) << 16;
+                const uint64_t bh = mn ? operand_desc<true>(smem_u32(b) + k * 2048) + far
+                                       : operand_desc<false>(smem_u32(b) + block);
+                const uint64_t bl = mn ? operand_desc<true>(smem_u32(b) + k * 2048 + kOperandBytes) + far
+                                       : operand_desc<false>(smem_u32(b) + block + kOperandBytes);
+                mma<false>(tmem + 128, ah, bl, idesc, k > 0);
+                mma<false>(tmem, ah, bh, idesc, k > 0);
+                mma<false>(tmem + 128, al, bh, idesc, 1);
+            }
+            commit<false>(bar);
+        }
+        __syncwarp();
+        const bool ok = mbar_wait(bar, phase, abort_flag);
+        phase ^= 1;
+        tc_fence_after();
+        if (!here) return ok;
+        const float whole = 1.0f + blocks * kCutOff;
+        const uint32_t from = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + static_cast<uint32_t>(col0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float v[32], w[32];
+            tmem_ld32_two(from + c * 32, from + 128 + c * 32, v, w);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(v[j], whole, w[j] * 0x1p-11f);
+        }
+        return ok;
+    };
+    const int m_blocks = (mt.m + kBlock - 1) / kBlock, n_blocks = (mt.n + kBlock - 1) / kBlock;
+    const bool of_s = warp % 4 * 32 < m_blocks * kBlock && col0 < mt.m, of_x = warp % 4 * 32 < mt.m && col0 < mt.n;
+    bool ok = true;
+    for (int k = 0; k < steps.n; ++k) {
+        const Step &s = steps.step[k];
+        ok = product(x, x, false, n_blocks, of_s) && ok;
+        float scale = exp2f(static_cast<float>(s.s - 2 * s.x)), unit = exp2f(static_cast<float>(-2 * s.x));
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (!of_s) break;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = acc[8 * c + j] * scale;
+                if (row == col0 + 8 * c + j) {
+                    d[row] = acc[8 * c + j] * unit;
+                    v[j] = 0.0f;
+                }
+            }
+            put(r, c, v);
+        }
+        ok = product(r, r, false, m_blocks, of_s) && ok;
+        const float by_s = exp2f(static_cast<float>(s.b_exp - s.s));
+        scale = s.c * exp2f(static_cast<float>(s.b_exp - 2 * s.s));
+        unit = s.c * exp2f(static_cast<float>(-2 * s.s));
+        const float di = d[row];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (!of_s) break;
+            float v[8], old[8];
+            get(r, c, old);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int col = col0 + 8 * c + j;
+                v[j] = fmaf(fmaf(s.c * by_s, di + d[col], s.b * by_s), old[j], scale * acc[8 * c + j]);
+                if (row == col) {
+                    e[row] = fmaf(fmaf(s.c, di, s.b), di, unit * acc[8 * c + j]);
+                    v[j] = 0.0f;
+                }
+            }
+            put(q, c, v);
+        }
+        ok = product(q, x, true, m_blocks, of_x) && ok;
+        const bool last = k == steps.n - 1;
+        const int to = last ? 0 : s.x_after;
+        scale = exp2f(static_cast<float>(to - s.b_exp - s.x));
+        const float own = exp2f(static_cast<float>(to - s.x)) * (s.a + e[row]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (!of_x) break;
+            float v[8], old[8];
+            get(x, c, old);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = fmaf(own, old[j], scale * acc[8 * c + j]);
+                if (last) tile[row * kTilePitch + col0 + 8 * c + j] = v[j];
+            }
+            if (!last) put(x, c, v);
+        }
+        if (!__syncthreads_and(ok)) break;
+    }
+    if (!ok && lane == 0) atomicCAS(err, 0ull, static_cast<unsigned long long>(MTC_ERR_RUNTIME));
+    const bool out_along = mt.out_cs == 1 || mt.out_rs != 1;
+    for (int i = threadIdx.x; i < mt.m * mt.n; i += kWholeThreads) {
+        const int row = out_along ? i / mt.n : i % mt.m, col = out_along ? i % mt.n : i / mt.m;
+        mt.dst[row * mt.out_rs + col * mt.out_cs] = tile[row * kTilePitch + col];
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+    }
+}
+
 // ------------------------------------------------------------------- host --
 
 // The workspace as rows of 128 bytes, in boxes of 64.
@@ -1115,6 +1325,26 @@ int run_products(const Matrix *matrices, int count, const Step *steps, int n, ch
 int products(const Matrix *matrices, int count, const Step *steps, int n_steps, char *workspace, size_t bytes, cudaStream_t stream) {
     return count <= 8 ? run_products<8>(matrices, count, steps, n_steps, workspace, bytes, stream)
                       : run_products<kMostMatrices>(matrices, count, steps, n_steps, workspace, bytes, stream);
+}
+
+int whole_matrices(const Matrix *matrices, int count, const Step *steps, int n_steps, float eps, cudaStream_t stream) {
+    WholeSteps w;
+    std::memset(&w, 0, sizeof(w));
+    w.n = n_steps;
+    w.eps = eps;
+    for (int k = 0; k < n_steps; ++k) w.step[k] = steps[k];
+    unsigned long long *err = nullptr;
+    MTC_TRY(device_error_word(&err));
+    for (int at = 0; at < count; at += kMostMatrices) {
+        const int n = count - at < kMostMatrices ? count - at : kMostMatrices;
+        MTC_TRY(with_table(matrices + at, n, [&](const auto &t) {
+            constexpr int N = sizeof(t.matrix) / sizeof(t.matrix[0]);
+            MTC_CUDA_TRY(cudaFuncSetAttribute(k_whole<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWholeBytes));
+            k_whole<N><<<n, kWholeThreads, kWholeBytes, stream>>>(t, w, err);
+            return check_launch("orthogonalize (one tile)");
+        }));
+    }
+    return MTC_OK;
 }
 
 }  // namespace ortho
