@@ -341,7 +341,8 @@ int mtc_linear_cross_entropy_grad(const mtc_desc *x, const mtc_desc *weight, con
  * -1; so are those of a token outside [0, V), which also sets the device error word.
  * Logits of -inf have probability 0.  A row of nothing else has lse, log_probs and
  * top_log_probs -inf and entropy 0.  A NaN or +inf in a row makes its floats NaN; a
- * NaN counts as the largest logit.  Needs no workspace. */
+ * NaN counts as the largest logit.  What a row gives depends on its own logits and
+ * their alignment, not on the other rows.  Needs no workspace. */
 int mtc_token_log_probs(const mtc_desc *logits, const mtc_desc *tokens, float scale, int64_t ignore_token,
                         const mtc_desc *log_probs, const mtc_desc *lse, const mtc_desc *entropy,
                         const mtc_desc *top_log_probs, const mtc_desc *top_tokens, void *stream);
@@ -383,12 +384,15 @@ int mtc_clip_global_norm(const mtc_desc *tensors, int32_t n, float max_norm, con
  *
  * Products have float32 accuracy: small matrices are worked on in float32, others
  * as pairs of 16-bit floats, which hold an element of X, S or of the polynomial to
- * 2^-22 of itself or to 2^-49 of the largest it could be, whichever is more.
+ * 2^-22 of itself or to 2^-49 of the largest it could be, whichever is more; the
+ * diagonals of S and of the polynomial are kept apart in float32.  The same call gives
+ * the same bits; in a list with other matrices one may be split differently, and so
+ * rounded differently.
  *
- * Workspace (but for small matrices): 8 bytes an element and 8 for each element of S,
- * sides padded to a multiple of 256 (of 128 where the shorter one is 128 or less),
- * for as many matrices at a time as take 4 GiB together, one at least; where the
- * pool cannot give that, for fewer. */
+ * Workspace (none for small matrices and those of up to 128 x 128): 8 bytes an element
+ * and 8 for each element of S, sides padded to a multiple of 256 (of 128 where the
+ * shorter one is 128 or less), for as many matrices at a time as take 4 GiB together,
+ * one at least; where the pool cannot give that, for fewer. */
 int mtc_orthogonalize(const mtc_desc *tensors, int32_t n, const float *coefficients, int32_t steps, float eps,
                       const mtc_desc *outs, void *stream);
 

@@ -507,7 +507,7 @@ def orthogonalize(tensors: Sequence[View], outs: Sequence[View] | None = None,
         raise ValueError(f"{len(outs)} outputs for {len(tensors)} tensors")
     to = arr if outs is None else _packed_all(outs)
     flat = [float(v) for step in coefficients for v in step]
-    if len(flat) != 3 * len(coefficients):
+    if any(len(step) != 3 for step in coefficients):
         raise ValueError("coefficients are not of three numbers a step")
     table = (ctypes.c_float * max(len(flat), 1))(*flat)
     return _run("mtc_orthogonalize", (arr, len(tensors), table, len(coefficients), eps, to, _stream(stream)),

@@ -277,6 +277,27 @@ def test_a_large_matrix(cuda):
     assert (got.double() - want).norm() <= norm_bound(t, CUBIC[:2])
 
 
+def test_more_than_one_group(cuda):
+    """Five matrices whose packed operands take more than is taken at a time; one input may come again."""
+    import torch
+
+    t = matrix(27, 8192, 8200)
+    steps = CUBIC[:1]
+    outs = [torch.full_like(t, 99.0) for _ in range(5)]
+    abi.orthogonalize([view(t)] * 5, [view(o) for o in outs], coefficients=steps)
+    abi.check_device_errors(0)
+    want, tol = reference(t, steps), norm_bound(t, steps)
+    assert all((o.double() - want).norm() <= tol for o in outs)
+
+
+def test_paths_agree_where_they_meet(cuda):
+    """The sizes on both sides of each change of the path, in one list and alone."""
+    for shape in ((59, 61), (61, 61), (62, 62), (128, 128), (128, 129), (127, 300), (129, 129), (64, 300), (64, 330), (5, 5000)):
+        t = matrix(28, *shape)
+        check([t])
+        check([t, matrix(29, 60, 60), matrix(30, 100, 90), matrix(31, 300, 280)])
+
+
 def test_elements_behind_32_bits(cuda):
     """A batch whose last matrices lie behind 2^31 elements."""
     import torch

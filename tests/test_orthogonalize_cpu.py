@@ -73,6 +73,8 @@ def test_python_wrapper():
         abi.orthogonalize([v(0, 3)], [], stream=0)
     with pytest.raises(ValueError, match="three numbers"):
         abi.orthogonalize([v(0, 3)], coefficients=[(1.0, 2.0)], stream=0)
+    with pytest.raises(ValueError, match="three numbers"):
+        abi.orthogonalize([v(0, 3)], coefficients=[(1.0, 2.0), (1.0, 2.0, 3.0, 4.0)], stream=0)
     with pytest.raises(ValueError, match="no matrix"):
         abi.orthogonalize([v(3)], stream=0)
     with pytest.raises(ValueError, match="steps"):
