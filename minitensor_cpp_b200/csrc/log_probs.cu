@@ -77,7 +77,8 @@ __device__ __forceinline__ int64_t at(const RowArgs &a, Operand o, int64_t row) 
 // -------------------------------------------------------------- statistics --
 
 constexpr float kLn2 = 0.69314718055994531f;
-constexpr float kFloor = -200.0f;  // exponents below it are zeros of float32, of base 2 and of base e
+constexpr float kFloor = -200.0f;  // exponents of 2 below it are zeros of float32
+// (In sums, what is below 2^-126 of the largest term is one too: exp2_fast flushes it.)
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

@@ -5,14 +5,14 @@ Tolerances are worst-case rounding bounds, U = 2^-24 being half a step of float3
 d = scale (x - max), p = exp(d) / S and E = sum p |d|:
  - d is off by 3 U |d| (the difference, the product, the factor in base 2);
  - an exponential by another 2^-22 = 4 U of itself (the hardware's 2^x), so a sum of them
-   by 3 U E + 4 U, and by its additions: a thread adds V / 256 of them at most, rescales
+   by 3 U |d| + 4 U each, and by its additions: a thread adds V / 256 of them at most, rescales
    them once for each 32 and twice when threads join (5 U each, beside the 3 U |d| that
-   count the parts of d), and 10 steps join the threads: eps = (V / 200 + 64) U + 3 U E of
-   the sum without its largest terms, which are exactly 1;
- - log S = log1p(S - 1) by eps (S - 1) / S and 4 U of itself;
- - E by the same of each |d| p: sum p |d| (3 U |d| + 8 U) + 2 eps E;
- - p by 3 U |d| + 4 U (expf) + eps (S - 1) / S + 2 U of itself, and where the token is the
-   largest logit 1 - p = (S - 1) / S by eps + 4 U of itself.
+   count the parts of d), and 10 steps join the threads: S - 1, whose largest terms are
+   exactly 1, by eps (S - 1) with eps = (V / 200 + 64) U, and by 3 U sum |d| exp(d) = 3 U S E;
+ - log S = log1p(S - 1) by that over S, eps (S - 1) / S + 3 U E, and 4 U of itself;
+ - E by the same of each |d| p: sum p |d| (3 U |d| + 8 U) + 2 (eps + 3 U E) E;
+ - p by 3 U |d| + 4 U (the exponential) + eps (S - 1) / S + 3 U E + 2 U of itself, and where
+   the token is the largest logit 1 - p = (S - 1) / S by eps + 4 U of itself and 3 U E.
 """
 import ctypes
 import math
@@ -52,9 +52,9 @@ def reference(x, t, scale, k=0):
     da = torch.where(e > 0, d.abs(), 0.0)
     spread = (p * da).sum(1, keepdim=True)
     log_s = torch.log1p(others)
-    eps = (vocab / 200 + 64) * U + 3 * U * spread
-    dlog_s = eps * others / s + 4 * U * log_s
-    dspread = (p * da * (3 * U * da + 8 * U)).sum(1, keepdim=True) + 2 * eps * spread
+    eps = (vocab / 200 + 64) * U
+    dlog_s = eps * others / s + 3 * U * spread + 4 * U * log_s
+    dspread = (p * da * (3 * U * da + 8 * U)).sum(1, keepdim=True) + 2 * (eps + 3 * U * spread) * spread
     lse = torch.where(empty, -INF, top + log_s)
     logp = torch.where(empty, -INF, d - log_s)
     dlogp = 3 * U * d.abs() + dlog_s + U * (d.abs() + log_s)
@@ -87,7 +87,7 @@ def grad_reference(x, t, dlp, dent, scale):
     p = r["p"].nan_to_num(nan=0.0)
     own = b * (r["d"] + r["spread"])
     g = -p * (a + own)
-    rel = 3 * U * r["da"] + 6 * U + r["eps"] * r["share"]
+    rel = 3 * U * r["da"] + 6 * U + r["eps"] * r["share"] + 3 * U * r["spread"]
     tol = p * rel * (a.abs() + own.abs()) + p * b.abs() * (3 * U * r["da"] + r["dspread"] + U * (r["da"] + r["spread"]))
     if t is not None and dlp is not None:
         hot = torch.zeros_like(p).scatter_(1, torch.where(r["live"], t, 0).unsqueeze(1), 1.0)
@@ -95,7 +95,7 @@ def grad_reference(x, t, dlp, dent, scale):
         g = g + hot * (a * (p + torch.where(r["is_top"], r["share"], 1.0 - p)))
         # (p and 1 - p of the token together: what is left of 1)
         g = torch.where(hot > 0, a * left - p * own, g)
-        tol = tol + hot * a.abs() * torch.where(r["is_top"], (r["eps"] + 4 * U) * left, U)
+        tol = tol + hot * a.abs() * torch.where(r["is_top"], (r["eps"] + 4 * U) * left + 3 * U * r["spread"], U)
     return g, tol + 5 * U * g.abs() + 1e-40
 
 
