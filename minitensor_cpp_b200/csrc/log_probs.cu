@@ -16,7 +16,7 @@
 // the maximum of what it has seen and sums relative to it, rescaled where a batch raises the
 // maximum.  The gradient reads the row a second time, last elements first, out of L2.  (A cluster a
 // row, a thread's elements in registers, was slower: 2^28 logits of 131072 classes 478 us at best
-// against 500, of 16000 420 against 401, of 50003 538 against 464: its CTAs wait for one another.)
+// against 459, of 16000 420 against 379, of 50003 538 against 441: its CTAs wait for one another.)
 //
 // The k likeliest (k <= 32) need no second pass over the row.  Of 32 groups of threads each has
 // a maximum, and the k-th largest of these is a bound that k elements reach; of the others few
@@ -308,6 +308,15 @@ struct Slope {
 // The k-th largest of the lanes' values.
 __device__ __forceinline__ int kth_of_warp(int v, int k) {
     const int lane = threadIdx.x % 32;
+    if (k <= 8) {  // the largest taken away one by one: fewer instructions than to sort
+        int top = v;
+        for (int i = 0; i < k; ++i) {
+            top = __reduce_max_sync(0xFFFFFFFFu, v);
+            const unsigned int at = __ballot_sync(0xFFFFFFFFu, v == top);
+            if (lane == __ffs(at) - 1) v = kNothing;
+        }
+        return top;
+    }
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -461,6 +470,7 @@ __global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_
 // ------------------------------------------------------------- a CTA a row --
 
 constexpr int kBatch = 8;      // vectors of four that a thread has in flight
+constexpr int kAgain = 2;      // and the second time (one: 131072 classes 501 us, two 458, four 447; 50003: 480, 462, 480)
 constexpr int kList = 512;
 constexpr int kThreadsOfSm = 1024;  // 64 registers each
 
@@ -727,14 +737,19 @@ __global__ void __launch_bounds__(T, kThreadsOfSm / T) k_cta_rows(const RowArgs 
             continue;
         }
         const bool whole = VEC && a.dcs == 1 && ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(src.p)) & 15) == 0;
-        for (int b = batches - 1; b >= 0; --b) {
+        for (int b = batches * (kBatch / kAgain) - 1; b >= 0; --b) {
+            float4 x[kAgain];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int j = thread + T * (b * kBatch + u);
+            for (int u = 0; u < kAgain; ++u) {
+                const int j = thread + T * (b * kAgain + u);
+                x[u] = src.vec(j < src.vecs ? j : src.vecs - 1);
+            }
+#pragma unroll
+            for (int u = 0; u < kAgain; ++u) {
+                const int j = thread + T * (b * kAgain + u);
                 if (j >= src.vecs) continue;
-                const float4 v = src.vec(j);
                 const int i = src.head + 4 * j;
-                const float4 g = make_float4(slope(v.x), slope(v.y), slope(v.z), slope(v.w));
+                const float4 g = make_float4(slope(x[u].x), slope(x[u].y), slope(x[u].z), slope(x[u].w));
                 if (whole) {
                     __stcs(reinterpret_cast<float4 *>(to + i), g);
                 } else {
@@ -808,13 +823,15 @@ int launch_forward(const RowArgs &a, cudaStream_t stream) {
 
 // Some 64 elements a thread, two batches, so that the rows at work are few enough for L2 (126 MB,
 // half of which is another die's) when they are read again.  2^28 logits:
-//   1500 classes  CTAs of 32 435 us;  64 elements a lane of a warp 561
-//   4000          of 64 396;  of 32 461
-//   8000          of 128 396;  of 64 447, of 256 439
-//   16000         of 256 401;  of 128 449, of 512 453
-//   32000         of 512 412;  of 256 453
-//   50003         of 1024 464;  of 512 471
-//   131072        of 1024 500;  of 512 545
+//   1500 classes  CTAs of 32 410 us;  64 elements a lane of a warp 561
+//   4000          of 64 371;  of 32 418
+//   8000          of 128 371;  of 64 412, of 256 439
+//   16000         of 256 379;  of 128 420, of 512 453
+//   24000         of 256 398;  of 512 447
+//   32000         of 512 392;  of 256 418
+//   50003         of 512 441;  of 1024 463
+//   65536         of 1024 414;  of 512 426
+//   131072        of 1024 459;  of 512 483
 int launch_gradient(const RowArgs &a, cudaStream_t stream) {
     if (a.vocab <= 32) return launch_warps<1, true>(a, stream);
     if (a.vocab <= 128) return launch_warps<4, true>(a, stream);
@@ -824,7 +841,7 @@ int launch_gradient(const RowArgs &a, cudaStream_t stream) {
     if (a.vocab <= 6000) return launch_ctas<64, true>(a, stream);
     if (a.vocab <= 12000) return launch_ctas<128, true>(a, stream);
     if (a.vocab <= 24000) return launch_ctas<256, true>(a, stream);
-    if (a.vocab <= 48000) return launch_ctas<512, true>(a, stream);
+    if (a.vocab <= 56000) return launch_ctas<512, true>(a, stream);
     return launch_ctas<1024, true>(a, stream);
 }
 
