@@ -382,17 +382,18 @@ int mtc_clip_global_norm(const mtc_desc *tensors, int32_t n, float max_norm, con
  * matrix NaN.  outs[k] has tensors[k]'s shape and may be the same view (in place);
  * other overlaps are not allowed.
  *
- * Products have float32 accuracy: small matrices are worked on in float32, others
+ * Products have float32 accuracy: matrices of few rows are worked on in float32, others
  * as pairs of 16-bit floats, which hold an element of X, S or of the polynomial to
  * 2^-22 of itself or to 2^-49 of the largest it could be, whichever is more; the
  * diagonals of S and of the polynomial are kept apart in float32.  The same call gives
  * the same bits; in a list with other matrices one may be split differently, and so
  * rounded differently.
  *
- * Workspace (none for small matrices and those of up to 128 x 128): 8 bytes an element
- * and 8 for each element of S, sides padded to a multiple of 256 (of 128 where the
- * shorter one is 128 or less), for as many matrices at a time as take 4 GiB together,
- * one at least; where the pool cannot give that, for fewer. */
+ * Workspace: 8 bytes an element and 8 for each element of S, sides padded to a multiple
+ * of 256 (of 128 where the shorter one is 128 or less), for as many matrices at a time as
+ * take 4 GiB together, one at least; where the pool cannot give that, for fewer.  None for
+ * matrices of up to 128 x 128, nor for those whose shorter side is at most 48, or 64 with
+ * the longer at most 2048, and that take at most 1 MB, the shorter side padded to fours. */
 int mtc_orthogonalize(const mtc_desc *tensors, int32_t n, const float *coefficients, int32_t steps, float eps,
                       const mtc_desc *outs, void *stream);
 

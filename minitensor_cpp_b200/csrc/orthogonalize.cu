@@ -7,8 +7,8 @@
 // the elements of X, S and B are below it and its polynomials, which gives the packed operands
 // of the tensor cores fixed scales: nothing is looked at while the products run.
 //
-// Small matrices are worked on by a CTA each, in shared memory: in float32 (k_small), or on the
-// tensor cores where both sides are 128 or less and the products are enough.  All others are
+// Matrices of few rows are worked on in shared memory, in float32 (k_slabs), others of up to 128 x
+// 128 by a CTA each that has them there on the tensor cores.  All others are
 // packed into pairs of 16-bit floats once and then stay so, from one product's epilogue to the
 // next one's operands (orthogonalize_tc.cu).
 #include <cuda_fp16.h>
@@ -28,8 +28,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double part[kThreads / 32];
+    __shared__ double part[THREADS / 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     __syncthreads();
@@ -37,130 +38,237 @@ __device__ __forceinline__ double block_sum(double v) {
     __syncthreads();
     v = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) v += part[i];
+    for (int i = 0; i < THREADS / 32; ++i) v += part[i];
     return v;
 }
 
-// ---------------------------------------------------------- small matrices --
+// ------------------------------------------------- matrices of few rows --
+//
+// Up to 64 rows, in float32: the CTAs of a cluster (or one) have equal parts of the columns in
+// shared memory for all steps.  Each adds up the products of its own columns, S is the sum of
+// the CTAs' in their order, everything of m x m is worked out by all of them, and B X needs no
+// other columns than its own, so X is replaced where it lies.  S and B are symmetric: tiles of 4 x 4
+// on and above the diagonal are worked out, and where that leaves threads, they share K.
+// Bound by shared memory (of B X a warp reads 20 lines of 128 bytes for 64 multiply-adds) and, where
+// there is little to do, by the syncs: five steps of 3 x 64 take 25 us, of 48 x 48 39 (packed for the
+// tensor cores of one CTA 46), of 60 x 2000 113 (in 17 launches, as tiles of 128 rows, 182), 64 of
+// 10 x 8192 152 (1410).  256 threads that work out all of S took 64 us for 48 x 48, and where each
+// CTA of eight added up all parts itself, 376 for 60 x 2000.
 
-struct SmallSteps {
+struct SlabSteps {
     int n;
     float eps;
     float a[kMostSteps], b[kMostSteps], c[kMostSteps];
 };
 
-// Shared memory of a small matrix: X twice and two squares, rows in whole float4 and 4 floats
-// apart from a multiple of the banks.
-__host__ __device__ inline int small_pitch(int cols) { return (cols + 3) / 4 * 4 + 4; }
-inline size_t small_bytes(int m, int n) {
+constexpr int kSlabRows = 64, kMostCluster = 8, kSlabThreads = 512;
+constexpr int kJoin = 17 * kSlabThreads;  // floats in which the threads' parts of S are added up
+
+// Rows of an odd number of float4, so that eight neighbours' lie in different banks.
+__host__ __device__ inline int slab_pitch(int cols) { return ((cols + 3) / 4 | 1) * 4; }
+__host__ __device__ inline int slab_columns(int n, int ctas) { return ((n + ctas - 1) / ctas + 3) / 4 * 4; }
+inline size_t slab_bytes(int m, int n, int ctas) {
     const size_t rows = (m + 3) / 4 * 4;
-    return 4 * rows * 2 * (static_cast<size_t>(small_pitch(n)) + small_pitch(m));
+    return 4 * (rows * (static_cast<size_t>(slab_pitch(slab_columns(n, ctas))) + 3 * slab_pitch(m)) + kJoin);
+}
+constexpr size_t kMostSlab = 224 * 1024;
+
+__device__ __forceinline__ uint32_t of_cta(const void *p, int rank) {
+    uint32_t out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(out) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+    return out;
 }
 
-// to[i][j] = p old[i][j] + q sum_k x[i][k] y[j][k]; a thread has rows i, i + R, ... and columns
-// j, j + R, ... (R a fourth of the rows), so that neighbours read neighbouring rows.
-__device__ __forceinline__ void small_by_rows(const float *x, int pitch, int K, int R, const float *old, float *to,
-                                              int to_pitch, float p, float q) {
-    for (int t = threadIdx.x; t < R * R; t += kThreads) {
-        const int ti = t / R, tj = t % R;
-        float acc[4][4] = {};
-        for (int k = 0; k < K; k += 4) {
-            float4 u[4], v[4];
+__device__ __forceinline__ void all_ctas() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// acc += x[row + R i][k..] . x[col + R j][k..] over k = first, first + step, ... below K; rows and
+// columns R apart, so that neighbours read neighbouring rows.
+__device__ __forceinline__ void slab_products(const float *x, int pitch, int row, int col, int R, int first, int step, int K,
+                                              float (&acc)[4][4]) {
+#pragma unroll 2
+    for (int k = first; k < K; k += step) {
+        float4 u[4], v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                u[i] = *reinterpret_cast<const float4 *>(x + (ti + R * i) * pitch + k);
-                v[i] = *reinterpret_cast<const float4 *>(x + (tj + R * i) * pitch + k);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    acc[i][j] = fmaf(u[i].x, v[j].x, acc[i][j]);
-                    acc[i][j] = fmaf(u[i].y, v[j].y, acc[i][j]);
-                    acc[i][j] = fmaf(u[i].z, v[j].z, acc[i][j]);
-                    acc[i][j] = fmaf(u[i].w, v[j].w, acc[i][j]);
-                }
+        for (int i = 0; i < 4; ++i) {
+            u[i] = *reinterpret_cast<const float4 *>(x + (row + R * i) * pitch + k);
+            v[i] = *reinterpret_cast<const float4 *>(x + (col + R * i) * pitch + k);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int at = (ti + R * i) * to_pitch + tj + R * j;
-                to[at] = old != nullptr ? fmaf(p, old[at], q * acc[i][j]) : q * acc[i][j];
+                acc[i][j] = fmaf(u[i].x, v[j].x, acc[i][j]);
+                acc[i][j] = fmaf(u[i].y, v[j].y, acc[i][j]);
+                acc[i][j] = fmaf(u[i].z, v[j].z, acc[i][j]);
+                acc[i][j] = fmaf(u[i].w, v[j].w, acc[i][j]);
             }
     }
 }
 
-// to[i][j] = a x[i][j] + sum_k s[i][k] x[k][j]; a thread has rows i, i + R, ... and four columns.
-__device__ __forceinline__ void small_apply(const float *s, int s_pitch, const float *x, int pitch, int m, int R, int C,
-                                            float *to, float a) {
-    for (int t = threadIdx.x; t < R * C; t += kThreads) {
-        const int ti = t / C, tj = t % C;
-        float acc[4][4] = {};
-        for (int k = 0; k < m; k += 4) {
-            float4 u[4], v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                u[i] = *reinterpret_cast<const float4 *>(s + (ti + R * i) * s_pitch + k);
-                v[i] = *reinterpret_cast<const float4 *>(x + (k + i) * pitch + 4 * tj);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    acc[i][0] = fmaf(w[q], v[q].x, acc[i][0]);
-                    acc[i][1] = fmaf(w[q], v[q].y, acc[i][1]);
-                    acc[i][2] = fmaf(w[q], v[q].z, acc[i][2]);
-                    acc[i][3] = fmaf(w[q], v[q].w, acc[i][3]);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = (ti + R * i) * pitch + 4 * tj;
-            const float4 o = *reinterpret_cast<const float4 *>(x + at);
-            *reinterpret_cast<float4 *>(to + at) = make_float4(fmaf(a, o.x, acc[i][0]), fmaf(a, o.y, acc[i][1]),
-                                                               fmaf(a, o.z, acc[i][2]), fmaf(a, o.w, acc[i][3]));
-        }
-    }
+__device__ __forceinline__ void write_both(float *s, int pitch, int r, int c, float v) {
+    s[r * pitch + c] = v;
+    s[c * pitch + r] = v;
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads) k_small(const __grid_constant__ Table<N> table, const SmallSteps steps) {
+__global__ void __launch_bounds__(kSlabThreads) k_slabs(const __grid_constant__ Table<N> table, const SlabSteps steps) {
     extern __shared__ __align__(16) float smem[];
-    const Matrix &mt = table.matrix[blockIdx.x];
-    const int m = mt.m, n = mt.n, rows = (m + 3) / 4 * 4, pitch = small_pitch(n), s_pitch = small_pitch(m);
-    float *x = smem, *y = x + rows * pitch, *s = y + rows * pitch, *b = s + rows * s_pitch;
+    __shared__ double squares_of;
+    uint32_t size_u, rank_u;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size_u));
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank_u));
+    const int size = static_cast<int>(size_u), rank = static_cast<int>(rank_u), thread = threadIdx.x;
+    const Matrix &mt = table.matrix[blockIdx.x / size_u];
+    const int m = mt.m, rows = (m + 3) / 4 * 4, R = rows / 4;
+    const int per = slab_columns(mt.n, size), c0 = rank * per, L = max(min(mt.n - c0, per), 0);
+    const int pitch = slab_pitch(per), s_pitch = slab_pitch(m), square = rows * s_pitch, total = rows * pitch;
+    float *const x = smem, *const s = x + total, *const b = s + square, *const parts = b + square, *const join = parts + square;
     // rows and columns up to whole fours are zeros, and stay so
     const bool along = mt.cs == 1 || mt.rs != 1;
     double squares = 0.0;
-    const int total = rows * pitch;
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-        const int r = along ? i / pitch : i % rows, c = along ? i % pitch : i / rows;
-        const float v = r < m && c < n ? mt.src[r * mt.rs + c * mt.cs] : 0.0f;
-        x[r * pitch + c] = v;
-        squares += static_cast<double>(v) * v;
+    for (int first = thread; first < total; first += 4 * kSlabThreads) {
+        float v[4];
+        int to[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = first + u * kSlabThreads;
+            const int r = along ? i / pitch : i % rows, c = along ? i % pitch : i / rows;
+            to[u] = r * pitch + c;
+            v[u] = r < m && c < L ? mt.src[r * mt.rs + (c0 + c) * mt.cs] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (first + u * kSlabThreads < total) {
+                x[to[u]] = v[u];
+                squares += static_cast<double>(v[u]) * v[u];
+            }
     }
-    const double inverse = inverse_norm(block_sum(squares), steps.eps);
-    for (int i = threadIdx.x; i < total; i += kThreads) x[i] = static_cast<float>(x[i] * inverse);
+    squares = block_sum<kSlabThreads>(squares);
+    if (size > 1) {
+        if (thread == 0) squares_of = squares;
+        all_ctas();
+        squares = 0.0;
+        for (int c = 0; c < size; ++c) {
+            double v;
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(of_cta(&squares_of, c)) : "memory");
+            squares += v;
+        }
+    }
+    const Factor factor(inverse_norm(squares, steps.eps), 0);
+    for (int i = thread; i < total; i += kSlabThreads) x[i] = factor(x[i]);
     __syncthreads();
-    const int R = rows / 4, C = (n + 3) / 4;
+    // the tiles of S on and above the diagonal, each of `groups` threads that share its K
+    const int tiles = R * (R + 1) / 2, groups = kSlabThreads / tiles, group = thread / tiles, tile = thread % tiles;
+    const int sums = max(groups / 16, 1);  // of an element of S, by as many threads
+    float *const halfway = join + 16 * kSlabThreads;
+    int row = 0, col = tile;
+    while (col >= R - row) col -= R - row++;
+    col += row;
+    const int wide = kSlabThreads / R, ti = thread / wide;  // columns' fours of a pass of B X
     for (int k = 0; k < steps.n; ++k) {
-        small_by_rows(x, pitch, n, R, nullptr, s, s_pitch, 0.0f, 1.0f);
+        float *const mine = size > 1 ? parts : s;
+        if (group < groups) {
+            float acc[4][4] = {};
+            slab_products(x, pitch, row, col, R, 4 * group, 4 * groups, L, acc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) join[(group * 16 + e) * tiles + tile] = acc[e / 4][e % 4];
+        }
         __syncthreads();
-        small_by_rows(s, s_pitch, m, R, s, b, s_pitch, steps.b[k], steps.c[k]);
+        if (group / 16 < sums && group < groups)
+            for (int e = group % 16; e < 16; e += min(groups, 16)) {
+                float sum = 0.0f;
+                for (int g = group / 16; g < groups; g += sums) sum += join[(g * 16 + e) * tiles + tile];
+                if (sums > 1) halfway[(group / 16 * 16 + e) * tiles + tile] = sum;
+                else write_both(mine, s_pitch, row + R * (e / 4), col + R * (e % 4), sum);
+            }
+        if (sums > 1) {
+            __syncthreads();
+            if (group < 16) {
+                float sum = 0.0f;
+                for (int p = 0; p < sums; ++p) sum += halfway[(p * 16 + group) * tiles + tile];
+                write_both(mine, s_pitch, row + R * (group / 4), col + R * (group % 4), sum);
+            }
+        }
+        if (size > 1) {
+            all_ctas();  // also: all are through with the last S
+            for (int o = 4 * (rank + size * thread); o < square; o += 4 * size * kSlabThreads) {
+                float4 v[kMostCluster];
+#pragma unroll
+                for (int c = 0; c < kMostCluster; ++c)
+                    if (c < size)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(v[c].x), "=f"(v[c].y), "=f"(v[c].z), "=f"(v[c].w) : "r"(of_cta(parts + o, c)) : "memory");
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < kMostCluster; ++c)
+                    if (c < size) sum = make_float4(sum.x + v[c].x, sum.y + v[c].y, sum.z + v[c].z, sum.w + v[c].w);
+#pragma unroll
+                for (int c = 0; c < kMostCluster; ++c)
+                    if (c < size)
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
+                                     :: "r"(of_cta(s + o, c)), "f"(sum.x), "f"(sum.y), "f"(sum.z), "f"(sum.w) : "memory");
+            }
+            all_ctas();
+        } else {
+            __syncthreads();
+        }
+        if (group == 0) {
+            float acc[4][4] = {};
+            slab_products(s, s_pitch, row, col, R, 0, 4, m, acc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = row + R * (e / 4), c = col + R * (e % 4);
+                const float v = fmaf(steps.b[k], s[r * s_pitch + c], steps.c[k] * acc[e / 4][e % 4]);
+                write_both(b, s_pitch, r, c, v);
+            }
+        }
         __syncthreads();
-        small_apply(b, s_pitch, x, pitch, m, R, C, y, steps.a[k]);
+        for (int first = 0; 4 * first < L; first += wide) {
+            const int tj = first + thread % wide;
+            const bool here = ti < R && 4 * tj < L;
+            float acc[4][4] = {};
+            if (here) {
+#pragma unroll 2
+                for (int q = 0; q < m; q += 4) {
+                    float4 u[4], v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u[i] = *reinterpret_cast<const float4 *>(b + (ti + R * i) * s_pitch + q);
+                        v[i] = *reinterpret_cast<const float4 *>(x + (q + i) * pitch + 4 * tj);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            acc[i][0] = fmaf(w[h], v[h].x, acc[i][0]);
+                            acc[i][1] = fmaf(w[h], v[h].y, acc[i][1]);
+                            acc[i][2] = fmaf(w[h], v[h].z, acc[i][2]);
+                            acc[i][3] = fmaf(w[h], v[h].w, acc[i][3]);
+                        }
+                    }
+                }
+            }
+            __syncthreads();  // these columns have been read
+            if (here) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float4 *const at = reinterpret_cast<float4 *>(x + (ti + R * i) * pitch + 4 * tj);
+                    const float4 o = *at;
+                    *at = make_float4(fmaf(steps.a[k], o.x, acc[i][0]), fmaf(steps.a[k], o.y, acc[i][1]),
+                                      fmaf(steps.a[k], o.z, acc[i][2]), fmaf(steps.a[k], o.w, acc[i][3]));
+                }
+            }
+        }
         __syncthreads();
-        float *const t = x;
-        x = y;
-        y = t;
     }
     const bool out_along = mt.out_cs == 1 || mt.out_rs != 1;
-    for (int i = threadIdx.x; i < m * n; i += kThreads) {
-        const int r = out_along ? i / n : i % m, c = out_along ? i % n : i / m;
-        mt.dst[r * mt.out_rs + c * mt.out_cs] = x[r * pitch + c];
+    for (int i = thread; i < m * L; i += kSlabThreads) {
+        const int r = out_along ? i / L : i % m, c = out_along ? i % L : i / m;
+        mt.dst[r * mt.out_rs + (c0 + c) * mt.out_cs] = x[r * pitch + c];
     }
 }
 
@@ -202,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) k_squares(const __grid_constant__ Ta
         const Unit at{static_cast<int>(i / cols) * kUnitRows, static_cast<int>(i % cols) * 64};
         read_unit(mt, at, [&](int, int, float v) { acc += static_cast<double>(v) * v; });
     }
-    acc = block_sum(acc);
+    acc = block_sum<kThreads>(acc);
     if (threadIdx.x == 0) partials[mt.part + static_cast<int>(blockIdx.x) - table.first[k]] = acc;
 }
 
@@ -216,7 +324,7 @@ __global__ void __launch_bounds__(kThreads) k_pack_matrices(const __grid_constan
     const Matrix &mt = table.matrix[k];
     double squares = 0.0;
     for (int i = threadIdx.x; i < mt.parts; i += kThreads) squares += partials[mt.part + i];
-    const Factor factor(inverse_norm(block_sum(squares), eps), scale);
+    const Factor factor(inverse_norm(block_sum<kThreads>(squares), eps), scale);
     const int u = static_cast<int>(blockIdx.x) - table.first[k];
     const Unit at{u / mt.x_blocks * kUnitRows, u % mt.x_blocks * 64};
     read_unit(mt, at, [&](int r, int c, float v) { tile[r * 65 + c] = factor(v); });
@@ -323,19 +431,34 @@ void add_matrices(const mtc_desc &in, const mtc_desc &out, std::vector<Matrix> &
     }
 }
 
-// A CTA's matrix in float32: in shared memory, and of few products.  Up to 128 columns the other way
-// is a CTA with the tensor cores (48 x 48: 38 us here, 47 there; 64 x 64: 50 and 48.5), beyond 17
-// launches (64 x 100: 160 us there, and in proportion to its products some 70 here).
+// The fewest CTAs whose shared memory takes the matrix's columns, or 0.
+int slab_ctas(const Matrix &mt) {
+    for (int c = 1; c <= kMostCluster; c *= 2)
+        if (slab_bytes(mt.m, mt.n, c) <= kMostSlab) return c;
+    return 0;
+}
+
+// Of few rows: worked on in float32.  Up to 128 columns the other way is a CTA with the tensor cores
+// (56 x 56: 46.6 us here, 47.6 there; 60 x 60 50 and 47.6; 44 x 128 45.6 and 51.7), beyond 17 launches,
+// whose time goes with the columns alone, as rows are padded to 128 (five steps of 64 matrices of
+// 48 x 6000 951 and 1116, 64 x 2000 408 and 469, but 52 x 4000 818 and 800, 64 x 2600 797 and 590).
 bool is_small(const Matrix &mt) {
     const int64_t m = mt.m, n = mt.n;
-    return 2 * m * m * n + m * m * m <= (n <= 128 ? 3 * 60 * 60 * 60 : 9 * 64 * 64 * 64) &&
-           small_bytes(mt.m, mt.n) <= 200 * 1024;
+    if (m > kSlabRows || slab_ctas(mt) == 0) return false;
+    return n <= 128 ? 2 * m * m * n + m * m * m <= 3 * 58 * 58 * 58 : m <= 48 || m * m * n <= 1 << 23;
 }
 
 bool is_whole(const Matrix &mt) { return mt.n <= 128; }
 
-int run_small(const std::vector<Matrix> &all, const std::vector<Step> &steps, float eps, cudaStream_t stream) {
-    SmallSteps s;
+// CTAs that run at once: a cluster lies in one part of the GPU, and what is left over of each stays
+// empty (64 x 2048 on clusters of eight: 15 of them 134 us, 16 of them 255; on four 208 both).
+int64_t room() { return sm_count(current_device()) * 5 / 6; }
+
+// On `ctas` CTAs each, as all of them need, or more while SMs are left over and that pays for the
+// clusters' barriers: 32 columns and 25000 products of B X for each (1 x 8192 on one CTA 58 us, on
+// four 37, on eight 33; 64 x 200 on two 74, on four 68; but 16 x 128 on one 25, on two 27).
+int run_slabs(const std::vector<Matrix> &all, int ctas, const std::vector<Step> &steps, float eps, cudaStream_t stream) {
+    SlabSteps s;
     std::memset(&s, 0, sizeof(s));
     s.n = static_cast<int>(steps.size());
     s.eps = eps;
@@ -344,16 +467,50 @@ int run_small(const std::vector<Matrix> &all, const std::vector<Step> &steps, fl
         s.b[k] = steps[k].b;
         s.c[k] = steps[k].c;
     }
+    int64_t most = 0, columns = 0;  // products of a matrix's B X
+    for (const Matrix &m : all) {
+        const int64_t rows = (m.m + 3) / 4 * 4;
+        most = std::max(most, rows * rows * m.n);
+        columns = std::max<int64_t>(columns, m.n);
+    }
+    const int64_t matrices = static_cast<int64_t>(all.size());
+    while (ctas < kMostCluster && 2 * ctas * matrices <= room() && most / ctas > 25000 && columns / ctas >= 64) ctas *= 2;
     for (size_t at = 0; at < all.size(); at += kMostMatrices) {
         const int count = static_cast<int>(std::min<size_t>(kMostMatrices, all.size() - at));
         size_t bytes = 0;
-        for (int i = 0; i < count; ++i) bytes = std::max(bytes, small_bytes(all[at + i].m, all[at + i].n));
+        for (int i = 0; i < count; ++i) bytes = std::max(bytes, slab_bytes(all[at + i].m, all[at + i].n, ctas));
         MTC_TRY(with_table(all.data() + at, count, [&](const auto &t) {
             constexpr int N = sizeof(t.matrix) / sizeof(t.matrix[0]);
-            MTC_CUDA_TRY(cudaFuncSetAttribute(k_small<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-            k_small<N><<<count, kThreads, bytes, stream>>>(t, s);
-            return check_launch("orthogonalize (small)");
+            MTC_CUDA_TRY(cudaFuncSetAttribute(k_slabs<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSlab));
+            cudaLaunchAttribute attr;
+            std::memset(&attr, 0, sizeof(attr));
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = static_cast<unsigned>(ctas);
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cudaLaunchConfig_t config;
+            std::memset(&config, 0, sizeof(config));
+            config.gridDim = static_cast<unsigned>(count * ctas);
+            config.blockDim = kSlabThreads;
+            config.dynamicSmemBytes = bytes;
+            config.stream = stream;
+            config.attrs = &attr;
+            config.numAttrs = 1;
+            MTC_CUDA_TRY(cudaLaunchKernelEx(&config, k_slabs<N>, t, s));
+            return check_launch("orthogonalize (few rows)");
         }));
+    }
+    return MTC_OK;
+}
+
+int run_small(const std::vector<Matrix> &all, const std::vector<Step> &steps, float eps, cudaStream_t stream) {
+    int most = 1;
+    for (const Matrix &m : all) most = std::max(most, slab_ctas(m));
+    if (static_cast<int64_t>(all.size()) * most <= room()) return run_slabs(all, most, steps, eps, stream);  // one launch
+    for (int ctas = 1; ctas <= kMostCluster; ctas *= 2) {
+        std::vector<Matrix> some;
+        for (const Matrix &m : all)
+            if (slab_ctas(m) == ctas) some.push_back(m);
+        if (!some.empty()) MTC_TRY(run_slabs(some, ctas, steps, eps, stream));
     }
     return MTC_OK;
 }
@@ -461,14 +618,9 @@ int run(const mtc_desc *tensors, int32_t n, const float *coefficients, int32_t n
         }
     }
     if (!whole.empty()) {  // small ones along with them, on other SMs, not after them
-        for (size_t i = 0; i < small.size();) {
-            if (!is_whole(small[i])) {
-                ++i;
-                continue;
-            }
-            whole.push_back(small[i]);
-            small.erase(small.begin() + static_cast<std::ptrdiff_t>(i));
-        }
+        const auto rest = std::stable_partition(small.begin(), small.end(), [](const Matrix &m) { return !is_whole(m); });
+        whole.insert(whole.end(), rest, small.end());
+        small.erase(rest, small.end());
         MTC_TRY(whole_matrices(whole.data(), static_cast<int>(whole.size()), steps.data(), static_cast<int>(steps.size()), eps, stream));
     }
     return small.empty() ? MTC_OK : run_small(small, steps, eps, stream);

@@ -433,3 +433,42 @@ def test_a_training_step(cuda):
     h2 = -(lp2.exp() * lp2).sum(1)
     loss2 = -((advantage.double() * lp2.gather(1, at).squeeze(1) + beta * h2) * live).sum() / count
     assert (loss2 - loss).item() < 0
+
+
+# of up to 64 rows: from one CTA's columns to a cluster's of eight, and beyond them; parts of the
+# columns that are empty, of no whole four, and one column more than a part
+FEW_ROWS = [(1, 129), (1, 13300), (1, 13301), (1, 106390), (1, 106500), (2, 50001), (4, 26600), (5, 8190), (7, 141), (8, 6003),
+            (12, 8192), (16, 26007), (29, 4001), (32, 12161), (33, 3000), (48, 1031), (60, 2000), (61, 129), (64, 129), (64, 300),
+            (64, 1027), (64, 4281), (64, 4400), (65, 1027)]
+
+
+@pytest.mark.parametrize("shape", FEW_ROWS)
+def test_few_rows(cuda, shape):
+    """Alone, where CTAs are left over, and in batches; transposed and in place."""
+    import torch
+
+    for seed, kind in enumerate(("noise", "rank", "decay")):
+        t = matrix(seed + 40, *shape, kind=kind)
+        got, = run([t], QUINTIC[:1])
+        abi.check_device_errors(0)
+        want, tol = one_step_bound(t, QUINTIC[0])
+        within(got, want, tol, f"{shape}, {kind}")
+        check([t])
+    ts = matrix(43, 40, *shape)
+    got, = check([ts])
+    check([ts.mT, matrix(44, 50, 60), matrix(45, 3, shape[0], 200)])
+    abi.orthogonalize([view(ts)])
+    assert torch.equal(ts, got)
+
+
+def test_few_rows_that_hold_no_numbers(cuda):
+    """In one CTA's part of the columns only: NaN all over that matrix, and there alone."""
+    import torch
+
+    ts = matrix(46, 5, 6, 30000)
+    ts[1] = 0.0
+    ts[2, 5, 29999], ts[3, 0, 15000] = float("nan"), -math.inf
+    for eps in (0.0, EPS):
+        got, = run([ts], eps=eps)
+        abi.check_device_errors(0)
+        assert (got[1] == 0).all() and got[2:4].isnan().all() and got[[0, 4]].isfinite().all()
