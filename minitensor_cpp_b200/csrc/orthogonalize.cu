@@ -50,7 +50,7 @@ __device__ __forceinline__ double block_sum(double v) {
 // other columns than its own, so X is replaced where it lies.  S and B are symmetric: tiles of 4 x 4
 // on and above the diagonal are worked out, and where that leaves threads, they share K.
 // Bound by shared memory (of B X a warp reads 20 lines of 128 bytes for 64 multiply-adds) and, where
-// there is little to do, by the syncs: five steps of 3 x 64 take 25 us, of 48 x 48 39 (packed for the
+// there is little to do, by the syncs: five steps of 3 x 64 take 15 us, of 48 x 48 39 (packed for the
 // tensor cores of one CTA 46), of 60 x 2000 113 (in 17 launches, as tiles of 128 rows, 182), 64 of
 // 10 x 8192 152 (1410).  256 threads that work out all of S took 64 us for 48 x 48, and where each
 // CTA of eight added up all parts itself, 376 for 60 x 2000.
@@ -160,8 +160,9 @@ __global__ void __launch_bounds__(kSlabThreads) k_slabs(const __grid_constant__ 
     const Factor factor(inverse_norm(squares, steps.eps), 0);
     for (int i = thread; i < total; i += kSlabThreads) x[i] = factor(x[i]);
     __syncthreads();
-    // the tiles of S on and above the diagonal, each of `groups` threads that share its K
-    const int tiles = R * (R + 1) / 2, groups = kSlabThreads / tiles, group = thread / tiles, tile = thread % tiles;
+    // the tiles of S on and above the diagonal, each of `groups` threads that share its K (and have some: with
+    // all 512 3 x 64 took 25 us)
+    const int tiles = R * (R + 1) / 2, groups = min(kSlabThreads / tiles, per / 4), group = thread / tiles, tile = thread % tiles;
     const int sums = max(groups / 16, 1);  // of an element of S, by as many threads
     float *const halfway = join + 16 * kSlabThreads;
     int row = 0, col = tile;
