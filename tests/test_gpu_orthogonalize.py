@@ -472,3 +472,26 @@ def test_few_rows_that_hold_no_numbers(cuda):
         got, = run([ts], eps=eps)
         abi.check_device_errors(0)
         assert (got[1] == 0).all() and got[2:4].isnan().all() and got[[0, 4]].isfinite().all()
+
+
+def test_few_rows_recorded(cuda):
+    """Clusters of several sizes in a graph of torch's (no workspace), replayed over new inputs beside eager calls."""
+    import torch
+
+    shapes = [(10, 3000), (3, 8192), (4, 33, 2000), (60, 1500), (20, 20)]
+    ts, side = [matrix(50 + i, *s) for i, s in enumerate(shapes)], torch.cuda.Stream()
+    outs = [torch.zeros_like(t) for t in ts]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        abi.orthogonalize([view(t) for t in ts], [view(o) for o in outs])
+    for seed in (60, 70):
+        for i, t in enumerate(ts):
+            t.copy_(matrix(seed + i, *t.shape))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        want = [run(ts) for _ in range(3)][-1]  # meanwhile
+        torch.cuda.synchronize()
+        for t, o, w in zip(ts, outs, want):
+            assert torch.equal(o, w)
+        check(ts)
