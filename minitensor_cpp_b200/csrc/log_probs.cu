@@ -272,10 +272,11 @@ __device__ __forceinline__ bool token_of(const RowArgs &a, long long t, bool rep
     return true;
 }
 
-// The gradient of a row: -p (by_entropy u + shift) with d = u ln 2, and of the token's element
-// apart.
+// The gradient of a row: -p (by_entropy u + shift) with d = u ln 2 and shift = by_prob + own, and
+// of the token's element apart: the entropy's part of it by `own`, which a rounded shift does
+// not give back where it is little next to by_prob.
 struct Slope {
-    float m, scale2, by_entropy, shift, inverse, by_prob, spread, others;
+    float m, scale2, by_entropy, shift, inverse, by_prob, own, others;
     bool whole;  // else every element is `fill`
     float fill;
 
@@ -285,8 +286,8 @@ struct Slope {
         scale2 = a.scale2;
         by_prob = a.dlog_probs != nullptr ? a.dlog_probs[at(a, kDLogProbs, row)] * a.scale : 0.0f;
         by_entropy = a.dentropy != nullptr ? a.dentropy[at(a, kDEntropy, row)] * a.scale : 0.0f;
-        spread = s.spread;
-        shift = fmaf(by_entropy, spread, by_prob);
+        own = by_entropy * s.spread;
+        shift = fmaf(by_entropy, s.spread, by_prob);
         by_entropy *= kLn2;
         inverse = 1.0f / s.total;
         others = s.others;
@@ -299,7 +300,7 @@ struct Slope {
     }
     __device__ __forceinline__ float of_token(float x) const {
         const float u = fmaxf((x - m) * scale2, kFloor), p = exp2_full(u) * inverse;
-        return by_prob * (x == m ? others * inverse : 1.0f - p) - p * fmaf(by_entropy, u, shift - by_prob);
+        return by_prob * (x == m ? others * inverse : 1.0f - p) - p * fmaf(by_entropy, u, own);
     }
 };
 

@@ -507,3 +507,41 @@ def test_the_same_inputs_give_the_same_bits(cuda):
             again = run(x, t, 1.0, 20)
             assert all(torch.equal(again[n], first[n]) for n in first)
             assert torch.equal(run_grad(x, t, dlp, dent), grad)
+
+
+SIGNS = [(1.0, 1.0), (1.0, -1.0), (-1.0, 0.01), (1.0, 0.01), (-0.01, -1.0), (1.0, 100.0)]
+
+
+@pytest.mark.parametrize("vocab", [5, 1000, 2000, 3001, 32000])
+@pytest.mark.parametrize("dlp, dent", SIGNS)
+@pytest.mark.parametrize("scale", [1.0, 0.7])
+def test_gradient_of_a_sure_token_keeps_the_digits_of_what_is_left(cuda, vocab, dlp, dent, scale):
+    """1 - p of the token from 1e-3 to 1e-12, left to all others or to one of them.
+
+    The token being the largest logit, its element is a (1 - p) - p b E with a = scale dlp and b =
+    scale dent.  1 - p is off by (eps + 4 U) of itself and 3 U E (above), a by U; b by U, its
+    product with E by U, E by `dspread`, p as above with d = 0, the products by U each, the
+    difference by U of itself."""
+    import torch
+
+    n = 40
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(n, vocab, device=cuda, generator=g) * 0.5
+    t = torch.randint(0, vocab, (n,), device=cuda, generator=g)
+    row = torch.arange(n, device=cuda)
+    left = torch.logspace(-3, -12, n // 2, device=cuda).repeat(2)
+    other = (t + 1 + torch.randint(0, vocab - 1, (n,), device=cuda, generator=g)) % vocab
+    x[n // 2:], x[row, other] = -INF, torch.randn(n, device=cuda, generator=g)
+    x[row, t] = -INF
+    x[row, t] = torch.logsumexp(x * scale, 1) / scale - left.log() / scale
+    a, b = torch.full((n,), dlp, device=cuda), torch.full((n,), dent, device=cuda)
+    got = run_grad(x, t, a, b, scale)[row, t]
+    _, r = reference(x, t, scale)
+    at = lambda v: v.expand(n, vocab).gather(1, t.unsqueeze(1)).squeeze(1)
+    assert at(r["is_top"]).all()
+    a, b = abs(f32(dlp) * f32(scale)), abs(f32(dent) * f32(scale))
+    share, p, spread, dspread = at(r["share"]), at(r["p"]), at(r["spread"]), at(r["dspread"])
+    want = f32(dlp) * f32(scale) * share - p * (f32(dent) * f32(scale)) * spread
+    tol = a * ((r["eps"] + 6 * U) * share + 3 * U * spread)
+    tol += p * b * (dspread + spread * (9 * U + r["eps"] * share + 3 * U * spread)) + U * want.abs() + 1e-42
+    within(got, want, tol, f"{vocab} classes, {dlp}, {dent}")
