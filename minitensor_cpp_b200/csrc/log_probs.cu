@@ -8,7 +8,7 @@
 //
 // S is kept as n + r, the number of elements that equal M and the sum of the others, so that
 // log S = log1p(n - 1 + r), 1 - p_t and E of a row that is sure of its token keep the digits of
-// what is left.  The gradient takes its statistics from the row anew instead of from the
+// what is left.  (Of 129 to 512 classes where the others come to less than 1/8: see k_warp_rows.)  The gradient takes its statistics from the row anew instead of from the
 // caller: a log-sum-exp rounded to float32 would cost them.
 //
 // Bound by HBM: 4 bytes an element, and for the gradient 8.  Up to 1024 classes (2048 without
@@ -166,23 +166,43 @@ struct Stats {
         }
     }
 
-    // The same where m is at hand already, without a look for it: n + r and e alone.
+    // The same where m is at hand already, two elements an instruction where that is possible.
     template <int N>
-    __device__ __forceinline__ void add_all(const float (&x)[N], float scale2) {
-        float r1 = 0.0f, e1 = 0.0f;
+    __device__ __forceinline__ void add_below(const float (&x)[N], float scale2) {
+        if constexpr (N == 1) {
+            add(x, m, scale2);
+        } else {
+            float n1 = 0.0f, r1 = 0.0f;
+            float2 es = make_float2(e, 0.0f);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float u = fmaxf((x[i] - m) * scale2, kFloor), y = exp2_fast(u);
-            r += y;
-            e = fmaf(y, u, e);
-            if (i + 1 < N) {
-                const float v = fmaxf((x[i + 1] - m) * scale2, kFloor), z = exp2_fast(v);
-                r1 += z;
-                e1 = fmaf(z, v, e1);
+            for (int i = 0; i < N; i += 2) {
+                float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(-m, -m)), make_float2(scale2, scale2));
+                u = make_float2(fmaxf(u.x, kFloor), fmaxf(u.y, kFloor));
+                const float2 y = make_float2(exp2_fast(u.x), exp2_fast(u.y));
+                if (x[i] == m) n += 1.0f;
+                else r += y.x;
+                if (x[i + 1] == m) n1 += 1.0f;
+                else r1 += y.y;
+                es = __ffma2_rn(y, u, es);
             }
+            n += n1;
+            r += r1;
+            e = es.x + es.y;
         }
-        r += r1;
-        e += e1;
+    }
+
+    // Without a look for m: the sum of all elements from FIRST on, by halves, so that a 1 among
+    // them is rounded log2 N times at the most, and theirs of u 2^u.
+    template <int FIRST, int COUNT, int N>
+    __device__ __forceinline__ float sum_all(const float (&x)[N], float scale2, float (&es)[2]) const {
+        if constexpr (COUNT == 1) {
+            const float u = fmaxf((x[FIRST] - m) * scale2, kFloor), y = exp2_fast(u);
+            es[FIRST % 2] = fmaf(y, u, es[FIRST % 2]);
+            return y;
+        } else {
+            const float half = sum_all<FIRST, COUNT / 2>(x, scale2, es);
+            return half + sum_all<FIRST + COUNT / 2, COUNT - COUNT / 2>(x, scale2, es);
+        }
     }
 
     // Of a warp's lanes together, the same in all.
@@ -376,28 +396,34 @@ __global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_
         }
         const float largest = largest_of(x);
         const int mine = index(0) < a.vocab ? ordered(largest) : kNothing;
-        const float top = from_ordered(__reduce_max_sync(0xFFFFFFFFu, mine));
+        const int most = __reduce_max_sync(0xFFFFFFFFu, mine);
+        const float top = from_ordered(most);
         Stats st;
         if (!(top < INFINITY)) {
             st.bad = true;
         } else if (top > -INFINITY) {
-            // Sums with the largest logit's 1 among them, unless the others are little next to it: 4
-            // instructions an element instead of 8.
             st.m = top;
-            st.add_all(x, a.scale2);
-            st.sum_warp();
-            if (st.r < 1.0625f) {
-                st = Stats();
-                st.m = top;
-#pragma unroll 4
-                for (int v = lane; v < a.vocab; v += 32) {
-                    const float one[1] = {src[v * cs]};
-                    st.add(one, one[0], a.scale2);
-                }
+            if constexpr (R != 16) {
+                st.add_below(x, a.scale2);
                 st.sum_warp();
             } else {
-                st.n = 1.0f;
-                st.r -= 1.0f;
+                // Without a look at each element for the largest (2^28 logits of 200 classes 625 us, with it 680;
+                // of 500 268 and 294; but of 1000 236 and 205, of 2000 227 and 187): a lane that has it takes its 1
+                // out again before the lanes' sums are added.  Until then it costs the others up to log2 R = 4
+                // roundings of a sum above 1, which is 36 2^-24 of them where they are 1/8 of it.  Where they are
+                // less, they are added without it (rows sure of their class: 778 us of 200, 322 of 500).
+                float es[2] = {};
+                st.r = st.sum_all<0, R>(x, a.scale2, es);
+                st.e = es[0] + es[1];
+                if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, mine == most)) - 1) st.r -= 1.0f;
+                st.n = lane == 0 ? 1.0f : 0.0f;
+                st.sum_warp();
+                if (st.r < 0.125f) {
+                    st = Stats();
+                    st.m = top;
+                    st.add_below(x, a.scale2);
+                    st.sum_warp();
+                }
             }
         }
         const Row s(st);

@@ -545,3 +545,23 @@ def test_gradient_of_a_sure_token_keeps_the_digits_of_what_is_left(cuda, vocab, 
     tol = a * ((r["eps"] + 6 * U) * share + 3 * U * spread)
     tol += p * b * (dspread + spread * (9 * U + r["eps"] * share + 3 * U * spread)) + U * want.abs() + 1e-42
     within(got, want, tol, f"{vocab} classes, {dlp}, {dent}")
+
+
+@pytest.mark.parametrize("vocab", [3, 33, 100, 500, 1000, 1500, 2000, 2001])
+@pytest.mark.parametrize("equal", [True, False])
+def test_rows_whose_others_are_some_of_the_largest(cuda, vocab, equal):
+    """S - 1 from 0.02 to 2: the largest logit's 1 must not take the others' digits, within the bounds above."""
+    import torch
+
+    n = 400
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.zeros(n, vocab, device=cuda) if equal else torch.randn(n, vocab, device=cuda, generator=g)
+    t = torch.randint(0, vocab, (n,), device=cuda, generator=g)
+    row = torch.arange(n, device=cuda)
+    x[row, t] = -INF
+    x -= (torch.logsumexp(x, 1) - torch.logspace(math.log10(0.02), math.log10(2.0), n, device=cuda).log()).unsqueeze(1)
+    x[row, t] = 0.0
+    dlp, dent = (torch.randn(n, device=cuda, generator=g) for _ in range(2))
+    check(x, t, dlp, dent, 1.0, 2)
+    t = (t + 1) % vocab
+    check(x, t, dlp, dent, 1.0 / 0.7, 1)
