@@ -941,6 +941,33 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     }
 }
 
+// What a step's epilogues multiply by.
+struct Scales {
+    float gram, d_unit;                // S = X X^T: of the sums of products, and of those that give D
+    float square, p, r, b, c, e_unit;  // B from S
+    float apply, own, a;               // X
+};
+
+// In 64 bits until a coefficient is in: a power of two of its own may leave float32, and 0 times
+// it is 0.
+Scales scales_of(const Step &s, bool last) {
+    auto two = [](int e) { return std::ldexp(1.0, e); };
+    const int to = last ? 0 : s.x_after;
+    Scales f;
+    f.gram = static_cast<float>(two(s.s - 2 * s.x));
+    f.d_unit = static_cast<float>(two(-2 * s.x));
+    f.square = static_cast<float>(s.c * two(s.b_exp - 2 * s.s));
+    f.p = static_cast<float>(s.b * two(s.b_exp - s.s));
+    f.r = static_cast<float>(s.c * two(s.b_exp - s.s));
+    f.b = s.b;
+    f.c = s.c;
+    f.e_unit = static_cast<float>(s.c * two(-2 * s.s));
+    f.apply = static_cast<float>(two(to - s.b_exp - s.x));
+    f.own = static_cast<float>(two(to - s.x));
+    f.a = s.a;
+    return f;
+}
+
 // --------------------------------------------------- matrices of one tile --
 //
 // Up to 128 x 128: a CTA has X, R and Q in shared memory as blocks' images, 64 KB each, and goes
@@ -955,9 +982,9 @@ constexpr int kWholeBytes = 3 * kImage + 1024 + 2 * 128 * 4 + 64;
 static_assert(kWholeBytes <= 227 * 1024 && 128 * kTilePitch * 4 <= 2 * kImage, "shared memory");
 
 struct WholeSteps {
-    int n;
+    int n, scale;  // (exponent of X's scale at first)
     float eps;
-    Step step[kMostSteps];
+    Scales step[kMostSteps];
 };
 
 __device__ __forceinline__ double whole_sum(double v, double *part) {
@@ -1006,7 +1033,7 @@ __global__ void __launch_bounds__(kWholeThreads, 1)
         tile[row * kTilePitch + col] = v;
     }
     tc_fence_before();
-    const Factor factor(inverse_norm(whole_sum(squares, part), steps.eps), steps.step[0].x);
+    const Factor factor(inverse_norm(whole_sum(squares, part), steps.eps), steps.scale);
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     // a thread's row and the first of its 64 columns, which are one block
@@ -1080,27 +1107,23 @@ __global__ void __launch_bounds__(kWholeThreads, 1)
     const bool of_s = warp % 4 * 32 < m_blocks * kBlock && col0 < mt.m, of_x = warp % 4 * 32 < mt.m && col0 < mt.n;
     bool ok = true;
     for (int k = 0; k < steps.n; ++k) {
-        const Step &s = steps.step[k];
+        const Scales &s = steps.step[k];
         ok = product(x, x, false, n_blocks, of_s) && ok;
-        float scale = exp2f(static_cast<float>(s.s - 2 * s.x)), unit = exp2f(static_cast<float>(-2 * s.x));
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             if (!of_s) break;
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[j] = acc[8 * c + j] * scale;
+                v[j] = acc[8 * c + j] * s.gram;
                 if (row == col0 + 8 * c + j) {
-                    d[row] = acc[8 * c + j] * unit;
+                    d[row] = acc[8 * c + j] * s.d_unit;
                     v[j] = 0.0f;
                 }
             }
             put(r, c, v);
         }
         ok = product(r, r, false, m_blocks, of_s) && ok;
-        const float by_s = exp2f(static_cast<float>(s.b_exp - s.s));
-        scale = s.c * exp2f(static_cast<float>(s.b_exp - 2 * s.s));
-        unit = s.c * exp2f(static_cast<float>(-2 * s.s));
         const float di = d[row];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -1110,9 +1133,9 @@ __global__ void __launch_bounds__(kWholeThreads, 1)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int col = col0 + 8 * c + j;
-                v[j] = fmaf(fmaf(s.c * by_s, di + d[col], s.b * by_s), old[j], scale * acc[8 * c + j]);
+                v[j] = fmaf(fmaf(s.r, di + d[col], s.p), old[j], s.square * acc[8 * c + j]);
                 if (row == col) {
-                    e[row] = fmaf(fmaf(s.c, di, s.b), di, unit * acc[8 * c + j]);
+                    e[row] = fmaf(fmaf(s.c, di, s.b), di, s.e_unit * acc[8 * c + j]);
                     v[j] = 0.0f;
                 }
             }
@@ -1120,9 +1143,7 @@ __global__ void __launch_bounds__(kWholeThreads, 1)
         }
         ok = product(q, x, true, m_blocks, of_x) && ok;
         const bool last = k == steps.n - 1;
-        const int to = last ? 0 : s.x_after;
-        scale = exp2f(static_cast<float>(to - s.b_exp - s.x));
-        const float own = exp2f(static_cast<float>(to - s.x)) * (s.a + e[row]);
+        const float own = s.own * (s.a + e[row]);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             if (!of_x) break;
@@ -1130,7 +1151,7 @@ __global__ void __launch_bounds__(kWholeThreads, 1)
             get(x, c, old);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[j] = fmaf(own, old[j], scale * acc[8 * c + j]);
+                v[j] = fmaf(own, old[j], s.apply * acc[8 * c + j]);
                 if (last) tile[row * kTilePitch + col0 + 8 * c + j] = v[j];
             }
             if (!last) put(x, c, v);
@@ -1293,28 +1314,26 @@ int run_products(const Matrix *matrices, int count, const Step *steps, int n, ch
     MTC_TRY(choose_shape(gram, kSymmetric, true, gram_shape));
     MTC_TRY(choose_shape(square, kSymmetric, false, square_shape));
     MTC_TRY(choose_shape(apply, kApply, false, apply_shape));
-    auto two = [](int e) { return std::ldexp(1.0, e); };
     for (int k = 0; k < n; ++k) {
-        const Step &s = steps[k];
+        const Scales f = scales_of(steps[k], k == n - 1);
         gram.from = 0;
         gram.last = k % 2;  // (which X it is)
-        gram.q = static_cast<float>(two(s.s - 2 * s.x));
-        gram.unit = static_cast<float>(two(-2 * s.x));
+        gram.q = f.gram;
+        gram.unit = f.d_unit;
         MTC_TRY((launch_product<kSymmetric, N>(map, gram, gram_shape, stream)));
         square.from = 1;
-        square.q = static_cast<float>(s.c * two(s.b_exp - 2 * s.s));
-        square.p = static_cast<float>(s.b * two(s.b_exp - s.s));
-        square.r = static_cast<float>(s.c * two(s.b_exp - s.s));
-        square.b = s.b;
-        square.c = s.c;
-        square.unit = static_cast<float>(s.c * two(-2 * s.s));
+        square.q = f.square;
+        square.p = f.p;
+        square.r = f.r;
+        square.b = f.b;
+        square.c = f.c;
+        square.unit = f.e_unit;
         MTC_TRY((launch_product<kSymmetric, N>(map, square, square_shape, stream)));
-        const int to = k == n - 1 ? 0 : s.x_after;
         apply.from = k % 2;
         apply.last = k == n - 1;
-        apply.q = static_cast<float>(two(to - s.b_exp - s.x));
-        apply.p = static_cast<float>(two(to - s.x));
-        apply.r = s.a;
+        apply.q = f.apply;
+        apply.p = f.own;
+        apply.r = f.a;
         MTC_TRY((launch_product<kApply, N>(map, apply, apply_shape, stream)));
     }
     return MTC_OK;
@@ -1331,8 +1350,9 @@ int whole_matrices(const Matrix *matrices, int count, const Step *steps, int n_s
     WholeSteps w;
     std::memset(&w, 0, sizeof(w));
     w.n = n_steps;
+    w.scale = steps[0].x;
     w.eps = eps;
-    for (int k = 0; k < n_steps; ++k) w.step[k] = steps[k];
+    for (int k = 0; k < n_steps; ++k) w.step[k] = scales_of(steps[k], k == n_steps - 1);
     unsigned long long *err = nullptr;
     MTC_TRY(device_error_word(&err));
     for (int at = 0; at < count; at += kMostMatrices) {

@@ -495,3 +495,14 @@ def test_few_rows_recorded(cuda):
         for t, o, w in zip(ts, outs, want):
             assert torch.equal(o, w)
         check(ts)
+
+
+@pytest.mark.parametrize("shape", [(30, 40), (100, 100), (90, 128), (120, 700), (300, 200)])
+def test_coefficients_at_their_limit(cuda, shape):
+    """Singular values at 2^20 before a step, with polynomials of nothing, of little and of much: on each path."""
+    t = matrix(80, *shape)
+    for steps in ([(2.0 ** 20, 0.0, 0.0), (0.5, 0.0, 0.0)], [(2.0 ** 20, 0.0, 0.0), (0.0, 0.0, 0.0)],
+                  [(2.0 ** 20, 0.0, 0.0), (1.0, -(2.0 ** -41), 0.0)], [(2.0 ** 20, 0.0, 0.0), (0.5, 0.0, 2.0 ** -82)],
+                  [(0.0, 2.0 ** 20, 0.0), (2.0 ** -20, 0.0, 0.0)], [(2.0 ** 10, 0.0, 0.0), (2.0 ** 10, 0.0, 0.0), (-1.0, 0.0, 0.0)]):
+        got, = check([t], steps)
+        assert got.isfinite().all(), steps
