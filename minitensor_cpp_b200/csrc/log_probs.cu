@@ -359,7 +359,11 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
 constexpr int kWarpList = 64;
 
 // R elements a lane: the 32 lanes side by side, or in vectors of four, 32 vectors side by side.
-enum Lanes { kApart, kUnit, kVectors };
+// Which of the two goes by the number of classes (next to each other), so that a row's sums, and with
+// them its bits, do not depend on what the other rows lie on: kFours are vectors that some or all rows cannot load
+// as such.  (2^28 logits of 1000 classes, rows 1002 apart, 220 us, all off 16 bytes 237, their
+// gradients 507 and 501; with the lanes side by side 218 and 217, 583 and 587.)
+enum Lanes { kApart, kUnit, kFours, kVectors };
 
 template <int R, Lanes LANES, bool GRAD>
 __global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_warp_rows(const RowArgs a) {
@@ -378,9 +382,10 @@ __global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_
         }
         const float *src = a.logits + at(a, kLogits, row);
         const int64_t cs = LANES != kApart ? 1 : a.cs;
-        auto index = [&](int j) { return LANES == kVectors ? 4 * (lane + 32 * (j / 4)) + j % 4 : lane + 32 * j; };
+        constexpr bool FOURS = LANES >= kFours;
+        auto index = [&](int j) { return FOURS ? 4 * (lane + 32 * (j / 4)) + j % 4 : lane + 32 * j; };
         float x[R];
-        if (LANES == kVectors) {
+        if (LANES == kVectors || (LANES == kFours && reinterpret_cast<uintptr_t>(src) % 16 == 0)) {
 #pragma unroll
             for (int j = 0; j < R; j += 4) {
                 float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_
             const Slope slope(a, row, s);
             float *to = a.dlogits + at(a, kDLogits, row);
             auto of = [&](int j) { return !slope.whole ? slope.fill : index(j) == token ? slope.of_token(x[j]) : slope(x[j]); };
-            if (LANES == kVectors && a.dcs == 1 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+            if (FOURS && a.dcs == 1 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
 #pragma unroll
                 for (int j = 0; j < R; j += 4)
                     if (index(j) < a.vocab)
@@ -454,7 +459,7 @@ __global__ void __launch_bounds__(32 * kWarps, R >= 64 ? 2 : R >= 32 ? 3 : 4) k_
 #pragma unroll
         for (int j = 0; j < R; ++j) hits |= static_cast<Hits>(x[j] >= bound ? 1 : 0) << j;
         if (index(R - 1) >= a.vocab) {  // (what is no element)
-            const int n = LANES == kVectors ? 4 * ((a.vocab / 4 - lane + 31) / 32) : (a.vocab - lane + 31) / 32;
+            const int n = FOURS ? 4 * ((a.vocab / 4 - lane + 31) / 32) : (a.vocab - lane + 31) / 32;
             hits &= (static_cast<Hits>(1) << n) - 1;
         }
         int found = __reduce_add_sync(0xFFFFFFFFu, R > 32 ? __popcll(hits) : __popc(hits));
@@ -808,9 +813,11 @@ int launch_warps(const RowArgs &a, cudaStream_t stream) {
     const int64_t ctas = (a.rows + kWarps - 1) / (kWarps), most = static_cast<int64_t>(sm_count(current_device())) * 64;
     const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
     // (by the logits alone: the same logits give the same bits, wherever the gradient goes)
-    bool vectors = R >= 4 && a.cs == 1 && a.vocab % 4 == 0 && aligned16(a.logits);
-    for (int i = 0; i < a.rank; ++i) vectors = vectors && a.stride[kLogits][i] % 4 == 0;
-    if (vectors) k_warp_rows<R, R >= 4 ? kVectors : kUnit, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
+    const bool fours = R >= 4 && a.cs == 1 && a.vocab % 4 == 0;
+    bool alike = true;  // in alignment
+    for (int i = 0; i < a.rank; ++i) alike = alike && a.stride[kLogits][i] % 4 == 0;
+    if (fours && alike && aligned16(a.logits)) k_warp_rows<R, R >= 4 ? kVectors : kUnit, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
+    else if (fours) k_warp_rows<R, R >= 4 ? kFours : kUnit, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
     else if (a.cs == 1) k_warp_rows<R, kUnit, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
     else k_warp_rows<R, kApart, GRAD><<<grid, 32 * kWarps, 0, stream>>>(a);
     return check_launch("log probabilities (warps)");

@@ -565,3 +565,26 @@ def test_rows_whose_others_are_some_of_the_largest(cuda, vocab, equal):
     check(x, t, dlp, dent, 1.0, 2)
     t = (t + 1) % vocab
     check(x, t, dlp, dent, 1.0 / 0.7, 1)
+
+
+@pytest.mark.parametrize("vocab", [32, 100, 128, 200, 512, 1000, 1004, 2000, 2048, 3000, 9000])
+@pytest.mark.parametrize("gap", [0, 1, 2, 3])
+def test_a_row_gives_the_same_bits_alone_and_among_others(cuda, vocab, gap):
+    """Also where rows of one call lie on 16 bytes and others do not."""
+    import torch
+
+    n = 9
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(n * (vocab + gap) + 8, device=cuda, generator=g).mul_(2.0)[4:4 + n * (vocab + gap)]
+    x = x.view(n, vocab + gap)[:, :vocab]
+    t = torch.randint(0, vocab, (n,), device=cuda, generator=g)
+    dlp, dent = (torch.randn(n, device=cuda, generator=g) for _ in range(2))
+    check(x, t, dlp, dent, 1.0, 3)
+    want, grad = run(x, t, 1.0, 3), run_grad(x, t, dlp, dent)
+    for i in range(n):
+        one = slice(i, i + 1)
+        got = run(x[one], t[one], 1.0, 3)
+        assert all(torch.equal(got[name], want[name][one]) for name in want), i
+        assert torch.equal(run_grad(x[one], t[one], dlp[one], dent[one]), grad[one]), i
+        held = torch.full_like(x[one], 7.0)
+        assert torch.equal(run_grad(x[one], t[one], dlp[one], dent[one], to=held), grad[one]), i
