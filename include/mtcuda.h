@@ -336,7 +336,7 @@ int mtc_linear_cross_entropy_grad(const mtc_desc *x, const mtc_desc *weight, con
  * logits [.., V] Float32, tokens Int64 and log_probs, lse, entropy Float32 of the
  * leading shape, top_log_probs Float32 and top_tokens Int64 with an axis of k behind
  * it, 1 <= k <= 32 and k <= V.  Every operand but the logits may be NULL; log_probs
- * needs tokens.  0 < scale <= 2^100.
+ * needs tokens.  2^-100 <= scale <= 2^100.
  * A row whose token is `ignore_token` is not read: its floats are 0, its top_tokens
  * -1; so are those of a token outside [0, V), which also sets the device error word.
  * Logits of -inf have probability 0.  A row of nothing else has lse, log_probs and

@@ -239,7 +239,9 @@ struct Row {
     __device__ __forceinline__ float log_prob(float x, float scale) const {
         if (bad) return __int_as_float(0x7FC00000);
         if (empty) return -INFINITY;
-        return (x - m) * scale - log_total;
+        const float d = x - m;
+        if (d == -INFINITY) return x * scale - m * scale - log_total;  // a difference beyond float32, or x is -inf
+        return d * scale - log_total;
     }
 };
 
@@ -906,8 +908,9 @@ int fill_args(const RowOperands &o, float scale, int64_t ignore, RowArgs &a) {
         MTC_TRY(need_leading(o.d[k], logits, k == kTopLogProbs || k == kTopTokens || k == kDLogits, names[k]));
         if (k != kTokens && k != kDLogProbs && k != kDEntropy) MTC_TRY(need_distinct(o.d[k], names[k]));
     }
-    if (!(scale > 0.0f && scale <= 0x1p100f))
-        return fail(MTC_ERR_INVALID_ARGUMENT, "scale %g is not in (0, 2^100]", scale);
+    // (below it, differences beyond float32 would be more than nothing in the sums)
+    if (!(scale >= 0x1p-100f && scale <= 0x1p100f))
+        return fail(MTC_ERR_INVALID_ARGUMENT, "scale %g is not in [2^-100, 2^100]", scale);
     if (vocab == 0) return fail(MTC_ERR_INVALID_ARGUMENT, "logits over no classes");
     if (vocab > INT_MAX / 2) return fail(MTC_ERR_UNSUPPORTED, "%lld classes", static_cast<long long>(vocab));
     std::memset(&a, 0, sizeof(a));

@@ -588,3 +588,20 @@ def test_a_row_gives_the_same_bits_alone_and_among_others(cuda, vocab, gap):
         assert torch.equal(run_grad(x[one], t[one], dlp[one], dent[one]), grad[one]), i
         held = torch.full_like(x[one], 7.0)
         assert torch.equal(run_grad(x[one], t[one], dlp[one], dent[one], to=held), grad[one]), i
+
+
+@pytest.mark.parametrize("vocab", [6, 600, 3000])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -60, 1e-3, 0.25, 0.7])
+def test_log_probabilities_of_differences_beyond_float32(cuda, vocab, scale):
+    """x - max overflows where scale (x - max) does not."""
+    import torch
+
+    x, t, dlp, dent = data(5, vocab, 20)
+    x[0], x[0, 0] = 3e38, -3e38
+    x[1], x[1, 1] = LOWEST, -LOWEST
+    x[2, 2], x[2, 3] = 2e38, LOWEST
+    x[3, 0], x[3, 1], x[3, 2] = 1e38, -2.5e38, -INF
+    t[:4] = torch.tensor([0, 0, 3, 1], device=cuda)
+    got = check(x, t, dlp, dent, scale, min(vocab, 32))
+    if scale < 0.5:
+        assert got["log_probs"][:4].isfinite().all()

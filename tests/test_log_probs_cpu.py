@@ -103,3 +103,12 @@ def test_python_wrappers_hand_every_operand_over():
             abi.token_log_probs_grad(v(0, 7), v(0, 7), stream=0, **{**fine, name: wrong})
     with pytest.raises(ValueError, match="scale"):
         abi.token_log_probs(v(0, 7), scale=-2.0, stream=0)
+
+
+def test_log_probs_refuse_scales_that_float32_differences_do_not_bear():
+    for scale in (1e-45, 2.0 ** -126, 2.0 ** -101):
+        assert log_probs(scale=scale) == abi.ERR_INVALID_ARGUMENT
+        assert grad(scale=scale) == abi.ERR_INVALID_ARGUMENT
+    for scale in (2.0 ** -100, 2.0 ** 100):
+        assert log_probs(desc([0, 9]), ints([0]), desc([0]), scale=scale) == abi.OK
+        assert grad(desc([0, 9]), ints([0]), desc([0]), None, desc([0, 9]), scale=scale) == abi.OK
