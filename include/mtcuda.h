@@ -378,9 +378,10 @@ int mtc_clip_global_norm(const mtc_desc *tensors, int32_t n, float max_norm, con
  * for each matrix T of `n` Float32 tensors [.., M, N]; leading axes are a batch of
  * matrices.  `coefficients` lies in host memory; 1 <= steps <= 32; eps >= 0.
  * Coefficients that let singular values of [0, 1] grow beyond 2^20 (b S + c S^2
- * beyond 2^40) are refused.  A matrix of zeros stays one; a NaN or an infinity makes its whole
- * matrix NaN.  outs[k] has tensors[k]'s shape and may be the same view (in place);
- * other overlaps are not allowed.
+ * beyond 2^40) are refused, and so are those that bring all of them below 2^-60, or below
+ * 2^-30 ahead of a step with b or c (to 0 is fine).  A matrix of zeros stays one; a NaN
+ * or an infinity makes its whole matrix NaN.  outs[k] has tensors[k]'s shape and may be
+ * the same view (in place); other overlaps are not allowed.
  *
  * Products have float32 accuracy: matrices of few rows are worked on in float32, others
  * as pairs of 16-bit floats, which hold an element of X, S or of the polynomial to

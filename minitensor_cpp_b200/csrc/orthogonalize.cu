@@ -394,6 +394,10 @@ int follow_steps(const float *coefficients, int32_t n, std::vector<Step> &steps)
         const double factor = largest_factor(t.b, t.c, s), next = largest_value(t.a, t.b, t.c, s);
         if (!(factor <= 0x1p40 && next <= 0x1p20))
             return fail(MTC_ERR_INVALID_ARGUMENT, "step %d: with these coefficients singular values grow to %g", k, next);
+        // (scales end at 2^74, where what is smaller would lose digits of its pairs)
+        if ((next > 0.0 && next < 0x1p-60) || (s > 0.0 && s < 0x1p-30 && (t.b != 0.0f || t.c != 0.0f)))
+            return fail(MTC_ERR_INVALID_ARGUMENT, "step %d: with these coefficients all singular values fall to %g", k,
+                        next < s ? next : s);
         t.x = scale_for(s);
         t.s = scale_for(s * s);
         t.b_exp = scale_for(factor);

@@ -506,3 +506,12 @@ def test_coefficients_at_their_limit(cuda, shape):
                   [(0.0, 2.0 ** 20, 0.0), (2.0 ** -20, 0.0, 0.0)], [(2.0 ** 10, 0.0, 0.0), (2.0 ** 10, 0.0, 0.0), (-1.0, 0.0, 0.0)]):
         got, = check([t], steps)
         assert got.isfinite().all(), steps
+
+
+@pytest.mark.parametrize("shape", [(30, 40), (100, 100), (90, 128), (120, 700), (300, 200)])
+def test_coefficients_that_shrink_up_to_their_limit(cuda, shape):
+    t = matrix(81, *shape)
+    for steps in ([(2.0 ** -60, 0.0, 0.0)], [(2.0 ** -30, 0.0, 0.0), (1.0, 2.0 ** 60, 0.0)], [(2.0 ** -59, -(2.0 ** -60), 0.0)],
+                  [(2.0 ** -30, 0.0, 0.0), (0.0, 2.0 ** 60, 2.0 ** 119)], [(2.0 ** -40, 0.0, 0.0), (2.0 ** 40, 0.0, 0.0)],
+                  [(0.0, 0.0, 0.0), (1.0, 1.0, 1.0)]):
+        check([t], steps)

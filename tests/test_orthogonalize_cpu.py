@@ -83,3 +83,21 @@ def test_python_wrapper():
         abi.orthogonalize([v(0, 3)], eps=-1.0, stream=0)
     with pytest.raises(ValueError, match="differs in shape"):
         abi.orthogonalize([v(3, 3)], [v(3, 4)], stream=0)
+
+
+SHRINK = [[(2.0 ** -50, 0.0, 0.0), (1.0, 2.0 ** 100, 0.0)], [(2.0 ** -100, 2.0 ** -100, 0.0)], [(2.0 ** -61, 0.0, 0.0)],
+          [(2.0 ** -31, 0.0, 0.0), (1.0, 1.0, 0.0)], [(2.0 ** -31, 0.0, 0.0), (1.0, 0.0, 1.0)], [(0.0, 0.0, 2.0 ** -62)],
+          [(2.0 ** -40, 0.0, 0.0), (2.0 ** -40, 0.0, 0.0), (2.0 ** 40, 0.0, 0.0)]]
+
+
+@pytest.mark.parametrize("steps", SHRINK)
+def test_refused_coefficients_that_leave_next_to_nothing(steps):
+    """Their values would fall out of the scales of the packed operands, and lose digits."""
+    assert call([desc([300, 200])], steps=steps) == abi.ERR_INVALID_ARGUMENT
+    assert b"fall" in abi.lib().mtc_last_error()
+
+
+def test_coefficients_up_to_there_are_taken():
+    for steps in ([(2.0 ** -60, 0.0, 0.0)], [(2.0 ** -30, 0.0, 0.0), (1.0, 2.0 ** 60, 0.0)], [(0.0, 0.0, 0.0), (1.0, 1.0, 1.0)],
+                  [(2.0 ** -40, 0.0, 0.0), (2.0 ** 40, 0.0, 0.0)], [(2.0 ** -10, 0.0, 2.0 ** -30)] * 4):
+        assert call([desc([0, 200])], steps=steps) == abi.OK
