@@ -605,3 +605,46 @@ def test_log_probabilities_of_differences_beyond_float32(cuda, vocab, scale):
     got = check(x, t, dlp, dent, scale, min(vocab, 32))
     if scale < 0.5:
         assert got["log_probs"][:4].isfinite().all()
+
+
+# both sides of the classes at which a row goes to other threads (forward: 32, 128, 512, 1024, 2048 to
+# more elements of a lane, 4000, 12000, 24000, 100000 to more threads of a CTA; the gradient's CTAs:
+# 1024, 3500, 6000, 12000, 24000, 56000), and CTAs of 32 threads with 0 to 3 elements ahead and behind
+BORDERS = [2047, 2048, 2049, 2050, 2051, 2301, 2999, 3002, 3499, 3500, 3501, 3999, 4000, 4001, 5999, 6000, 6001, 11999, 12000,
+           12001, 23999, 24000, 24001, 55999, 56000, 56001, 99999, 100000, 100001]
+
+
+@pytest.mark.parametrize("vocab", BORDERS)
+def test_borders_of_the_number_of_threads(cuda, vocab):
+    import torch
+
+    for n, ignored, scale, k in ((5, 0.0, 1.0, 1), (6, 0.3, 1.0 / 0.7, 32), (41, 0.1, 0.25, 5)):
+        check(*data(n, vocab, vocab + n, ignored), scale, k)
+    x, t, dlp, dent = data(9, vocab, vocab, masked=0.9)
+    x[1], x[2, 3], x[4], x[5, vocab - 1] = -INF, float("nan"), 2.5, INF
+    got = run(x, t, 1.0, 20)
+    got["dlogits"] = run_grad(x, t, dlp, dent)
+    for name in ("lse", "entropy", "dlogits"):
+        assert got[name][[2, 5]].isnan().all(), name
+    assert got["top_tokens"][[2, 5], 0].tolist() == [3, vocab - 1]
+    fine = torch.tensor([0, 1, 3, 4, 6, 7, 8], device=cuda)
+    check(x[fine], t[fine], dlp[fine], dent[fine], 1.0, 20)
+
+
+@pytest.mark.parametrize("vocab, threads, near", [(2051, 32, 9), (3001, 32, 7), (3999, 32, 5), (8001, 64, 5), (20000, 128, 4),
+                                                 (50003, 256, 3), (99999, 256, 2), (140001, 512, 2)])
+@pytest.mark.parametrize("equal", [True, False])
+def test_likeliest_that_crowd_in_a_few_threads(cuda, vocab, threads, near, equal):
+    """Neighbouring threads read the largest logits, of which there are more than the 512 of a list."""
+    import torch
+
+    x, t, dlp, dent = data(4, vocab, near)
+    of = torch.arange(vocab, device=cuda)
+    for row in range(4):
+        ahead = (-row * vocab) % 4  # of a contiguous row's first vector
+        owner = (of - ahead).clamp(min=0) // 4 % threads
+        those = (owner >= 9) & (owner < 9 + near) & (of >= ahead)
+        assert those.sum() > 512
+        x[row, those] = x[row, those].round() + 50.0 if equal else x[row, those] + 50.0
+    for k in (1, 3, 32):
+        check(x, t, dlp, dent, 1.0, k)

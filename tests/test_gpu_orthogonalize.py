@@ -515,3 +515,10 @@ def test_coefficients_that_shrink_up_to_their_limit(cuda, shape):
                   [(2.0 ** -30, 0.0, 0.0), (0.0, 2.0 ** 60, 2.0 ** 119)], [(2.0 ** -40, 0.0, 0.0), (2.0 ** 40, 0.0, 0.0)],
                   [(0.0, 0.0, 0.0), (1.0, 1.0, 1.0)]):
         check([t], steps)
+
+
+def test_operands_behind_2_31_bytes(cuda):
+    """A matrix whose packed operands take 2.7 GB, and one of odd sizes that has all of its own behind them."""
+    big, odd = matrix(82, 13000, 13100), matrix(83, 601, 707)
+    check([big, odd], CUBIC[:3])
+    check([odd], CUBIC[:3])
