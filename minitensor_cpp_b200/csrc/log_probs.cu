@@ -239,9 +239,7 @@ struct Row {
     __device__ __forceinline__ float log_prob(float x, float scale) const {
         if (bad) return __int_as_float(0x7FC00000);
         if (empty) return -INFINITY;
-        const float d = x - m;
-        if (d == -INFINITY) return x * scale - m * scale - log_total;  // a difference beyond float32, or x is -inf
-        return d * scale - log_total;
+        return fmaf(0.5f, x, -0.5f * m) * (2.0f * scale) - log_total;  // (x - m may be beyond float32)
     }
 };
 
