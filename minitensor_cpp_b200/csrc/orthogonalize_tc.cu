@@ -1107,7 +1107,7 @@ __global__ void __launch_bounds__(kWholeThreads, 1)
     const bool of_s = warp % 4 * 32 < m_blocks * kBlock && col0 < mt.m, of_x = warp % 4 * 32 < mt.m && col0 < mt.n;
     bool ok = true;
     for (int k = 0; k < steps.n; ++k) {
-        const Scales &s = steps.step[k];
+        const Scales s = steps.step[k];  // (a copy: read where they are used, 2 us of 50 more)
         ok = product(x, x, false, n_blocks, of_s) && ok;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
