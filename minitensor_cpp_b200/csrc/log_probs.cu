@@ -836,7 +836,7 @@ int launch_ctas(const RowArgs &a, cudaStream_t stream) {
 // bit whatever other rows the call has.  (For few rows more would be a little faster: of 32000
 // classes one row with 20 alternatives takes 12.4 us by 512 threads and 15.4 by 256.)
 // Times of 2^28 logits, without alternatives, with 5 and with 20:
-//   1500 classes  64 elements a lane 222, 363, 463 us;  a CTA of 32 238, 432, 811
+//   1500 classes  64 elements a lane 226, 363, 466 us;  a CTA of 32 238, 432, 811
 //   3000          CTAs of 32 211, 297, 525;  of 64 223, 367, 617
 //   8000          of 64 162, 205, 310;  of 128 177, 250, 377
 //   16000         of 128 164, 193, 261;  of 256 183, 242, 326

@@ -122,10 +122,11 @@ inline int need_apart(const mtc_desc *outs, int n) {
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 #ifdef __CUDACC__
-// Launches a kernel that calls wait_for_previous() first: its CTAs may take their places while
-// the kernel before it on the stream runs out, which hides most of the launch.  Only for the
-// second and later kernels of a call; each of them waits for the one before, so all earlier
-// ones are done as well.
+// Launches a kernel that calls wait_for_previous() first: the launch is prepared while the kernel
+// before it on the stream runs, which hides some 2 us of it (17 launches 219 us, without it 253; in a
+// graph 217 and 222).  No kernel lets the next one begin earlier than at its own end, so the CTAs
+// take their places when the last ones before them have left.  Only for the second and later
+// kernels of a call; each of them waits for the one before, so all earlier ones are done as well.
 template <class... P, class... A>
 int launch_dependent(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
                      A &&...args) {

@@ -31,6 +31,8 @@
 // memory, which its smaller tiles leave, and has one ring of six: its blocks take half the time,
 // and two stages of lo would not cover a load.  Warp 0 loads (TMA: the workspace is one tensor of rows of 128 bytes), warp 1 issues,
 // warps 4..11 are the epilogue, two for each quarter of the tensor memory's lanes.
+// ptxas assigns the 168 registers of the launch to all warps, also to the epilogue's, which have 208:
+// single tiles' X spills 62 words, pairs' X 26 and their symmetric products 51.
 // Every wait is bounded; on expiry the device error word is set and the roles leave.
 #include <cuda_fp16.h>
 
