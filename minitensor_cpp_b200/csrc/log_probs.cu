@@ -8,7 +8,8 @@
 //
 // S is kept as n + r, the number of elements that equal M and the sum of the others, so that
 // log S = log1p(n - 1 + r), 1 - p_t and E of a row that is sure of its token keep the digits of
-// what is left.  (Of 129 to 512 classes where the others come to less than 1/8: see k_warp_rows.)  The gradient takes its statistics from the row anew instead of from the
+// what is left (of 129 to 512 classes only where the others come to less than 1/8: see
+// k_warp_rows).  The gradient takes its statistics from the row anew instead of from the
 // caller: a log-sum-exp rounded to float32 would cost them.
 //
 // Bound by HBM: 4 bytes an element, and for the gradient 8.  Up to 1024 classes (2048 without
@@ -359,10 +360,10 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
 constexpr int kWarpList = 64;
 
 // R elements a lane: the 32 lanes side by side, or in vectors of four, 32 vectors side by side.
-// Which of the two goes by the number of classes (next to each other), so that a row's sums, and with
-// them its bits, do not depend on what the other rows lie on: kFours are vectors that some or all rows cannot load
-// as such.  (2^28 logits of 1000 classes, rows 1002 apart, 220 us, all off 16 bytes 237, their
-// gradients 507 and 501; with the lanes side by side 218 and 217, 583 and 587.)
+// Which of the two goes by the number of classes (next to each other), so that a row's sums, and
+// with them its bits, do not depend on what the other rows lie on: kFours are vectors that some or
+// all rows cannot load as such.  (2^28 logits of 1000 classes, rows 1002 apart, 220 us, all off 16
+// bytes 237, their gradients 507 and 501; with the lanes side by side 218 and 217, 583 and 587.)
 enum Lanes { kApart, kUnit, kFours, kVectors };
 
 template <int R, Lanes LANES, bool GRAD>
